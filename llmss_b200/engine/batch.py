@@ -8,6 +8,40 @@ import torch
 
 
 @dataclass
+class SharedPrefix:
+    """Groups of sequences that begin with the same cached tokens: attention reads those once per group.
+
+    Group j holds the sequences first[j] .. first[j + 1] - 1 of the batch; their first lens[j] tokens lie in the pages block_tables[j] (0: nothing
+    is shared).  The sequences' own block tables name the same pages at their front and their lengths count the shared tokens.  Sequences outside
+    of first[0] .. first[-1] have no shared part.  ``max_len`` and ``max_rows`` bound lens and the query rows of a group; the tensors may change
+    under them, as in a captured step."""
+    block_tables: torch.Tensor  # [G, max_blocks] int32
+    lens: torch.Tensor          # [G] int32
+    first: torch.Tensor         # [G + 1] int32, ascending
+    num_groups: int
+    max_len: int
+    max_rows: int
+
+    @staticmethod
+    def build(groups: Sequence[Sequence[int]], block_tables: Sequence[Sequence[int]], lens: Sequence[int], q_lens: Sequence[int],
+              device) -> Optional["SharedPrefix"]:
+        """``groups``: sequence numbers of each group, consecutive and ascending; ``block_tables`` / ``lens``: a group's shared pages and tokens;
+        ``q_lens``: query rows of every sequence of the batch.  None where nothing is shared."""
+        if not groups or max(lens) == 0:
+            return None
+        flat = [i for g in groups for i in g]
+        if flat != list(range(flat[0], flat[0] + len(flat))) or not all(groups):
+            raise ValueError(f"SharedPrefix: groups of consecutive sequences, got {list(groups)}")
+        width = max(1, max(len(t) for t in block_tables))
+        i32 = dict(dtype=torch.int32)
+        return SharedPrefix(
+            block_tables=torch.tensor([list(t) + [0] * (width - len(t)) for t in block_tables], **i32).to(device),
+            lens=torch.tensor(list(lens), **i32).to(device),
+            first=torch.tensor([g[0] for g in groups] + [groups[-1][-1] + 1], **i32).to(device), num_groups=len(groups), max_len=max(lens),
+            max_rows=max(sum(q_lens[i] for i in g) for g in groups))
+
+
+@dataclass
 class BatchInput:
     tokens: torch.Tensor        # [T] int32 token ids, sequences packed back to back
     positions: torch.Tensor     # [T] int32 absolute position of each token
@@ -23,6 +57,7 @@ class BatchInput:
     is_fresh_prefill: bool      # no sequence has prior context (seq_len == q_len)
     decode_splits: int = 0      # split-KV factor frozen at graph-capture time (0 = choose per call)
     state_slots: Optional[torch.Tensor] = None   # [B] int32 state slot of each sequence (recurrent models); < 0 = inert row
+    prefix: Optional[SharedPrefix] = None        # cached tokens that groups of sequences share
 
     @staticmethod
     def build(token_lists: Sequence[Sequence[int]], context_lens: Sequence[int], block_tables: Sequence[Sequence[int]],

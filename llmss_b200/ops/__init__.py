@@ -15,6 +15,7 @@ import torch
 
 from . import cuda_impl as cu
 from . import reference as ref
+from .pages import QuantPages
 from .reference import (DECAY_HEAD, DECAY_TOKEN_CHANNEL, DECAY_TOKEN_HEAD, GATE_NONE, GATE_SIGMOID, GATE_SILU, UNARY_NEG_EXP,
                         UNARY_TANH, distance_bias_table, rotary_frequencies, window_bias_table)
 from .reference import (ACT_GELU_ERF, ACT_GELU_TANH, ACT_IDS, ACT_NONE, ACT_RELU, ACT_RELU2, ACT_SILU, NORM_DYT, NORM_LAYER,
@@ -109,6 +110,12 @@ def norm_residual(x, residual, weight, bias, eps: float, kind: int, x2=None):
 
 def rope_kv_write(qkv, positions, slot_mapping, k_cache, v_cache, hq, hkv, d, rotary_dim, style, base,
                   q_off, k_off, v_off):
+    """Rotate q and k in place and append k, v to the pages (``slot_mapping`` < 0: not written; the slots of a call are distinct).
+
+    Into ``QuantPages`` k (rotated) and v are quantised from 32 bits, a scale per token and head; the k and v columns stay as they are."""
+    if isinstance(k_cache, QuantPages):
+        write = cu.rope_kv_write_q8 if _cuda(qkv) else ref.rope_kv_write_q8
+        return write(qkv, positions, slot_mapping, k_cache, v_cache, hq, hkv, d, rotary_dim, style, base, q_off, k_off, v_off)
     if _cuda(qkv):
         return cu.rope_kv_write(qkv, positions, slot_mapping, k_cache, v_cache, hq, hkv, d, rotary_dim, style, base,
                                 q_off, k_off, v_off)
@@ -123,10 +130,21 @@ def attention(qkv, out, batch, k_cache, v_cache, hq, hkv, d, scale, q_off, k_off
     fresh prefill (no prior context)        -> varlen causal prefill kernel (K8);
     multi-token queries over prior context  -> the same kernel in paged mode (K / V from the cache);
     unsupported head sizes / page sizes     -> generic gather path (oracle math).
+
+    ``QuantPages``: keys and values are always those of the pages (a prompt's own too, so that a result does not depend on how the
+    prompt was cut into portions).  ``batch.prefix``: tokens that groups of sequences share are read once per group, from pages of either
+    kind.  Both take any mix of lengths; rows without a visible key become zero, rows of no sequence stay as they are.
     """
     T = qkv.shape[0]
     q_view = qkv[:, q_off:q_off + hq * d]
     out_view = out[:, out_off:out_off + hq * d]
+    if batch.prefix is not None or isinstance(k_cache, QuantPages):
+        if _cuda(qkv):
+            cu.attention_pages(q_view, out_view, batch, k_cache, v_cache, hq, hkv, d, scale)
+        else:
+            n = int(batch.cu_q[-1])
+            out_view[:n] = ref.attention_pages(q_view[:n].reshape(n, hq, d), k_cache, v_cache, batch, scale).reshape(n, hq * d)
+        return out
     if _cuda(qkv):
         if d not in (64, 128, 256):
             _warn_once(f"head_dim={d} has no sm_100a attention kernel (64/128/256 do); using the generic PyTorch path")

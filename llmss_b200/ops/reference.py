@@ -13,6 +13,8 @@ from typing import Optional, Tuple
 import torch
 import torch.nn.functional as F
 
+from .pages import QuantPages, quantise
+
 ACT_NONE, ACT_GELU_TANH, ACT_GELU_ERF, ACT_RELU, ACT_SILU, ACT_RELU2 = 0, 1, 2, 3, 4, 5
 ACT_IDS = {
     None: ACT_NONE, "none": ACT_NONE,
@@ -121,6 +123,65 @@ def rope_kv_write(qkv, positions, slot_mapping, k_cache, v_cache, hq: int, hkv: 
     blk, off = slots // bs, slots % bs
     k_cache[blk, :, off, :] = k[valid].to(k_cache.dtype)
     v_cache[blk, :, off, :] = v[valid].to(v_cache.dtype)
+
+
+def rope_kv_write_q8(qkv, positions, slot_mapping, k_pages, v_pages, hq: int, hkv: int, d: int, rotary_dim: int, style: int, base: float,
+                     q_off: int, k_off: int, v_off: int):
+    """rope_kv_write into 8-bit pages: q rotated in place, rotated k and v quantised from 32 bits (pages.quantise); the k and v columns stay as they
+    are.  Angles in 64 bits, so that positions far into a long context keep theirs."""
+    T = qkv.shape[0]
+    q = qkv[:, q_off:q_off + hq * d].reshape(T, hq, d).float()
+    k = qkv[:, k_off:k_off + hkv * d].reshape(T, hkv, d).float()
+    v = qkv[:, v_off:v_off + hkv * d].reshape(T, hkv, d).float()
+    if style != ROPE_NONE and rotary_dim > 0:
+        inv = base ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=qkv.device) / rotary_dim)
+        angle = positions.double()[:, None] * inv
+        cos, sin = angle.cos().float(), angle.sin().float()
+        qkv[:, q_off:q_off + hq * d] = apply_rope(q, cos, sin, rotary_dim, style).reshape(T, hq * d).to(qkv.dtype)
+        k = apply_rope(k, cos, sin, rotary_dim, style)
+    bs = k_pages.shape[2]
+    valid = (slot_mapping >= 0) & (slot_mapping < k_pages.shape[0] * bs)
+    slots = slot_mapping[valid].long()
+    blk, off = slots // bs, slots % bs
+    for pages, x in ((k_pages, k), (v_pages, v)):
+        codes, scale = quantise(x[valid], pages.dtype)
+        pages.data.view(torch.int8)[blk, :, off] = codes.view(torch.int8)
+        pages.scale[blk, :, off] = scale
+
+
+def attention_pages(q, k_pages, v_pages, batch, scale: float):
+    """attention_paged over 16-bit pages or QuantPages; a sequence's first tokens come from the pages of its group in ``batch.prefix``."""
+    T, hq, d = q.shape
+    hkv, bs = k_pages.shape[1], k_pages.shape[2]
+    out = torch.zeros(T, hq, d, dtype=q.dtype, device=q.device)
+    cu, lens = batch.cu_q.tolist(), batch.seq_lens.tolist()
+    shared = [(0, 0)] * len(lens)
+    if batch.prefix is not None:
+        first, n = batch.prefix.first.tolist(), batch.prefix.lens.tolist()
+        for j in range(batch.prefix.num_groups):
+            shared[first[j]:first[j + 1]] = [(j, n[j])] * (first[j + 1] - first[j])
+
+    def rows(pages, table, lo, hi):
+        """[hkv, hi - lo, d] of the tokens lo .. hi - 1"""
+        blocks = table[lo // bs:-(-hi // bs)].long()
+        x = pages.data[blocks].float() * pages.scale[blocks][..., None] if isinstance(pages, QuantPages) else pages[blocks].float()
+        return x.permute(1, 0, 2, 3).reshape(hkv, -1, d)[:, lo % bs:lo % bs + hi - lo]
+
+    for i, L in enumerate(lens):
+        q0, q1 = cu[i], cu[i + 1]
+        if q1 == q0 or L == 0:
+            continue
+        j, n = shared[i]
+        n = min(n, L)
+        kv = [torch.cat(([rows(x, batch.prefix.block_tables[j], 0, n)] if n else []) + [rows(x, batch.block_tables[i], n, L)], 1)
+              for x in (k_pages, v_pages)]
+        k, v = (x.repeat_interleave(hq // hkv, dim=0) for x in kv)
+        s = torch.matmul(q[q0:q1].float().transpose(0, 1), k.transpose(1, 2)) * scale
+        hidden = torch.arange(L, device=q.device) > torch.arange(L - (q1 - q0), L, device=q.device)[:, None]
+        o = torch.matmul(torch.softmax(s.masked_fill(hidden, float("-inf")), dim=-1), v)
+        o[:, :max(0, q1 - q0 - L)] = 0                      # rows in front of the sequence's first token see nothing
+        out[q0:q1] = o.transpose(0, 1).to(q.dtype)
+    return out
 
 
 def attention_paged(q, k_cache, v_cache, block_tables, seq_lens, cu_q, scale: float):
