@@ -1,71 +1,9 @@
-// Causal attention over a paged cache in 16 or 8 bits, with cached tokens that groups of sequences share.
-//
-//   s_jk = scale (q_j . K_k)      K_k = ks_k code_k      p = softmax over the keys k <= pos_j      out_j = sum_k p_jk vs_k code_k
-//
-// A sequence of a group (SharedGroups) finds its first len keys in the group's pages and the others in its own; a softmax over both is the merge
-// of the two parts by their maxima and sums.
-#include "common.cuh"
-
-#include <cuda_fp8.h>
+// Attention over cache pages: the choice of kernels, the merge of their parts, and a simple kernel for every shape.
+#include "attn_pages.cuh"
 
 namespace {
 
-constexpr int kF16Pages = 0, kInt8 = 1, kE4M3 = 2;    // page formats; 0: the queries' own 16-bit type
-
-struct AttnArgs {
-  const void* q;
-  const void* k;
-  const void* v;
-  const float* ks;
-  const float* vs;
-  void* out;
-  const int* tables;        // [num_seqs][max_blocks]
-  const int* seq_lens;
-  const int* cu;            // [num_seqs + 1]
-  const int* g_tables;      // [groups][g_max_blocks]
-  const int* g_lens;
-  const int* g_first;       // [groups + 1]
-  int64_t ldq, ldo;
-  int num_seqs, total_q, max_blocks, g_max_blocks, groups;
-  int hq, hkv, d, page, num_blocks;
-  float scale_log2;
-};
-
-// sequence that owns query row t (cu ascending), -1: none
-__device__ __forceinline__ int seq_of_row(const int* cu, int lo, int hi, int t) {
-  if (t < cu[lo] || t >= cu[hi]) return -1;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= t) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
-
-// group of a sequence, -1: none
-__device__ __forceinline__ int group_of_seq(const AttnArgs& a, int s) {
-  if (a.groups == 0 || s < a.g_first[0] || s >= a.g_first[a.groups]) return -1;
-  int lo = 0, hi = a.groups;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.g_first[mid] <= s) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
-
-// a block id that does not exist reads block 0: a wrong table costs a wrong result, not a fault
-__device__ __forceinline__ int checked_block(int id, int num_blocks) { return (unsigned)id < (unsigned)num_blocks ? id : 0; }
-
-template <typename T, int FMT>
-__device__ __forceinline__ float page_value(const void* p, int64_t i) {
-  if constexpr (FMT == kInt8) return (float)reinterpret_cast<const int8_t*>(p)[i];
-  else if constexpr (FMT == kE4M3) {
-    __nv_fp8_e4m3 c;
-    c.__x = reinterpret_cast<const uint8_t*>(p)[i];
-    return (float)c;
-  } else return to_f32(reinterpret_cast<const T*>(p)[i]);
-}
+using namespace pages;
 
 // ---------------------------------------------------------------------------------------------------------------- any shape
 // One block per query row and head, its four warps on keys in turn, everything in 32 bits: head sizes and page sizes that the tiled kernels do not take.
@@ -130,6 +68,127 @@ __global__ void __launch_bounds__(128) attn_pages_any_kernel(const __grid_consta
   }
 }
 
+// ---------------------------------------------------------------------------------------------------------------- merge
+// A warp per query row and head joins the parts of its softmax: m = max m_i, l = sum l_i 2^(m_i - m), out = sum O_i 2^(m_i - m) / l.  Reads what the
+// kernels before it left in L2; launched to start as they end (programmatic dependent launch), so that it costs no launch latency of its own.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) attn_pages_merge_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ PartArgs p) {
+  constexpr int N = D / 32;
+  const int w = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int t = w / a.hq, head = w % a.hq;
+  if (t >= a.total_q) return;
+  const int s = seq_of_row(a.cu, 0, a.num_seqs, t);      // lengths are not written by the kernels before
+  if (s < 0) return;
+  const int g = group_of_seq(a, s), group = a.hq / a.hkv, kvh = head / group;
+  float o[N], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) o[i] = 0.f;
+  auto add = [&](const float* part) {
+    const float2 ml = *reinterpret_cast<const float2*>(part + D);
+    float x[N];
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float2 v = *reinterpret_cast<const float2*>(part + i * 32 + lane * 2);
+      x[i] = v.x, x[i + 1] = v.y;
+    }
+    const float mn = fmaxf(m, ml.x), base = mn == -INFINITY ? 0.f : mn;
+    const float f = m == mn ? 1.f : exp2f(m - base), e = exp2f(ml.x - base);
+    l = l * f + ml.y * e;
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = o[i] * f + x[i] * e;
+    m = mn;
+  };
+  const Seg own = own_segment(a, s);
+  const bool has_own = own.hi > own.lo;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  auto few = [&](int seg, int row0, float* whole) {       // false: the result is written already
+    const FewInfo in = p.info[(int64_t)seg * a.hkv + kvh];
+    if (in.first_slot < 0) {
+      if (a.groups == 0) return false;
+      add(whole + ((int64_t)t * a.hq + head) * (D + 2));
+      return true;
+    }
+    const int n = (t - row0) * group + head % group;
+    if (n >= p.rows) return true;
+    add(p.slots + ((int64_t)in.first_slot * p.rows + n) * (D + 2));
+    for (int j = in.first_block + 1; j <= in.last_block; ++j) add(p.slots + ((int64_t)(2 * j) * p.rows + n) * (D + 2));
+    return true;
+  };
+  auto stretches = [&](const float* parts, int lo, int hi, int chunk, int splits) {
+    const int n = min(splits, (hi - lo + chunk - 1) / chunk);
+    for (int i = 0; i < n; ++i) add(parts + (((int64_t)i * a.total_q + t) * a.hq + head) * (D + 2));
+  };
+  if (has_own) {
+    if (p.few_own) {
+      if (!few(s, own.row0, p.whole_own)) return;
+    } else {
+      stretches(p.tile_own, own.lo, own.hi, p.own_chunk, p.own_splits);
+    }
+  }
+  if (g >= 0) {
+    const Seg gs = group_segment(a, g);
+    if (gs.hi > 0) {
+      if (p.few_groups) few((p.few_own ? a.num_seqs : 0) + g, gs.row0, p.whole_group);
+      else stretches(p.tile_group, 0, gs.hi, p.group_chunk, p.group_splits);
+    }
+  }
+  // no visible key: zero (l is NaN where a score was)
+  const float inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
+  T* out = reinterpret_cast<T*>(a.out) + (int64_t)t * a.ldo + (int64_t)head * D;
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    T v[2] = {from_f32<T>(o[i] * inv), from_f32<T>(o[i + 1] * inv)};
+    *reinterpret_cast<uint32_t*>(out + i * 32 + lane * 2) = *reinterpret_cast<const uint32_t*>(v);
+  }
+}
+
+template <typename T, int D>
+int launch_merge(const AttnArgs& a, const PartArgs& p, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3((unsigned)(((int64_t)a.total_q * a.hq + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  LLMSS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attn_pages_merge_kernel<T, D>, a, p));
+  return 0;
+}
+
+// ---------------------------------------------------------------------------------------------------------------- the choice
+struct Plan {
+  bool any;             // the simple kernel for the whole call
+  bool few_own, few_groups;
+  int blocks, rows;
+  int64_t slots, info, whole, floats;
+};
+
+// head sizes and pages of the tiled kernels
+bool tiled(int d, int page) { return (d == 64 || d == 128 || d == 256) && page % 16 == 0; }
+
+Plan plan_call(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv, int d, int page, int fmt, int groups, int g_max_len, int g_max_rows) {
+  Plan p;
+  memset(&p, 0, sizeof(p));
+  (void)max_kv, (void)g_max_len;
+  p.any = true;
+  if (hkv <= 0 || hq % hkv != 0 || !tiled(d, page)) return p;
+  const int64_t g = hq / hkv;
+  p.few_own = max_q * g <= 16;
+  p.few_groups = groups > 0 && g_max_rows * g <= 16;
+  if (!p.few_own || (groups > 0 && !p.few_groups)) return p;
+  p.any = false;
+  p.rows = max_q * g <= 8 && (groups == 0 || g_max_rows * g <= 8) ? 8 : 16;
+  p.blocks = few_blocks(fmt, d, p.rows);
+  p.slots = (int64_t)2 * p.blocks * p.rows * (d + 2);
+  p.info = (int64_t)(num_seqs + groups) * hkv * 4;
+  p.whole = groups > 0 ? (int64_t)total_q * hq * (d + 2) : 0;
+  p.floats = p.slots + p.info + 2 * p.whole;
+  return p;
+}
+
 int check_args(const AttnArgs& a, int fmt, int dtype) {
   LLMSS_REQUIRE(dtype == LLMSS_F16 || dtype == LLMSS_BF16, "attn_pages: dtype must be f16/bf16");
   LLMSS_REQUIRE(fmt >= kF16Pages && fmt <= kE4M3, "attn_pages: page format %d unknown", fmt);
@@ -150,9 +209,8 @@ int check_args(const AttnArgs& a, int fmt, int dtype) {
 // Floats of scratch that llmss_attn_pages takes for a call of these sizes (0: none).
 LLMSS_API int64_t llmss_attn_pages_scratch_floats(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv, int d, int block_size, int fmt,
                                                   int groups, int g_max_len, int g_max_rows) {
-  (void)num_seqs, (void)max_q, (void)max_kv, (void)total_q, (void)hq, (void)hkv, (void)d, (void)block_size, (void)fmt, (void)groups, (void)g_max_len,
-      (void)g_max_rows;
-  return 0;
+  if (num_seqs <= 0 || total_q <= 0 || max_q <= 0) return 0;
+  return plan_call(num_seqs, max_q, max_kv, total_q, hq, hkv, d, block_size, fmt, groups, g_max_len, g_max_rows).floats;
 }
 
 // q [total_q][>= hq * d] (row stride ldq); K / V pages [num_blocks][hkv][block_size][d] of the queries' type (fmt 0) or of bytes with 32-bit scales
@@ -194,7 +252,25 @@ LLMSS_API int llmss_attn_pages(const void* q, int64_t ldq, const void* k_pages, 
   LLMSS_REQUIRE(num_seqs >= 0 && max_q >= 0 && max_kv >= 0 && total_q >= 0 && groups >= 0, "attn_pages: negative size");
   if (num_seqs == 0 || total_q == 0 || max_q == 0) return 0;
   if (int e = check_args(a, fmt, dtype)) return e;
-  (void)scratch, (void)scratch_floats;
+  const Plan plan = plan_call(num_seqs, max_q, max_kv, total_q, hq, hkv, d, block_size, fmt, a.groups, g_max_len, g_max_rows);
+  if (!plan.any) {
+    LLMSS_REQUIRE(scratch != nullptr && scratch_floats >= plan.floats && ((uintptr_t)scratch % 16) == 0, "attn_pages: %lld floats of 16-byte aligned scratch needed",
+                  (long long)plan.floats);
+    PartArgs p;
+    memset(&p, 0, sizeof(p));
+    p.slots = (float*)scratch;
+    p.info = (FewInfo*)(p.slots + plan.slots);
+    p.whole_own = p.slots + plan.slots + plan.info;
+    p.whole_group = p.whole_own + plan.whole;
+    p.rows = plan.rows;
+    p.few_own = plan.few_own;
+    p.few_groups = plan.few_groups;
+    if (int e = few_launch(a, p, fmt, dtype, plan.blocks, stream)) return e;
+#define LLMSS_MERGE(T_) return d == 64 ? launch_merge<T_, 64>(a, p, stream) : d == 128 ? launch_merge<T_, 128>(a, p, stream) : launch_merge<T_, 256>(a, p, stream)
+    if (dtype == LLMSS_F16) LLMSS_MERGE(__half);
+    LLMSS_MERGE(__nv_bfloat16);
+#undef LLMSS_MERGE
+  }
   const dim3 grid(total_q, hq);
   LLMSS_REQUIRE(grid.y <= 65535, "attn_pages: %d heads", hq);
 #define LLMSS_ANY(T_, F_) LLMSS_CHECK_CUDA(launch_pdl(attn_pages_any_kernel<T_, F_>, grid, dim3(128), 0, stream, a))

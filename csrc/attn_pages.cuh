@@ -1,0 +1,140 @@
+// Shared by the kernels of attention over cache pages (attn_pages.cu, attn_pages_few.cu, attn_pages_tile.cu).
+//
+// Causal attention over a paged cache in 16 or 8 bits, with cached tokens that groups of sequences share.
+//
+//   s_jk = scale (q_j . K_k)      K_k = ks_k code_k      p = softmax over the keys k <= pos_j      out_j = sum_k p_jk vs_k code_k
+//
+// A sequence of a group (SharedGroups) finds its first len keys in the group's pages and the others in its own; a softmax over both is the merge
+// of the two parts by their maxima and sums.
+#pragma once
+#include "common.cuh"
+
+#include <cuda_fp8.h>
+
+namespace pages {
+
+constexpr int kF16Pages = 0, kInt8 = 1, kE4M3 = 2;    // page formats; 0: the queries' own 16-bit type
+
+struct AttnArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  const float* ks;
+  const float* vs;
+  void* out;
+  const int* tables;        // [num_seqs][max_blocks]
+  const int* seq_lens;
+  const int* cu;            // [num_seqs + 1]
+  const int* g_tables;      // [groups][g_max_blocks]
+  const int* g_lens;
+  const int* g_first;       // [groups + 1]
+  int64_t ldq, ldo;
+  int num_seqs, total_q, max_blocks, g_max_blocks, groups;
+  int hq, hkv, d, page, num_blocks;
+  float scale_log2;
+};
+
+// sequence that owns query row t (cu ascending), -1: none
+__device__ __forceinline__ int seq_of_row(const int* cu, int lo, int hi, int t) {
+  if (t < cu[lo] || t >= cu[hi]) return -1;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cu[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// group of a sequence, -1: none
+__device__ __forceinline__ int group_of_seq(const AttnArgs& a, int s) {
+  if (a.groups == 0 || s < a.g_first[0] || s >= a.g_first[a.groups]) return -1;
+  int lo = 0, hi = a.groups;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.g_first[mid] <= s) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// a block id that does not exist reads block 0: a wrong table costs a wrong result, not a fault
+__device__ __forceinline__ int checked_block(int id, int num_blocks) { return (unsigned)id < (unsigned)num_blocks ? id : 0; }
+
+template <typename T, int FMT>
+__device__ __forceinline__ float page_value(const void* p, int64_t i) {
+  if constexpr (FMT == kInt8) return (float)reinterpret_cast<const int8_t*>(p)[i];
+  else if constexpr (FMT == kE4M3) {
+    __nv_fp8_e4m3 c;
+    c.__x = reinterpret_cast<const uint8_t*>(p)[i];
+    return (float)c;
+  } else return to_f32(reinterpret_cast<const T*>(p)[i]);
+}
+
+// ---------------------------------------------------------------------------------------------------------------- parts of a softmax
+// A part: out = O / l relative to the maximum m (log2): O [d] and (m, l), all 32-bit.  Parts of the same row join in the merge kernel (attn_pages.cu).
+//
+// Lists of few rows (attn_pages_few.cu) are cut where their blocks' runs end: `info` says for each (segment, key head) where its parts lie.
+struct FewInfo {
+  int first_slot;      // of `slots`; < 0: one part, in `whole` (with groups) or already the result (without)
+  int first_block;     // the parts behind the first are the slots 2 j, j = first_block + 1 .. last_block
+  int last_block;
+  int pad;
+};
+
+struct PartArgs {
+  float* slots;        // [2 blocks][rows][d + 2]
+  FewInfo* info;       // [segments][hkv]
+  float* whole_own;    // [total_q][hq][d + 2]
+  float* whole_group;
+  float* tile_own;     // [splits][total_q][hq][d + 2]
+  float* tile_group;
+  int rows;            // of a slot
+  int few_own, few_groups;        // lists of sequences / groups are cut into runs
+  int own_splits, group_splits;   // or into this many stretches of keys each (0: not)
+  int own_chunk, group_chunk;     // keys of a stretch
+};
+
+struct Seg {
+  int lo, hi;          // keys lo .. hi - 1
+  int row0, rows;      // query rows (tokens)
+  const int* table;
+};
+
+// first query row of sequence i, whatever the tables say inside of the call's rows
+__device__ __forceinline__ int row_of(const AttnArgs& a, int i) { return min(max(a.cu[min(max(i, 0), a.num_seqs)], 0), a.total_q); }
+
+__device__ __forceinline__ Seg own_segment(const AttnArgs& a, int i) {
+  Seg s;
+  const int g = group_of_seq(a, i);
+  s.row0 = row_of(a, i);
+  s.rows = row_of(a, i + 1) - s.row0;
+  s.hi = min(a.seq_lens[i], a.max_blocks * a.page);
+  s.lo = g < 0 ? 0 : min(a.g_lens[g], a.g_max_blocks * a.page);
+  s.table = a.tables + (int64_t)i * a.max_blocks;
+  return s;
+}
+__device__ __forceinline__ Seg group_segment(const AttnArgs& a, int g) {
+  Seg s;
+  s.row0 = row_of(a, a.g_first[g]);
+  s.rows = row_of(a, a.g_first[g + 1]) - s.row0;
+  s.lo = 0;
+  s.hi = min(a.g_lens[g], a.g_max_blocks * a.page);
+  s.table = a.g_tables + (int64_t)g * a.g_max_blocks;
+  return s;
+}
+// last key that query row t of sequence s sees
+__device__ __forceinline__ int row_pos(const AttnArgs& a, int s, int t) {
+  return min(a.seq_lens[s] - a.cu[s + 1] + t, a.max_blocks * a.page - 1);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {  // 2^x, one MUFU; 2^-inf = 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// host side: which kernels a call takes, and its scratch
+int few_blocks(int fmt, int d, int rows);                                            // attn_pages_few.cu: blocks of one launch
+int few_launch(const AttnArgs& a, const PartArgs& p, int fmt, int dtype, int blocks, cudaStream_t stream);
+
+}  // namespace pages
