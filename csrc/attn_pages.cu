@@ -105,18 +105,18 @@ __global__ void __launch_bounds__(256) attn_pages_merge_kernel(const __grid_cons
     const FewInfo in = p.info[(int64_t)seg * a.hkv + kvh];
     if (in.first_slot < 0) {
       if (a.groups == 0) return false;
-      add(whole + ((int64_t)t * a.hq + head) * (D + 2));
+      add(whole + ((int64_t)t * a.hq + head) * (D + kPad));
       return true;
     }
     const int n = (t - row0) * group + head % group;
     if (n >= p.rows) return true;
-    add(p.slots + ((int64_t)in.first_slot * p.rows + n) * (D + 2));
-    for (int j = in.first_block + 1; j <= in.last_block; ++j) add(p.slots + ((int64_t)(2 * j) * p.rows + n) * (D + 2));
+    add(p.slots + ((int64_t)in.first_slot * p.rows + n) * (D + kPad));
+    for (int j = in.first_block + 1; j <= in.last_block; ++j) add(p.slots + ((int64_t)(2 * j) * p.rows + n) * (D + kPad));
     return true;
   };
   auto stretches = [&](const float* parts, int lo, int hi, int chunk, int splits) {
     const int n = min(splits, (hi - lo + chunk - 1) / chunk);
-    for (int i = 0; i < n; ++i) add(parts + (((int64_t)i * a.total_q + t) * a.hq + head) * (D + 2));
+    for (int i = 0; i < n; ++i) add(parts + (((int64_t)i * a.total_q + t) * a.hq + head) * (D + kPad));
   };
   if (has_own) {
     if (p.few_own) {
@@ -162,30 +162,58 @@ int launch_merge(const AttnArgs& a, const PartArgs& p, cudaStream_t stream) {
 struct Plan {
   bool any;             // the simple kernel for the whole call
   bool few_own, few_groups;
-  int blocks, rows;
-  int64_t slots, info, whole, floats;
+  int blocks, rows;     // of the kernel for few rows
+  TilePlan tile;
+  int own_splits, own_chunk, group_splits, group_chunk;
+  bool direct;          // the tiled kernel writes the result itself
+  int64_t slots, info, whole, tile_own, tile_group, floats;
 };
 
 // head sizes and pages of the tiled kernels
 bool tiled(int d, int page) { return (d == 64 || d == 128 || d == 256) && page % 16 == 0; }
 
+// Stretches of keys for `blocks` blocks of the tiled kernel: as many as fill the 148 SMs, but none shorter than 256 keys (four tiles; a block's start
+// takes as long as about three).
+void stretches(int64_t blocks, int keys, int& splits, int& chunk) {
+  int64_t n = blocks > 0 ? 148 / blocks : 1;
+  if (n > (keys + 255) / 256) n = (keys + 255) / 256;
+  if (n < 1) n = 1;
+  chunk = (int)(((keys + n - 1) / n + 63) / 64 * 64);
+  if (chunk < 64) chunk = 64;
+  splits = keys > 0 ? (keys + chunk - 1) / chunk : 1;
+}
+
 Plan plan_call(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv, int d, int page, int fmt, int groups, int g_max_len, int g_max_rows) {
   Plan p;
   memset(&p, 0, sizeof(p));
-  (void)max_kv, (void)g_max_len;
   p.any = true;
   if (hkv <= 0 || hq % hkv != 0 || !tiled(d, page)) return p;
-  const int64_t g = hq / hkv;
-  p.few_own = max_q * g <= 16;
-  p.few_groups = groups > 0 && g_max_rows * g <= 16;
-  if (!p.few_own || (groups > 0 && !p.few_groups)) return p;
   p.any = false;
-  p.rows = max_q * g <= 8 && (groups == 0 || g_max_rows * g <= 8) ? 8 : 16;
-  p.blocks = few_blocks(fmt, d, p.rows);
-  p.slots = (int64_t)2 * p.blocks * p.rows * (d + 2);
-  p.info = (int64_t)(num_seqs + groups) * hkv * 4;
-  p.whole = groups > 0 ? (int64_t)total_q * hq * (d + 2) : 0;
-  p.floats = p.slots + p.info + 2 * p.whole;
+  const int64_t g = hq / hkv, own = max_q * g, grouped = groups > 0 ? g_max_rows * g : 0;
+  // up to 16 rows of a key head fit the narrow side of the warp-level product; a tile of 128 costs the tiled kernel the same whatever is in it
+  p.few_own = own <= 16;
+  p.few_groups = groups > 0 && grouped <= 16;
+  if (p.few_own || p.few_groups) {
+    p.rows = (!p.few_own || own <= 8) && (!p.few_groups || grouped <= 8) ? 8 : 16;
+    p.blocks = few_blocks(fmt, d, p.rows);
+    p.slots = (int64_t)2 * p.blocks * p.rows * (d + kPad);
+    p.info = ((int64_t)(p.few_own ? num_seqs : 0) + (p.few_groups ? groups : 0)) * hkv * 4;
+    p.whole = groups > 0 ? (int64_t)total_q * hq * (d + kPad) : 0;
+  }
+  const bool tile_own = !p.few_own, tile_groups = groups > 0 && !p.few_groups;
+  p.tile.rows = tile_rows(d, own > 16 && own > grouped ? own : grouped);
+  if (tile_own) {
+    p.tile.own_tiles = (int)((own + p.tile.rows - 1) / p.tile.rows);
+    stretches((int64_t)p.tile.own_tiles * hkv * num_seqs, max_kv, p.own_splits, p.own_chunk);
+    p.direct = groups == 0 && p.own_splits == 1;
+    if (!p.direct) p.tile_own = (int64_t)p.own_splits * total_q * hq * (d + kPad);
+  }
+  if (tile_groups) {
+    p.tile.group_tiles = (int)((grouped + p.tile.rows - 1) / p.tile.rows);
+    stretches((int64_t)p.tile.group_tiles * hkv * groups, g_max_len, p.group_splits, p.group_chunk);
+    p.tile_group = (int64_t)p.group_splits * total_q * hq * (d + kPad);
+  }
+  p.floats = p.slots + p.info + (p.few_own ? p.whole : 0) + (p.few_groups ? p.whole : 0) + p.tile_own + p.tile_group;
   return p;
 }
 
@@ -197,6 +225,7 @@ int check_args(const AttnArgs& a, int fmt, int dtype) {
   LLMSS_REQUIRE(a.page > 0 && a.num_blocks > 0 && a.max_blocks >= 0, "attn_pages: bad pages (block_size=%d, %d blocks)", a.page, a.num_blocks);
   LLMSS_REQUIRE((int64_t)a.max_blocks * a.page < (1ll << 31) && (int64_t)a.g_max_blocks * a.page < (1ll << 31), "attn_pages: contexts of 2^31 tokens and more");
   LLMSS_REQUIRE((int64_t)a.hq * a.d <= a.ldq && (int64_t)a.hq * a.d <= a.ldo, "attn_pages: q / out columns exceed the row stride");
+  LLMSS_REQUIRE(a.scale_log2 > 0.f && a.scale_log2 < INFINITY, "attn_pages: the score scale must be positive and finite");
   LLMSS_REQUIRE(fmt == kF16Pages || (a.ks != nullptr && a.vs != nullptr), "attn_pages: 8-bit pages need scales");
   LLMSS_REQUIRE(a.groups == 0 || (a.g_tables != nullptr && a.g_lens != nullptr && a.g_first != nullptr), "attn_pages: groups need tables, lengths and firsts");
   LLMSS_REQUIRE(a.ldq % 8 == 0 && a.ldo % 8 == 0 && (((uintptr_t)a.q | (uintptr_t)a.out | (uintptr_t)a.k | (uintptr_t)a.v) % 16) == 0,
@@ -210,7 +239,7 @@ int check_args(const AttnArgs& a, int fmt, int dtype) {
 LLMSS_API int64_t llmss_attn_pages_scratch_floats(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv, int d, int block_size, int fmt,
                                                   int groups, int g_max_len, int g_max_rows) {
   if (num_seqs <= 0 || total_q <= 0 || max_q <= 0) return 0;
-  return plan_call(num_seqs, max_q, max_kv, total_q, hq, hkv, d, block_size, fmt, groups, g_max_len, g_max_rows).floats;
+  return plan_call(num_seqs, max_q, max_kv, total_q, hq, hkv, d, block_size, fmt, g_max_len > 0 ? groups : 0, g_max_len, g_max_rows).floats;
 }
 
 // q [total_q][>= hq * d] (row stride ldq); K / V pages [num_blocks][hkv][block_size][d] of the queries' type (fmt 0) or of bytes with 32-bit scales
@@ -242,7 +271,7 @@ LLMSS_API int llmss_attn_pages(const void* q, int64_t ldq, const void* k_pages, 
   a.total_q = total_q;
   a.max_blocks = max_blocks;
   a.g_max_blocks = g_max_blocks;
-  a.groups = g_max_len > 0 && g_max_blocks > 0 ? groups : 0;
+  a.groups = g_max_len > 0 ? groups : 0;
   a.hq = hq;
   a.hkv = hkv;
   a.d = d;
@@ -254,18 +283,35 @@ LLMSS_API int llmss_attn_pages(const void* q, int64_t ldq, const void* k_pages, 
   if (int e = check_args(a, fmt, dtype)) return e;
   const Plan plan = plan_call(num_seqs, max_q, max_kv, total_q, hq, hkv, d, block_size, fmt, a.groups, g_max_len, g_max_rows);
   if (!plan.any) {
-    LLMSS_REQUIRE(scratch != nullptr && scratch_floats >= plan.floats && ((uintptr_t)scratch % 16) == 0, "attn_pages: %lld floats of 16-byte aligned scratch needed",
+    LLMSS_REQUIRE(plan.floats == 0 || (scratch != nullptr && scratch_floats >= plan.floats && ((uintptr_t)scratch % 16) == 0), "attn_pages: %lld floats of 16-byte aligned scratch needed",
                   (long long)plan.floats);
     PartArgs p;
     memset(&p, 0, sizeof(p));
-    p.slots = (float*)scratch;
-    p.info = (FewInfo*)(p.slots + plan.slots);
-    p.whole_own = p.slots + plan.slots + plan.info;
-    p.whole_group = p.whole_own + plan.whole;
+    float* at = (float*)scratch;
+    auto take = [&](int64_t n) {
+      float* x = at;
+      at += n;
+      return x;
+    };
+    p.slots = take(plan.slots);
+    p.info = (FewInfo*)take(plan.info);
+    p.whole_own = take(plan.few_own ? plan.whole : 0);
+    p.whole_group = take(plan.few_groups ? plan.whole : 0);
+    p.tile_own = take(plan.tile_own);
+    p.tile_group = take(plan.tile_group);
     p.rows = plan.rows;
     p.few_own = plan.few_own;
     p.few_groups = plan.few_groups;
-    if (int e = few_launch(a, p, fmt, dtype, plan.blocks, stream)) return e;
+    p.own_splits = plan.own_splits;
+    p.own_chunk = plan.own_chunk;
+    p.group_splits = plan.group_splits;
+    p.group_chunk = plan.group_chunk;
+    const bool tiles = plan.tile.own_tiles > 0 || plan.tile.group_tiles > 0;
+    if (tiles)
+      if (int e = tile_launch(a, p, plan.tile, fmt, dtype, stream)) return e;
+    if (plan.direct) return 0;
+    if (plan.few_own || plan.few_groups)
+      if (int e = few_launch(a, p, fmt, dtype, plan.blocks, tiles, stream)) return e;
 #define LLMSS_MERGE(T_) return d == 64 ? launch_merge<T_, 64>(a, p, stream) : d == 128 ? launch_merge<T_, 128>(a, p, stream) : launch_merge<T_, 256>(a, p, stream)
     if (dtype == LLMSS_F16) LLMSS_MERGE(__half);
     LLMSS_MERGE(__nv_bfloat16);

@@ -71,7 +71,9 @@ __device__ __forceinline__ float page_value(const void* p, int64_t i) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------- parts of a softmax
-// A part: out = O / l relative to the maximum m (log2): O [d] and (m, l), all 32-bit.  Parts of the same row join in the merge kernel (attn_pages.cu).
+// A part of a row: O [d], then the reference m (log2) and the sum l relative to which O stands, and two numbers of padding; all 32-bit.  Parts of the
+// same row join in the merge kernel (attn_pages.cu).
+constexpr int kPad = 4;
 //
 // Lists of few rows (attn_pages_few.cu) are cut where their blocks' runs end: `info` says for each (segment, key head) where its parts lie.
 struct FewInfo {
@@ -82,11 +84,11 @@ struct FewInfo {
 };
 
 struct PartArgs {
-  float* slots;        // [2 blocks][rows][d + 2]
+  float* slots;        // [2 blocks][rows][d + kPad]
   FewInfo* info;       // [segments][hkv]
-  float* whole_own;    // [total_q][hq][d + 2]
+  float* whole_own;    // [total_q][hq][d + kPad]
   float* whole_group;
-  float* tile_own;     // [splits][total_q][hq][d + 2]
+  float* tile_own;     // [splits][total_q][hq][d + kPad]
   float* tile_group;
   int rows;            // of a slot
   int few_own, few_groups;        // lists of sequences / groups are cut into runs
@@ -135,6 +137,13 @@ __device__ __forceinline__ float exp2_fast(float x) {  // 2^x, one MUFU; 2^-inf 
 
 // host side: which kernels a call takes, and its scratch
 int few_blocks(int fmt, int d, int rows);                                            // attn_pages_few.cu: blocks of one launch
-int few_launch(const AttnArgs& a, const PartArgs& p, int fmt, int dtype, int blocks, cudaStream_t stream);
+// `beside`: starts beside the kernel launched before it, whose results it does not need, and ends behind it
+int few_launch(const AttnArgs& a, const PartArgs& p, int fmt, int dtype, int blocks, bool beside, cudaStream_t stream);
+int tile_rows(int d, int64_t rows);                                                  // attn_pages_tile.cu: query rows of a block
+// row tiles and stretches of keys of sequences (own) and of groups; 0 tiles: not this kernel's
+struct TilePlan {
+  int own_tiles, group_tiles, rows;
+};
+int tile_launch(const AttnArgs& a, const PartArgs& p, const TilePlan& t, int fmt, int dtype, cudaStream_t stream);
 
 }  // namespace pages

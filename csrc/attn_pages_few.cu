@@ -45,6 +45,7 @@ struct Few {
 struct FewArgs {
   int segs;            // lists per key head: sequences (own) and groups
   int own;
+  int beside;          // wait for the kernel before at the end instead of at the start
 };
 
 template <int UNIT>
@@ -108,7 +109,7 @@ attn_pages_few_kernel(const __grid_constant__ AttnArgs a, const __grid_constant_
   int* s_pos = reinterpret_cast<int*>(s_qs + ROWS);                         // [ROWS] last visible key
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
   pdl_launch_dependents();
-  pdl_wait();
+  if (!f.beside) pdl_wait();
 
   // this block's run of the lists
   long long units = 0;
@@ -121,7 +122,10 @@ attn_pages_few_kernel(const __grid_constant__ AttnArgs a, const __grid_constant_
   long long per = (total + gridDim.x - 1) / gridDim.x;
   if (per < kLeastUnits) per = kLeastUnits;
   const long long begin = per * blockIdx.x, end = min(begin + per, total);
-  if (begin >= end) return;
+  if (begin >= end) {
+    pdl_wait();
+    return;
+  }
   int seg = 0;
   long long before = 0;                    // units of the lists of earlier segments, one key head
   for (int b = 0; b < f.segs; b += 32) {
@@ -143,6 +147,8 @@ attn_pages_few_kernel(const __grid_constant__ AttnArgs a, const __grid_constant_
     before += __shfl_sync(0xffffffffu, inc, 31);
   }
 
+  // f16 ends at 2^16 and has no numbers below 2^-24: what is rounded to it is formed times 2^7 (at most 2^15)
+  constexpr float kUp = std::is_same<M, __half>::value ? 7.0f : 0.0f;
   const int group = a.hq / a.hkv;
   const uint8_t* kp = reinterpret_cast<const uint8_t*>(a.k);
   const uint8_t* vp = reinterpret_cast<const uint8_t*>(a.v);
@@ -422,13 +428,13 @@ attn_pages_few_kernel(const __grid_constant__ AttnArgs a, const __grid_constant_
           float p[4];
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const float z = x[i][nt][c], mm = m[nt][c & 1] == -INFINITY ? 0.f : m[nt][c & 1];
+            const float z = x[i][nt][c], mm = m[nt][c & 1] == -INFINITY ? 0.f : m[nt][c & 1] - (FMT == kF16Pages ? kUp : 0.f);
             const float e = exp2_fast(z - mm);
             l[nt][c & 1] += e;
             if constexpr (FMT == kF16Pages) p[c] = e;
             else {
               // a hidden key: 0 whatever its scale is
-              const float mm2 = m2[nt][c & 1] == -INFINITY ? 0.f : m2[nt][c & 1];
+              const float mm2 = m2[nt][c & 1] == -INFINITY ? 0.f : m2[nt][c & 1] - kUp;
               p[c] = z == -INFINITY ? 0.f : exp2_fast(z + lv[i][c >> 1] - mm2);
             }
           }
@@ -493,8 +499,8 @@ attn_pages_few_kernel(const __grid_constant__ AttnArgs a, const __grid_constant_
         const int i = nt * 8 + 2 * t + c;
         if (i < nrows) {
           if (r == 0) {
-            s_m[warp * ROWS + i] = m[nt][c];
-            s_m2[warp * ROWS + i] = FMT != kF16Pages ? m2[nt][c] : m[nt][c];
+            s_m[warp * ROWS + i] = m[nt][c] - (FMT == kF16Pages ? kUp : 0.f);       // what l and O stand relative to
+            s_m2[warp * ROWS + i] = (FMT != kF16Pages ? m2[nt][c] : m[nt][c]) - kUp;
             s_l[warp * ROWS + i] = sum;
           }
           float* dst = s_o + (warp * ROWS + i) * LD;
@@ -509,7 +515,7 @@ attn_pages_few_kernel(const __grid_constant__ AttnArgs a, const __grid_constant_
     const bool whole = u0 == 0 && u1 == n;
     const bool last = whole && a.groups == 0;          // the result itself
     float* part = nullptr;
-    if (!last && !whole) part = pa.slots + (int64_t)(2 * blockIdx.x + (cur > begin ? 1 : 0)) * ROWS * (D + 2);
+    if (!last && !whole) part = pa.slots + (int64_t)(2 * blockIdx.x + (cur > begin ? 1 : 0)) * ROWS * (D + kPad);
     if (u0 == 0 && threadIdx.x == 0) {
       FewInfo in;
       in.first_slot = whole ? -1 : 2 * (int)blockIdx.x + (cur > begin ? 1 : 0);
@@ -544,18 +550,18 @@ attn_pages_few_kernel(const __grid_constant__ AttnArgs a, const __grid_constant_
         T w[4] = {from_f32<T>(y.x * inv), from_f32<T>(y.y * inv), from_f32<T>(y.z * inv), from_f32<T>(y.w * inv)};
         *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + (int64_t)tok * a.ldo + (int64_t)head * D + c) = *reinterpret_cast<const uint2*>(w);
       } else {
-        float* dst = whole ? (seg < f.own ? pa.whole_own : pa.whole_group) + ((int64_t)tok * a.hq + head) * (D + 2) : part + i * (D + 2);
-        *reinterpret_cast<float2*>(dst + c) = make_float2(y.x * back, y.y * back);
-        *reinterpret_cast<float2*>(dst + c + 2) = make_float2(y.z * back, y.w * back);
+        float* dst = whole ? (seg < f.own ? pa.whole_own : pa.whole_group) + ((int64_t)tok * a.hq + head) * (D + kPad) : part + i * (D + kPad);
+        *reinterpret_cast<float4*>(dst + c) = make_float4(y.x * back, y.y * back, y.z * back, y.w * back);
         if (c == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(mx, sum);
       }
     }
     cur += u1 - u0;
   }
+  pdl_wait();
 }
 
 template <typename T, int FMT, int D, int NT>
-int launch(const AttnArgs& a, const PartArgs& p, int blocks, cudaStream_t stream) {
+int launch(const AttnArgs& a, const PartArgs& p, int blocks, bool beside, cudaStream_t stream) {
   using C = Few<FMT, D, NT>;
   static PerDeviceSmem configured;
   auto kern = attn_pages_few_kernel<T, FMT, D, NT>;
@@ -563,7 +569,19 @@ int launch(const AttnArgs& a, const PartArgs& p, int blocks, cudaStream_t stream
   FewArgs f;
   f.own = p.few_own ? a.num_seqs : 0;
   f.segs = f.own + (p.few_groups ? a.groups : 0);
-  LLMSS_CHECK_CUDA(launch_pdl(kern, dim3(blocks), dim3(32 * kWarps), (size_t)C::SMEM, stream, a, p, f));
+  f.beside = beside;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(32 * kWarps);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = beside || llmss_pdl_enabled() ? 1 : 0;
+  LLMSS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, a, p, f));
   return 0;
 }
 
@@ -583,13 +601,13 @@ int few_blocks(int fmt, int d, int rows) {
   return 148 * ctas;
 }
 
-int few_launch(const AttnArgs& a, const PartArgs& p, int fmt, int dtype, int blocks, cudaStream_t stream) {
+int few_launch(const AttnArgs& a, const PartArgs& p, int fmt, int dtype, int blocks, bool beside, cudaStream_t stream) {
   const int d = a.d;
 #define LLMSS_FEW_F(T_)                                                                                                              \
-  LLMSS_FEW_D(if (p.rows == 8) return fmt == kInt8 ? launch<T_, kInt8, D, 1>(a, p, blocks, stream)                                   \
-                                   : fmt == kE4M3 ? launch<T_, kE4M3, D, 1>(a, p, blocks, stream) : launch<T_, kF16Pages, D, 1>(a, p, blocks, stream); \
-              return fmt == kInt8 ? launch<T_, kInt8, D, 2>(a, p, blocks, stream)                                                    \
-                                  : fmt == kE4M3 ? launch<T_, kE4M3, D, 2>(a, p, blocks, stream) : launch<T_, kF16Pages, D, 2>(a, p, blocks, stream))
+  LLMSS_FEW_D(if (p.rows == 8) return fmt == kInt8 ? launch<T_, kInt8, D, 1>(a, p, blocks, beside, stream)                                   \
+                                   : fmt == kE4M3 ? launch<T_, kE4M3, D, 1>(a, p, blocks, beside, stream) : launch<T_, kF16Pages, D, 1>(a, p, blocks, beside, stream); \
+              return fmt == kInt8 ? launch<T_, kInt8, D, 2>(a, p, blocks, beside, stream)                                                    \
+                                  : fmt == kE4M3 ? launch<T_, kE4M3, D, 2>(a, p, blocks, beside, stream) : launch<T_, kF16Pages, D, 2>(a, p, blocks, beside, stream))
   if (dtype == LLMSS_F16) {
     LLMSS_FEW_F(__half);
   }

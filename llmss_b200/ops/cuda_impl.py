@@ -378,7 +378,7 @@ def attention_pages(q_view, out_view, batch, k_pages, v_pages, hq, hkv, d, scale
                               _int32("cu_q", batch.cu_q, q_view, B + 1), B, batch.max_q, batch.max_kv, T, hq, hkv, d, shape[2], shape[0],
                               float(scale), fmt, _DT[q_view.dtype], *g, _ptr(scratch), floats, _stream())
     _lib.check(rc, "llmss_attn_pages")
-    _count(2 if floats else 1)
+    _count(1 if not floats else 3 if g[4] and (batch.max_q * hq <= 16 * hkv) != (p.max_rows * hq <= 16 * hkv) else 2)
 
 
 # --------------------------------------------------------------------------- embed / sample
