@@ -194,8 +194,8 @@ Plan plan_call(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv
   p.few_own = own <= 16;
   p.few_groups = groups > 0 && grouped <= 16;
   if (p.few_own || p.few_groups) {
-    p.rows = (!p.few_own || own <= 8) && (!p.few_groups || grouped <= 8) ? 8 : 16;
-    p.blocks = few_blocks(fmt, d, p.rows);
+    p.rows = (int)(p.few_own && (!p.few_groups || own >= grouped) ? own : grouped);
+    p.blocks = few_blocks(fmt, d, p.rows, (p.few_own ? num_seqs : 0) + (p.few_groups ? groups : 0));
     p.slots = (int64_t)2 * p.blocks * p.rows * (d + kPad);
     p.info = ((int64_t)(p.few_own ? num_seqs : 0) + (p.few_groups ? groups : 0)) * hkv * 4;
     p.whole = groups > 0 ? (int64_t)total_q * hq * (d + kPad) : 0;
@@ -224,6 +224,11 @@ int check_args(const AttnArgs& a, int fmt, int dtype) {
   LLMSS_REQUIRE(a.d > 0 && a.d % 8 == 0 && a.d <= 256, "attn_pages: head_dim=%d must be a multiple of 8 up to 256", a.d);
   LLMSS_REQUIRE(a.page > 0 && a.num_blocks > 0 && a.max_blocks >= 0, "attn_pages: bad pages (block_size=%d, %d blocks)", a.page, a.num_blocks);
   LLMSS_REQUIRE((int64_t)a.max_blocks * a.page < (1ll << 31) && (int64_t)a.g_max_blocks * a.page < (1ll << 31), "attn_pages: contexts of 2^31 tokens and more");
+  LLMSS_REQUIRE(((int64_t)(a.num_seqs + a.groups) * (a.max_blocks > a.g_max_blocks ? a.max_blocks : a.g_max_blocks)) * (a.page / 16 + 1) * a.hkv < (1ll << 31),
+                "attn_pages: lists of 2^35 keys and more (%d sequences of up to %d pages)", a.num_seqs, a.max_blocks);
+  LLMSS_REQUIRE((int64_t)a.page * a.page * (a.max_blocks > a.g_max_blocks ? a.max_blocks : a.g_max_blocks) < (1ll << 39), "attn_pages: pages too large (%d)", a.page);
+  LLMSS_REQUIRE((int64_t)a.num_blocks * a.hkv * a.page < (1ll << 31), "attn_pages: 2^31 cache rows and more");
+  LLMSS_REQUIRE((((uintptr_t)a.ks | (uintptr_t)a.vs) % 16) == 0, "attn_pages: scales must be 16-byte aligned");
   LLMSS_REQUIRE((int64_t)a.hq * a.d <= a.ldq && (int64_t)a.hq * a.d <= a.ldo, "attn_pages: q / out columns exceed the row stride");
   LLMSS_REQUIRE(a.scale_log2 > 0.f && a.scale_log2 < INFINITY, "attn_pages: the score scale must be positive and finite");
   LLMSS_REQUIRE(fmt == kF16Pages || (a.ks != nullptr && a.vs != nullptr), "attn_pages: 8-bit pages need scales");

@@ -136,7 +136,7 @@ __device__ __forceinline__ float exp2_fast(float x) {  // 2^x, one MUFU; 2^-inf 
 }
 
 // host side: which kernels a call takes, and its scratch
-int few_blocks(int fmt, int d, int rows);                                            // attn_pages_few.cu: blocks of one launch
+int few_blocks(int fmt, int d, int rows, int segs);                                       // attn_pages_few.cu: blocks of one launch
 // `beside`: starts beside the kernel launched before it, whose results it does not need, and ends behind it
 int few_launch(const AttnArgs& a, const PartArgs& p, int fmt, int dtype, int blocks, bool beside, cudaStream_t stream);
 int tile_rows(int d, int64_t rows);                                                  // attn_pages_tile.cu: query rows of a block

@@ -209,13 +209,28 @@ attn_pages_tile_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
       return i == 0 ? 0 : value ? (i - 2) / 2 : (i + 1) / 2;
     };
     const int total = 2 * n_tiles;
-    // global place of chunk c of this thread in tile j, or null outside of the list
-    auto source = [&](int j, int c, int64_t& row) {
-      const int x = c * (32 * kLoaders) + tid, key = base + j * BN + x / PER;
-      const bool in = key >= s.lo && key < k_hi;
-      row = 0;
-      if (in) row = ((int64_t)checked_block(__ldg(s.table + key / a.page), a.num_blocks) * a.hkv + kvh) * a.page + key % a.page;
-      return in;
+    // cache rows of a tile's four runs of 16 keys (a run lies in one page), one per lane of each four; looked up a tile ahead of the copies
+    auto look_up = [&](int j) {
+      const int key = base + j * BN + (lane & 3) * 16;
+      return key < k_hi ? ((uint32_t)checked_block(__ldg(s.table + key / a.page), a.num_blocks) * a.hkv + kvh) * a.page + key % a.page : 0u;
+    };
+    uint32_t runs = look_up(0), runs_before = 0, runs_next = 0;       // of the newest tile of keys, of the one before, of the next one
+    int newest = -1;
+    // turn to the i-th of the ring: its tile, and the cache row of this thread's chunk c with whether that lies in the list
+    auto turn = [&](int i, bool& value, uint32_t& mine) {
+      const int j = tile_of(i, value);
+      if (!value) {
+        if (j > 0) runs_before = runs, runs = runs_next;
+        newest = j;
+        runs_next = look_up(j + 1);
+      }
+      mine = j == newest ? runs : runs_before;
+      return base + j * BN;
+    };
+    auto place = [&](int first, uint32_t mine, int c, uint32_t& row) {
+      const int key = (c * (32 * kLoaders) + tid) / PER;
+      row = __shfl_sync(0xffffffffu, mine, key >> 4) + (key & 15);
+      return first + key >= s.lo && first + key < k_hi;
     };
     if constexpr (FMT == kF16Pages) {
       constexpr int LAG = C::SLOTS - 2;                  // tiles in flight
@@ -227,16 +242,17 @@ attn_pages_tile_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
       for (int i = 0; i < total + LAG; ++i) {
         if (i < total) {
           bool value;
-          const int j = tile_of(i, value);
+          uint32_t mine;
+          const int first = turn(i, value, mine);
           mbar_wait(&bar_empty[i % C::SLOTS], ((i / C::SLOTS) & 1) ^ 1, 80);
           const uint32_t dst = smem_u32(s_kv + (i % C::SLOTS) * C::SLOT);
           const uint8_t* src = reinterpret_cast<const uint8_t*>(value ? a.v : a.k);
 #pragma unroll
           for (int c = 0; c < C::CH; ++c) {
-            int64_t row;
-            const bool in = source(j, c, row);
+            uint32_t row;
+            const bool in = place(first, mine, c, row);
             const int x = c * (32 * kLoaders) + tid, key = x / PER, ch = x % PER;
-            copy16(dst + (ch >> 3) * (BN * 128) + key * 128 + (((ch & 7) ^ (key & 7)) << 4), src + row * (D * 2) + ch * 16, in ? 16 : 0);
+            copy16(dst + (ch >> 3) * (BN * 128) + key * 128 + (((ch & 7) ^ (key & 7)) << 4), src + (in ? (uint64_t)row * (D * 2) + ch * 16 : 0), in ? 16 : 0);
           }
         }
         copies_commit();
@@ -249,17 +265,18 @@ attn_pages_tile_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
       auto fetch = [&](int i) {
         if (i < total) {
           bool value;
-          const int j = tile_of(i, value);
+          uint32_t mine;
+          const int first = turn(i, value, mine);
           uint8_t* raw = s_raw + (i % C::RAWS) * C::RAW;
           const uint8_t* src = reinterpret_cast<const uint8_t*>(value ? a.v : a.k);
           const float* sc = value ? a.vs : a.ks;
 #pragma unroll
           for (int c = 0; c < C::CH; ++c) {
-            int64_t row;
-            const bool in = source(j, c, row);
+            uint32_t row;
+            const bool in = place(first, mine, c, row);
             const int x = c * (32 * kLoaders) + tid;
-            copy16(smem_u32(raw + x * 16), src + row * D + (x % PER) * 16, in ? 16 : 0);
-            copy4(smem_u32(raw + C::CH * 32 * kLoaders * 16 + x * 4), sc + row, in ? 4 : 0);
+            copy16(smem_u32(raw + x * 16), src + (in ? (uint64_t)row * D + (x % PER) * 16 : 0), in ? 16 : 0);
+            copy4(smem_u32(raw + C::CH * 32 * kLoaders * 16 + x * 4), sc + (in ? row : 0), in ? 4 : 0);
           }
         }
         copies_commit();
