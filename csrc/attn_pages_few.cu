@@ -142,8 +142,21 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   for (int i = threadIdx.x; i < min(f.segs, kKept); i += 32 * kWarps) s_units[i] = units_of<UNIT>(segment<UNIT>(a, f, i));
   __syncthreads();
   auto count = [&](int i) { return i < kKept ? s_units[i] : units_of<UNIT>(segment<UNIT>(a, f, i)); };
-  unsigned units = 0;                      // the host has checked that all lists are below 2^31
-  for (int b = 0; b < f.segs; b += 32) units += __reduce_add_sync(0xffffffffu, b + lane < f.segs ? count(b + lane) : 0);
+  // (the host has checked that all lists together are below 2^31)
+  auto scan = [&](int b, int& n) {         // lists b .. b + 31: this lane's units, and those up to it
+    n = b + lane < f.segs ? count(b + lane) : 0;
+    int inc = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += x;
+    }
+    return inc;
+  };
+  int n0;
+  const int inc0 = scan(0, n0);
+  unsigned units = __shfl_sync(0xffffffffu, inc0, 31);
+  for (int b = 32; b < f.segs; b += 32) units += __reduce_add_sync(0xffffffffu, b + lane < f.segs ? count(b + lane) : 0);
   const unsigned total = units * a.hkv;
   const unsigned per = max((total + gridDim.x - 1) / gridDim.x, (unsigned)kLeastUnits);
   const unsigned begin = min(per * blockIdx.x, total), end = min(begin + per, total);
@@ -154,13 +167,8 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   int seg = 0;
   unsigned before = 0;                     // units of the lists of earlier segments, one key head
   for (int b = 0; b < f.segs; b += 32) {
-    const int n = b + lane < f.segs ? count(b + lane) : 0;
-    int inc = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += x;
-    }
+    int n = n0, inc = inc0;
+    if (b > 0) inc = scan(b, n);
     const unsigned hit = __ballot_sync(0xffffffffu, (before + inc) * a.hkv > begin);
     if (hit) {
       const int w = __ffs(hit) - 1;
@@ -201,6 +209,7 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   Place w;
   w.seg = seg, w.before = before, w.cur = begin;
   open(w);
+  Place z = w;                             // the products' place
   int blocks[SUB];
   bool more = true;
   auto settle = [&]() {                    // to a unit that exists; its blocks are looked up here and used at the next copy
@@ -257,50 +266,62 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   if constexpr (C::ROW == 128) v_off[0] = 2 * t * 128 + ((r ^ (2 * t)) << 4), v_off[1] = v1 * 128 + ((r ^ v1) << 4);
   else v_off[0] = 2 * t * 64 + (((r >> 1) ^ t) << 4) + (r & 1) * 8, v_off[1] = v1 * 64 + (((r >> 1) ^ (v1 >> 1)) << 4) + (r & 1) * 8;
 
-  Place z;
-  z.seg = seg, z.before = before;
+  // a list's queries, read while the list before is finished: rows warp, warp + kWarps ..
+  constexpr int QR = ROWS / kWarps, QC = (D + 127) / 128;
+  uint2 q_raw[QR][QC];
+  int q_pos[QR];
+  auto read_queries = [&]() {
+#pragma unroll
+    for (int k = 0; k < QR; ++k) {
+      const int i = warp + k * kWarps, tok = z.s.row0 + i / group;
+      const bool live = i < min(z.s.rows * group, f.rows);
+      const T* qr = reinterpret_cast<const T*>(a.q) + (int64_t)tok * a.ldq + (int64_t)(z.kvh * group + i % group) * D;
+#pragma unroll
+      for (int c = 0; c < QC; ++c) {
+        q_raw[k][c] = make_uint2(0u, 0u);
+        if (live && c * 128 + lane * 4 < D) q_raw[k][c] = *reinterpret_cast<const uint2*>(qr + c * 128 + lane * 4);
+      }
+      q_pos[k] = -1;
+      if (live) {
+        const int sq = z.seg < f.own ? z.seg : seq_of_row(a.cu, 0, a.num_seqs, tok);
+        q_pos[k] = sq < 0 ? -1 : min(row_pos(a, sq, tok), z.s.hi - 1);
+      }
+    }
+  };
+  read_queries();
+
   for (unsigned cur = begin; cur < end;) {
-    z.cur = cur;
-    open(z);
-    const Seg& s = z.s;
+    const Seg s = z.s;
     const int n = z.n, kvh = z.kvh, u0 = z.u0, u1 = z.u1, base = z.base;
     seg = z.seg;
     const int nrows = min(s.rows * group, f.rows);
 
     // ---- queries: fragments, score factors, last visible keys
     __syncthreads();                       // the list before is done with the buffers
-    for (int i = warp; i < ROWS; i += kWarps) {
-      const int tok = s.row0 + i / group;
-      const bool live = i < nrows;
-      const T* qr = reinterpret_cast<const T*>(a.q) + (int64_t)tok * a.ldq + (int64_t)(kvh * group + i % group) * D;
-      uint2 raw[(D + 127) / 128];
-      float m = 0.f;
 #pragma unroll
-      for (int c = 0; c < (D + 127) / 128; ++c) {
-        raw[c] = make_uint2(0u, 0u);
-        const int d0 = c * 128 + lane * 4;
-        if (live && d0 < D) raw[c] = *reinterpret_cast<const uint2*>(qr + d0);
-        if constexpr (FMT != kF16Pages) {
-          const T* e = reinterpret_cast<const T*>(&raw[c]);
+    for (int k = 0; k < QR; ++k) {
+      const int i = warp + k * kWarps;
+      float up = 1.f, qs = a.scale_log2, sum = 0.f;
+      if constexpr (FMT != kF16Pages) {
+        float m = 0.f;
+#pragma unroll
+        for (int c = 0; c < QC; ++c) {
+          const T* e = reinterpret_cast<const T*>(&q_raw[k][c]);
 #pragma unroll
           for (int j = 0; j < 4; ++j) m = fmaxf(m, fabsf(to_f32(e[j])));
         }
-      }
-      float up = 1.f, qs = a.scale_log2;
-      if constexpr (FMT != kF16Pages) {
         m = warp_max(m);
         const int e = m > 0.f && m < INFINITY ? max(-126, min(126, (int)((__float_as_uint(m) >> 23) & 255) - 127)) : 0;
         up = __int_as_float((127 - e) << 23);
         qs *= __int_as_float((127 + e) << 23);
       }
-      float sum = 0.f;
 #pragma unroll
-      for (int c = 0; c < (D + 127) / 128; ++c) {
+      for (int c = 0; c < QC; ++c) {
         const int d0 = c * 128 + lane * 4;
         if (d0 < D) {
-          uint2 w = raw[c];
+          uint2 w = q_raw[k][c];
           if constexpr (FMT != kF16Pages) {
-            const T* e = reinterpret_cast<const T*>(&raw[c]);
+            const T* e = reinterpret_cast<const T*>(&q_raw[k][c]);
             float x[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[j] = to_f32(e[j]) * up;
@@ -321,12 +342,7 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
       if (lane == 0) {
         s_qb[i] = qs * 128.f * sum;
         s_qs[i] = FMT == kInt8 ? qs * 16777216.f : qs;
-        int pos = -1;
-        if (live) {
-          const int sq = seg < f.own ? seg : seq_of_row(a.cu, 0, a.num_seqs, tok);
-          pos = sq < 0 ? -1 : min(row_pos(a, sq, tok), s.hi - 1);
-        }
-        s_pos[i] = pos;
+        s_pos[i] = q_pos[k];
       }
     }
     __syncthreads();
@@ -595,6 +611,12 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
           }
         }
       }
+    const unsigned next = cur + (u1 - u0);
+    if (next < end) {
+      z.cur = next;
+      open(z);
+      read_queries();
+    }
     __syncthreads();
     const bool whole = u0 == 0 && u1 == n;
     const bool last = whole && a.groups == 0;          // the result itself
@@ -639,7 +661,7 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         if (c == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(mx, sum);
       }
     }
-    cur += u1 - u0;
+    cur = next;
   }
   pdl_wait();
 }

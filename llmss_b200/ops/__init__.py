@@ -135,16 +135,17 @@ def attention(qkv, out, batch, k_cache, v_cache, hq, hkv, d, scale, q_off, k_off
     prompt was cut into portions).  ``batch.prefix``: tokens that groups of sequences share are read once per group, from pages of either
     kind.  Both take any mix of lengths; rows without a visible key become zero, rows of no sequence stay as they are.
     """
+    if batch.prefix is not None or isinstance(k_cache, QuantPages):
+        if _cuda(qkv):
+            cu.attention_pages(qkv, out, batch, k_cache, v_cache, hq, hkv, d, scale, q_off, out_off)
+        else:
+            n = int(batch.cu_q[-1])
+            out[:n, out_off:out_off + hq * d] = ref.attention_pages(qkv[:n, q_off:q_off + hq * d].reshape(n, hq, d), k_cache, v_cache, batch,
+                                                                    scale).reshape(n, hq * d)
+        return out
     T = qkv.shape[0]
     q_view = qkv[:, q_off:q_off + hq * d]
     out_view = out[:, out_off:out_off + hq * d]
-    if batch.prefix is not None or isinstance(k_cache, QuantPages):
-        if _cuda(qkv):
-            cu.attention_pages(q_view, out_view, batch, k_cache, v_cache, hq, hkv, d, scale)
-        else:
-            n = int(batch.cu_q[-1])
-            out_view[:n] = ref.attention_pages(q_view[:n].reshape(n, hq, d), k_cache, v_cache, batch, scale).reshape(n, hq * d)
-        return out
     if _cuda(qkv):
         if d not in (64, 128, 256):
             _warn_once(f"head_dim={d} has no sm_100a attention kernel (64/128/256 do); using the generic PyTorch path")

@@ -311,72 +311,81 @@ def attn_prefill_paged(q_view, k_cache, v_cache, block_tables, seq_lens, out_vie
 
 
 # --------------------------------------------------------------------------- 8-bit pages, shared prefixes
-def _on_its_device(fn):
-    """Launches go to the current device's stream: a call whose tensors lie on another device makes that one current for itself."""
-    @functools.wraps(fn)
-    def run(x, *args, **kw):
-        if x.get_device() == torch._C._cuda_getDevice():
-            return fn(x, *args, **kw)
-        with torch.cuda.device(x.device):
-            return fn(x, *args, **kw)
-    return run
+_HALVES = (torch.float16, torch.bfloat16)
 
 
-def _int32(name, t, like, n=None):
-    if t.dtype is not torch.int32 or not t.is_contiguous() or t.get_device() != like.get_device() or (n is not None and t.numel() < n):
-        raise ValueError(f"{name}: contiguous int32 on {like.device}{'' if n is None else f', {n} numbers or more'}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
+def _wrong_ints(dev, *tensors):
+    """Whether one of the tensors is not contiguous int32 on device ``dev``."""
+    for t in tensors:
+        if t.dtype is not torch.int32 or not t.is_contiguous() or t.get_device() != dev:
+            return True
+    return False
 
 
-@_on_its_device
 def rope_kv_write_q8(qkv, positions, slot_mapping, k_pages, v_pages, hq, hkv, d, rotary_dim, style, base, q_off, k_off, v_off):
-    lib = _lib.load()
+    dev = qkv.get_device()
+    if dev != torch._C._cuda_getDevice():       # launches go to the current device's stream
+        with torch.cuda.device(dev):
+            return rope_kv_write_q8(qkv, positions, slot_mapping, k_pages, v_pages, hq, hkv, d, rotary_dim, style, base, q_off, k_off, v_off)
     T, _, ld = _rows2d(qkv)
-    shape = k_pages.shape
-    if shape != v_pages.shape or k_pages.dtype is not v_pages.dtype or shape[1] != hkv or shape[3] != d or k_pages.device != qkv.device:
-        raise ValueError(f"rope_kv_write: pages {tuple(shape)} / {tuple(v_pages.shape)} for {hkv} heads of {d} on {qkv.device}")
-    if qkv.dtype not in (torch.float16, torch.bfloat16):
+    k, v = k_pages.data, v_pages.data
+    shape, dtype = k.shape, k.dtype
+    if shape != v.shape or dtype is not v.dtype or shape[1] != hkv or shape[3] != d or k.get_device() != dev or v.get_device() != dev:
+        raise ValueError(f"rope_kv_write: pages {tuple(shape)} of {dtype} / {tuple(v.shape)} of {v.dtype} for {hkv} heads of {d} on {qkv.device}")
+    if qkv.dtype not in _HALVES:
         raise TypeError(f"rope_kv_write: 8-bit pages are written from float16 or bfloat16, got {qkv.dtype}")
-    rc = lib.llmss_rope_kv_write_q8(qkv.data_ptr(), _int32("positions", positions, qkv, T), _int32("slot_mapping", slot_mapping, qkv, T),
-                                    k_pages.data.data_ptr(), k_pages.scale.data_ptr(), v_pages.data.data_ptr(), v_pages.scale.data_ptr(), T, ld, hq,
-                                    hkv, d, rotary_dim, style, float(base), q_off, k_off, v_off, shape[2], shape[0], FORMATS[k_pages.dtype],
-                                    _DT[qkv.dtype], _stream())
+    if _wrong_ints(dev, positions, slot_mapping) or positions.numel() < T or slot_mapping.numel() < T:
+        raise ValueError(f"rope_kv_write: positions and slot_mapping are contiguous int32 on {qkv.device}, {T} numbers or more")
+    rc = _lib.load().llmss_rope_kv_write_q8(qkv.data_ptr(), positions.data_ptr(), slot_mapping.data_ptr(), k.data_ptr(), k_pages.scale.data_ptr(),
+                                            v.data_ptr(), v_pages.scale.data_ptr(), T, ld, hq, hkv, d, rotary_dim, style, float(base), q_off, k_off,
+                                            v_off, shape[2], shape[0], FORMATS[dtype], _DT[qkv.dtype], _stream())
     _lib.check(rc, "llmss_rope_kv_write_q8")
     _count()
 
 
-@_on_its_device
-def attention_pages(q_view, out_view, batch, k_pages, v_pages, hq, hkv, d, scale):
-    """Attention over 8-bit pages, and over pages of either kind that groups of sequences share (``batch.prefix``)."""
-    lib = _lib.load()
-    T, _, ldq = _rows2d(q_view)
-    quant, shape, p, bt = isinstance(k_pages, QuantPages), k_pages.shape, batch.prefix, batch.block_tables
-    if quant != isinstance(v_pages, QuantPages) or k_pages.dtype is not v_pages.dtype or shape != v_pages.shape or len(shape) != 4 \
-            or shape[1] != hkv or shape[3] != d or k_pages.device != q_view.device or v_pages.device != q_view.device:
-        raise ValueError(f"attention: pages {tuple(shape)} / {tuple(v_pages.shape)} of {k_pages.dtype} / {v_pages.dtype} for {hkv} heads of {d}")
-    if q_view.dtype not in (torch.float16, torch.bfloat16) or out_view.dtype is not q_view.dtype or out_view.shape != q_view.shape \
-            or out_view.stride(1) != 1 or out_view.device != q_view.device:
-        raise TypeError(f"attention: float16 or bfloat16 queries and an output like them, got {q_view.dtype} {tuple(q_view.shape)} and "
-                        f"{out_view.dtype} {tuple(out_view.shape)}")
-    if quant:
-        k, v, ks, vs, fmt = k_pages.data, v_pages.data, k_pages.scale.data_ptr(), v_pages.scale.data_ptr(), FORMATS[k_pages.dtype]
+_NO_GROUPS = (None, 0, None, None, 0, 0, 0)
+
+
+def attention_pages(qkv, out, batch, k_pages, v_pages, hq, hkv, d, scale, q_off=0, out_off=0):
+    """Attention over 8-bit pages, and over pages of either kind that groups of sequences share (``batch.prefix``): queries are the columns
+    q_off .. of ``qkv``, results the columns out_off .. of ``out``."""
+    dev = qkv.get_device()
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return attention_pages(qkv, out, batch, k_pages, v_pages, hq, hkv, d, scale, q_off, out_off)
+    dtype, B, p = qkv.dtype, batch.num_seqs, batch.prefix
+    if type(k_pages) is QuantPages and type(v_pages) is QuantPages:
+        k, v, ks, vs = k_pages.data, v_pages.data, k_pages.scale.data_ptr(), v_pages.scale.data_ptr()
+        fmt = FORMATS[k.dtype]
     else:
         k, v, ks, vs, fmt = k_pages, v_pages, None, None, 0
-        if k.dtype is not q_view.dtype or not (k.is_contiguous() and v.is_contiguous()):
-            raise ValueError(f"attention: contiguous pages of the queries' type or QuantPages, got {k.dtype} for {q_view.dtype}")
-    B = batch.num_seqs
-    g = (None, 0, None, None, 0, 0, 0)
+        if k.dtype is not dtype or not (k.is_contiguous() and v.is_contiguous()):
+            raise ValueError(f"attention: contiguous pages of the queries' type, or QuantPages both, got {k.dtype} and {v.dtype} for {dtype}")
+    shape = k.shape
+    if shape != v.shape or k.dtype is not v.dtype or len(shape) != 4 or shape[1] != hkv or shape[3] != d or k.get_device() != dev or v.get_device() != dev:
+        raise ValueError(f"attention: pages {tuple(shape)} of {k.dtype} / {tuple(v.shape)} of {v.dtype} for {hkv} heads of {d} on {qkv.device}")
+    (T, wide), (ldq, one) = qkv.shape, qkv.stride()
+    (rows, out_wide), (ldo, out_one) = out.shape, out.stride()
+    if dtype not in _HALVES or out.dtype is not dtype or rows < T or one != 1 or out_one != 1 or out.get_device() != dev \
+            or q_off < 0 or out_off < 0 or q_off + hq * d > wide or out_off + hq * d > out_wide:
+        raise TypeError(f"attention: float16 or bfloat16 queries and an output like them, {hq} heads of {d}, got {dtype} {tuple(qkv.shape)} and "
+                        f"{out.dtype} {tuple(out.shape)}")
+    bt, sl, cu_q = batch.block_tables, batch.seq_lens, batch.cu_q
+    if _wrong_ints(dev, bt, sl, cu_q) or bt.shape[0] < B or sl.numel() < B or cu_q.numel() < B + 1:
+        raise ValueError(f"attention: block_tables, seq_lens and cu_q are contiguous int32 on {qkv.device}, of {B} sequences or more")
+    g = _NO_GROUPS
     if p is not None and p.max_len > 0 and p.block_tables.shape[1] > 0:
         G = p.num_groups
-        g = (_int32("prefix.block_tables", p.block_tables, q_view, G), p.block_tables.shape[1], _int32("prefix.lens", p.lens, q_view, G),
-             _int32("prefix.first", p.first, q_view, G + 1), G, p.max_len, p.max_rows)
+        if _wrong_ints(dev, p.block_tables, p.lens, p.first) or p.block_tables.shape[0] < G or p.lens.numel() < G or p.first.numel() < G + 1:
+            raise ValueError(f"attention: prefix.block_tables, lens and first are contiguous int32 on {qkv.device}, of {G} groups or more")
+        g = (p.block_tables.data_ptr(), p.block_tables.shape[1], p.lens.data_ptr(), p.first.data_ptr(), G, p.max_len, p.max_rows)
+    lib = _lib.load()
     floats = lib.llmss_attn_pages_scratch_floats(B, batch.max_q, batch.max_kv, T, hq, hkv, d, shape[2], fmt, g[4], g[5], g[6])
     # a scratch of the call's own: two streams, or two captured graphs, never meet in it
-    scratch = torch.empty(floats, dtype=torch.float32, device=q_view.device) if floats else None
-    rc = lib.llmss_attn_pages(q_view.data_ptr(), ldq, k.data_ptr(), ks, v.data_ptr(), vs, _int32("block_tables", bt, q_view, B), bt.shape[1],
-                              _int32("seq_lens", batch.seq_lens, q_view, B), out_view.data_ptr(), out_view.stride(0),
-                              _int32("cu_q", batch.cu_q, q_view, B + 1), B, batch.max_q, batch.max_kv, T, hq, hkv, d, shape[2], shape[0],
-                              float(scale), fmt, _DT[q_view.dtype], *g, _ptr(scratch), floats, _stream())
+    scratch = torch.empty(floats, dtype=torch.float32, device=qkv.device) if floats else None
+    rc = lib.llmss_attn_pages(qkv.data_ptr() + 2 * q_off, ldq, k.data_ptr(), ks, v.data_ptr(), vs, bt.data_ptr(), bt.shape[1], sl.data_ptr(),
+                              out.data_ptr() + 2 * out_off, ldo, cu_q.data_ptr(), B, batch.max_q, batch.max_kv, T, hq, hkv, d, shape[2], shape[0],
+                              float(scale), fmt, _DT[dtype], *g, None if scratch is None else scratch.data_ptr(), floats, _stream())
     _lib.check(rc, "llmss_attn_pages")
     _count(1 if not floats else 3 if g[4] and (batch.max_q * hq <= 16 * hkv) != (p.max_rows * hq <= 16 * hkv) else 2)
 

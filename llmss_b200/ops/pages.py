@@ -22,12 +22,12 @@ class QuantPages:
     def __init__(self, data: torch.Tensor, scale: torch.Tensor):
         if data.dtype not in FORMATS:
             raise TypeError(f"QuantPages: pages are int8 or float8_e4m3fn, got {data.dtype}")
-        if data.dim() != 4 or scale.dtype is not torch.float32 or scale.shape != data.shape[:3]:
+        if scale.dtype is not torch.float32 or data.dim() != 4 or scale.shape != data.shape[:3]:
             raise ValueError(f"QuantPages: pages [blocks, heads, block, d] with 32-bit scales [blocks, heads, block], got {tuple(data.shape)} and "
                              f"{scale.dtype} {tuple(scale.shape)}")
         if not (data.is_contiguous() and scale.is_contiguous()):
             raise ValueError("QuantPages: pages and scales must be contiguous")
-        if data.device != scale.device:
+        if data.get_device() != scale.get_device():
             raise ValueError(f"QuantPages: pages on {data.device}, scales on {scale.device}")
         self.data, self.scale = data, scale
 
