@@ -3,6 +3,39 @@
 
 namespace {
 
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_entry() {
+  static EncodeTiled fn = nullptr;
+  if (fn == nullptr) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess) fn = (EncodeTiled)p;
+  }
+  return fn;
+}
+
+}  // namespace
+
+namespace pages {
+
+int encode_pages(CUtensorMap* map, const void* base, int64_t rows, int bytes, int box_rows) {
+  EncodeTiled enc = encode_entry();
+  LLMSS_REQUIRE(enc != nullptr, "attn_pages: cuTensorMapEncodeTiled entry point not available");
+  cuuint64_t dims[2] = {(cuuint64_t)bytes, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)bytes};
+  cuuint32_t box[2] = {(cuuint32_t)(bytes < 128 ? bytes : 128), (cuuint32_t)box_rows};
+  cuuint32_t one[2] = {1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         bytes < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  LLMSS_REQUIRE(r == CUDA_SUCCESS, "attn_pages: cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+  return 0;
+}
+
+}  // namespace pages
+
+namespace {
+
 using namespace pages;
 
 // ---------------------------------------------------------------------------------------------------------------- any shape
@@ -172,14 +205,17 @@ struct Plan {
 // head sizes and pages of the tiled kernels
 bool tiled(int d, int page) { return (d == 64 || d == 128 || d == 256) && page % 16 == 0; }
 
-// Stretches of keys for `blocks` blocks of the tiled kernel: as many as fill the 148 SMs, but none shorter than 256 keys (four tiles; a block's start
-// takes as long as about three).
-void stretches(int64_t blocks, int keys, int& splits, int& chunk) {
-  int64_t n = blocks > 0 ? 148 / blocks : 1;
-  if (n > (keys + 255) / 256) n = (keys + 255) / 256;
-  if (n < 1) n = 1;
-  chunk = (int)(((keys + n - 1) / n + 63) / 64 * 64);
-  if (chunk < 64) chunk = 64;
+// Stretches of keys for `blocks` blocks of the tiled kernel, as many as make the call shortest: the blocks' waves over 148 SMs times a block's tiles of 64
+// keys, where its start and end take as long as about five (measured: 6000 and 1100 clocks), and a merge that no other part of the call asks for as about
+// eight.
+void stretches(int64_t blocks, int keys, bool merged, int& splits, int& chunk) {
+  const int64_t tiles = (keys + 63) / 64;
+  int64_t best = 1, cost = -1;
+  for (int64_t n = 1; n <= 148 && n <= (tiles + 1) / 2; ++n) {
+    const int64_t c = (blocks * n + 147) / 148 * ((tiles + n - 1) / n + 5) + (n > 1 && !merged ? 8 : 0);
+    if (cost < 0 || c < cost) best = n, cost = c;
+  }
+  chunk = (int)(tiles > 0 ? (tiles + best - 1) / best * 64 : 64);
   splits = keys > 0 ? (keys + chunk - 1) / chunk : 1;
 }
 
@@ -204,13 +240,16 @@ Plan plan_call(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv
   p.tile.rows = tile_rows(d, own > 16 && own > grouped ? own : grouped);
   if (tile_own) {
     p.tile.own_tiles = (int)((own + p.tile.rows - 1) / p.tile.rows);
-    stretches((int64_t)p.tile.own_tiles * hkv * num_seqs, max_kv, p.own_splits, p.own_chunk);
+    // behind a prefix a sequence's own keys are few: the longest sequence less the longest prefix stands for them.  A guess costs time alone: the last stretch
+    // of a list takes whatever is left of it, and a block without keys is not free (a microsecond on its SM)
+    const int keys = groups > 0 ? (max_kv - g_max_len > max_q ? max_kv - g_max_len : max_q) : max_kv;
+    stretches((int64_t)p.tile.own_tiles * hkv * num_seqs, keys, groups > 0, p.own_splits, p.own_chunk);
     p.direct = groups == 0 && p.own_splits == 1;
     if (!p.direct) p.tile_own = (int64_t)p.own_splits * total_q * hq * (d + kPad);
   }
   if (tile_groups) {
     p.tile.group_tiles = (int)((grouped + p.tile.rows - 1) / p.tile.rows);
-    stretches((int64_t)p.tile.group_tiles * hkv * groups, g_max_len, p.group_splits, p.group_chunk);
+    stretches((int64_t)p.tile.group_tiles * hkv * groups, g_max_len, true, p.group_splits, p.group_chunk);
     p.tile_group = (int64_t)p.group_splits * total_q * hq * (d + kPad);
   }
   p.floats = p.slots + p.info + (p.few_own ? p.whole : 0) + (p.few_groups ? p.whole : 0) + p.tile_own + p.tile_group;

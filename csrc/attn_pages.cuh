@@ -9,6 +9,7 @@
 #pragma once
 #include "common.cuh"
 
+#include <cuda.h>
 #include <cuda_fp8.h>
 
 namespace pages {
@@ -135,6 +136,14 @@ __device__ __forceinline__ float exp2_fast(float x) {  // 2^x, one MUFU; 2^-inf 
   return y;
 }
 
+__device__ __forceinline__ void bulk_copy(void* dst, const void* src, int bytes, uint64_t* bar) {   // addresses and size multiples of 16
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+
+// pages as rows of bytes, copied in swizzled boxes of box_rows rows by up to 128 bytes
+int encode_pages(CUtensorMap* map, const void* base, int64_t rows, int bytes, int box_rows);
 // host side: which kernels a call takes, and its scratch
 int few_blocks(int fmt, int d, int rows, int segs);                                       // attn_pages_few.cu: blocks of one launch
 // `beside`: starts beside the kernel launched before it, whose results it does not need, and ends behind it

@@ -19,8 +19,6 @@
 // its parts in scratch, at most two per block, and the merge kernel joins them.
 #include "attn_pages.cuh"
 
-#include <cuda.h>
-
 namespace {
 
 using namespace pages;
@@ -97,11 +95,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {   // 8 x 8 of 16-bi
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
-}
-__device__ __forceinline__ void bulk_copy(void* dst, const void* src, int bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes),
-               "r"(smem_u32(bar))
-               : "memory");
 }
 // Key of a unit that stands in row i of the first product.  Neighbouring rows lie in chunk places that differ by four, and the even rows in places that
 // differ by two, so that under the 128-byte swizzle (chunk ^ key & 7) no eight lanes meet in a bank, neither reading keys nor reading values.
@@ -666,32 +659,6 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   pdl_wait();
 }
 
-typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                                CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiled encode_entry() {
-  static EncodeTiled fn = nullptr;
-  if (fn == nullptr) {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess) fn = (EncodeTiled)p;
-  }
-  return fn;
-}
-
-// pages as rows of bytes, in boxes of 16 rows
-int encode_pages(CUtensorMap* map, const void* base, int64_t rows, int bytes) {
-  EncodeTiled enc = encode_entry();
-  LLMSS_REQUIRE(enc != nullptr, "attn_pages: cuTensorMapEncodeTiled entry point not available");
-  cuuint64_t dims[2] = {(cuuint64_t)bytes, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)bytes};
-  cuuint32_t box[2] = {(cuuint32_t)(bytes < 128 ? bytes : 128), 16};
-  cuuint32_t one[2] = {1, 1};
-  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         bytes < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  LLMSS_REQUIRE(r == CUDA_SUCCESS, "attn_pages: cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
-  return 0;
-}
-
 template <typename T, int FMT, int D, int NT>
 int launch(const AttnArgs& a, const PartArgs& p, int blocks, bool beside, cudaStream_t stream) {
   using C = Few<FMT, D, NT>;
@@ -707,8 +674,8 @@ int launch(const AttnArgs& a, const PartArgs& p, int blocks, bool beside, cudaSt
   LLMSS_CHECK_CUDA(configured.ensure(kern, C::smem(C::ROWS, kKept)));
   const int64_t rows = (int64_t)a.num_blocks * a.hkv * a.page;
   CUtensorMap map_k, map_v;
-  if (int e = encode_pages(&map_k, a.k, rows, D * C::ESZ)) return e;
-  if (int e = encode_pages(&map_v, a.v, rows, D * C::ESZ)) return e;
+  if (int e = encode_pages(&map_k, a.k, rows, D * C::ESZ, 16)) return e;
+  if (int e = encode_pages(&map_v, a.v, rows, D * C::ESZ, 16)) return e;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3(blocks);

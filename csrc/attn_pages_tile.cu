@@ -4,14 +4,14 @@
 // A block takes up to 256 rows (128 for 256 columns): a row is a (token, query head) of one key head, so that grouped heads fill a tile's 128 rows and every
 // key is read once for all of them.  It walks its keys in tiles of 64:
 //
-//   loading warps   copy keys and values page by page (cp.async; 8-bit codes through a ring of their own, then converted) into a ring of 128-byte
-//                   swizzled tiles, keys a tile ahead of values; what lies outside of the list is filled with zeros and never looked at
+//   copying warp    keys and values page by page (TMA) into a ring of 128-byte swizzled tiles, keys a tile ahead of values; 8-bit codes into a ring of
+//                   their own, from which
+//   converting warps (8-bit) write the tiles.  Values that lie outside of the list become zeros, keys there are never looked at
 //   issuing warp    S_j = Q K_j^T (two S buffers per 128 rows), O += P_j V_j with P_j in tensor memory over S_j
 //   softmax warps   a thread per row: its S row from tensor memory, mask, running maximum (moved when exceeded by 2^8) and sum in 32 bits, P back
 //
 // 8-bit codes are converted once per block for all its rows: code * scale is rounded to the queries' type, which is a rounding of the same size as a
-// 16-bit cache has, and well below the code's own step; with the scales multiplied to the scores instead, every row would pay for them.  Copies are not
-// TMA's because the conversion and the zeros pass through threads anyway.
+// 16-bit cache has, and well below the code's own step; with the scales multiplied to the scores instead, every row would pay for them.
 //
 // A list whose rows are few is cut into stretches of keys (grid x), whose parts the merge kernel joins.
 #include "attn_pages.cuh"
@@ -22,20 +22,21 @@ using namespace pages;
 using namespace umma_lo;
 
 constexpr int BM = 128, BN = 64;
-constexpr int kLoaders = 4;
 
 template <int FMT, int D, int NQ>
 struct Tile {
-  static constexpr int ESZ = FMT == kF16Pages ? 2 : 1;
   static constexpr int SOFT = 4 * NQ;                                   // softmax warps
-  static constexpr int THREADS = 32 * (SOFT + 1 + kLoaders);
+  // 8-bit: four warps would convert a tile in twice the time that the products take
+  static constexpr int CONVERT = FMT == kF16Pages ? 0 : 8;
+  static constexpr int THREADS = 32 * (SOFT + 2 + CONVERT);
   static constexpr int Q_BYTES = NQ * BM * D * 2;
   static constexpr int SLOT = BN * D * 2;                               // a tile of keys or values
   static constexpr int SLOTS = D == 256 ? (FMT == kF16Pages ? 4 : 3) : 6;
-  static constexpr int CH = BN * D * ESZ / 16 / (32 * kLoaders);        // 16-byte chunks of a tile per loading thread
-  static constexpr int RAW = FMT == kF16Pages ? 0 : CH * 32 * kLoaders * 20;   // codes, and a scale per chunk
-  static constexpr int RAWS = FMT == kF16Pages ? 0 : (D == 256 ? 3 : 4);
+  static constexpr int RAW = FMT == kF16Pages ? 0 : BN * D + BN * 4;    // codes, then scales
+  static constexpr int RAWS = FMT == kF16Pages ? 0 : D == 256 ? 3 : 4;
   static constexpr int SMEM = 1024 + Q_BYTES + SLOTS * SLOT + RAWS * RAW + 512;
+  static constexpr int OUT_ROW = D * 4 + kPad * 4;                      // a part; the result's rows are shorter
+  static_assert(SOFT * 32 * OUT_ROW <= Q_BYTES + SLOTS * SLOT, "outputs are staged where queries, keys and values were");
   static constexpr int TMEM = NQ * (2 * BN + D) <= 256 ? 256 : 512;
 };
 
@@ -44,6 +45,7 @@ struct TileArgs {
   int own_splits, group_splits;
   int own_chunk, group_chunk;     // keys, multiples of BN
   int segs_own;                   // sequences (0: not this launch's)
+  int run;                        // keys of a tile that lie in one page: 16, 32 or 64
   int direct;                     // the result itself, not a part
 };
 
@@ -53,9 +55,6 @@ __host__ __device__ constexpr uint32_t idesc(int fmt, int n, int b_mn) {
 }
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {   // bytes 0: zeros
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void copy4(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -121,21 +120,25 @@ __device__ __forceinline__ void convert4(uint32_t w, float scale, uint32_t& lo, 
 
 template <typename T, int FMT, int D, int NQ>
 __global__ void __launch_bounds__(Tile<FMT, D, NQ>::THREADS, 1)
-attn_pages_tile_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ PartArgs pa, const TileArgs ta) {
+attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnArgs a, const __grid_constant__ PartArgs pa, const TileArgs ta) {
   using C = Tile<FMT, D, NQ>;
   constexpr int DSUB = D / 64;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* s_q = smem;                                   // [NQ][DSUB][128 rows][128 bytes]
   uint8_t* s_kv = s_q + C::Q_BYTES;                      // [SLOTS][DSUB][64 keys][128 bytes]
-  uint8_t* s_raw = s_kv + C::SLOTS * C::SLOT;            // [RAWS][CH][128 threads] codes, then scales
+  uint8_t* s_raw = s_kv + C::SLOTS * C::SLOT;            // [RAWS][64 keys of codes | 64 scales]
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_raw + C::RAWS * C::RAW);
   uint64_t* bar_full = bars;                             // [SLOTS]
   uint64_t* bar_empty = bars + C::SLOTS;
   uint64_t* bar_s = bars + 2 * C::SLOTS;                 // [NQ][2] S ready
   uint64_t* bar_p = bar_s + 2 * NQ;                      // [NQ][2] P written
   uint64_t* bar_o = bar_p + 2 * NQ;                      // [NQ][2] P V done
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_o + 2 * NQ);
+  uint64_t* bar_q = bar_o + 2 * NQ;                      // queries are in place
+  uint64_t* bar_part = bar_q + 1;                        // a tile at the list's end, before its zeros
+  uint64_t* bar_raw = bar_part + 1;                      // [RAWS] codes have come
+  uint64_t* bar_used = bar_raw + C::RAWS;                // [RAWS] codes have been converted
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_used + C::RAWS);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
@@ -161,17 +164,9 @@ attn_pages_tile_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
   const int base = k_lo & ~(BN - 1);
   const int n_tiles = k_hi > k_lo ? (k_hi - base + BN - 1) / BN : 0;
 
-  // queries into their swizzled tiles; rows beyond the last are zeros
-  for (int i = threadIdx.x; i < NQ * BM * (D / 8); i += C::THREADS) {
-    const int row = i / (D / 8), ch = i % (D / 8), n = n0 + row;
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (n < nrows && n_tiles > 0)
-      v = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + (int64_t)(s.row0 + n / group) * a.ldq + (int64_t)(kvh * group + n % group) * D + ch * 8);
-    *reinterpret_cast<uint4*>(s_q + (row / BM) * (BM * D * 2) + (ch >> 3) * (BM * 128) + (row % BM) * 128 + (((ch & 7) ^ (row & 7)) << 4)) = v;
-  }
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::SLOTS; ++i) {
-      mbar_init(&bar_full[i], kLoaders);
+      mbar_init(&bar_full[i], FMT == kF16Pages ? 1 : C::CONVERT);
       mbar_init(&bar_empty[i], 1);
     }
     for (int i = 0; i < 2 * NQ; ++i) {
@@ -179,13 +174,18 @@ attn_pages_tile_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
       mbar_init(&bar_p[i], 4);
       mbar_init(&bar_o[i], 1);
     }
+    mbar_init(bar_q, C::SOFT);
+    mbar_init(bar_part, 1);
+    for (int i = 0; i < C::RAWS; ++i) {
+      mbar_init(&bar_raw[i], 1);
+      mbar_init(&bar_used[i], C::CONVERT);
+    }
     fence_mbar_init();
   }
   if (warp == C::SOFT) {
     tmem_alloc(tmem_slot, C::TMEM);
     tmem_relinquish();
   }
-  fence_proxy_async_smem();
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
@@ -196,114 +196,120 @@ attn_pages_tile_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
   auto key_at = [&](int j) { return j == 0 ? 0 : 2 * j - 1; };
   auto value_at = [&](int j) { return j + 1 < n_tiles ? 2 * j + 2 : 2 * n_tiles - 1; };
 
-  if (warp > C::SOFT) {
-    // ===================== loading warps
-    const int tid = threadIdx.x - 32 * (C::SOFT + 1);
-    constexpr int PER = D * C::ESZ / 16;                 // chunks of a key
-    auto tile_of = [&](int i, bool& value) {             // i-th of the ring -> tile
-      if (i == 2 * n_tiles - 1) {
-        value = true;
-        return n_tiles - 1;
-      }
-      value = i >= 2 && (i & 1) == 0;
-      return i == 0 ? 0 : value ? (i - 2) / 2 : (i + 1) / 2;
-    };
+  if (warp == C::SOFT + 1) {
+    // ===================== copying warp: all of it runs the loop, one lane issues
     const int total = 2 * n_tiles;
-    // cache rows of a tile's four runs of 16 keys (a run lies in one page), one per lane of each four; looked up a tile ahead of the copies
+    const uint64_t policy = l2_policy_evict_last();
+    const int run = ta.run, runs = BN / run;
+    // cache rows of a tile's runs, one per lane; looked up a tile ahead of the copies
     auto look_up = [&](int j) {
-      const int key = base + j * BN + (lane & 3) * 16;
+      const int key = base + j * BN + min(lane, runs - 1) * run;
       return key < k_hi ? ((uint32_t)checked_block(__ldg(s.table + key / a.page), a.num_blocks) * a.hkv + kvh) * a.page + key % a.page : 0u;
     };
-    uint32_t runs = look_up(0), runs_before = 0, runs_next = 0;       // of the newest tile of keys, of the one before, of the next one
-    int newest = -1;
-    // turn to the i-th of the ring: its tile, and the cache row of this thread's chunk c with whether that lies in the list
-    auto turn = [&](int i, bool& value, uint32_t& mine) {
-      const int j = tile_of(i, value);
+    uint32_t rows = n_tiles > 0 ? look_up(0) : 0, rows_before = 0, rows_next = 0;   // of the newest tile of keys, of the one before, of the next one
+    uint32_t part_phase = 0;
+    for (int i = 0; i < total; ++i) {
+      // the ring holds K0, K1, V0, K2, V1 ..
+      const bool value = i == total - 1 || (i >= 2 && (i & 1) == 0);
+      const int j = i == total - 1 ? n_tiles - 1 : i == 0 ? 0 : value ? (i - 2) / 2 : (i + 1) / 2;
       if (!value) {
-        if (j > 0) runs_before = runs, runs = runs_next;
-        newest = j;
-        runs_next = look_up(j + 1);
+        if (j > 0) rows_before = rows, rows = rows_next;
+        rows_next = look_up(j + 1);
       }
-      mine = j == newest ? runs : runs_before;
-      return base + j * BN;
-    };
-    auto place = [&](int first, uint32_t mine, int c, uint32_t& row) {
-      const int key = (c * (32 * kLoaders) + tid) / PER;
-      row = __shfl_sync(0xffffffffu, mine, key >> 4) + (key & 15);
-      return first + key >= s.lo && first + key < k_hi;
-    };
-    if constexpr (FMT == kF16Pages) {
-      constexpr int LAG = C::SLOTS - 2;                  // tiles in flight
-      auto finish = [&](int i) {
-        fence_proxy_async_smem();
+      const uint32_t mine = value && j < n_tiles - 1 ? rows_before : rows;
+      const int first = base + j * BN;
+      const int here = min(runs, (k_hi - first + run - 1) / run);       // runs that lie in the list
+      if constexpr (FMT == kF16Pages) {
+        const int slot = i % C::SLOTS;
+        mbar_wait(&bar_empty[slot], ((i / C::SLOTS) & 1) ^ 1, 80);
+        const bool part = value && (first < s.lo || first + BN > k_hi);
+        uint64_t* bar = part ? bar_part : &bar_full[slot];
+        uint8_t* dst = s_kv + slot * C::SLOT;
+        if (elect_one()) mbar_arrive_expect_tx(bar, here * run * D * 2);
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bar_full[i % C::SLOTS]);
-      };
-      for (int i = 0; i < total + LAG; ++i) {
-        if (i < total) {
-          bool value;
-          uint32_t mine;
-          const int first = turn(i, value, mine);
-          mbar_wait(&bar_empty[i % C::SLOTS], ((i / C::SLOTS) & 1) ^ 1, 80);
-          const uint32_t dst = smem_u32(s_kv + (i % C::SLOTS) * C::SLOT);
-          const uint8_t* src = reinterpret_cast<const uint8_t*>(value ? a.v : a.k);
+        for (int x = 0; x < here; ++x) {
+          const int row = (int)__shfl_sync(0xffffffffu, mine, x);
+          if (elect_one()) {
 #pragma unroll
-          for (int c = 0; c < C::CH; ++c) {
-            uint32_t row;
-            const bool in = place(first, mine, c, row);
-            const int x = c * (32 * kLoaders) + tid, key = x / PER, ch = x % PER;
-            copy16(dst + (ch >> 3) * (BN * 128) + key * 128 + (((ch & 7) ^ (key & 7)) << 4), src + (in ? (uint64_t)row * (D * 2) + ch * 16 : 0), in ? 16 : 0);
+            for (int c = 0; c < DSUB; ++c) tma_load_2d(dst + c * (BN * 128) + x * run * 128, value ? &map_v : &map_k, bar, c * 128, row, policy);
           }
+          __syncwarp();
         }
-        copies_commit();
-        if (i >= LAG) {
-          copies_wait<LAG>();
-          finish(i - LAG);
+        if (part) {
+          // zeros where the list does not reach: 0 x NaN would be NaN
+          mbar_wait(bar_part, part_phase, 78);
+          part_phase ^= 1;
+          for (int x = lane; x < BN * DSUB * 8; x += 32) {
+            const int key = first + (x >> 3) % BN;
+            if (key < s.lo || key >= k_hi) *reinterpret_cast<uint4*>(dst + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar_full[slot]);
+        }
+      } else {
+        const int slot = i % C::RAWS;
+        mbar_wait(&bar_used[slot], ((i / C::RAWS) & 1) ^ 1, 80);
+        uint8_t* dst = s_raw + slot * C::RAW;
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(value ? a.v : a.k);
+        const float* sc = value ? a.vs : a.ks;
+        if (elect_one()) mbar_arrive_expect_tx(&bar_raw[slot], here * run * (D + 4));
+        __syncwarp();
+        for (int x = 0; x < here; ++x) {
+          const uint32_t row = __shfl_sync(0xffffffffu, mine, x);
+          if (elect_one()) {
+            bulk_copy(dst + x * run * D, src + (uint64_t)row * D, run * D, &bar_raw[slot]);
+            bulk_copy(dst + BN * D + x * run * 4, sc + row, run * 4, &bar_raw[slot]);
+          }
+          __syncwarp();
         }
       }
-    } else {
-      auto fetch = [&](int i) {
-        if (i < total) {
-          bool value;
-          uint32_t mine;
-          const int first = turn(i, value, mine);
-          uint8_t* raw = s_raw + (i % C::RAWS) * C::RAW;
-          const uint8_t* src = reinterpret_cast<const uint8_t*>(value ? a.v : a.k);
-          const float* sc = value ? a.vs : a.ks;
+    }
+  } else if (warp > C::SOFT + 1) {
+    // ===================== converting warps
+    if constexpr (FMT != kF16Pages) {
+      const int tid = threadIdx.x - 32 * (C::SOFT + 2);
+      constexpr int PER = D / 16, KEYS = 32 * C::CONVERT / PER;      // 16-byte chunks of a key, keys between a thread's chunks
+      constexpr int CH = BN / KEYS;                                // a thread's chunks of a tile
+      const int key0 = tid / PER, ch = tid % PER;                  // this thread's first key, its place in every key
+      // eight lanes write one key: lanes of odd 64-column halves begin with their second chunk, so that no two meet in a bank
+      const int flip = (ch >> 2) & 1;
+      const uint32_t to = (ch >> 2) * (BN * 128) + key0 * 128, c0 = ((2 * (ch & 3) + flip) ^ (key0 & 7)) << 4;
+      static_assert(KEYS % 8 == 0, "every eighth key has the same place in the swizzle");
+      const int total = 2 * n_tiles;
+      for (int i = 0; i < total; ++i) {
+        const bool value = i == total - 1 || (i >= 2 && (i & 1) == 0);
+        const int j = i == total - 1 ? n_tiles - 1 : i == 0 ? 0 : value ? (i - 2) / 2 : (i + 1) / 2;
+        const int first = base + j * BN;
+        const bool all = first >= s.lo && first + BN <= k_hi;
+        const uint8_t* raw = s_raw + (i % C::RAWS) * C::RAW;
+        mbar_wait(&bar_raw[i % C::RAWS], (i / C::RAWS) & 1, 77);
+        uint4 w[CH];
+        float scale[CH];
 #pragma unroll
-          for (int c = 0; c < C::CH; ++c) {
-            uint32_t row;
-            const bool in = place(first, mine, c, row);
-            const int x = c * (32 * kLoaders) + tid;
-            copy16(smem_u32(raw + x * 16), src + (in ? (uint64_t)row * D + (x % PER) * 16 : 0), in ? 16 : 0);
-            copy4(smem_u32(raw + C::CH * 32 * kLoaders * 16 + x * 4), sc + (in ? row : 0), in ? 4 : 0);
+        for (int c = 0; c < CH; ++c) {
+          const int key = key0 + c * KEYS;
+          w[c] = *reinterpret_cast<const uint4*>(raw + key * D + ch * 16);
+          scale[c] = *reinterpret_cast<const float*>(raw + BN * D + key * 4);
+          if (!all && (first + key < s.lo || first + key >= k_hi)) {   // zeros where the list does not reach
+            w[c] = make_uint4(0u, 0u, 0u, 0u);
+            scale[c] = 0.f;
           }
         }
-        copies_commit();
-      };
-      for (int i = 0; i < C::RAWS - 1; ++i) fetch(i);
-      for (int i = 0; i < total; ++i) {
-        fetch(i + C::RAWS - 1);
-        copies_wait<C::RAWS - 1>();                      // a thread converts what it copied itself
-        const uint8_t* raw = s_raw + (i % C::RAWS) * C::RAW;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar_used[i % C::RAWS]);
         mbar_wait(&bar_empty[i % C::SLOTS], ((i / C::SLOTS) & 1) ^ 1, 81);
-        uint8_t* dst = s_kv + (i % C::SLOTS) * C::SLOT;
+        uint8_t* dst = s_kv + (i % C::SLOTS) * C::SLOT + to;
 #pragma unroll
-        for (int c = 0; c < C::CH; ++c) {
-          const int x = c * (32 * kLoaders) + tid, key = x / PER, ch = x % PER;
-          const uint4 w = *reinterpret_cast<const uint4*>(raw + x * 16);
-          const float scale = *reinterpret_cast<const float*>(raw + C::CH * 32 * kLoaders * 16 + x * 4);
+        for (int c = 0; c < CH; ++c) {
           uint4 y[2];
-          convert4<T, FMT>(w.x, scale, y[0].x, y[0].y);
-          convert4<T, FMT>(w.y, scale, y[0].z, y[0].w);
-          convert4<T, FMT>(w.z, scale, y[1].x, y[1].y);
-          convert4<T, FMT>(w.w, scale, y[1].z, y[1].w);
-          // eight lanes write one key: lanes of odd 64-column halves begin with their second chunk, so that no two meet in a bank
-          const int flip = (ch >> 2) & 1;
-          uint8_t* to = dst + (ch >> 2) * (BN * 128) + key * 128;
-          const int c0 = 2 * (ch & 3) + flip, c1 = c0 ^ 1;
-          *reinterpret_cast<uint4*>(to + ((c0 ^ (key & 7)) << 4)) = flip ? y[1] : y[0];
-          *reinterpret_cast<uint4*>(to + ((c1 ^ (key & 7)) << 4)) = flip ? y[0] : y[1];
+          convert4<T, FMT>(w[c].x, scale[c], y[0].x, y[0].y);
+          convert4<T, FMT>(w[c].y, scale[c], y[0].z, y[0].w);
+          convert4<T, FMT>(w[c].z, scale[c], y[1].x, y[1].y);
+          convert4<T, FMT>(w[c].w, scale[c], y[1].z, y[1].w);
+          uint8_t* at = dst + c * (KEYS * 128);
+          *reinterpret_cast<uint4*>(at + c0) = flip ? y[1] : y[0];
+          *reinterpret_cast<uint4*>(at + (c0 ^ 16)) = flip ? y[0] : y[1];
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -329,6 +335,7 @@ attn_pages_tile_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
       __syncwarp();
     };
     auto wait_full = [&](int i) { mbar_wait(&bar_full[i % C::SLOTS], (i / C::SLOTS) & 1, 82); };
+    if (n_tiles > 0) mbar_wait(bar_q, 0, 79);
     for (int j = 0; j < min(n_tiles, 2); ++j) {
       wait_full(key_at(j));
       tcgen05_fence_after();
@@ -368,12 +375,35 @@ attn_pages_tile_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
     const uint32_t off = (uint32_t)(quarter * 32) << 16;
     const bool live = n < nrows;
     const int tok = s.row0 + n / group;
+    const int head = kvh * group + n % group;
+    // this warp's 32 rows of queries into their swizzled tile; rows beyond the last are zeros
+    if (n_tiles > 0) {
+      const uint32_t dst = smem_u32(s_q + q * (BM * D * 2));
+      const int64_t at = live ? (int64_t)tok * a.ldq + (int64_t)head * D : -1;
+      constexpr int STEP = 32 / (D / 8 < 32 ? D / 8 : 32);         // rows of one copy of the warp
+      const int ch = lane % (32 / STEP);
+#pragma unroll 4
+      for (int i = 0; i < 32; i += STEP) {
+        const int row = i + lane / (32 / STEP);
+        const int64_t from = __shfl_sync(0xffffffffu, at, row);
+        const int rt = quarter * 32 + row;
+        copy16(dst + (ch >> 3) * (BM * 128) + rt * 128 + (((ch & 7) ^ (rt & 7)) << 4), reinterpret_cast<const T*>(a.q) + (from < 0 ? 0 : from + ch * 8),
+               from < 0 ? 0 : 16);
+      }
+      copies_commit();
+    }
     int pos = 0x7fffffff;                                 // rows beyond the last look at everything and are dropped
     if (live) {
       const int sq = is_own ? (int)blockIdx.z : seq_of_row(a.cu, 0, a.num_seqs, tok);
       pos = sq < 0 ? -1 : row_pos(a, sq, tok);
     }
     pos = min(pos, k_hi - 1);
+    if (n_tiles > 0) {
+      copies_wait<0>();
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_q);
+    }
     const float scale = a.scale_log2;
     // f16 ends at 2^16 and has no numbers below 2^-24: probabilities are formed times 2^7 (at most 2^15), so that those down to 2^-21 keep all bits
     constexpr float kUp = std::is_same<T, __half>::value ? 7.0f : 0.0f;
@@ -450,11 +480,18 @@ attn_pages_tile_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
       mbar_wait(&bar_o[q * 2 + ((n_tiles - 1) & 1)], ((n_tiles - 1) >> 1) & 1, 87);
       tcgen05_fence_after();
     }
-    const int head = kvh * group + n % group;
+    // every product has been formed, so queries, keys and values make room: rows go through shared memory, each lane's in a place of its own (a row is
+    // 16 bytes longer than a multiple of 128, so that eight lanes never meet in a bank), and from there as whole rows (a lane's 16 bytes to a row of its
+    // own would be 32 transactions per instruction: 9600 clocks for 256 rows of 132 numbers)
+    if constexpr (NQ > 1) {
+      // the other tile's products read keys and values too
+      mbar_wait(&bar_o[(q ^ 1) * 2 + ((n_tiles - 1) & 1)], n_tiles > 0 ? ((n_tiles - 1) >> 1) & 1 : 1, 88);
+    }
     // no visible key: zero (the sum is NaN where a score was)
     const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
-    T* out = reinterpret_cast<T*>(a.out) + (int64_t)tok * a.ldo + (int64_t)head * D;
-    float* part = (is_own ? pa.tile_own : pa.tile_group) + (((int64_t)split * a.total_q + tok) * a.hq + head) * (D + kPad);
+    const int row_bytes = ta.direct ? D * 2 : C::OUT_ROW;
+    const int stride = ta.direct ? D * 2 + 16 : C::OUT_ROW;
+    uint8_t* mine = smem + (q * BM + quarter * 32 + lane) * stride;
 #pragma unroll 1
     for (int c = 0; c < D / 32; ++c) {
       uint32_t r[32];
@@ -465,22 +502,29 @@ attn_pages_tile_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
 #pragma unroll
         for (int i = 0; i < 32; ++i) r[i] = 0u;
       }
-      if (live) {
-        if (ta.direct) {
+      if (ta.direct) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            float f8[8];
+        for (int i = 0; i < 32; i += 8) {
+          float f8[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f8[e] = __uint_as_float(r[i + e]) * inv;
-            *reinterpret_cast<uint4*>(out + c * 32 + i) = pack8<T>(f8);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(part + c * 32 + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+          for (int e = 0; e < 8; ++e) f8[e] = __uint_as_float(r[i + e]) * inv;
+          *reinterpret_cast<uint4*>(mine + c * 64 + i * 2) = pack8<T>(f8);
         }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(mine + c * 128 + i * 4) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
       }
     }
-    if (live && !ta.direct) *reinterpret_cast<float2*>(part + D) = make_float2(m_run - kUp, l_run);
+    if (!ta.direct) *reinterpret_cast<float4*>(mine + D * 4) = make_float4(m_run - kUp, l_run, 0.f, 0.f);
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (live) {
+      void* to = ta.direct ? (void*)(reinterpret_cast<T*>(a.out) + (int64_t)tok * a.ldo + (int64_t)head * D)
+                           : (void*)((is_own ? pa.tile_own : pa.tile_group) + (((int64_t)split * a.total_q + tok) * a.hq + head) * (D + kPad));
+      asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(smem_u32(mine)), "r"(row_bytes) : "memory");
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
   }
 
   tcgen05_fence_before();
@@ -507,10 +551,19 @@ int launch(const AttnArgs& a, const PartArgs& p, const TilePlan& t, cudaStream_t
   ta.group_chunk = p.group_chunk;
   ta.segs_own = t.own_tiles > 0 ? a.num_seqs : 0;
   ta.direct = a.groups == 0 && p.own_splits == 1;
+  ta.run = a.page % 64 == 0 ? 64 : a.page % 32 == 0 ? 32 : 16;
+  CUtensorMap map_k, map_v;
+  memset(&map_k, 0, sizeof(map_k));
+  memset(&map_v, 0, sizeof(map_v));
+  if (FMT == kF16Pages) {
+    const int64_t rows = (int64_t)a.num_blocks * a.hkv * a.page;
+    if (int e = encode_pages(&map_k, a.k, rows, D * 2, ta.run)) return e;
+    if (int e = encode_pages(&map_v, a.v, rows, D * 2, ta.run)) return e;
+  }
   const int64_t x = (int64_t)t.own_tiles * p.own_splits, y = (int64_t)t.group_tiles * p.group_splits;
   const dim3 grid((unsigned)(x > y ? x : y), a.hkv, ta.segs_own + (t.group_tiles > 0 ? a.groups : 0));
   LLMSS_REQUIRE(grid.y <= 65535 && grid.z <= 65535 && (x > y ? x : y) < (1ll << 31), "attn_pages: grid too large (%d key heads, %u lists)", a.hkv, grid.z);
-  LLMSS_CHECK_CUDA(launch_pdl(kern, grid, dim3(C::THREADS), (size_t)C::SMEM, stream, a, p, ta));
+  LLMSS_CHECK_CUDA(launch_pdl(kern, grid, dim3(C::THREADS), (size_t)C::SMEM, stream, map_k, map_v, a, p, ta));
   return 0;
 }
 
