@@ -104,10 +104,12 @@ __global__ void __launch_bounds__(128) attn_pages_any_kernel(const __grid_consta
 // ---------------------------------------------------------------------------------------------------------------- merge
 // A warp per query row and head joins the parts of its softmax: m = max m_i, l = sum l_i 2^(m_i - m), out = sum O_i 2^(m_i - m) / l.  Reads what the
 // kernels before it left in L2; launched to start as they end (programmatic dependent launch), so that it costs no launch latency of its own.
-template <typename T, int D>
+// WARPS of them share a row where rows are few: parts are many then, and each costs a read from L2.
+template <typename T, int D, int WARPS>
 __global__ void __launch_bounds__(256) attn_pages_merge_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ PartArgs p) {
   constexpr int N = D / 32;
-  const int w = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int w = WARPS == 1 ? blockIdx.x * 8 + warp : blockIdx.x, mine = WARPS == 1 ? 0 : warp;
   const int t = w / a.hq, head = w % a.hq;
   if (t >= a.total_q) return;
   const int s = seq_of_row(a.cu, 0, a.num_seqs, t);      // lengths are not written by the kernels before
@@ -116,20 +118,35 @@ __global__ void __launch_bounds__(256) attn_pages_merge_kernel(const __grid_cons
   float o[N], m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) o[i] = 0.f;
-  auto add = [&](const float* part) {
-    const float2 ml = *reinterpret_cast<const float2*>(part + D);
-    float x[N];
-#pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const float2 v = *reinterpret_cast<const float2*>(part + i * 32 + lane * 2);
-      x[i] = v.x, x[i + 1] = v.y;
+  // parts at first, first + stride ..: a lane looks at one part's maximum and sum, then all lanes add up the parts with their weights
+  auto add = [&](const float* first, int64_t stride, int count) {
+    if constexpr (WARPS > 1) {             // every WARPS-th part
+      first += mine * stride;
+      stride *= WARPS;
+      count = count > mine ? (count - mine + WARPS - 1) / WARPS : 0;
     }
-    const float mn = fmaxf(m, ml.x), base = mn == -INFINITY ? 0.f : mn;
-    const float f = m == mn ? 1.f : exp2f(m - base), e = exp2f(ml.x - base);
-    l = l * f + ml.y * e;
+    for (int b = 0; b < count; b += 32) {
+      const int k = min(32, count - b);
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (lane < k) ml = *reinterpret_cast<const float2*>(first + (b + lane) * stride + D);
+      const float mn = fmaxf(m, warp_max(ml.x)), base = mn == -INFINITY ? 0.f : mn;
+      const float f = m == mn ? 1.f : exp2f(m - base), e = exp2f(ml.x - base);
+      l = l * f + warp_sum(ml.y * e);
+      m = mn;
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = o[i] * f + x[i] * e;
-    m = mn;
+      for (int i = 0; i < N; ++i) o[i] *= f;
+#pragma unroll 4
+      for (int j = 0; j < k; ++j) {
+        const float w = __shfl_sync(0xffffffffu, e, j);
+        const float* part = first + (b + j) * stride;
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+          const float2 v = *reinterpret_cast<const float2*>(part + i * 32 + lane * 2);
+          o[i] += w == 0.f ? 0.f : w * v.x;
+          o[i + 1] += w == 0.f ? 0.f : w * v.y;
+        }
+      }
+    }
   };
   const Seg own = own_segment(a, s);
   const bool has_own = own.hi > own.lo;
@@ -138,18 +155,18 @@ __global__ void __launch_bounds__(256) attn_pages_merge_kernel(const __grid_cons
     const FewInfo in = p.info[(int64_t)seg * a.hkv + kvh];
     if (in.first_slot < 0) {
       if (a.groups == 0) return false;
-      add(whole + ((int64_t)t * a.hq + head) * (D + kPad));
+      add(whole + ((int64_t)t * a.hq + head) * (D + kPad), 0, 1);
       return true;
     }
     const int n = (t - row0) * group + head % group;
     if (n >= p.rows) return true;
-    add(p.slots + ((int64_t)in.first_slot * p.rows + n) * (D + kPad));
-    for (int j = in.first_block + 1; j <= in.last_block; ++j) add(p.slots + ((int64_t)(2 * j) * p.rows + n) * (D + kPad));
+    const int64_t slot = (int64_t)p.rows * (D + kPad);
+    add(p.slots + in.first_slot * slot + n * (D + kPad), 0, 1);
+    add(p.slots + (int64_t)2 * (in.first_warp + 1) * slot + n * (D + kPad), 2 * slot, in.last_warp - in.first_warp);
     return true;
   };
   auto stretches = [&](const float* parts, int lo, int hi, int chunk, int splits) {
-    const int n = min(splits, (hi - lo + chunk - 1) / chunk);
-    for (int i = 0; i < n; ++i) add(parts + (((int64_t)i * a.total_q + t) * a.hq + head) * (D + kPad));
+    add(parts + ((int64_t)t * a.hq + head) * (D + kPad), (int64_t)a.total_q * a.hq * (D + kPad), min(splits, (hi - lo + chunk - 1) / chunk));
   };
   if (has_own) {
     if (p.few_own) {
@@ -165,6 +182,30 @@ __global__ void __launch_bounds__(256) attn_pages_merge_kernel(const __grid_cons
       else stretches(p.tile_group, 0, gs.hi, p.group_chunk, p.group_splits);
     }
   }
+  if constexpr (WARPS > 1) {
+    __shared__ float s_ml[WARPS][2];
+    __shared__ float s_o[WARPS][D];
+    if (lane == 0) s_ml[warp][0] = m, s_ml[warp][1] = l;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) *reinterpret_cast<float2*>(&s_o[warp][i * 32 + lane * 2]) = make_float2(o[i], o[i + 1]);
+    __syncthreads();
+    if (warp > 0) return;
+    m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int j = 0; j < WARPS; ++j) m = fmaxf(m, s_ml[j][0]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < WARPS; ++j) {
+      const float f = exp2f(s_ml[j][0] - (m == -INFINITY ? 0.f : m));
+      l += s_ml[j][1] * f;
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        const float2 v = *reinterpret_cast<const float2*>(&s_o[j][i * 32 + lane * 2]);
+        o[i] += v.x * f, o[i + 1] += v.y * f;
+      }
+    }
+  }
   // no visible key: zero (l is NaN where a score was)
   const float inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
   T* out = reinterpret_cast<T*>(a.out) + (int64_t)t * a.ldo + (int64_t)head * D;
@@ -176,10 +217,14 @@ __global__ void __launch_bounds__(256) attn_pages_merge_kernel(const __grid_cons
 }
 
 template <typename T, int D>
-int launch_merge(const AttnArgs& a, const PartArgs& p, cudaStream_t stream) {
+int launch_merge(const AttnArgs& a, const PartArgs& p, int parts, cudaStream_t stream) {
+  const int64_t rows = (int64_t)a.total_q * a.hq;
+  // fewer rows than eight warps on each of 148 SMs, many parts of each: 8 sequences of 24000 tokens, 32 heads (28 parts) 83 -> 75 us with the merge; with two
+  // parts a row (64 sequences of 1040 tokens, 16 heads) eight warps would cost 6 us of 99
+  const bool shared = rows < 1184 && parts >= 8;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3((unsigned)(((int64_t)a.total_q * a.hq + 7) / 8));
+  cfg.gridDim = dim3((unsigned)(shared ? rows : (rows + 7) / 8));
   cfg.blockDim = dim3(256);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -187,7 +232,7 @@ int launch_merge(const AttnArgs& a, const PartArgs& p, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  LLMSS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attn_pages_merge_kernel<T, D>, a, p));
+  LLMSS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, shared ? attn_pages_merge_kernel<T, D, 8> : attn_pages_merge_kernel<T, D, 1>, a, p));
   return 0;
 }
 
@@ -232,7 +277,7 @@ Plan plan_call(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv
   if (p.few_own || p.few_groups) {
     p.rows = (int)(p.few_own && (!p.few_groups || own >= grouped) ? own : grouped);
     p.blocks = few_blocks(fmt, d, p.rows, (p.few_own ? num_seqs : 0) + (p.few_groups ? groups : 0));
-    p.slots = (int64_t)2 * p.blocks * p.rows * (d + kPad);
+    p.slots = (int64_t)2 * p.blocks * kFewWarps * p.rows * (d + kPad);
     p.info = ((int64_t)(p.few_own ? num_seqs : 0) + (p.few_groups ? groups : 0)) * hkv * 4;
     p.whole = groups > 0 ? (int64_t)total_q * hq * (d + kPad) : 0;
   }
@@ -356,7 +401,11 @@ LLMSS_API int llmss_attn_pages(const void* q, int64_t ldq, const void* k_pages, 
     if (plan.direct) return 0;
     if (plan.few_own || plan.few_groups)
       if (int e = few_launch(a, p, fmt, dtype, plan.blocks, tiles, stream)) return e;
-#define LLMSS_MERGE(T_) return d == 64 ? launch_merge<T_, 64>(a, p, stream) : d == 128 ? launch_merge<T_, 128>(a, p, stream) : launch_merge<T_, 256>(a, p, stream)
+    // parts of a row, about: runs of a list, or stretches
+    const int64_t lists = ((int64_t)(plan.few_own ? num_seqs : 0) + (plan.few_groups ? a.groups : 0)) * hkv;
+    const int64_t runs = lists > 0 ? (int64_t)plan.blocks * kFewWarps / lists : 0;
+    const int parts = (int)(runs > plan.own_splits + plan.group_splits ? runs : plan.own_splits + plan.group_splits);
+#define LLMSS_MERGE(T_) return d == 64 ? launch_merge<T_, 64>(a, p, parts, stream) : d == 128 ? launch_merge<T_, 128>(a, p, parts, stream) : launch_merge<T_, 256>(a, p, parts, stream)
     if (dtype == LLMSS_F16) LLMSS_MERGE(__half);
     LLMSS_MERGE(__nv_bfloat16);
 #undef LLMSS_MERGE

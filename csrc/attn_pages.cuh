@@ -76,16 +76,16 @@ __device__ __forceinline__ float page_value(const void* p, int64_t i) {
 // same row join in the merge kernel (attn_pages.cu).
 constexpr int kPad = 4;
 //
-// Lists of few rows (attn_pages_few.cu) are cut where their blocks' runs end: `info` says for each (segment, key head) where its parts lie.
+// Lists of few rows (attn_pages_few.cu) are cut where their warps' runs end: `info` says for each (segment, key head) where its parts lie.
 struct FewInfo {
   int first_slot;      // of `slots`; < 0: one part, in `whole` (with groups) or already the result (without)
-  int first_block;     // the parts behind the first are the slots 2 j, j = first_block + 1 .. last_block
-  int last_block;
+  int first_warp;     // the parts behind the first are the slots 2 j, j = first_warp + 1 .. last_warp (warps' numbers)
+  int last_warp;
   int pad;
 };
 
 struct PartArgs {
-  float* slots;        // [2 blocks][rows][d + kPad]
+  float* slots;        // [2 warps][rows][d + kPad]
   FewInfo* info;       // [segments][hkv]
   float* whole_own;    // [total_q][hq][d + kPad]
   float* whole_group;
@@ -145,6 +145,7 @@ __device__ __forceinline__ void bulk_copy(void* dst, const void* src, int bytes,
 // pages as rows of bytes, copied in swizzled boxes of box_rows rows by up to 128 bytes
 int encode_pages(CUtensorMap* map, const void* base, int64_t rows, int bytes, int box_rows);
 // host side: which kernels a call takes, and its scratch
+constexpr int kFewWarps = 4;       // attn_pages_few.cu: warps of a block
 int few_blocks(int fmt, int d, int rows, int segs);                                       // attn_pages_few.cu: blocks of one launch
 // `beside`: starts beside the kernel launched before it, whose results it does not need, and ends behind it
 int few_launch(const AttnArgs& a, const PartArgs& p, int fmt, int dtype, int blocks, bool beside, cudaStream_t stream);

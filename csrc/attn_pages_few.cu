@@ -14,17 +14,17 @@
 // The scale of a value row joins its probability in the exponent, with a maximum of its own, so that what is rounded to f16 is at most 2^8 whatever the
 // scales are.  Maxima move when a score exceeds them by 2^8 only.
 //
-// The work of a call is the sum of all (sequence, key head) lists in units of 16 keys (32 where a key is 64 bytes); each block takes an equal run of it,
-// wherever sequences begin and end, its four warps every fourth unit.  A list within a block's run is finished there; one that crosses runs leaves
-// its parts in scratch, at most two per block, and the merge kernel joins them.
+// The work of a call is the sum of all (sequence, key head) lists in units of 16 keys (32 where a key is 64 bytes); each warp takes an equal run of it,
+// wherever sequences begin and end, and waits for no other.  A list within a warp's run is finished there; one that crosses runs leaves its parts in
+// scratch, at most two per warp, and the merge kernel joins them.
 #include "attn_pages.cuh"
 
 namespace {
 
 using namespace pages;
 
-constexpr int kWarps = 4;
-constexpr int kLeastUnits = 8;     // of a block's run: two per warp
+constexpr int kWarps = kFewWarps;
+constexpr int kLeastUnits = 2;     // of a warp's run
 constexpr int kKept = 2048;        // lists whose lengths a block keeps in shared memory
 
 template <int FMT, int D, int NT>
@@ -36,21 +36,18 @@ struct Few {
   static constexpr int VW = D * ESZ / 32;             // of a value row
   static constexpr int EPC = 16 / ESZ;                // elements of 16 bytes
   static constexpr int KS = D / 16;                   // products of 16 columns
-  static constexpr int ROWS = 8 * NT;
-  static constexpr int LD = D + 4;                    // row of the merge buffer (floats)
-  static constexpr int Q_BYTES = NT * KS * 32 * 8;
+  static constexpr int Q_BYTES = NT * KS * 32 * 8;    // a warp's fragments of a list's queries
   static constexpr int ROW = D * ESZ < 128 ? D * ESZ : 128;   // bytes of a swizzled row: a key is BOXES of them
   static constexpr int BOXES = D * ESZ / ROW;
   static constexpr int HALF = UNIT * D * ESZ;         // keys, or values, of a unit
   static constexpr int STAGES = HALF <= 2048 ? 3 : 2;
   static constexpr int SCALES = FMT == kF16Pages ? 0 : 2 * UNIT * 4;
-  // without the merge buffer, which has as many rows as the call needs
-  static constexpr int FIXED = 1024 + kWarps * STAGES * (2 * HALF + SCALES) + Q_BYTES + ROWS * 12 + kWarps * (3 * ROWS * 4 + STAGES * 8);
+  static constexpr int FIXED = 1024 + kWarps * (STAGES * (2 * HALF + SCALES + 8) + Q_BYTES);
   static constexpr int MIN_CTAS = 4 * NT * KS <= 64 ? 3 : 2;   // outputs stay in registers; what else a thread holds is about 100
-  static int smem(int rows, int segs) { return FIXED + kWarps * rows * LD * 4 + 4 * (segs < kKept ? segs : kKept); }
+  static int smem(int segs) { return FIXED + 4 * (segs < kKept ? segs : kKept); }
   // blocks of an SM: by registers, and by 228 KB of shared memory less 1 KB per block
-  static int ctas(int rows, int segs) {
-    const int n = 233472 / (smem(rows, segs) + 1024);
+  static int ctas(int segs) {
+    const int n = 233472 / (smem(segs) + 1024);
     return n < MIN_CTAS ? n : MIN_CTAS;
   }
 };
@@ -58,7 +55,7 @@ struct Few {
 struct FewArgs {
   int segs;            // lists per key head: sequences (own) and groups
   int own;
-  int rows;            // of the merge buffer: query rows of a list at most
+  int rows;            // query rows of a list at most
   uint32_t page_magic; // (key / 16) 2 this >> 32: the key's page
   int beside;          // wait for the kernel before at the end instead of at the start
 };
@@ -106,21 +103,14 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                       const __grid_constant__ PartArgs pa, const FewArgs f) {
   using C = Few<FMT, D, NT>;
   using M = typename std::conditional<FMT == kF16Pages, T, __half>::type;   // type of the products
-  constexpr int UNIT = C::UNIT, SUB = C::SUB, KW = C::KW, VW = C::VW, KS = C::KS, EPC = C::EPC, ROWS = C::ROWS, LD = C::LD, STAGES = C::STAGES;
+  constexpr int UNIT = C::UNIT, SUB = C::SUB, KW = C::KW, VW = C::VW, KS = C::KS, EPC = C::EPC, STAGES = C::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* s_ring = smem;                                                   // [warps][STAGES][keys | values]
   float* s_scales = reinterpret_cast<float*>(s_ring + kWarps * STAGES * 2 * C::HALF);   // [warps][STAGES][of keys | of values]
   uint64_t* s_full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(s_scales) + kWarps * STAGES * C::SCALES);   // [warps][STAGES]
-  uint2* s_q = reinterpret_cast<uint2*>(s_full + kWarps * STAGES);          // [NT][KS][32] fragments
-  float* s_o = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(s_q) + C::Q_BYTES);   // [warps][rows][LD]
-  float* s_m = s_o + kWarps * f.rows * LD;                                  // [warps][ROWS] each: m, m', l
-  float* s_m2 = s_m + kWarps * ROWS;
-  float* s_l = s_m2 + kWarps * ROWS;
-  float* s_qs = s_l + kWarps * ROWS;                                        // [ROWS] score factor
-  float* s_qb = s_qs + ROWS;                                                // [ROWS] what 128 added to a score
-  int* s_pos = reinterpret_cast<int*>(s_qb + ROWS);                         // [ROWS] last visible key
-  int* s_units = s_pos + ROWS;                                              // [min(segs, kKept)]
+  uint2* s_q = reinterpret_cast<uint2*>(s_full + kWarps * STAGES);          // [warps][NT][KS][32] fragments, each lane's its own
+  int* s_units = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(s_q) + kWarps * C::Q_BYTES);   // [min(segs, kKept)]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
   pdl_launch_dependents();
   if (!f.beside) pdl_wait();
@@ -131,7 +121,9 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     fence_mbar_init();
   }
 
-  // this block's run of the lists
+  s_q += warp * NT * KS * 32 + lane;
+
+  // this warp's run of the lists
   for (int i = threadIdx.x; i < min(f.segs, kKept); i += 32 * kWarps) s_units[i] = units_of<UNIT>(segment<UNIT>(a, f, i));
   __syncthreads();
   auto count = [&](int i) { return i < kKept ? s_units[i] : units_of<UNIT>(segment<UNIT>(a, f, i)); };
@@ -151,8 +143,9 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   unsigned units = __shfl_sync(0xffffffffu, inc0, 31);
   for (int b = 32; b < f.segs; b += 32) units += __reduce_add_sync(0xffffffffu, b + lane < f.segs ? count(b + lane) : 0);
   const unsigned total = units * a.hkv;
-  const unsigned per = max((total + gridDim.x - 1) / gridDim.x, (unsigned)kLeastUnits);
-  const unsigned begin = min(per * blockIdx.x, total), end = min(begin + per, total);
+  const unsigned workers = gridDim.x * kWarps, me = blockIdx.x * kWarps + warp;
+  const unsigned per = max((total + workers - 1) / workers, (unsigned)kLeastUnits);
+  const unsigned begin = min(per * me, total), end = min(begin + per, total);
   if (begin >= end) {
     pdl_wait();
     return;
@@ -177,7 +170,7 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   const int group = a.hq / a.hkv;
   auto page_of = [&](int key) { return (int)__umulhi((unsigned)key >> 4 << 1, f.page_magic); };
 
-  // a place in the block's run: a list, or the part of it that lies in the run, and this warp's unit in it
+  // a place in the run: a list, or the part of it that lies in the run, and a unit in it
   struct Place {
     Seg s;
     unsigned before, cur;    // units before the segment (one key head), place of the list's part in the run
@@ -195,7 +188,7 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     w.u0 = at - w.kvh * w.n;
     w.u1 = min((unsigned)w.n, w.u0 + (end - w.cur));
     w.base = w.s.lo & ~(UNIT - 1);
-    w.u = w.u0 + warp;
+    w.u = w.u0;
   };
   const uint64_t policy = l2_policy_evict_first();
   // copies run ahead of the products, from one list into the next
@@ -242,7 +235,7 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
       }
     }
     __syncwarp();
-    w.u += kWarps;
+    ++w.u;
     settle();
   };
   settle();
@@ -259,99 +252,90 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   if constexpr (C::ROW == 128) v_off[0] = 2 * t * 128 + ((r ^ (2 * t)) << 4), v_off[1] = v1 * 128 + ((r ^ v1) << 4);
   else v_off[0] = 2 * t * 64 + (((r >> 1) ^ t) << 4) + (r & 1) * 8, v_off[1] = v1 * 64 + (((r >> 1) ^ (v1 >> 1)) << 4) + (r & 1) * 8;
 
-  // a list's queries, read while the list before is finished: rows warp, warp + kWarps ..
-  constexpr int QR = ROWS / kWarps, QC = (D + 127) / 128;
-  uint2 q_raw[QR][QC];
-  int q_pos[QR];
-  auto read_queries = [&]() {
-#pragma unroll
-    for (int k = 0; k < QR; ++k) {
-      const int i = warp + k * kWarps, tok = z.s.row0 + i / group;
-      const bool live = i < min(z.s.rows * group, f.rows);
-      const T* qr = reinterpret_cast<const T*>(a.q) + (int64_t)tok * a.ldq + (int64_t)(z.kvh * group + i % group) * D;
-#pragma unroll
-      for (int c = 0; c < QC; ++c) {
-        q_raw[k][c] = make_uint2(0u, 0u);
-        if (live && c * 128 + lane * 4 < D) q_raw[k][c] = *reinterpret_cast<const uint2*>(qr + c * 128 + lane * 4);
-      }
-      q_pos[k] = -1;
-      if (live) {
-        const int sq = z.seg < f.own ? z.seg : seq_of_row(a.cu, 0, a.num_seqs, tok);
-        q_pos[k] = sq < 0 ? -1 : min(row_pos(a, sq, tok), z.s.hi - 1);
-      }
-    }
-  };
-  read_queries();
-
   for (unsigned cur = begin; cur < end;) {
     const Seg s = z.s;
     const int n = z.n, kvh = z.kvh, u0 = z.u0, u1 = z.u1, base = z.base;
     seg = z.seg;
     const int nrows = min(s.rows * group, f.rows);
 
-    // ---- queries: fragments, score factors, last visible keys
-    __syncthreads();                       // the list before is done with the buffers
+    // ---- queries: row r (and r + 8) lies in the four lanes that hold its fragments, a lane's 16 bytes of a key facing its own columns of the row
+    float qs[NT][2], qb[NT][2];            // of rows 2t, 2t + 1: score factor, what 128 added to a score
+    int pos[NT][2], all_pos = 0x7fffffff, max_pos = -1;   // and their last visible keys; the least and the largest of all rows
 #pragma unroll
-    for (int k = 0; k < QR; ++k) {
-      const int i = warp + k * kWarps;
-      float up = 1.f, qs = a.scale_log2, sum = 0.f;
-      if constexpr (FMT != kF16Pages) {
-        float m = 0.f;
+    for (int nt = 0; nt < NT; ++nt) {
+      const int i = nt * 8 + r, tok = s.row0 + i / group;
+      const bool live = i < nrows;
+      const T* qr = reinterpret_cast<const T*>(a.q) + (int64_t)tok * a.ldq + (int64_t)(kvh * group + i % group) * D + t * EPC;
+      uint4 raw[KS / 4][2];                // 16 columns each
 #pragma unroll
-        for (int c = 0; c < QC; ++c) {
-          const T* e = reinterpret_cast<const T*>(&q_raw[k][c]);
+      for (int c = 0; c < KS / 4; ++c)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) m = fmaxf(m, fabsf(to_f32(e[j])));
+        for (int h = 0; h < 2; ++h) {
+          const int d0 = EPC == 16 ? c * 64 + h * 8 : (2 * c + h) * 32;
+          raw[c][h] = live ? *reinterpret_cast<const uint4*>(qr + d0) : make_uint4(0u, 0u, 0u, 0u);
         }
-        m = warp_max(m);
-        const int e = m > 0.f && m < INFINITY ? max(-126, min(126, (int)((__float_as_uint(m) >> 23) & 255) - 127)) : 0;
+      float up = 1.f, f_q = a.scale_log2, sum = 0.f;
+      if constexpr (FMT != kF16Pages) {
+        float mx = 0.f;
+#pragma unroll
+        for (int c = 0; c < KS / 4; ++c)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float x[8];
+            unpack8<T>(raw[c][h], x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
+          }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const int e = mx > 0.f && mx < INFINITY ? max(-126, min(126, (int)((__float_as_uint(mx) >> 23) & 255) - 127)) : 0;
         up = __int_as_float((127 - e) << 23);
-        qs *= __int_as_float((127 + e) << 23);
+        f_q *= __int_as_float((127 + e) << 23);
       }
 #pragma unroll
-      for (int c = 0; c < QC; ++c) {
-        const int d0 = c * 128 + lane * 4;
-        if (d0 < D) {
-          uint2 w = q_raw[k][c];
-          if constexpr (FMT != kF16Pages) {
-            const T* e = reinterpret_cast<const T*>(&q_raw[k][c]);
-            float x[4];
+      for (int c = 0; c < KS / 4; ++c)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = to_f32(e[j]) * up;
-            // int8: a word's bytes 0, 2 and 1, 3 are converted together
-            const __half2 lo = FMT == kInt8 ? __floats2half2_rn(x[0], x[2]) : __floats2half2_rn(x[0], x[1]);
-            const __half2 hi = FMT == kInt8 ? __floats2half2_rn(x[1], x[3]) : __floats2half2_rn(x[2], x[3]);
-            w = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-            if constexpr (FMT == kInt8) {
-              const float2 l2 = __half22float2(lo), h2 = __half22float2(hi);
-              sum += (l2.x + l2.y) + (h2.x + h2.y);
+        for (int h = 0; h < 2; ++h) {
+          uint2 w[2] = {make_uint2(raw[c][h].x, raw[c][h].y), make_uint2(raw[c][h].z, raw[c][h].w)};
+          if constexpr (FMT != kF16Pages) {
+            float x[8];
+            unpack8<T>(raw[c][h], x);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              float y[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) y[e] = x[4 * k + e] * up;
+              // int8: a word's bytes 0, 2 and 1, 3 are converted together
+              const __half2 lo = FMT == kInt8 ? __floats2half2_rn(y[0], y[2]) : __floats2half2_rn(y[0], y[1]);
+              const __half2 hi = FMT == kInt8 ? __floats2half2_rn(y[1], y[3]) : __floats2half2_rn(y[2], y[3]);
+              w[k] = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+              if constexpr (FMT == kInt8) {
+                const float2 l2 = __half22float2(lo), h2 = __half22float2(hi);
+                sum += (l2.x + l2.y) + (h2.x + h2.y);
+              }
             }
           }
-          const int cc = d0 / EPC, step = ((cc >> 2) * EPC + d0 % EPC) / 4;
-          s_q[((i >> 3) * KS + step) * 32 + (i & 7) * 4 + (cc & 3)] = w;
+          s_q[(nt * KS + (2 * c + h) * 2) * 32] = w[0];
+          s_q[(nt * KS + (2 * c + h) * 2 + 1) * 32] = w[1];
         }
+      if constexpr (FMT == kInt8) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
       }
-      if constexpr (FMT == kInt8) sum = warp_sum(sum);
-      if (lane == 0) {
-        s_qb[i] = qs * 128.f * sum;
-        s_qs[i] = FMT == kInt8 ? qs * 16777216.f : qs;
-        s_pos[i] = q_pos[k];
+      int p = -1;
+      if (live) {
+        const int sq = seg < f.own ? seg : seq_of_row(a.cu, 0, a.num_seqs, tok);
+        p = sq < 0 ? -1 : min(row_pos(a, sq, tok), s.hi - 1);
       }
-    }
-    __syncthreads();
-    float qs[NT][2], qb[NT][2];
-    int pos[NT][2], all_pos = 0x7fffffff, max_pos = -1;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+      all_pos = min(all_pos, __reduce_min_sync(0xffffffffu, live ? p : 0x7fffffff));
+      max_pos = max(max_pos, __reduce_max_sync(0xffffffffu, p));
+      const float f_s = FMT == kInt8 ? f_q * 16777216.f : f_q, f_b = f_q * 128.f * sum;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        qs[nt][c] = s_qs[nt * 8 + 2 * t + c];
-        qb[nt][c] = s_qb[nt * 8 + 2 * t + c];
-        pos[nt][c] = s_pos[nt * 8 + 2 * t + c];
+        qs[nt][c] = __shfl_sync(0xffffffffu, f_s, (2 * t + c) * 4);
+        qb[nt][c] = __shfl_sync(0xffffffffu, f_b, (2 * t + c) * 4);
+        pos[nt][c] = __shfl_sync(0xffffffffu, p, (2 * t + c) * 4);
       }
-    for (int i = 0; i < nrows; ++i) {
-      all_pos = min(all_pos, s_pos[i]);
-      max_pos = max(max_pos, s_pos[i]);
     }
 
     float o[NT][KS][4], m[NT][2], m2[NT][2], l[NT][2];
@@ -370,7 +354,7 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
       }
     }
 
-    for (int u = u0 + warp; u < u1; u += kWarps) {
+    for (int u = u0; u < u1; ++u) {
       const int tok0 = base + u * UNIT;
       // some key of the unit is hidden from some row: the list's ends, and the causal border
       const bool edge = tok0 < s.lo || tok0 + UNIT - 1 > all_pos;
@@ -412,7 +396,7 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              const uint2 qf = s_q[(nt * KS + c * STEPS + st) * 32 + lane];
+              const uint2 qf = s_q[(nt * KS + c * STEPS + st) * 32];
               mma_16816<M>(x[i][nt], f0[0], f0[1], f1[0], f1[1], qf.x, qf.y);
             }
           }
@@ -576,7 +560,18 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
       if (++stage == STAGES) stage = 0, phase ^= 1;
     }
 
-    // ---- the four warps' parts
+    // ---- the list's result, or its part
+    const bool whole = u0 == 0 && u1 == n;
+    const bool last = whole && a.groups == 0;          // the result itself
+    const int slot = 2 * (int)me + (cur > begin ? 1 : 0);
+    if (u0 == 0 && lane == 0) {
+      FewInfo in;
+      in.first_slot = whole ? -1 : slot;
+      in.first_warp = me;
+      in.last_warp = (cur + n - 1) / per;
+      in.pad = 0;
+      pa.info[(int64_t)seg * a.hkv + kvh] = in;
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -585,76 +580,51 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 #pragma unroll
         for (int w = 4; w < 32; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
         const int i = nt * 8 + 2 * t + c;
-        if (i < nrows) {
-          if (r == 0) {
-            s_m[warp * ROWS + i] = m[nt][c] - (FMT == kF16Pages ? kUp : 0.f);       // what l and O stand relative to
-            s_m2[warp * ROWS + i] = (FMT != kF16Pages ? m2[nt][c] : m[nt][c]) - kUp;
-            s_l[warp * ROWS + i] = sum;
-          }
-          float* dst = s_o + (warp * f.rows + i) * LD;
-#pragma unroll
-          for (int k = 0; k < KS / 2; ++k) {           // rows f[4k] .. f[4k + 3] of the lane: neighbouring columns
-            const int e = 4 * k, col = VW >= 4 ? ((e / EPC) * 8 + r) * EPC + e % EPC : r * (D / 8) + e;
-            float4 y = make_float4(o[nt][2 * k][c], o[nt][2 * k][c + 2], o[nt][2 * k + 1][c], o[nt][2 * k + 1][c + 2]);
-            if constexpr (FMT == kInt8) {
-              const float off = -128.f * ps[nt][c];
-              y = make_float4(fmaf(y.x, 16777216.f, off), fmaf(y.y, 16777216.f, off), fmaf(y.z, 16777216.f, off), fmaf(y.w, 16777216.f, off));
-            }
-            *reinterpret_cast<float4*>(dst + col) = y;
+        if (i >= nrows) continue;
+        // what l and O stand relative to
+        const float ref = m[nt][c] - (FMT == kF16Pages ? kUp : 0.f);
+        float back = 1.f, off = 0.f;
+        if constexpr (FMT != kF16Pages) {
+          back = m2[nt][c] == -INFINITY ? 0.f : exp2f(m2[nt][c] - kUp - (m[nt][c] == -INFINITY ? 0.f : m[nt][c]));   // no value has a scale: zero
+          if constexpr (FMT == kInt8) {
+            off = -128.f * ps[nt][c] * back;
+            back *= 16777216.f;
           }
         }
+        const int tok = s.row0 + i / group, head = kvh * group + i % group;
+        if (last) {
+          // sum is NaN where a score was; a row without a visible key is zero
+          const float inv = pos[nt][c] < s.lo ? 0.f : 1.0f / sum;
+          back *= inv, off *= inv;
+          T* dst = reinterpret_cast<T*>(a.out) + (int64_t)tok * a.ldo + (int64_t)head * D;
+#pragma unroll
+          for (int k = 0; k < KS / 4; ++k) {           // eight neighbouring columns
+            const int e = 8 * k, col = VW >= 4 ? ((e / EPC) * 8 + r) * EPC + e % EPC : r * (D / 8) + e;
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              y[2 * j] = fmaf(o[nt][4 * k + j][c], back, off);
+              y[2 * j + 1] = fmaf(o[nt][4 * k + j][c + 2], back, off);
+            }
+            *reinterpret_cast<uint4*>(dst + col) = pack8<T>(y);
+          }
+        } else {
+          float* dst = whole ? (seg < f.own ? pa.whole_own : pa.whole_group) + ((int64_t)tok * a.hq + head) * (D + kPad)
+                             : pa.slots + ((int64_t)slot * f.rows + i) * (D + kPad);
+#pragma unroll
+          for (int k = 0; k < KS / 2; ++k) {
+            const int e = 4 * k, col = VW >= 4 ? ((e / EPC) * 8 + r) * EPC + e % EPC : r * (D / 8) + e;
+            *reinterpret_cast<float4*>(dst + col) = make_float4(fmaf(o[nt][2 * k][c], back, off), fmaf(o[nt][2 * k][c + 2], back, off),
+                                                                fmaf(o[nt][2 * k + 1][c], back, off), fmaf(o[nt][2 * k + 1][c + 2], back, off));
+          }
+          if (r == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(ref, sum);
+        }
       }
-    const unsigned next = cur + (u1 - u0);
-    if (next < end) {
-      z.cur = next;
+    cur += u1 - u0;
+    if (cur < end) {
+      z.cur = cur;
       open(z);
-      read_queries();
     }
-    __syncthreads();
-    const bool whole = u0 == 0 && u1 == n;
-    const bool last = whole && a.groups == 0;          // the result itself
-    float* part = nullptr;
-    if (!last && !whole) part = pa.slots + (int64_t)(2 * blockIdx.x + (cur > begin ? 1 : 0)) * f.rows * (D + kPad);
-    if (u0 == 0 && threadIdx.x == 0) {
-      FewInfo in;
-      in.first_slot = whole ? -1 : 2 * (int)blockIdx.x + (cur > begin ? 1 : 0);
-      in.first_block = blockIdx.x;
-      in.last_block = (cur + n - 1) / per;
-      in.pad = 0;
-      pa.info[(int64_t)seg * a.hkv + kvh] = in;
-    }
-    for (int e = threadIdx.x; e < nrows * (D / 4); e += 32 * kWarps) {
-      const int i = e / (D / 4), c = (e % (D / 4)) * 4;
-      float mx = -INFINITY, mx2 = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        mx = fmaxf(mx, s_m[w * ROWS + i]);
-        mx2 = fmaxf(mx2, s_m2[w * ROWS + i]);
-      }
-      const float z = mx == -INFINITY ? 0.f : mx, z2 = mx2 == -INFINITY ? 0.f : mx2;
-      float sum = 0.f;
-      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        sum += exp2_fast(s_m[w * ROWS + i] - z) * s_l[w * ROWS + i];
-        const float g = exp2_fast(s_m2[w * ROWS + i] - z2);
-        const float4 v = *reinterpret_cast<const float4*>(s_o + (w * f.rows + i) * LD + c);
-        y.x = fmaf(g, v.x, y.x), y.y = fmaf(g, v.y, y.y), y.z = fmaf(g, v.z, y.z), y.w = fmaf(g, v.w, y.w);
-      }
-      const float back = FMT == kF16Pages ? 1.f : mx2 == -INFINITY ? 0.f : exp2f(z2 - z);   // no value has a scale: zero
-      const int tok = s.row0 + i / group, head = kvh * group + i % group;
-      if (last) {
-        // sum is NaN where a score was; a row without a visible key is zero
-        const float inv = s_pos[i] < s.lo ? 0.f : back / sum;
-        T w[4] = {from_f32<T>(y.x * inv), from_f32<T>(y.y * inv), from_f32<T>(y.z * inv), from_f32<T>(y.w * inv)};
-        *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + (int64_t)tok * a.ldo + (int64_t)head * D + c) = *reinterpret_cast<const uint2*>(w);
-      } else {
-        float* dst = whole ? (seg < f.own ? pa.whole_own : pa.whole_group) + ((int64_t)tok * a.hq + head) * (D + kPad) : part + i * (D + kPad);
-        *reinterpret_cast<float4*>(dst + c) = make_float4(y.x * back, y.y * back, y.z * back, y.w * back);
-        if (c == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(mx, sum);
-      }
-    }
-    cur = next;
   }
   pdl_wait();
 }
@@ -670,8 +640,8 @@ int launch(const AttnArgs& a, const PartArgs& p, int blocks, bool beside, cudaSt
   f.rows = p.rows;
   f.page_magic = (uint32_t)(((1ull << 31) + a.page / 16 - 1) / (a.page / 16));
   f.beside = beside;
-  const int smem = C::smem(p.rows, f.segs);
-  LLMSS_CHECK_CUDA(configured.ensure(kern, C::smem(C::ROWS, kKept)));
+  const int smem = C::smem(f.segs);
+  LLMSS_CHECK_CUDA(configured.ensure(kern, C::smem(kKept)));
   const int64_t rows = (int64_t)a.num_blocks * a.hkv * a.page;
   CUtensorMap map_k, map_v;
   if (int e = encode_pages(&map_k, a.k, rows, D * C::ESZ, 16)) return e;
@@ -702,8 +672,8 @@ namespace pages {
 
 int few_blocks(int fmt, int d, int rows, int segs) {
   int ctas = 1;
-  LLMSS_FEW_D(ctas = fmt == kF16Pages ? (rows <= 8 ? Few<kF16Pages, D, 1>::ctas(rows, segs) : Few<kF16Pages, D, 2>::ctas(rows, segs))
-                                      : (rows <= 8 ? Few<kInt8, D, 1>::ctas(rows, segs) : Few<kInt8, D, 2>::ctas(rows, segs)));
+  LLMSS_FEW_D(ctas = fmt == kF16Pages ? (rows <= 8 ? Few<kF16Pages, D, 1>::ctas(segs) : Few<kF16Pages, D, 2>::ctas(segs))
+                                      : (rows <= 8 ? Few<kInt8, D, 1>::ctas(segs) : Few<kInt8, D, 2>::ctas(segs)));
   return 148 * ctas;
 }
 

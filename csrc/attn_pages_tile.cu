@@ -91,6 +91,24 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
   }
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {   // NaN where one of them is
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// 2^x without the MUFU pipe: x = n + r with r in [-0.5, 0.5], a cubic fitted to 2^r there (relative error 1.1e-4, below a rounding of the probability to
+// 16 bits), n added to the exponent; 2^-125 for what is below, and for NaN
+__device__ __forceinline__ float exp2_fma(float x) {
+  x = fmaxf(x, -125.0f);
+  const float t = x + 12582912.0f;                 // 1.5 * 2^23: the integer part lands in the low bits
+  const float r = x - (t - 12582912.0f);
+  float p = fmaf(r, 0.05459282f, 0.24221784f);
+  p = fmaf(r, p, 0.6933686f);
+  p = fmaf(r, p, 1.0f);
+  return __int_as_float(__float_as_int(p) + ((__float_as_int(t) - 0x4B400000) << 23));
+}
+
 // four codes -> code * scale in the 16-bit type, two words
 template <typename T, int FMT>
 __device__ __forceinline__ void convert4(uint32_t w, float scale, uint32_t& lo, uint32_t& hi) {
@@ -198,43 +216,28 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 
   if (warp == C::SOFT + 1) {
     // ===================== copying warp: all of it runs the loop, one lane issues
-    const int total = 2 * n_tiles;
     const uint64_t policy = l2_policy_evict_last();
     const int run = ta.run, runs = BN / run;
-    // cache rows of a tile's runs, one per lane; looked up a tile ahead of the copies
-    auto look_up = [&](int j) {
-      const int key = base + j * BN + min(lane, runs - 1) * run;
-      return key < k_hi ? ((uint32_t)checked_block(__ldg(s.table + key / a.page), a.num_blocks) * a.hkv + kvh) * a.page + key % a.page : 0u;
-    };
-    uint32_t rows = n_tiles > 0 ? look_up(0) : 0, rows_before = 0, rows_next = 0;   // of the newest tile of keys, of the one before, of the next one
-    uint32_t part_phase = 0;
-    for (int i = 0; i < total; ++i) {
-      // the ring holds K0, K1, V0, K2, V1 ..
-      const bool value = i == total - 1 || (i >= 2 && (i & 1) == 0);
-      const int j = i == total - 1 ? n_tiles - 1 : i == 0 ? 0 : value ? (i - 2) / 2 : (i + 1) / 2;
-      if (!value) {
-        if (j > 0) rows_before = rows, rows = rows_next;
-        rows_next = look_up(j + 1);
-      }
-      const uint32_t mine = value && j < n_tiles - 1 ? rows_before : rows;
+    uint32_t part_phase = 0, phase = 1;      // of the ring's barriers, the other way round: a slot's first use waits for nobody
+    int slot = 0;
+    // tile j of keys or values from the cache rows of its runs, in lanes from ..
+    auto copy = [&](int j, bool value, uint32_t rows, int from) {
       const int first = base + j * BN;
       const int here = min(runs, (k_hi - first + run - 1) / run);       // runs that lie in the list
       if constexpr (FMT == kF16Pages) {
-        const int slot = i % C::SLOTS;
-        mbar_wait(&bar_empty[slot], ((i / C::SLOTS) & 1) ^ 1, 80);
+        mbar_wait(&bar_empty[slot], phase, 80);
         const bool part = value && (first < s.lo || first + BN > k_hi);
         uint64_t* bar = part ? bar_part : &bar_full[slot];
         uint8_t* dst = s_kv + slot * C::SLOT;
         if (elect_one()) mbar_arrive_expect_tx(bar, here * run * D * 2);
-        __syncwarp();
         for (int x = 0; x < here; ++x) {
-          const int row = (int)__shfl_sync(0xffffffffu, mine, x);
+          const int row = (int)__shfl_sync(0xffffffffu, rows, from + x);
           if (elect_one()) {
 #pragma unroll
             for (int c = 0; c < DSUB; ++c) tma_load_2d(dst + c * (BN * 128) + x * run * 128, value ? &map_v : &map_k, bar, c * 128, row, policy);
           }
-          __syncwarp();
         }
+        __syncwarp();
         if (part) {
           // zeros where the list does not reach: 0 x NaN would be NaN
           mbar_wait(bar_part, part_phase, 78);
@@ -247,23 +250,38 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
           __syncwarp();
           if (lane == 0) mbar_arrive(&bar_full[slot]);
         }
+        if (++slot == C::SLOTS) slot = 0, phase ^= 1;
       } else {
-        const int slot = i % C::RAWS;
-        mbar_wait(&bar_used[slot], ((i / C::RAWS) & 1) ^ 1, 80);
+        mbar_wait(&bar_used[slot], phase, 80);
         uint8_t* dst = s_raw + slot * C::RAW;
         const uint8_t* src = reinterpret_cast<const uint8_t*>(value ? a.v : a.k);
         const float* sc = value ? a.vs : a.ks;
         if (elect_one()) mbar_arrive_expect_tx(&bar_raw[slot], here * run * (D + 4));
-        __syncwarp();
         for (int x = 0; x < here; ++x) {
-          const uint32_t row = __shfl_sync(0xffffffffu, mine, x);
+          const uint32_t row = __shfl_sync(0xffffffffu, rows, from + x);
           if (elect_one()) {
             bulk_copy(dst + x * run * D, src + (uint64_t)row * D, run * D, &bar_raw[slot]);
             bulk_copy(dst + BN * D + x * run * 4, sc + row, run * 4, &bar_raw[slot]);
           }
-          __syncwarp();
+        }
+        __syncwarp();
+        if (++slot == C::RAWS) slot = 0, phase ^= 1;
+      }
+    };
+    // keys a tile ahead of values, the rows of the runs eight tiles at a time (four lanes each)
+    uint32_t rows = 0, rows_before = 0;
+    for (int j = 0; j <= n_tiles; ++j) {
+      if ((j & 7) == 0) {
+        rows_before = rows;
+        const int key = base + (j + (lane >> 2)) * BN + min(lane & 3, runs - 1) * run;
+        rows = 0;
+        if (key < k_hi) {
+          const int pg = key / a.page;
+          rows = ((uint32_t)checked_block(__ldg(s.table + pg), a.num_blocks) * a.hkv + kvh) * a.page + (key - pg * a.page);
         }
       }
+      if (j < n_tiles) copy(j, false, rows, (j & 7) * 4);
+      if (j > 0) copy(j - 1, true, (j & 7) == 0 ? rows_before : rows, ((j - 1) & 7) * 4);
     }
   } else if (warp > C::SOFT + 1) {
     // ===================== converting warps
@@ -276,14 +294,13 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       const int flip = (ch >> 2) & 1;
       const uint32_t to = (ch >> 2) * (BN * 128) + key0 * 128, c0 = ((2 * (ch & 3) + flip) ^ (key0 & 7)) << 4;
       static_assert(KEYS % 8 == 0, "every eighth key has the same place in the swizzle");
-      const int total = 2 * n_tiles;
-      for (int i = 0; i < total; ++i) {
-        const bool value = i == total - 1 || (i >= 2 && (i & 1) == 0);
-        const int j = i == total - 1 ? n_tiles - 1 : i == 0 ? 0 : value ? (i - 2) / 2 : (i + 1) / 2;
+      int slot = 0, raw_slot = 0;
+      uint32_t phase = 1, raw_phase = 0;
+      auto convert = [&](int j) {
         const int first = base + j * BN;
         const bool all = first >= s.lo && first + BN <= k_hi;
-        const uint8_t* raw = s_raw + (i % C::RAWS) * C::RAW;
-        mbar_wait(&bar_raw[i % C::RAWS], (i / C::RAWS) & 1, 77);
+        const uint8_t* raw = s_raw + raw_slot * C::RAW;
+        mbar_wait(&bar_raw[raw_slot], raw_phase, 77);
         uint4 w[CH];
         float scale[CH];
 #pragma unroll
@@ -297,9 +314,10 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
           }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bar_used[i % C::RAWS]);
-        mbar_wait(&bar_empty[i % C::SLOTS], ((i / C::SLOTS) & 1) ^ 1, 81);
-        uint8_t* dst = s_kv + (i % C::SLOTS) * C::SLOT + to;
+        if (lane == 0) mbar_arrive(&bar_used[raw_slot]);
+        if (++raw_slot == C::RAWS) raw_slot = 0, raw_phase ^= 1;
+        mbar_wait(&bar_empty[slot], phase, 81);
+        uint8_t* dst = s_kv + slot * C::SLOT + to;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
           uint4 y[2];
@@ -313,7 +331,12 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bar_full[i % C::SLOTS]);
+        if (lane == 0) mbar_arrive(&bar_full[slot]);
+        if (++slot == C::SLOTS) slot = 0, phase ^= 1;
+      };
+      for (int j = 0; j <= n_tiles; ++j) {
+        if (j < n_tiles) convert(j);
+        if (j > 0) convert(j - 1);
       }
     }
   } else if (warp == C::SOFT) {
@@ -408,6 +431,7 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     // f16 ends at 2^16 and has no numbers below 2^-24: probabilities are formed times 2^7 (at most 2^15), so that those down to 2^-21 keep all bits
     constexpr float kUp = std::is_same<T, __half>::value ? 7.0f : 0.0f;
     float m_run = -INFINITY, l_run = 0.f;
+    bool bad = false;                                     // a score of the row is NaN: so is the result, whatever the exponentials made of it
     for (int j = 0; j < n_tiles; ++j) {
       const int b = j & 1, kb = base + j * BN;
       mbar_wait(&bar_s[q * 2 + b], (j >> 1) & 1, 85);
@@ -433,9 +457,10 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll
       for (int i = 0; i < BN; i += 8) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], fmaxf(sc[i + 2 * u], sc[i + 2 * u + 1]));
+        for (int u = 0; u < 4; ++u) mx[u] = max_nan(mx[u], max_nan(sc[i + 2 * u], sc[i + 2 * u + 1]));
       }
-      const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+      const float m_tile = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * scale;
+      bad = bad || m_tile != m_tile;
       const bool grow = m_tile > m_run + 8.0f;
       const float m_new = grow ? m_tile : m_run;
       const float alpha = grow && j > 0 ? exp2_fast(m_run - m_new) : 1.0f;
@@ -449,7 +474,8 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         for (int i = 0; i < 32; i += 2) {
           float e0, e1;
           ffma2(e0, e1, sc[c * 32 + i], sc[c * 32 + i + 1], scale, scale, neg, neg);
-          const float p0 = exp2_fast(e0), p1 = exp2_fast(e1);
+          // every fourth exponential on the FMA pipe: the MUFU pipe alone would need as many clocks as a tile's products
+          const float p0 = exp2_fast(e0), p1 = (i & 2) ? exp2_fast(e1) : exp2_fma(e1);
           fadd2(la[(i >> 1) & 3], lb[(i >> 1) & 3], la[(i >> 1) & 3], lb[(i >> 1) & 3], p0, p1);
           pk[i >> 1] = pack16<T>(p0, p1);
         }
@@ -487,7 +513,8 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       // the other tile's products read keys and values too
       mbar_wait(&bar_o[(q ^ 1) * 2 + ((n_tiles - 1) & 1)], n_tiles > 0 ? ((n_tiles - 1) >> 1) & 1 : 1, 88);
     }
-    // no visible key: zero (the sum is NaN where a score was)
+    if (bad) l_run = __int_as_float(0x7fc00000);
+    // no visible key: zero
     const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
     const int row_bytes = ta.direct ? D * 2 : C::OUT_ROW;
     const int stride = ta.direct ? D * 2 + 16 : C::OUT_ROW;
@@ -523,7 +550,7 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                            : (void*)((is_own ? pa.tile_own : pa.tile_group) + (((int64_t)split * a.total_q + tok) * a.hq + head) * (D + kPad));
       asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(smem_u32(mine)), "r"(row_bytes) : "memory");
       asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-      asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+      asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the rows have left; the grid's end makes them seen
     }
   }
 

@@ -2,15 +2,17 @@
 //
 //   k' = R(pos) k      scale = max_i |x_i| / qmax      code_i = round(x_i / scale)      x = k' or v, in 32 bits; qmax 127 (int8) or 448 (e4m3)
 //
-// A row (one token, one head) lies in d / 8 neighbouring lanes, 16 bytes each, so its largest value takes log2(d / 8) shuffles and nothing is
-// stored between: each value is read once and its code written once.  The divisions are the correctly rounded ones: codes are defined by them (a
-// product with the reciprocal rounds other values at the half steps), and they hide behind the loads.  The scales stand apart from the codes, so that a
+// A row (one token, one head) lies in d / 16 neighbouring lanes, two times 16 bytes each, the two halves of a rotated pair in one lane, so its largest value
+// takes log2(d / 16) shuffles and nothing is stored between: each value is read once and its code written once.  Codes are defined by the correctly rounded
+// quotient x / scale (a product with the reciprocal rounds other values at the half steps).  It is formed from r = 1 / scale, one per row, by Markstein's
+// correction: q = x r, q + r (x - q scale); a division per value would make the instructions, not the memory, the bound (8192 tokens of 32 heads of
+// 128: 130 us).  The scales stand apart from the codes, so that a
 // page's codes stay one block of block_size * d bytes whatever the head size.  Rows with a NaN or an infinity get scale NaN: what reads them sees it.
 // Angles are formed from turns in 64 bits, pos * f - rint(pos * f), one per token and frequency: at position 30000 the 32-bit product is off by
 // 2e-3 radians, half a bf16 step of the result.
 //
-// One block handles a token: its sines and cosines are formed once for all heads (a sine per lane and head would take as long as the copy).  A prompt's
-// tokens have a block each; a step's few tokens are split over blocks of 8 rows' warps, so that they are in flight at once.
+// One block handles a token: its sines and cosines are formed once for all heads and stay in registers (a sine per lane and head would take as long as the
+// copy).  A prompt's tokens have a block each; a step's few tokens are split over blocks, down to a row's warp each, so that they are in flight at once.
 #include "common.cuh"
 
 #include <cuda_fp8.h>
@@ -18,7 +20,7 @@
 
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
 
 struct QArgs {
   const int* positions;
@@ -35,26 +37,55 @@ struct QArgs {
   double turns[128];              // base^(-2 i / rotary_dim) / (2 pi)
 };
 
+__device__ __forceinline__ float max_nan(float a, float b) {   // NaN where one of them is
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t s) {
+  uint32_t r;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(s));
+  return r;
+}
+
+// eight codes of a row with this scale (r = 1 / scale)
 template <int FMT>
-__device__ __forceinline__ uint2 codes8(const float (&f)[8], float scale) {
-  uint2 r = make_uint2(0u, 0u);
-  if (!(scale > 0.f)) return r;   // a row of zeros, or one that is not finite
-  if constexpr (FMT == 1) {
-    uint32_t w[2] = {0u, 0u};
+__device__ __forceinline__ uint2 codes8(const float (&f)[8], float scale, float r) {
+  if (!(scale > 0.f)) return make_uint2(0u, 0u);   // a row of zeros, or one that is not finite
+  float q[8];
+  if (scale >= 0x1p-100f) {                        // the row's lanes agree
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int c = min(127, max(-127, __float2int_rn(__fdiv_rn(f[i], scale))));
-      w[i >> 2] |= ((uint32_t)c & 0xffu) << (8 * (i & 3));
+    for (int i = 0; i < 8; i += 2) {
+      float e0, e1;
+      fmul2(q[i], q[i + 1], f[i], f[i + 1], r, r);
+      ffma2(e0, e1, q[i], q[i + 1], -scale, -scale, f[i], f[i + 1]);
+      ffma2(q[i], q[i + 1], e0, e1, r, r, q[i], q[i + 1]);
     }
-    r = make_uint2(w[0], w[1]);
+  } else {                                         // the reciprocal, or what is left of a quotient, has no 32-bit number
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = __fdiv_rn(f[i], scale);
+  }
+  if constexpr (FMT == 1) {
+    uint32_t w[8];
+    if (scale < 0x1p-100f) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[i] = fminf(127.f, fmaxf(-127.f, q[i]));   // a scale below the normal numbers may be half a step off
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {               // 1.5 * 2^23 + q: rounded to a whole number, whose low byte is the code
+      float a, b;
+      fadd2(a, b, q[i], q[i + 1], 12582912.0f, 12582912.0f);
+      w[i] = __float_as_uint(a), w[i + 1] = __float_as_uint(b);
+    }
+    return make_uint2(prmt(prmt(w[0], w[1], 0x0040), prmt(w[2], w[3], 0x0040), 0x5410), prmt(prmt(w[4], w[5], 0x0040), prmt(w[6], w[7], 0x0040), 0x5410));
   } else {
     uint32_t h[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      h[i] = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(f[2 * i], scale), __fdiv_rn(f[2 * i + 1], scale)), __NV_SATFINITE, __NV_E4M3);
-    r = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+    for (int i = 0; i < 8; ++i) q[i] = copysignf(q[i], f[i]);   // the correction of -0 is +0
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __nv_cvt_float2_to_fp8x2(make_float2(q[2 * i], q[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+    return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
   }
-  return r;
 }
 
 template <typename T, int FMT>
@@ -69,89 +100,109 @@ __global__ void __launch_bounds__(32 * kWarps) rope_kv_write_q8_kernel(T* __rest
   const int slot = a.slots[t];
   const bool store = slot >= 0 && (int64_t)slot < a.num_slots;
   T* row = qkv + (int64_t)t * a.ld;
-  const int sub = lane / a.lanes, c = (lane % a.lanes) * 8;     // row of the warp, column of the row
-  // item -> this lane's vector; rows beyond the last head are the lanes' own business (`live`)
+  const int sub = lane / a.lanes, i = lane % a.lanes;           // row of the warp, place in the row
+  const int half = a.rotary_dim >> 1;
+  // this lane's two vectors of a row (first columns); NEOX: a pair's halves
+  const bool apart = a.style == LLMSS_ROPE_NEOX && i < half / 8;
+  const int ca = apart ? i * 8 : i * 16, cb = apart ? i * 8 + half : i * 16 + 8;
+  const bool turn_a = ca < a.rotary_dim, turn_b = cb < a.rotary_dim, has_b = cb < a.d;
+  // item -> this lane's row; rows beyond the last head are nobody's
   auto place = [&](int it, int& kind, int& h, T*& p) {
     kind = it < a.q_items ? 0 : it < a.q_items + a.kv_items ? 1 : 2;
     h = (it - (kind == 0 ? 0 : kind == 1 ? a.q_items : a.q_items + a.kv_items)) * a.per_warp + sub;
-    p = row + (kind == 0 ? a.q_off : kind == 1 ? a.k_off : a.v_off) + h * a.d + c;
-    return sub < a.per_warp && h < (kind == 0 ? a.hq : a.hkv) && (kind != 0 || c < a.rotary_dim) && (kind == 0 || store);
+    p = row + (kind == 0 ? a.q_off : kind == 1 ? a.k_off : a.v_off) + h * a.d;
+    return sub < a.per_warp && h < (kind == 0 ? a.hq : a.hkv) && (kind == 0 ? turn_a : store);
   };
   int kind = 0, h = 0;
   T* p = nullptr;
-  uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+  uint4 ra = make_uint4(0u, 0u, 0u, 0u), rb = ra;
   bool live = first < items && place(first, kind, h, p);
-  if (live) raw = *reinterpret_cast<const uint4*>(p);           // in flight while the angles are formed
-  const int half = a.rotary_dim >> 1;
+  if (live) {                                                   // in flight while the angles are formed
+    ra = *reinterpret_cast<const uint4*>(p + ca);
+    if (has_b) rb = *reinterpret_cast<const uint4*>(p + cb);
+  }
+  float cs[8], sn[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) cs[e] = 1.f, sn[e] = 0.f;
   if (a.style != LLMSS_ROPE_NONE) {
     const double pos = (double)a.positions[t];
-    for (int i = threadIdx.x; i < half; i += 32 * kWarps) {
-      const double x = pos * a.turns[i];
-      sincospif(2.0f * (float)(x - rint(x)), &s_sin[i], &s_cos[i]);
+    for (int x = threadIdx.x; x < half; x += 32 * kWarps) {
+      const double turns = pos * a.turns[x];
+      sincospif(2.0f * (float)(turns - rint(turns)), &s_sin[x], &s_cos[x]);
     }
     __syncthreads();
+    // of this lane's pairs: NEOX eight neighbouring ones, GPT-J four of each vector
+    const int fa = apart ? ca : ca >> 1, fb = apart ? ca + 4 : cb >> 1;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (turn_a) cs[e] = s_cos[fa + e], sn[e] = s_sin[fa + e];
+      if (turn_b) cs[4 + e] = s_cos[fb + e], sn[4 + e] = s_sin[fb + e];
+    }
   }
   for (int it = first; it < items; it += step) {
     int kind2 = 0, h2 = 0;
     T* p2 = nullptr;
-    uint4 raw2 = make_uint4(0u, 0u, 0u, 0u);
+    uint4 ra2 = make_uint4(0u, 0u, 0u, 0u), rb2 = ra2;
     const bool live2 = it + step < items && place(it + step, kind2, h2, p2);
-    if (live2) raw2 = *reinterpret_cast<const uint4*>(p2);
-    float f[8];
-    unpack8<T>(raw, f);
-    if (kind < 2 && a.style == LLMSS_ROPE_GPTJ) {
-      if (c < a.rotary_dim) {
+    if (live2) {
+      ra2 = *reinterpret_cast<const uint4*>(p2 + ca);
+      if (has_b) rb2 = *reinterpret_cast<const uint4*>(p2 + cb);
+    }
+    float x[8], y[8];
+    unpack8<T>(ra, x);
+    unpack8<T>(rb, y);
+    if (kind < 2 && a.style == LLMSS_ROPE_NEOX) {
+      if (apart) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float sn = s_sin[(c >> 1) + i], cs = s_cos[(c >> 1) + i], x1 = f[2 * i], x2 = f[2 * i + 1];
-          f[2 * i] = x1 * cs - x2 * sn;
-          f[2 * i + 1] = x2 * cs + x1 * sn;
+        for (int e = 0; e < 8; e += 2) {
+          float u0, u1, w0, w1;
+          fmul2(u0, u1, y[e], y[e + 1], -sn[e], -sn[e + 1]);
+          fmul2(w0, w1, x[e], x[e + 1], sn[e], sn[e + 1]);
+          ffma2(x[e], x[e + 1], x[e], x[e + 1], cs[e], cs[e + 1], u0, u1);
+          ffma2(y[e], y[e + 1], y[e], y[e + 1], cs[e], cs[e + 1], w0, w1);
         }
       }
-    } else if (kind < 2 && a.style == LLMSS_ROPE_NEOX) {
-      // the partner of column c is half a rotation away, in another lane of the row (half is a multiple of 8)
-      const bool lo = c < half;
-      const int other = lo ? lane + half / 8 : lane - half / 8;
-      float g[8];
+    } else if (kind < 2 && a.style == LLMSS_ROPE_GPTJ) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) g[i] = __shfl_sync(0xffffffffu, f[i], other & 31);
-      if (c < a.rotary_dim) {
-        const int w = lo ? c : c - half;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float sn = s_sin[w + i], cs = s_cos[w + i];
-          f[i] = lo ? f[i] * cs - g[i] * sn : f[i] * cs + g[i] * sn;
-        }
+      for (int e = 0; e < 4; ++e) {                             // columns that are not turned: cos 1, sin 0
+        const float x0 = x[2 * e], x1 = x[2 * e + 1], y0 = y[2 * e], y1 = y[2 * e + 1];
+        x[2 * e] = x0 * cs[e] - x1 * sn[e];
+        x[2 * e + 1] = x1 * cs[e] + x0 * sn[e];
+        y[2 * e] = y0 * cs[4 + e] - y1 * sn[4 + e];
+        y[2 * e + 1] = y1 * cs[4 + e] + y0 * sn[4 + e];
       }
     }
     if (kind == 0) {
-      if (live) *reinterpret_cast<uint4*>(p) = pack8<T>(f);
-    } else if (store) {                                          // uniform over the warp
-      float m = 0.f;
-      bool fin = true;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        m = fmaxf(m, fabsf(f[i]));
-        fin = fin && isfinite(f[i]);
+      if (live) {
+        *reinterpret_cast<uint4*>(p + ca) = pack8<T>(x);
+        if (turn_b) *reinterpret_cast<uint4*>(p + cb) = pack8<T>(y);
       }
-      if (!fin) m = INFINITY;                                    // a maximum drops NaNs: infinity stands for both
+    } else if (store) {                                          // uniform over the block
+      float m = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = max_nan(m, max_nan(fabsf(x[e]), fabsf(y[e])));
       if (a.per_warp > 1) {
-        for (int o = a.lanes >> 1; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        for (int o = a.lanes >> 1; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
       } else {
         if (!live) m = 0.f;
-        m = warp_max(m);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
       }
       const float scale = isfinite(m) ? __fdiv_rn(m, FMT == 1 ? 127.0f : 448.0f) : __int_as_float(0x7fc00000);
+      const float r = __frcp_rn(scale);
       if (live) {
-        const int64_t r = ((int64_t)(slot / a.block_size) * a.hkv + h) * a.block_size + slot % a.block_size;
-        *reinterpret_cast<uint2*>((kind == 1 ? a.k : a.v) + r * a.d + c) = codes8<FMT>(f, scale);
-        if (c == 0) (kind == 1 ? a.k_scale : a.v_scale)[r] = scale;
+        const int64_t at = ((int64_t)(slot / a.block_size) * a.hkv + h) * a.block_size + slot % a.block_size;
+        uint8_t* dst = (kind == 1 ? a.k : a.v) + at * a.d;
+        *reinterpret_cast<uint2*>(dst + ca) = codes8<FMT>(x, scale, r);
+        if (has_b) *reinterpret_cast<uint2*>(dst + cb) = codes8<FMT>(y, scale, r);
+        if (i == 0) (kind == 1 ? a.k_scale : a.v_scale)[at] = scale;
       }
     }
     kind = kind2;
     h = h2;
     p = p2;
-    raw = raw2;
+    ra = ra2;
+    rb = rb2;
     live = live2;
   }
 }
@@ -197,7 +248,7 @@ LLMSS_API int llmss_rope_kv_write_q8(void* qkv, const int* positions, const int*
   a.k_off = k_off;
   a.v_off = v_off;
   a.block_size = block_size;
-  a.lanes = d / 8;
+  a.lanes = (d + 15) / 16;
   a.per_warp = (a.lanes & (a.lanes - 1)) == 0 ? 32 / a.lanes : 1;
   a.q_items = a.rotary_dim > 0 ? (hq + a.per_warp - 1) / a.per_warp : 0;
   a.kv_items = (hkv + a.per_warp - 1) / a.per_warp;
