@@ -48,29 +48,21 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t s) {
   return r;
 }
 
-// eight codes of a row with this scale (r = 1 / scale)
-template <int FMT>
-__device__ __forceinline__ uint2 codes8(const float (&f)[8], float scale, float r) {
-  if (!(scale > 0.f)) return make_uint2(0u, 0u);   // a row of zeros, or one that is not finite
-  float q[8];
-  if (scale >= 0x1p-100f) {                        // the row's lanes agree
+// quotients x / scale, correctly rounded for scales of 2^-100 and more, r = 1 / scale
+__device__ __forceinline__ void quotients(float (&q)[8], const float (&x)[8], float scale, float r) {
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      float e0, e1;
-      fmul2(q[i], q[i + 1], f[i], f[i + 1], r, r);
-      ffma2(e0, e1, q[i], q[i + 1], -scale, -scale, f[i], f[i + 1]);
-      ffma2(q[i], q[i + 1], e0, e1, r, r, q[i], q[i + 1]);
-    }
-  } else {                                         // the reciprocal, or what is left of a quotient, has no 32-bit number
-#pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = __fdiv_rn(f[i], scale);
+  for (int i = 0; i < 8; i += 2) {
+    float e0, e1;
+    fmul2(q[i], q[i + 1], x[i], x[i + 1], r, r);
+    ffma2(e0, e1, q[i], q[i + 1], -scale, -scale, x[i], x[i + 1]);
+    ffma2(q[i], q[i + 1], e0, e1, r, r, q[i], q[i + 1]);
   }
+}
+
+template <int FMT>
+__device__ __forceinline__ uint2 codes8(const float (&q)[8]) {
   if constexpr (FMT == 1) {
     uint32_t w[8];
-    if (scale < 0x1p-100f) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) q[i] = fminf(127.f, fmaxf(-127.f, q[i]));   // a scale below the normal numbers may be half a step off
-    }
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {               // 1.5 * 2^23 + q: rounded to a whole number, whose low byte is the code
       float a, b;
@@ -81,10 +73,8 @@ __device__ __forceinline__ uint2 codes8(const float (&f)[8], float scale, float 
   } else {
     uint32_t h[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = copysignf(q[i], f[i]);   // the correction of -0 is +0
-#pragma unroll
     for (int i = 0; i < 4; ++i) h[i] = __nv_cvt_float2_to_fp8x2(make_float2(q[2 * i], q[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
-    return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+    return make_uint2(prmt(h[0], h[1], 0x5410), prmt(h[2], h[3], 0x5410));
   }
 }
 
@@ -94,33 +84,38 @@ __global__ void __launch_bounds__(32 * kWarps) rope_kv_write_q8_kernel(T* __rest
   pdl_wait();
   __shared__ float s_cos[128], s_sin[128];
   const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int items = a.q_items + 2 * a.kv_items;
   const int step = gridDim.y * kWarps;
   const int first = blockIdx.y * kWarps + warp;
   const int slot = a.slots[t];
   const bool store = slot >= 0 && (int64_t)slot < a.num_slots;
   T* row = qkv + (int64_t)t * a.ld;
+  const int64_t at0 = store ? (int64_t)(slot / a.block_size) * a.hkv * a.block_size + slot % a.block_size : 0;   // cache row of head 0
   const int sub = lane / a.lanes, i = lane % a.lanes;           // row of the warp, place in the row
   const int half = a.rotary_dim >> 1;
   // this lane's two vectors of a row (first columns); NEOX: a pair's halves
   const bool apart = a.style == LLMSS_ROPE_NEOX && i < half / 8;
   const int ca = apart ? i * 8 : i * 16, cb = apart ? i * 8 + half : i * 16 + 8;
   const bool turn_a = ca < a.rotary_dim, turn_b = cb < a.rotary_dim, has_b = cb < a.d;
-  // item -> this lane's row; rows beyond the last head are nobody's
-  auto place = [&](int it, int& kind, int& h, T*& p) {
-    kind = it < a.q_items ? 0 : it < a.q_items + a.kv_items ? 1 : 2;
-    h = (it - (kind == 0 ? 0 : kind == 1 ? a.q_items : a.q_items + a.kv_items)) * a.per_warp + sub;
-    p = row + (kind == 0 ? a.q_off : kind == 1 ? a.k_off : a.v_off) + h * a.d;
-    return sub < a.per_warp && h < (kind == 0 ? a.hq : a.hkv) && (kind == 0 ? turn_a : store);
+  // rows of one kind: this warp's every step-th group of per_warp heads
+  auto row_of = [&](int it, int off, int heads, bool wanted, T*& p) {
+    const int h = it * a.per_warp + sub;
+    p = row + off + h * a.d;
+    return wanted && h < heads && sub < a.per_warp;
   };
-  int kind = 0, h = 0;
-  T* p = nullptr;
+  // the kinds' items follow one another, q, k, v: where a warp begins in each, so that a step's few items spread over all warps
+  const int fq = first, fk = a.q_items > 0 ? (first + step - a.q_items % step) % step : first, fv = (fk + step - a.kv_items % step) % step;
   uint4 ra = make_uint4(0u, 0u, 0u, 0u), rb = ra;
-  bool live = first < items && place(first, kind, h, p);
-  if (live) {                                                   // in flight while the angles are formed
-    ra = *reinterpret_cast<const uint4*>(p + ca);
-    if (has_b) rb = *reinterpret_cast<const uint4*>(p + cb);
-  }
+  T* p = nullptr;
+  bool live = false;
+  auto fetch = [&](int it, int items, int off, int heads, bool wanted) {
+    live = it < items && row_of(it, off, heads, wanted, p);
+    ra = rb = make_uint4(0u, 0u, 0u, 0u);
+    if (live) {
+      ra = *reinterpret_cast<const uint4*>(p + ca);
+      if (has_b) rb = *reinterpret_cast<const uint4*>(p + cb);
+    }
+  };
+  if (fk < a.kv_items) fetch(fk, a.kv_items, a.k_off, a.hkv, store);    // in flight while the angles are formed
   float cs[8], sn[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) cs[e] = 1.f, sn[e] = 0.f;
@@ -139,19 +134,8 @@ __global__ void __launch_bounds__(32 * kWarps) rope_kv_write_q8_kernel(T* __rest
       if (turn_b) cs[4 + e] = s_cos[fb + e], sn[4 + e] = s_sin[fb + e];
     }
   }
-  for (int it = first; it < items; it += step) {
-    int kind2 = 0, h2 = 0;
-    T* p2 = nullptr;
-    uint4 ra2 = make_uint4(0u, 0u, 0u, 0u), rb2 = ra2;
-    const bool live2 = it + step < items && place(it + step, kind2, h2, p2);
-    if (live2) {
-      ra2 = *reinterpret_cast<const uint4*>(p2 + ca);
-      if (has_b) rb2 = *reinterpret_cast<const uint4*>(p2 + cb);
-    }
-    float x[8], y[8];
-    unpack8<T>(ra, x);
-    unpack8<T>(rb, y);
-    if (kind < 2 && a.style == LLMSS_ROPE_NEOX) {
+  auto turn = [&](float (&x)[8], float (&y)[8]) {
+    if (a.style == LLMSS_ROPE_NEOX) {
       if (apart) {
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
@@ -162,7 +146,7 @@ __global__ void __launch_bounds__(32 * kWarps) rope_kv_write_q8_kernel(T* __rest
           ffma2(y[e], y[e + 1], y[e], y[e + 1], cs[e], cs[e + 1], w0, w1);
         }
       }
-    } else if (kind < 2 && a.style == LLMSS_ROPE_GPTJ) {
+    } else if (a.style == LLMSS_ROPE_GPTJ) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {                             // columns that are not turned: cos 1, sin 0
         const float x0 = x[2 * e], x1 = x[2 * e + 1], y0 = y[2 * e], y1 = y[2 * e + 1];
@@ -172,38 +156,78 @@ __global__ void __launch_bounds__(32 * kWarps) rope_kv_write_q8_kernel(T* __rest
         y[2 * e + 1] = y1 * cs[4 + e] + y0 * sn[4 + e];
       }
     }
-    if (kind == 0) {
-      if (live) {
-        *reinterpret_cast<uint4*>(p + ca) = pack8<T>(x);
-        if (turn_b) *reinterpret_cast<uint4*>(p + cb) = pack8<T>(y);
-      }
-    } else if (store) {                                          // uniform over the block
-      float m = 0.f;
+  };
+  constexpr float kTop = FMT == 1 ? 127.0f : 448.0f;
+  // the row in x, y (zeros where the lane has none) -> codes and scale of cache row h
+  auto put = [&](float (&x)[8], float (&y)[8], bool mine, int h, uint8_t* codes, float* scales) {
+    float m = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) m = max_nan(m, max_nan(fabsf(x[e]), fabsf(y[e])));
-      if (a.per_warp > 1) {
-        for (int o = a.lanes >> 1; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-      } else {
-        if (!live) m = 0.f;
+    for (int e = 0; e < 8; ++e) m = max_nan(m, max_nan(fabsf(x[e]), fabsf(y[e])));
+    if (a.per_warp > 1) {
+      for (int o = a.lanes >> 1; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    } else {
+      if (!mine) m = 0.f;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-      }
-      const float scale = isfinite(m) ? __fdiv_rn(m, FMT == 1 ? 127.0f : 448.0f) : __int_as_float(0x7fc00000);
-      const float r = __frcp_rn(scale);
-      if (live) {
-        const int64_t at = ((int64_t)(slot / a.block_size) * a.hkv + h) * a.block_size + slot % a.block_size;
-        uint8_t* dst = (kind == 1 ? a.k : a.v) + at * a.d;
-        *reinterpret_cast<uint2*>(dst + ca) = codes8<FMT>(x, scale, r);
-        if (has_b) *reinterpret_cast<uint2*>(dst + cb) = codes8<FMT>(y, scale, r);
-        if (i == 0) (kind == 1 ? a.k_scale : a.v_scale)[at] = scale;
-      }
+      for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
     }
-    kind = kind2;
-    h = h2;
-    p = p2;
-    ra = ra2;
-    rb = rb2;
-    live = live2;
+    float scale, q[8], w[8];
+    if (__any_sync(0xffffffffu, m > 0.f && m < 0x1p-90f)) {
+      // a reciprocal, or what is left of a quotient, might have no 32-bit number; a scale below the normal numbers may be half a step off
+      scale = __fdiv_rn(m, kTop);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        q[e] = scale > 0.f ? fminf(kTop, fmaxf(-kTop, __fdiv_rn(x[e], scale))) + 0.f : 0.f;
+        w[e] = scale > 0.f ? fminf(kTop, fmaxf(-kTop, __fdiv_rn(y[e], scale))) + 0.f : 0.f;
+      }
+    } else {
+      scale = m * (1.0f / kTop);
+      scale = fmaf(fmaf(-scale, kTop, m), 1.0f / kTop, scale);
+      const float r = m > 0.f ? __frcp_rn(scale) : 0.f;
+      quotients(q, x, scale, r);
+      quotients(w, y, scale, r);
+    }
+    const bool finite = m < INFINITY;                           // not of NaN
+    const uint32_t keep = finite ? 0xffffffffu : 0u;
+    if (mine) {
+      const int64_t at = at0 + h * a.block_size;
+      uint8_t* dst = codes + at * a.d;
+      const uint2 c = codes8<FMT>(q), d = codes8<FMT>(w);
+      *reinterpret_cast<uint2*>(dst + ca) = make_uint2(c.x & keep, c.y & keep);
+      if (has_b) *reinterpret_cast<uint2*>(dst + cb) = make_uint2(d.x & keep, d.y & keep);
+      if (i == 0) scales[at] = finite ? scale : __int_as_float(0x7fc00000);
+    }
+  };
+  float x[8], y[8];
+  for (int it = fk; it < a.kv_items; it += step) {
+    unpack8<T>(ra, x);
+    unpack8<T>(rb, y);
+    const bool mine = live;
+    if (it + step < a.kv_items) fetch(it + step, a.kv_items, a.k_off, a.hkv, store);
+    else fetch(fv, a.kv_items, a.v_off, a.hkv, store);
+    turn(x, y);
+    if (store) put(x, y, mine, it * a.per_warp + sub, a.k, a.k_scale);
+  }
+  if (fk >= a.kv_items) fetch(fv, a.kv_items, a.v_off, a.hkv, store);
+  for (int it = fv; it < a.kv_items; it += step) {
+    unpack8<T>(ra, x);
+    unpack8<T>(rb, y);
+    const bool mine = live;
+    if (it + step < a.kv_items) fetch(it + step, a.kv_items, a.v_off, a.hkv, store);
+    else fetch(fq, a.q_items, a.q_off, a.hq, turn_a);
+    if (store) put(x, y, mine, it * a.per_warp + sub, a.v, a.v_scale);
+  }
+  if (fv >= a.kv_items) fetch(fq, a.q_items, a.q_off, a.hq, turn_a);
+  for (int it = fq; it < a.q_items; it += step) {
+    unpack8<T>(ra, x);
+    unpack8<T>(rb, y);
+    const bool mine = live;
+    T* to = p;
+    fetch(it + step, a.q_items, a.q_off, a.hq, turn_a);
+    turn(x, y);
+    if (mine) {
+      *reinterpret_cast<uint4*>(to + ca) = pack8<T>(x);
+      if (turn_b) *reinterpret_cast<uint4*>(to + cb) = pack8<T>(y);
+    }
   }
 }
 

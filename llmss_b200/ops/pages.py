@@ -59,5 +59,5 @@ def quantise(x: torch.Tensor, dtype):
     amax = x.abs().amax(-1)
     # a tensor below the line: torch divides by a plain number on the GPU through its reciprocal, which rounds twice
     scale = torch.where(torch.isfinite(x).all(-1), amax / torch.full_like(amax, QMAX[dtype]), torch.nan)
-    y = torch.where(scale[..., None] > 0, x / scale[..., None], 0.0).clamp(-QMAX[dtype], QMAX[dtype])
+    y = torch.where(scale[..., None] > 0, x / scale[..., None], 0.0).clamp(-QMAX[dtype], QMAX[dtype]) + 0.0      # -0 becomes 0
     return (y.round().to(dtype) if dtype == torch.int8 else y.to(dtype)), scale
