@@ -236,6 +236,38 @@ int launch_merge(const AttnArgs& a, const PartArgs& p, int parts, cudaStream_t s
   return 0;
 }
 
+// ---------------------------------------------------------------------------------------------------------------- codes as 16-bit pages
+// 64 keys of one sequence and key head: code * scale in the queries' type, [sequence][head][pad][d] of keys, then of values; a page per sequence, so that the
+// table names itself.  Bound by memory: 1 byte read, 2 written per value.
+template <typename T, int FMT>
+__global__ void __launch_bounds__(256) attn_pages_expand_kernel(const __grid_constant__ AttnArgs a, T* __restrict__ out, int* __restrict__ table, int pad) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int s = blockIdx.z, kvh = blockIdx.y, key0 = blockIdx.x * 64;
+  if (blockIdx.x == 0 && kvh == 0 && threadIdx.x == 0) table[s] = s;
+  const int len = min(min(a.seq_lens[s], a.max_blocks * a.page), pad);
+  if (key0 >= len) return;
+  const int per = a.d / 16;
+  const int64_t plane = (int64_t)a.num_seqs * a.hkv * pad * a.d;
+#pragma unroll 4
+  for (int x = threadIdx.x; x < 2 * 64 * per; x += 256) {
+    const int value = x >= 64 * per, y = value ? x - 64 * per : x;
+    const int key = key0 + y / per, c = (y % per) * 16;
+    if (key >= len) continue;
+    const int64_t row = ((int64_t)checked_block(a.tables[(int64_t)s * a.max_blocks + key / a.page], a.num_blocks) * a.hkv + kvh) * a.page + key % a.page;
+    const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(value ? a.v : a.k) + row * a.d + c);
+    const float scale = (value ? a.vs : a.ks)[row];
+    uint4 lo, hi;
+    convert4<T, FMT>(w.x, scale, lo.x, lo.y);
+    convert4<T, FMT>(w.y, scale, lo.z, lo.w);
+    convert4<T, FMT>(w.z, scale, hi.x, hi.y);
+    convert4<T, FMT>(w.w, scale, hi.z, hi.w);
+    T* to = out + value * plane + (((int64_t)s * a.hkv + kvh) * pad + key) * a.d + c;
+    *reinterpret_cast<uint4*>(to) = lo;
+    *reinterpret_cast<uint4*>(to + 8) = hi;
+  }
+}
+
 // ---------------------------------------------------------------------------------------------------------------- the choice
 struct Plan {
   bool any;             // the simple kernel for the whole call
@@ -244,7 +276,8 @@ struct Plan {
   TilePlan tile;
   int own_splits, own_chunk, group_splits, group_chunk;
   bool direct;          // the tiled kernel writes the result itself
-  int64_t slots, info, whole, tile_own, tile_group, floats;
+  int pad;              // codes become 16-bit pages of this many keys first (0: not)
+  int64_t slots, info, whole, tile_own, tile_group, expanded, floats;
 };
 
 // head sizes and pages of the tiled kernels
@@ -290,6 +323,14 @@ Plan plan_call(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv
     const int keys = groups > 0 ? (max_kv - g_max_len > max_q ? max_kv - g_max_len : max_q) : max_kv;
     stretches((int64_t)p.tile.own_tiles * hkv * num_seqs, keys, groups > 0, p.own_splits, p.own_chunk);
     p.direct = groups == 0 && p.own_splits == 1;
+    // Every row tile converts all codes for itself, which takes the tiled kernel from 1100 to 2000 clocks per 64 keys; once for all costs a pass over the
+    // cache (about 1200 clocks of an SM per 64 keys, and a launch).  Portions of 1000 tokens over 1800, 16 tiles: 240 -> 150 us; from three tiles on.  Up to
+    // 1 GB of scratch
+    const int64_t pad = ((int64_t)max_kv + 63) / 64 * 64, expanded = (int64_t)num_seqs * hkv * pad * d + (num_seqs + 3) / 4 * 4;
+    if (fmt != kF16Pages && groups == 0 && p.tile.own_tiles >= 3 && expanded <= (1ll << 28) && pad <= (1 << 19)) {
+      p.pad = (int)pad;
+      p.expanded = expanded;
+    }
     if (!p.direct) p.tile_own = (int64_t)p.own_splits * total_q * hq * (d + kPad);
   }
   if (tile_groups) {
@@ -297,7 +338,7 @@ Plan plan_call(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv
     stretches((int64_t)p.tile.group_tiles * hkv * groups, g_max_len, true, p.group_splits, p.group_chunk);
     p.tile_group = (int64_t)p.group_splits * total_q * hq * (d + kPad);
   }
-  p.floats = p.slots + p.info + (p.few_own ? p.whole : 0) + (p.few_groups ? p.whole : 0) + p.tile_own + p.tile_group;
+  p.floats = p.slots + p.info + (p.few_own ? p.whole : 0) + (p.few_groups ? p.whole : 0) + p.tile_own + p.tile_group + p.expanded;
   return p;
 }
 
@@ -334,12 +375,15 @@ LLMSS_API int64_t llmss_attn_pages_scratch_floats(int num_seqs, int max_q, int m
 // q [total_q][>= hq * d] (row stride ldq); K / V pages [num_blocks][hkv][block_size][d] of the queries' type (fmt 0) or of bytes with 32-bit scales
 // [num_blocks][hkv][block_size] (fmt 1 int8, 2 e4m3); sequence i owns the rows cu_q[i] .. cu_q[i + 1] - 1, the last positions of its seq_lens[i] cached
 // tokens.  groups > 0: the sequences g_first[j] .. g_first[j + 1] - 1 find their first g_lens[j] tokens in the pages g_tables[j].  max_q, max_kv,
-// g_max_len, g_max_rows bound the lengths.  out may alias q.  Rows of sequences without a visible key become zero; rows of no sequence stay as they are.
+// g_max_len, g_max_rows bound the lengths.  *launches: kernels launched (null: not wanted).  out may alias q.  Rows of sequences without a visible key become zero; rows of no sequence stay as they are.
 LLMSS_API int llmss_attn_pages(const void* q, int64_t ldq, const void* k_pages, const float* k_scale, const void* v_pages, const float* v_scale,
                                const int* block_tables, int max_blocks, const int* seq_lens, void* out, int64_t ldo, const int* cu_q, int num_seqs,
                                int max_q, int max_kv, int total_q, int hq, int hkv, int d, int block_size, int num_blocks, float scale, int fmt,
                                int dtype, const int* g_tables, int g_max_blocks, const int* g_lens, const int* g_first, int groups, int g_max_len,
-                               int g_max_rows, void* scratch, int64_t scratch_floats, cudaStream_t stream) {
+                               int g_max_rows, void* scratch, int64_t scratch_floats, int* launches, cudaStream_t stream) {
+  int none = 0;
+  if (launches == nullptr) launches = &none;
+  *launches = 0;
   AttnArgs a;
   memset(&a, 0, sizeof(a));
   a.q = q;
@@ -396,11 +440,38 @@ LLMSS_API int llmss_attn_pages(const void* q, int64_t ldq, const void* k_pages, 
     p.group_splits = plan.group_splits;
     p.group_chunk = plan.group_chunk;
     const bool tiles = plan.tile.own_tiles > 0 || plan.tile.group_tiles > 0;
-    if (tiles)
+    float* expanded = take(plan.expanded);
+    if (plan.pad > 0) {
+      // from here on the cache is the 16-bit copy, one page per sequence
+      int* table = (int*)(expanded + (int64_t)num_seqs * hkv * plan.pad * d);
+      const dim3 grid(plan.pad / 64, hkv, num_seqs);
+      LLMSS_REQUIRE(grid.y <= 65535 && grid.z <= 65535, "attn_pages: grid too large (%d key heads, %d sequences)", hkv, num_seqs);
+#define LLMSS_EXPAND(T_)                                                                                                                                     \
+  LLMSS_CHECK_CUDA(fmt == kInt8 ? launch_pdl(attn_pages_expand_kernel<T_, kInt8>, grid, dim3(256), 0, stream, a, (T_*)expanded, table, plan.pad)             \
+                                : launch_pdl(attn_pages_expand_kernel<T_, kE4M3>, grid, dim3(256), 0, stream, a, (T_*)expanded, table, plan.pad))
+      if (dtype == LLMSS_F16) LLMSS_EXPAND(__half);
+      else LLMSS_EXPAND(__nv_bfloat16);
+#undef LLMSS_EXPAND
+      ++*launches;
+      a.k = expanded;
+      a.v = (const uint16_t*)expanded + (int64_t)num_seqs * hkv * plan.pad * d;
+      a.ks = a.vs = nullptr;
+      a.tables = table;
+      a.max_blocks = 1;
+      a.page = plan.pad;
+      a.num_blocks = num_seqs;
+      fmt = kF16Pages;
+    }
+    if (tiles) {
       if (int e = tile_launch(a, p, plan.tile, fmt, dtype, stream)) return e;
+      ++*launches;
+    }
     if (plan.direct) return 0;
-    if (plan.few_own || plan.few_groups)
+    if (plan.few_own || plan.few_groups) {
       if (int e = few_launch(a, p, fmt, dtype, plan.blocks, tiles, stream)) return e;
+      ++*launches;
+    }
+    ++*launches;
     // parts of a row, about: runs of a list, or stretches
     const int64_t lists = ((int64_t)(plan.few_own ? num_seqs : 0) + (plan.few_groups ? a.groups : 0)) * hkv;
     const int64_t runs = lists > 0 ? (int64_t)plan.blocks * kFewWarps / lists : 0;
@@ -423,6 +494,7 @@ LLMSS_API int llmss_attn_pages(const void* q, int64_t ldq, const void* k_pages, 
     else LLMSS_ANY(__nv_bfloat16, kF16Pages);
   }
 #undef LLMSS_ANY
+  ++*launches;
   LLMSS_CHECK_CUDA(cudaGetLastError());
   return 0;
 }

@@ -136,6 +136,44 @@ __device__ __forceinline__ float exp2_fast(float x) {  // 2^x, one MUFU; 2^-inf 
   return y;
 }
 
+template <typename T>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+// four codes -> code * scale in the 16-bit type, two words
+template <typename T, int FMT>
+__device__ __forceinline__ void convert4(uint32_t w, float scale, uint32_t& lo, uint32_t& hi) {
+  float f[4];
+  if constexpr (FMT == kInt8) {
+    // 2^23 + (code + 128) as 32-bit numbers, less 2^23 + 128: exact
+    w ^= 0x80808080u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t u;
+      asm("prmt.b32 %0, %1, %2, %3;" : "=r"(u) : "r"(w), "r"(0x4B000000u), "r"(0x7540 + i));   // bytes: code, 0, 0, 0x4B
+      f[i] = __uint_as_float(u);
+    }
+    fadd2(f[0], f[1], f[0], f[1], -8388736.0f, -8388736.0f);
+    fadd2(f[2], f[3], f[2], f[3], -8388736.0f, -8388736.0f);
+  } else {
+    uint32_t a, b;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(a), "=r"(b) : "r"(w));
+    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&a)), y = __half22float2(*reinterpret_cast<const __half2*>(&b));
+    f[0] = x.x, f[1] = x.y, f[2] = y.x, f[3] = y.y;
+  }
+  fmul2(f[0], f[1], f[0], f[1], scale, scale);
+  fmul2(f[2], f[3], f[2], f[3], scale, scale);
+  lo = pack16<T>(f[0], f[1]);
+  hi = pack16<T>(f[2], f[3]);
+}
+
 __device__ __forceinline__ void bulk_copy(void* dst, const void* src, int bytes, uint64_t* bar) {   // addresses and size multiples of 16
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes),
                "r"(smem_u32(bar))

@@ -4,14 +4,15 @@
 // A block takes up to 256 rows (128 for 256 columns): a row is a (token, query head) of one key head, so that grouped heads fill a tile's 128 rows and every
 // key is read once for all of them.  It walks its keys in tiles of 64:
 //
-//   copying warp    keys and values page by page (TMA) into a ring of 128-byte swizzled tiles, keys a tile ahead of values; 8-bit codes into a ring of
-//                   their own, from which
+//   copying warps   one keys, one values, page by page (TMA), into a ring of 128-byte swizzled tiles, keys a tile ahead of values; 8-bit codes into a
+//                   ring of their own (bulk copies), from which
 //   converting warps (8-bit) write the tiles.  Values that lie outside of the list become zeros, keys there are never looked at
 //   issuing warp    S_j = Q K_j^T (two S buffers per 128 rows), O += P_j V_j with P_j in tensor memory over S_j
 //   softmax warps   a thread per row: its S row from tensor memory, mask, running maximum (moved when exceeded by 2^8) and sum in 32 bits, P back
 //
 // 8-bit codes are converted once per block for all its rows: code * scale is rounded to the queries' type, which is a rounding of the same size as a
-// 16-bit cache has, and well below the code's own step; with the scales multiplied to the scores instead, every row would pay for them.
+// 16-bit cache has, and well below the code's own step; with the scales multiplied to the scores instead, every row would pay for them.  Prompts of many
+// row tiles have their codes converted once for all blocks (attn_pages.cu) and come here as 16-bit pages.
 //
 // A list whose rows are few is cut into stretches of keys (grid x), whose parts the merge kernel joins.
 #include "attn_pages.cuh"
@@ -28,15 +29,14 @@ struct Tile {
   static constexpr int SOFT = 4 * NQ;                                   // softmax warps
   // 8-bit: four warps would convert a tile in twice the time that the products take
   static constexpr int CONVERT = FMT == kF16Pages ? 0 : 8;
-  static constexpr int THREADS = 32 * (SOFT + 2 + CONVERT);
+  static constexpr int THREADS = 32 * (SOFT + 3 + CONVERT);
   static constexpr int Q_BYTES = NQ * BM * D * 2;
   static constexpr int SLOT = BN * D * 2;                               // a tile of keys or values
   static constexpr int SLOTS = D == 256 ? (FMT == kF16Pages ? 4 : 3) : 6;
   static constexpr int RAW = FMT == kF16Pages ? 0 : BN * D + BN * 4;    // codes, then scales
   static constexpr int RAWS = FMT == kF16Pages ? 0 : D == 256 ? 3 : 4;
   static constexpr int SMEM = 1024 + Q_BYTES + SLOTS * SLOT + RAWS * RAW + 512;
-  static constexpr int OUT_ROW = D * 4 + kPad * 4;                      // a part; the result's rows are shorter
-  static_assert(SOFT * 32 * OUT_ROW <= Q_BYTES + SLOTS * SLOT, "outputs are staged where queries, keys and values were");
+  static_assert(SOFT * 32 * (D * 4 + 16) <= Q_BYTES + SLOTS * SLOT, "outputs are staged where queries, keys and values were");
   static constexpr int TMEM = NQ * (2 * BN + D) <= 256 ? 256 : 512;
 };
 
@@ -46,6 +46,7 @@ struct TileArgs {
   int own_chunk, group_chunk;     // keys, multiples of BN
   int segs_own;                   // sequences (0: not this launch's)
   int run;                        // keys of a tile that lie in one page: 16, 32 or 64
+  uint32_t page_magic;            // (key / 16) 2 this >> 32: the key's page
   int direct;                     // the result itself, not a part
 };
 
@@ -80,17 +81,6 @@ __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[
 }
 __device__ __forceinline__ void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack16(float a, float b) {
-  if constexpr (std::is_same<T, __half>::value) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  } else {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-}
-
 __device__ __forceinline__ float max_nan(float a, float b) {   // NaN where one of them is
   float d;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
@@ -107,33 +97,6 @@ __device__ __forceinline__ float exp2_fma(float x) {
   p = fmaf(r, p, 0.6933686f);
   p = fmaf(r, p, 1.0f);
   return __int_as_float(__float_as_int(p) + ((__float_as_int(t) - 0x4B400000) << 23));
-}
-
-// four codes -> code * scale in the 16-bit type, two words
-template <typename T, int FMT>
-__device__ __forceinline__ void convert4(uint32_t w, float scale, uint32_t& lo, uint32_t& hi) {
-  float f[4];
-  if constexpr (FMT == kInt8) {
-    // 2^23 + (code + 128) as 32-bit numbers, less 2^23 + 128: exact
-    w ^= 0x80808080u;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t u;
-      asm("prmt.b32 %0, %1, %2, %3;" : "=r"(u) : "r"(w), "r"(0x4B000000u), "r"(0x7540 + i));   // bytes: code, 0, 0, 0x4B
-      f[i] = __uint_as_float(u);
-    }
-    fadd2(f[0], f[1], f[0], f[1], -8388736.0f, -8388736.0f);
-    fadd2(f[2], f[3], f[2], f[3], -8388736.0f, -8388736.0f);
-  } else {
-    uint32_t a, b;
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(a), "=r"(b) : "r"(w));
-    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&a)), y = __half22float2(*reinterpret_cast<const __half2*>(&b));
-    f[0] = x.x, f[1] = x.y, f[2] = y.x, f[3] = y.y;
-  }
-  fmul2(f[0], f[1], f[0], f[1], scale, scale);
-  fmul2(f[2], f[3], f[2], f[3], scale, scale);
-  lo = pack16<T>(f[0], f[1]);
-  hi = pack16<T>(f[2], f[3]);
 }
 
 template <typename T, int FMT, int D, int NQ>
@@ -160,6 +123,10 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
+  if (FMT == kF16Pages && threadIdx.x == 32 * (C::SOFT + 1)) {
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
+  }
   pdl_wait();
 
   // the block's list, rows and keys
@@ -182,6 +149,15 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   const int base = k_lo & ~(BN - 1);
   const int n_tiles = k_hi > k_lo ? (k_hi - base + BN - 1) / BN : 0;
 
+  // the copying warps: cache rows of the runs of eight tiles from j on, one per lane (four lanes a tile)
+  auto look_up = [&](int j) {
+    const int key = base + (j + (lane >> 2)) * BN + min(lane & 3, BN / ta.run - 1) * ta.run;
+    if (key >= k_hi) return 0u;
+    const int pg = (int)__umulhi((unsigned)key >> 4 << 1, ta.page_magic);
+    return ((uint32_t)checked_block(__ldg(s.table + pg), a.num_blocks) * a.hkv + kvh) * a.page + (key - pg * a.page);
+  };
+  uint32_t run_rows = 0;
+  if (warp == C::SOFT + 1 || warp == C::SOFT + 2) run_rows = look_up(0);
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::SLOTS; ++i) {
       mbar_init(&bar_full[i], FMT == kF16Pages ? 1 : C::CONVERT);
@@ -214,18 +190,18 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   auto key_at = [&](int j) { return j == 0 ? 0 : 2 * j - 1; };
   auto value_at = [&](int j) { return j + 1 < n_tiles ? 2 * j + 2 : 2 * n_tiles - 1; };
 
-  if (warp == C::SOFT + 1) {
-    // ===================== copying warp: all of it runs the loop, one lane issues
+  if (warp == C::SOFT + 1 || warp == C::SOFT + 2) {
+    // ===================== copying warps: all of one runs its loop, one lane issues
     const uint64_t policy = l2_policy_evict_last();
     const int run = ta.run, runs = BN / run;
-    uint32_t part_phase = 0, phase = 1;      // of the ring's barriers, the other way round: a slot's first use waits for nobody
-    int slot = 0;
+    uint32_t part_phase = 0;
     // tile j of keys or values from the cache rows of its runs, in lanes from ..
-    auto copy = [&](int j, bool value, uint32_t rows, int from) {
+    auto copy = [&](int j, bool value, uint32_t rows, int from, int place) {
       const int first = base + j * BN;
       const int here = min(runs, (k_hi - first + run - 1) / run);       // runs that lie in the list
       if constexpr (FMT == kF16Pages) {
-        mbar_wait(&bar_empty[slot], phase, 80);
+        const int slot = place % C::SLOTS;
+        mbar_wait(&bar_empty[slot], ((place / C::SLOTS) & 1) ^ 1, 80);     // a slot's first use waits for nobody
         const bool part = value && (first < s.lo || first + BN > k_hi);
         uint64_t* bar = part ? bar_part : &bar_full[slot];
         uint8_t* dst = s_kv + slot * C::SLOT;
@@ -250,9 +226,9 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
           __syncwarp();
           if (lane == 0) mbar_arrive(&bar_full[slot]);
         }
-        if (++slot == C::SLOTS) slot = 0, phase ^= 1;
       } else {
-        mbar_wait(&bar_used[slot], phase, 80);
+        const int slot = place % C::RAWS;
+        mbar_wait(&bar_used[slot], ((place / C::RAWS) & 1) ^ 1, 80);
         uint8_t* dst = s_raw + slot * C::RAW;
         const uint8_t* src = reinterpret_cast<const uint8_t*>(value ? a.v : a.k);
         const float* sc = value ? a.vs : a.ks;
@@ -265,28 +241,17 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
           }
         }
         __syncwarp();
-        if (++slot == C::RAWS) slot = 0, phase ^= 1;
       }
     };
-    // keys a tile ahead of values, the rows of the runs eight tiles at a time (four lanes each)
-    uint32_t rows = 0, rows_before = 0;
-    for (int j = 0; j <= n_tiles; ++j) {
-      if ((j & 7) == 0) {
-        rows_before = rows;
-        const int key = base + (j + (lane >> 2)) * BN + min(lane & 3, runs - 1) * run;
-        rows = 0;
-        if (key < k_hi) {
-          const int pg = key / a.page;
-          rows = ((uint32_t)checked_block(__ldg(s.table + pg), a.num_blocks) * a.hkv + kvh) * a.page + (key - pg * a.page);
-        }
-      }
-      if (j < n_tiles) copy(j, false, rows, (j & 7) * 4);
-      if (j > 0) copy(j - 1, true, (j & 7) == 0 ? rows_before : rows, ((j - 1) & 7) * 4);
+    const bool value = warp == C::SOFT + 2;
+    for (int j = 0; j < n_tiles; ++j) {
+      if (j > 0 && (j & 7) == 0) run_rows = look_up(j);
+      copy(j, value, run_rows, (j & 7) * 4, value ? value_at(j) : key_at(j));
     }
-  } else if (warp > C::SOFT + 1) {
+  } else if (warp > C::SOFT + 2) {
     // ===================== converting warps
     if constexpr (FMT != kF16Pages) {
-      const int tid = threadIdx.x - 32 * (C::SOFT + 2);
+      const int tid = threadIdx.x - 32 * (C::SOFT + 3);
       constexpr int PER = D / 16, KEYS = 32 * C::CONVERT / PER;      // 16-byte chunks of a key, keys between a thread's chunks
       constexpr int CH = BN / KEYS;                                // a thread's chunks of a tile
       const int key0 = tid / PER, ch = tid % PER;                  // this thread's first key, its place in every key
@@ -474,8 +439,9 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         for (int i = 0; i < 32; i += 2) {
           float e0, e1;
           ffma2(e0, e1, sc[c * 32 + i], sc[c * 32 + i + 1], scale, scale, neg, neg);
-          // every fourth exponential on the FMA pipe: the MUFU pipe alone would need as many clocks as a tile's products
-          const float p0 = exp2_fast(e0), p1 = (i & 2) ? exp2_fast(e1) : exp2_fma(e1);
+          // every fourth exponential on the FMA pipe: the MUFU pipe alone would need as many clocks as a tile's products.  Not beside converting warps, where
+          // instructions are what is short
+          const float p0 = exp2_fast(e0), p1 = FMT != kF16Pages || (i & 2) ? exp2_fast(e1) : exp2_fma(e1);
           fadd2(la[(i >> 1) & 3], lb[(i >> 1) & 3], la[(i >> 1) & 3], lb[(i >> 1) & 3], p0, p1);
           pk[i >> 1] = pack16<T>(p0, p1);
         }
@@ -507,8 +473,8 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       tcgen05_fence_after();
     }
     // every product has been formed, so queries, keys and values make room: rows go through shared memory, each lane's in a place of its own (a row is
-    // 16 bytes longer than a multiple of 128, so that eight lanes never meet in a bank), and from there as whole rows (a lane's 16 bytes to a row of its
-    // own would be 32 transactions per instruction: 9600 clocks for 256 rows of 132 numbers)
+    // 16 bytes longer than a multiple of 128, so that eight lanes never meet in a bank), and from there by the whole warp (a lane's 16 bytes to a row of its
+    // own are 32 transactions per instruction: 9600 clocks for 256 rows of 132 numbers; a bulk copy per row: 6400)
     if constexpr (NQ > 1) {
       // the other tile's products read keys and values too
       mbar_wait(&bar_o[(q ^ 1) * 2 + ((n_tiles - 1) & 1)], n_tiles > 0 ? ((n_tiles - 1) >> 1) & 1 : 1, 88);
@@ -516,9 +482,9 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     if (bad) l_run = __int_as_float(0x7fc00000);
     // no visible key: zero
     const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
-    const int row_bytes = ta.direct ? D * 2 : C::OUT_ROW;
-    const int stride = ta.direct ? D * 2 + 16 : C::OUT_ROW;
-    uint8_t* mine = smem + (q * BM + quarter * 32 + lane) * stride;
+    const int stride = ta.direct ? D * 2 + 16 : D * 4 + 16;
+    uint8_t* stage = smem + (q * BM + quarter * 32) * stride;
+    uint8_t* mine = stage + lane * stride;
 #pragma unroll 1
     for (int c = 0; c < D / 32; ++c) {
       uint32_t r[32];
@@ -542,16 +508,34 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(mine + c * 128 + i * 4) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
       }
     }
-    if (!ta.direct) *reinterpret_cast<float4*>(mine + D * 4) = make_float4(m_run - kUp, l_run, 0.f, 0.f);
-    fence_proxy_async_smem();
-    __syncwarp();
+    uint8_t* to = nullptr;
     if (live) {
-      void* to = ta.direct ? (void*)(reinterpret_cast<T*>(a.out) + (int64_t)tok * a.ldo + (int64_t)head * D)
-                           : (void*)((is_own ? pa.tile_own : pa.tile_group) + (((int64_t)split * a.total_q + tok) * a.hq + head) * (D + kPad));
-      asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(smem_u32(mine)), "r"(row_bytes) : "memory");
-      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-      asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the rows have left; the grid's end makes them seen
+      if (ta.direct) {
+        to = reinterpret_cast<uint8_t*>(reinterpret_cast<T*>(a.out) + (int64_t)tok * a.ldo + (int64_t)head * D);
+      } else {
+        float* part = (is_own ? pa.tile_own : pa.tile_group) + (((int64_t)split * a.total_q + tok) * a.hq + head) * (D + kPad);
+        *reinterpret_cast<float2*>(part + D) = make_float2(m_run - kUp, l_run);
+        to = reinterpret_cast<uint8_t*>(part);
+      }
     }
+    __syncwarp();
+    auto rows_out = [&](auto bytes) {
+      constexpr int PER = decltype(bytes)::value / 16, LANES = PER < 32 ? PER : 32;   // 16 bytes of a row per lane
+#pragma unroll 4
+      for (int i = 0; i < 32; i += 32 / LANES) {
+        const int row = i + lane / LANES;
+        const uint64_t at = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(to), row);
+        if (at != 0) {
+#pragma unroll
+          for (int c = 0; c < PER; c += LANES) {
+            const int x = (c + lane % LANES) * 16;
+            *reinterpret_cast<uint4*>(at + x) = *reinterpret_cast<const uint4*>(stage + row * stride + x);
+          }
+        }
+      }
+    };
+    if (ta.direct) rows_out(std::integral_constant<int, D * 2>{});
+    else rows_out(std::integral_constant<int, D * 4>{});
   }
 
   tcgen05_fence_before();
@@ -578,6 +562,7 @@ int launch(const AttnArgs& a, const PartArgs& p, const TilePlan& t, cudaStream_t
   ta.group_chunk = p.group_chunk;
   ta.segs_own = t.own_tiles > 0 ? a.num_seqs : 0;
   ta.direct = a.groups == 0 && p.own_splits == 1;
+  ta.page_magic = (uint32_t)(((1ull << 31) + a.page / 16 - 1) / (a.page / 16));
   ta.run = a.page % 64 == 0 ? 64 : a.page % 32 == 0 ? 32 : 16;
   CUtensorMap map_k, map_v;
   memset(&map_k, 0, sizeof(map_k));

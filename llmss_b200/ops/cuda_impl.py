@@ -343,6 +343,8 @@ def rope_kv_write_q8(qkv, positions, slot_mapping, k_pages, v_pages, hq, hkv, d,
     _count()
 
 
+_LAUNCHED = C.c_int(0)                     # kernels of the last call
+_LAUNCHED_AT = C.addressof(_LAUNCHED)
 _NO_GROUPS = (None, 0, None, None, 0, 0, 0)
 
 
@@ -385,9 +387,9 @@ def attention_pages(qkv, out, batch, k_pages, v_pages, hq, hkv, d, scale, q_off=
     scratch = torch.empty(floats, dtype=torch.float32, device=qkv.device) if floats else None
     rc = lib.llmss_attn_pages(qkv.data_ptr() + 2 * q_off, ldq, k.data_ptr(), ks, v.data_ptr(), vs, bt.data_ptr(), bt.shape[1], sl.data_ptr(),
                               out.data_ptr() + 2 * out_off, ldo, cu_q.data_ptr(), B, batch.max_q, batch.max_kv, T, hq, hkv, d, shape[2], shape[0],
-                              float(scale), fmt, _DT[dtype], *g, None if scratch is None else scratch.data_ptr(), floats, _stream())
+                              float(scale), fmt, _DT[dtype], *g, None if scratch is None else scratch.data_ptr(), floats, _LAUNCHED_AT, _stream())
     _lib.check(rc, "llmss_attn_pages")
-    _count(1 if not floats else 3 if g[4] and (batch.max_q * hq <= 16 * hkv) != (p.max_rows * hq <= 16 * hkv) else 2)
+    _count(_LAUNCHED.value)
 
 
 # --------------------------------------------------------------------------- embed / sample
