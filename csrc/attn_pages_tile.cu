@@ -7,7 +7,8 @@
 //   copying warps   one keys, one values, page by page (TMA), into a ring of 128-byte swizzled tiles, keys a tile ahead of values; 8-bit codes into a
 //                   ring of their own (bulk copies), from which
 //   converting warps (8-bit) write the tiles.  Values that lie outside of the list become zeros, keys there are never looked at
-//   issuing warp    S_j = Q K_j^T (two S buffers per 128 rows), O += P_j V_j with P_j in tensor memory over S_j
+//   issuing warps   one per 128 rows: S_j = Q K_j^T (two S buffers), O += P_j V_j with P_j in tensor memory over S_j.  (A product takes about 60 clocks to
+//                   issue beside the other warps, so that one warp for 256 rows took 2100 clocks a tile where the products take 1100)
 //   softmax warps   a thread per row: its S row from tensor memory, mask, running maximum (moved when exceeded by 2^8) and sum in 32 bits, P back
 //
 // 8-bit codes are converted once per block for all its rows: code * scale is rounded to the queries' type, which is a rounding of the same size as a
@@ -29,7 +30,8 @@ struct Tile {
   static constexpr int SOFT = 4 * NQ;                                   // softmax warps
   // 8-bit: four warps would convert a tile in twice the time that the products take
   static constexpr int CONVERT = FMT == kF16Pages ? 0 : 8;
-  static constexpr int THREADS = 32 * (SOFT + 3 + CONVERT);
+  static constexpr int COPY = SOFT + NQ;                                // first copying warp
+  static constexpr int THREADS = 32 * (COPY + 2 + CONVERT);
   static constexpr int Q_BYTES = NQ * BM * D * 2;
   static constexpr int SLOT = BN * D * 2;                               // a tile of keys or values
   static constexpr int SLOTS = D == 256 ? (FMT == kF16Pages ? 4 : 3) : 6;
@@ -115,15 +117,15 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   uint64_t* bar_s = bars + 2 * C::SLOTS;                 // [NQ][2] S ready
   uint64_t* bar_p = bar_s + 2 * NQ;                      // [NQ][2] P written
   uint64_t* bar_o = bar_p + 2 * NQ;                      // [NQ][2] P V done
-  uint64_t* bar_q = bar_o + 2 * NQ;                      // queries are in place
-  uint64_t* bar_part = bar_q + 1;                        // a tile at the list's end, before its zeros
+  uint64_t* bar_q = bar_o + 2 * NQ;                      // [NQ] queries are in place
+  uint64_t* bar_part = bar_q + NQ;                       // a tile at the list's end, before its zeros
   uint64_t* bar_raw = bar_part + 1;                      // [RAWS] codes have come
   uint64_t* bar_used = bar_raw + C::RAWS;                // [RAWS] codes have been converted
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_used + C::RAWS);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
-  if (FMT == kF16Pages && threadIdx.x == 32 * (C::SOFT + 1)) {
+  if (FMT == kF16Pages && threadIdx.x == 32 * C::COPY) {
     tma_prefetch_desc(&map_k);
     tma_prefetch_desc(&map_v);
   }
@@ -157,18 +159,18 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     return ((uint32_t)checked_block(__ldg(s.table + pg), a.num_blocks) * a.hkv + kvh) * a.page + (key - pg * a.page);
   };
   uint32_t run_rows = 0;
-  if (warp == C::SOFT + 1 || warp == C::SOFT + 2) run_rows = look_up(0);
+  if (warp == C::COPY || warp == C::COPY + 1) run_rows = look_up(0);
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::SLOTS; ++i) {
       mbar_init(&bar_full[i], FMT == kF16Pages ? 1 : C::CONVERT);
-      mbar_init(&bar_empty[i], 1);
+      mbar_init(&bar_empty[i], NQ);
     }
     for (int i = 0; i < 2 * NQ; ++i) {
       mbar_init(&bar_s[i], 1);
       mbar_init(&bar_p[i], 4);
       mbar_init(&bar_o[i], 1);
     }
-    mbar_init(bar_q, C::SOFT);
+    for (int i = 0; i < NQ; ++i) mbar_init(&bar_q[i], 4);
     mbar_init(bar_part, 1);
     for (int i = 0; i < C::RAWS; ++i) {
       mbar_init(&bar_raw[i], 1);
@@ -190,7 +192,7 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   auto key_at = [&](int j) { return j == 0 ? 0 : 2 * j - 1; };
   auto value_at = [&](int j) { return j + 1 < n_tiles ? 2 * j + 2 : 2 * n_tiles - 1; };
 
-  if (warp == C::SOFT + 1 || warp == C::SOFT + 2) {
+  if (warp == C::COPY || warp == C::COPY + 1) {
     // ===================== copying warps: all of one runs its loop, one lane issues
     const uint64_t policy = l2_policy_evict_last();
     const int run = ta.run, runs = BN / run;
@@ -243,15 +245,15 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         __syncwarp();
       }
     };
-    const bool value = warp == C::SOFT + 2;
+    const bool value = warp == C::COPY + 1;
     for (int j = 0; j < n_tiles; ++j) {
       if (j > 0 && (j & 7) == 0) run_rows = look_up(j);
       copy(j, value, run_rows, (j & 7) * 4, value ? value_at(j) : key_at(j));
     }
-  } else if (warp > C::SOFT + 2) {
+  } else if (warp > C::COPY + 1) {
     // ===================== converting warps
     if constexpr (FMT != kF16Pages) {
-      const int tid = threadIdx.x - 32 * (C::SOFT + 3);
+      const int tid = threadIdx.x - 32 * (C::COPY + 2);
       constexpr int PER = D / 16, KEYS = 32 * C::CONVERT / PER;      // 16-byte chunks of a key, keys between a thread's chunks
       constexpr int CH = BN / KEYS;                                // a thread's chunks of a tile
       const int key0 = tid / PER, ch = tid % PER;                  // this thread's first key, its place in every key
@@ -304,56 +306,52 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         if (j > 0) convert(j - 1);
       }
     }
-  } else if (warp == C::SOFT) {
-    // ===================== issuing warp: all of it runs the loop, one lane issues
+  } else if (warp >= C::SOFT) {
+    // ===================== issuing warps: all of one runs its loop, one lane issues
+    const int q = warp - C::SOFT;
     const int fmt = std::is_same<T, __half>::value ? 0 : 1;
     const uint32_t id_s = idesc(fmt, BN, 0), id_o = idesc(fmt, D, 1);
-    const uint32_t q_lo = desc_lo(smem_u32(s_q)), k_lo0 = desc_lo(smem_u32(s_kv)), v_lo0 = desc_lo(smem_u32(s_kv), BN * 128);
-    auto scores = [&](int q, int j) {
-      const uint32_t ql = q_lo + q * (BM * D * 2 / 16), kl = k_lo0 + (key_at(j) % C::SLOTS) * (C::SLOT / 16);
+    const uint32_t ql = desc_lo(smem_u32(s_q)) + q * (BM * D * 2 / 16), k_lo = desc_lo(smem_u32(s_kv)), v_lo = desc_lo(smem_u32(s_kv), BN * 128);
+    const uint32_t ts = t_s(q, 0), to = t_o(q);
+    // places in the ring: keys 0, 1, 3, 5 .., values 2, 4 .. and one behind the last keys
+    int k_slot = 0, v_slot = n_tiles > 1 ? 2 : 1;
+    uint32_t k_phase = 0, v_phase = 0;
+    auto scores = [&](int j) {
+      mbar_wait(&bar_full[k_slot], k_phase, 82);
+      tcgen05_fence_after();
+      const uint32_t kl = k_lo + k_slot * (C::SLOT / 16), d = ts + (j & 1) * BN;
       if (elect_one()) {
 #pragma unroll
         for (int c = 0; c < DSUB; ++c)
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_ss(t_s(q, j & 1), ql + (c * (BM * 128) + k * 32) / 16, kl + (c * (BN * 128) + k * 32) / 16, id_s, (c | k) ? 1u : 0u);
+          for (int k = 0; k < 4; ++k) umma_ss(d, ql + (c * (BM * 128) + k * 32) / 16, kl + (c * (BN * 128) + k * 32) / 16, id_s, (c | k) ? 1u : 0u);
         umma_commit(&bar_s[q * 2 + (j & 1)]);
-        if (q == NQ - 1) umma_commit(&bar_empty[key_at(j) % C::SLOTS]);
+        umma_commit(&bar_empty[k_slot]);
       }
       __syncwarp();
+      k_slot += j == 0 ? 1 : 2;
+      if (k_slot >= C::SLOTS) k_slot -= C::SLOTS, k_phase ^= 1;
     };
-    auto wait_full = [&](int i) { mbar_wait(&bar_full[i % C::SLOTS], (i / C::SLOTS) & 1, 82); };
-    if (n_tiles > 0) mbar_wait(bar_q, 0, 79);
-    for (int j = 0; j < min(n_tiles, 2); ++j) {
-      wait_full(key_at(j));
-      tcgen05_fence_after();
-#pragma unroll
-      for (int q = 0; q < NQ; ++q) scores(q, j);
-    }
+    if (n_tiles > 0) mbar_wait(&bar_q[q], 0, 79);
+    for (int j = 0; j < min(n_tiles, 2); ++j) scores(j);
     for (int j = 0; j < n_tiles; ++j) {
       const int b = j & 1;
-      wait_full(value_at(j));
+      mbar_wait(&bar_full[v_slot], v_phase, 82);
+      mbar_wait(&bar_p[q * 2 + b], (j >> 1) & 1, 83);
+      tcgen05_fence_after();
+      const uint32_t vl = v_lo + v_slot * (C::SLOT / 16), p = ts + b * BN;
+      if (elect_one()) {
 #pragma unroll
-      for (int q = 0; q < NQ; ++q) {
-        mbar_wait(&bar_p[q * 2 + b], (j >> 1) & 1, 83);
-        tcgen05_fence_after();
-        const uint32_t vl = v_lo0 + (value_at(j) % C::SLOTS) * (C::SLOT / 16);
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < BN / 16; ++k) umma_ts(t_o(q), t_s(q, b) + k * 8, vl + k * 128, id_o, (j > 0 || k > 0) ? 1u : 0u);
-          umma_commit(&bar_o[q * 2 + b]);
-          if (q == NQ - 1) umma_commit(&bar_empty[value_at(j) % C::SLOTS]);
-        }
-        __syncwarp();
+        for (int k = 0; k < BN / 16; ++k) umma_ts(to, p + k * 8, vl + k * 128, id_o, (j > 0 || k > 0) ? 1u : 0u);
+        umma_commit(&bar_o[q * 2 + b]);
+        umma_commit(&bar_empty[v_slot]);
       }
+      __syncwarp();
+      v_slot += j + 2 < n_tiles ? 2 : 1;
+      if (v_slot >= C::SLOTS) v_slot -= C::SLOTS, v_phase ^= 1;
       if (j + 2 < n_tiles) {
-        wait_full(key_at(j + 2));
-#pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-          mbar_wait(&bar_o[q * 2 + b], (j >> 1) & 1, 84);    // P_j has been read: S_{j+2} goes over it
-          tcgen05_fence_after();
-          scores(q, j + 2);
-        }
+        mbar_wait(&bar_o[q * 2 + b], (j >> 1) & 1, 84);        // P_j has been read: S_{j+2} goes over it
+        scores(j + 2);
       }
     }
   } else {
@@ -390,7 +388,7 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       copies_wait<0>();
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar_q);
+      if (lane == 0) mbar_arrive(&bar_q[q]);
     }
     const float scale = a.scale_log2;
     // f16 ends at 2^16 and has no numbers below 2^-24: probabilities are formed times 2^7 (at most 2^15), so that those down to 2^-21 keep all bits
