@@ -123,7 +123,8 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   uint64_t* bar_used = bar_raw + C::RAWS;                // [RAWS] codes have been converted
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_used + C::RAWS);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // by a shuffle: numbers that the compiler knows to be the same in all lanes need no copies into uniform registers at every product
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   pdl_launch_dependents();
   if (FMT == kF16Pages && threadIdx.x == 32 * C::COPY) {
     tma_prefetch_desc(&map_k);
@@ -149,7 +150,7 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   const int k_lo = max(s.lo, s.lo + split * chunk);
   const int k_hi = split == splits - 1 ? k_end : min(k_end, s.lo + (split + 1) * chunk);
   const int base = k_lo & ~(BN - 1);
-  const int n_tiles = k_hi > k_lo ? (k_hi - base + BN - 1) / BN : 0;
+  const int n_tiles = __shfl_sync(0xffffffffu, k_hi > k_lo ? (k_hi - base + BN - 1) / BN : 0, 0);
 
   // the copying warps: cache rows of the runs of eight tiles from j on, one per lane (four lanes a tile)
   auto look_up = [&](int j) {
@@ -185,7 +186,7 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   auto t_s = [&](int q, int b) { return tmem + q * (2 * BN + D) + b * BN; };
   auto t_o = [&](int q) { return tmem + q * (2 * BN + D) + 2 * BN; };
   // places of tiles in the ring: K0, then K_{j+1}, V_j, and V of the last tile
