@@ -40,6 +40,8 @@ def get_args(argv=None):
     parser.add_argument("--seed", type=int, default=0)
     parser.add_argument("--sliding_window", action="store_true",
                         help="keep generating past the model's context over the most recent tokens (rotary-position models)")
+    parser.add_argument("--kv_cache_dtype", type=str, default=None, choices=["int8", "fp8"],
+                        help="keep the KV cache in 8 bits (models with multi-head keys and values)")
     return parser.parse_args(argv)
 
 
@@ -66,7 +68,7 @@ def main(argv=None):
 
     engine = Engine.from_pretrained(args.pretrained_model_path, dtype=getattr(torch, args.dtype), device=device,
                                     process_group=process_group, max_batch=max(1, len(args.prompts or args.prompt_ids)),
-                                    eos_token_id=None, sliding_window=args.sliding_window)
+                                    eos_token_id=None, sliding_window=args.sliding_window, kv_cache_dtype=args.kv_cache_dtype)
     max_len = engine.runner.max_seq_len
 
     # rank 0 tokenises; ids are shared with one broadcast (reference N5, generate.py:73-85)

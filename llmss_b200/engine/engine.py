@@ -57,13 +57,14 @@ class Engine:
                  num_blocks: Optional[int] = None, use_cuda_graph: Optional[bool] = None,
                  max_prefill_tokens: int = 16384, eos_token_id: Optional[int] = None,
                  prefill_chunk: Optional[int] = None, sliding_window: bool = False, prefix_cache: bool = False,
-                 pool_tokens: Optional[int] = None):
+                 pool_tokens: Optional[int] = None, kv_cache_dtype: Optional[str] = None, shared_prefix: bool = False):
         self.model = model
         self.core = model.core if hasattr(model, "core") else model
         self.comm = self.core.comm
         self.runner = ModelRunner(self.core, max_batch=max_batch, max_seq_len=max_seq_len, block_size=block_size,
                                   num_blocks=num_blocks, use_cuda_graph=use_cuda_graph, prefill_chunk=prefill_chunk,
-                                  sliding_window=sliding_window, prefix_cache=prefix_cache, pool_tokens=pool_tokens)
+                                  sliding_window=sliding_window, prefix_cache=prefix_cache, pool_tokens=pool_tokens,
+                                  kv_cache_dtype=kv_cache_dtype, shared_prefix=shared_prefix)
         self.max_batch = max_batch
         self.max_prefill_tokens = max_prefill_tokens
         self.eos_token_id = eos_token_id
@@ -227,7 +228,7 @@ class Engine:
         if not self.running:
             return outs
         if self._dirty:
-            self.running = [s for s in self.running if not s.finished]
+            self.running = self.runner.by_prefix([s for s in self.running if not s.finished])
             self.runner.set_batch(self.running)
             self._dirty = False
             if not self.running:

@@ -33,6 +33,36 @@ class KVCache:
         self.data[:, :, dst:dst + n] = old.data[:, :, src:src + n]
 
 
+class QuantKVCache:
+    """KVCache in 8 bits: codes (``"int8"`` or ``"fp8"``, e4m3) and a 32-bit scale per token and head, about half of the 16-bit cache's bytes
+    (d + 4 instead of 2 d per token, head and side).  ``k(layer)`` / ``v(layer)`` are ``ops.QuantPages``."""
+
+    def __init__(self, num_layers: int, num_blocks: int, block_size: int, kv_heads: int, head_dim: int, kind: str, device):
+        from ..ops.pages import NAMES, QuantPages
+
+        if kind not in NAMES:
+            raise ValueError(f"8-bit cache pages are {' or '.join(map(repr, sorted(NAMES)))}, got {kind!r}")
+        self.num_layers, self.num_blocks, self.block_size = num_layers, num_blocks, block_size
+        self.kv_heads, self.head_dim = kv_heads, head_dim
+        self.data = torch.zeros(num_layers, 2, num_blocks, kv_heads, block_size, head_dim, dtype=torch.int8, device=device).view(NAMES[kind])
+        self.scale = torch.zeros(num_layers, 2, num_blocks, kv_heads, block_size, dtype=torch.float32, device=device)
+        self.pages = [[QuantPages(self.data[i, j], self.scale[i, j]) for j in range(2)] for i in range(num_layers)]
+
+    def k(self, layer: int):
+        return self.pages[layer][0]
+
+    def v(self, layer: int):
+        return self.pages[layer][1]
+
+    @staticmethod
+    def bytes_per_block(num_layers, block_size, kv_heads, head_dim) -> int:
+        return num_layers * 2 * block_size * kv_heads * (head_dim + 4)
+
+    def copy_blocks_from(self, old: "QuantKVCache", src: int, dst: int, n: int):
+        self.data.view(torch.int8)[:, :, dst:dst + n] = old.data.view(torch.int8)[:, :, src:src + n]
+        self.scale[:, :, dst:dst + n] = old.scale[:, :, src:src + n]
+
+
 class LatentCache:
     """Paged cache of latent-attention layers: ONE vector per token and layer run (the RMS-normed down-projection
     from which keys and values of every head are re-derived), instead of a key and a value per head.

@@ -22,10 +22,12 @@ import torch
 from .. import ops
 from ..models.decoder import DecoderLM
 from ..utils.metrics import METRICS
-from .batch import BatchInput
+from .batch import BatchInput, SharedPrefix
 from .kv_cache import BlockAllocator, SlotAllocator
 
 _BUCKETS = (1, 2, 4, 8, 16, 24, 32, 48, 64, 96, 128, 192, 256)
+_MAX_GROUPS = 8                                                                        # prefixes of one step
+_SHARE_MIN_BYTES = int(os.environ.get("LLMSS_SHARE_MIN_BYTES", str(64 << 20)))      # reads per layer that sharing saves
 
 
 @dataclass
@@ -81,7 +83,8 @@ class ModelRunner:
     def __init__(self, core: DecoderLM, max_batch: int = 64, max_seq_len: Optional[int] = None,
                  block_size: Optional[int] = None, num_blocks: Optional[int] = None,
                  use_cuda_graph: Optional[bool] = None, prefill_chunk: Optional[int] = None,
-                 sliding_window: bool = False, prefix_cache: bool = False, pool_tokens: Optional[int] = None):
+                 sliding_window: bool = False, prefix_cache: bool = False, pool_tokens: Optional[int] = None,
+                 kv_cache_dtype: Optional[str] = None, shared_prefix: bool = False):
         self.core, self.spec = core, core.spec
         self.device, self.dtype = core.device, core.dtype
         self.max_batch = max_batch
@@ -110,7 +113,11 @@ class ModelRunner:
         if num_blocks is None:
             num_blocks = 1 + max_batch * self.max_blocks_per_seq
         # multi-head K / V pages, latent planes, or pages plus state slots: the model knows
-        self.kv = core.make_cache(num_blocks, block_size, max_seqs=max_batch)
+        # 8-bit pages ("int8" / "fp8"): half the bytes per cached token, so that the attention of a step reads half as much and a pool holds twice as much
+        if kv_cache_dtype is not None and not isinstance(core, DecoderLM):
+            raise ValueError(f"kv_cache_dtype={kv_cache_dtype!r}: {type(core).__name__} keeps its own kind of cache")
+        self.quantised = kv_cache_dtype is not None
+        self.kv = core.make_cache(num_blocks, block_size, max_seqs=max_batch, **({"kv_dtype": kv_cache_dtype} if self.quantised else {}))
         self.alloc = BlockAllocator(num_blocks)
         self.slots = SlotAllocator(max_batch) if self.recurrent else None
         self._outstanding = 0   # blocks reserved at admission and not yet allocated
@@ -122,13 +129,20 @@ class ModelRunner:
         if prefix_cache and self.recurrent:
             raise ValueError("prefix_cache: a model with recurrent layers cannot resume from cached pages alone")
         self.prefix_enabled = bool(prefix_cache)
+        # Decode steps whose sequences hold the same cached blocks at their front read those once for all of them
+        if shared_prefix and not (prefix_cache and isinstance(core, DecoderLM)):
+            raise ValueError("shared_prefix: needs prefix_cache and a model with multi-head K / V pages")
+        if shared_prefix and self.sliding:
+            raise ValueError("shared_prefix: a sliding window takes blocks off the front of a sequence")
+        self.shared_prefix = bool(shared_prefix)
+        self._prefix: Optional[tuple] = None     # (groups, bound on their tokens) of the bound batch, None: no sharing
         self._nodes: Dict[tuple, tuple] = {}
         self._block_key: Dict[int, tuple] = {}
         self._next_node = 1
         self.alloc.on_evict = self._forget_block
         self.cuda = self.device.type == "cuda"
         self.use_graph = self.cuda if use_cuda_graph is None else (use_cuda_graph and self.cuda)
-        self.graphs: Dict[tuple, torch.cuda.CUDAGraph] = {}   # (padded batch, vocab-parallel greedy) -> graph
+        self.graphs: Dict[tuple, torch.cuda.CUDAGraph] = {}   # (padded batch, vocab-parallel greedy, bounds of shared prefixes) -> graph
         self.launches_per_graph: Dict[int, int] = {}   # own-kernel launches captured per decode graph
         self._all_greedy = True
         self._vp_sampling_ok = True
@@ -180,6 +194,10 @@ class ModelRunner:
         self.d_last_idx = torch.arange(B, dtype=torch.int64, device=self.device)
         self.d_cu = torch.arange(B + 1, dtype=torch.int32, device=self.device)
         self.batch_seqs: List[SeqState] = []
+        if self.shared_prefix:
+            G = 2 * _MAX_GROUPS                  # with the rows between them
+            self.h_pfx = torch.zeros(G * mb + 2 * G + 1, dtype=torch.int32, pin_memory=pin)     # [block tables | tokens | first rows]
+            self.d_pfx = torch.zeros_like(self.h_pfx, device=self.device)
 
     def _dev_views(self, B: int):
         buf, MB, mb = self.d_in, self.max_batch, self.max_blocks_per_seq
@@ -350,6 +368,77 @@ class ModelRunner:
             s.output.append(int(t))
         return [int(t) for t in toks]
 
+    # ------------------------------------------------------------------ shared prefixes
+    def by_prefix(self, seqs: List[SeqState]) -> List[SeqState]:
+        """The sequences in an order that puts those with the same blocks at their front next to each other (as they are without shared_prefix)."""
+        return sorted(seqs, key=lambda s: s.blocks) if self.shared_prefix else seqs
+
+    def prefix_groups(self, seqs: Sequence[SeqState]):
+        """[(first row, rows, common blocks)] of neighbours with a common front worth its own pass: what the sequences would read again for themselves
+        takes memory longer than the second kernel and the merge do (about 10 us, 64 MB)."""
+        out, i = [], 0
+        per_token = 2 * self.core.hkv * (self.core.d + 4 if self.quantised else 2 * self.core.d)
+        while i < len(seqs):
+            j, common = i + 1, list(seqs[i].blocks[:seqs[i].length // self.block_size])
+            while j < len(seqs) and common:
+                n = 0
+                for a, b in zip(common, seqs[j].blocks[:seqs[j].length // self.block_size]):
+                    if a != b:
+                        break
+                    n += 1
+                if n == 0:
+                    break
+                common = common[:n]
+                j += 1
+            if j - i > 1:
+                out.append((i, j - i, common))
+            i = j
+        worth = lambda g: (g[1] - 1) * len(g[2]) * self.block_size * per_token
+        if sum(map(worth, out)) < _SHARE_MIN_BYTES:
+            return []
+        return sorted(sorted(out, key=worth, reverse=True)[:_MAX_GROUPS])
+
+    def _bind_prefix(self, seqs: Sequence[SeqState]):
+        """Groups of the bound batch into the step's static buffers.  Rows between groups belong to groups of no tokens."""
+        self._prefix = None
+        groups = self.prefix_groups(seqs) if self.shared_prefix else []
+        if not groups:
+            return
+        spans, at = [], groups[0][0]
+        for first, rows, common in groups:
+            if first > at:
+                spans.append((at, []))
+            spans.append((first, common))
+            at = first + rows
+        n = 1
+        while n < len(spans):
+            n *= 2
+        G, mb = 2 * _MAX_GROUPS, self.max_blocks_per_seq
+        ends = [s[0] for s in spans[1:]] + [at]
+        self.h_pfx.zero_()
+        for k in range(n):
+            if k < len(spans):
+                first, common = spans[k]
+                self.h_pfx[k * mb:k * mb + len(common)] = torch.tensor(common, dtype=torch.int32)
+                self.h_pfx[G * mb + k] = len(common) * self.block_size
+                self.h_pfx[G * mb + G + k] = first
+                self.h_pfx[G * mb + G + k + 1] = ends[k]
+            else:
+                self.h_pfx[G * mb + G + k + 1] = ends[-1]
+        self.d_pfx.copy_(self.h_pfx)           # behind the steps that are enqueued; the pinned buffer is not rewritten before it has been read
+        bound = self.block_size
+        while bound < max(len(c) for _, c in spans) * self.block_size:
+            bound *= 2
+        self._prefix = (n, min(bound, self.max_blocks_per_seq * self.block_size))
+
+    def _step_prefix(self, Bp: int) -> Optional[SharedPrefix]:
+        if self._prefix is None:
+            return None
+        n, bound = self._prefix
+        G, mb = 2 * _MAX_GROUPS, self.max_blocks_per_seq
+        return SharedPrefix(block_tables=self.d_pfx[:G * mb].view(G, mb), lens=self.d_pfx[G * mb:G * mb + G], first=self.d_pfx[G * mb + G:],
+                            num_groups=n, max_len=bound, max_rows=Bp)
+
     # ------------------------------------------------------------------ decode
     def _bucket(self, B: int) -> int:
         for b in _BUCKETS:
@@ -394,6 +483,7 @@ class ModelRunner:
             self.np_sslot_row[i] = s.state_slot
             if s.output:
                 self.np_tok[i] = s.output[-1]
+        self._bind_prefix(seqs)
         self.d_samp_i.copy_(self.h_samp_i, non_blocking=True)
         self.d_samp_f.copy_(self.h_samp_f, non_blocking=True)
         self.d_rng.copy_(rng.to(self.device))
@@ -457,7 +547,7 @@ class ModelRunner:
         batch = BatchInput(tokens=tok, positions=pos, slot_mapping=slot, block_tables=bt, seq_lens=slen,
                            cu_q=self.d_cu[:Bp + 1], last_idx=self.d_last_idx[:Bp], num_seqs=Bp, max_q=1,
                            max_kv=self.max_seq_len, is_decode=True, is_fresh_prefill=False, decode_splits=splits,
-                           state_slots=sslot if self.recurrent else None)
+                           state_slots=sslot if self.recurrent else None, prefix=self._step_prefix(Bp))
         # the sampler writes into the token region: it is both this step's result and the next
         # step's input (device-side feedback loop; no host round trip needed between steps)
         if vp_greedy:
@@ -480,8 +570,8 @@ class ModelRunner:
             return 1
         if Bp in self._tuned_splits:
             return self._tuned_splits[Bp]
-        if not hasattr(self.core, "hkv"):
-            return 0    # models without multi-head K / V pages pick their own split per call
+        if self.quantised or not hasattr(self.core, "hkv"):
+            return 0    # 8-bit pages and models without multi-head K / V pages pick their own split per call
         from ..ops import cuda_impl as cu
 
         return cu.decode_splits(Bp, self.core.hq, self.core.hkv, self.core.d, self.max_seq_len, self.dtype,
@@ -492,7 +582,7 @@ class ModelRunner:
         (batch bucket, heads per rank, current context length) and keep the fastest.  Read-only on the
         KV cache; ~1 ms once per captured graph."""
         c = self.core
-        if not hasattr(c, "hkv"):
+        if self.quantised or not hasattr(c, "hkv"):
             return 0
         if not self.cuda or c.d not in (64, 128, 256):
             return 1
@@ -531,7 +621,7 @@ class ModelRunner:
     def capture(self, Bp: int, vp: bool = False):
         """Warm up and capture the decode graph for a padded batch size, on inert inputs
         (slot -1, seq_len 0: no cache writes), then restore the live step state."""
-        if not self.use_graph or (Bp, vp) in self.graphs:
+        if not self.use_graph or (Bp, vp, self._prefix) in self.graphs:
             return
         splits = self._tuned_splits[Bp] if Bp in self._tuned_splits else self.autotune_decode_splits(Bp)
         saved_in, saved_rng = self.d_in.clone(), self.d_rng.clone()
@@ -559,7 +649,7 @@ class ModelRunner:
         self.launches_per_graph[Bp] = _lib.LAUNCHES["count"] - n0
         if self.graph_pool is None:
             self.graph_pool = g.pool()
-        self.graphs[(Bp, vp)] = g
+        self.graphs[(Bp, vp, self._prefix)] = g
         self.d_in.copy_(saved_in)
         self.d_rng.copy_(saved_rng)
         torch.cuda.synchronize()
@@ -569,7 +659,7 @@ class ModelRunner:
         if not self.use_graph:
             self._decode_body(Bp, self._splits_for(Bp), vp)
             return
-        self.graphs[(Bp, vp)].replay()
+        self.graphs[(Bp, vp, self._prefix)].replay()
         self.stats["graph_replays"] += 1
 
     @torch.no_grad()
@@ -582,7 +672,7 @@ class ModelRunner:
         B = len(self.batch_seqs)
         Bp = self._bucket(B)
         MB = self.max_batch
-        if self.use_graph and (Bp, self._vp_greedy()) not in self.graphs:
+        if self.use_graph and (Bp, self._vp_greedy(), self._prefix) not in self.graphs:
             self.capture(Bp, self._vp_greedy())
         self._fill_step_inputs()
         src = self._stage()

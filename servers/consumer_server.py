@@ -25,6 +25,10 @@ def get_args():
                                 help="prompts that start with the same tokens share the KV blocks of the common prefix")
     consumer_group.add_argument("--sliding_window", action="store_true",
                                 help="past max_seq_len, keep generating over the most recent tokens (rotary-position models)")
+    consumer_group.add_argument("--kv_cache_dtype", type=str, default=None, choices=["int8", "fp8"],
+                                help="keep the KV cache in 8 bits (models with multi-head keys and values)")
+    consumer_group.add_argument("--shared_prefix", action="store_true",
+                                help="with --prefix_cache: a step reads a prefix that several sequences share once for all of them")
     broker_group = parser.add_argument_group("broker")
     broker_group.add_argument("--redis_host", type=str, default="127.0.0.1")
     broker_group.add_argument("--redis_port", type=int, default=20000)
@@ -50,7 +54,8 @@ def main():
     engine = Engine.from_pretrained(args.pretrained_model_path, dtype=getattr(torch, args.dtype),
                                     process_group=process_group, max_batch=args.max_batch, max_seq_len=args.max_seq_len,
                                     sliding_window=args.sliding_window, prefix_cache=args.prefix_cache,
-                                    prefill_chunk=args.prefill_chunk)
+                                    prefill_chunk=args.prefill_chunk, kv_cache_dtype=args.kv_cache_dtype,
+                                    shared_prefix=args.shared_prefix)
     engine.comm.barrier()
     ConsumerLoop(engine, tokenizer, broker).run_forever()
 

@@ -433,3 +433,66 @@ def test_calls_that_are_refused():
         ops.rope_kv_write(qkv, pos, pos - 1, k, v, 4, 2, 64, 24, ops.ROPE_NEOX, 1e4, 0, 256, 384)
     with pytest.raises(KernelError, match="column ranges"):
         ops.rope_kv_write(qkv, pos, pos - 1, k, v, 4, 2, 64, 64, ops.ROPE_NEOX, 1e4, 0, 256, 392)
+
+
+# ----------------------------------------------------------------------------- the engine
+@pytest.mark.parametrize("family", ["gptj", "llama", "gpt_bigcode", "opt"])
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+def test_engine_on_8_bit_pages(tmp_path, family, kind):
+    """Logits of prompts and of steps over what they left, on the kernels and on the plain forms with the same pages' kind."""
+    from llmss_b200.engine.engine import Engine
+    from llmss_b200.engine.runner import SamplingParams
+    from tiny import make_tiny
+
+    make_tiny(family, tmp_path, hidden=256)
+    path = str(tmp_path)
+    g = torch.Generator().manual_seed(3)
+    prompts = [torch.randint(1, 128, (n,), generator=g).tolist() for n in (5, 44, 33, 1)]
+    kw = dict(max_batch=4, max_seq_len=64, kv_cache_dtype=kind)
+    gpu, cpu = Engine.from_pretrained(path, dtype=HF, device="cuda", **kw), Engine.from_pretrained(path, device="cpu", **kw)
+    for step in range(3):
+        toks = prompts if step == 0 else [[7 + step], [9], [11 + step], [2]]
+        a, b = (e.feed([(i, t, [len(t) - 1]) for i, t in enumerate(toks)]) for e in (gpu, cpu))
+        # activations in f16 against 32 bits: codes near a half step may fall to either side, a step of 1 / 127 or 1 / 16 of a value among dozens
+        assert (a.float().cpu() - b).abs().max() < (0.03 if kind == "int8" else 0.06) * b.abs().max()
+    sp = SamplingParams(max_new_tokens=10, is_greedy=True)
+    graph, eager = (Engine.from_pretrained(path, dtype=HF, device="cuda", use_cuda_graph=u, **kw) for u in (True, False))
+    assert graph.generate(prompts, sp) == eager.generate(prompts, sp) and graph.runner.stats["graph_replays"] > 0
+
+
+@pytest.mark.parametrize("kind", [None, "int8"])
+def test_engine_reads_a_shared_prefix_once(tmp_path, monkeypatch, kind):
+    from llmss_b200.engine import runner as R2
+    from llmss_b200.engine.batch import BatchInput
+    from llmss_b200.engine.engine import Engine
+    from llmss_b200.engine.runner import SamplingParams
+    from llmss_b200.utils.checkpoint import write_random_checkpoint
+
+    monkeypatch.setattr(R2, "_SHARE_MIN_BYTES", 0)
+    path = str(write_random_checkpoint(tmp_path, "gptj-tiny", dtype=torch.float32, device="cpu", std=0.08))
+    g = torch.Generator().manual_seed(4)
+    draw = lambda n: torch.randint(1, 400, (n,), generator=g).tolist()
+    a, b = draw(70), draw(40)
+    prompts = [a + draw(5), b + draw(3), draw(9), a + draw(11), b + draw(8), a + draw(1)]
+    eng = Engine.from_pretrained(path, dtype=HF, device="cuda", max_batch=8, max_seq_len=128, block_size=16, prefix_cache=True, shared_prefix=True,
+                                 kv_cache_dtype=kind)
+    eng.generate([a + [3], b + [4]], SamplingParams(max_new_tokens=2, is_greedy=True))
+    for p in prompts:
+        eng.add_request(p, SamplingParams(max_new_tokens=20, is_greedy=True))
+    for _ in range(4):
+        eng.step()
+    r = eng.runner
+    assert r._prefix is not None and r.stats["graph_replays"] >= 3
+    # the step's logits with and without the groups: the same numbers, up to roundings of 16-bit activations
+    r._fill_step_inputs()
+    r.d_in.copy_(r.h_in)
+    tok, pos, slot, slen, bt, _ = r._dev_views(8)
+    logits = []
+    for prefix in (None, r._step_prefix(8)):
+        batch = BatchInput(tokens=tok, positions=pos, slot_mapping=slot, block_tables=bt, seq_lens=slen, cu_q=r.d_cu[:9], last_idx=r.d_last_idx[:8], num_seqs=8,
+                           max_q=1, max_kv=r.max_seq_len, is_decode=True, is_fresh_prefill=False, prefix=prefix)
+        logits.append(r.core.forward(batch, r.kv, last_only=False)[:6].float())
+    assert (logits[0] - logits[1]).abs().max() < 0.01 * logits[0].abs().max()
+    while eng.has_work():
+        eng.step()
+    assert r.alloc.num_free == r.alloc.num_blocks - 1

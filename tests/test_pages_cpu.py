@@ -137,3 +137,120 @@ def test_merge_of_two_parts_is_the_softmax_over_both():
     w = [math.exp(p[0] - m) for p in parts]
     o = sum(a * p[2] for a, p in zip(w, parts)) / sum(a * p[1] for a, p in zip(w, parts))
     assert torch.allclose(o, torch.softmax(s, 0) @ v)
+
+
+# ----------------------------------------------------------------------------- the engine
+def _tiny(tmp_path, preset="gptj-tiny"):
+    from llmss_b200.utils.checkpoint import write_random_checkpoint
+
+    return str(write_random_checkpoint(tmp_path, preset, dtype=torch.float32, device="cpu", std=0.08))
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+def test_engine_on_8_bit_pages(tmp_path, kind):
+    from llmss_b200.engine.engine import Engine
+    from llmss_b200.engine.runner import SamplingParams
+
+    path = _tiny(tmp_path)
+    g = torch.Generator().manual_seed(2)
+    prompts = [torch.randint(1, 500, (n,), generator=g).tolist() for n in (5, 37, 20, 1)]
+    kw = dict(device="cpu", max_seq_len=128, block_size=16)
+    full, eng = Engine.from_pretrained(path, max_batch=4, **kw), Engine.from_pretrained(path, max_batch=4, kv_cache_dtype=kind, **kw)
+    assert eng.runner.kv.data.element_size() == 1
+    want, got = (e.feed([(i, p, range(len(p))) for i, p in enumerate(prompts)]) for e in (full, eng))
+    # what quantising keys and values does to the logits of this model: a few steps of the largest of a row
+    assert (got - want).abs().max() < (0.05 if kind == "int8" else 0.25) * want.abs().max() and not torch.equal(got, want)
+    # a prompt cut into portions reads the same pages: the same logits, up to the order of 32-bit sums
+    cut = Engine.from_pretrained(path, max_batch=4, kv_cache_dtype=kind, **kw)
+    parts = [cut.feed([(1, prompts[1][a:b], range(b - a))]) for a, b in ((0, 16), (16, 17), (17, 37))]
+    assert torch.allclose(torch.cat(parts), got[5:42], atol=1e-4)
+    eng2, chunked = (Engine.from_pretrained(path, max_batch=2, kv_cache_dtype=kind, prefill_chunk=c, **kw) for c in (None, 7))
+    sp = SamplingParams(max_new_tokens=8, is_greedy=True)
+    assert eng2.generate(prompts, sp) == chunked.generate(prompts, sp)
+    assert eng2.runner.alloc.num_free == eng2.runner.alloc.num_blocks - 1
+
+
+def test_engine_refuses_what_has_no_such_pages(tmp_path):
+    from llmss_b200.engine.engine import Engine
+
+    path = _tiny(tmp_path / "a")
+    with pytest.raises(ValueError, match="'fp8' or 'int8'"):
+        Engine.from_pretrained(path, device="cpu", max_batch=2, max_seq_len=64, kv_cache_dtype="int4")
+    with pytest.raises(ValueError, match="prefix_cache"):
+        Engine.from_pretrained(path, device="cpu", max_batch=2, max_seq_len=64, shared_prefix=True)
+    with pytest.raises(ValueError, match="sliding"):
+        Engine.from_pretrained(path, device="cpu", max_batch=2, max_seq_len=64, shared_prefix=True, prefix_cache=True, sliding_window=True)
+    native = _tiny(tmp_path / "b", "bedovik-tiny")
+    with pytest.raises(ValueError, match="kind of cache"):
+        Engine.from_pretrained(native, device="cpu", max_batch=2, max_seq_len=64, kv_cache_dtype="int8")
+
+
+def test_quant_cache_copies_blocks():
+    from llmss_b200.engine.kv_cache import QuantKVCache
+
+    a, b = (QuantKVCache(2, 4, 16, 2, 8, "fp8", "cpu") for _ in range(2))
+    a.data.view(torch.int8).random_(0, 100)
+    a.scale.uniform_()
+    b.copy_blocks_from(a, 1, 2, 2)
+    assert torch.equal(b.k(1).values()[2:4], a.k(1).values()[1:3]) and torch.equal(b.v(0).values()[2:4], a.v(0).values()[1:3])
+    assert not b.scale[:, :, :2].any()
+    assert QuantKVCache.bytes_per_block(2, 16, 2, 8) == 2 * 2 * 16 * 2 * 12
+
+
+@pytest.mark.parametrize("kind", [None, "int8"])
+def test_engine_reads_a_shared_prefix_once(tmp_path, monkeypatch, kind):
+    """Two system prompts and a request of its own, decoded together: the tokens of an engine without sharing, and the groups that the step had."""
+    from llmss_b200.engine import runner as R2
+    from llmss_b200.engine.engine import Engine
+    from llmss_b200.engine.runner import SamplingParams
+
+    monkeypatch.setattr(R2, "_SHARE_MIN_BYTES", 0)
+    path = _tiny(tmp_path)
+    g = torch.Generator().manual_seed(4)
+    draw = lambda n: torch.randint(1, 500, (n,), generator=g).tolist()
+    a, b = draw(40), draw(20)
+    prompts = [a + draw(5), b + draw(3), draw(9), a + draw(11), b + draw(8), a + draw(1)]
+    sp = [SamplingParams(max_new_tokens=n, is_greedy=True) for n in (9, 12, 7, 4, 12, 10)]
+    kw = dict(device="cpu", max_batch=6, max_seq_len=128, block_size=16, prefix_cache=True, kv_cache_dtype=kind)
+    plain, eng = Engine.from_pretrained(path, **kw), Engine.from_pretrained(path, shared_prefix=True, **kw)
+    seen = []
+    bind = eng.runner._bind_prefix
+
+    def watch(seqs):
+        bind(seqs)
+        seen.append(eng.runner.prefix_groups(seqs))
+
+    eng.runner._bind_prefix = watch
+    for e in (plain, eng):                      # a first wave registers the prefixes
+        e.generate([a + [3], b + [4]], SamplingParams(max_new_tokens=2, is_greedy=True))
+    assert eng.generate(prompts, sp) == plain.generate(prompts, sp)
+    sizes = [sorted((n, len(c)) for _, n, c in s) for s in seen]
+    assert [(2, 1), (3, 2)] in sizes            # b's one block for two, a's two blocks for three
+    assert eng.runner._prefix is None or eng.runner._prefix[0] >= 1
+    assert eng.runner.alloc.num_free == eng.runner.alloc.num_blocks - 1
+
+
+def test_groups_and_the_rows_between_them(tmp_path, monkeypatch):
+    from types import SimpleNamespace
+
+    from llmss_b200.engine import runner as R2
+    from llmss_b200.engine.engine import Engine
+
+    monkeypatch.setattr(R2, "_SHARE_MIN_BYTES", 0)
+    r = Engine.from_pretrained(_tiny(tmp_path), device="cpu", max_batch=40, max_seq_len=128, block_size=16, prefix_cache=True, shared_prefix=True).runner
+    seq = lambda blocks, length: SimpleNamespace(blocks=blocks, length=length)
+    seqs = [seq([9, 1], 20), seq([2, 3, 4], 40), seq([2, 3, 5], 40), seq([7], 16), seq([8, 6], 17), seq([8, 10], 17), seq([11], 3)]
+    assert r.prefix_groups(seqs) == [(1, 2, [2, 3]), (4, 2, [8])]
+    r._bind_prefix(seqs)
+    p = r._step_prefix(8)
+    assert p.num_groups == 4 and p.first[:5].tolist() == [1, 3, 4, 6, 6] and p.lens[:4].tolist() == [32, 0, 16, 0]
+    assert p.block_tables[0, :2].tolist() == [2, 3] and p.block_tables[2, 0] == 8 and p.max_len == 32
+    # a block that is not full yet is nobody else's
+    assert r.prefix_groups([seq([2], 15), seq([2], 15)]) == []
+    # more groups than a step takes: those that save most, still in order
+    many = [seq([100 + i // 2, 200 + i], 20) for i in range(24)]
+    assert [f for f, _, _ in r.prefix_groups(many)] == list(range(0, 16, 2))
+    monkeypatch.setattr(R2, "_SHARE_MIN_BYTES", 1 << 30)
+    assert r.prefix_groups(seqs) == []
+    r._bind_prefix(seqs)
+    assert r._step_prefix(8) is None
