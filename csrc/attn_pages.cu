@@ -237,32 +237,49 @@ int launch_merge(const AttnArgs& a, const PartArgs& p, int parts, cudaStream_t s
 }
 
 // ---------------------------------------------------------------------------------------------------------------- codes as 16-bit pages
-// 64 keys of one sequence and key head: code * scale in the queries' type, [sequence][head][pad][d] of keys, then of values; a page per sequence, so that the
-// table names itself.  Bound by memory: 1 byte read, 2 written per value.
-template <typename T, int FMT>
-__global__ void __launch_bounds__(256) attn_pages_expand_kernel(const __grid_constant__ AttnArgs a, T* __restrict__ out, int* __restrict__ table, int pad) {
+// 64 keys of one sequence and key head as f16 (TileScales), [sequence][head][pad][d] of keys, then of values; a page per sequence, so that the table names
+// itself.  Bound by memory: 1 byte read, 2 written per value.
+template <int FMT>
+__global__ void __launch_bounds__(256) attn_pages_expand_kernel(const __grid_constant__ AttnArgs a, __half* __restrict__ out, TileScales* __restrict__ scales,
+                                                                int* __restrict__ table, int pad) {
   pdl_launch_dependents();
   pdl_wait();
+  __shared__ float s_scale[2][64];
+  __shared__ int s_exp[2];
   const int s = blockIdx.z, kvh = blockIdx.y, key0 = blockIdx.x * 64;
   if (blockIdx.x == 0 && kvh == 0 && threadIdx.x == 0) table[s] = s;
   const int len = min(min(a.seq_lens[s], a.max_blocks * a.page), pad);
-  if (key0 >= len) return;
+  if (key0 >= len) return;                 // the tiled kernel looks at no tile without a key
   const int per = a.d / 16;
-  const int64_t plane = (int64_t)a.num_seqs * a.hkv * pad * a.d;
+  const int64_t list = ((int64_t)s * a.hkv + kvh) * pad, plane = (int64_t)a.num_seqs * a.hkv * pad;
+  auto cache_row = [&](int key) {
+    return ((int64_t)checked_block(a.tables[(int64_t)s * a.max_blocks + key / a.page], a.num_blocks) * a.hkv + kvh) * a.page + key % a.page;
+  };
+  if (threadIdx.x < 128) {
+    const int value = threadIdx.x >> 6, key = key0 + (threadIdx.x & 63);
+    s_scale[value][threadIdx.x & 63] = key < len ? (value ? a.vs : a.ks)[cache_row(key)] : 0.f;
+  }
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    const int value = threadIdx.x >> 5, lane = threadIdx.x & 31, e = tile_exponent(s_scale[value][lane], s_scale[value][lane + 32]);
+    if (lane == 0) s_exp[value] = e;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) scales[((int64_t)s * a.hkv + kvh) * (pad / 64) + blockIdx.x] = tile_scales(s_exp[0], s_exp[1]);
+  const float down[2] = {two_to(-s_exp[0]), two_to(-s_exp[1])};
 #pragma unroll 4
   for (int x = threadIdx.x; x < 2 * 64 * per; x += 256) {
     const int value = x >= 64 * per, y = value ? x - 64 * per : x;
-    const int key = key0 + y / per, c = (y % per) * 16;
+    const int at = y / per, key = key0 + at, c = (y % per) * 16;
     if (key >= len) continue;
-    const int64_t row = ((int64_t)checked_block(a.tables[(int64_t)s * a.max_blocks + key / a.page], a.num_blocks) * a.hkv + kvh) * a.page + key % a.page;
-    const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(value ? a.v : a.k) + row * a.d + c);
-    const float scale = (value ? a.vs : a.ks)[row];
+    const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(value ? a.v : a.k) + cache_row(key) * a.d + c);
+    const float scale = s_scale[value][at] * (value ? down[1] : down[0]);
     uint4 lo, hi;
-    convert4<T, FMT>(w.x, scale, lo.x, lo.y);
-    convert4<T, FMT>(w.y, scale, lo.z, lo.w);
-    convert4<T, FMT>(w.z, scale, hi.x, hi.y);
-    convert4<T, FMT>(w.w, scale, hi.z, hi.w);
-    T* to = out + value * plane + (((int64_t)s * a.hkv + kvh) * pad + key) * a.d + c;
+    convert4<FMT>(w.x, scale, lo.x, lo.y);
+    convert4<FMT>(w.y, scale, lo.z, lo.w);
+    convert4<FMT>(w.z, scale, hi.x, hi.y);
+    convert4<FMT>(w.w, scale, hi.z, hi.w);
+    __half* to = out + (value * plane + list + key) * a.d + c;
     *reinterpret_cast<uint4*>(to) = lo;
     *reinterpret_cast<uint4*>(to + 8) = hi;
   }
@@ -326,7 +343,7 @@ Plan plan_call(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv
     // Every row tile converts all codes for itself, which takes the tiled kernel from 1100 to 2000 clocks per 64 keys; once for all costs a pass over the
     // cache (about 1200 clocks of an SM per 64 keys, and a launch).  Portions of 1000 tokens over 1800, 16 tiles: 240 -> 150 us; from three tiles on.  Up to
     // 1 GB of scratch
-    const int64_t pad = ((int64_t)max_kv + 63) / 64 * 64, expanded = (int64_t)num_seqs * hkv * pad * d + (num_seqs + 3) / 4 * 4;
+    const int64_t pad = ((int64_t)max_kv + 63) / 64 * 64, expanded = (int64_t)num_seqs * hkv * (pad * d + pad / 64 * 4) + (num_seqs + 3) / 4 * 4;
     if (fmt != kF16Pages && groups == 0 && p.tile.own_tiles >= 3 && expanded <= (1ll << 28) && pad <= (1 << 19)) {
       p.pad = (int)pad;
       p.expanded = expanded;
@@ -443,24 +460,22 @@ LLMSS_API int llmss_attn_pages(const void* q, int64_t ldq, const void* k_pages, 
     float* expanded = take(plan.expanded);
     if (plan.pad > 0) {
       // from here on the cache is the 16-bit copy, one page per sequence
-      int* table = (int*)(expanded + (int64_t)num_seqs * hkv * plan.pad * d);
+      const int64_t plane = (int64_t)num_seqs * hkv * plan.pad;
+      TileScales* scales = (TileScales*)(expanded + plane * d);
+      int* table = (int*)(scales + plane / 64);
       const dim3 grid(plan.pad / 64, hkv, num_seqs);
       LLMSS_REQUIRE(grid.y <= 65535 && grid.z <= 65535, "attn_pages: grid too large (%d key heads, %d sequences)", hkv, num_seqs);
-#define LLMSS_EXPAND(T_)                                                                                                                                     \
-  LLMSS_CHECK_CUDA(fmt == kInt8 ? launch_pdl(attn_pages_expand_kernel<T_, kInt8>, grid, dim3(256), 0, stream, a, (T_*)expanded, table, plan.pad)             \
-                                : launch_pdl(attn_pages_expand_kernel<T_, kE4M3>, grid, dim3(256), 0, stream, a, (T_*)expanded, table, plan.pad))
-      if (dtype == LLMSS_F16) LLMSS_EXPAND(__half);
-      else LLMSS_EXPAND(__nv_bfloat16);
-#undef LLMSS_EXPAND
+      LLMSS_CHECK_CUDA(fmt == kInt8 ? launch_pdl(attn_pages_expand_kernel<kInt8>, grid, dim3(256), 0, stream, a, (__half*)expanded, scales, table, plan.pad)
+                                    : launch_pdl(attn_pages_expand_kernel<kE4M3>, grid, dim3(256), 0, stream, a, (__half*)expanded, scales, table, plan.pad));
       ++*launches;
       a.k = expanded;
-      a.v = (const uint16_t*)expanded + (int64_t)num_seqs * hkv * plan.pad * d;
-      a.ks = a.vs = nullptr;
+      a.v = (const uint16_t*)expanded + plane * d;
+      a.tile_scales = scales;
       a.tables = table;
       a.max_blocks = 1;
       a.page = plan.pad;
       a.num_blocks = num_seqs;
-      fmt = kF16Pages;
+      fmt = kScaled16;
     }
     if (tiles) {
       if (int e = tile_launch(a, p, plan.tile, fmt, dtype, stream)) return e;

@@ -15,6 +15,7 @@
 namespace pages {
 
 constexpr int kF16Pages = 0, kInt8 = 1, kE4M3 = 2;    // page formats; 0: the queries' own 16-bit type
+constexpr int kScaled16 = 3;                          // inside: 8-bit pages as f16 with an exponent per 64 keys (TileScales)
 
 struct AttnArgs {
   const void* q;
@@ -22,6 +23,7 @@ struct AttnArgs {
   const void* v;
   const float* ks;
   const float* vs;
+  const struct TileScales* tile_scales;   // kScaled16: [sequence][hkv][page / 64]
   void* out;
   const int* tables;        // [num_seqs][max_blocks]
   const int* seq_lens;
@@ -147,8 +149,29 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
   }
 }
 
-// four codes -> code * scale in the 16-bit type, two words
-template <typename T, int FMT>
+// Tiles of 64 keys in f16: code * scale / 2^E, E the exponent above the tile's largest scale, so that nothing leaves f16's range and a rounding is 2^-12 of
+// the number (2^-25 of the tile's largest scale at least).  What goes with a tile: 2^E of the keys, E and 2^-E of the values.
+struct TileScales {
+  float k_up, v_exp, v_down, pad;
+};
+// E from two scales per lane (0 where the list has no key); scales that are not finite do not count, they make their own NaN
+__device__ __forceinline__ int tile_exponent(float a, float b) {
+  const unsigned x = __float_as_uint(a), y = __float_as_uint(b);
+  const unsigned top = __reduce_max_sync(0xffffffffu, max(x < 0x7f800000u ? x : 0u, y < 0x7f800000u ? y : 0u));
+  return max(-60, min(100, (int)(top >> 23) - 126));
+}
+__device__ __forceinline__ float two_to(int e) { return __int_as_float((127 + e) << 23); }
+__device__ __forceinline__ TileScales tile_scales(int ek, int ev) {
+  TileScales t;
+  t.k_up = two_to(ek);
+  t.v_exp = (float)ev;
+  t.v_down = two_to(-ev);
+  t.pad = 0.f;
+  return t;
+}
+
+// four codes -> code * scale in f16, two words
+template <int FMT>
 __device__ __forceinline__ void convert4(uint32_t w, float scale, uint32_t& lo, uint32_t& hi) {
   float f[4];
   if constexpr (FMT == kInt8) {
@@ -170,8 +193,8 @@ __device__ __forceinline__ void convert4(uint32_t w, float scale, uint32_t& lo, 
   }
   fmul2(f[0], f[1], f[0], f[1], scale, scale);
   fmul2(f[2], f[3], f[2], f[3], scale, scale);
-  lo = pack16<T>(f[0], f[1]);
-  hi = pack16<T>(f[2], f[3]);
+  lo = pack16<__half>(f[0], f[1]);
+  hi = pack16<__half>(f[2], f[3]);
 }
 
 __device__ __forceinline__ void bulk_copy(void* dst, const void* src, int bytes, uint64_t* bar) {   // addresses and size multiples of 16

@@ -11,9 +11,11 @@
 //                   issue beside the other warps, so that one warp for 256 rows took 2100 clocks a tile where the products take 1100)
 //   softmax warps   a thread per row: its S row from tensor memory, mask, running maximum (moved when exceeded by 2^8) and sum in 32 bits, P back
 //
-// 8-bit codes are converted once per block for all its rows: code * scale is rounded to the queries' type, which is a rounding of the same size as a
-// 16-bit cache has, and well below the code's own step; with the scales multiplied to the scores instead, every row would pay for them.  Prompts of many
-// row tiles have their codes converted once for all blocks (attn_pages.cu) and come here as 16-bit pages.
+// 8-bit codes are converted once per block for all its rows, to f16 whatever the queries' type (code * scale rounded to bf16 is off by as much as the whole
+// rest of the arithmetic: 4e-3 of a result instead of 1.8e-3; scales multiplied to scores and probabilities instead cost 100 instructions per row and tile,
+// a fifth of the speed).  A power of two per tile keeps them in range (TileScales): that of the keys joins the scores' factor, that of the values the
+// exponent of the probabilities, which stand relative to the largest one so far.  bf16 queries become f16 after division by the power of two below their
+// row's largest value.  Prompts of many row tiles have their codes converted once for all blocks (attn_pages.cu) and come here as 16-bit pages.
 //
 // A list whose rows are few is cut into stretches of keys (grid x), whose parts the merge kernel joins.
 #include "attn_pages.cuh"
@@ -29,15 +31,19 @@ template <int FMT, int D, int NQ>
 struct Tile {
   static constexpr int SOFT = 4 * NQ;                                   // softmax warps
   // 8-bit: four warps would convert a tile in twice the time that the products take
-  static constexpr int CONVERT = FMT == kF16Pages ? 0 : 8;
+  static constexpr bool BYTES = FMT == kInt8 || FMT == kE4M3, SCALED = FMT != kF16Pages;
+  static constexpr int CONVERT = !BYTES ? 0 : NQ == 2 ? 4 : 8;
   static constexpr int COPY = SOFT + NQ;                                // first copying warp
   static constexpr int THREADS = 32 * (COPY + 2 + CONVERT);
   static constexpr int Q_BYTES = NQ * BM * D * 2;
   static constexpr int SLOT = BN * D * 2;                               // a tile of keys or values
-  static constexpr int SLOTS = D == 256 ? (FMT == kF16Pages ? 4 : 3) : 6;
-  static constexpr int RAW = FMT == kF16Pages ? 0 : BN * D + BN * 4;    // codes, then scales
-  static constexpr int RAWS = FMT == kF16Pages ? 0 : D == 256 ? 3 : 4;
-  static constexpr int SMEM = 1024 + Q_BYTES + SLOTS * SLOT + RAWS * RAW + 512;
+  static constexpr int SLOTS = D == 256 ? (BYTES ? 3 : 4) : 6;
+  static constexpr int RAW = BYTES ? BN * D : 0;                        // a tile of codes
+  static constexpr int RAWS = BYTES ? (D == 256 ? 3 : 4) : 0;
+  // scales of the last eight tiles, keys' and values', and what goes with a tile: keys of tile j + 8 come after the softmax of tile j, whatever the rings'
+  // depths here
+  static constexpr int SCALES = (BYTES ? 8 * 2 * BN * 4 : 0) + (SCALED ? 8 * 16 : 0);
+  static constexpr int SMEM = 1024 + Q_BYTES + SLOTS * SLOT + RAWS * RAW + SCALES + 512;
   static_assert(SOFT * 32 * (D * 4 + 16) <= Q_BYTES + SLOTS * SLOT, "outputs are staged where queries, keys and values were");
   static constexpr int TMEM = NQ * (2 * BN + D) <= 256 ? 256 : 512;
 };
@@ -105,13 +111,16 @@ template <typename T, int FMT, int D, int NQ>
 __global__ void __launch_bounds__(Tile<FMT, D, NQ>::THREADS, 1)
 attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnArgs a, const __grid_constant__ PartArgs pa, const TileArgs ta) {
   using C = Tile<FMT, D, NQ>;
+  using M = typename std::conditional<C::SCALED, __half, T>::type;   // type of the products
   constexpr int DSUB = D / 64;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* s_q = smem;                                   // [NQ][DSUB][128 rows][128 bytes]
   uint8_t* s_kv = s_q + C::Q_BYTES;                      // [SLOTS][DSUB][64 keys][128 bytes]
-  uint8_t* s_raw = s_kv + C::SLOTS * C::SLOT;            // [RAWS][64 keys of codes | 64 scales]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(s_raw + C::RAWS * C::RAW);
+  uint8_t* s_raw = s_kv + C::SLOTS * C::SLOT;            // [RAWS][64 keys of codes]
+  float* s_scale = reinterpret_cast<float*>(s_raw + C::RAWS * C::RAW);   // [8 tiles][keys', values'][64] (8-bit)
+  TileScales* s_tile = reinterpret_cast<TileScales*>(s_raw + C::RAWS * C::RAW + C::SCALES) - 8;   // [8 tiles]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_raw + C::RAWS * C::RAW + C::SCALES);
   uint64_t* bar_full = bars;                             // [SLOTS]
   uint64_t* bar_empty = bars + C::SLOTS;
   uint64_t* bar_s = bars + 2 * C::SLOTS;                 // [NQ][2] S ready
@@ -126,7 +135,7 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   // by a shuffle: numbers that the compiler knows to be the same in all lanes need no copies into uniform registers at every product
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   pdl_launch_dependents();
-  if (FMT == kF16Pages && threadIdx.x == 32 * C::COPY) {
+  if (!C::BYTES && threadIdx.x == 32 * C::COPY) {
     tma_prefetch_desc(&map_k);
     tma_prefetch_desc(&map_v);
   }
@@ -163,7 +172,7 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   if (warp == C::COPY || warp == C::COPY + 1) run_rows = look_up(0);
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::SLOTS; ++i) {
-      mbar_init(&bar_full[i], FMT == kF16Pages ? 1 : C::CONVERT);
+      mbar_init(&bar_full[i], C::BYTES ? C::CONVERT : 1);
       mbar_init(&bar_empty[i], NQ);
     }
     for (int i = 0; i < 2 * NQ; ++i) {
@@ -202,13 +211,22 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     auto copy = [&](int j, bool value, uint32_t rows, int from, int place) {
       const int first = base + j * BN;
       const int here = min(runs, (k_hi - first + run - 1) / run);       // runs that lie in the list
-      if constexpr (FMT == kF16Pages) {
+      // scales of both sides come with the keys: the softmax looks at them before the values are there
+      auto scales = [&](uint64_t* bar, uint32_t row, int x) {
+        float* to = s_scale + (j & 7) * (2 * BN) + x * run;
+        bulk_copy(to, a.ks + row, run * 4, bar);
+        bulk_copy(to + BN, a.vs + row, run * 4, bar);
+      };
+      if constexpr (!C::BYTES) {
         const int slot = place % C::SLOTS;
         mbar_wait(&bar_empty[slot], ((place / C::SLOTS) & 1) ^ 1, 80);     // a slot's first use waits for nobody
         const bool part = value && (first < s.lo || first + BN > k_hi);
         uint64_t* bar = part ? bar_part : &bar_full[slot];
         uint8_t* dst = s_kv + slot * C::SLOT;
-        if (elect_one()) mbar_arrive_expect_tx(bar, here * run * D * 2);
+        if (elect_one()) {
+          mbar_arrive_expect_tx(bar, here * run * D * 2 + (C::SCALED && !value ? 16 : 0));
+          if (C::SCALED && !value) bulk_copy(&s_tile[j & 7], a.tile_scales + ((int64_t)blockIdx.z * a.hkv + kvh) * (a.page / BN) + first / BN, 16, bar);
+        }
         for (int x = 0; x < here; ++x) {
           const int row = (int)__shfl_sync(0xffffffffu, rows, from + x);
           if (elect_one()) {
@@ -234,13 +252,12 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         mbar_wait(&bar_used[slot], ((place / C::RAWS) & 1) ^ 1, 80);
         uint8_t* dst = s_raw + slot * C::RAW;
         const uint8_t* src = reinterpret_cast<const uint8_t*>(value ? a.v : a.k);
-        const float* sc = value ? a.vs : a.ks;
-        if (elect_one()) mbar_arrive_expect_tx(&bar_raw[slot], here * run * (D + 4));
+        if (elect_one()) mbar_arrive_expect_tx(&bar_raw[slot], here * run * (D + (value ? 0 : 8)));
         for (int x = 0; x < here; ++x) {
           const uint32_t row = __shfl_sync(0xffffffffu, rows, from + x);
           if (elect_one()) {
             bulk_copy(dst + x * run * D, src + (uint64_t)row * D, run * D, &bar_raw[slot]);
-            bulk_copy(dst + BN * D + x * run * 4, sc + row, run * 4, &bar_raw[slot]);
+            if (!value) scales(&bar_raw[slot], row, x);
           }
         }
         __syncwarp();
@@ -253,7 +270,7 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     }
   } else if (warp > C::COPY + 1) {
     // ===================== converting warps
-    if constexpr (FMT != kF16Pages) {
+    if constexpr (C::BYTES) {
       const int tid = threadIdx.x - 32 * (C::COPY + 2);
       constexpr int PER = D / 16, KEYS = 32 * C::CONVERT / PER;      // 16-byte chunks of a key, keys between a thread's chunks
       constexpr int CH = BN / KEYS;                                // a thread's chunks of a tile
@@ -264,22 +281,30 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       static_assert(KEYS % 8 == 0, "every eighth key has the same place in the swizzle");
       int slot = 0, raw_slot = 0;
       uint32_t phase = 1, raw_phase = 0;
-      auto convert = [&](int j) {
+      auto convert = [&](int j, bool value) {
         const int first = base + j * BN;
         const bool all = first >= s.lo && first + BN <= k_hi;
         const uint8_t* raw = s_raw + raw_slot * C::RAW;
         mbar_wait(&bar_raw[raw_slot], raw_phase, 77);
         uint4 w[CH];
         float scale[CH];
+        float* sc = s_scale + (j & 7) * (2 * BN);
+        // every warp finds the tile's exponents for itself
+        auto inside = [&](int key) { return all || (first + key >= s.lo && first + key < k_hi); };
+        auto exponent = [&](const float* x) { return tile_exponent(inside(lane) ? x[lane] : 0.f, inside(lane + 32) ? x[lane + 32] : 0.f); };
+        const int ev = exponent(sc + BN);
+        int e = ev;
+        if (!value) {
+          e = exponent(sc);
+          if (tid == 0) s_tile[j & 7] = tile_scales(e, ev);
+        }
+        const float down = two_to(-e);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
           const int key = key0 + c * KEYS;
           w[c] = *reinterpret_cast<const uint4*>(raw + key * D + ch * 16);
-          scale[c] = *reinterpret_cast<const float*>(raw + BN * D + key * 4);
-          if (!all && (first + key < s.lo || first + key >= k_hi)) {   // zeros where the list does not reach
-            w[c] = make_uint4(0u, 0u, 0u, 0u);
-            scale[c] = 0.f;
-          }
+          scale[c] = sc[(value ? BN : 0) + key] * down;
+          if (!inside(key)) w[c] = make_uint4(0u, 0u, 0u, 0u), scale[c] = 0.f;   // zeros where the list does not reach
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar_used[raw_slot]);
@@ -289,10 +314,10 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
           uint4 y[2];
-          convert4<T, FMT>(w[c].x, scale[c], y[0].x, y[0].y);
-          convert4<T, FMT>(w[c].y, scale[c], y[0].z, y[0].w);
-          convert4<T, FMT>(w[c].z, scale[c], y[1].x, y[1].y);
-          convert4<T, FMT>(w[c].w, scale[c], y[1].z, y[1].w);
+          convert4<FMT>(w[c].x, scale[c], y[0].x, y[0].y);
+          convert4<FMT>(w[c].y, scale[c], y[0].z, y[0].w);
+          convert4<FMT>(w[c].z, scale[c], y[1].x, y[1].y);
+          convert4<FMT>(w[c].w, scale[c], y[1].z, y[1].w);
           uint8_t* at = dst + c * (KEYS * 128);
           *reinterpret_cast<uint4*>(at + c0) = flip ? y[1] : y[0];
           *reinterpret_cast<uint4*>(at + (c0 ^ 16)) = flip ? y[0] : y[1];
@@ -303,14 +328,14 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         if (++slot == C::SLOTS) slot = 0, phase ^= 1;
       };
       for (int j = 0; j <= n_tiles; ++j) {
-        if (j < n_tiles) convert(j);
-        if (j > 0) convert(j - 1);
+        if (j < n_tiles) convert(j, false);
+        if (j > 0) convert(j - 1, true);
       }
     }
   } else if (warp >= C::SOFT) {
     // ===================== issuing warps: all of one runs its loop, one lane issues
     const int q = warp - C::SOFT;
-    const int fmt = std::is_same<T, __half>::value ? 0 : 1;
+    const int fmt = std::is_same<M, __half>::value ? 0 : 1;
     const uint32_t id_s = idesc(fmt, BN, 0), id_o = idesc(fmt, D, 1);
     const uint32_t ql = desc_lo(smem_u32(s_q)) + q * (BM * D * 2 / 16), k_lo = desc_lo(smem_u32(s_kv)), v_lo = desc_lo(smem_u32(s_kv), BN * 128);
     const uint32_t ts = t_s(q, 0), to = t_o(q);
@@ -364,18 +389,36 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     const int tok = s.row0 + n / group;
     const int head = kvh * group + n % group;
     // this warp's 32 rows of queries into their swizzled tile; rows beyond the last are zeros
+    float scale = a.scale_log2;
     if (n_tiles > 0) {
-      const uint32_t dst = smem_u32(s_q + q * (BM * D * 2));
+      uint8_t* dst = s_q + q * (BM * D * 2);
       const int64_t at = live ? (int64_t)tok * a.ldq + (int64_t)head * D : -1;
-      constexpr int STEP = 32 / (D / 8 < 32 ? D / 8 : 32);         // rows of one copy of the warp
-      const int ch = lane % (32 / STEP);
+      constexpr int LANES = D / 8 < 32 ? D / 8 : 32, STEP = 32 / LANES;    // lanes of a row, rows of one copy of the warp
+      const int ch = lane % LANES;
 #pragma unroll 4
       for (int i = 0; i < 32; i += STEP) {
-        const int row = i + lane / (32 / STEP);
+        const int row = i + lane / LANES;
         const int64_t from = __shfl_sync(0xffffffffu, at, row);
         const int rt = quarter * 32 + row;
-        copy16(dst + (ch >> 3) * (BM * 128) + rt * 128 + (((ch & 7) ^ (rt & 7)) << 4), reinterpret_cast<const T*>(a.q) + (from < 0 ? 0 : from + ch * 8),
-               from < 0 ? 0 : 16);
+        uint8_t* to = dst + (ch >> 3) * (BM * 128) + rt * 128 + (((ch & 7) ^ (rt & 7)) << 4);
+        const T* src = reinterpret_cast<const T*>(a.q) + (from < 0 ? 0 : from + ch * 8);
+        if constexpr (std::is_same<M, T>::value) {
+          copy16(smem_u32(to), src, from < 0 ? 0 : 16);
+        } else {
+          float x[8], mx = 0.f;
+          unpack8<T>(from < 0 ? make_uint4(0u, 0u, 0u, 0u) : *reinterpret_cast<const uint4*>(src), x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
+#pragma unroll
+          for (int o = LANES / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+          const int e = mx > 0.f && mx < INFINITY ? max(-126, min(126, (int)((__float_as_uint(mx) >> 23) & 255) - 127)) : 0;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) x[k] *= two_to(-e);
+          *reinterpret_cast<uint4*>(to) = pack8<__half>(x);
+          // the row's factor goes to its own thread
+          const float up_q = __shfl_sync(0xffffffffu, two_to(e), (lane % STEP) * LANES);
+          if (lane / STEP == i / STEP) scale *= up_q;
+        }
       }
       copies_commit();
     }
@@ -391,10 +434,11 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar_q[q]);
     }
-    const float scale = a.scale_log2;
     // f16 ends at 2^16 and has no numbers below 2^-24: probabilities are formed times 2^7 (at most 2^15), so that those down to 2^-21 keep all bits
-    constexpr float kUp = std::is_same<T, __half>::value ? 7.0f : 0.0f;
+    constexpr float kUp = std::is_same<M, __half>::value ? 7.0f : 0.0f;
     float m_run = -INFINITY, l_run = 0.f;
+    // sums are of probabilities times 2^up: with scales, less the exponent of the values' largest so far
+    float up = C::SCALED ? INFINITY : kUp;
     bool bad = false;                                     // a score of the row is NaN: so is the result, whatever the exponentials made of it
     for (int j = 0; j < n_tiles; ++j) {
       const int b = j & 1, kb = base + j * BN;
@@ -411,6 +455,12 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll
           for (int i = 0; i < 32; ++i) sc[c * 32 + i] = __uint_as_float(r[c][i]);
       }
+      TileScales ts = {1.f, 0.f, 1.f, 0.f};
+      float s_scl = scale;
+      if constexpr (C::SCALED) {
+        ts = s_tile[j & 7];
+        s_scl = scale * ts.k_up;
+      }
       const int hi = pos - kb, lo = k_lo - kb;
       if (__any_sync(0xffffffffu, hi < BN - 1 || lo > 0)) {
 #pragma unroll
@@ -423,13 +473,16 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll
         for (int u = 0; u < 4; ++u) mx[u] = max_nan(mx[u], max_nan(sc[i + 2 * u], sc[i + 2 * u + 1]));
       }
-      const float m_tile = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * scale;
+      const float m_tile = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * s_scl;
       bad = bad || m_tile != m_tile;
       const bool grow = m_tile > m_run + 8.0f;
       const float m_new = grow ? m_tile : m_run;
-      const float alpha = grow && j > 0 ? exp2_fast(m_run - m_new) : 1.0f;
+      float up_new = up;
+      if constexpr (C::SCALED) up_new = fminf(up, kUp - ts.v_exp);
+      const float alpha = j > 0 && m_new > -INFINITY && (grow || up_new != up) ? exp2_fast((m_run - m_new) + (up_new - up)) : 1.0f;
       m_run = m_new;
-      const float neg = m_new == -INFINITY ? 0.f : kUp - m_new;
+      up = up_new;
+      const float neg = m_new == -INFINITY ? 0.f : (C::SCALED ? up + ts.v_exp : up) - m_new;
       float la[4] = {0.f, 0.f, 0.f, 0.f}, lb[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < BN / 32; ++c) {
@@ -437,12 +490,12 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
           float e0, e1;
-          ffma2(e0, e1, sc[c * 32 + i], sc[c * 32 + i + 1], scale, scale, neg, neg);
-          // every fourth exponential on the FMA pipe: the MUFU pipe alone would need as many clocks as a tile's products.  Not beside converting warps, where
-          // instructions are what is short
-          const float p0 = exp2_fast(e0), p1 = FMT != kF16Pages || (i & 2) ? exp2_fast(e1) : exp2_fma(e1);
+          ffma2(e0, e1, sc[c * 32 + i], sc[c * 32 + i + 1], s_scl, s_scl, neg, neg);
+          // every fourth exponential on the FMA pipe: the MUFU pipe alone would need as many clocks as a tile's products.  Not where warps
+          // convert: there instructions are what is short
+          const float p0 = exp2_fast(e0), p1 = C::BYTES || (i & 2) ? exp2_fast(e1) : exp2_fma(e1);
           fadd2(la[(i >> 1) & 3], lb[(i >> 1) & 3], la[(i >> 1) & 3], lb[(i >> 1) & 3], p0, p1);
-          pk[i >> 1] = pack16<T>(p0, p1);
+          pk[i >> 1] = pack16<M>(p0, p1);
         }
         tmem_st_x16(t_s(q, b) + off + c * 16, pk);
       }
@@ -462,7 +515,7 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         }
         tmem_st_done();
       }
-      l_run = l_run * alpha + l_tile;
+      l_run = l_run * alpha + (C::SCALED ? l_tile * ts.v_down : l_tile);
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar_p[q * 2 + b]);
@@ -474,10 +527,8 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     // every product has been formed, so queries, keys and values make room: rows go through shared memory, each lane's in a place of its own (a row is
     // 16 bytes longer than a multiple of 128, so that eight lanes never meet in a bank), and from there by the whole warp (a lane's 16 bytes to a row of its
     // own are 32 transactions per instruction: 9600 clocks for 256 rows of 132 numbers; a bulk copy per row: 6400)
-    if constexpr (NQ > 1) {
-      // the other tile's products read keys and values too
-      mbar_wait(&bar_o[(q ^ 1) * 2 + ((n_tiles - 1) & 1)], n_tiles > 0 ? ((n_tiles - 1) >> 1) & 1 : 1, 88);
-    }
+    // the other tile's products read keys and values too; its barriers' phases may lie behind by more than one, so that its own warps have to say it
+    if constexpr (NQ > 1) asm volatile("bar.sync 1, %0;" ::"n"(32 * C::SOFT) : "memory");
     if (bad) l_run = __int_as_float(0x7fc00000);
     // no visible key: zero
     const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
@@ -513,7 +564,7 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         to = reinterpret_cast<uint8_t*>(reinterpret_cast<T*>(a.out) + (int64_t)tok * a.ldo + (int64_t)head * D);
       } else {
         float* part = (is_own ? pa.tile_own : pa.tile_group) + (((int64_t)split * a.total_q + tok) * a.hq + head) * (D + kPad);
-        *reinterpret_cast<float2*>(part + D) = make_float2(m_run - kUp, l_run);
+        *reinterpret_cast<float2*>(part + D) = make_float2(m_run - (up < INFINITY ? up : 0.f), l_run);
         to = reinterpret_cast<uint8_t*>(part);
       }
     }
@@ -566,7 +617,7 @@ int launch(const AttnArgs& a, const PartArgs& p, const TilePlan& t, cudaStream_t
   CUtensorMap map_k, map_v;
   memset(&map_k, 0, sizeof(map_k));
   memset(&map_v, 0, sizeof(map_v));
-  if (FMT == kF16Pages) {
+  if (!C::BYTES) {
     const int64_t rows = (int64_t)a.num_blocks * a.hkv * a.page;
     if (int e = encode_pages(&map_k, a.k, rows, D * 2, ta.run)) return e;
     if (int e = encode_pages(&map_v, a.v, rows, D * 2, ta.run)) return e;
@@ -593,6 +644,7 @@ namespace pages {
 int tile_rows(int d, int64_t rows) { return d < 256 && rows > BM ? 2 * BM : BM; }
 
 int tile_launch(const AttnArgs& a, const PartArgs& p, const TilePlan& t, int fmt, int dtype, cudaStream_t stream) {
+  if (fmt == kScaled16) return dtype == LLMSS_F16 ? by_size<__half, kScaled16>(a, p, t, stream) : by_size<__nv_bfloat16, kScaled16>(a, p, t, stream);
   if (dtype == LLMSS_F16)
     return fmt == kInt8 ? by_size<__half, kInt8>(a, p, t, stream) : fmt == kE4M3 ? by_size<__half, kE4M3>(a, p, t, stream) : by_size<__half, kF16Pages>(a, p, t, stream);
   return fmt == kInt8   ? by_size<__nv_bfloat16, kInt8>(a, p, t, stream)

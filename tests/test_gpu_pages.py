@@ -278,17 +278,18 @@ def test_values_of_very_different_size(kind, dtype, new):
     ops.attention(q, out, batch, k, v, 8, 2, 128, 0.1, 0, 0, 0)
     want = attend64(q, k, v, batch, seen, 8, 2, 128, 0.1)
     tol = _bound(q, k, v, batch, seen, 8, 2, 128, 0.1, dtype) + UNIT[dtype] * want.abs()
+    # f16 has a step of 2^-24 below 2^-14: half of it, 2^-25 absolute, where the relative bounds above count less.  Operands of 8-bit pages are f16:
+    # values stand relative to a power of two below twice the largest scale of their 64 keys, s, so they are off by 2^-24 s each, and their weights add up to
+    # 1; a probability stands times 2^7 relative to a reference not above the row's maximum, and times the ratio of its keys' power of two to the largest
+    # one: off by 2^-32 (largest / own), on a value of at most qmax own, so 2^-31 qmax s for every key.  A result in f16 is off by 2^-25
+    at = 0
+    for i, (a, L) in enumerate(zip(new, batch.seq_lens.tolist())):
+        block = torch.tensor([seen.tables[i][p // 64] for p in range(L)], device="cuda")
+        top = v.scale.double()[block, :, torch.arange(L, device="cuda") % 64].amax(0)                               # [key heads]
+        tol[at:at + a] += (top * (2.0 ** -24 + L * QMAX[kind] * 2.0 ** -31))[:, None].expand(2, 512).reshape(1, -1)
+        at += a
     if dtype == HF:
-        # f16 has a step of 2^-24 below 2^-14, half of it is 2^-25 absolute: once for the result, once for the values (their weights add up to 1), and once
-        # for a probability, which stands times 2^7 relative to a reference not above the row's maximum: 2^-32 |v| for every key, where the relative bound
-        # above counts u p |v| alone and p may be below 2^-21
-        tol += 2 * 2.0 ** -25
-        at = 0
-        for i, (a, L) in enumerate(zip(new, batch.seq_lens.tolist())):
-            block = torch.tensor([seen.tables[i][p // 64] for p in range(L)], device="cuda")
-            total = values64(v).abs()[block, :, torch.arange(L, device="cuda") % 64].sum(0)                     # [key heads, d]
-            tol[at:at + a] += 2.0 ** -32 * total[:, None].expand(2, 4, 128).reshape(1, -1)
-            at += a
+        tol += 2.0 ** -25
     assert ((out.double() - want).abs() <= tol).all()
 
 
