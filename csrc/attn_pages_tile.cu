@@ -395,18 +395,25 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       const int64_t at = live ? (int64_t)tok * a.ldq + (int64_t)head * D : -1;
       constexpr int LANES = D / 8 < 32 ? D / 8 : 32, STEP = 32 / LANES;    // lanes of a row, rows of one copy of the warp
       const int ch = lane % LANES;
-#pragma unroll 4
+      auto place = [&](int row) {
+        const int rt = quarter * 32 + row;
+        return dst + (ch >> 3) * (BM * 128) + rt * 128 + (((ch & 7) ^ (rt & 7)) << 4);
+      };
+#pragma unroll
       for (int i = 0; i < 32; i += STEP) {
         const int row = i + lane / LANES;
         const int64_t from = __shfl_sync(0xffffffffu, at, row);
-        const int rt = quarter * 32 + row;
-        uint8_t* to = dst + (ch >> 3) * (BM * 128) + rt * 128 + (((ch & 7) ^ (rt & 7)) << 4);
-        const T* src = reinterpret_cast<const T*>(a.q) + (from < 0 ? 0 : from + ch * 8);
-        if constexpr (std::is_same<M, T>::value) {
-          copy16(smem_u32(to), src, from < 0 ? 0 : 16);
-        } else {
+        copy16(smem_u32(place(row)), reinterpret_cast<const T*>(a.q) + (from < 0 ? 0 : from + ch * 8), from < 0 ? 0 : 16);
+      }
+      copies_commit();
+      if constexpr (!std::is_same<M, T>::value) {
+        // to f16 where they lie: a lane takes what it copied itself (loads of four rows at a time into registers waited four times for memory)
+        copies_wait<0>();
+#pragma unroll 4
+        for (int i = 0; i < 32; i += STEP) {
+          uint4* to = reinterpret_cast<uint4*>(place(i + lane / LANES));
           float x[8], mx = 0.f;
-          unpack8<T>(from < 0 ? make_uint4(0u, 0u, 0u, 0u) : *reinterpret_cast<const uint4*>(src), x);
+          unpack8<T>(*to, x);
 #pragma unroll
           for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
 #pragma unroll
@@ -414,13 +421,12 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
           const int e = mx > 0.f && mx < INFINITY ? max(-126, min(126, (int)((__float_as_uint(mx) >> 23) & 255) - 127)) : 0;
 #pragma unroll
           for (int k = 0; k < 8; ++k) x[k] *= two_to(-e);
-          *reinterpret_cast<uint4*>(to) = pack8<__half>(x);
+          *to = pack8<__half>(x);
           // the row's factor goes to its own thread
           const float up_q = __shfl_sync(0xffffffffu, two_to(e), (lane % STEP) * LANES);
           if (lane / STEP == i / STEP) scale *= up_q;
         }
       }
-      copies_commit();
     }
     int pos = 0x7fffffff;                                 // rows beyond the last look at everything and are dropped
     if (live) {
