@@ -395,37 +395,41 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       const int64_t at = live ? (int64_t)tok * a.ldq + (int64_t)head * D : -1;
       constexpr int LANES = D / 8 < 32 ? D / 8 : 32, STEP = 32 / LANES;    // lanes of a row, rows of one copy of the warp
       const int ch = lane % LANES;
-      auto place = [&](int row) {
+      auto place = [&](int row, int ch) {
         const int rt = quarter * 32 + row;
         return dst + (ch >> 3) * (BM * 128) + rt * 128 + (((ch & 7) ^ (rt & 7)) << 4);
       };
-#pragma unroll
+      // loops, not lines: what runs once comes from memory, eight instructions at a time
+#pragma unroll 2
       for (int i = 0; i < 32; i += STEP) {
         const int row = i + lane / LANES;
         const int64_t from = __shfl_sync(0xffffffffu, at, row);
-        copy16(smem_u32(place(row)), reinterpret_cast<const T*>(a.q) + (from < 0 ? 0 : from + ch * 8), from < 0 ? 0 : 16);
+        copy16(smem_u32(place(row, ch)), reinterpret_cast<const T*>(a.q) + (from < 0 ? 0 : from + ch * 8), from < 0 ? 0 : 16);
       }
       copies_commit();
       if constexpr (!std::is_same<M, T>::value) {
-        // to f16 where they lie: a lane takes what it copied itself (loads of four rows at a time into registers waited four times for memory)
+        // to f16 where they lie, each row by its own thread
         copies_wait<0>();
+        __syncwarp();
+        uint32_t top = 0;                                 // largest absolute value, as bits: NaN lies above infinity
 #pragma unroll 4
-        for (int i = 0; i < 32; i += STEP) {
-          uint4* to = reinterpret_cast<uint4*>(place(i + lane / LANES));
-          float x[8], mx = 0.f;
+        for (int c = 0; c < D / 8; ++c) {
+          const uint4 w = *reinterpret_cast<const uint4*>(place(lane, c));
+          top = __vmaxu2(top, __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)));
+        }
+        top = max(top & 0xffffu, top >> 16) >> 7;         // bf16: eight bits of exponent above seven of fraction
+        const int e = top == 255 ? 0 : max(-126, min(126, (int)top - 127));
+        const float down = two_to(-e);
+#pragma unroll 4
+        for (int c = 0; c < D / 8; ++c) {
+          uint4* to = reinterpret_cast<uint4*>(place(lane, c));
+          float x[8];
           unpack8<T>(*to, x);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
-#pragma unroll
-          for (int o = LANES / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-          const int e = mx > 0.f && mx < INFINITY ? max(-126, min(126, (int)((__float_as_uint(mx) >> 23) & 255) - 127)) : 0;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) x[k] *= two_to(-e);
+          for (int k = 0; k < 8; ++k) x[k] *= down;
           *to = pack8<__half>(x);
-          // the row's factor goes to its own thread
-          const float up_q = __shfl_sync(0xffffffffu, two_to(e), (lane % STEP) * LANES);
-          if (lane / STEP == i / STEP) scale *= up_q;
         }
+        scale *= two_to(e);
       }
     }
     int pos = 0x7fffffff;                                 // rows beyond the last look at everything and are dropped
