@@ -96,26 +96,25 @@ __global__ void __launch_bounds__(32 * kWarps) rope_kv_write_q8_kernel(T* __rest
   const bool apart = a.style == LLMSS_ROPE_NEOX && i < half / 8;
   const int ca = apart ? i * 8 : i * 16, cb = apart ? i * 8 + half : i * 16 + 8;
   const bool turn_a = ca < a.rotary_dim, turn_b = cb < a.rotary_dim, has_b = cb < a.d;
-  // rows of one kind: this warp's every step-th group of per_warp heads
-  auto row_of = [&](int it, int off, int heads, bool wanted, T*& p) {
-    const int h = it * a.per_warp + sub;
-    p = row + off + h * a.d;
-    return wanted && h < heads && sub < a.per_warp;
-  };
-  // the kinds' items follow one another, q, k, v: where a warp begins in each, so that a step's few items spread over all warps
-  const int fq = first, fk = a.q_items > 0 ? (first + step - a.q_items % step) % step : first, fv = (fk + step - a.kv_items % step) % step;
+  // items are rows of k, then of v, then of q, per_warp heads each; a warp takes every step-th.  One loop for the three kinds: what a step's few tokens run
+  // comes cold from memory, and three loops are three times the instructions
+  const int items = 2 * a.kv_items + a.q_items;
   uint4 ra = make_uint4(0u, 0u, 0u, 0u), rb = ra;
   T* p = nullptr;
   bool live = false;
-  auto fetch = [&](int it, int items, int off, int heads, bool wanted) {
-    live = it < items && row_of(it, off, heads, wanted, p);
+  int kind = 0, h = 0;                                          // 0 k, 1 v, 2 q; head
+  auto fetch = [&](int it) {
+    kind = it < a.kv_items ? 0 : it < 2 * a.kv_items ? 1 : 2;
+    h = (it - min(kind, 2) * a.kv_items) * a.per_warp + sub;
+    p = row + (kind == 0 ? a.k_off : kind == 1 ? a.v_off : a.q_off) + h * a.d;
+    live = it < items && sub < a.per_warp && (kind == 2 ? turn_a && h < a.hq : store && h < a.hkv);
     ra = rb = make_uint4(0u, 0u, 0u, 0u);
     if (live) {
       ra = *reinterpret_cast<const uint4*>(p + ca);
       if (has_b) rb = *reinterpret_cast<const uint4*>(p + cb);
     }
   };
-  if (fk < a.kv_items) fetch(fk, a.kv_items, a.k_off, a.hkv, store);    // in flight while the angles are formed
+  fetch(first);                                                 // in flight while the angles are formed
   float cs[8], sn[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) cs[e] = 1.f, sn[e] = 0.f;
@@ -197,36 +196,22 @@ __global__ void __launch_bounds__(32 * kWarps) rope_kv_write_q8_kernel(T* __rest
       if (i == 0) scales[at] = finite ? scale : __int_as_float(0x7fc00000);
     }
   };
-  float x[8], y[8];
-  for (int it = fk; it < a.kv_items; it += step) {
+  for (int it = first; it < items; it += step) {
+    float x[8], y[8];
     unpack8<T>(ra, x);
     unpack8<T>(rb, y);
     const bool mine = live;
-    if (it + step < a.kv_items) fetch(it + step, a.kv_items, a.k_off, a.hkv, store);
-    else fetch(fv, a.kv_items, a.v_off, a.hkv, store);
-    turn(x, y);
-    if (store) put(x, y, mine, it * a.per_warp + sub, a.k, a.k_scale);
-  }
-  if (fk >= a.kv_items) fetch(fv, a.kv_items, a.v_off, a.hkv, store);
-  for (int it = fv; it < a.kv_items; it += step) {
-    unpack8<T>(ra, x);
-    unpack8<T>(rb, y);
-    const bool mine = live;
-    if (it + step < a.kv_items) fetch(it + step, a.kv_items, a.v_off, a.hkv, store);
-    else fetch(fq, a.q_items, a.q_off, a.hq, turn_a);
-    if (store) put(x, y, mine, it * a.per_warp + sub, a.v, a.v_scale);
-  }
-  if (fv >= a.kv_items) fetch(fq, a.q_items, a.q_off, a.hq, turn_a);
-  for (int it = fq; it < a.q_items; it += step) {
-    unpack8<T>(ra, x);
-    unpack8<T>(rb, y);
-    const bool mine = live;
+    const int kind0 = kind, h0 = h;
     T* to = p;
-    fetch(it + step, a.q_items, a.q_off, a.hq, turn_a);
-    turn(x, y);
-    if (mine) {
-      *reinterpret_cast<uint4*>(to + ca) = pack8<T>(x);
-      if (turn_b) *reinterpret_cast<uint4*>(to + cb) = pack8<T>(y);
+    fetch(it + step);
+    if (kind0 != 1) turn(x, y);
+    if (kind0 == 2) {
+      if (mine) {
+        *reinterpret_cast<uint4*>(to + ca) = pack8<T>(x);
+        if (turn_b) *reinterpret_cast<uint4*>(to + cb) = pack8<T>(y);
+      }
+    } else if (store) {
+      put(x, y, mine, h0, kind0 == 0 ? a.k : a.v, kind0 == 0 ? a.k_scale : a.v_scale);
     }
   }
 }
