@@ -106,8 +106,9 @@ __global__ void __launch_bounds__(128) attn_pages_any_kernel(const __grid_consta
 // kernels before it left in L2; launched to start as they end (programmatic dependent launch), so that it costs no launch latency of its own.
 // WARPS of them share a row where rows are few: parts are many then, and each costs a read from L2.
 template <typename T, int D, int WARPS>
-__global__ void __launch_bounds__(256) attn_pages_merge_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ PartArgs p) {
-  constexpr int N = D / 32;
+__global__ void __launch_bounds__(256, D < 256 && WARPS == 1 ? 5 : 4) attn_pages_merge_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ PartArgs p) {
+  constexpr int N = D / 32, VEC = N < 4 ? N : 4;          // columns of a lane, VEC neighbouring ones
+  using Vec = typename std::conditional<VEC == 4, float4, float2>::type;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int w = WARPS == 1 ? blockIdx.x * 8 + warp : blockIdx.x, mine = WARPS == 1 ? 0 : warp;
   const int t = w / a.hq, head = w % a.hq;
@@ -118,68 +119,81 @@ __global__ void __launch_bounds__(256) attn_pages_merge_kernel(const __grid_cons
   float o[N], m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) o[i] = 0.f;
-  // parts at first, first + stride ..: a lane looks at one part's maximum and sum, then all lanes add up the parts with their weights
-  auto add = [&](const float* first, int64_t stride, int count) {
-    if constexpr (WARPS > 1) {             // every WARPS-th part
-      first += mine * stride;
-      stride *= WARPS;
-      count = count > mine ? (count - mine + WARPS - 1) / WARPS : 0;
-    }
-    for (int b = 0; b < count; b += 32) {
-      const int k = min(32, count - b);
-      float2 ml = make_float2(-INFINITY, 0.f);
-      if (lane < k) ml = *reinterpret_cast<const float2*>(first + (b + lane) * stride + D);
-      const float mn = fmaxf(m, warp_max(ml.x)), base = mn == -INFINITY ? 0.f : mn;
-      const float f = m == mn ? 1.f : exp2f(m - base), e = exp2f(ml.x - base);
-      l = l * f + warp_sum(ml.y * e);
-      m = mn;
+  const Seg own = own_segment(a, s);
+  const Seg gs = g >= 0 ? group_segment(a, g) : Seg{};
+  const bool has_own = own.hi > own.lo, has_group = g >= 0 && gs.hi > 0;
+  // parts lie in up to four runs: the own keys' first and others, the group's first and others (stretches of keys: the others only).  They are added in one
+  // loop: with one per run a row waited for memory four times, and for the instructions of each
+  // Places are counted in 16 bytes from the scratch's begin (p.slots): 32 bits, since registers decide how many rows are in flight.
+  uint32_t run[4] = {0, 0, 0, 0}, step[4] = {0, 0, 0, 0};
+  int ends[4] = {0, 0, 0, 0};
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  constexpr uint32_t ROW = (D + kPad) / 4;
+  const uint32_t slot = p.rows * ROW, at = (uint32_t)(t * a.hq + head) * ROW;
+  auto place = [&](const float* x) { return (uint32_t)((x - p.slots) >> 2); };
 #pragma unroll
-      for (int i = 0; i < N; ++i) o[i] *= f;
-#pragma unroll 4
-      for (int j = 0; j < k; ++j) {
-        const float w = __shfl_sync(0xffffffffu, e, j);
-        const float* part = first + (b + j) * stride;
-#pragma unroll
-        for (int i = 0; i < N; i += 2) {
-          const float2 v = *reinterpret_cast<const float2*>(part + i * 32 + lane * 2);
-          o[i] += w == 0.f ? 0.f : w * v.x;
-          o[i + 1] += w == 0.f ? 0.f : w * v.y;
+  for (int x = 0; x < 2; ++x) {                           // own keys, the group's
+    int first = 0, others = 0;
+    if (x == 0 ? has_own : has_group) {
+      const Seg& sg = x == 0 ? own : gs;
+      if (x == 0 ? p.few_own : p.few_groups) {
+        const FewInfo in = p.info[(int64_t)(x == 0 ? s : (p.few_own ? a.num_seqs : 0) + g) * a.hkv + kvh];
+        const int n = (t - sg.row0) * group + head % group;
+        if (in.first_slot < 0) {
+          if (a.groups == 0) return;                      // the result is written already
+          run[2 * x] = place(x == 0 ? p.whole_own : p.whole_group) + at;
+          first = 1;
+        } else if (n < p.rows) {
+          run[2 * x] = in.first_slot * slot + n * ROW;
+          run[2 * x + 1] = 2 * (in.first_warp + 1) * slot + n * ROW;
+          step[2 * x + 1] = 2 * slot;
+          first = 1, others = in.last_warp - in.first_warp;
         }
+      } else {
+        const int chunk = x == 0 ? p.own_chunk : p.group_chunk;
+        run[2 * x + 1] = place(x == 0 ? p.tile_own : p.tile_group) + at;
+        step[2 * x + 1] = (uint32_t)(a.total_q * a.hq) * ROW;
+        others = min(x == 0 ? p.own_splits : p.group_splits, (sg.hi - sg.lo + chunk - 1) / chunk);
       }
     }
-  };
-  const Seg own = own_segment(a, s);
-  const bool has_own = own.hi > own.lo;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  auto few = [&](int seg, int row0, float* whole) {       // false: the result is written already
-    const FewInfo in = p.info[(int64_t)seg * a.hkv + kvh];
-    if (in.first_slot < 0) {
-      if (a.groups == 0) return false;
-      add(whole + ((int64_t)t * a.hq + head) * (D + kPad), 0, 1);
-      return true;
-    }
-    const int n = (t - row0) * group + head % group;
-    if (n >= p.rows) return true;
-    const int64_t slot = (int64_t)p.rows * (D + kPad);
-    add(p.slots + in.first_slot * slot + n * (D + kPad), 0, 1);
-    add(p.slots + (int64_t)2 * (in.first_warp + 1) * slot + n * (D + kPad), 2 * slot, in.last_warp - in.first_warp);
-    return true;
-  };
-  auto stretches = [&](const float* parts, int lo, int hi, int chunk, int splits) {
-    add(parts + ((int64_t)t * a.hq + head) * (D + kPad), (int64_t)a.total_q * a.hq * (D + kPad), min(splits, (hi - lo + chunk - 1) / chunk));
-  };
-  if (has_own) {
-    if (p.few_own) {
-      if (!few(s, own.row0, p.whole_own)) return;
-    } else {
-      stretches(p.tile_own, own.lo, own.hi, p.own_chunk, p.own_splits);
-    }
+    ends[2 * x] = (x > 0 ? ends[1] : 0) + first;
+    ends[2 * x + 1] = ends[2 * x] + others;
   }
-  if (g >= 0) {
-    const Seg gs = group_segment(a, g);
-    if (gs.hi > 0) {
-      if (p.few_groups) few((p.few_own ? a.num_seqs : 0) + g, gs.row0, p.whole_group);
-      else stretches(p.tile_group, 0, gs.hi, p.group_chunk, p.group_splits);
+  // a lane looks at one part's maximum and sum, then all lanes add up the parts with their weights; with WARPS, every WARPS-th part
+  const int count = ends[3] > mine ? (ends[3] - mine + WARPS - 1) / WARPS : 0;
+  for (int b = 0; b < count; b += 32) {
+    const int k = min(32, count - b);
+    float2 ml = make_float2(-INFINITY, 0.f);
+    uint32_t from = 0;
+    if (lane < k) {
+      const int x = (b + lane) * WARPS + mine;
+      from = x < ends[0] ? run[0] : x < ends[1] ? run[1] + (x - ends[0]) * step[1] : x < ends[2] ? run[2] : run[3] + (x - ends[2]) * step[3];
+      ml = *reinterpret_cast<const float2*>(p.slots + (int64_t)from * 4 + D);
+    }
+    const float mn = fmaxf(m, warp_max(ml.x)), base = mn == -INFINITY ? 0.f : mn;
+    const float f = m == mn ? 1.f : exp2f(m - base), e = exp2f(ml.x - base);
+    l = l * f + warp_sum(ml.y * e);
+    m = mn;
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] *= f;
+    constexpr int AT_ONCE = 4;                            // parts on their way
+    for (int j = 0; j < k; j += AT_ONCE) {
+      float w[AT_ONCE];
+      Vec v[AT_ONCE][N / VEC];
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        w[u] = __shfl_sync(0xffffffffu, e, j + u);        // 0 of lanes without a part
+        const float* part = p.slots + (int64_t)__shfl_sync(0xffffffffu, from, j + u) * 4;
+#pragma unroll
+        for (int i = 0; i < N / VEC; ++i) {
+          v[u][i] = Vec{};
+          if (w[u] != 0.f) v[u][i] = *reinterpret_cast<const Vec*>(part + i * 32 * VEC + lane * VEC);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u)
+#pragma unroll
+        for (int i = 0; i < N; ++i) o[i] = fmaf(w[u], reinterpret_cast<const float*>(&v[u][i / VEC])[i % VEC], o[i]);
     }
   }
   if constexpr (WARPS > 1) {
@@ -187,7 +201,7 @@ __global__ void __launch_bounds__(256) attn_pages_merge_kernel(const __grid_cons
     __shared__ float s_o[WARPS][D];
     if (lane == 0) s_ml[warp][0] = m, s_ml[warp][1] = l;
 #pragma unroll
-    for (int i = 0; i < N; i += 2) *reinterpret_cast<float2*>(&s_o[warp][i * 32 + lane * 2]) = make_float2(o[i], o[i + 1]);
+    for (int i = 0; i < N; ++i) s_o[warp][i * 32 + lane] = o[i];      // its own numbers, as they lie in the lane
     __syncthreads();
     if (warp > 0) return;
     m = -INFINITY, l = 0.f;
@@ -200,19 +214,21 @@ __global__ void __launch_bounds__(256) attn_pages_merge_kernel(const __grid_cons
       const float f = exp2f(s_ml[j][0] - (m == -INFINITY ? 0.f : m));
       l += s_ml[j][1] * f;
 #pragma unroll
-      for (int i = 0; i < N; i += 2) {
-        const float2 v = *reinterpret_cast<const float2*>(&s_o[j][i * 32 + lane * 2]);
-        o[i] += v.x * f, o[i + 1] += v.y * f;
-      }
+      for (int i = 0; i < N; ++i) o[i] = fmaf(s_o[j][i * 32 + lane], f, o[i]);
     }
   }
   // no visible key: zero (l is NaN where a score was)
   const float inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
   T* out = reinterpret_cast<T*>(a.out) + (int64_t)t * a.ldo + (int64_t)head * D;
 #pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    T v[2] = {from_f32<T>(o[i] * inv), from_f32<T>(o[i + 1] * inv)};
-    *reinterpret_cast<uint32_t*>(out + i * 32 + lane * 2) = *reinterpret_cast<const uint32_t*>(v);
+  for (int i = 0; i < N; i += VEC) {
+    T v[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = from_f32<T>(o[i + e] * inv);
+    using Out = typename std::conditional<VEC == 4, uint2, uint32_t>::type;
+    Out x;
+    memcpy(&x, v, sizeof(x));
+    *reinterpret_cast<Out*>(out + i * 32 + lane * VEC) = x;
   }
 }
 
@@ -435,6 +451,7 @@ LLMSS_API int llmss_attn_pages(const void* q, int64_t ldq, const void* k_pages, 
   if (!plan.any) {
     LLMSS_REQUIRE(plan.floats == 0 || (scratch != nullptr && scratch_floats >= plan.floats && ((uintptr_t)scratch % 16) == 0), "attn_pages: %lld floats of 16-byte aligned scratch needed",
                   (long long)plan.floats);
+    LLMSS_REQUIRE(plan.floats < (1ll << 34), "attn_pages: 64 GB of scratch and more");   // the merge kernel's places
     PartArgs p;
     memset(&p, 0, sizeof(p));
     float* at = (float*)scratch;

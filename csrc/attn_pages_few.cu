@@ -239,7 +239,7 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     settle();
   };
   settle();
-#pragma unroll
+#pragma unroll 1                           // instructions come cold from memory: few of them before the first copies
   for (int i = 0; i < STAGES; ++i)
     if (more) copy(i);
   int stage = 0;
