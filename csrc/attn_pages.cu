@@ -330,6 +330,29 @@ void stretches(int64_t blocks, int keys, bool merged, int& splits, int& chunk) {
   splits = keys > 0 ? (keys + chunk - 1) / chunk : 1;
 }
 
+// Prefixes by the tiled kernel, a sequence's own keys by the one for few rows: one after the other on all 148 SMs (beside a block of the first there is room for one
+// of the second at most), or at the same time, the second on the SMs that fewer stretches of the first leave.  The estimates, in microseconds, were fitted to decode
+// steps of 24 to 64 sequences with 60 to 3000 tokens of their own behind 1500 to 12000: a tile of 64 keys 1.15 (8 bits 1.45), an SM reading own keys 88 GB/s
+// (8 bits, where it converts, 37) with 0.35 for each list, all of them 6.2 TB/s, starts 7 (8 bits 10) and 7.  64 sequences of 200 tokens behind 4096: 36.9 -> 24.7; of 3000 tokens: 147 -> 134;
+// 48 of 300 behind three prefixes of 2500, int8: 41.0 -> 32.5.  Returns the SMs of the second kernel.
+int side_by_side(int64_t lists, int len, double own_lists, double own_bytes, double part_bytes, int d, int fmt, int& splits, int& chunk) {
+  const bool wide = fmt == kF16Pages;
+  const int64_t tiles = (len + 63) / 64;
+  const double start = wide ? 7 : 10, per_tile = (wide ? 1.15 : 1.45) * d / 128, part = part_bytes / 4e6, all = own_bytes / 6.2e6, one = own_bytes / (wide ? 88e3 : 37e3) + 0.35 * own_lists;
+  auto prefix = [&](int64_t n) { return start + per_tile * ((lists * n + 147) / 148) * ((tiles + n - 1) / n); };
+  auto own = [&](int64_t sms) { return 7 + (one / sms > all ? one / sms : all); };
+  double best = prefix(splits) + own(148) + part * splits;
+  int64_t at = 0;
+  for (int64_t n = 1; lists * n < 148 && n <= (tiles + 1) / 2; ++n) {
+    const double a = prefix(n), b = own(148 - lists * n), c = (1.1 * a > b ? 1.1 * a : b) + part * n;
+    if (c < best) best = c, at = n;
+  }
+  if (at == 0) return 148;
+  chunk = (int)((tiles + at - 1) / at * 64);
+  splits = (len + chunk - 1) / chunk;
+  return 148 - (int)lists * splits;
+}
+
 Plan plan_call(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv, int d, int page, int fmt, int groups, int g_max_len, int g_max_rows) {
   Plan p;
   memset(&p, 0, sizeof(p));
@@ -340,13 +363,6 @@ Plan plan_call(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv
   // up to 16 rows of a key head fit the narrow side of the warp-level product; a tile of 128 costs the tiled kernel the same whatever is in it
   p.few_own = own <= 16;
   p.few_groups = groups > 0 && grouped <= 16;
-  if (p.few_own || p.few_groups) {
-    p.rows = (int)(p.few_own && (!p.few_groups || own >= grouped) ? own : grouped);
-    p.blocks = few_blocks(fmt, d, p.rows, (p.few_own ? num_seqs : 0) + (p.few_groups ? groups : 0));
-    p.slots = (int64_t)2 * p.blocks * kFewWarps * p.rows * (d + kPad);
-    p.info = ((int64_t)(p.few_own ? num_seqs : 0) + (p.few_groups ? groups : 0)) * hkv * 4;
-    p.whole = groups > 0 ? (int64_t)total_q * hq * (d + kPad) : 0;
-  }
   const bool tile_own = !p.few_own, tile_groups = groups > 0 && !p.few_groups;
   p.tile.rows = tile_rows(d, own > 16 && own > grouped ? own : grouped);
   if (tile_own) {
@@ -366,10 +382,25 @@ Plan plan_call(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv
     }
     if (!p.direct) p.tile_own = (int64_t)p.own_splits * total_q * hq * (d + kPad);
   }
+  int few_sms = 148;
   if (tile_groups) {
     p.tile.group_tiles = (int)((grouped + p.tile.rows - 1) / p.tile.rows);
-    stretches((int64_t)p.tile.group_tiles * hkv * groups, g_max_len, true, p.group_splits, p.group_chunk);
+    const int64_t lists = (int64_t)p.tile.group_tiles * hkv * groups;
+    stretches(lists, g_max_len, true, p.group_splits, p.group_chunk);
+    if (p.few_own) {
+      // three quarters of the longest: sequences differ, and a tiled kernel that takes longer than the other costs more than one that takes less
+      const double keys = 0.75 * (max_kv > g_max_len ? max_kv - g_max_len : 1);
+      few_sms = side_by_side(lists, g_max_len, (double)num_seqs * hkv, keys * num_seqs * hkv * d * (fmt == kF16Pages ? 4 : 2), (double)total_q * hq * (d + kPad) * 4, d, fmt,
+                             p.group_splits, p.group_chunk);
+    }
     p.tile_group = (int64_t)p.group_splits * total_q * hq * (d + kPad);
+  }
+  if (p.few_own || p.few_groups) {
+    p.rows = (int)(p.few_own && (!p.few_groups || own >= grouped) ? own : grouped);
+    p.blocks = few_blocks(fmt, d, p.rows, (p.few_own ? num_seqs : 0) + (p.few_groups ? groups : 0)) / 148 * few_sms;
+    p.slots = (int64_t)2 * p.blocks * kFewWarps * p.rows * (d + kPad);
+    p.info = ((int64_t)(p.few_own ? num_seqs : 0) + (p.few_groups ? groups : 0)) * hkv * 4;
+    p.whole = groups > 0 ? (int64_t)total_q * hq * (d + kPad) : 0;
   }
   p.floats = p.slots + p.info + (p.few_own ? p.whole : 0) + (p.few_groups ? p.whole : 0) + p.tile_own + p.tile_group + p.expanded;
   return p;
