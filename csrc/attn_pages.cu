@@ -373,8 +373,8 @@ Plan plan_call(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv
     stretches((int64_t)p.tile.own_tiles * hkv * num_seqs, keys, groups > 0, p.own_splits, p.own_chunk);
     p.direct = groups == 0 && p.own_splits == 1;
     // Every row tile converts all codes for itself, which takes the tiled kernel from 1100 to 2000 clocks per 64 keys; once for all costs a pass over the
-    // cache (about 1200 clocks of an SM per 64 keys, and a launch).  Portions of 1000 tokens over 1800, 16 tiles: 240 -> 150 us; from three tiles on.  Up to
-    // 1 GB of scratch
+    // cache (about 1200 clocks of an SM per 64 keys, and a launch).  4 portions of 1000 tokens over 1800, 16 tiles each: 251 -> 183 us; three tiles 89 -> 87
+    // (16 sequences 198 -> 170), two tiles 69 -> 68, one 47 -> 47: from three tiles on.  Up to 1 GB of scratch
     const int64_t pad = ((int64_t)max_kv + 63) / 64 * 64, expanded = (int64_t)num_seqs * hkv * (pad * d + pad / 64 * 4) + (num_seqs + 3) / 4 * 4;
     if (fmt != kF16Pages && groups == 0 && p.tile.own_tiles >= 3 && expanded <= (1ll << 28) && pad <= (1 << 19)) {
       p.pad = (int)pad;

@@ -4,7 +4,7 @@
 //
 //   s_jk = scale (q_j . K_k)      K_k = ks_k code_k      p = softmax over the keys k <= pos_j      out_j = sum_k p_jk vs_k code_k
 //
-// A sequence of a group (SharedGroups) finds its first len keys in the group's pages and the others in its own; a softmax over both is the merge
+// A sequence of a group (SharedPrefix) finds its first len keys in the group's pages and the others in its own; a softmax over both is the merge
 // of the two parts by their maxima and sums.
 #pragma once
 #include "common.cuh"

@@ -30,7 +30,7 @@ constexpr int BM = 128, BN = 64;
 template <int FMT, int D, int NQ>
 struct Tile {
   static constexpr int SOFT = 4 * NQ;                                   // softmax warps
-  // 8-bit: four warps would convert a tile in twice the time that the products take
+  // 8-bit: four warps convert a tile in the time that the products of two times 128 rows take, which is twice that of 128
   static constexpr bool BYTES = FMT == kInt8 || FMT == kE4M3, SCALED = FMT != kF16Pages;
   static constexpr int CONVERT = !BYTES ? 0 : NQ == 2 ? 4 : 8;
   static constexpr int COPY = SOFT + NQ;                                // first copying warp
