@@ -144,20 +144,21 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   }
   pdl_wait();
 
-  // the block's list, rows and keys
-  const bool is_own = (int)blockIdx.z < ta.segs_own;
+  // the block's list, rows and keys: groups' lists first, since they are long, and of a list's rows the last first, since they see most
+  const int in_groups = ta.group_tiles * ta.group_splits * a.hkv * a.groups;      // (group_tiles 0: groups are not this launch's)
+  const bool is_own = (int)blockIdx.x >= in_groups;
+  const int at = is_own ? blockIdx.x - in_groups : blockIdx.x;
   const int tiles = is_own ? ta.own_tiles : ta.group_tiles, splits = is_own ? ta.own_splits : ta.group_splits;
   const int chunk = is_own ? ta.own_chunk : ta.group_chunk;
-  if ((int)blockIdx.x >= tiles * splits) return;
-  // long causal ranges first
-  const int tile = tiles - 1 - (int)blockIdx.x / splits, split = (int)blockIdx.x % splits;
-  const Seg s = is_own ? own_segment(a, blockIdx.z) : group_segment(a, blockIdx.z - ta.segs_own);
-  const int kvh = blockIdx.y, group = a.hq / a.hkv;
+  const int part = at % (tiles * splits), list = at / (tiles * splits), kvh = list % a.hkv, seg = list / a.hkv;
+  const int tile = tiles - 1 - part / splits, split = part % splits;
+  const Seg s = is_own ? own_segment(a, seg) : group_segment(a, seg);
+  const int group = a.hq / a.hkv;
   const int nrows = s.rows * group, n0 = tile * (NQ * BM);
   if (n0 >= nrows) return;
   const int n_last = min(nrows, n0 + NQ * BM) - 1;
   int k_end = s.hi;
-  if (is_own) k_end = min(k_end, row_pos(a, blockIdx.z, s.row0 + n_last / group) + 1);
+  if (is_own) k_end = min(k_end, row_pos(a, seg, s.row0 + n_last / group) + 1);
   // stretch `split` of the list; the last one takes what lies behind it (lengths beyond the bounds the call gave)
   const int k_lo = max(s.lo, s.lo + split * chunk);
   const int k_hi = split == splits - 1 ? k_end : min(k_end, s.lo + (split + 1) * chunk);
@@ -228,7 +229,7 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         uint8_t* dst = s_kv + slot * C::SLOT;
         if (elect_one()) {
           mbar_arrive_expect_tx(bar, here * run * D * 2 + (C::SCALED && !value ? 16 : 0));
-          if (C::SCALED && !value) bulk_copy(&s_tile[j & 7], a.tile_scales + ((int64_t)blockIdx.z * a.hkv + kvh) * (a.page / BN) + first / BN, 16, bar);
+          if (C::SCALED && !value) bulk_copy(&s_tile[j & 7], a.tile_scales + ((int64_t)seg * a.hkv + kvh) * (a.page / BN) + first / BN, 16, bar);
         }
         for (int x = 0; x < here; ++x) {
           const int row = (int)__shfl_sync(0xffffffffu, rows, from + x);
@@ -437,7 +438,7 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     }
     int pos = 0x7fffffff;                                 // rows beyond the last look at everything and are dropped
     if (live) {
-      const int sq = is_own ? (int)blockIdx.z : seq_of_row(a.cu, 0, a.num_seqs, tok);
+      const int sq = is_own ? seg : seq_of_row(a.cu, 0, a.num_seqs, tok);
       pos = sq < 0 ? -1 : row_pos(a, sq, tok);
     }
     pos = min(pos, k_hi - 1);
@@ -635,9 +636,9 @@ int launch(const AttnArgs& a, const PartArgs& p, const TilePlan& t, cudaStream_t
     if (int e = encode_pages(&map_k, a.k, rows, D * 2, ta.run)) return e;
     if (int e = encode_pages(&map_v, a.v, rows, D * 2, ta.run)) return e;
   }
-  const int64_t x = (int64_t)t.own_tiles * p.own_splits, y = (int64_t)t.group_tiles * p.group_splits;
-  const dim3 grid((unsigned)(x > y ? x : y), a.hkv, ta.segs_own + (t.group_tiles > 0 ? a.groups : 0));
-  LLMSS_REQUIRE(grid.y <= 65535 && grid.z <= 65535 && (x > y ? x : y) < (1ll << 31), "attn_pages: grid too large (%d key heads, %u lists)", a.hkv, grid.z);
+  const int64_t blocks = ((int64_t)t.own_tiles * p.own_splits * ta.segs_own + (int64_t)t.group_tiles * p.group_splits * a.groups) * a.hkv;
+  LLMSS_REQUIRE(blocks < (1ll << 31), "attn_pages: grid too large (%lld blocks)", (long long)blocks);
+  const dim3 grid((unsigned)blocks);
   LLMSS_CHECK_CUDA(launch_pdl(kern, grid, dim3(C::THREADS), (size_t)C::SMEM, stream, map_k, map_v, a, p, ta));
   return 0;
 }
