@@ -188,6 +188,23 @@ def test_many_sequences_behind_a_long_prefix(kind, hq, hkv, d):
     _check(new, [1024 + 7 * i % 90 for i in range(40)], 64, [(list(range(40)), 1024)], hq, hkv, d, kind, BF, seed=1)
 
 
+@pytest.mark.parametrize("kind", [None, I8, E4])
+@pytest.mark.parametrize("hq,hkv,d", [(32, 8, 128), (48, 1, 128)])
+def test_one_long_sequence_among_short_ones(kind, hq, hkv, d):
+    """Its list is cut into far more parts than a warp has lanes; the others are a part each."""
+    for groups in ([], [(list(range(40)), 64)]):
+        if kind is None and not groups:
+            continue                     # 16-bit pages without a prefix are another kernel's
+        _check([1] * 40, [20000] + [64 + i for i in range(39)], 64, groups, hq, hkv, d, kind, BF, seed=6)
+
+
+@pytest.mark.parametrize("kind", [None, I8])
+@pytest.mark.parametrize("seqs,own,prefix", [(3, 4000, 64), (60, 3, 6400), (100, 40, 640), (17, 700, 2560)])
+def test_prefix_and_own_keys_of_very_different_size(kind, seqs, own, prefix):
+    """Whatever share of the machine either part gets."""
+    _check([1] * seqs, [prefix + (own + 13 * i) % (own + 1) for i in range(seqs)], 64, [(list(range(seqs)), prefix)], 32, 8, 128, kind, BF, seed=7)
+
+
 @pytest.mark.parametrize("kind", [I8, E4])
 def test_output_over_the_queries_columns(kind):
     """The fused block writes the context over its queries."""
