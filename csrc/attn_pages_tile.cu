@@ -36,7 +36,7 @@ struct Tile {
   static constexpr int COPY = SOFT + NQ;                                // first copying warp
   static constexpr int THREADS = 32 * (COPY + 2 + CONVERT);
   // 16-bit pages: registers, and shared memory for five tiles where two times 128 rows share them, that leave room for a block of the kernels which run
-  // beside this one (125 and six: 24 questions behind a prefix 164 us instead of 160, 4 portions of 1000 tokens over 1800 190 instead of 187)
+  // beside this one (with 125 and six, 16 questions behind a prefix and 4 portions of 1000 tokens over 1800 took 2 % longer)
   static constexpr int REGS = BYTES ? 128 : 112;
   static constexpr int Q_BYTES = NQ * BM * D * 2;
   static constexpr int SLOT = BN * D * 2;                               // a tile of keys or values
