@@ -341,11 +341,14 @@ int side_by_side(int64_t lists, int len, double own_lists, double own_bytes, dou
   const double start = wide ? 7 : 10, per_tile = (wide ? 1.15 : 1.45) * d / 128, part = part_bytes / 4e6, all = own_bytes / 6.2e6, one = own_bytes / (wide ? 88e3 : 37e3) + 0.35 * own_lists;
   auto prefix = [&](int64_t n) { return start + per_tile * ((lists * n + 147) / 148) * ((tiles + n - 1) / n); };
   auto own = [&](int64_t sms) { return 7 + (one / sms > all ? one / sms : all); };
+  // a captured step knows bounds alone, and own keys may be far fewer: prefixes take twice as long as on all SMs at most (64 sequences of 200 tokens behind
+  // 4096 with a bound of 8192: 70.6 -> 28.7)
+  const double longest = 2 * prefix(splits);
   double best = prefix(splits) + own(148) + part * splits;
   int64_t at = 0;
   for (int64_t n = 1; lists * n < 148 && n <= (tiles + 1) / 2; ++n) {
     const double a = prefix(n), b = own(148 - lists * n), c = (1.1 * a > b ? 1.1 * a : b) + part * n;
-    if (c < best) best = c, at = n;
+    if (a <= longest && c < best) best = c, at = n;
   }
   if (at == 0) return 148;
   chunk = (int)((tiles + at - 1) / at * 64);
