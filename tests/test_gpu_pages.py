@@ -370,6 +370,44 @@ def test_replayed_steps_follow_their_inputs(kind, groups):
             assert torch.equal(out, w)
 
 
+@pytest.mark.parametrize("kind,groups", [(I8, []), (E4, [(list(range(9)), 192)]), (None, [(list(range(9)), 192)])])
+@pytest.mark.parametrize("new", [1, 30, 200])
+def test_calls_on_two_streams_at_once(kind, groups, new):
+    """Each has a scratch of its own, and a call's result has the same bits every time."""
+    hq, hkv, d = 16, 2, 128
+    calls = []
+    for seed in (11, 12):
+        batch, seen = make_batch([new] * 9, [200 + 40 * i for i in range(9)], 64, groups, "cuda", seed=seed)
+        k, v = (make_pages(seen.blocks, hkv, 64, d, kind, BF, "cuda", seed=2 * seed + i) for i in range(2))
+        q = torch.randn(9 * new, hq * d, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda").to(BF)
+        calls.append((q, batch, k, v))
+    run = lambda c, out: ops.attention(c[0], out, c[1], c[2], c[3], hq, hkv, d, d ** -0.5, 0, 0, 0)
+    want = [run(c, torch.empty_like(c[0])).clone() for c in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = [[torch.empty_like(c[0]) for _ in range(12)] for c in calls]
+    torch.cuda.synchronize()
+    for n in range(12):
+        for c, s, outs in zip(calls, streams, got):
+            with torch.cuda.stream(s):
+                run(c, outs[n])
+    torch.cuda.synchronize()
+    for w, outs in zip(want, got):
+        assert all(torch.equal(o, w) for o in outs)
+
+
+def test_more_rows_than_cached_tokens():
+    """Rows before a sequence's first position see nothing."""
+    for new, hq, hkv in (([5, 1, 3], 4, 4), ([40, 1, 9], 16, 2)):
+        batch, seen = make_batch(new, [20, 30, 64], 16, [], "cuda", seed=3)
+        batch.seq_lens[0] = 3
+        for kind in (I8, E4):
+            k, v = (make_pages(seen.blocks, hkv, 16, 128, kind, BF, "cuda", seed=i) for i in range(2))
+            out = torch.full((sum(new), hq * 128), float("nan"), dtype=BF, device="cuda")
+            ops.attention(torch.randn(sum(new), hq * 128, device="cuda").to(BF), out, batch, k, v, hq, hkv, 128, 0.1, 0, 0, 0)
+            assert not out[:new[0] - 3].any() and torch.isfinite(out.float()).all() and out[new[0] - 3:].any(-1).all()
+
+
 def test_write_and_attention_together():
     """A layer's step as a model runs it: a prompt in portions and then single tokens behind a shared prefix, cache in 8 bits."""
     hq, hkv, d, page = 8, 2, 128, 64
