@@ -112,8 +112,8 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   uint2* s_q = reinterpret_cast<uint2*>(s_full + kWarps * STAGES);          // [warps][NT][KS][32] fragments, each lane's its own
   int* s_units = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(s_q) + kWarps * C::Q_BYTES);   // [min(segs, kKept)]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
-  pdl_launch_dependents();
-  if (!f.beside) pdl_wait();
+  if (!f.beside) pdl_wait();               // (beside: the kernel before lets this one start when its own wait is over)
+  pdl_launch_dependents();                 // the merge reads lengths in front of its wait
   uint8_t* ring = s_ring + warp * STAGES * 2 * C::HALF;
   uint64_t* full = s_full + warp * STAGES;
   if (lane == 0) {

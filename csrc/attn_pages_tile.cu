@@ -137,12 +137,13 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 
   // by a shuffle: numbers that the compiler knows to be the same in all lanes need no copies into uniform registers at every product
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  pdl_launch_dependents();
   if (!C::BYTES && threadIdx.x == 32 * C::COPY) {
     tma_prefetch_desc(&map_k);
     tma_prefetch_desc(&map_v);
   }
   pdl_wait();
+  // behind the wait: the kernel for few rows starts beside this one without a wait of its own, and reads what the kernels before this one wrote
+  pdl_launch_dependents();
 
   // the block's list, rows and keys: groups' lists first, since they are long, and of a list's rows the last first, since they see most
   const int in_groups = ta.group_tiles * ta.group_splits * a.hkv * a.groups;      // (group_tiles 0: groups are not this launch's)

@@ -552,3 +552,15 @@ def test_engine_reads_a_shared_prefix_once(tmp_path, monkeypatch, kind):
     while eng.has_work():
         eng.step()
     assert r.alloc.num_free == r.alloc.num_blocks - 1
+
+
+def test_with_early_launches():
+    """LLMSS_PDL=1 lets every kernel start before the one in front of it has ended; the variable is read once per process."""
+    import os
+    import subprocess
+    import sys
+
+    which = "write_and_attention_together or replayed_steps or two_streams or very_different_size"
+    r = subprocess.run([sys.executable, "-m", "pytest", __file__, "-x", "-q", "-m", "gpu", "-k", which, "-p", "no:cacheprovider"],
+                       env={**os.environ, "LLMSS_PDL": "1"}, capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0, r.stdout[-2000:]
