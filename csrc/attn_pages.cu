@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(256, D < 256 && WARPS == 1 ? 5 : 4) attn_pages
   for (int i = 0; i < N; ++i) o[i] = 0.f;
   const Seg own = own_segment(a, s);
   const Seg gs = g >= 0 ? group_segment(a, g) : Seg{};
-  const bool has_own = own.hi > own.lo, has_group = g >= 0 && gs.hi > 0;
+  const bool sees = row_pos(a, s, t) >= 0, has_own = sees && own.hi > own.lo, has_group = sees && g >= 0 && gs.hi > 0;
   // parts lie in up to four runs: the own keys' first and others, the group's first and others (stretches of keys: the others only).  They are added in one
   // loop: with one per run a row waited for memory four times, and for the instructions of each
   // Places are counted in 16 bytes from the scratch's begin (p.slots): 32 bits, since registers decide how many rows are in flight.
@@ -217,8 +217,8 @@ __global__ void __launch_bounds__(256, D < 256 && WARPS == 1 ? 5 : 4) attn_pages
       for (int i = 0; i < N; ++i) o[i] = fmaf(s_o[j][i * 32 + lane], f, o[i]);
     }
   }
-  // no visible key: zero (l is NaN where a score was)
-  const float inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
+  // a row that sees nothing, and so has no parts, is zero; NaN where a score was; where all visible scores are minus infinity l is 0, and the row NaN
+  const float inv = ends[3] == 0 ? 0.f : 1.f / l;
   T* out = reinterpret_cast<T*>(a.out) + (int64_t)t * a.ldo + (int64_t)head * D;
 #pragma unroll
   for (int i = 0; i < N; i += VEC) {

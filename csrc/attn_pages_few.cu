@@ -594,7 +594,8 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         const int tok = s.row0 + i / group, head = kvh * group + i % group;
         if (last) {
           // sum is NaN where a score was; a row without a visible key is zero
-          const float inv = pos[nt][c] < s.lo ? 0.f : 1.0f / sum;
+          const bool sees = pos[nt][c] >= s.lo;
+          const float inv = 1.0f / sum;
           back *= inv, off *= inv;
           T* dst = reinterpret_cast<T*>(a.out) + (int64_t)tok * a.ldo + (int64_t)head * D;
 #pragma unroll
@@ -603,8 +604,8 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             float y[8];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              y[2 * j] = fmaf(o[nt][4 * k + j][c], back, off);
-              y[2 * j + 1] = fmaf(o[nt][4 * k + j][c + 2], back, off);
+              y[2 * j] = sees ? fmaf(o[nt][4 * k + j][c], back, off) : 0.f;
+              y[2 * j + 1] = sees ? fmaf(o[nt][4 * k + j][c + 2], back, off) : 0.f;
             }
             *reinterpret_cast<uint4*>(dst + col) = pack8<T>(y);
           }

@@ -99,9 +99,10 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // NaN where one 
 }
 
 // 2^x without the MUFU pipe: x = n + r with r in [-0.5, 0.5], a cubic fitted to 2^r there (relative error 1.1e-4, below a rounding of the probability to
-// 16 bits), n added to the exponent; 2^-125 for what is below, and for NaN
+// 16 bits), n added to the exponent.  At -127 r is 0 and the polynomial 1.0, whose exponent becomes that of zero: 0 for what is below (hidden keys weigh
+// nothing, however large their values), and for NaN
 __device__ __forceinline__ float exp2_fma(float x) {
-  x = fmaxf(x, -125.0f);
+  x = fmaxf(x, -127.0f);
   const float t = x + 12582912.0f;                 // 1.5 * 2^23: the integer part lands in the low bits
   const float r = x - (t - 12582912.0f);
   float p = fmaf(r, 0.05459282f, 0.24221784f);
@@ -545,8 +546,8 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     // the other tile's products read keys and values too; its barriers' phases may lie behind by more than one, so that its own warps have to say it
     if constexpr (NQ > 1) asm volatile("bar.sync 1, %0;" ::"n"(32 * C::SOFT) : "memory");
     if (bad) l_run = __int_as_float(0x7fc00000);
-    // no visible key: zero
-    const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
+    const bool sees = pos >= k_lo;                        // no visible key: zero
+    const float inv = 1.0f / l_run;
     const int stride = ta.direct ? D * 2 + 16 : D * 4 + 16;
     uint8_t* stage = smem + (q * BM + quarter * 32) * stride;
     uint8_t* mine = stage + lane * stride;
@@ -565,7 +566,7 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         for (int i = 0; i < 32; i += 8) {
           float f8[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f8[e] = __uint_as_float(r[i + e]) * inv;
+          for (int e = 0; e < 8; ++e) f8[e] = sees ? __uint_as_float(r[i + e]) * inv : 0.f;
           *reinterpret_cast<uint4*>(mine + c * 64 + i * 2) = pack8<T>(f8);
         }
       } else {
