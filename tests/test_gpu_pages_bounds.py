@@ -1,0 +1,51 @@
+"""Attention over cache pages on the GPU within bounds that count each rounding: a result of zeros, or one without 16 of its keys, is outside of them."""
+import pytest
+import torch
+
+from llmss_b200 import ops
+from pages_bounds import expected
+from pages_oracle import make_batch, make_pages
+
+pytestmark = pytest.mark.gpu
+
+BF, HF = torch.bfloat16, torch.float16
+I8, E4 = torch.int8, torch.float8_e4m3fn
+
+CASES = {
+    # name: query lengths, context before them, page, prefix groups, heads
+    "single_tokens": ([1] * 5, [63, 64, 2000, 17, 131], 64, [], (32, 8, 128)),
+    "single_tokens_of_many_heads": ([1] * 4, [300, 900, 31, 64], 16, [], (48, 1, 128)),
+    "wide_heads": ([1] * 6, [700, 64, 1040, 90, 333, 20], 64, [], (16, 16, 256)),
+    "some_tokens": ([2, 1, 4], [200, 700, 61], 32, [], (4, 4, 128)),
+    "portions": ([64, 130, 1, 7], [0, 100, 1300, 64], 64, [], (8, 2, 128)),
+    "long_portions": ([200, 333], [500, 40], 64, [], (16, 2, 128)),
+    "small_heads": ([150, 40], [0, 600], 16, [], (16, 16, 64)),
+    "other_head_sizes": ([1, 30, 2], [200, 100, 0], 16, [], (6, 3, 96)),
+    "step_behind_a_prefix": ([1] * 40, [1024 + 7 * i % 90 for i in range(40)], 64, [(list(range(40)), 1024)], (32, 8, 128)),
+    "step_of_many_heads_behind_a_prefix": ([1] * 9, [640 + 5 * i for i in range(9)], 64, [(list(range(9)), 640)], (48, 1, 128)),
+    "own_keys_longer_than_the_prefix": ([1] * 17, [256 + (700 + 13 * i) % 701 for i in range(17)], 64, [(list(range(17)), 256)], (32, 8, 128)),
+    "two_prefixes": ([1] * 7, [130, 140, 129, 64, 65, 400, 20], 16, [([0, 1, 2], 128), ([3, 4], 64)], (8, 2, 128)),
+    "questions_behind_a_prefix": ([33, 20, 9], [1000, 960, 970], 64, [([0, 1, 2], 960)], (16, 16, 64)),
+    "prefix_that_ends_inside_a_page": ([3, 2], [100, 120], 32, [([0, 1], 100)], (4, 4, 128)),
+}
+
+
+@pytest.mark.parametrize("q_scale", [0.05, 1.0, 30.0])
+@pytest.mark.parametrize("dtype,kind", [(BF, None), (HF, None), (BF, I8), (HF, I8), (BF, E4), (HF, E4)])
+@pytest.mark.parametrize("case", sorted(CASES))
+def test_results_within_their_roundings(case, dtype, kind, q_scale):
+    new, ctx, page, groups, (hq, hkv, d) = CASES[case]
+    if kind is None and not groups:
+        pytest.skip("16-bit pages without a prefix are another kernel's")
+    batch, seen = make_batch(new, ctx, page, groups, "cuda", seed=len(case))
+    k, v = (make_pages(seen.blocks, hkv, page, d, kind, dtype, "cuda", seed=7 + i) for i in range(2))
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q = (torch.randn(sum(new), hq * d, generator=g, device="cuda") * q_scale).to(dtype)
+    scale = d ** -0.5
+    want, tol, less = expected(q, k, v, batch, seen, hq, hkv, d, scale)
+    # what the bounds are worth
+    assert (want.abs() > tol).double().mean() > 0.9
+    assert ((less - want).abs() > tol).double().mean() > (0.1 if q_scale <= 1 else 0.01)      # (sharp: a few keys of each row alone count)
+    got = ops.attention(q, torch.full_like(q, float("nan")), batch, k, v, hq, hkv, d, scale, 0, 0, 0).double()
+    off = (got - want).abs()
+    assert (off <= tol).all(), f"off by {float(off.max()):.3g}; up to {float((off / tol).max()):.3g} times the bound, {int((off > tol).sum())} of {off.numel()}"
