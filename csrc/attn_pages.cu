@@ -53,32 +53,11 @@ __global__ void __launch_bounds__(128) attn_pages_any_kernel(const __grid_consta
   const int g = group_of_seq(a, s);
   const int shared = g < 0 ? 0 : min(a.g_lens[g], a.g_max_blocks * a.page);
   const int kvh = head / (a.hq / a.hkv);
-  float q[8], o[8], m = -INFINITY, l = 0.f;
-  const T* qr = reinterpret_cast<const T*>(a.q) + (int64_t)t * a.ldq + (int64_t)head * a.d;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    q[i] = lane + 32 * i < a.d ? to_f32(qr[lane + 32 * i]) : 0.f;
-    o[i] = 0.f;
-  }
-  for (int j = warp; j < seen; j += 4) {
+  float o[8], m, l;
+  row_softmax<T, T, FMT>(a, t, head, warp, 4, seen, [&](int j) {
     const int* table = j < shared ? a.g_tables + (int64_t)g * a.g_max_blocks : a.tables + (int64_t)s * a.max_blocks;
-    const int64_t r = ((int64_t)checked_block(table[j / a.page], a.num_blocks) * a.hkv + kvh) * a.page + j % a.page;
-    float x = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (lane + 32 * i < a.d) x = fmaf(q[i], page_value<T, FMT>(a.k, r * a.d + lane + 32 * i), x);
-    x = warp_sum(x) * a.scale_log2;
-    if constexpr (FMT != kF16Pages) x *= a.ks[r];
-    const float mn = fmaxf(m, x), al = m == mn ? 1.f : exp2f(m - mn), p = x == -INFINITY ? 0.f : exp2f(x - mn);
-    l = l * al + p;
-    const float pv = FMT != kF16Pages ? p * a.vs[r] : p;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      o[i] *= al;
-      if (lane + 32 * i < a.d) o[i] = fmaf(pv, page_value<T, FMT>(a.v, r * a.d + lane + 32 * i), o[i]);
-    }
-    m = mn;
-  }
+    return ((int64_t)checked_block(table[j / a.page], a.num_blocks) * a.hkv + kvh) * a.page + j % a.page;
+  }, o, m, l);
   __shared__ float s_m[4], s_l[4], s_o[4][256];
   if (lane == 0) {
     s_m[warp] = m;

@@ -149,6 +149,82 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
   }
 }
 
+// ---------------------------------------------------------------------------------------------------------------- a row by itself
+// By a warp: the softmax of one row over the keys first, first + step .. below end, in 32 bits; lane i holds the columns i, i + 32 .. .  Looks at no key
+// that is not its row's.  M: type of 16-bit pages; row_of(key): its row of the cache.
+template <typename T, typename M, int FMT, typename RowOf>
+__device__ __forceinline__ void row_softmax(const AttnArgs& a, int tok, int head, int first, int step, int end, RowOf row_of, float (&o)[8], float& m, float& l) {
+  const int lane = threadIdx.x & 31;
+  float q[8];
+  const T* qr = reinterpret_cast<const T*>(a.q) + (int64_t)tok * a.ldq + (int64_t)head * a.d;
+  m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    q[i] = lane + 32 * i < a.d ? to_f32(qr[lane + 32 * i]) : 0.f;
+    o[i] = 0.f;
+  }
+  for (int j = first; j < end; j += step) {
+    const int64_t r = row_of(j);
+    float x = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (lane + 32 * i < a.d) x = fmaf(q[i], page_value<M, FMT>(a.k, r * a.d + lane + 32 * i), x);
+    x = warp_sum(x) * a.scale_log2;
+    if constexpr (FMT == kScaled16) x *= a.tile_scales[r / 64].k_up;
+    else if constexpr (FMT != kF16Pages) x *= a.ks[r];
+    const float mn = fmaxf(m, x), al = m == mn ? 1.f : exp2f(m - mn), p = x == -INFINITY ? 0.f : exp2f(x - mn);
+    l = l * al + p;
+    float pv = p;
+    if constexpr (FMT == kScaled16) pv *= 1.f / a.tile_scales[r / 64].v_down;
+    else if constexpr (FMT != kF16Pages) pv *= a.vs[r];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      o[i] *= al;
+      if (lane + 32 * i < a.d) o[i] = fmaf(pv, page_value<M, FMT>(a.v, r * a.d + lane + 32 * i), o[i]);
+    }
+    m = mn;
+  }
+}
+
+// A product over a tile of keys brings a value that is not finite to every row (0 x NaN is NaN), those included that do not see its key.  So a row whose
+// result is not finite is looked at once more, by a warp: where a hidden key of its tiles, of `from` .. `to` without first .. last, has such a value, the row
+// is formed anew over first .. last alone.  Costs a look at the results of rows that do not see all keys of their tiles: 4 portions of 1000 tokens over 1800
+// take as long as before (values looked at as they come into shared memory: 188 -> 205 us); that the code is there at all, 23.8 -> 24.8 us for a step of
+// 64 sequences behind 4096.
+struct RowKeys {
+  const int* table;
+  int kvh, from, first, last, to;
+};
+__device__ __forceinline__ int64_t cache_row(const AttnArgs& a, const RowKeys& k, int key) {
+  return ((int64_t)checked_block(k.table[key / a.page], a.num_blocks) * a.hkv + k.kvh) * a.page + key % a.page;
+}
+template <typename M, int FMT>
+__device__ __noinline__ bool hidden_unfinite(const AttnArgs& a, const RowKeys& k) {
+  bool found = false;
+  for (int key = k.from; key <= k.to; ++key) {
+    if (key >= k.first && key <= k.last) continue;
+    const int64_t r = cache_row(a, k, key);
+    if constexpr (FMT == kInt8 || FMT == kE4M3) found = found || !(fabsf(a.vs[r]) < INFINITY);
+    for (int c = threadIdx.x & 31; c < a.d; c += 32) found = found || !(fabsf(page_value<M, FMT>(a.v, r * a.d + c)) < INFINITY);
+  }
+  return __any_sync(0xffffffffu, found);
+}
+// to `part` ([d], maximum, sum), or where that is null to the output
+template <typename T, typename M, int FMT>
+__device__ __noinline__ void row_anew(const AttnArgs& a, const RowKeys& k, int tok, int head, float* part) {
+  float o[8], m, l;
+  row_softmax<T, M, FMT>(a, tok, head, k.first, 1, k.last + 1, [&](int key) { return cache_row(a, k, key); }, o, m, l);
+  const int lane = threadIdx.x & 31;
+  T* out = reinterpret_cast<T*>(a.out) + (int64_t)tok * a.ldo + (int64_t)head * a.d;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (lane + 32 * i >= a.d) continue;
+    if (part != nullptr) part[lane + 32 * i] = o[i];
+    else out[lane + 32 * i] = from_f32<T>(k.last < k.first ? 0.f : o[i] / l);
+  }
+  if (part != nullptr && lane == 0) *reinterpret_cast<float2*>(part + a.d) = make_float2(m, l);
+}
+
 // Tiles of 64 keys in f16: code * scale / 2^E, E the exponent above the tile's largest scale, so that nothing leaves f16's range and a rounding is 2^-12 of
 // the number (2^-25 of the tile's largest scale at least).  What goes with a tile: 2^E of the keys, E and 2^-E of the values.
 struct TileScales {

@@ -60,7 +60,6 @@ struct FewArgs {
   int beside;          // wait for the kernel before at the end instead of at the start
 };
 
-template <int UNIT>
 __device__ __forceinline__ Seg segment(const AttnArgs& a, const FewArgs& f, int i) { return i < f.own ? own_segment(a, i) : group_segment(a, i - f.own); }
 template <int UNIT>
 __device__ __forceinline__ int units_of(const Seg& s) {
@@ -97,6 +96,20 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {   // 8 x 8 of 16-bi
 // differ by two, so that under the 128-byte swizzle (chunk ^ key & 7) no eight lanes meet in a bank, neither reading keys nor reading values.
 __device__ __forceinline__ int key_of(int i) { return (i & 1) ? ((i - 1) ^ 5) : i; }   // 0 5 2 7 4 1 6 3
 
+// Rows (bits of `rows`) of a list, or of its part (slot >= 0): formed anew over the keys from .. to that they see.
+template <typename T, int FMT, int D>
+__device__ __noinline__ void rows_anew(const AttnArgs& a, const PartArgs& pa, int own, int seg, int kvh, int from, int to, int slot, unsigned rows) {
+  const Seg s = seg < own ? own_segment(a, seg) : group_segment(a, seg - own);
+  const int group = a.hq / a.hkv;
+  for (; rows != 0; rows &= rows - 1) {
+    const int i = __ffs(rows) - 1, tok = s.row0 + i / group, head = kvh * group + i % group;
+    const int sq = seg < own ? seg : seq_of_row(a.cu, 0, a.num_seqs, tok), last = sq < 0 ? -1 : min(row_pos(a, sq, tok), min(to, s.hi - 1));
+    const RowKeys k = {s.table, kvh, from, max(from, s.lo), last, to};
+    float* whole = (seg < own ? pa.whole_own : pa.whole_group) + ((int64_t)tok * a.hq + head) * (D + kPad);
+    row_anew<T, T, FMT>(a, k, tok, head, slot >= 0 ? pa.slots + ((int64_t)slot * pa.rows + i) * (D + kPad) : a.groups == 0 ? nullptr : whole);
+  }
+}
+
 template <typename T, int FMT, int D, int NT>
 __global__ void __launch_bounds__(32 * kWarps, Few<FMT, D, NT>::MIN_CTAS)
 attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnArgs a,
@@ -124,9 +137,9 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   s_q += warp * NT * KS * 32 + lane;
 
   // this warp's run of the lists
-  for (int i = threadIdx.x; i < min(f.segs, kKept); i += 32 * kWarps) s_units[i] = units_of<UNIT>(segment<UNIT>(a, f, i));
+  for (int i = threadIdx.x; i < min(f.segs, kKept); i += 32 * kWarps) s_units[i] = units_of<UNIT>(segment(a, f, i));
   __syncthreads();
-  auto count = [&](int i) { return i < kKept ? s_units[i] : units_of<UNIT>(segment<UNIT>(a, f, i)); };
+  auto count = [&](int i) { return i < kKept ? s_units[i] : units_of<UNIT>(segment(a, f, i)); };
   // (the host has checked that all lists together are below 2^31)
   auto scan = [&](int b, int& n) {         // lists b .. b + 31: this lane's units, and those up to it
     n = b + lane < f.segs ? count(b + lane) : 0;
@@ -182,7 +195,7 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
       w.before += w.n;
       w.n = count(++w.seg);
     }
-    w.s = segment<UNIT>(a, f, w.seg);
+    w.s = segment(a, f, w.seg);
     const unsigned at = w.cur - w.before * a.hkv;
     w.kvh = at / w.n;
     w.u0 = at - w.kvh * w.n;
@@ -561,6 +574,7 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     }
 
     // ---- the list's result, or its part
+    unsigned anew = 0;                                 // rows whose result is not finite, perhaps by a value that they do not see (0 x NaN is NaN)
     const bool whole = u0 == 0 && u1 == n;
     const bool last = whole && a.groups == 0;          // the result itself
     const int slot = 2 * (int)me + (cur > begin ? 1 : 0);
@@ -580,7 +594,16 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 #pragma unroll
         for (int w = 4; w < 32; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
         const int i = nt * 8 + 2 * t + c;
-        if (i >= nrows) continue;
+        bool again = false;
+        if (FMT != kInt8 && all_pos < max_pos) {       // some row does not see keys that others see (int8: a hidden value is 0 x a number)
+          float unfinite = 0.f;                        // NaN where a result is not finite
+#pragma unroll
+          for (int k = 0; k < KS; ++k) unfinite = fmaf(o[nt][k][c], 0.f, fmaf(o[nt][k][c + 2], 0.f, unfinite));
+          const unsigned row = __reduce_or_sync(0xffffffffu, i < nrows && sum == sum && unfinite != 0.f ? 1u << i : 0u);
+          again = (row >> i & 1) != 0;
+          anew |= row;
+        }
+        if (i >= nrows || again) continue;
         // what l and O stand relative to
         const float ref = m[nt][c] - (FMT == kF16Pages ? kUp : 0.f);
         float back = 1.f, off = 0.f;
@@ -621,6 +644,7 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
           if (r == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(ref, sum);
         }
       }
+    if (FMT != kInt8 && anew != 0) rows_anew<T, FMT, D>(a, pa, f.own, seg, kvh, base + u0 * UNIT, base + u1 * UNIT - 1, whole ? -1 : slot, anew);
     cur += u1 - u0;
     if (cur < end) {
       z.cur = cur;

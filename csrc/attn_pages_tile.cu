@@ -111,9 +111,86 @@ __device__ __forceinline__ float exp2_fma(float x) {
   return __int_as_float(__float_as_int(p) + ((__float_as_int(t) - 0x4B400000) << 23));
 }
 
+// what a block computes
+struct Block {
+  Seg s;
+  bool is_own;
+  int seg, kvh, split;      // list, key head, stretch of its keys
+  int n0, nrows;            // first row, rows of the list
+  int k_lo, k_hi;           // keys
+};
+// groups' lists first, since they are long, and of a list's rows the last first, since they see most
+template <int NQ>
+__device__ __forceinline__ Block block_of(const AttnArgs& a, const TileArgs& ta) {
+  Block b;
+  const int in_groups = ta.group_tiles * ta.group_splits * a.hkv * a.groups;      // (group_tiles 0: groups are not this launch's)
+  b.is_own = (int)blockIdx.x >= in_groups;
+  const int at = b.is_own ? blockIdx.x - in_groups : blockIdx.x;
+  const int tiles = b.is_own ? ta.own_tiles : ta.group_tiles, splits = b.is_own ? ta.own_splits : ta.group_splits;
+  const int chunk = b.is_own ? ta.own_chunk : ta.group_chunk;
+  const int part = at % (tiles * splits), list = at / (tiles * splits);
+  b.kvh = list % a.hkv, b.seg = list / a.hkv;
+  const int tile = tiles - 1 - part / splits;
+  b.split = part % splits;
+  b.s = b.is_own ? own_segment(a, b.seg) : group_segment(a, b.seg);
+  const int group = a.hq / a.hkv;
+  b.nrows = b.s.rows * group, b.n0 = tile * (NQ * BM);
+  int k_end = b.s.hi;
+  if (b.is_own && b.n0 < b.nrows) k_end = min(k_end, row_pos(a, b.seg, b.s.row0 + (min(b.nrows, b.n0 + NQ * BM) - 1) / group) + 1);
+  // stretch `split` of the list; the last one takes what lies behind it (lengths beyond the bounds the call gave)
+  b.k_lo = max(b.s.lo, b.s.lo + b.split * chunk);
+  b.k_hi = b.split == splits - 1 ? k_end : min(k_end, b.s.lo + (b.split + 1) * chunk);
+  return b;
+}
+
+// keys of row n of a block's list
+template <int NQ>
+__device__ __forceinline__ RowKeys keys_of(const AttnArgs& a, const Block& b, int n, int& tok, int& head) {
+  const int group = a.hq / a.hkv;
+  tok = b.s.row0 + n / group, head = b.kvh * group + n % group;
+  const int sq = b.is_own ? b.seg : seq_of_row(a.cu, 0, a.num_seqs, tok);
+  return {b.s.table, b.kvh, max(b.k_lo & ~(BN - 1), b.s.lo), b.k_lo, sq < 0 ? -1 : min(row_pos(a, sq, tok), b.k_hi - 1), b.k_hi - 1};
+}
+// By a softmax warp: of its rows (sums in tensor memory, a lane each) those whose result is not finite because of a hidden key.
+template <typename T, int FMT, int D, int NQ>
+__device__ __noinline__ unsigned spoiled_rows(const AttnArgs& a, const TileArgs& ta, uint32_t sums, bool mine) {
+  using M = typename std::conditional<Tile<FMT, D, NQ>::SCALED, __half, T>::type;
+  float x[4] = {0.f, 0.f, 0.f, 0.f};                     // NaN where a sum is not finite
+#pragma unroll 1
+  for (int c = 0; c < D; c += 32) {
+    uint32_t r[32];
+    tmem_ld_32x32b_x32(sums + c, r);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+      ffma2(x[0], x[1], __uint_as_float(r[i]), __uint_as_float(r[i + 1]), 0.f, 0.f, x[0], x[1]);
+      ffma2(x[2], x[3], __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]), 0.f, 0.f, x[2], x[3]);
+    }
+  }
+  unsigned spoiled = 0, rows = __ballot_sync(0xffffffffu, mine && (x[0] + x[1]) + (x[2] + x[3]) != 0.f);
+  if (rows == 0) return 0;
+  const Block b = block_of<NQ>(a, ta);
+  for (; rows != 0; rows &= rows - 1) {
+    int tok, head;
+    if (hidden_unfinite<M, FMT>(a, keys_of<NQ>(a, b, b.n0 + (threadIdx.x & ~31) + __ffs(rows) - 1, tok, head))) spoiled |= rows & (0u - rows);
+  }
+  return spoiled;
+}
+template <typename T, int FMT, int D, int NQ>
+__device__ __noinline__ void rows_anew(const AttnArgs& a, const PartArgs& pa, const TileArgs& ta, unsigned rows) {
+  using M = typename std::conditional<Tile<FMT, D, NQ>::SCALED, __half, T>::type;
+  const Block b = block_of<NQ>(a, ta);
+  for (; rows != 0; rows &= rows - 1) {
+    int tok, head;
+    const RowKeys k = keys_of<NQ>(a, b, b.n0 + (threadIdx.x & ~31) + __ffs(rows) - 1, tok, head);
+    float* part = (b.is_own ? pa.tile_own : pa.tile_group) + (((int64_t)b.split * a.total_q + tok) * a.hq + head) * (D + kPad);
+    row_anew<T, M, FMT>(a, k, tok, head, ta.direct ? nullptr : part);
+  }
+}
+
 template <typename T, int FMT, int D, int NQ>
 __global__ void __maxnreg__((Tile<FMT, D, NQ>::REGS))
-attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnArgs a, const __grid_constant__ PartArgs pa, const TileArgs ta) {
+attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnArgs a, const __grid_constant__ PartArgs pa, const __grid_constant__ TileArgs ta) {
   using C = Tile<FMT, D, NQ>;
   using M = typename std::conditional<C::SCALED, __half, T>::type;   // type of the products
   constexpr int DSUB = D / 64;
@@ -146,24 +223,12 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   // behind the wait: the kernel for few rows starts beside this one without a wait of its own, and reads what the kernels before this one wrote
   pdl_launch_dependents();
 
-  // the block's list, rows and keys: groups' lists first, since they are long, and of a list's rows the last first, since they see most
-  const int in_groups = ta.group_tiles * ta.group_splits * a.hkv * a.groups;      // (group_tiles 0: groups are not this launch's)
-  const bool is_own = (int)blockIdx.x >= in_groups;
-  const int at = is_own ? blockIdx.x - in_groups : blockIdx.x;
-  const int tiles = is_own ? ta.own_tiles : ta.group_tiles, splits = is_own ? ta.own_splits : ta.group_splits;
-  const int chunk = is_own ? ta.own_chunk : ta.group_chunk;
-  const int part = at % (tiles * splits), list = at / (tiles * splits), kvh = list % a.hkv, seg = list / a.hkv;
-  const int tile = tiles - 1 - part / splits, split = part % splits;
-  const Seg s = is_own ? own_segment(a, seg) : group_segment(a, seg);
+  const Block blk = block_of<NQ>(a, ta);
+  const Seg s = blk.s;
+  const bool is_own = blk.is_own;
+  const int seg = blk.seg, kvh = blk.kvh, split = blk.split, n0 = blk.n0, nrows = blk.nrows, k_lo = blk.k_lo, k_hi = blk.k_hi;
   const int group = a.hq / a.hkv;
-  const int nrows = s.rows * group, n0 = tile * (NQ * BM);
   if (n0 >= nrows) return;
-  const int n_last = min(nrows, n0 + NQ * BM) - 1;
-  int k_end = s.hi;
-  if (is_own) k_end = min(k_end, row_pos(a, seg, s.row0 + n_last / group) + 1);
-  // stretch `split` of the list; the last one takes what lies behind it (lengths beyond the bounds the call gave)
-  const int k_lo = max(s.lo, s.lo + split * chunk);
-  const int k_hi = split == splits - 1 ? k_end : min(k_end, s.lo + (split + 1) * chunk);
   const int base = k_lo & ~(BN - 1);
   const int n_tiles = __shfl_sync(0xffffffffu, k_hi > k_lo ? (k_hi - base + BN - 1) / BN : 0, 0);
 
@@ -455,6 +520,7 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     float m_run = -INFINITY, l_run = 0.f;
     // sums are of probabilities times 2^up: with scales, less the exponent of the values' largest so far
     float up = C::SCALED ? INFINITY : kUp;
+    bool partly = false;                                  // some row of the warp does not see some key of its tiles
     bool bad = false;                                     // a score of the row is NaN: so is the result, whatever the exponentials made of it
     for (int j = 0; j < n_tiles; ++j) {
       const int b = j & 1, kb = base + j * BN;
@@ -479,6 +545,7 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       }
       const int hi = pos - kb, lo = k_lo - kb;
       if (__any_sync(0xffffffffu, hi < BN - 1 || lo > 0)) {
+        partly = true;
 #pragma unroll
         for (int i = 0; i < BN; ++i)
           if (i > hi || i < lo) sc[i] = -INFINITY;
@@ -575,7 +642,9 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       }
     }
     uint8_t* to = nullptr;
-    if (live) {
+    // (out of line: what a block runs once comes cold from memory)
+    const unsigned anew = partly ? spoiled_rows<T, FMT, D, NQ>(a, ta, t_o(q) + off, live && !bad) : 0u;
+    if (live && (anew >> lane & 1) == 0) {
       if (ta.direct) {
         to = reinterpret_cast<uint8_t*>(reinterpret_cast<T*>(a.out) + (int64_t)tok * a.ldo + (int64_t)head * D);
       } else {
@@ -602,6 +671,7 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     };
     if (ta.direct) rows_out(std::integral_constant<int, D * 2>{});
     else rows_out(std::integral_constant<int, D * 4>{});
+    if (anew != 0) rows_anew<T, FMT, D, NQ>(a, pa, ta, anew);
   }
 
   tcgen05_fence_before();

@@ -178,7 +178,11 @@ def attention_pages(q, k_pages, v_pages, batch, scale: float):
         k, v = (x.repeat_interleave(hq // hkv, dim=0) for x in kv)
         s = torch.matmul(q[q0:q1].float().transpose(0, 1), k.transpose(1, 2)) * scale
         hidden = torch.arange(L, device=q.device) > torch.arange(L - (q1 - q0), L, device=q.device)[:, None]
-        o = torch.matmul(torch.softmax(s.masked_fill(hidden, float("-inf")), dim=-1), v)
+        p = torch.softmax(s.masked_fill(hidden, float("-inf")), dim=-1)
+        bad = ~torch.isfinite(v)
+        o = torch.matmul(p, v.masked_fill(bad, 0))
+        for key in bad.any(-1).any(0).nonzero().flatten().tolist():      # to the rows that see the key alone: 0 x NaN is NaN
+            o[:, max(0, key - (L - (q1 - q0))):] += v[:, key:key + 1].masked_fill(~bad[:, key:key + 1], 0)
         o[:, :max(0, q1 - q0 - L)] = 0                      # rows in front of the sequence's first token see nothing
         out[q0:q1] = o.transpose(0, 1).to(q.dtype)
     return out

@@ -4,6 +4,7 @@ import torch
 
 from llmss_b200 import ops
 from llmss_b200.engine.batch import SharedPrefix
+from llmss_b200.ops.pages import QuantPages
 from pages_bounds import expected
 from pages_oracle import make_batch, make_pages
 
@@ -78,6 +79,54 @@ HIDDEN = {
     "few_rows_behind_a_prefix": ([3, 1], [70, 80], 64, [([0, 1], 64)], (0, 1)),
     "portions_behind_a_prefix": ([70, 21], [70, 80], 64, [([0, 1], 64)], (0, 30)),
 }
+
+
+def _spoil(pages, table, page, pos, head, column, filler):
+    """Token ``pos`` of one key head is ``filler`` at one column (16-bit pages), or its scale is."""
+    b, o = table[pos // page], pos % page
+    if isinstance(pages, QuantPages):
+        pages.scale[b, head, o] = filler
+    else:
+        pages[b, head, o, column] = filler
+
+
+@pytest.mark.parametrize("kind,dtype", [(None, BF), (None, HF), (I8, BF), (E4, HF)])
+@pytest.mark.parametrize("filler", [NAN, INF])
+@pytest.mark.parametrize("hq,hkv,d", [(4, 2, 64), (8, 2, 128), (12, 2, 256), (6, 2, 96)])
+@pytest.mark.parametrize("case", sorted(HIDDEN))
+def test_rows_before_a_token_do_not_see_its_values(case, hq, hkv, d, filler, kind, dtype):
+    new, ctx, page, groups, (seq, tok) = HIDDEN[case]
+    batch, seen = make_batch(new, ctx, page, groups, "cuda", seed=5)
+    if kind is None and not groups:
+        batch.prefix = nothing_shared(len(new))
+    k, v = (make_pages(seen.blocks, hkv, page, d, kind, dtype, "cuda", seed=i) for i in range(2))
+    q = queries(sum(new), hq * d, dtype)
+    want, tol, _ = expected(q, k, v, batch, seen, hq, hkv, d, d ** -0.5)
+    column = d // 2 + 3
+    for pages in (v, k):
+        _spoil(pages, seen.tables[seq], page, ctx[seq] + tok, 1, column, filler)
+        out = ops.attention(q, torch.full_like(q, 7.0), batch, k, v, hq, hkv, d, d ** -0.5, 0, 0, 0)
+        over = q.clone()                                        # and over its own queries
+        ops.attention(over, over, batch, k, v, hq, hkv, d, d ** -0.5, 0, 0, 0)
+        assert ((over == out) | (torch.isnan(over) & torch.isnan(out))).all()
+        row = sum(new[:seq]) + tok                              # the first row that sees the token
+        after = slice(row, sum(new[:seq + 1]))
+        sees = torch.zeros(sum(new), hq, d, dtype=torch.bool, device="cuda")
+        if pages is k or kind is not None:
+            sees[after, hq // 2:] = True                        # a score, or every value of the token
+        else:
+            sees[after, hq // 2:, column] = True
+        sees = sees.view(sum(new), -1)
+        off = (out.double() - want).abs()
+        assert (off <= tol)[~sees].all(), f"{int((~(off <= tol))[~sees].sum())} results that do not see it changed"
+        got = out.float()[sees]
+        if filler != filler:
+            assert torch.isnan(got).all()
+        elif pages is v:                                        # a code of 0 times infinity is NaN
+            assert (got == INF).all() if kind is None else not torch.isfinite(got).any()
+        if pages is v:
+            _spoil(v, seen.tables[seq], page, ctx[seq] + tok, 1, column, 0.5)
+            want, tol, _ = expected(q, k, v, batch, seen, hq, hkv, d, d ** -0.5)
 
 
 @pytest.mark.parametrize("hq,hkv,d", [(4, 2, 64), (8, 2, 128), (12, 2, 256)])
