@@ -140,9 +140,9 @@ def attention(qkv, out, batch, k_cache, v_cache, hq, hkv, d, scale, q_off, k_off
         if _cuda(qkv):
             cu.attention_pages(qkv, out, batch, k_cache, v_cache, hq, hkv, d, scale, q_off, out_off)
         else:
-            n = int(batch.cu_q[-1])
-            out[:n, out_off:out_off + hq * d] = ref.attention_pages(qkv[:n, q_off:q_off + hq * d].reshape(n, hq, d), k_cache, v_cache, batch,
-                                                                    scale).reshape(n, hq * d)
+            lo, hi = int(batch.cu_q[0]), int(batch.cu_q[batch.num_seqs])
+            o = ref.attention_pages(qkv[:, q_off:q_off + hq * d].reshape(-1, hq, d), k_cache, v_cache, batch, scale)
+            out[lo:hi, out_off:out_off + hq * d] = o[lo:hi].reshape(-1, hq * d)
         return out
     T = qkv.shape[0]
     q_view = qkv[:, q_off:q_off + hq * d]

@@ -154,10 +154,10 @@ def attention_pages(q, k_pages, v_pages, batch, scale: float):
     T, hq, d = q.shape
     hkv, bs = k_pages.shape[1], k_pages.shape[2]
     out = torch.zeros(T, hq, d, dtype=q.dtype, device=q.device)
-    cu, lens = batch.cu_q.tolist(), batch.seq_lens.tolist()
+    cu, lens = batch.cu_q.tolist(), batch.seq_lens.tolist()[:batch.num_seqs]        # the tensors may be longer, as a step's buffers are
     shared = [(0, 0)] * len(lens)
     if batch.prefix is not None:
-        first, n = batch.prefix.first.tolist(), batch.prefix.lens.tolist()
+        first, n = [min(i, len(lens)) for i in batch.prefix.first.tolist()], batch.prefix.lens.tolist()
         for j in range(batch.prefix.num_groups):
             shared[first[j]:first[j + 1]] = [(j, n[j])] * (first[j + 1] - first[j])
 

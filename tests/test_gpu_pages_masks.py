@@ -170,3 +170,21 @@ def test_keys_that_are_infinite(hq, hkv, d, new, ctx, groups, dtype):
         kk[(seen.fronts[0] if groups and p < 64 else seen.tables[0])[p // 64], 1, p % 64, 5] = INF
     out = ops.attention(q, torch.empty_like(q), batch, kk, v, hq, hkv, d, d ** -0.5, 0, 0, 0).float().view(-1, hq, d)
     assert torch.isnan(out[:a, hq // 2:]).all() and torch.isfinite(out[:a, :hq // 2]).all()
+
+
+@pytest.mark.parametrize("kind", [None, I8, E4])
+@pytest.mark.parametrize("new", [[1, 1, 1], [3, 1, 2], [40, 1, 30]])
+def test_buffers_longer_than_the_batch_and_rows_of_no_sequence(new, kind):
+    """As the plain form on the CPU has it."""
+    hq, hkv, d = 8, 2, 128
+    batch, seen = make_batch(new, [90, 70, 64], 64, [([0, 1], 64)], "cuda", seed=1)
+    k, v = (make_pages(seen.blocks, hkv, 64, d, kind, BF, "cuda", seed=i) for i in range(2))
+    T = sum(new)
+    q = queries(T + 5, hq * d, BF)
+    want, tol, _ = expected(q[2:2 + T], k, v, batch, seen, hq, hkv, d, d ** -0.5)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    batch.cu_q = torch.cat([batch.cu_q + 2, torch.tensor([T + 4, 0], **i32)])
+    batch.seq_lens = torch.cat([batch.seq_lens, torch.tensor([7, 7], **i32)])
+    batch.block_tables = torch.cat([batch.block_tables, batch.block_tables[:2]])
+    out = ops.attention(q, torch.full_like(q, 7.0), batch, k, v, hq, hkv, d, d ** -0.5, 0, 0, 0)
+    assert ((out[2:2 + T].double() - want).abs() <= tol).all() and (out[:2] == 7).all() and (out[2 + T:] == 7).all()

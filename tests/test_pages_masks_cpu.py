@@ -24,3 +24,17 @@ def test_rows_before_a_token_do_not_see_its_values(kind, filler):
     sees[tok:9, 2:, column if kind is None else slice(None)] = True
     sees = sees.view(13, -1)
     assert ((out.double() - want).abs()[~sees] < 1e-5).all() and not torch.isfinite(out[sees]).any()
+
+
+def test_buffers_longer_than_the_batch_and_rows_of_no_sequence():
+    """A step's buffers hold more sequences than it has; rows in front of the first sequence and behind the last stay as they are."""
+    hq, hkv, d, page = 4, 2, 32, 16
+    batch, seen = make_batch([3, 1, 2], [20, 40, 33], page, [([0, 1], 16)], "cpu", seed=1)
+    k, v = (make_pages(seen.blocks, hkv, page, d, torch.int8, torch.float32, "cpu", seed=i) for i in range(2))
+    q = torch.randn(9, hq * d, generator=torch.Generator().manual_seed(2))
+    want = attend64(q[2:8], k, v, batch, seen, hq, hkv, d, 0.2)
+    batch.cu_q = torch.cat([batch.cu_q + 2, torch.tensor([99, 0], dtype=torch.int32)])
+    batch.seq_lens = torch.cat([batch.seq_lens, torch.tensor([7, 7], dtype=torch.int32)])
+    batch.block_tables = torch.cat([batch.block_tables, batch.block_tables[:2]])
+    out = ops.attention(q, torch.full_like(q, 7.0), batch, k, v, hq, hkv, d, 0.2, 0, 0, 0)
+    assert (out[2:8].double() - want).abs().max() < 1e-5 and (out[:2] == 7).all() and (out[8:] == 7).all()
