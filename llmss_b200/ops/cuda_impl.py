@@ -327,7 +327,11 @@ def rope_kv_write_q8(qkv, positions, slot_mapping, k_pages, v_pages, hq, hkv, d,
     if dev != torch._C._cuda_getDevice():       # launches go to the current device's stream
         with torch.cuda.device(dev):
             return rope_kv_write_q8(qkv, positions, slot_mapping, k_pages, v_pages, hq, hkv, d, rotary_dim, style, base, q_off, k_off, v_off)
-    T, _, ld = _rows2d(qkv)
+    T, wide, ld = _rows2d(qkv)
+    if type(v_pages) is not QuantPages:
+        raise ValueError(f"rope_kv_write: keys in 8-bit pages and values in {type(v_pages).__name__}: QuantPages both")
+    if max(q_off + hq * d, k_off + hkv * d, v_off + hkv * d) > wide:        # the stride of a view may be longer than its rows, and end behind its memory
+        raise _lib.KernelError(f"rope_kv_write: q/k/v column ranges at {q_off}, {k_off}, {v_off} of {hq} and {hkv} heads of {d} exceed the {wide} columns")
     k, v = k_pages.data, v_pages.data
     shape, dtype = k.shape, k.dtype
     if shape != v.shape or dtype is not v.dtype or shape[1] != hkv or shape[3] != d or k.get_device() != dev or v.get_device() != dev:
@@ -361,7 +365,7 @@ def attention_pages(qkv, out, batch, k_pages, v_pages, hq, hkv, d, scale, q_off=
         fmt = FORMATS[k.dtype]
     else:
         k, v, ks, vs, fmt = k_pages, v_pages, None, None, 0
-        if k.dtype is not dtype or not (k.is_contiguous() and v.is_contiguous()):
+        if type(v) is QuantPages or k.dtype is not dtype or not (k.is_contiguous() and v.is_contiguous()):
             raise ValueError(f"attention: contiguous pages of the queries' type, or QuantPages both, got {k.dtype} and {v.dtype} for {dtype}")
     shape = k.shape
     if shape != v.shape or k.dtype is not v.dtype or len(shape) != 4 or shape[1] != hkv or shape[3] != d or k.get_device() != dev or v.get_device() != dev:

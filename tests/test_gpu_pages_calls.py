@@ -1,0 +1,27 @@
+"""8-bit cache pages and shared prefixes on the GPU: calls that are refused before anything is launched, and counts of what is."""
+import pytest
+import torch
+
+from llmss_b200 import ops
+from llmss_b200.ops._lib import KernelError
+from llmss_b200.ops.pages import QuantPages
+from pages_oracle import make_batch, make_pages
+
+pytestmark = pytest.mark.gpu
+
+BF = torch.bfloat16
+I8 = torch.int8
+
+
+def test_write_refuses_columns_behind_a_views_rows():
+    """The stride of a view may be longer than its rows: what follows the last one is not the caller's."""
+    hq, hkv, d = 4, 2, 64
+    whole = torch.zeros(3, 1024, dtype=BF, device="cuda")
+    k, v = (QuantPages(torch.zeros(2, hkv, 16, d, dtype=I8, device="cuda"), torch.zeros(2, hkv, 16, device="cuda")) for _ in range(2))
+    pos = torch.arange(3, dtype=torch.int32, device="cuda")
+    ops.rope_kv_write(whole[:, 512:], pos, pos, k, v, hq, hkv, d, 0, ops.ROPE_NONE, 1e4, 0, 256, 384)
+    for offsets in ((0, 256, 448), (320, 0, 128), (0, 464, 256)):
+        with pytest.raises(KernelError, match="column ranges"):
+            ops.rope_kv_write(whole[:, 512:], pos, pos, k, v, hq, hkv, d, 0, ops.ROPE_NONE, 1e4, *offsets)
+    with pytest.raises(ValueError, match="QuantPages both"):
+        ops.rope_kv_write(whole, pos, pos, k, v.data, hq, hkv, d, 0, ops.ROPE_NONE, 1e4, 0, 256, 384)
