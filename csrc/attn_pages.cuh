@@ -114,7 +114,7 @@ __device__ __forceinline__ Seg own_segment(const AttnArgs& a, int i) {
   s.row0 = row_of(a, i);
   s.rows = row_of(a, i + 1) - s.row0;
   s.hi = min(a.seq_lens[i], a.max_blocks * a.page);
-  s.lo = g < 0 ? 0 : min(a.g_lens[g], a.g_max_blocks * a.page);
+  s.lo = g < 0 ? 0 : max(0, min(a.g_lens[g], a.g_max_blocks * a.page));
   s.table = a.tables + (int64_t)i * a.max_blocks;
   return s;
 }

@@ -25,3 +25,18 @@ def test_write_refuses_columns_behind_a_views_rows():
             ops.rope_kv_write(whole[:, 512:], pos, pos, k, v, hq, hkv, d, 0, ops.ROPE_NONE, 1e4, *offsets)
     with pytest.raises(ValueError, match="QuantPages both"):
         ops.rope_kv_write(whole, pos, pos, k, v.data, hq, hkv, d, 0, ops.ROPE_NONE, 1e4, 0, 256, 384)
+
+
+@pytest.mark.parametrize("kind", [None, I8])
+@pytest.mark.parametrize("new", [[1, 1, 1], [30, 2, 41]])
+def test_a_negative_length_shares_nothing(kind, new):
+    """Lengths lie in device memory, where no call can look at them: a wrong one is a wrong result at most."""
+    hq, hkv, d = 8, 2, 128
+    batch, seen = make_batch(new, [90, 70, 64], 64, [([0, 1], 64)], "cuda", seed=1)
+    k, v = (make_pages(seen.blocks, hkv, 64, d, kind, BF, "cuda", seed=i) for i in range(2))
+    q = torch.randn(sum(new), hq * d, device="cuda").to(BF)
+    outs = []
+    for n in (0, -64, -5):
+        batch.prefix.lens[0] = n
+        outs.append(ops.attention(q, torch.empty_like(q), batch, k, v, hq, hkv, d, 0.1, 0, 0, 0))
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2]) and torch.isfinite(outs[0].float()).all()
