@@ -347,8 +347,6 @@ def rope_kv_write_q8(qkv, positions, slot_mapping, k_pages, v_pages, hq, hkv, d,
     _count()
 
 
-_LAUNCHED = C.c_int(0)                     # kernels of the last call
-_LAUNCHED_AT = C.addressof(_LAUNCHED)
 _NO_GROUPS = (None, 0, None, None, 0, 0, 0)
 
 
@@ -376,6 +374,7 @@ def attention_pages(qkv, out, batch, k_pages, v_pages, hq, hkv, d, scale, q_off=
             or q_off < 0 or out_off < 0 or q_off + hq * d > wide or out_off + hq * d > out_wide:
         raise TypeError(f"attention: float16 or bfloat16 queries and an output like them, {hq} heads of {d}, got {dtype} {tuple(qkv.shape)} and "
                         f"{out.dtype} {tuple(out.shape)}")
+    q_at, out_at = qkv.data_ptr() + 2 * q_off, out.data_ptr() + 2 * out_off
     bt, sl, cu_q = batch.block_tables, batch.seq_lens, batch.cu_q
     if _wrong_ints(dev, bt, sl, cu_q) or bt.shape[0] < B or sl.numel() < B or cu_q.numel() < B + 1:
         raise ValueError(f"attention: block_tables, seq_lens and cu_q are contiguous int32 on {qkv.device}, of {B} sequences or more")
@@ -389,11 +388,12 @@ def attention_pages(qkv, out, batch, k_pages, v_pages, hq, hkv, d, scale, q_off=
     floats = lib.llmss_attn_pages_scratch_floats(B, batch.max_q, batch.max_kv, T, hq, hkv, d, shape[2], fmt, g[4], g[5], g[6])
     # a scratch of the call's own: two streams, or two captured graphs, never meet in it
     scratch = torch.empty(floats, dtype=torch.float32, device=qkv.device) if floats else None
-    rc = lib.llmss_attn_pages(qkv.data_ptr() + 2 * q_off, ldq, k.data_ptr(), ks, v.data_ptr(), vs, bt.data_ptr(), bt.shape[1], sl.data_ptr(),
-                              out.data_ptr() + 2 * out_off, ldo, cu_q.data_ptr(), B, batch.max_q, batch.max_kv, T, hq, hkv, d, shape[2], shape[0],
-                              float(scale), fmt, _DT[dtype], *g, None if scratch is None else scratch.data_ptr(), floats, _LAUNCHED_AT, _stream())
+    launched = C.c_int(0)
+    rc = lib.llmss_attn_pages(q_at, ldq, k.data_ptr(), ks, v.data_ptr(), vs, bt.data_ptr(), bt.shape[1], sl.data_ptr(),
+                              out_at, ldo, cu_q.data_ptr(), B, batch.max_q, batch.max_kv, T, hq, hkv, d, shape[2], shape[0],
+                              float(scale), fmt, _DT[dtype], *g, None if scratch is None else scratch.data_ptr(), floats, C.addressof(launched), _stream())
     _lib.check(rc, "llmss_attn_pages")
-    _count(_LAUNCHED.value)
+    _count(launched.value)
 
 
 # --------------------------------------------------------------------------- embed / sample
