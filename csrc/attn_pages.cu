@@ -421,7 +421,7 @@ LLMSS_API int64_t llmss_attn_pages_scratch_floats(int num_seqs, int max_q, int m
 // q [total_q][>= hq * d] (row stride ldq); K / V pages [num_blocks][hkv][block_size][d] of the queries' type (fmt 0) or of bytes with 32-bit scales
 // [num_blocks][hkv][block_size] (fmt 1 int8, 2 e4m3); sequence i owns the rows cu_q[i] .. cu_q[i + 1] - 1, the last positions of its seq_lens[i] cached
 // tokens.  groups > 0: the sequences g_first[j] .. g_first[j + 1] - 1 find their first g_lens[j] tokens in the pages g_tables[j].  max_q, max_kv,
-// g_max_len, g_max_rows bound the lengths.  *launches: kernels launched (null: not wanted).  out may alias q.  Rows of sequences without a visible key become zero; rows of no sequence stay as they are.
+// g_max_len, g_max_rows bound the lengths.  *launches: kernels launched (null: not wanted).  out is q itself or shares no memory with it.  Rows of sequences without a visible key become zero; rows of no sequence stay as they are.
 LLMSS_API int llmss_attn_pages(const void* q, int64_t ldq, const void* k_pages, const float* k_scale, const void* v_pages, const float* v_scale,
                                const int* block_tables, int max_blocks, const int* seq_lens, void* out, int64_t ldo, const int* cu_q, int num_seqs,
                                int max_q, int max_kv, int total_q, int hq, int hkv, int d, int block_size, int num_blocks, float scale, int fmt,

@@ -545,7 +545,7 @@ int llmss_rope_kv_write_q8(void* qkv, const int* positions, const int* slot_mapp
 /* Causal attention over pages in the queries' 16-bit type (fmt 0, no scales) or in 8 bits.  groups > 0: the sequences g_first[j] .. g_first[j + 1] - 1
  * find their first g_lens[j] tokens in the pages g_tables[j], which are read once per group; g_max_len and g_max_rows bound g_lens and the query rows
  * of a group.  scratch: llmss_attn_pages_scratch_floats of the same sizes, 16-byte aligned.  *launches: kernels launched (host; null: not wanted).  A row without a visible key becomes zero; a
- * value that is not finite reaches the rows that see its key, no others; out may alias q. */
+ * value that is not finite reaches the rows that see its key, no others; out is q itself or shares no memory with it. */
 int64_t llmss_attn_pages_scratch_floats(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv, int d, int block_size, int fmt,
                                         int groups, int g_max_len, int g_max_rows);
 int llmss_attn_pages(const void* q, int64_t ldq, const void* k_pages, const float* k_scale, const void* v_pages, const float* v_scale,

@@ -135,6 +135,7 @@ def attention(qkv, out, batch, k_cache, v_cache, hq, hkv, d, scale, q_off, k_off
     prompt was cut into portions).  ``batch.prefix``: tokens that groups of sequences share are read once per group, from pages of either
     kind.  Both take any mix of lengths; rows without a visible key become zero, rows of no sequence stay as they are, and keys that a row
     does not see never reach it, whatever lies there.
+    The output's columns are those of the queries or share no memory with them.
     """
     if batch.prefix is not None or isinstance(k_cache, QuantPages):
         if _cuda(qkv):

@@ -352,7 +352,7 @@ _NO_GROUPS = (None, 0, None, None, 0, 0, 0)
 
 def attention_pages(qkv, out, batch, k_pages, v_pages, hq, hkv, d, scale, q_off=0, out_off=0):
     """Attention over 8-bit pages, and over pages of either kind that groups of sequences share (``batch.prefix``): queries are the columns
-    q_off .. of ``qkv``, results the columns out_off .. of ``out``."""
+    q_off .. of ``qkv``, results the columns out_off .. of ``out``.  They may be the very same columns, and else share no memory."""
     dev = qkv.get_device()
     if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
@@ -375,6 +375,9 @@ def attention_pages(qkv, out, batch, k_pages, v_pages, hq, hkv, d, scale, q_off=
         raise TypeError(f"attention: float16 or bfloat16 queries and an output like them, {hq} heads of {d}, got {dtype} {tuple(qkv.shape)} and "
                         f"{out.dtype} {tuple(out.shape)}")
     q_at, out_at = qkv.data_ptr() + 2 * q_off, out.data_ptr() + 2 * out_off
+    if (q_at != out_at or (ldq != ldo and T > 1)) and out_at < q_at + 2 * ((T - 1) * ldq + hq * d) and q_at < out_at + 2 * ((T - 1) * ldo + hq * d) \
+            and not (ldq == ldo and hq * d <= (out_at - q_at) // 2 % ldq <= ldq - hq * d):
+        raise ValueError("attention: the output overlaps the queries without being them: lists of keys are worked on at once")
     bt, sl, cu_q = batch.block_tables, batch.seq_lens, batch.cu_q
     if _wrong_ints(dev, bt, sl, cu_q) or bt.shape[0] < B or sl.numel() < B or cu_q.numel() < B + 1:
         raise ValueError(f"attention: block_tables, seq_lens and cu_q are contiguous int32 on {qkv.device}, of {B} sequences or more")

@@ -40,3 +40,28 @@ def test_a_negative_length_shares_nothing(kind, new):
         batch.prefix.lens[0] = n
         outs.append(ops.attention(q, torch.empty_like(q), batch, k, v, hq, hkv, d, 0.1, 0, 0, 0))
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2]) and torch.isfinite(outs[0].float()).all()
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [30, 2, 41]])
+def test_an_output_that_overlaps_the_queries_is_refused(new):
+    """Lists of keys are worked on at once, so that one would write what another still reads.  The queries' own columns and columns beside them are fine."""
+    hq, hkv, d = 8, 2, 64
+    batch, seen = make_batch(new, [90, 70, 64], 64, [], "cuda", seed=1)
+    k, v = (make_pages(seen.blocks, hkv, 64, d, I8, BF, "cuda", seed=i) for i in range(2))
+    T, w = sum(new), hq * d
+    x = torch.randn(T + 4, 3 * w, device="cuda").to(BF)
+    call = lambda q, out, q_off, out_off: ops.attention(q, out, batch, k, v, hq, hkv, d, 0.1, q_off, 0, 0, out_off=out_off)
+    want = call(x.clone()[:T], torch.empty(T, w, dtype=BF, device="cuda"), w, 0)
+    for out_off in (w - 64, w + 8, 2 * w - 8):
+        with pytest.raises(ValueError, match="overlaps"):
+            call(x[:T], x[:T], w, out_off)
+    with pytest.raises(ValueError, match="overlaps"):
+        call(x[:T], x[1:T + 1], w, w)                                       # a row further
+    with pytest.raises(ValueError, match="overlaps"):
+        call(x[:T], x.view(-1)[w:].as_strided((T, w), (w, 1)), w, 0)        # rows of another stride
+    for out_off in (0, 2 * w, w):
+        y = x.clone()
+        got = call(y[:T], y[:T], w, out_off)
+        assert torch.equal(got[:, out_off:out_off + w], want)
+    y = x.clone()
+    assert torch.equal(call(y[:T, w:], y[:T, :w], 0, 0), want)               # views of one tensor, side by side
