@@ -27,6 +27,7 @@ from .kv_cache import BlockAllocator, SlotAllocator
 
 _BUCKETS = (1, 2, 4, 8, 16, 24, 32, 48, 64, 96, 128, 192, 256)
 _MAX_GROUPS = 8                                                                        # prefixes of one step
+_MAX_PREFIX_GRAPHS = 32                                                                # captured steps with shared prefixes, those used last
 _SHARE_MIN_BYTES = int(os.environ.get("LLMSS_SHARE_MIN_BYTES", str(64 << 20)))      # reads per layer that sharing saves
 
 
@@ -143,7 +144,7 @@ class ModelRunner:
         self.cuda = self.device.type == "cuda"
         self.use_graph = self.cuda if use_cuda_graph is None else (use_cuda_graph and self.cuda)
         self.graphs: Dict[tuple, torch.cuda.CUDAGraph] = {}   # (padded batch, vocab-parallel greedy, bounds of shared prefixes) -> graph
-        self.launches_per_graph: Dict[int, int] = {}   # own-kernel launches captured per decode graph
+        self.launches_per_graph: Dict[object, int] = {}   # own-kernel launches captured per decode graph: by padded batch, or with its prefixes' bounds
         self._all_greedy = True
         self._vp_sampling_ok = True
         self._vp_plain_rows = False
@@ -635,12 +636,23 @@ class ModelRunner:
         self.tuning_log[Bp] = {"ctx": L, "us_per_call": table, "picked": best, "heuristic": base}
         return best
 
+    @staticmethod
+    def _launch_key(Bp: int, prefix):
+        return Bp if prefix is None else (Bp, prefix)
+
     def capture(self, Bp: int, vp: bool = False):
         """Warm up and capture the decode graph for a padded batch size, on inert inputs
         (slot -1, seq_len 0: no cache writes), then restore the live step state."""
         if not self.use_graph or (Bp, vp, self._prefix) in self.graphs:
             return
         splits = self._tuned_splits[Bp] if Bp in self._tuned_splits else self.autotune_decode_splits(Bp)
+        shared = [k for k in self.graphs if k[2] is not None]
+        if self._prefix is not None and len(shared) >= _MAX_PREFIX_GRAPHS:
+            torch.cuda.synchronize()             # steps are enqueued ahead: not while one is replayed
+            old = self.graphs.pop(shared[0])
+            old.reset()
+            if all(k[0] != shared[0][0] or k[2] != shared[0][2] for k in self.graphs):
+                self.launches_per_graph.pop(self._launch_key(shared[0][0], shared[0][2]), None)
         saved_in, saved_rng = self.d_in.clone(), self.d_rng.clone()
         inert = torch.zeros_like(self.h_in)
         MB = self.max_batch
@@ -663,7 +675,7 @@ class ModelRunner:
         n0 = _lib.LAUNCHES["count"]
         with torch.cuda.graph(g, pool=self.graph_pool):
             self._decode_body(Bp, splits, vp)
-        self.launches_per_graph[Bp] = _lib.LAUNCHES["count"] - n0
+        self.launches_per_graph[self._launch_key(Bp, self._prefix)] = _lib.LAUNCHES["count"] - n0
         if self.graph_pool is None:
             self.graph_pool = g.pool()
         self.graphs[(Bp, vp, self._prefix)] = g
@@ -676,7 +688,10 @@ class ModelRunner:
         if not self.use_graph:
             self._decode_body(Bp, self._splits_for(Bp), vp)
             return
-        self.graphs[(Bp, vp, self._prefix)].replay()
+        key = (Bp, vp, self._prefix)
+        if self._prefix is not None:
+            self.graphs[key] = self.graphs.pop(key)          # in the order of their last use
+        self.graphs[key].replay()
         self.stats["graph_replays"] += 1
 
     @torch.no_grad()
