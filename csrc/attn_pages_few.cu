@@ -66,11 +66,6 @@ __device__ __forceinline__ int units_of(const Seg& s) {
   return s.hi > s.lo && s.rows > 0 ? (s.hi - (s.lo & ~(UNIT - 1)) + UNIT - 1) / UNIT : 0;
 }
 
-__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t s) {
-  uint32_t r;
-  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(s));
-  return r;
-}
 // bytes 0 and 2 of w, two's complement, as f16 numbers below the normal range: the bits 0x00uu are u 2^-24, u = code + 128, without rounding
 __device__ __forceinline__ uint32_t int8_pair(uint32_t w) {
   uint32_t u;

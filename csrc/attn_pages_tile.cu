@@ -92,24 +92,8 @@ __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[
 }
 __device__ __forceinline__ void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ float max_nan(float a, float b) {   // NaN where one of them is
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-
-// 2^x without the MUFU pipe: x = n + r with r in [-0.5, 0.5], a cubic fitted to 2^r there (relative error 1.1e-4, below a rounding of the probability to
-// 16 bits), n added to the exponent.  At -127 r is 0 and the polynomial 1.0, whose exponent becomes that of zero: 0 for what is below (hidden keys weigh
-// nothing, however large their values), and for NaN
-__device__ __forceinline__ float exp2_fma(float x) {
-  x = fmaxf(x, -127.0f);
-  const float t = x + 12582912.0f;                 // 1.5 * 2^23: the integer part lands in the low bits
-  const float r = x - (t - 12582912.0f);
-  float p = fmaf(r, 0.05459282f, 0.24221784f);
-  p = fmaf(r, p, 0.6933686f);
-  p = fmaf(r, p, 1.0f);
-  return __int_as_float(__float_as_int(p) + ((__float_as_int(t) - 0x4B400000) << 23));
-}
+// 2^x without the MUFU pipe; 0 for what is below -127 (hidden keys weigh nothing, however large their values), and for NaN
+__device__ __forceinline__ float exp2_fma(float x) { return exp2_cubic(fmaxf(x, -127.0f)); }
 
 // what a block computes
 struct Block {

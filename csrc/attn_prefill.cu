@@ -146,20 +146,9 @@ __device__ __forceinline__ float ex2_approx(float x) {  // 2^x, one MUFU; 2^-inf
   return y;
 }
 
-// 2^x on the FMA pipe (no MUFU): round-to-nearest split x = n + r, r in [-0.5, 0.5], cubic for 2^r (relative error
-// 1.1e-4, far below the bf16 / fp16 rounding of P), exponent added into the float's bits.  A quarter of the
-// exponentials of the softmax go this way: at head_dim 128 / 64 the MUFU pipe (16 ex2 per clock and SM) needs as
-// many cycles per tile as the tensor pipe, so the two cannot both run at full rate unless some of the exps move.
-__device__ __forceinline__ float ex2_fma(float x) {
-  x = fmaxf(x, -125.0f);
-  const float t = x + 12582912.0f;                 // 1.5 * 2^23: the integer part lands in the low mantissa bits
-  const int n = __float_as_int(t) - 0x4B400000;
-  const float r = x - (t - 12582912.0f);
-  float p = fmaf(r, 0.05459282f, 0.24221784f);   // least-squares cubic on [-0.5, 0.5]: max relative error 1.1e-4
-  p = fmaf(r, p, 0.6933686f);
-  p = fmaf(r, p, 1.0f);
-  return __int_as_float(__float_as_int(p) + (n << 23));
-}
+// A quarter of the exponentials of the softmax go to the FMA pipe: at head_dim 128 / 64 the MUFU pipe (16 ex2 per clock and SM) needs as many cycles per
+// tile as the tensor pipe, so the two cannot both run at full rate unless some of the exps move.
+__device__ __forceinline__ float ex2_fma(float x) { return exp2_cubic(fmaxf(x, -125.0f)); }
 
 using namespace umma_lo;
 

@@ -308,6 +308,30 @@ __device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const void* map
       : "memory");
 }
 
+// ---------------------------------------------------------------- numbers
+// 2^x on the FMA pipe, for x in [-127, 128): round-to-nearest split x = n + r, r in [-0.5, 0.5], least-squares cubic for 2^r (relative error 1.1e-4, below
+// the rounding of a probability to 16 bits), n added into the float's exponent.  At -127 r is 0 and the cubic 1.0, so that the result is exactly 0.
+__device__ __forceinline__ float exp2_cubic(float x) {
+  const float t = x + 12582912.0f;                 // 1.5 * 2^23: the integer part lands in the low mantissa bits
+  const int n = __float_as_int(t) - 0x4B400000;
+  const float r = x - (t - 12582912.0f);
+  float p = fmaf(r, 0.05459282f, 0.24221784f);
+  p = fmaf(r, p, 0.6933686f);
+  p = fmaf(r, p, 1.0f);
+  return __int_as_float(__float_as_int(p) + (n << 23));
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {   // NaN where one of them is
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t s) {   // four bytes of eight
+  uint32_t r;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(s));
+  return r;
+}
+
 // ---------------------------------------------------------------- packed arithmetic
 // Packed fp32x2 arithmetic (one issue slot for two numbers): the softmax warps of the prompt-attention kernel are bound by
 // instruction issue (ncu: issue 50 %, tensor pipe 45 % before this), so the scale-and-shift, the row-sum and the soft cap run

@@ -37,16 +37,6 @@ struct QArgs {
   double turns[128];              // base^(-2 i / rotary_dim) / (2 pi)
 };
 
-__device__ __forceinline__ float max_nan(float a, float b) {   // NaN where one of them is
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t s) {
-  uint32_t r;
-  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(s));
-  return r;
-}
 
 // quotients x / scale, correctly rounded for scales of 2^-100 and more, r = 1 / scale
 __device__ __forceinline__ void quotients(float (&q)[8], const float (&x)[8], float scale, float r) {

@@ -39,14 +39,6 @@ class QuantPages:
     def dtype(self):
         return self.data.dtype
 
-    @property
-    def device(self):
-        return self.data.device
-
-    @property
-    def is_cuda(self):
-        return self.data.is_cuda
-
     def values(self, dtype=torch.float32) -> torch.Tensor:
         """The numbers that the codes stand for."""
         return (self.data.float() * self.scale[..., None]).to(dtype)
