@@ -49,3 +49,56 @@ def test_results_within_their_roundings(case, dtype, kind, q_scale):
     got = ops.attention(q, torch.full_like(q, float("nan")), batch, k, v, hq, hkv, d, scale, 0, 0, 0).double()
     off = (got - want).abs()
     assert (off <= tol).all(), f"off by {float(off.max()):.3g}; up to {float((off / tol).max()):.3g} times the bound, {int((off > tol).sum())} of {off.numel()}"
+
+
+@pytest.mark.parametrize("kind", [None, I8, E4])
+@pytest.mark.parametrize("new", [[1, 1, 1], [3, 1, 2], [150, 40, 1]])
+@pytest.mark.parametrize("page", [48, 80, 112, 144, 256, 5, 24])
+def test_pages_of_any_size(page, new, kind):
+    hq, hkv, d = 8, 2, 128
+    ctx = [700, page, 2 * page + 7]
+    batch, seen = make_batch(new, ctx, page, [([1, 2], page)] if kind is None or page % 3 else [], "cuda", seed=page)
+    k, v = (make_pages(seen.blocks, hkv, page, d, kind, BF, "cuda", seed=i) for i in range(2))
+    q = torch.randn(sum(new), hq * d, generator=torch.Generator().manual_seed(1)).to(BF).cuda()
+    want, tol, _ = expected(q, k, v, batch, seen, hq, hkv, d, d ** -0.5)
+    got = ops.attention(q, torch.full_like(q, float("nan")), batch, k, v, hq, hkv, d, d ** -0.5, 0, 0, 0).double()
+    assert ((got - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("kind", [None, I8])
+@pytest.mark.parametrize("tokens", [1, 20])
+def test_more_sequences_than_a_block_keeps_lengths_of(kind, tokens):
+    n, hq, hkv, d = 2500, 4, 2, 64
+    new = [tokens] * 3 + [1] * (n - 3)
+    groups = [(list(range(2 * i, 2 * i + 2)), 16) for i in range(n // 2)] if kind is None else []
+    batch, seen = make_batch(new, [16 + i * 7 % 50 for i in range(n)], 16, groups, "cuda", seed=1)
+    k, v = (make_pages(seen.blocks, hkv, 16, d, kind, BF, "cuda", seed=i) for i in range(2))
+    q = torch.randn(sum(new), hq * d, generator=torch.Generator().manual_seed(1)).to(BF).cuda()
+    want, tol, _ = expected(q, k, v, batch, seen, hq, hkv, d, d ** -0.5)
+    got = ops.attention(q, torch.full_like(q, float("nan")), batch, k, v, hq, hkv, d, d ** -0.5, 0, 0, 0).double()
+    assert ((got - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("kind", [None, I8, E4])
+@pytest.mark.parametrize("new", [[1], [7], [200]])
+def test_a_context_of_300000_tokens(new, kind):
+    """The bounds hold over the whole length: nothing is left out at its ends or between."""
+    hq, hkv, d = 6, 1, 64
+    groups = [([0], 64)] if kind is None else []
+    batch, seen = make_batch(new, [300000], 64, groups, "cuda", seed=1)
+    k, v = (make_pages(seen.blocks, hkv, 64, d, kind, BF, "cuda", seed=i) for i in range(2))
+    q = torch.randn(sum(new), hq * d, generator=torch.Generator().manual_seed(1)).to(BF).cuda()
+    want, tol, _ = expected(q, k, v, batch, seen, hq, hkv, d, d ** -0.5)
+    got = ops.attention(q, torch.full_like(q, float("nan")), batch, k, v, hq, hkv, d, d ** -0.5, 0, 0, 0).double()
+    assert ((got - want).abs() <= tol).all()
+    marked = torch.zeros(300000 + new[0])
+    marked[[0, 63, 64, 4095, 150001, 262144, 299999]] = 1.0        # large values of single keys are seen with their weight
+    for p in marked.nonzero().flatten().tolist():
+        table = seen.fronts[0] if groups and p < 64 else seen.tables[0]
+        if kind is None:
+            v[table[p // 64], 0, p % 64] = 1000.0
+        else:
+            v.scale[table[p // 64], 0, p % 64] *= 1000.0
+    want, tol, _ = expected(q, k, v, batch, seen, hq, hkv, d, d ** -0.5)
+    got = ops.attention(q, torch.full_like(q, float("nan")), batch, k, v, hq, hkv, d, d ** -0.5, 0, 0, 0).double()
+    assert ((got - want).abs() <= tol).all()
