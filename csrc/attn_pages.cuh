@@ -225,8 +225,9 @@ __device__ __noinline__ void row_anew(const AttnArgs& a, const RowKeys& k, int t
   if (part != nullptr && lane == 0) *reinterpret_cast<float2*>(part + a.d) = make_float2(m, l);
 }
 
-// Tiles of 64 keys in f16: code * scale / 2^E, E the exponent above the tile's largest scale, so that nothing leaves f16's range and a rounding is 2^-12 of
-// the number (2^-25 of the tile's largest scale at least).  What goes with a tile: 2^E of the keys, E and 2^-E of the values.
+// Tiles of 64 keys in f16: code * scale / 2^E, E the exponent above the tile's largest scale, so that nothing leaves f16's range and a rounding is 2^-11 of
+// the number or, where that is more, 2^-24 of the tile's largest scale.  E is held within -80 .. 120, which is every scale of rows of 16-bit numbers down to
+// 2^-80: numbers below 2^-94 lose bits.  What goes with a tile: 2^E of the keys, E and 2^-E of the values.
 struct TileScales {
   float k_up, v_exp, v_down, pad;
 };
@@ -234,7 +235,7 @@ struct TileScales {
 __device__ __forceinline__ int tile_exponent(float a, float b) {
   const unsigned x = __float_as_uint(a), y = __float_as_uint(b);
   const unsigned top = __reduce_max_sync(0xffffffffu, max(x < 0x7f800000u ? x : 0u, y < 0x7f800000u ? y : 0u));
-  return max(-60, min(100, (int)(top >> 23) - 126));
+  return max(-80, min(120, (int)(top >> 23) - 126));
 }
 __device__ __forceinline__ float two_to(int e) { return __int_as_float((127 + e) << 23); }
 __device__ __forceinline__ TileScales tile_scales(int ek, int ev) {

@@ -604,11 +604,10 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         float back = 1.f, off = 0.f;
         if constexpr (FMT != kF16Pages) {
           back = m2[nt][c] == -INFINITY ? 0.f : exp2f(m2[nt][c] - kUp - (m[nt][c] == -INFINITY ? 0.f : m[nt][c]));   // no value has a scale: zero
-          if constexpr (FMT == kInt8) {
-            off = -128.f * ps[nt][c] * back;
-            back *= 16777216.f;
-          }
+          if constexpr (FMT == kInt8) off = -128.f * ps[nt][c] * back;
         }
+        // int8: sums are of code 2^-24.  They are lifted before the factor, which may be as large as the values are
+        auto value = [&](float x) { return fmaf(FMT == kInt8 ? x * 16777216.f : x, back, off); };
         const int tok = s.row0 + i / group, head = kvh * group + i % group;
         if (last) {
           // sum is NaN where a score was; a row without a visible key is zero
@@ -622,8 +621,8 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             float y[8];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              y[2 * j] = sees ? fmaf(o[nt][4 * k + j][c], back, off) : 0.f;
-              y[2 * j + 1] = sees ? fmaf(o[nt][4 * k + j][c + 2], back, off) : 0.f;
+              y[2 * j] = sees ? value(o[nt][4 * k + j][c]) : 0.f;
+              y[2 * j + 1] = sees ? value(o[nt][4 * k + j][c + 2]) : 0.f;
             }
             *reinterpret_cast<uint4*>(dst + col) = pack8<T>(y);
           }
@@ -633,8 +632,7 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 #pragma unroll
           for (int k = 0; k < KS / 2; ++k) {
             const int e = 4 * k, col = VW >= 4 ? ((e / EPC) * 8 + r) * EPC + e % EPC : r * (D / 8) + e;
-            *reinterpret_cast<float4*>(dst + col) = make_float4(fmaf(o[nt][2 * k][c], back, off), fmaf(o[nt][2 * k][c + 2], back, off),
-                                                                fmaf(o[nt][2 * k + 1][c], back, off), fmaf(o[nt][2 * k + 1][c + 2], back, off));
+            *reinterpret_cast<float4*>(dst + col) = make_float4(value(o[nt][2 * k][c]), value(o[nt][2 * k][c + 2]), value(o[nt][2 * k + 1][c]), value(o[nt][2 * k + 1][c + 2]));
           }
           if (r == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(ref, sum);
         }

@@ -502,7 +502,8 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     // f16 ends at 2^16 and has no numbers below 2^-24: probabilities are formed times 2^7 (at most 2^15), so that those down to 2^-21 keep all bits
     constexpr float kUp = std::is_same<M, __half>::value ? 7.0f : 0.0f;
     float m_run = -INFINITY, l_run = 0.f;
-    // sums are of probabilities times 2^up: with scales, less the exponent of the values' largest so far
+    // outputs are sums of probabilities times 2^up: with scales, less the exponent of the values' largest so far.  The sum of probabilities stands relative
+    // to the maximum alone then: keys count whose values are far smaller than others
     float up = C::SCALED ? INFINITY : kUp;
     bool partly = false;                                  // some row of the warp does not see some key of its tiles
     bool bad = false;                                     // a score of the row is NaN: so is the result, whatever the exponentials made of it
@@ -547,9 +548,12 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       float up_new = up;
       if constexpr (C::SCALED) up_new = fminf(up, kUp - ts.v_exp);
       const float alpha = j > 0 && m_new > -INFINITY && (grow || up_new != up) ? exp2_fast((m_run - m_new) + (up_new - up)) : 1.0f;
+      const float fade = C::SCALED ? (j > 0 && grow ? exp2_fast(m_run - m_new) : 1.0f) : alpha;
       m_run = m_new;
       up = up_new;
-      const float neg = m_new == -INFINITY ? 0.f : (C::SCALED ? up + ts.v_exp : up) - m_new;
+      // of this tile's probabilities; below 2^-32 they are zeros in f16, and by a factor of 2^-60 their sum still is what it is
+      const float lift = C::SCALED ? fmaxf(up + ts.v_exp, -60.0f) : up;
+      const float neg = m_new == -INFINITY ? 0.f : lift - m_new;
       float la[4] = {0.f, 0.f, 0.f, 0.f}, lb[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < BN / 32; ++c) {
@@ -582,7 +586,7 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         }
         tmem_st_done();
       }
-      l_run = l_run * alpha + (C::SCALED ? l_tile * ts.v_down : l_tile);
+      l_run = l_run * fade + (C::SCALED ? l_tile * exp2_fast(-lift) : l_tile);
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar_p[q * 2 + b]);
@@ -598,7 +602,8 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     if constexpr (NQ > 1) asm volatile("bar.sync 1, %0;" ::"n"(32 * C::SOFT) : "memory");
     if (bad) l_run = __int_as_float(0x7fc00000);
     const bool sees = pos >= k_lo;                        // no visible key: zero
-    const float inv = 1.0f / l_run;
+    const float down = C::SCALED ? exp2f(-up) : 1.0f;     // of outputs, to the sum's reference
+    const float inv = down / l_run;
     const int stride = ta.direct ? D * 2 + 16 : D * 4 + 16;
     uint8_t* stage = smem + (q * BM + quarter * 32) * stride;
     uint8_t* mine = stage + lane * stride;
@@ -622,7 +627,7 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(mine + c * 128 + i * 4) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+        for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(mine + c * 128 + i * 4) = make_float4(__uint_as_float(r[i]) * down, __uint_as_float(r[i + 1]) * down, __uint_as_float(r[i + 2]) * down, __uint_as_float(r[i + 3]) * down);
       }
     }
     uint8_t* to = nullptr;
@@ -633,7 +638,7 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         to = reinterpret_cast<uint8_t*>(reinterpret_cast<T*>(a.out) + (int64_t)tok * a.ldo + (int64_t)head * D);
       } else {
         float* part = (is_own ? pa.tile_own : pa.tile_group) + (((int64_t)split * a.total_q + tok) * a.hq + head) * (D + kPad);
-        *reinterpret_cast<float2*>(part + D) = make_float2(m_run - (up < INFINITY ? up : 0.f), l_run);
+        *reinterpret_cast<float2*>(part + D) = make_float2(C::SCALED ? m_run : m_run - up, l_run);
         to = reinterpret_cast<uint8_t*>(part);
       }
     }

@@ -102,3 +102,23 @@ def test_a_context_of_300000_tokens(new, kind):
     want, tol, _ = expected(q, k, v, batch, seen, hq, hkv, d, d ** -0.5)
     got = ops.attention(q, torch.full_like(q, float("nan")), batch, k, v, hq, hkv, d, d ** -0.5, 0, 0, 0).double()
     assert ((got - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("kind", [I8, E4])
+@pytest.mark.parametrize("new", [[1, 1], [70, 3], [300, 40]])
+@pytest.mark.parametrize("sizes", [(None, 80), (80, None), (-60, 60), (100, -60), (-75, -75), (118, 118), (0, 40)])
+def test_pages_whose_values_differ_by_many_orders(sizes, new, kind):
+    """All values of a sequence's first page against all of the others: 2^this, or zeros.  Keys weigh what their scores say, whatever their values are."""
+    hq, hkv, d = 8, 2, 128
+    batch, seen = make_batch(new, [700, 350], 64, [], "cuda", seed=2)
+    k, v = (make_pages(seen.blocks, hkv, 64, d, kind, BF, "cuda", seed=i) for i in range(2))
+    for table in seen.tables:
+        for n, b in enumerate(table):
+            size = sizes[0 if n == 0 else 1]
+            v.scale[b] *= 0.0 if size is None else 2.0 ** size
+            if size is None:
+                v.data.view(torch.int8)[b] = 0
+    q = torch.randn(sum(new), hq * d, generator=torch.Generator().manual_seed(1)).to(BF).cuda()
+    want, tol, _ = expected(q, k, v, batch, seen, hq, hkv, d, d ** -0.5)
+    got = ops.attention(q, torch.full_like(q, float("nan")), batch, k, v, hq, hkv, d, d ** -0.5, 0, 0, 0).double()
+    assert ((got - want).abs() <= tol).all()
