@@ -353,7 +353,7 @@ Plan plan_call(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv
     // of a list takes whatever is left of it, and a block without keys is not free (a microsecond on its SM)
     const int keys = groups > 0 ? (max_kv - g_max_len > max_q ? max_kv - g_max_len : max_q) : max_kv;
     stretches((int64_t)p.tile.own_tiles * hkv * num_seqs, keys, groups > 0, p.own_splits, p.own_chunk);
-    p.direct = groups == 0 && p.own_splits == 1;
+    p.direct = groups == 0 && p.own_splits == 1 && fmt != kF16Pages;      // (16-bit pages come here without groups where a prefix has no tokens, if at all)
     // Every row tile converts all codes for itself, which takes the tiled kernel from 1100 to 2000 clocks per 64 keys; once for all costs a pass over the
     // cache (about 1200 clocks of an SM per 64 keys, and a launch).  4 portions of 1000 tokens over 1800, 16 tiles each: 251 -> 183 us; three tiles 89 -> 87
     // (16 sequences 198 -> 170), two tiles 69 -> 68, one 47 -> 47: from three tiles on.  Up to 1 GB of scratch
@@ -486,6 +486,7 @@ LLMSS_API int llmss_attn_pages(const void* q, int64_t ldq, const void* k_pages, 
     p.own_chunk = plan.own_chunk;
     p.group_splits = plan.group_splits;
     p.group_chunk = plan.group_chunk;
+    p.direct = plan.direct;
     const bool tiles = plan.tile.own_tiles > 0 || plan.tile.group_tiles > 0;
     float* expanded = take(plan.expanded);
     if (plan.pad > 0) {

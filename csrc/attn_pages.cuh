@@ -97,6 +97,7 @@ struct PartArgs {
   int few_own, few_groups;        // lists of sequences / groups are cut into runs
   int own_splits, group_splits;   // or into this many stretches of keys each (0: not)
   int own_chunk, group_chunk;     // keys of a stretch
+  int direct;                     // the tiled kernel writes results, not parts
 };
 
 struct Seg {
@@ -189,8 +190,8 @@ __device__ __forceinline__ void row_softmax(const AttnArgs& a, int tok, int head
 // A product over a tile of keys brings a value that is not finite to every row (0 x NaN is NaN), those included that do not see its key.  So a row whose
 // result is not finite is looked at once more, by a warp: where a hidden key of its tiles, of `from` .. `to` without first .. last, has such a value, the row
 // is formed anew over first .. last alone.  Costs a look at the results of rows that do not see all keys of their tiles: 4 portions of 1000 tokens over 1800
-// take as long as before (values looked at as they come into shared memory: 188 -> 205 us); that the code is there at all, 23.8 -> 24.8 us for a step of
-// 64 sequences behind 4096.
+// take as long as before (values looked at as they come into shared memory: 188 -> 205 us); that the code is there at all, 23.7 -> 24.4 us for a step of
+// 64 sequences behind 4096 (looked at in front of the rows' stores 24.8, in the merge kernel 25.5).
 struct RowKeys {
   const int* table;
   int kvh, from, first, last, to;

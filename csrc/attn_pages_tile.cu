@@ -164,6 +164,7 @@ template <typename T, int FMT, int D, int NQ>
 __device__ __noinline__ void rows_anew(const AttnArgs& a, const PartArgs& pa, const TileArgs& ta, unsigned rows) {
   using M = typename std::conditional<Tile<FMT, D, NQ>::SCALED, __half, T>::type;
   const Block b = block_of<NQ>(a, ta);
+  __syncwarp();                                          // behind the rows as they were
   for (; rows != 0; rows &= rows - 1) {
     int tok, head;
     const RowKeys k = keys_of<NQ>(a, b, b.n0 + (threadIdx.x & ~31) + __ffs(rows) - 1, tok, head);
@@ -631,8 +632,10 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       }
     }
     uint8_t* to = nullptr;
-    // (out of line: what a block runs once comes cold from memory)
-    const unsigned anew = partly ? spoiled_rows<T, FMT, D, NQ>(a, ta, t_o(q) + off, live && !bad) : 0u;
+    // (out of line: what a block runs once comes cold from memory.  A direct result may go over the queries: those rows are left out here)
+    unsigned anew = 0;
+    if constexpr (C::SCALED)
+      if (partly) anew = spoiled_rows<T, FMT, D, NQ>(a, ta, t_o(q) + off, live && !bad);
     if (live && (anew >> lane & 1) == 0) {
       if (ta.direct) {
         to = reinterpret_cast<uint8_t*>(reinterpret_cast<T*>(a.out) + (int64_t)tok * a.ldo + (int64_t)head * D);
@@ -660,6 +663,8 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     };
     if (ta.direct) rows_out(std::integral_constant<int, D * 2>{});
     else rows_out(std::integral_constant<int, D * 4>{});
+    if constexpr (!C::SCALED)
+      if (partly) anew = spoiled_rows<T, FMT, D, NQ>(a, ta, t_o(q) + off, live && !bad);
     if (anew != 0) rows_anew<T, FMT, D, NQ>(a, pa, ta, anew);
   }
 
@@ -686,7 +691,7 @@ int launch(const AttnArgs& a, const PartArgs& p, const TilePlan& t, cudaStream_t
   ta.own_chunk = p.own_chunk;
   ta.group_chunk = p.group_chunk;
   ta.segs_own = t.own_tiles > 0 ? a.num_seqs : 0;
-  ta.direct = a.groups == 0 && p.own_splits == 1;
+  ta.direct = p.direct;
   ta.page_magic = (uint32_t)(((1ull << 31) + a.page / 16 - 1) / (a.page / 16));
   ta.run = a.page % 64 == 0 ? 64 : a.page % 32 == 0 ? 32 : 16;
   CUtensorMap map_k, map_v;
