@@ -313,7 +313,9 @@ void stretches(int64_t blocks, int keys, bool merged, int& splits, int& chunk) {
 // of the second at most), or at the same time, the second on the SMs that fewer stretches of the first leave.  The estimates, in microseconds, were fitted to decode
 // steps of 24 to 64 sequences with 60 to 3000 tokens of their own behind 1500 to 12000: a tile of 64 keys 1.15 (8 bits 1.45), an SM reading own keys 88 GB/s
 // (8 bits, where it converts, 37) with 0.35 for each list, all of them 6.2 TB/s, starts 7 (8 bits 10) and 7.  64 sequences of 200 tokens behind 4096: 36.9 -> 24.7; of 3000 tokens: 147 -> 134;
-// 48 of 300 behind three prefixes of 2500, int8: 41.0 -> 32.5.  Returns the SMs of the second kernel.
+// 48 of 300 behind three prefixes of 2500, int8: 41.0 -> 32.5.  All of these with the lengths' own bounds.  A captured step knows more generous ones, the
+// estimate follows them, and the gain shrinks: the first with bounds of 4096 on the prefix and 8192 on all tokens 29, of 8192 on both 48; the last as four
+// groups of up to 4096 tokens and 48 rows 50.  Returns the SMs of the second kernel.
 int side_by_side(int64_t lists, int len, double own_lists, double own_bytes, double part_bytes, int d, int fmt, int& splits, int& chunk) {
   const bool wide = fmt == kF16Pages;
   const int64_t tiles = (len + 63) / 64;
@@ -321,7 +323,7 @@ int side_by_side(int64_t lists, int len, double own_lists, double own_bytes, dou
   auto prefix = [&](int64_t n) { return start + per_tile * ((lists * n + 147) / 148) * ((tiles + n - 1) / n); };
   auto own = [&](int64_t sms) { return 7 + (one / sms > all ? one / sms : all); };
   // a captured step knows bounds alone, and own keys may be far fewer: prefixes take twice as long as on all SMs at most (64 sequences of 200 tokens behind
-  // 4096 with a bound of 8192: 70.6 -> 28.7)
+  // 4096, all tokens bounded by 8192: 70.6 -> 28.7)
   const double longest = 2 * prefix(splits);
   double best = prefix(splits) + own(148) + part * splits;
   int64_t at = 0;

@@ -11,8 +11,8 @@
 //
 //   x = s log2(e), y = x + log2(vs):  l = sum 2^(x - m),  O = sum 2^(y - m') code,  out = O 2^(m' - m) / l
 //
-// The scale of a value row joins its probability in the exponent, with a maximum of its own, so that what is rounded to f16 is at most 2^8 whatever the
-// scales are.  Maxima move when a score exceeds them by 2^8 only.
+// The scale of a value row joins its probability in the exponent, with a maximum of its own.  Maxima move when a score exceeds them by 8 only, and what is
+// rounded to f16 is formed times 2^7, so that it is at most 2^15 whatever the scales are.
 //
 // The work of a call is the sum of all (sequence, key head) lists in units of 16 keys (32 where a key is 64 bytes); each warp takes an equal run of it,
 // wherever sequences begin and end, and waits for no other.  A list within a warp's run is finished there; one that crosses runs leaves its parts in

@@ -131,8 +131,8 @@ def attention(qkv, out, batch, k_cache, v_cache, hq, hkv, d, scale, q_off, k_off
     multi-token queries over prior context  -> the same kernel in paged mode (K / V from the cache);
     unsupported head sizes / page sizes     -> generic gather path (oracle math).
 
-    ``QuantPages``: keys and values are always those of the pages (a prompt's own too, so that a result does not depend on how the
-    prompt was cut into portions).  ``batch.prefix``: tokens that groups of sequences share are read once per group, from pages of either
+    ``QuantPages``: keys and values are always those of the pages (a prompt's own too, so that a result depends on how the prompt was
+    cut into portions by its last bits alone: keys are rounded relative to the largest of 64 neighbours).  ``batch.prefix``: tokens that groups of sequences share are read once per group, from pages of either
     kind.  Both take any mix of lengths; rows without a visible key become zero, rows of no sequence stay as they are, and keys that a row
     does not see never reach it, whatever lies there.
     The output's columns are those of the queries or share no memory with them.

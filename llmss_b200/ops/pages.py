@@ -1,9 +1,10 @@
 """Cache pages in 8 bits: codes and a 32-bit scale per token and head.
 
 A page holds what the 16-bit pages hold, [num_blocks, kv_heads, block_size, head_dim], in a byte per value; ``scale`` [num_blocks, kv_heads,
-block_size] turns a row's codes into numbers, value = code * scale.  One scale per row, because a row is written once, by one warp, when its token
-comes, and nothing that is in the cache has to be read or changed for it.  Integers (``torch.int8``) have even steps of 1 / 127 of a row's largest
-value, which suits rows whose values are of one size; ``torch.float8_e4m3fn`` has steps of 1 / 16 of each value, which suits rows with a few large ones.
+block_size] turns a row's codes into numbers, value = code * scale (scales are 0 or more, or NaN).  One scale per row, because a row is written once, by
+one warp, when its token comes, and nothing that is in the cache has to be read or changed for it.  Integers (``torch.int8``) have even steps of 1 / 127 of
+a row's largest value, which suits rows whose values are of one size; ``torch.float8_e4m3fn`` has steps of 1 / 16 of each value, which suits rows with a
+few large ones.
 """
 from __future__ import annotations
 
