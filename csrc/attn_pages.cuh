@@ -192,6 +192,7 @@ __device__ __forceinline__ void row_softmax(const AttnArgs& a, int tok, int head
 // is formed anew over first .. last alone.  Costs a look at the results of rows that do not see all keys of their tiles: 4 portions of 1000 tokens over 1800
 // take as long as before (values looked at as they come into shared memory: 188 -> 205 us); that the code is there at all, 23.7 -> 24.4 us for a step of
 // 64 sequences behind 4096 (looked at in front of the rows' stores 24.8, in the merge kernel 25.5).
+// Where it happens it is slow, 0.7 us per key of a row and warp: 2 portions of 2000 tokens over 1000, 32 heads, 0.3 ms; with one NaN token near their front 27.
 struct RowKeys {
   const int* table;
   int kvh, from, first, last, to;
@@ -203,7 +204,10 @@ template <typename M, int FMT>
 __device__ __noinline__ bool hidden_unfinite(const AttnArgs& a, const RowKeys& k) {
   bool found = false;
   for (int key = k.from; key <= k.to; ++key) {
-    if (key >= k.first && key <= k.last) continue;
+    if (key >= k.first && key <= k.last) {
+      key = k.last;
+      continue;
+    }
     const int64_t r = cache_row(a, k, key);
     if constexpr (FMT == kInt8 || FMT == kE4M3) found = found || !(fabsf(a.vs[r]) < INFINITY);
     for (int c = threadIdx.x & 31; c < a.d; c += 32) found = found || !(fabsf(page_value<M, FMT>(a.v, r * a.d + c)) < INFINITY);
