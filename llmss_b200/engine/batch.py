@@ -13,8 +13,8 @@ class SharedPrefix:
 
     Group j holds the sequences first[j] .. first[j + 1] - 1 of the batch; their first lens[j] tokens lie in the pages block_tables[j] (0: nothing
     is shared).  The sequences' own block tables name the same pages at their front and their lengths count the shared tokens.  Sequences outside
-    of first[0] .. first[-1] have no shared part.  ``max_len`` and ``max_rows`` bound lens and the query rows of a group; the tensors may change
-    under them, as in a captured step."""
+    of first[0] .. first[-1] have no shared part.  ``max_len`` and ``max_rows`` bound lens and the query rows of a group that shares something; the
+    tensors may change under them, as in a captured step."""
     block_tables: torch.Tensor  # [G, max_blocks] int32
     lens: torch.Tensor          # [G] int32
     first: torch.Tensor         # [G + 1] int32, ascending

@@ -136,7 +136,7 @@ class ModelRunner:
         if shared_prefix and self.sliding:
             raise ValueError("shared_prefix: a sliding window takes blocks off the front of a sequence")
         self.shared_prefix = bool(shared_prefix)
-        self._prefix: Optional[tuple] = None     # (groups, bound on their tokens) of the bound batch, None: no sharing
+        self._prefix: Optional[tuple] = None     # (groups, bounds on their tokens and rows) of the bound batch, None: no sharing
         self._nodes: Dict[tuple, tuple] = {}
         self._block_key: Dict[int, tuple] = {}
         self._next_node = 1
@@ -371,12 +371,21 @@ class ModelRunner:
 
     # ------------------------------------------------------------------ shared prefixes
     def by_prefix(self, seqs: List[SeqState]) -> List[SeqState]:
-        """The sequences in an order that puts those with the same blocks at their front next to each other (as they are without shared_prefix)."""
-        return sorted(seqs, key=lambda s: s.blocks) if self.shared_prefix else seqs
+        """The sequences in an order that puts those with the same blocks at their front next to each other, and those that share none behind them, so that
+        few rows lie between groups (as they are without shared_prefix)."""
+        if not self.shared_prefix:
+            return seqs
+        seqs = sorted(seqs, key=lambda s: s.blocks)
+        shares = lambda a, b: bool(a.blocks and b.blocks) and a.blocks[0] == b.blocks[0]
+        alone = [not (i > 0 and shares(seqs[i - 1], s) or i + 1 < len(seqs) and shares(s, seqs[i + 1])) for i, s in enumerate(seqs)]
+        return [s for s, a in zip(seqs, alone) if not a] + [s for s, a in zip(seqs, alone) if a]
 
     def prefix_groups(self, seqs: Sequence[SeqState]):
         """[(first row, rows, common blocks)] of neighbours with a common front worth its own pass: what the sequences would read again for themselves
-        takes memory longer than the second kernel and the merge do (about 10 us, 64 MB).
+        takes memory longer than the second kernel and the merge do (about 10 us, 64 MB).  Steps alone and shared, in us a layer, with these bounds:
+        16 sequences behind one prefix, 16 bits, 67 MB: 26.1, 19.8.  More than 16 query heads a key head, 16 bits, need two kernels for many rows, and
+        twice as much: 64 sequences of 48 heads, 95 MB: 27.5, 32.6; 183 MB: 53.5, 36.3.  8 bits are converted for every group, an eighth more for each
+        behind the second: two prefixes, 68 MB: 31.7, 24.4; eight, 67 MB: 61.7, 65.6; eight, 121 MB: 48.5, 48.8.
 
         Fronts may be nested (documents behind one system prompt): of all choices of up to ``_MAX_GROUPS`` runs of neighbours the one that saves most
         reads, over the sum of (rows - 1) x common blocks, so that a sequence which shares little does not cut the front of those beside it."""
@@ -404,9 +413,12 @@ class ModelRunner:
             more = most > best[1:, j - 1]
             best[1:, j] = np.where(more, most, best[1:, j - 1])
             start[1:, j] = np.where(more, i, -1)
-        if best[-1, n] * per_block < _SHARE_MIN_BYTES:
+        least = _SHARE_MIN_BYTES * (2 if self.core.hq > 16 * self.core.hkv and not self.quantised else 1)
+        # what g groups save less what they cost, the fewest where that is the same
+        worth = best[:, n] * per_block - (np.arange(_MAX_GROUPS + 1) - 2).clip(0) * (least // 8 if self.quantised else 0)
+        out, g, j = [], int(worth.argmax()), n
+        if worth[g] < least:
             return []
-        out, g, j = [], int(best[:, n].argmax()), n                     # the fewest groups that save as much
         while g > 0 and j > 1:
             i = int(start[g, j])
             if i < 0:
@@ -444,18 +456,21 @@ class ModelRunner:
             else:
                 self.h_pfx[G * mb + G + k + 1] = ends[-1]
         self.d_pfx.copy_(self.h_pfx)           # behind the steps that are enqueued; the pinned buffer is not rewritten before it has been read
-        bound = self.block_size
-        while bound < max(len(c) for _, c in spans) * self.block_size:
-            bound *= 2
-        self._prefix = (n, min(bound, self.max_blocks_per_seq * self.block_size))
+        # kernels are chosen and cut by bounds, so these lie close: eighths of an octave of tokens, the padded sizes of a batch for the rows of a group
+        # (64 sequences behind 4200 tokens: 48.1 us with the next power of two, 31.3 so; 8 groups of 8 sequences behind 1024, int8: 64.8 and 48.8)
+        longest = max(len(c) for _, c in spans)
+        eighth = max(1, (1 << (longest - 1).bit_length()) // 8)
+        bound = -(-longest // eighth) * eighth
+        rows = max(r for _, r, _ in groups)
+        self._prefix = (n, min(bound, self.max_blocks_per_seq) * self.block_size, next((b for b in _BUCKETS if b >= rows), rows))
 
     def _step_prefix(self, Bp: int) -> Optional[SharedPrefix]:
         if self._prefix is None:
             return None
-        n, bound = self._prefix
+        n, bound, rows = self._prefix
         G, mb = 2 * _MAX_GROUPS, self.max_blocks_per_seq
         return SharedPrefix(block_tables=self.d_pfx[:G * mb].view(G, mb), lens=self.d_pfx[G * mb:G * mb + G], first=self.d_pfx[G * mb + G:],
-                            num_groups=n, max_len=bound, max_rows=Bp)
+                            num_groups=n, max_len=bound, max_rows=min(rows, Bp))
 
     # ------------------------------------------------------------------ decode
     def _bucket(self, B: int) -> int:

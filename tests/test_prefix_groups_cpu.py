@@ -8,8 +8,8 @@ from llmss_b200.engine import runner as R2
 from llmss_b200.engine.runner import ModelRunner
 
 
-def groups_of(seqs, hkv=8, d=128, page=64):
-    r = SimpleNamespace(core=SimpleNamespace(hkv=hkv, d=d), quantised=False, block_size=page)
+def groups_of(seqs, hkv=8, d=128, page=64, hq=None, quantised=False):
+    r = SimpleNamespace(core=SimpleNamespace(hq=hq or hkv, hkv=hkv, d=d), quantised=quantised, block_size=page)
     return ModelRunner.prefix_groups(r, seqs)
 
 
@@ -81,3 +81,44 @@ def test_a_full_batch_is_looked_at_quickly():
     got = groups_of(seqs)
     assert [(i, n, len(c)) for i, n, c in got] == [(64 * k, 64, 101) for k in range(4)]
     assert time.perf_counter() - t < 1.0          # 10 ms
+
+
+@pytest.mark.parametrize("sizes,hq,hkv,quantised,shared", [
+    ((16,), 32, 8, False, True), ((8,), 32, 8, False, False),                  # one prefix of 18 and 17 blocks: 71 and 31 MB
+    ((8,) * 8, 32, 8, True, False), ((8,) * 2, 32, 32, True, True),            # 8 bits, nine blocks: 68 MB each, eight groups and two
+    ((64,), 48, 1, False, False), ((64,), 48, 1, True, False),                 # 46 blocks and more than 16 query heads a key head: 95 and 49 MB
+])
+def test_sharing_has_to_pay_for_its_kernels(sizes, hq, hkv, quantised, shared):
+    ids = iter(range(10 ** 6))
+    blocks = {16: 18, 8: 17 if not quantised else 9, 64: 46}
+    seqs = []
+    for n in sizes:
+        doc = [next(ids) for _ in range(blocks[n])]
+        seqs += [seq(doc + [next(ids)]) for _ in range(n)]
+    got = groups_of(seqs, hkv=hkv, hq=hq, quantised=quantised)
+    assert [n for _, n, _ in got] == (list(sizes) if shared else [])
+
+
+def test_sequences_that_share_nothing_stand_behind_the_groups():
+    r = SimpleNamespace(shared_prefix=True)
+    order = ModelRunner.by_prefix(r, [seq([9, 1]), seq([3]), seq([2, 5]), seq([9, 4]), seq([]), seq([2, 6]), seq([7])])
+    assert [s.blocks for s in order] == [[2, 5], [2, 6], [9, 1], [9, 4], [], [3], [7]]
+    assert ModelRunner.by_prefix(SimpleNamespace(shared_prefix=False), order[::-1]) == order[::-1]
+
+
+def test_bounds_lie_close_to_the_groups(tmp_path, monkeypatch):
+    from llmss_b200.engine.engine import Engine
+    from llmss_b200.utils.checkpoint import write_random_checkpoint
+
+    import torch
+
+    monkeypatch.setattr(R2, "_SHARE_MIN_BYTES", 0)
+    path = str(write_random_checkpoint(tmp_path, "gptj-tiny", dtype=torch.float32, device="cpu", std=0.08))
+    r = Engine.from_pretrained(path, device="cpu", max_batch=64, max_seq_len=128, block_size=1, prefix_cache=True, shared_prefix=True).runner
+    for rows, blocks, want in ((3, 1, (1, 4)), (5, 8, (8, 8)), (9, 9, (10, 16)), (17, 33, (40, 24)), (40, 64, (64, 48)), (2, 65, (80, 2)), (2, 127, (128, 2))):
+        seqs = [seq(list(range(blocks)) + [1000 + i], page=1) for i in range(rows)] + [seq([500 + i], page=1) for i in range(20)]
+        r._bind_prefix(seqs)
+        p = r._step_prefix(64)
+        assert (p.max_len, p.max_rows) == want and p.num_groups == 1
+        assert max(p.lens.tolist()) <= p.max_len and rows <= p.max_rows
+    assert r._step_prefix(1).max_rows == 1
