@@ -315,7 +315,7 @@ void stretches(int64_t blocks, int keys, bool merged, int& splits, int& chunk) {
 // (8 bits, where it converts, 37) with 0.35 for each list, all of them 6.2 TB/s, starts 7 (8 bits 10) and 7.  64 sequences of 200 tokens behind 4096: 36.9 -> 24.7; of 3000 tokens: 147 -> 134;
 // 48 of 300 behind three prefixes of 2500, int8: 41.0 -> 32.5.  All of these with the lengths' own bounds.  A captured step knows more generous ones, the
 // estimate follows them, and the gain shrinks: the first with bounds of 4096 on the prefix and 8192 on all tokens 29, of 8192 on both 48; the last as four
-// groups of up to 4096 tokens and 48 rows 50.  Returns the SMs of the second kernel.
+// groups of up to 4096 tokens and 48 rows 50, of 2560 tokens and 16 rows 44.  Returns the SMs of the second kernel.
 int side_by_side(int64_t lists, int len, double own_lists, double own_bytes, double part_bytes, int d, int fmt, int& splits, int& chunk) {
   const bool wide = fmt == kF16Pages;
   const int64_t tiles = (len + 63) / 64;
