@@ -132,10 +132,10 @@ def attention(qkv, out, batch, k_cache, v_cache, hq, hkv, d, scale, q_off, k_off
     unsupported head sizes / page sizes     -> generic gather path (oracle math).
 
     ``QuantPages``: keys and values are always those of the pages (a prompt's own too, so that a result depends on how the prompt was
-    cut into portions by its last bits alone: keys are rounded relative to the largest of 64 neighbours).  ``batch.prefix``: tokens that groups of sequences share are read once per group, from pages of either
-    kind.  Both take any mix of lengths; rows without a visible key become zero, rows of no sequence stay as they are, and keys that a row
-    does not see never reach it, whatever lies there.
-    The output's columns are those of the queries or share no memory with them.
+    cut into portions by its last bits alone: keys are rounded relative to the largest of 64 neighbours).  ``batch.prefix``: tokens that
+    groups of sequences share are read once per group, from pages of either kind.  Both take any mix of lengths; rows without a visible key
+    become zero, rows of no sequence stay as they are, and keys that a row does not see never reach it, whatever lies there.  The output's
+    columns are those of the queries or share no memory with them.
     """
     if batch.prefix is not None or isinstance(k_cache, QuantPages):
         if _cuda(qkv):
