@@ -36,8 +36,9 @@ struct Tile {
   static constexpr int COPY = SOFT + NQ;                                // first copying warp
   static constexpr int THREADS = 32 * (COPY + 2 + CONVERT);
   // 16-bit pages: registers, and shared memory for five tiles where two times 128 rows share them, that leave room for a block of the kernels which run
-  // beside this one (with 125 and six, 16 questions behind a prefix and 4 portions of 1000 tokens over 1800 took 2 % longer)
-  static constexpr int REGS = BYTES ? 128 : 112;
+  // beside this one (with 125 and six, 16 questions behind a prefix took 2 % longer).  Nothing runs beside codes converted before: 128 registers keep
+  // them from spilling (4 portions of 1000 tokens over 1800 202 -> 196 us)
+  static constexpr int REGS = SCALED ? 128 : 112;
   static constexpr int Q_BYTES = NQ * BM * D * 2;
   static constexpr int SLOT = BN * D * 2;                               // a tile of keys or values
   static constexpr int SLOTS = D == 256 ? (BYTES ? 3 : 4) : NQ == 2 && !BYTES ? 5 : 6;
