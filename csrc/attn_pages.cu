@@ -40,7 +40,7 @@ using namespace pages;
 
 // ---------------------------------------------------------------------------------------------------------------- any shape
 // One block per query row and head, its four warps on keys in turn, everything in 32 bits: head sizes and page sizes that the tiled kernels do not take.
-template <typename T, int FMT>
+template <typename T, int FMT, bool TREE>
 __global__ void __launch_bounds__(128) attn_pages_any_kernel(const __grid_constant__ AttnArgs a) {
   pdl_launch_dependents();
   pdl_wait();
@@ -49,15 +49,23 @@ __global__ void __launch_bounds__(128) attn_pages_any_kernel(const __grid_consta
   if (s < 0) return;
   const int q_len = a.cu[s + 1] - a.cu[s];
   const int len = min(a.seq_lens[s], a.max_blocks * a.page);
-  const int seen = min(len, a.seq_lens[s] - q_len + (t - a.cu[s]) + 1);     // keys 0 .. seen - 1
+  const int seen = TREE ? len : min(len, a.seq_lens[s] - q_len + (t - a.cu[s]) + 1);     // keys 0 .. seen - 1
   const int g = group_of_seq(a, s);
   const int shared = g < 0 ? 0 : min(a.g_lens[g], a.g_max_blocks * a.page);
   const int kvh = head / (a.hq / a.hkv);
   float o[8], m, l;
-  row_softmax<T, T, FMT>(a, t, head, warp, 4, seen, [&](int j) {
+  int sees = seen > 0;
+  if constexpr (TREE) sees = 0;
+  row_softmax<T, T, FMT, TREE>(a, t, head, warp, 4, seen, [&](int j) {
+    if constexpr (TREE) {
+      const int own = j - (a.seq_lens[s] - q_len);
+      if (own >= 0 && (tree_bits(a, t, own) & 1u) == 0) return (int64_t)-1;       // hidden
+      sees = 1;
+    }
     const int* table = j < shared ? a.g_tables + (int64_t)g * a.g_max_blocks : a.tables + (int64_t)s * a.max_blocks;
     return ((int64_t)checked_block(table[j / a.page], a.num_blocks) * a.hkv + kvh) * a.page + j % a.page;
   }, o, m, l);
+  if constexpr (TREE) sees = __syncthreads_or(sees);
   __shared__ float s_m[4], s_l[4], s_o[4][256];
   if (lane == 0) {
     s_m[warp] = m;
@@ -76,7 +84,7 @@ __global__ void __launch_bounds__(128) attn_pages_any_kernel(const __grid_consta
   T* orow = reinterpret_cast<T*>(a.out) + (int64_t)t * a.ldo + (int64_t)head * a.d;
   for (int c = threadIdx.x; c < a.d; c += 128) {
     const float y = w[0] * s_o[0][c] + w[1] * s_o[1][c] + w[2] * s_o[2][c] + w[3] * s_o[3][c];
-    orow[c] = from_f32<T>(seen > 0 ? y / sum : 0.f);     // a row that sees nothing is zero
+    orow[c] = from_f32<T>(sees ? y / sum : 0.f);     // a row that sees nothing is zero
   }
 }
 
@@ -391,6 +399,7 @@ Plan plan_call(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv
 }
 
 int check_args(const AttnArgs& a, int fmt, int dtype) {
+  LLMSS_REQUIRE(a.mask_words >= 0 && (int64_t)a.mask_words * 32 < (1ll << 31), "attn_pages: masks of %d words", a.mask_words);
   LLMSS_REQUIRE(dtype == LLMSS_F16 || dtype == LLMSS_BF16, "attn_pages: dtype must be f16/bf16");
   LLMSS_REQUIRE(fmt >= kF16Pages && fmt <= kE4M3, "attn_pages: page format %d unknown", fmt);
   LLMSS_REQUIRE(a.hq > 0 && a.hkv > 0 && a.hq % a.hkv == 0, "attn_pages: bad head grouping hq=%d hkv=%d", a.hq, a.hkv);
@@ -411,24 +420,10 @@ int check_args(const AttnArgs& a, int fmt, int dtype) {
   return 0;
 }
 
-}  // namespace
-
-// Floats of scratch that llmss_attn_pages takes for a call of these sizes (0: none).
-LLMSS_API int64_t llmss_attn_pages_scratch_floats(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv, int d, int block_size, int fmt,
-                                                  int groups, int g_max_len, int g_max_rows) {
-  if (num_seqs <= 0 || total_q <= 0 || max_q <= 0) return 0;
-  return plan_call(num_seqs, max_q, max_kv, total_q, hq, hkv, d, block_size, fmt, g_max_len > 0 ? groups : 0, g_max_len, g_max_rows).floats;
-}
-
-// q [total_q][>= hq * d] (row stride ldq); K / V pages [num_blocks][hkv][block_size][d] of the queries' type (fmt 0) or of bytes with 32-bit scales
-// [num_blocks][hkv][block_size] (fmt 1 int8, 2 e4m3); sequence i owns the rows cu_q[i] .. cu_q[i + 1] - 1, the last positions of its seq_lens[i] cached
-// tokens.  groups > 0: the sequences g_first[j] .. g_first[j + 1] - 1 find their first g_lens[j] tokens in the pages g_tables[j].  max_q, max_kv,
-// g_max_len, g_max_rows bound the lengths.  *launches: kernels launched (null: not wanted).  out is q itself or shares no memory with it.  Rows of sequences without a visible key become zero; rows of no sequence stay as they are.
-LLMSS_API int llmss_attn_pages(const void* q, int64_t ldq, const void* k_pages, const float* k_scale, const void* v_pages, const float* v_scale,
-                               const int* block_tables, int max_blocks, const int* seq_lens, void* out, int64_t ldo, const int* cu_q, int num_seqs,
-                               int max_q, int max_kv, int total_q, int hq, int hkv, int d, int block_size, int num_blocks, float scale, int fmt,
-                               int dtype, const int* g_tables, int g_max_blocks, const int* g_lens, const int* g_first, int groups, int g_max_len,
-                               int g_max_rows, void* scratch, int64_t scratch_floats, int* launches, cudaStream_t stream) {
+int attend(const void* q, int64_t ldq, const void* k_pages, const float* k_scale, const void* v_pages, const float* v_scale, const int* block_tables, int max_blocks,
+           const int* seq_lens, void* out, int64_t ldo, const int* cu_q, int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv, int d, int block_size,
+           int num_blocks, float scale, int fmt, int dtype, const int* g_tables, int g_max_blocks, const int* g_lens, const int* g_first, int groups,
+           int g_max_len, int g_max_rows, const void* masks, int mask_words, void* scratch, int64_t scratch_floats, int* launches, cudaStream_t stream) {
   int none = 0;
   if (launches == nullptr) launches = &none;
   *launches = 0;
@@ -459,10 +454,13 @@ LLMSS_API int llmss_attn_pages(const void* q, int64_t ldq, const void* k_pages, 
   a.page = block_size;
   a.num_blocks = num_blocks;
   a.scale_log2 = scale * 1.4426950408889634f;
+  a.masks = (const uint32_t*)masks;
+  a.mask_words = mask_words;
   LLMSS_REQUIRE(num_seqs >= 0 && max_q >= 0 && max_kv >= 0 && total_q >= 0 && groups >= 0, "attn_pages: negative size");
   if (num_seqs == 0 || total_q == 0 || max_q == 0) return 0;
   if (int e = check_args(a, fmt, dtype)) return e;
-  const Plan plan = plan_call(num_seqs, max_q, max_kv, total_q, hq, hkv, d, block_size, fmt, a.groups, g_max_len, g_max_rows);
+  Plan plan = plan_call(num_seqs, max_q, max_kv, total_q, hq, hkv, d, block_size, fmt, a.groups, g_max_len, g_max_rows);
+  if (masks != nullptr) plan.any = true;
   if (!plan.any) {
     LLMSS_REQUIRE(plan.floats == 0 || (scratch != nullptr && scratch_floats >= plan.floats && ((uintptr_t)scratch % 16) == 0), "attn_pages: %lld floats of 16-byte aligned scratch needed",
                   (long long)plan.floats);
@@ -531,7 +529,9 @@ LLMSS_API int llmss_attn_pages(const void* q, int64_t ldq, const void* k_pages, 
   }
   const dim3 grid(total_q, hq);
   LLMSS_REQUIRE(grid.y <= 65535, "attn_pages: %d heads", hq);
-#define LLMSS_ANY(T_, F_) LLMSS_CHECK_CUDA(launch_pdl(attn_pages_any_kernel<T_, F_>, grid, dim3(128), 0, stream, a))
+#define LLMSS_ANY(T_, F_)                                                                                                                          \
+  LLMSS_CHECK_CUDA(masks != nullptr ? launch_pdl(attn_pages_any_kernel<T_, F_, true>, grid, dim3(128), 0, stream, a)                                \
+                                    : launch_pdl(attn_pages_any_kernel<T_, F_, false>, grid, dim3(128), 0, stream, a))
   if (dtype == LLMSS_F16) {
     if (fmt == kInt8) LLMSS_ANY(__half, kInt8);
     else if (fmt == kE4M3) LLMSS_ANY(__half, kE4M3);
@@ -545,4 +545,46 @@ LLMSS_API int llmss_attn_pages(const void* q, int64_t ldq, const void* k_pages, 
   ++*launches;
   LLMSS_CHECK_CUDA(cudaGetLastError());
   return 0;
+}
+
+}  // namespace
+
+// Floats of scratch that llmss_attn_pages takes for a call of these sizes (0: none).
+LLMSS_API int64_t llmss_attn_pages_scratch_floats(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv, int d, int block_size, int fmt,
+                                                  int groups, int g_max_len, int g_max_rows) {
+  if (num_seqs <= 0 || total_q <= 0 || max_q <= 0) return 0;
+  return plan_call(num_seqs, max_q, max_kv, total_q, hq, hkv, d, block_size, fmt, g_max_len > 0 ? groups : 0, g_max_len, g_max_rows).floats;
+}
+
+// q [total_q][>= hq * d] (row stride ldq); K / V pages [num_blocks][hkv][block_size][d] of the queries' type (fmt 0) or of bytes with 32-bit scales
+// [num_blocks][hkv][block_size] (fmt 1 int8, 2 e4m3); sequence i owns the rows cu_q[i] .. cu_q[i + 1] - 1, the last positions of its seq_lens[i] cached
+// tokens.  groups > 0: the sequences g_first[j] .. g_first[j + 1] - 1 find their first g_lens[j] tokens in the pages g_tables[j].  max_q, max_kv,
+// g_max_len, g_max_rows bound the lengths.  *launches: kernels launched (null: not wanted).  out is q itself or shares no memory with it.  Rows of sequences without a visible key become zero; rows of no sequence stay as they are.
+LLMSS_API int llmss_attn_pages(const void* q, int64_t ldq, const void* k_pages, const float* k_scale, const void* v_pages, const float* v_scale,
+                               const int* block_tables, int max_blocks, const int* seq_lens, void* out, int64_t ldo, const int* cu_q, int num_seqs,
+                               int max_q, int max_kv, int total_q, int hq, int hkv, int d, int block_size, int num_blocks, float scale, int fmt,
+                               int dtype, const int* g_tables, int g_max_blocks, const int* g_lens, const int* g_first, int groups, int g_max_len,
+                               int g_max_rows, void* scratch, int64_t scratch_floats, int* launches, cudaStream_t stream) {
+  return attend(q, ldq, k_pages, k_scale, v_pages, v_scale, block_tables, max_blocks, seq_lens, out, ldo, cu_q, num_seqs, max_q, max_kv, total_q, hq,
+                hkv, d, block_size, num_blocks, scale, fmt, dtype, g_tables, g_max_blocks, g_lens, g_first, groups, g_max_len, g_max_rows, nullptr, 0, scratch,
+                scratch_floats, launches, stream);
+}
+
+// The same for trees of drafted tokens (and their scratch).
+LLMSS_API int64_t llmss_attn_tree_scratch_floats(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv, int d, int block_size, int fmt,
+                                                 int groups, int g_max_len, int g_max_rows) {
+  return 0;
+}
+
+// llmss_attn_pages where a row sees all tokens in front of its sequence's new ones (those of its rows), and of the new ones those whose bit its mask
+// [total_q][mask_words] has.  Bits behind the sequence's last token, and tokens behind the mask's last bit, do not count.
+LLMSS_API int llmss_attn_tree(const void* q, int64_t ldq, const void* k_pages, const float* k_scale, const void* v_pages, const float* v_scale,
+                              const int* block_tables, int max_blocks, const int* seq_lens, void* out, int64_t ldo, const int* cu_q, int num_seqs,
+                              int max_q, int max_kv, int total_q, int hq, int hkv, int d, int block_size, int num_blocks, float scale, int fmt,
+                              int dtype, const int* g_tables, int g_max_blocks, const int* g_lens, const int* g_first, int groups, int g_max_len,
+                              int g_max_rows, const void* masks, int mask_words, void* scratch, int64_t scratch_floats, int* launches, cudaStream_t stream) {
+  LLMSS_REQUIRE(masks != nullptr, "attn_tree: masks are null");
+  return attend(q, ldq, k_pages, k_scale, v_pages, v_scale, block_tables, max_blocks, seq_lens, out, ldo, cu_q, num_seqs, max_q, max_kv, total_q, hq,
+                hkv, d, block_size, num_blocks, scale, fmt, dtype, g_tables, g_max_blocks, g_lens, g_first, groups, g_max_len, g_max_rows, masks, mask_words, scratch,
+                scratch_floats, launches, stream);
 }

@@ -35,7 +35,20 @@ struct AttnArgs {
   int num_seqs, total_q, max_blocks, g_max_blocks, groups;
   int hq, hkv, d, page, num_blocks;
   float scale_log2;
+  // trees of drafted tokens (null: causal): bit j of a row: it sees token j of its sequence's new ones
+  const uint32_t* masks;    // [total_q][mask_words]
+  int mask_words;
 };
+
+// bits b .. b + 31 of the keys that a row of a tree sees, counted from its sequence's first new token: all cached tokens in front of it, none behind the mask
+__device__ __forceinline__ uint32_t tree_bits(const AttnArgs& a, int tok, int b) {
+  const uint32_t* mask = a.masks + (int64_t)tok * a.mask_words;
+  const int w = b >> 5;
+  const uint32_t lo = w < 0 ? ~0u : w < a.mask_words ? mask[w] : 0u;
+  if ((b & 31) == 0) return lo;
+  const uint32_t hi = w + 1 < 0 ? ~0u : w + 1 < a.mask_words ? mask[w + 1] : 0u;
+  return __funnelshift_r(lo, hi, b & 31);
+}
 
 // sequence that owns query row t (cu ascending), -1: none
 __device__ __forceinline__ int seq_of_row(const int* cu, int lo, int hi, int t) {
@@ -152,8 +165,8 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
 
 // ---------------------------------------------------------------------------------------------------------------- a row by itself
 // By a warp: the softmax of one row over the keys first, first + step .. below end, in 32 bits; lane i holds the columns i, i + 32 .. .  Looks at no key
-// that is not its row's.  M: type of 16-bit pages; row_of(key): its row of the cache.
-template <typename T, typename M, int FMT, typename RowOf>
+// that is not its row's.  M: type of 16-bit pages; row_of(key): its row of the cache, with HIDDEN negative for a key that the row does not see.
+template <typename T, typename M, int FMT, bool HIDDEN = false, typename RowOf>
 __device__ __forceinline__ void row_softmax(const AttnArgs& a, int tok, int head, int first, int step, int end, RowOf row_of, float (&o)[8], float& m, float& l) {
   const int lane = threadIdx.x & 31;
   float q[8];
@@ -166,6 +179,7 @@ __device__ __forceinline__ void row_softmax(const AttnArgs& a, int tok, int head
   }
   for (int j = first; j < end; j += step) {
     const int64_t r = row_of(j);
+    if (HIDDEN && r < 0) continue;
     float x = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i)

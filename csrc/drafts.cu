@@ -1,0 +1,325 @@
+// Steps that check drafted tokens: their metadata from request lengths, and what is accepted of them.
+#include "common.cuh"
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------------------------- metadata of a step
+//   cu[i + 1] = cu[i] + new[i]     seq_len[i] = ctx[i] + new[i]     slot(i, j) = table[i][(ctx + j) / page] page + (ctx + j) % page
+//   position = ctx + j, or in a tree ctx + depth(j), and mask(j) = mask(parent(j)) | 1 << j
+//
+// A block takes rows of one sequence (the last one the rows behind all sequences), a thread a row, and adds up the lengths in front of its sequence for
+// itself: with B blocks that is B^2 / 2 reads from L2, which are fewer clocks than a second launch up to thousands of sequences.  Bound by the launch
+// and by one chain of reads: lengths, page, parents.
+struct LayoutArgs {
+  const int* context;
+  const int* fresh;       // new tokens
+  const int* pages;       // page_counts: lists of page ids back to back; else [B][max_blocks]
+  const int* page_counts;
+  const int* parents;
+  long long* last;
+  int* seq_lens;
+  int* cu;
+  int* positions;
+  int* slots;
+  int* tables;
+  uint32_t* masks;
+  int64_t num_pages;
+  int num_seqs, rows, page, max_blocks, words;
+};
+
+__device__ __forceinline__ int64_t block_sum(int64_t x, int64_t* s_part) {   // by all threads
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  if (lane == 0) s_part[warp] = x;
+  __syncthreads();
+  x = 0;
+  for (int i = 0; i < warps; ++i) x += s_part[i];
+  __syncthreads();
+  return x;
+}
+
+__global__ void __launch_bounds__(256) step_layout_kernel(const LayoutArgs a) {
+  extern __shared__ uint32_t s_masks[];     // [threads][words]
+  __shared__ int64_t s_part[8];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int i = blockIdx.x, tid = threadIdx.x;
+  int64_t mine = 0, pages_mine = 0;
+  for (int s = tid; s < i; s += blockDim.x) {
+    mine += max(a.fresh[s], 0);
+    if (a.page_counts != nullptr) pages_mine += max(a.page_counts[s], 0);
+  }
+  const int row0 = (int)min(block_sum(mine, s_part), (int64_t)a.rows);
+  if (i == a.num_seqs) {
+    if (blockIdx.y == 0 && tid == 0) a.cu[i] = row0;
+    for (int t = row0 + blockIdx.y * blockDim.x + tid; t < a.rows; t += gridDim.y * blockDim.x) {
+      a.positions[t] = 0;
+      a.slots[t] = -1;
+      for (int w = 0; w < a.words; ++w) a.masks[(int64_t)t * a.words + w] = 0u;
+    }
+    return;
+  }
+  const int ctx = max(a.context[i], 0), n = min(max(a.fresh[i], 0), a.rows - row0);
+  const int* table;
+  int count;
+  if (a.page_counts != nullptr) {
+    const int64_t first = block_sum(pages_mine, s_part);
+    table = a.pages + first;
+    count = (int)min((int64_t)max(a.page_counts[i], 0), max(a.num_pages - first, (int64_t)0));
+    for (int b = blockIdx.y * blockDim.x + tid; b < a.max_blocks; b += gridDim.y * blockDim.x) a.tables[(int64_t)i * a.max_blocks + b] = b < count ? table[b] : 0;
+  } else {
+    table = a.pages + (int64_t)i * a.max_blocks;
+    count = a.max_blocks;
+  }
+  if (blockIdx.y == 0 && tid == 0) {
+    a.cu[i] = row0;
+    a.seq_lens[i] = ctx + n;
+    a.last[i] = (long long)row0 + n - 1;
+  }
+  for (int j0 = blockIdx.y * blockDim.x; j0 < n; j0 += gridDim.y * blockDim.x) {
+    const int j = j0 + tid;
+    if (j < n) {
+      const int at = (ctx + j) / a.page, id = (unsigned)at < (unsigned)count ? table[at] : -1;
+      a.slots[row0 + j] = id < 0 ? -1 : id * a.page + (ctx + j) % a.page;
+      int depth = j;
+      if (a.words > 0) {
+        uint32_t* mask = s_masks + tid * a.words;
+        for (int w = 0; w < a.words; ++w) mask[w] = 0u;
+        depth = -1;
+        for (int up = j; up >= 0; ++depth) {             // parents come before their children, so this ends
+          if (up < 32 * a.words) mask[up >> 5] |= 1u << (up & 31);
+          const int p = a.parents[row0 + up];
+          up = p < up ? p : -1;
+        }
+      }
+      a.positions[row0 + j] = ctx + depth;
+    }
+    if (a.words > 0) {
+      __syncthreads();
+      const int live = min(n - j0, (int)blockDim.x) * a.words;
+      for (int x = tid; x < live; x += blockDim.x) a.masks[(int64_t)(row0 + j0) * a.words + x] = s_masks[x];
+      __syncthreads();
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- what is accepted of a tree
+//   path[0] = 0     path[k + 1] = the first child of path[k] whose token is sampled[path[k]], until there is none
+//   tokens[k] = sampled[path[k]]     cache row of ctx + k = that of ctx + path[k], in all layers
+//
+// Every block walks its sequence's tree by one warp from shared memory, and then moves its share of the rows; a thread takes the same 16 bytes of a row
+// for all k.  Paths ascend, path[k] >= k, so that what is written over at k was read before: rows are moved in place, several on their way at once.
+// Bound by memory where paths are long and by the launch and the walk (a chain of three reads and a ballot per accepted token) elsewhere.
+constexpr int kMaxTree = 1024, kMaxSets = 8;
+
+struct RowSet {
+  uint8_t* base;
+  int row_bytes, unit;    // of a cache row; bytes that a thread moves at once: 16, 4 or 1
+};
+struct AcceptArgs {
+  const int* tokens;
+  const int* parents;
+  const int* sampled;
+  const int* cu;
+  const int* seq_lens;
+  const int* block_tables;
+  int* out_tokens;
+  int* counts;
+  int* path;
+  int* context;
+  RowSet sets[kMaxSets];
+  int num_sets, planes, heads, per_block;    // (plane, head) pairs of a block
+  int num_seqs, rows, max_q, max_blocks, page, num_blocks;
+  int write;                                 // the path as well: one launch of a call does
+};
+
+template <typename V>
+__device__ __forceinline__ void move_rows(const AcceptArgs& a, const RowSet& set, int pair0, int pairs, int count, const int* s_src, const int* s_dst) {
+  constexpr int AHEAD = 4;
+  const int units = set.row_bytes / (int)sizeof(V);
+  for (int x = threadIdx.x; x < pairs * units; x += blockDim.x) {
+    const int pair = pair0 + x / units, plane = pair / a.heads, head = pair % a.heads;
+    // row of (block, head, place): (block heads + head) page + place; s_src holds block heads page + place
+    uint8_t* base = set.base + ((int64_t)plane * a.num_blocks * a.heads * a.page + (int64_t)head * a.page) * set.row_bytes + (int64_t)(x % units) * sizeof(V);
+    for (int k0 = 1; k0 < count; k0 += AHEAD) {
+      V v[AHEAD];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u)
+        if (k0 + u < count && s_src[k0 + u] >= 0) v[u] = *reinterpret_cast<const V*>(base + (int64_t)s_src[k0 + u] * set.row_bytes);
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u)
+        if (k0 + u < count && s_src[k0 + u] >= 0) *reinterpret_cast<V*>(base + (int64_t)s_dst[k0 + u] * set.row_bytes) = v[u];
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256) accept_drafts_kernel(const __grid_constant__ AcceptArgs a) {
+  extern __shared__ int s_tree[];           // tokens, parents, sampled, path: [max_q] each; then rows to move, from and to
+  __shared__ int s_count;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int i = blockIdx.x;
+  const int row0 = min(max(a.cu[i], 0), a.rows), n = min(min(max(a.cu[i + 1], row0), a.rows) - row0, a.max_q);
+  const int ctx = a.seq_lens[i] - n;
+  int *s_tok = s_tree, *s_par = s_tok + a.max_q, *s_got = s_par + a.max_q, *s_path = s_got + a.max_q, *s_src = s_path + a.max_q, *s_dst = s_src + a.max_q;
+  for (int j = threadIdx.x; j < n; j += blockDim.x) {
+    s_tok[j] = a.tokens[row0 + j];
+    s_par[j] = a.parents[row0 + j];
+    s_got[j] = a.sampled[row0 + j];
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    int count = 0, node = n > 0 ? 0 : -1;
+    while (node >= 0) {
+      if (threadIdx.x == 0) s_path[count] = node;
+      ++count;
+      const int want = s_got[node];
+      int next = -1;
+      for (int c = node + 1; c < n && next < 0; c += 32) {
+        const int j = c + threadIdx.x;
+        const unsigned hit = __ballot_sync(0xffffffffu, j < n && s_par[j] == node && s_tok[j] == want);
+        if (hit != 0) next = c + __ffs(hit) - 1;
+      }
+      node = next;
+    }
+    if (threadIdx.x == 0) s_count = count;
+  }
+  __syncthreads();
+  const int count = s_count;
+  if (a.write && blockIdx.y == 0) {
+    for (int k = threadIdx.x; k < a.max_q; k += blockDim.x) {
+      a.path[(int64_t)i * a.max_q + k] = k < count ? s_path[k] : -1;
+      a.out_tokens[(int64_t)i * a.max_q + k] = k < count ? s_got[s_path[k]] : -1;
+    }
+    if (threadIdx.x == 0) {
+      a.counts[i] = count;
+      a.context[i] = ctx + count;
+    }
+  }
+  bool moves = false;
+  for (int k = threadIdx.x; k < count; k += blockDim.x) {
+    // blocks that do not exist are left alone
+    auto row = [&](int key) {
+      if (key < 0 || key / a.page >= a.max_blocks) return -1;
+      const int id = a.block_tables[(int64_t)i * a.max_blocks + key / a.page];
+      return (unsigned)id < (unsigned)a.num_blocks ? id * a.heads * a.page + key % a.page : -1;
+    };
+    int src = -1, dst = -1;
+    if (s_path[k] != k) src = row(ctx + s_path[k]), dst = row(ctx + k);
+    s_src[k] = dst < 0 ? -1 : src;
+    s_dst[k] = dst;
+    moves = moves || (src >= 0 && dst >= 0);
+  }
+  if (!__syncthreads_or(moves)) return;
+  const int pair0 = blockIdx.y * a.per_block, pairs = min(a.per_block, a.planes * a.heads - pair0);
+  for (int s = 0; s < a.num_sets; ++s) {
+    const RowSet& set = a.sets[s];
+    if (set.unit == 16) move_rows<uint4>(a, set, pair0, pairs, count, s_src, s_dst);
+    else if (set.unit == 4) move_rows<uint32_t>(a, set, pair0, pairs, count, s_src, s_dst);
+    else move_rows<uint8_t>(a, set, pair0, pairs, count, s_src, s_dst);
+  }
+}
+
+}  // namespace
+
+// context [num_seqs] cached tokens, fresh [num_seqs] new ones (negative: 0); rows: of all outputs, what lies beyond is cut off.  page_counts [num_seqs]:
+// pages holds the sequences' lists of page ids back to back, num_pages of them, and tables [num_seqs][max_blocks] is written (0 behind a list); null:
+// pages is that table already and tables is not looked at.  parents [rows] (words > 0): place of a token's parent among its sequence's new tokens, -1 for
+// none; a parent that does not come before its child is none.  masks [rows][words]: bit j of a row: its sequence's token j is the row's own or its ancestor; up to 32 words.
+// last [num_seqs]: last row of a sequence.  Rows of no sequence: position 0, slot -1, no bit.  A place without a page (beyond the list, id < 0): slot -1.
+LLMSS_API int llmss_step_layout(const int* context, const int* fresh, const int* pages, int64_t num_pages, const int* page_counts, const int* parents, void* last,
+                                int* seq_lens, int* cu, int* positions, int* slots, int* tables, void* masks, int num_seqs, int rows, int max_new, int page,
+                                int max_blocks, int words, cudaStream_t stream) {
+  LLMSS_REQUIRE(num_seqs >= 0 && rows >= 0 && max_blocks >= 0 && num_pages >= 0 && max_new >= 0, "step_layout: negative size");
+  LLMSS_REQUIRE(num_seqs < (1 << 24), "step_layout: %d sequences", num_seqs);
+  LLMSS_REQUIRE(page > 0, "step_layout: pages of %d tokens", page);
+  LLMSS_REQUIRE(words >= 0 && words <= kMaxTree / 32, "step_layout: masks of %d words (up to %d)", words, kMaxTree / 32);
+  LLMSS_REQUIRE((words > 0) == (parents != nullptr), "step_layout: parents and masks belong together");
+  LLMSS_REQUIRE(page_counts == nullptr || tables != nullptr || (int64_t)num_seqs * max_blocks == 0, "step_layout: lists of pages need a table to write");
+  LLMSS_REQUIRE(cu != nullptr, "step_layout: cu is null");
+  LayoutArgs a;
+  memset(&a, 0, sizeof(a));
+  a.context = context;
+  a.fresh = fresh;
+  a.pages = pages;
+  a.page_counts = page_counts;
+  a.parents = parents;
+  a.last = (long long*)last;
+  a.seq_lens = seq_lens;
+  a.cu = cu;
+  a.positions = positions;
+  a.slots = slots;
+  a.tables = tables;
+  a.masks = (uint32_t*)masks;
+  a.num_pages = num_pages;
+  a.num_seqs = num_seqs;
+  a.rows = rows;
+  a.page = page;
+  a.max_blocks = max_blocks;
+  a.words = words;
+  // a thread per row of the longest sequence (256 a block), and no more blocks than fill the card twice
+  int threads = 32;
+  while (threads < 256 && threads < max_new) threads *= 2;
+  int chunks = (max_new + threads - 1) / threads;
+  if (chunks > 2048 / (num_seqs + 1) + 1) chunks = 2048 / (num_seqs + 1) + 1;
+  if (chunks < 1) chunks = 1;
+  LLMSS_CHECK_CUDA(launch_pdl(step_layout_kernel, dim3(num_seqs + 1, chunks), dim3(threads), (size_t)threads * words * 4, stream, a));
+  return 0;
+}
+
+// tokens, parents, sampled [rows]; sequence i owns the rows cu[i] .. cu[i + 1] - 1, the last positions of its seq_lens[i] cached tokens.  Its rows move in
+// num_sets (1 to 8) tensors [planes][num_blocks][heads][page][row_bytes].  out_tokens, path [num_seqs][max_q] (-1 behind the path), counts and
+// context (cached tokens with the path) [num_seqs]; all four null: rows are moved only.  max_q bounds the rows of a sequence, up to 1024; of more, those behind are not looked at.
+LLMSS_API int llmss_accept_drafts(const int* tokens, const int* parents, const int* sampled, const int* cu, const int* seq_lens, const int* block_tables,
+                                  int* out_tokens, int* counts, int* path, int* context, const void* const* bases, const int* row_bytes, int num_sets, int planes,
+                                  int num_blocks, int heads, int page, int num_seqs, int rows, int max_q, int max_blocks, cudaStream_t stream) {
+  LLMSS_REQUIRE(num_seqs >= 0 && rows >= 0 && max_q >= 0 && max_blocks >= 0 && planes >= 0 && num_blocks >= 0, "accept_drafts: negative size");
+  if (num_seqs == 0) return 0;
+  LLMSS_REQUIRE(max_q <= kMaxTree, "accept_drafts: %d tokens of a sequence (up to %d)", max_q, kMaxTree);
+  LLMSS_REQUIRE(num_sets >= 0 && num_sets <= kMaxSets, "accept_drafts: %d tensors of cache rows (up to %d)", num_sets, kMaxSets);
+  LLMSS_REQUIRE(page > 0 && heads > 0, "accept_drafts: pages of %d tokens and %d heads", page, heads);
+  LLMSS_REQUIRE((int64_t)num_blocks * heads * page < (1ll << 31), "accept_drafts: 2^31 cache rows and more");
+  LLMSS_REQUIRE((int64_t)planes * heads < (1ll << 31) && (int64_t)max_blocks * page < (1ll << 31), "accept_drafts: sizes of 2^31 and more");
+  LLMSS_REQUIRE((out_tokens != nullptr) == (counts != nullptr) && (counts != nullptr) == (path != nullptr) && (path != nullptr) == (context != nullptr),
+                "accept_drafts: all outputs or none");
+  AcceptArgs a;
+  memset(&a, 0, sizeof(a));
+  a.tokens = tokens;
+  a.parents = parents;
+  a.sampled = sampled;
+  a.cu = cu;
+  a.seq_lens = seq_lens;
+  a.block_tables = block_tables;
+  a.out_tokens = out_tokens;
+  a.counts = counts;
+  a.path = path;
+  a.context = context;
+  a.num_sets = num_sets;
+  a.planes = planes;
+  a.heads = heads;
+  a.num_seqs = num_seqs;
+  a.rows = rows;
+  a.max_q = max_q;
+  a.max_blocks = max_blocks;
+  a.page = page;
+  a.num_blocks = num_blocks;
+  a.write = out_tokens != nullptr;
+  int64_t widest = 1;
+  for (int s = 0; s < num_sets; ++s) {
+    LLMSS_REQUIRE(bases[s] != nullptr && row_bytes[s] > 0, "accept_drafts: tensor %d is null or has rows of %d bytes", s, row_bytes[s]);
+    a.sets[s].base = (uint8_t*)bases[s];
+    a.sets[s].row_bytes = row_bytes[s];
+    const int all = row_bytes[s] | (int)((uintptr_t)bases[s] & 15);
+    a.sets[s].unit = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
+    if (row_bytes[s] / a.sets[s].unit > widest) widest = row_bytes[s] / a.sets[s].unit;
+  }
+  // a block moves about 512 pieces per row of the path (two a thread)
+  const int64_t pairs = num_sets > 0 ? (int64_t)planes * heads : 0;
+  int64_t per = (512 + widest - 1) / widest;
+  if (pairs > per * 65535) per = (pairs + 65534) / 65535;
+  a.per_block = (int)per;
+  const int64_t shares = pairs > 0 ? (pairs + per - 1) / per : 1;
+  LLMSS_CHECK_CUDA(launch_pdl(accept_drafts_kernel, dim3(num_seqs, (unsigned)shares), dim3(256), (size_t)6 * max_q * 4, stream, a));
+  return 0;
+}

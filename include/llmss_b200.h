@@ -554,6 +554,29 @@ int llmss_attn_pages(const void* q, int64_t ldq, const void* k_pages, const floa
                      int dtype, const int* g_tables, int g_max_blocks, const int* g_lens, const int* g_first, int groups, int g_max_len,
                      int g_max_rows, void* scratch, int64_t scratch_floats, int* launches, llmss_stream_t stream);
 
+/* ---- steps that check drafted tokens (csrc/drafts.cu, csrc/attn_pages.cu) ----
+ * step_layout: cu [num_seqs + 1], seq_lens, last (int64) [num_seqs], positions, slots [rows] from cached (context) and new (fresh) tokens [num_seqs].
+ * page_counts: pages holds lists of page ids back to back, tables [num_seqs][max_blocks] is written; null: pages is that table.  parents [rows] (words > 0):
+ * place of a token's parent among its sequence's new ones, -1 none; positions are context + depth then, and masks [rows][words] have a bit for the token
+ * itself and each ancestor. */
+int llmss_step_layout(const int* context, const int* fresh, const int* pages, int64_t num_pages, const int* page_counts, const int* parents, void* last,
+                      int* seq_lens, int* cu, int* positions, int* slots, int* tables, void* masks, int num_seqs, int rows, int max_new, int page,
+                      int max_blocks, int words, llmss_stream_t stream);
+/* llmss_attn_pages where a row sees all tokens in front of its sequence's new ones, and of those the ones whose bit its mask [total_q][mask_words] has. */
+int64_t llmss_attn_tree_scratch_floats(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv, int d, int block_size, int fmt,
+                                       int groups, int g_max_len, int g_max_rows);
+int llmss_attn_tree(const void* q, int64_t ldq, const void* k_pages, const float* k_scale, const void* v_pages, const float* v_scale,
+                    const int* block_tables, int max_blocks, const int* seq_lens, void* out, int64_t ldo, const int* cu_q, int num_seqs,
+                    int max_q, int max_kv, int total_q, int hq, int hkv, int d, int block_size, int num_blocks, float scale, int fmt,
+                    int dtype, const int* g_tables, int g_max_blocks, const int* g_lens, const int* g_first, int groups, int g_max_len,
+                    int g_max_rows, const void* masks, int mask_words, void* scratch, int64_t scratch_floats, int* launches, llmss_stream_t stream);
+/* The path through each tree from its first token along children whose token is what was sampled at their parent: out_tokens, path [num_seqs][max_q]
+ * (-1 behind it), counts, context (cached tokens with the path) [num_seqs]; cache row context + path[k] moves to context + k in num_sets (up to 8) tensors
+ * [planes][num_blocks][heads][page][row_bytes] (bases, row_bytes: host).  All outputs null: rows are moved only. */
+int llmss_accept_drafts(const int* tokens, const int* parents, const int* sampled, const int* cu, const int* seq_lens, const int* block_tables,
+                        int* out_tokens, int* counts, int* path, int* context, const void* const* bases, const int* row_bytes, int num_sets, int planes,
+                        int num_blocks, int heads, int page, int num_seqs, int rows, int max_q, int max_blocks, llmss_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -42,6 +42,16 @@ class SharedPrefix:
 
 
 @dataclass
+class DraftTree:
+    """The new tokens of every sequence of a batch as a tree of guesses (``ops.step_layout`` makes the masks).
+
+    ``parents``: a token's parent by its place among its sequence's new tokens, -1 for none, parents before children.  ``masks``: bit j of a row: it sees
+    its sequence's new token j; attention goes by these alone."""
+    parents: torch.Tensor       # [T] int32
+    masks: torch.Tensor         # [T, words] int32
+
+
+@dataclass
 class BatchInput:
     tokens: torch.Tensor        # [T] int32 token ids, sequences packed back to back
     positions: torch.Tensor     # [T] int32 absolute position of each token
@@ -58,45 +68,42 @@ class BatchInput:
     decode_splits: int = 0      # split-KV factor frozen at graph-capture time (0 = choose per call)
     state_slots: Optional[torch.Tensor] = None   # [B] int32 state slot of each sequence (recurrent models); < 0 = inert row
     prefix: Optional[SharedPrefix] = None        # cached tokens that groups of sequences share
+    tree: Optional[DraftTree] = None             # new tokens are trees of guesses
 
     @staticmethod
     def build(token_lists: Sequence[Sequence[int]], context_lens: Sequence[int], block_tables: Sequence[Sequence[int]],
               block_size: int, device, max_blocks: Optional[int] = None, pad_to: int = 1,
-              state_slots: Optional[Sequence[int]] = None) -> "BatchInput":
-        """Host-side construction: ``token_lists[i]`` are the new tokens of sequence i, which
-        already has ``context_lens[i]`` tokens in the cache blocks ``block_tables[i]``."""
-        toks: List[int] = []
-        pos: List[int] = []
-        slots: List[int] = []
-        cu = [0]
-        seq_lens = []
-        for new, ctx, bt in zip(token_lists, context_lens, block_tables):
-            for j, t in enumerate(new):
-                p = ctx + j
-                toks.append(int(t))
-                pos.append(p)
-                slots.append(bt[p // block_size] * block_size + p % block_size)
-            cu.append(len(toks))
-            seq_lens.append(ctx + len(new))
+              state_slots: Optional[Sequence[int]] = None, parents: Optional[Sequence[Sequence[int]]] = None) -> "BatchInput":
+        """``token_lists[i]`` are the new tokens of sequence i, which already has ``context_lens[i]`` tokens in the cache blocks ``block_tables[i]``;
+        ``parents[i]``: they are a tree (DraftTree).  Goes to the device as one upload, what follows from the lengths is formed there."""
+        from ..ops import step_layout
+
+        q_lens = [len(t) for t in token_lists]
+        for n, ctx, bt in zip(q_lens, context_lens, block_tables):
+            if ctx + n > len(bt) * block_size and n:
+                raise IndexError(f"{ctx} + {n} tokens in {len(bt)} blocks of {block_size}")
+        B, T, counts = len(q_lens), sum(q_lens), [len(b) for b in block_tables]
+        mb = max_blocks or max(1, max(counts))
+        if max(counts, default=0) > mb:
+            raise ValueError(f"{max(counts)} blocks in a table of {mb}")
         # inert padding rows (token 0, slot -1, owned by no sequence) so that the packed length is a
         # multiple of `pad_to` (sequence-parallel prefill shards the rows evenly over the ranks)
-        while len(toks) % pad_to:
-            toks.append(0)
-            pos.append(0)
-            slots.append(-1)
-        B = len(token_lists)
-        mb = max_blocks or max(1, max(len(b) for b in block_tables))
-        bt_t = torch.zeros(B, mb, dtype=torch.int32)
-        for i, b in enumerate(block_tables):
-            if len(b):
-                bt_t[i, :len(b)] = torch.tensor(b, dtype=torch.int32)
-        qlens = [len(t) for t in token_lists]
-        i32 = dict(dtype=torch.int32)
+        rows = T + -T % pad_to
+        parts = [[x for t in token_lists for x in t] + [0] * (rows - T), list(context_lens), q_lens, counts, [b for bt in block_tables for b in bt]]
+        if parents is not None:
+            if [len(p) for p in parents] != q_lens:
+                raise ValueError(f"trees of {[len(p) for p in parents]} parents for {q_lens} tokens")
+            parts.append([x for p in parents for x in p] + [-1] * (rows - T))
+        if state_slots is not None:
+            parts.append(list(state_slots))
+        sizes = [len(p) for p in parts]
+        parts = list(torch.tensor([int(x) for p in parts for x in p], dtype=torch.int32).to(device).split(sizes))
+        tokens, context, new, counts, pages = parts[:5]
+        max_q = max(q_lens, default=0)
+        up = parts[5] if parents is not None else None
+        at = step_layout(context, new, pages, block_size, rows, max_q, page_counts=counts, max_blocks=mb, parents=up)
         return BatchInput(
-            tokens=torch.tensor(toks, **i32).to(device), positions=torch.tensor(pos, **i32).to(device),
-            slot_mapping=torch.tensor(slots, **i32).to(device), block_tables=bt_t.to(device),
-            seq_lens=torch.tensor(seq_lens, **i32).to(device), cu_q=torch.tensor(cu, **i32).to(device),
-            last_idx=(torch.tensor(cu[1:], dtype=torch.int64) - 1).to(device),
-            num_seqs=B, max_q=max(qlens) if qlens else 0, max_kv=max(seq_lens) if seq_lens else 0,
-            is_decode=all(q == 1 for q in qlens), is_fresh_prefill=all(c == 0 for c in context_lens),
-            state_slots=None if state_slots is None else torch.tensor(list(state_slots), **i32).to(device))
+            tokens=tokens, positions=at.positions, slot_mapping=at.slot_mapping, block_tables=at.block_tables, seq_lens=at.seq_lens, cu_q=at.cu_q,
+            last_idx=at.last_idx, num_seqs=B, max_q=max_q, max_kv=max((c + n for c, n in zip(context_lens, q_lens)), default=0),
+            is_decode=all(q == 1 for q in q_lens), is_fresh_prefill=all(c == 0 for c in context_lens),
+            state_slots=None if state_slots is None else parts[-1], tree=None if up is None else DraftTree(parents=up, masks=at.masks))

@@ -29,6 +29,10 @@ class KVCache:
     def bytes_per_block(num_layers, block_size, kv_heads, head_dim, dtype) -> int:
         return num_layers * 2 * block_size * kv_heads * head_dim * torch.empty((), dtype=dtype).element_size()
 
+    def row_tensors(self) -> List[torch.Tensor]:
+        """What holds the cached rows, for ``ops.accept_drafts``."""
+        return [self.data]
+
     def copy_blocks_from(self, old: "KVCache", src: int, dst: int, n: int):
         self.data[:, :, dst:dst + n] = old.data[:, :, src:src + n]
 
@@ -57,6 +61,9 @@ class QuantKVCache:
     @staticmethod
     def bytes_per_block(num_layers, block_size, kv_heads, head_dim) -> int:
         return num_layers * 2 * block_size * kv_heads * (head_dim + 4)
+
+    def row_tensors(self) -> List[torch.Tensor]:
+        return [self.data, self.scale]
 
     def copy_blocks_from(self, old: "QuantKVCache", src: int, dst: int, n: int):
         self.data.view(torch.int8)[:, :, dst:dst + n] = old.data.view(torch.int8)[:, :, src:src + n]

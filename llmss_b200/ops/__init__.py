@@ -15,6 +15,7 @@ import torch
 
 from . import cuda_impl as cu
 from . import reference as ref
+from .drafts import Accepted, StepLayout
 from .pages import QuantPages
 from .reference import (DECAY_HEAD, DECAY_TOKEN_CHANNEL, DECAY_TOKEN_HEAD, GATE_NONE, GATE_SIGMOID, GATE_SILU, UNARY_NEG_EXP,
                         UNARY_TANH, distance_bias_table, rotary_frequencies, window_bias_table)
@@ -136,8 +137,12 @@ def attention(qkv, out, batch, k_cache, v_cache, hq, hkv, d, scale, q_off, k_off
     groups of sequences share are read once per group, from pages of either kind.  Both take any mix of lengths; rows without a visible key
     become zero, rows of no sequence stay as they are, and keys that a row does not see never reach it, whatever lies there.  The output's
     columns are those of the queries or share no memory with them.
+
+    ``batch.tree``: the batch's rows are trees of drafted tokens.  A row sees all of its sequence's cached tokens in front of the new ones, and of those the
+    ones whose bit its mask has (``step_layout`` makes masks of ancestors; any others do as well).  Over pages of either kind, as above, with or without a
+    prefix, whose tokens are cached ones.
     """
-    if batch.prefix is not None or isinstance(k_cache, QuantPages):
+    if batch.prefix is not None or batch.tree is not None or isinstance(k_cache, QuantPages):
         if _cuda(qkv):
             cu.attention_pages(qkv, out, batch, k_cache, v_cache, hq, hkv, d, scale, q_off, out_off)
         else:
@@ -206,6 +211,39 @@ def embed(tokens, wte, positions=None, wpe=None, pos_offset: int = 0, out_dtype=
     return h if out is None else out.copy_(h)
 
 
+# ----------------------------------------------------------------------------- steps that check drafted tokens
+def step_layout(context_lens, new_lens, pages, page_size, rows, max_new, page_counts=None, max_blocks=None, parents=None) -> StepLayout:
+    """Where the new tokens of a step go, from the requests' lengths alone: ``context_lens`` [B] cached tokens, ``new_lens`` [B] new ones (int32, on the
+    device that computes), packed back to back into ``rows`` rows.
+
+    ``page_counts`` [B] with ``max_blocks``: ``pages`` is the sequences' lists of page ids back to back, and block tables are made of them (0 behind a
+    list).  Without: ``pages`` are block tables [B or more, max_blocks].  ``max_new`` bounds new_lens; a larger one costs time, and with ``parents``
+    its masks end there.  ``parents`` [rows]: the new tokens of a sequence are a tree, a token's parent given by its place among them (-1: none; parents come
+    before their children, one that does not is none): positions are context + depth instead of context + place, and ``masks`` [rows,
+    ceil(max_new / 32)] have a bit for the token itself and each of its ancestors; trees of up to 1024 tokens.
+
+    Tokens lie in the cache in their order, slot of place j: that of token context + j; -1 where a list has no such page (or its id is below 0).  Rows of
+    no sequence: position 0, slot -1, no bit.  Sequences that do not fit into the rows are cut off there; negative lengths are 0."""
+    return (cu if _cuda(context_lens) else ref).step_layout(context_lens, new_lens, pages, page_size, rows, max_new, page_counts, max_blocks, parents)
+
+
+def accept_drafts(sampled, batch, pages) -> Accepted:
+    """The path through each tree of ``batch`` that agrees with ``sampled`` [rows], the token drawn at every row: from a sequence's first new token on to the
+    first child whose token is what was sampled at its parent, until there is none.  ``tokens`` of the result are what was sampled along it: those
+    that the sequence gains, of which the last is not in the cache yet.
+
+    ``pages``: tensors [.., blocks, heads, block_size, d] whose rows the step wrote, e.g. ``KVCache.row_tensors()``; others behind the first may have other
+    rows, or none of that dimension, as scales.  The path's rows move in them, from where the tree had them to where a sequence without a tree would have
+    them, in place and for all leading dimensions at once.  A row whose page does not exist (a block table of -1, or too short) is not moved.  A
+    sequence without new tokens gains nothing."""
+    return (cu if _cuda(sampled) else ref).accept_drafts(sampled, batch, list(pages))
+
+
+def _no_tree(batch):
+    if getattr(batch, "tree", None) is not None:
+        raise ValueError("trees of drafted tokens: ops.attention alone takes them")
+
+
 # ----------------------------------------------------------------------------- 32-bit residual stream, Dynamic Tanh
 def dyt_residual(resid, alpha: float, weight, bias, a=None, scale_a=None, b=None, scale_b=None, out_dtype=None,
                  want_norm: bool = True):
@@ -254,6 +292,7 @@ def latent_attention(q_abs, cache, batch, heads, rank, scale, out_dtype):
     16-bit compute with a rank the tcgen05 multi-query kernels cover (64 / 128 / 256) runs on those (the latent
     cache has their [blocks, 1, block_size, d] layout): decode batches on the split-KV decode kernel, portions of
     prompts on the paged prefill kernel.  Every other case (true 32-bit, other ranks) runs the generic kernel."""
+    _no_tree(batch)
     if _cuda(q_abs):
         return cu.latent_attention(q_abs, cache, batch, heads, rank, scale, out_dtype)
     return ref.latent_attention(q_abs, cache, batch.block_tables, batch.seq_lens, batch.cu_q, heads, rank, scale, out_dtype)
@@ -283,6 +322,7 @@ def _dispatch(name, probe, *args, **kw):
 
 def embed_bigram(tokens, wte, table, mul_prev, mul_cur, buckets, batch, prev_state):
     """Token embedding plus a hashed (previous token, token) embedding, 32-bit; see ops.reference.embed_bigram."""
+    _no_tree(batch)
     return _dispatch("embed_bigram", wte, tokens, wte, table, mul_prev, mul_cur, buckets, batch, prev_state)
 
 
@@ -293,10 +333,12 @@ def postnorm_residual(y, weight, eps, resid=None, y2=None, w_a=None, w_b=None, o
 
 
 def token_shift(x, mu, batch, prev_state, out_dtype=None):
+    _no_tree(batch)
     return _dispatch("token_shift", x, x, mu, batch, prev_state, out_dtype)
 
 
 def causal_conv(u, w, bias, act, batch, state, out_dtype=None):
+    _no_tree(batch)
     return _dispatch("causal_conv", u, u, w, bias, act, batch, state, out_dtype)
 
 
@@ -317,6 +359,7 @@ def attention_bias(q, k_cache, v_cache, batch, hq, hkv, dk, dv, scale, dist_bias
     ``keep_first``: first tokens that the window never hides; ``softcap``: cap * tanh(score / cap); ``diff`` = (lam, eps, factor): two
     maps per head, combined as rms_div(a1 - lam * a2) * factor; ``out``: view that receives [T, hq * dv].
     ``chunk``: keys outside the query's own block of ``chunk`` positions are hidden.  v_cache may be a column view of wider rows."""
+    _no_tree(batch)
     if _cuda(q):
         return cu.attention_bias(q, k_cache, v_cache, batch, hq, hkv, dk, dv, scale, dist_bias, gate, out_dtype, bias_over_scale,
                                  window, slopes, sinks, keep_first, softcap, diff, out, chunk)
@@ -335,6 +378,7 @@ def ssm_dt(dt_raw, dt_bias, a_log):
 def linear_scan(q, k, v, decay, decay_kind, batch, state, heads, qk_heads, dk, dv, bonus=None, v_scale=None,
                 read_before=False):
     """Gated linear recurrence (RWKV time mixing, lightning attention, state-space duality are parameter choices)."""
+    _no_tree(batch)
     return _dispatch("linear_scan", v, q, k, v, decay, decay_kind, batch, state, heads, qk_heads, dk, dv, bonus, v_scale,
                      read_before)
 
@@ -357,6 +401,7 @@ def hyper_residual(xs, y=None, mix=None, w_out=None, w_in=None, norm_w=None, eps
 
 def delta_scan(q, k, v, log_decay, beta, batch, state, heads, qk_heads, dk, dv, unit_eps=None, q_scale=1.0, beta_sigmoid=False):
     """Gated delta rule (decay, error-correcting write, read-out after the write); see ops.reference.delta_scan."""
+    _no_tree(batch)
     return _dispatch("delta_scan", v, q, k, v, log_decay, beta, batch, state, heads, qk_heads, dk, dv, unit_eps, q_scale,
                      beta_sigmoid)
 

@@ -14,7 +14,8 @@ from typing import Optional
 
 import torch
 
-from . import _lib
+from . import _lib, drafts
+from .drafts import wrong_ints as _wrong_ints
 from .pages import FORMATS, QuantPages
 from .reference import ACT_NONE
 
@@ -314,14 +315,6 @@ def attn_prefill_paged(q_view, k_cache, v_cache, block_tables, seq_lens, out_vie
 _HALVES = (torch.float16, torch.bfloat16)
 
 
-def _wrong_ints(dev, *tensors):
-    """Whether one of the tensors is not contiguous int32 on device ``dev``."""
-    for t in tensors:
-        if t.dtype is not torch.int32 or not t.is_contiguous() or t.get_device() != dev:
-            return True
-    return False
-
-
 def rope_kv_write_q8(qkv, positions, slot_mapping, k_pages, v_pages, hq, hkv, d, rotary_dim, style, base, q_off, k_off, v_off):
     dev = qkv.get_device()
     if dev != torch._C._cuda_getDevice():       # launches go to the current device's stream
@@ -351,8 +344,9 @@ _NO_GROUPS = (None, 0, None, None, 0, 0, 0)
 
 
 def attention_pages(qkv, out, batch, k_pages, v_pages, hq, hkv, d, scale, q_off=0, out_off=0):
-    """Attention over 8-bit pages, and over pages of either kind that groups of sequences share (``batch.prefix``): queries are the columns
-    q_off .. of ``qkv``, results the columns out_off .. of ``out``.  They may be the very same columns, and else share no memory."""
+    """Attention over 8-bit pages, and over pages of either kind that groups of sequences share (``batch.prefix``) or for trees of drafted tokens
+    (``batch.tree``): queries are the columns q_off .. of ``qkv``, results the columns out_off .. of ``out``.  They may be the very same columns, and
+    else share no memory."""
     dev = qkv.get_device()
     if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
@@ -387,16 +381,70 @@ def attention_pages(qkv, out, batch, k_pages, v_pages, hq, hkv, d, scale, q_off=
         if _wrong_ints(dev, p.block_tables, p.lens, p.first) or p.block_tables.shape[0] < G or p.lens.numel() < G or p.first.numel() < G + 1:
             raise ValueError(f"attention: prefix.block_tables, lens and first are contiguous int32 on {qkv.device}, of {G} groups or more")
         g = (p.block_tables.data_ptr(), p.block_tables.shape[1], p.lens.data_ptr(), p.first.data_ptr(), G, p.max_len, p.max_rows)
+    tree = ()
+    if batch.tree is not None:
+        masks = batch.tree.masks
+        if _wrong_ints(dev, masks) or masks.dim() != 2 or masks.shape[0] < T or 32 * masks.shape[1] < batch.max_q:
+            raise ValueError(f"attention: masks of a tree are contiguous int32 on {qkv.device}, a bit for each of {batch.max_q} tokens, {T} rows or more, "
+                             f"got {masks.dtype} {tuple(masks.shape)}")
+        tree = (masks.data_ptr(), masks.shape[1])
     lib = _lib.load()
-    floats = lib.llmss_attn_pages_scratch_floats(B, batch.max_q, batch.max_kv, T, hq, hkv, d, shape[2], fmt, g[4], g[5], g[6])
+    floats_of, call = (lib.llmss_attn_tree_scratch_floats, lib.llmss_attn_tree) if tree else (lib.llmss_attn_pages_scratch_floats, lib.llmss_attn_pages)
+    floats = floats_of(B, batch.max_q, batch.max_kv, T, hq, hkv, d, shape[2], fmt, g[4], g[5], g[6])
     # a scratch of the call's own: two streams, or two captured graphs, never meet in it
     scratch = torch.empty(floats, dtype=torch.float32, device=qkv.device) if floats else None
     launched = C.c_int(0)
-    rc = lib.llmss_attn_pages(q_at, ldq, k.data_ptr(), ks, v.data_ptr(), vs, bt.data_ptr(), bt.shape[1], sl.data_ptr(),
-                              out_at, ldo, cu_q.data_ptr(), B, batch.max_q, batch.max_kv, T, hq, hkv, d, shape[2], shape[0],
-                              float(scale), fmt, _DT[dtype], *g, None if scratch is None else scratch.data_ptr(), floats, C.addressof(launched), _stream())
-    _lib.check(rc, "llmss_attn_pages")
+    rc = call(q_at, ldq, k.data_ptr(), ks, v.data_ptr(), vs, bt.data_ptr(), bt.shape[1], sl.data_ptr(),
+              out_at, ldo, cu_q.data_ptr(), B, batch.max_q, batch.max_kv, T, hq, hkv, d, shape[2], shape[0],
+              float(scale), fmt, _DT[dtype], *g, *tree, None if scratch is None else scratch.data_ptr(), floats, C.addressof(launched), _stream())
+    _lib.check(rc, "llmss_attn_tree" if tree else "llmss_attn_pages")
     _count(launched.value)
+
+
+def step_layout(context_lens, new_lens, pages, page_size, rows, max_new, page_counts=None, max_blocks=None, parents=None):
+    dev = context_lens.get_device()
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return step_layout(context_lens, new_lens, pages, page_size, rows, max_new, page_counts, max_blocks, parents)
+    B, mb, words = drafts.check_layout(context_lens, new_lens, pages, page_size, rows, max_new, page_counts, max_blocks, parents)
+    # one allocation: views of it are cheaper than tensors
+    lists = page_counts is not None
+    last, lens, cu, positions, slots, tables, masks = torch.empty(4 * B + 1 + rows * (2 + words) + (B * mb if lists else 0), dtype=torch.int32, device=context_lens.device) \
+        .split([2 * B, B, B + 1, rows, rows, B * mb if lists else 0, rows * words])
+    tables = tables.view(B, mb) if lists else pages if pages.shape[0] == B else pages[:B]
+    rc = _lib.load().llmss_step_layout(context_lens.data_ptr(), new_lens.data_ptr(), pages.data_ptr(), pages.numel(), page_counts.data_ptr() if lists else None,
+                                       parents.data_ptr() if words else None, last.data_ptr(), lens.data_ptr(), cu.data_ptr(), positions.data_ptr(),
+                                       slots.data_ptr(), tables.data_ptr() if lists else None, masks.data_ptr() if words else None, B, rows, max_new,
+                                       page_size, mb, words, _stream())
+    _lib.check(rc, "llmss_step_layout")
+    _count()
+    return drafts.StepLayout(positions, slots, lens, cu, last.view(torch.int64), tables, masks.view(rows, words) if parents is not None else None)
+
+
+_MAX_SETS = 8          # cache tensors of one launch
+
+
+def accept_drafts(sampled, batch, pages):
+    dev = sampled.get_device()
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return accept_drafts(sampled, batch, pages)
+    planes, blocks, heads, size = drafts.check_accept(sampled, batch, pages)
+    B, wide, parents = batch.num_seqs, batch.max_q, batch.tree.parents
+    tokens, path, counts, context = torch.empty(2 * B * (wide + 1), dtype=torch.int32, device=sampled.device).split([B * wide, B * wide, B, B])
+    outs = (tokens.data_ptr(), counts.data_ptr(), path.data_ptr(), context.data_ptr())
+    pages = [x for x in pages if x.numel()]
+    lib = _lib.load()
+    for i in range(0, max(1, len(pages)), _MAX_SETS):
+        some = pages[i:i + _MAX_SETS]
+        bases = (C.c_void_p * _MAX_SETS)(*[x.data_ptr() for x in some])
+        widths = (C.c_int * _MAX_SETS)(*[x.numel() // (planes * blocks * heads * size) * x.element_size() for x in some])
+        rc = lib.llmss_accept_drafts(batch.tokens.data_ptr(), parents.data_ptr(), sampled.data_ptr(), batch.cu_q.data_ptr(), batch.seq_lens.data_ptr(),
+                                     batch.block_tables.data_ptr(), *(outs if i == 0 else (None,) * 4), C.addressof(bases), C.addressof(widths), len(some),
+                                     planes, blocks, heads, size, B, parents.numel(), wide, batch.block_tables.shape[1], _stream())
+        _lib.check(rc, "llmss_accept_drafts")
+        _count()
+    return drafts.Accepted(tokens.view(B, wide), counts, path.view(B, wide), context)
 
 
 # --------------------------------------------------------------------------- embed / sample

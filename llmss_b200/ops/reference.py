@@ -13,6 +13,7 @@ from typing import Optional, Tuple
 import torch
 import torch.nn.functional as F
 
+from . import drafts
 from .pages import QuantPages, quantise
 
 ACT_NONE, ACT_GELU_TANH, ACT_GELU_ERF, ACT_RELU, ACT_SILU, ACT_RELU2 = 0, 1, 2, 3, 4, 5
@@ -150,7 +151,8 @@ def rope_kv_write_q8(qkv, positions, slot_mapping, k_pages, v_pages, hq: int, hk
 
 
 def attention_pages(q, k_pages, v_pages, batch, scale: float):
-    """attention_paged over 16-bit pages or QuantPages; a sequence's first tokens come from the pages of its group in ``batch.prefix``."""
+    """attention_paged over 16-bit pages or QuantPages; a sequence's first tokens come from the pages of its group in ``batch.prefix``, and rows of a tree
+    (``batch.tree``) see those of its new tokens that their masks name."""
     T, hq, d = q.shape
     hkv, bs = k_pages.shape[1], k_pages.shape[2]
     out = torch.zeros(T, hq, d, dtype=q.dtype, device=q.device)
@@ -177,15 +179,96 @@ def attention_pages(q, k_pages, v_pages, batch, scale: float):
               for x in (k_pages, v_pages)]
         k, v = (x.repeat_interleave(hq // hkv, dim=0) for x in kv)
         s = torch.matmul(q[q0:q1].float().transpose(0, 1), k.transpose(1, 2)) * scale
-        hidden = torch.arange(L, device=q.device) > torch.arange(L - (q1 - q0), L, device=q.device)[:, None]
+        if batch.tree is None:
+            hidden = torch.arange(L, device=q.device) > torch.arange(L - (q1 - q0), L, device=q.device)[:, None]
+        else:
+            hidden = ~tree_sees(batch.tree.masks[q0:q1], torch.arange(L, device=q.device) - (L - (q1 - q0)))
         p = torch.softmax(s.masked_fill(hidden, float("-inf")), dim=-1)
         bad = ~torch.isfinite(v)
         o = torch.matmul(p, v.masked_fill(bad, 0))
         for key in bad.any(-1).any(0).nonzero().flatten().tolist():      # to the rows that see the key alone: 0 x NaN is NaN
-            o[:, max(0, key - (L - (q1 - q0))):] += v[:, key:key + 1].masked_fill(~bad[:, key:key + 1], 0)
-        o[:, :max(0, q1 - q0 - L)] = 0                      # rows in front of the sequence's first token see nothing
+            o[:, ~hidden[:, key]] += v[:, key:key + 1].masked_fill(~bad[:, key:key + 1], 0)
+        o[:, hidden.all(1)] = 0                             # rows that see nothing, as those in front of the sequence's first token
         out[q0:q1] = o.transpose(0, 1).to(q.dtype)
     return out
+
+
+def tree_sees(masks, place):
+    """[rows, keys]: whether a row of a tree sees a key, by the key's place among the sequence's new tokens (below 0: a cached one)."""
+    w = place.clamp(min=0) // 32
+    inside = w < masks.shape[1]
+    if masks.shape[1] == 0:
+        bits = torch.zeros(masks.shape[0], place.numel(), dtype=torch.bool, device=masks.device)
+    else:
+        bits = (masks[:, w.clamp(max=masks.shape[1] - 1)] >> (place % 32) & 1).bool()
+    return (place < 0) | (inside & bits)
+
+
+def step_layout(context_lens, new_lens, pages, page_size, rows, max_new, page_counts=None, max_blocks=None, parents=None):
+    B, max_blocks, words = drafts.check_layout(context_lens, new_lens, pages, page_size, rows, max_new, page_counts, max_blocks, parents)
+    dev, i32 = context_lens.device, dict(dtype=torch.int32)
+    up = parents.tolist() if words else None
+    positions, slots, masks = [0] * rows, [-1] * rows, [[0] * words for _ in range(rows)]
+    cu, lens, tables, at = [0], [], [], 0
+    if page_counts is not None:
+        flat = pages.tolist()
+        for n in page_counts.tolist():
+            tables.append(flat[at:at + max(n, 0)])
+            at += max(n, 0)
+    else:
+        tables = pages[:B].tolist()
+    for ctx, n, table in zip(context_lens.tolist(), new_lens.tolist(), tables):
+        ctx, row0 = max(ctx, 0), cu[-1]
+        n = min(max(n, 0), rows - row0)
+        for j in range(n):
+            block = table[(ctx + j) // page_size] if (ctx + j) // page_size < len(table) else -1
+            slots[row0 + j] = block * page_size + (ctx + j) % page_size if block >= 0 else -1
+            positions[row0 + j] = ctx + j
+            if words:
+                node, depth = j, -1
+                while node >= 0:
+                    depth += 1
+                    if node < 32 * words:
+                        masks[row0 + j][node // 32] |= 1 << node % 32
+                    node = up[row0 + node] if up[row0 + node] < node else -1
+                positions[row0 + j] = ctx + depth
+        cu.append(row0 + n)
+        lens.append(ctx + n)
+    bt = torch.zeros(B, max_blocks, **i32)
+    for i, t in enumerate(tables):
+        k = min(len(t), max_blocks)
+        bt[i, :k] = torch.tensor(t[:k], **i32)
+    words_of = torch.tensor([[w - (1 << 32) if w >> 31 else w for w in m] for m in masks], **i32).reshape(rows, words)
+    return drafts.StepLayout(torch.tensor(positions, **i32).to(dev), torch.tensor(slots, **i32).to(dev), torch.tensor(lens, **i32).to(dev),
+                             torch.tensor(cu, **i32).to(dev), (torch.tensor(cu[1:], dtype=torch.int64) - 1).to(dev), bt.to(dev),
+                             words_of.to(dev) if parents is not None else None)
+
+
+def accept_drafts(sampled, batch, pages):
+    planes, blocks, heads, size = drafts.check_accept(sampled, batch, pages)
+    B, wide, dev, i32 = batch.num_seqs, batch.max_q, sampled.device, dict(dtype=torch.int32)
+    T = batch.tree.parents.numel()
+    cu = [min(max(c, 0), T) for c in batch.cu_q.tolist()]
+    tokens, parents, got, lens = batch.tokens.tolist(), batch.tree.parents.tolist(), sampled.tolist(), batch.seq_lens.tolist()
+    out, path, counts, context = torch.full((B, wide), -1, **i32), torch.full((B, wide), -1, **i32), [], []
+    rows = [x.view(planes, blocks, heads, size, -1) for x in pages if x.numel()]
+    for i in range(B):
+        row0, n = cu[i], min(max(cu[i + 1] - cu[i], 0), wide)
+        ctx, node, k = lens[i] - n, 0 if n > 0 else -1, 0
+        table = batch.block_tables[i].tolist()
+        block_of = lambda key: table[key // size] if 0 <= key < len(table) * size and 0 <= table[key // size] < blocks else -1
+        while node >= 0:
+            path[i, k], out[i, k] = node, got[row0 + node]
+            if node != k and rows:
+                src, dst = block_of(ctx + node), block_of(ctx + k)
+                if src >= 0 and dst >= 0:
+                    for x in rows:
+                        x[:, dst, :, (ctx + k) % size] = x[:, src, :, (ctx + node) % size]
+            k += 1
+            node = next((c for c in range(node + 1, n) if parents[row0 + c] == node and tokens[row0 + c] == got[row0 + node]), -1)
+        counts.append(k)
+        context.append(ctx + k)
+    return drafts.Accepted(out.to(dev), torch.tensor(counts, **i32).to(dev), path.to(dev), torch.tensor(context, **i32).to(dev))
 
 
 def attention_paged(q, k_cache, v_cache, block_tables, seq_lens, cu_q, scale: float):

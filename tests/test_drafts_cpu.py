@@ -1,0 +1,256 @@
+"""Steps that check drafted tokens, in plain form on the CPU: their metadata, attention of trees, what is accepted, what is refused."""
+import random
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from drafts_oracle import ancestors, expected, path_of, random_parents, set_masks, words_of
+from llmss_b200 import ops
+from llmss_b200.engine.batch import BatchInput, DraftTree
+from llmss_b200.engine.kv_cache import KVCache, QuantKVCache
+from llmss_b200.ops.pages import QuantPages
+from pages_oracle import make_batch, make_pages
+
+I8, E4 = torch.int8, torch.float8_e4m3fn
+
+
+def ints(*v, **kw):
+    return torch.tensor(*v, dtype=torch.int32, **kw)
+
+
+# ----------------------------------------------------------------------------- metadata
+LENGTHS = {
+    "one": ([5], [1], 16),
+    "step": ([7, 16, 0, 31], [1, 1, 1, 1], 16),
+    "ragged": ([0, 3, 64, 100], [9, 1, 64, 33], 64),
+    "nothing_new": ([4, 9, 2], [0, 3, 0], 8),
+    "no_sequence": ([], [], 16),
+    "page_of_one": ([3, 0], [4, 2], 1),
+}
+
+
+def layout_lists(ctx, new, page, seed=0):
+    rng = random.Random(seed)
+    need = [-(-(c + n) // page) for c, n in zip(ctx, new)]
+    ids = list(range(1, 1 + sum(need)))
+    rng.shuffle(ids)
+    tables, at = [], 0
+    for k in need:
+        tables.append(ids[at:at + k])
+        at += k
+    return tables
+
+
+def layout_expected(ctx, new, tables, page, rows, width, trees, words):
+    cu, pos, slots, sets = [0], [], [], []
+    for i, (c, n) in enumerate(zip(ctx, new)):
+        cu.append(cu[-1] + n)
+        slots += [tables[i][(c + j) // page] * page + (c + j) % page for j in range(n)]
+        seen = ancestors(trees[i]) if trees else [None] * n
+        pos += [c + (len(s) - 1 if trees else j) for j, s in enumerate(seen)]
+        sets += seen
+    pad = rows - len(pos)
+    return dict(cu_q=cu, positions=pos + [0] * pad, slot_mapping=slots + [-1] * pad, seq_lens=[c + n for c, n in zip(ctx, new)], last_idx=[x - 1 for x in cu[1:]],
+                block_tables=[t + [0] * (width - len(t)) for t in tables], masks=words_of(sets + [set()] * pad, words).tolist() if trees is not None else None)
+
+
+@pytest.mark.parametrize("tree", [None, "chain", "star", "forest", "any"])
+@pytest.mark.parametrize("lists", [True, False])
+@pytest.mark.parametrize("name", sorted(LENGTHS))
+def test_step_layout(name, lists, tree):
+    ctx, new, page = LENGTHS[name]
+    tables, width, rows = layout_lists(ctx, new, page), 13, sum(new) + 3
+    width = max([13] + [len(t) for t in tables])
+    trees = None if tree is None else [random_parents(n, random.Random(i), tree) for i, n in enumerate(new)]
+    up = None if tree is None else ints([p for t in trees for p in t] + [7] * 3)
+    most = max(new, default=0)
+    padded = [t + [0] * (width - len(t)) for t in tables]
+    if lists:
+        got = ops.step_layout(ints(ctx), ints(new), ints([b for t in tables for b in t]), page, rows, most, page_counts=ints([len(t) for t in tables]),
+                              max_blocks=width, parents=up)
+    else:
+        got = ops.step_layout(ints(ctx), ints(new), ints(padded).reshape(len(new), width), page, rows, most, parents=up)
+    want = layout_expected(ctx, new, tables, page, rows, width, trees, -(-most // 32))
+    for n, x in want.items():
+        y = getattr(got, n)
+        assert (y is None) == (x is None)
+        if x is not None:
+            assert y.tolist() == x, n
+    assert got.last_idx.dtype == torch.int64 and all(getattr(got, n).dtype == torch.int32 for n in ("cu_q", "positions", "slot_mapping", "seq_lens", "block_tables"))
+
+
+def test_step_layout_of_lengths_that_do_not_fit():
+    """Rows cut off, lengths below zero, lists without a page, parents behind their children."""
+    table = ints([[3, -1], [5, 6], [7, 8]])
+    got = ops.step_layout(ints([6, -4, 2]), ints([4, -1, 5]), table, 4, 7, 5, parents=ints([-1, 2, 1, 0, 0, -5, 1]))
+    assert got.cu_q.tolist() == [0, 4, 4, 7] and got.seq_lens.tolist() == [10, 0, 5]
+    assert got.slot_mapping.tolist() == [-1] * 4 + [30, 31, 32]
+    assert got.positions.tolist() == [6, 6, 7, 7, 2, 2, 3]
+    assert got.masks[:, 0].tolist() == [1, 2, 6, 9, 1, 2, 6]
+    short = ops.step_layout(ints([2, 2]), ints([2, 3]), ints([9, 4]), 2, 5, 3, page_counts=ints([1, 1]), max_blocks=3)
+    assert short.slot_mapping.tolist() == [-1] * 5 and short.block_tables.tolist() == [[9, 0, 0], [4, 0, 0]]
+
+
+def test_masks_end_at_the_bound():
+    """A bound below the longest tree: its masks end there, positions do not."""
+    got = ops.step_layout(ints([0]), ints([40]), ints([[1, 2, 3]]), 16, 40, 32, parents=ints([j - 1 for j in range(40)]))
+    assert got.positions.tolist() == list(range(40))
+    assert got.masks[:, 0].tolist() == [-1 if j >= 31 else (1 << j + 1) - 1 for j in range(40)]
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(context_lens=torch.zeros(2)), ValueError), (dict(new_lens=ints([1])), ValueError), (dict(pages=ints([1, 2])), ValueError),
+    (dict(pages=ints([[1, 2]])), ValueError), (dict(max_blocks=3), ValueError), (dict(page_size=0), ValueError), (dict(rows=-1), ValueError),
+    (dict(max_new=-1), ValueError), (dict(parents=ints([0])), ValueError), (dict(parents=torch.zeros(4, dtype=torch.int64)), ValueError),
+    (dict(parents=ints([0] * 4), max_new=1025), ValueError), (dict(pages=ints([[1, 2], [3, 4], [5, 6], [7, 8]])[::2]), ValueError),
+    (dict(pages=ints([1, 2, 3]), page_counts=ints([2, 1])), ValueError), (dict(pages=ints([1, 2, 3]), page_counts=ints([3]), max_blocks=2), ValueError),
+    (dict(page_counts=ints([2, 2]), max_blocks=2), ValueError)])
+def test_step_layout_refusals(change, error):
+    args = dict(context_lens=ints([3, 4]), new_lens=ints([1, 2]), pages=ints([[1, 2], [3, 4]]), page_size=4, rows=4, max_new=2)
+    ops.step_layout(**args)
+    with pytest.raises(error):
+        ops.step_layout(**{**args, **change})
+
+
+@pytest.mark.parametrize("pad_to", [1, 8])
+def test_build_goes_by_the_lengths(pad_to):
+    new, ctx, page = [[5, 6, 7], [9], list(range(20))], [4, 31, 0], 16
+    tables = layout_lists(ctx, [len(n) for n in new], page)
+    b = BatchInput.build(new, ctx, tables, page, "cpu", max_blocks=5, pad_to=pad_to, state_slots=[2, 0, 1])
+    rows = 24
+    want = layout_expected(ctx, [3, 1, 20], tables, page, rows, 5, None, 0)
+    assert b.tokens.tolist() == [t for n in new for t in n] and b.tokens.numel() == rows if pad_to == 1 else b.tokens.numel() == rows
+    for n in ("positions", "slot_mapping", "seq_lens", "cu_q", "last_idx", "block_tables"):
+        assert getattr(b, n).tolist() == want[n]
+    assert (b.num_seqs, b.max_q, b.max_kv, b.is_decode, b.is_fresh_prefill) == (3, 20, 32, False, False) and b.state_slots.tolist() == [2, 0, 1]
+    assert b.tree is None
+    with pytest.raises(IndexError):
+        BatchInput.build([[1] * 20], [13], [[1, 2]], 16, "cpu")
+    with pytest.raises(ValueError):
+        BatchInput.build([[1]], [0], [[1, 2]], 16, "cpu", max_blocks=1)
+    with pytest.raises(ValueError):
+        BatchInput.build([[1, 2]], [0], [[1, 2]], 16, "cpu", parents=[[-1]])
+
+
+# ----------------------------------------------------------------------------- attention
+@pytest.mark.parametrize("kind", [None, I8, E4])
+@pytest.mark.parametrize("groups", [[], [([1, 2], 32)]])
+def test_rows_of_a_tree_see_their_ancestors(kind, groups):
+    hq, hkv, d, new, ctx = 4, 2, 64, [1, 9, 40, 0, 3], [0, 40, 33, 5, 17]
+    batch, seen = make_batch(new, ctx, 16, groups, "cpu")
+    rng = random.Random(1)
+    sets = [s for n in new for s in ancestors(random_parents(n, rng))]
+    set_masks(batch, seen, sets)
+    q = torch.randn(sum(new), hq * d, generator=torch.Generator().manual_seed(1)).bfloat16()
+    k, v = (make_pages(seen.blocks, hkv, 16, d, kind, torch.bfloat16, "cpu", seed=i) for i in range(2))
+    out = ops.attention(q, torch.empty_like(q), batch, k, v, hq, hkv, d, d ** -0.5, 0, 0, 0)
+    want, tol, less = expected(q, k, v, batch, seen, hq, hkv, d, d ** -0.5)
+    assert ((out.double() - want).abs() <= tol).all() and not ((less - want).abs() <= tol).all()
+
+
+def test_a_chain_is_causal_attention():
+    hq, hkv, d, new, ctx = 4, 2, 64, [1, 9, 40], [0, 40, 33]
+    batch, seen = make_batch(new, ctx, 16, [], "cpu")
+    q = torch.randn(sum(new), hq * d).bfloat16()
+    k, v = (make_pages(seen.blocks, hkv, 16, d, I8, torch.bfloat16, "cpu", seed=i) for i in range(2))
+    call = lambda: ops.attention(q, torch.empty_like(q), batch, k, v, hq, hkv, d, d ** -0.5, 0, 0, 0)
+    plain = call()
+    set_masks(batch, seen, [s for n in new for s in ancestors(random_parents(n, None, "chain"))])
+    assert torch.equal(call(), plain)
+
+
+def test_rows_that_see_nothing_and_values_that_no_row_sees():
+    """Masks need not be a tree's: empty ones, and a NaN in the place of a token that nobody sees."""
+    hq, hkv, d = 2, 1, 64
+    batch, seen = make_batch([3, 2], [0, 5], 16, [], "cpu")
+    set_masks(batch, seen, [{0, 2}, set(), {0}, set(), {0, 1}])
+    q = torch.randn(5, hq * d).bfloat16()
+    k, v = (make_pages(seen.blocks, hkv, 16, d, None, torch.bfloat16, "cpu", seed=i) for i in range(2))
+    v[seen.tables[0][0], 0, 1] = float("nan")
+    out = ops.attention(q, torch.full_like(q, 7.0), batch, k, v, hq, hkv, d, d ** -0.5, 0, 0, 0)
+    assert not out[1].any() and torch.isfinite(out.float()).all()
+    v[seen.tables[0][0], 0, 1] = 0.5
+    want, tol, _ = expected(q, k, v, batch, seen, hq, hkv, d, d ** -0.5)
+    assert ((out.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("name,args", [("latent_attention", (torch.zeros(1, 8), torch.zeros(1, 16, 8))), ("causal_conv", (torch.zeros(1, 4), None, None, 0)),
+                                       ("token_shift", (torch.zeros(1, 4), None)), ("attention_bias", (torch.zeros(1, 8), None, None))])
+def test_other_operators_refuse_trees(name, args):
+    batch = SimpleNamespace(tree=DraftTree(parents=ints([-1]), masks=ints([[1]])))
+    rest = {"latent_attention": (1, 8, 1.0, torch.float32), "causal_conv": (None,), "token_shift": (None,), "attention_bias": (1, 1, 8, 8, 1.0, None)}[name]
+    with pytest.raises(ValueError, match="trees"):
+        getattr(ops, name)(*args, batch, *rest)
+
+
+# ----------------------------------------------------------------------------- acceptance
+def drafted(new, ctx, page, vocab, seed, shape="any"):
+    """A batch of trees over scattered pages with few different tokens, so that paths are long and children alike."""
+    rng = random.Random(seed)
+    trees = [random_parents(n, rng, shape) for n in new]
+    tables = layout_lists(ctx, new, page, seed)
+    batch = BatchInput.build([[rng.randrange(vocab) for _ in range(n)] for n in new], ctx, tables, page, "cpu", parents=trees)
+    return batch, trees, tables, ints([rng.randrange(vocab) for _ in range(sum(new))])
+
+
+@pytest.mark.parametrize("vocab", [1, 2, 5])
+@pytest.mark.parametrize("shape", ["any", "chain", "star", "forest"])
+@pytest.mark.parametrize("new,ctx,page", [([1], [0], 16), ([12], [9], 4), ([0, 7, 1, 40], [3, 0, 30, 16], 16)])
+def test_accept_drafts(new, ctx, page, shape, vocab):
+    batch, trees, tables, sampled = drafted(new, ctx, page, vocab, 3, shape)
+    blocks = 1 + sum(len(t) for t in tables)
+    caches = [KVCache(3, blocks, page, 2, 8, torch.bfloat16, "cpu"), QuantKVCache(2, blocks, page, 3, 8, "fp8", "cpu"), QuantKVCache(2, blocks, page, 3, 8, "int8", "cpu")]
+    for cache in caches:
+        for i, x in enumerate(cache.row_tensors()):
+            x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(i)).mul(20).to(x.dtype))
+        before = [x.clone() for x in cache.row_tensors()]
+        got = ops.accept_drafts(sampled, batch, cache.row_tensors())
+        at = 0
+        for i, n in enumerate(new):
+            tok, smp = batch.tokens[at:at + n].tolist(), sampled[at:at + n].tolist()
+            path = path_of(trees[i], tok, smp)
+            pad = [-1] * (batch.max_q - len(path))
+            assert got.path[i].tolist() == path + pad and got.tokens[i].tolist() == [smp[p] for p in path] + pad
+            assert int(got.counts[i]) == len(path) and int(got.context_lens[i]) == ctx[i] + len(path)
+            for x, old in zip(cache.row_tensors(), before):
+                place = lambda y, key: y[:, :, tables[i][key // page], :, key % page]
+                for key in range(len(tables[i]) * page):
+                    k = key - ctx[i]
+                    want = place(old, ctx[i] + path[k] if 0 <= k < len(path) else key)
+                    assert torch.equal(place(x, key).float(), want.float())
+            at += n
+        assert torch.equal(cache.row_tensors()[0][:, :, 0].float(), before[0][:, :, 0].float())
+
+
+def test_accept_drafts_without_a_cache_and_with_tables_that_end():
+    batch, trees, tables, sampled = drafted([6], [3], 4, 1, 0, "star")
+    assert ops.accept_drafts(sampled, batch, []).path[0].tolist() == [0, 1, -1, -1, -1, -1]
+    batch.tree.parents[:] = ints([-1, 9, 0, 0, 2, 4])
+    cache = torch.arange(4 * 4 * 2.0).reshape(1, 1, 4, 1, 4, 2).contiguous()
+    batch.block_tables[:] = ints([[2, -1, 3]])
+    old = cache.clone()
+    got = ops.accept_drafts(sampled, batch, [cache])
+    assert got.path[0].tolist() == [0, 2, 4, 5, -1, -1] and torch.equal(cache, old)          # rows 4, 5, 6 have no page
+    batch.block_tables[:] = ints([[2, 1, 9]])                                               # block 9 does not exist
+    ops.accept_drafts(sampled, batch, [cache])
+    old[0, 0, 1, 0, 0], old[0, 0, 1, 0, 1] = old[0, 0, 1, 0, 1].clone(), old[0, 0, 1, 0, 3].clone()
+    assert torch.equal(cache, old)
+
+
+def test_accept_drafts_refusals():
+    batch, _, _, sampled = drafted([3, 2], [4, 4], 4, 2, 0)
+    good = torch.zeros(2, 2, 8, 3, 4, 16)
+    ops.accept_drafts(sampled, batch, [good, torch.zeros(2, 2, 8, 3, 4)])
+    for pages in ([torch.zeros(8, 4)], [good, torch.zeros(2, 2, 8, 3, 5)], [good.transpose(0, 1)[1:]], [good[..., :8]]):
+        with pytest.raises(ValueError):
+            ops.accept_drafts(sampled, batch, pages)
+    for s in (sampled[:3], sampled.long(), sampled[None].expand(2, -1)[:, ::2]):
+        with pytest.raises(ValueError):
+            ops.accept_drafts(s, batch, [good])
+    tree, batch.tree = batch.tree, None
+    with pytest.raises(ValueError, match="tree"):
+        ops.accept_drafts(sampled, batch, [good])
+    batch.tree, batch.max_q = tree, 1025
+    with pytest.raises(ValueError, match="1024"):
+        ops.accept_drafts(sampled, batch, [good])

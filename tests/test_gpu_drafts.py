@@ -1,0 +1,312 @@
+"""Steps that check drafted tokens on the GPU: metadata, attention of trees, what is accepted."""
+import random
+
+import pytest
+import torch
+
+from drafts_oracle import ancestors, expected, random_parents, set_masks
+from llmss_b200 import ops
+from llmss_b200.engine.batch import BatchInput
+from llmss_b200.engine.kv_cache import KVCache, QuantKVCache
+from llmss_b200.ops import reference as ref
+from llmss_b200.ops.pages import QuantPages
+from pages_oracle import make_batch, make_pages
+
+pytestmark = pytest.mark.gpu
+
+BF, HF = torch.bfloat16, torch.float16
+I8, E4 = torch.int8, torch.float8_e4m3fn
+INF, NAN = float("inf"), float("nan")
+
+
+def cuda(*xs):
+    return [x if x is None else x.cuda() for x in xs]
+
+
+def ints(*v):
+    return torch.tensor(*v, dtype=torch.int32)
+
+
+def queries(rows, width, dtype, seed=2):
+    return torch.randn(rows, width, generator=torch.Generator().manual_seed(seed)).to(dtype).cuda()
+
+
+# ----------------------------------------------------------------------------- metadata
+@pytest.mark.parametrize("tree", [None, "chain", "star", "forest", "any"])
+@pytest.mark.parametrize("lists", [True, False])
+@pytest.mark.parametrize("seqs,mean,page", [(1, 1, 16), (1, 300, 64), (3, 40, 16), (64, 1, 64), (70, 25, 32), (300, 5, 5), (9, 700, 16)])
+def test_step_layout(seqs, mean, page, lists, tree):
+    rng = random.Random(seqs + mean)
+    ctx, new = [rng.randrange(3 * mean + 5) for _ in range(seqs)], [rng.randrange(2 * mean) if seqs > 1 else mean for _ in range(seqs)]
+    counts = [max(0, -(-(c + n) // page) - (rng.random() < 0.1)) for c, n in zip(ctx, new)]         # some lists end early
+    flat = [rng.randrange(1, 5000) for _ in range(sum(counts))]
+    rows, most = sum(new) + rng.choice([0, 1, 300]), max(new)
+    up = None
+    if tree is not None:
+        if most > 1024:
+            pytest.skip("trees of up to 1024 tokens")
+        up = ints([p for n in new for p in random_parents(n, rng, tree)] + [3] * (rows - sum(new)))
+    if lists:
+        pages, extra = ints(flat), dict(page_counts=ints(counts), max_blocks=max(counts) + 2)
+    else:
+        table, at = torch.full((seqs + 1, max(counts) + 2), -1, dtype=torch.int32), 0
+        for i, k in enumerate(counts):
+            table[i, :k] = ints(flat[at:at + k])
+            at += k
+        pages, extra = table, {}
+    want = ops.step_layout(ints(ctx), ints(new), pages, page, rows, most, parents=up, **extra)
+    on = {n: x.cuda() if torch.is_tensor(x) else x for n, x in extra.items()}
+    got = ops.step_layout(ints(ctx).cuda(), ints(new).cuda(), pages.cuda(), page, rows, most, parents=None if up is None else up.cuda(), **on)
+    for name, a, b in zip(want._fields, want, got):
+        assert (a is None) == (b is None) and (a is None or (a.dtype is b.dtype and a.shape == b.shape and torch.equal(a, b.cpu()))), name
+
+
+def test_step_layout_of_lengths_that_do_not_fit():
+    args = [ints([6, -4, 2, 2 ** 31 - 1]), ints([4, -1, 5, 9]), ints([[3, -1], [5, 6], [7, 8], [1, 2]]), 4, 7, 9]
+    want = ref.step_layout(*args, parents=ints([-1, 2, 1, 0, 0, -5, 1]))
+    got = ops.step_layout(*cuda(*args[:3]), *args[3:], parents=ints([-1, 2, 1, 0, 0, -5, 1]).cuda())
+    for name, a, b in zip(want._fields, want, got):
+        if name != "seq_lens":                       # of 2^31 - 1 tokens and more there are none
+            assert torch.equal(a, b.cpu()), name
+    # counts far beyond the list: nothing is read behind it
+    got = ops.step_layout(*cuda(ints([0, 0, 0]), ints([3, 3, 3]), ints([9, 4])), 2, 9, 3, page_counts=ints([2 ** 31 - 1, 2 ** 31 - 1, 1]).cuda(), max_blocks=2)
+    assert got.slot_mapping.tolist() == [18, 19, 8] + [-1] * 6 and got.block_tables.tolist() == [[9, 4], [0, 0], [0, 0]]
+
+
+def test_build_is_the_same_on_both_devices():
+    rng = random.Random(3)
+    new, ctx = [[rng.randrange(99) for _ in range(n)] for n in (1, 40, 0, 7)], [5, 0, 3, 64]
+    tables = [[rng.randrange(1, 99) for _ in range(-(-(c + len(n)) // 16))] for n, c in zip(new, ctx)]
+    trees = [random_parents(len(n), rng) for n in new]
+    a, b = (BatchInput.build(new, ctx, tables, 16, dev, max_blocks=9, pad_to=16, state_slots=[1, 0, 3, 2], parents=trees) for dev in ("cpu", "cuda"))
+    for name in ("tokens", "positions", "slot_mapping", "block_tables", "seq_lens", "cu_q", "last_idx", "state_slots"):
+        x, y = getattr(a, name), getattr(b, name)
+        assert y.is_cuda and x.dtype is y.dtype and torch.equal(x, y.cpu())
+    assert torch.equal(a.tree.masks, b.tree.masks.cpu()) and torch.equal(a.tree.parents, b.tree.parents.cpu())
+
+
+# ----------------------------------------------------------------------------- attention
+# new tokens, cached ones, page size, groups
+TREES = {
+    "one_token": ([1], [37], 16, []),
+    "no_context": ([5, 20], [0, 0], 16, []),
+    "few": ([3, 1, 2, 4], [70, 9, 64, 0], 64, []),
+    "page_ends_inside": ([16, 9], [55, 120], 64, []),
+    "one_tile": ([12, 30, 1, 0, 17], [130, 250, 3, 20, 64], 32, []),
+    "many_tiles": ([130, 70], [300, 65], 64, []),
+    "longest": ([300, 5], [90, 700], 16, []),
+    "long_context": ([20, 6], [5000, 3001], 64, []),
+    "behind_a_prefix": ([9, 2, 33], [130, 64, 100], 64, [([0, 1, 2], 64)]),
+    "few_behind_a_prefix": ([2, 1, 3], [130, 64, 100], 64, [([0, 1], 64)]),
+}
+HEADS = [(4, 4, 64), (16, 2, 64), (8, 2, 128), (32, 8, 128), (4, 4, 256), (16, 1, 128), (6, 3, 96), (5, 1, 40)]
+
+
+@pytest.mark.parametrize("shape", ["any", "chain", "forest"])
+@pytest.mark.parametrize("kind,dtype", [(None, BF), (None, HF), (I8, BF), (E4, HF)])
+@pytest.mark.parametrize("hq,hkv,d", HEADS)
+@pytest.mark.parametrize("case", sorted(TREES))
+def test_rows_of_a_tree_see_their_ancestors(case, hq, hkv, d, kind, dtype, shape):
+    new, ctx, page, groups = TREES[case]
+    batch, seen = make_batch(new, ctx, page, groups, "cuda", seed=4)
+    rng = random.Random(len(case))
+    set_masks(batch, seen, [s for n in new for s in ancestors(random_parents(n, rng, shape))])
+    q = queries(sum(new), hq * d, dtype)
+    k, v = (make_pages(seen.blocks, hkv, page, d, kind, dtype, "cuda", seed=i) for i in range(2))
+    out = ops.attention(q, torch.full_like(q, NAN), batch, k, v, hq, hkv, d, d ** -0.5, 0, 0, 0)
+    want, tol, less = expected(q, k, v, batch, seen, hq, hkv, d, d ** -0.5)
+    assert ((out.double() - want).abs() <= tol).all(), f"{int((~((out.double() - want).abs() <= tol)).sum())} of {want.numel()}"
+    assert not ((less - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("kind", [None, I8])
+@pytest.mark.parametrize("hq,hkv,d", [(4, 4, 64), (8, 2, 128), (4, 4, 256), (6, 3, 96)])
+@pytest.mark.parametrize("case", sorted(TREES))
+def test_any_mask(case, hq, hkv, d, kind):
+    """Bits of any places, rows without one, more words than the batch needs, bits behind the last token."""
+    new, ctx, page, groups = TREES[case]
+    batch, seen = make_batch(new, ctx, page, groups, "cuda", seed=4)
+    rng = random.Random(len(case))
+    sets = [set(rng.sample(range(n + 3), rng.choice([0, 0, 1, n // 2, n]))) for n in new for _ in range(n)]
+    set_masks(batch, seen, sets, words=11)
+    q = queries(sum(new), hq * d, BF)
+    k, v = (make_pages(seen.blocks, hkv, page, d, kind, BF, "cuda", seed=i) for i in range(2))
+    out = ops.attention(q, torch.full_like(q, NAN), batch, k, v, hq, hkv, d, d ** -0.5, 0, 0, 0)
+    want, tol, _ = expected(q, k, v, batch, seen, hq, hkv, d, d ** -0.5)
+    assert ((out.double() - want).abs() <= tol).all()
+    at = 0
+    for n, c in zip(new, ctx):
+        for j in range(n):
+            if c == 0 and not any(x < n for x in sets[at + j]):
+                assert not out[at + j].any()
+        at += n
+
+
+@pytest.mark.parametrize("kind,dtype", [(None, BF), (None, HF), (I8, BF), (E4, HF)])
+@pytest.mark.parametrize("hq,hkv,d", [(4, 2, 64), (8, 2, 128), (4, 2, 256), (6, 2, 96)])
+@pytest.mark.parametrize("case", sorted(TREES))
+@pytest.mark.parametrize("filler", [NAN, INF])
+def test_what_a_row_does_not_see_does_not_reach_it(filler, case, hq, hkv, d, kind, dtype):
+    """A guess whose value or key is not finite reaches its descendants alone, all columns or one; results written over the queries are the same."""
+    new, ctx, page, groups = TREES[case]
+    if max(new) < 2:
+        pytest.skip("a tree of one token")
+    batch, seen = make_batch(new, ctx, page, groups, "cuda", seed=5)
+    rng = random.Random(len(case))
+    sets = [s for n in new for s in ancestors(random_parents(n, rng))]
+    set_masks(batch, seen, sets)
+    k, v = (make_pages(seen.blocks, hkv, page, d, kind, dtype, "cuda", seed=i) for i in range(2))
+    q = queries(sum(new), hq * d, dtype)
+    want, tol, _ = expected(q, k, v, batch, seen, hq, hkv, d, d ** -0.5)
+    seq = new.index(max(new))
+    row0 = sum(new[:seq])
+    for tok, pages in ((1, v), (max(new) - 1, v), (max(new) // 2, k)):
+        key, column = ctx[seq] + tok, d // 2 + 3
+        b, o = seen.tables[seq][key // page], key % page
+        if kind is None:
+            old = pages[b, 1, o, column].clone()
+            pages[b, 1, o, column] = filler
+        else:
+            old = pages.scale[b, 1, o].clone()
+            pages.scale[b, 1, o] = filler
+        out = ops.attention(q, torch.full_like(q, 7.0), batch, k, v, hq, hkv, d, d ** -0.5, 0, 0, 0)
+        over = q.clone()
+        ops.attention(over, over, batch, k, v, hq, hkv, d, d ** -0.5, 0, 0, 0)
+        assert ((over == out) | (torch.isnan(over) & torch.isnan(out))).all()
+        sees = torch.zeros(sum(new), hq, d, dtype=torch.bool, device="cuda")
+        for j in range(new[seq]):
+            if tok in sets[row0 + j]:
+                if pages is k or kind is not None:
+                    sees[row0 + j, hq // 2:] = True
+                else:
+                    sees[row0 + j, hq // 2:, column] = True
+        sees = sees.view(sum(new), -1)
+        off = (out.double() - want).abs()
+        assert (off <= tol)[~sees].all(), f"{int((~(off <= tol))[~sees].sum())} results that do not see it changed"
+        if filler != filler:
+            assert torch.isnan(out.float()[sees]).all()
+        elif pages is v:
+            assert (out.float()[sees] == INF).all() if kind is None else not torch.isfinite(out.float()[sees]).any()
+        if kind is None:
+            pages[b, 1, o, column] = old
+        else:
+            pages.scale[b, 1, o] = old
+
+
+@pytest.mark.parametrize("kind", [None, E4])
+@pytest.mark.parametrize("new", [[1, 2, 1], [9, 1, 30], [200, 3, 1]])
+def test_buffers_longer_than_the_batch_and_rows_of_no_sequence(new, kind):
+    hq, hkv, d = 8, 2, 128
+    batch, seen = make_batch(new, [90, 70, 64], 64, [], "cuda", seed=1)
+    T = sum(new)
+    rng = random.Random(0)
+    set_masks(batch, seen, [s for n in new for s in ancestors(random_parents(n, rng))])
+    k, v = (make_pages(seen.blocks, hkv, 64, d, kind, BF, "cuda", seed=i) for i in range(2))
+    q = queries(T + 5, hq * d, BF)
+    want, tol, _ = expected(q[2:2 + T], k, v, batch, seen, hq, hkv, d, d ** -0.5)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    batch.cu_q = torch.cat([batch.cu_q + 2, torch.tensor([T + 4, 0], **i32)])
+    batch.seq_lens = torch.cat([batch.seq_lens, torch.tensor([7, 7], **i32)])
+    batch.block_tables = torch.cat([batch.block_tables, batch.block_tables[:2]])
+    batch.tree.masks = torch.cat([torch.full((2, batch.tree.masks.shape[1]), -1, **i32), batch.tree.masks, torch.full((9, batch.tree.masks.shape[1]), -1, **i32)])
+    out = ops.attention(q, torch.full_like(q, 7.0), batch, k, v, hq, hkv, d, d ** -0.5, 0, 0, 0)
+    assert ((out[2:2 + T].double() - want).abs() <= tol).all() and (out[:2] == 7).all() and (out[2 + T:] == 7).all()
+
+
+@pytest.mark.parametrize("length", [0, 1, 2, 5, -3])
+def test_sequences_shorter_than_their_rows(length):
+    """Rows in front of a sequence's first token have no key of their own; a row that sees none is zero."""
+    hq, hkv, d, new = 8, 2, 128, [6, 40]
+    batch, seen = make_batch(new, [10, 20], 16, [], "cuda", seed=3)
+    batch.seq_lens[0] = length
+    rng = random.Random(0)
+    sets = [s for n in new for s in ancestors(random_parents(n, rng))]
+    set_masks(batch, seen, sets)
+    k, v = (make_pages(seen.blocks, hkv, 16, d, None, BF, "cuda", seed=i) for i in range(2))
+    q = queries(sum(new), hq * d, BF)
+    out = ops.attention(q, torch.full_like(q, NAN), batch, k, v, hq, hkv, d, d ** -0.5, 0, 0, 0)
+    for j in range(6):
+        if not any(x >= 6 - max(length, 0) for x in sets[j]):
+            assert not out[j].any()
+    if length >= 0:
+        want, tol, _ = expected(q, k, v, batch, seen, hq, hkv, d, d ** -0.5)
+        assert ((out.double() - want).abs() <= tol).all()
+
+
+def test_columns_of_wider_tensors_and_another_stream():
+    """Queries and outputs as columns of a layer's projection, on a stream of its own, with pages of another call beside it."""
+    hq, hkv, d, new = 8, 2, 128, [9, 40, 1]
+    batch, seen = make_batch(new, [90, 20, 33], 16, [], "cuda", seed=3)
+    rng = random.Random(0)
+    set_masks(batch, seen, [s for n in new for s in ancestors(random_parents(n, rng))])
+    k, v = (make_pages(seen.blocks, hkv, 16, d, None, BF, "cuda", seed=i) for i in range(2))
+    wide = queries(sum(new), 3 * hq * d, BF)
+    want, tol, _ = expected(wide[:, hq * d:2 * hq * d].contiguous(), k, v, batch, seen, hq, hkv, d, d ** -0.5)
+    out = torch.zeros(sum(new), 2 * hq * d, dtype=BF, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        ops.attention(wide, out, batch, k, v, hq, hkv, d, d ** -0.5, hq * d, 0, 0, out_off=hq * d)
+        torch.cuda.current_stream().synchronize()
+    assert ((out[:, hq * d:].double() - want).abs() <= tol).all() and not out[:, :hq * d].any()
+
+
+def test_attention_refusals():
+    batch, seen = make_batch([3, 2], [10, 20], 16, [], "cuda", seed=3)
+    set_masks(batch, seen, [{0}] * 5)
+    k, v = (make_pages(seen.blocks, 2, 16, 64, None, BF, "cuda", seed=i) for i in range(2))
+    q = queries(5, 4 * 64, BF)
+    call = lambda: ops.attention(q, torch.empty_like(q), batch, k, v, 4, 2, 64, 0.1, 0, 0, 0)
+    call()
+    good = batch.tree.masks
+    for masks in (good.cpu(), good.long(), good[:4], good.flatten(), good[:, :0], torch.cat([good, good], 1)[:, ::2]):
+        batch.tree.masks = masks
+        with pytest.raises(ValueError, match="masks"):
+            call()
+
+
+# ----------------------------------------------------------------------------- acceptance
+@pytest.mark.parametrize("vocab", [1, 3])
+@pytest.mark.parametrize("shape", ["any", "chain", "star"])
+@pytest.mark.parametrize("new,ctx,page", [([1], [0], 16), ([12], [9], 4), ([0, 7, 1, 40], [3, 0, 30, 16], 16), ([9] * 70, list(range(70)), 64), ([1000, 33], [5, 2], 64)])
+def test_accept_drafts(new, ctx, page, shape, vocab):
+    rng = random.Random(7)
+    trees = [random_parents(n, rng, shape) for n in new]
+    need = [-(-(c + n) // page) for c, n in zip(ctx, new)]
+    ids = list(range(1, 1 + sum(need)))
+    rng.shuffle(ids)
+    tables = [ids[sum(need[:i]):sum(need[:i + 1])] for i in range(len(new))]
+    batches = [BatchInput.build([[rng.randrange(vocab)] * n for n in new], ctx, tables, page, "cpu", parents=trees)]
+    batches[0].tokens.copy_(ints([rng.randrange(vocab) for _ in range(sum(new))]))
+    batches.append(BatchInput.build([[0] * n for n in new], ctx, tables, page, "cuda", parents=trees))
+    batches[1].tokens.copy_(batches[0].tokens)
+    sampled = ints([rng.randrange(vocab) for _ in range(sum(new))])
+    for make in (lambda dev: KVCache(3, 1 + len(ids), page, 2, 64, BF, dev), lambda dev: KVCache(2, 1 + len(ids), page, 3, 20, torch.float32, dev),
+                 lambda dev: KVCache(2, 1 + len(ids), page, 1, 5, HF, dev),
+                 lambda dev: QuantKVCache(2, 1 + len(ids), page, 3, 128, "fp8", dev), lambda dev: QuantKVCache(1, 1 + len(ids), page, 5, 8, "int8", dev)):
+        caches = [make("cpu"), make("cuda")]
+        for i, (x, y) in enumerate(zip(*(c.row_tensors() for c in caches))):
+            x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(i)).mul(20).to(x.dtype))
+            y.copy_(x)
+        want, got = (ops.accept_drafts(sampled.to(b.tokens.device), b, c.row_tensors()) for b, c in zip(batches, caches))
+        for a, b in zip(want, got):
+            assert a.dtype is b.dtype and torch.equal(a, b.cpu())
+        for x, y in zip(*(c.row_tensors() for c in caches)):
+            assert torch.equal(x.view(torch.uint8), y.cpu().view(torch.uint8))
+
+
+def test_accept_drafts_of_many_tensors_and_tables_that_end():
+    """A tensor per layer and side, more than a launch takes; pages that do not exist are left alone."""
+    tree = [-1, 0, 0, 2, 2, 4, 5]
+    batch = BatchInput.build([[1] * 7], [3], [[2, 1, 3]], 4, "cuda", parents=[tree])
+    batch.tree.parents.copy_(ints([-1, 9, 0, 9, 2, 4, 5]))
+    batch.block_tables.copy_(ints([[2, 77, 3]]))
+    cpu = BatchInput.build([[1] * 7], [3], [[2, 1, 3]], 4, "cpu", parents=[tree])
+    cpu.tree.parents.copy_(ints([-1, 9, 0, 9, 2, 4, 5]))
+    cpu.block_tables.copy_(ints([[2, 77, 3]]))
+    pages = [torch.randn(4, 2, 4, 8, generator=torch.Generator().manual_seed(i)) for i in range(19)]
+    on = [x.cuda() for x in pages]
+    sampled = torch.ones(7, dtype=torch.int32)
+    want, got = ops.accept_drafts(sampled, cpu, pages), ops.accept_drafts(sampled.cuda(), batch, on)
+    assert all(torch.equal(a, b.cpu()) for a, b in zip(want, got)) and all(torch.equal(x, y.cpu()) for x, y in zip(pages, on))
+    assert got.path[0].tolist() == [0, 2, 4, 5, 6, -1, -1]
+    assert ops.accept_drafts(sampled.cuda(), batch, []).counts.tolist() == [5]
