@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(128) attn_pages_any_kernel(const __grid_consta
 // A warp per query row and head joins the parts of its softmax: m = max m_i, l = sum l_i 2^(m_i - m), out = sum O_i 2^(m_i - m) / l.  Reads what the
 // kernels before it left in L2; launched to start as they end (programmatic dependent launch), so that it costs no launch latency of its own.
 // WARPS of them share a row where rows are few: parts are many then, and each costs a read from L2.
-template <typename T, int D, int WARPS>
+template <typename T, int D, int WARPS, bool TREE>
 __global__ void __launch_bounds__(256, D < 256 && WARPS == 1 ? 5 : 4) attn_pages_merge_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ PartArgs p) {
   constexpr int N = D / 32, VEC = N < 4 ? N : 4;          // columns of a lane, VEC neighbouring ones
   using Vec = typename std::conditional<VEC == 4, float4, float2>::type;
@@ -108,7 +108,16 @@ __global__ void __launch_bounds__(256, D < 256 && WARPS == 1 ? 5 : 4) attn_pages
   for (int i = 0; i < N; ++i) o[i] = 0.f;
   const Seg own = own_segment(a, s);
   const Seg gs = g >= 0 ? group_segment(a, g) : Seg{};
-  const bool sees = row_pos(a, s, t) >= 0, has_own = sees && own.hi > own.lo, has_group = sees && g >= 0 && gs.hi > 0;
+  bool sees;
+  if constexpr (TREE) {
+    // a cached token, or one of the new ones that lie in the cache (fewer than the rows where a length is too short)
+    const int ctx = tree_context(a, s), n = own.hi - ctx;
+    sees = ctx > 0;
+    for (int b = 0; b < n && !sees; b += 32) sees = (tree_bits(a, t, b) & bit_range(-ctx - b, n - 1 - b)) != 0;
+  } else {
+    sees = row_pos(a, s, t) >= 0;
+  }
+  const bool has_own = sees && own.hi > own.lo, has_group = sees && g >= 0 && gs.hi > 0;
   // parts lie in up to four runs: the own keys' first and others, the group's first and others (stretches of keys: the others only).  They are added in one
   // loop: with one per run a row waited for memory four times, and for the instructions of each
   // Places are counted in 16 bytes from the scratch's begin (p.slots): 32 bits, since registers decide how many rows are in flight.
@@ -235,7 +244,8 @@ int launch_merge(const AttnArgs& a, const PartArgs& p, int parts, cudaStream_t s
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  LLMSS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, shared ? attn_pages_merge_kernel<T, D, 8> : attn_pages_merge_kernel<T, D, 1>, a, p));
+  LLMSS_CHECK_CUDA(a.masks != nullptr ? cudaLaunchKernelEx(&cfg, shared ? attn_pages_merge_kernel<T, D, 8, true> : attn_pages_merge_kernel<T, D, 1, true>, a, p)
+                                      : cudaLaunchKernelEx(&cfg, shared ? attn_pages_merge_kernel<T, D, 8, false> : attn_pages_merge_kernel<T, D, 1, false>, a, p));
   return 0;
 }
 
@@ -345,7 +355,7 @@ int side_by_side(int64_t lists, int len, double own_lists, double own_bytes, dou
   return 148 - (int)lists * splits;
 }
 
-Plan plan_call(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv, int d, int page, int fmt, int groups, int g_max_len, int g_max_rows) {
+Plan plan_call(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv, int d, int page, int fmt, int groups, int g_max_len, int g_max_rows, bool tree) {
   Plan p;
   memset(&p, 0, sizeof(p));
   p.any = true;
@@ -363,7 +373,8 @@ Plan plan_call(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv
     // of a list takes whatever is left of it, and a block without keys is not free (a microsecond on its SM)
     const int keys = groups > 0 ? (max_kv - g_max_len > max_q ? max_kv - g_max_len : max_q) : max_kv;
     stretches((int64_t)p.tile.own_tiles * hkv * num_seqs, keys, groups > 0, p.own_splits, p.own_chunk);
-    p.direct = groups == 0 && p.own_splits == 1 && fmt != kF16Pages;      // (16-bit pages come here without groups where a prefix has no tokens, if at all)
+    // (causal rows over 16-bit pages come here without groups where a prefix has no tokens, if at all)
+    p.direct = groups == 0 && p.own_splits == 1 && (tree || fmt != kF16Pages);
     // Every row tile converts all codes for itself, which takes the tiled kernel from 1100 to 2000 clocks per 64 keys; once for all costs a pass over the
     // cache (about 1200 clocks of an SM per 64 keys, and a launch).  4 portions of 1000 tokens over 1800, 16 tiles each: 251 -> 183 us; three tiles 89 -> 87
     // (16 sequences 198 -> 170), two tiles 69 -> 68, one 47 -> 47: from three tiles on.  Up to 1 GB of scratch
@@ -459,8 +470,7 @@ int attend(const void* q, int64_t ldq, const void* k_pages, const float* k_scale
   LLMSS_REQUIRE(num_seqs >= 0 && max_q >= 0 && max_kv >= 0 && total_q >= 0 && groups >= 0, "attn_pages: negative size");
   if (num_seqs == 0 || total_q == 0 || max_q == 0) return 0;
   if (int e = check_args(a, fmt, dtype)) return e;
-  Plan plan = plan_call(num_seqs, max_q, max_kv, total_q, hq, hkv, d, block_size, fmt, a.groups, g_max_len, g_max_rows);
-  if (masks != nullptr) plan.any = true;
+  const Plan plan = plan_call(num_seqs, max_q, max_kv, total_q, hq, hkv, d, block_size, fmt, a.groups, g_max_len, g_max_rows, masks != nullptr);
   if (!plan.any) {
     LLMSS_REQUIRE(plan.floats == 0 || (scratch != nullptr && scratch_floats >= plan.floats && ((uintptr_t)scratch % 16) == 0), "attn_pages: %lld floats of 16-byte aligned scratch needed",
                   (long long)plan.floats);
@@ -553,7 +563,7 @@ int attend(const void* q, int64_t ldq, const void* k_pages, const float* k_scale
 LLMSS_API int64_t llmss_attn_pages_scratch_floats(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv, int d, int block_size, int fmt,
                                                   int groups, int g_max_len, int g_max_rows) {
   if (num_seqs <= 0 || total_q <= 0 || max_q <= 0) return 0;
-  return plan_call(num_seqs, max_q, max_kv, total_q, hq, hkv, d, block_size, fmt, g_max_len > 0 ? groups : 0, g_max_len, g_max_rows).floats;
+  return plan_call(num_seqs, max_q, max_kv, total_q, hq, hkv, d, block_size, fmt, g_max_len > 0 ? groups : 0, g_max_len, g_max_rows, false).floats;
 }
 
 // q [total_q][>= hq * d] (row stride ldq); K / V pages [num_blocks][hkv][block_size][d] of the queries' type (fmt 0) or of bytes with 32-bit scales
@@ -573,7 +583,8 @@ LLMSS_API int llmss_attn_pages(const void* q, int64_t ldq, const void* k_pages, 
 // The same for trees of drafted tokens (and their scratch).
 LLMSS_API int64_t llmss_attn_tree_scratch_floats(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv, int d, int block_size, int fmt,
                                                  int groups, int g_max_len, int g_max_rows) {
-  return 0;
+  if (num_seqs <= 0 || total_q <= 0 || max_q <= 0) return 0;
+  return plan_call(num_seqs, max_q, max_kv, total_q, hq, hkv, d, block_size, fmt, g_max_len > 0 ? groups : 0, g_max_len, g_max_rows, true).floats;
 }
 
 // llmss_attn_pages where a row sees all tokens in front of its sequence's new ones (those of its rows), and of the new ones those whose bit its mask

@@ -146,6 +146,15 @@ __device__ __forceinline__ int row_pos(const AttnArgs& a, int s, int t) {
   return min(a.seq_lens[s] - a.cu[s + 1] + t, a.max_blocks * a.page - 1);
 }
 
+// cached tokens of sequence s in front of its new ones
+__device__ __forceinline__ int tree_context(const AttnArgs& a, int s) { return a.seq_lens[s] - (a.cu[s + 1] - a.cu[s]); }
+
+// bits lo .. hi of a word, any numbers
+__device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
+  const uint32_t up_to = hi < 0 ? 0u : hi >= 31 ? ~0u : (2u << hi) - 1u;
+  return up_to & (lo <= 0 ? ~0u : lo >= 32 ? 0u : ~0u << lo);
+}
+
 __device__ __forceinline__ float exp2_fast(float x) {  // 2^x, one MUFU; 2^-inf = 0
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -211,16 +220,25 @@ struct RowKeys {
   const int* table;
   int kvh, from, first, last, to;
 };
+// of a row of a tree, which sees a key behind `last` if its mask says so
+struct TreeKeys : RowKeys {
+  int tok, ctx;              // the row, and its sequence's cached tokens
+};
+template <bool TREE>
+using KeysOf = typename std::conditional<TREE, TreeKeys, RowKeys>::type;
 __device__ __forceinline__ int64_t cache_row(const AttnArgs& a, const RowKeys& k, int key) {
   return ((int64_t)checked_block(k.table[key / a.page], a.num_blocks) * a.hkv + k.kvh) * a.page + key % a.page;
 }
-template <typename M, int FMT>
-__device__ __noinline__ bool hidden_unfinite(const AttnArgs& a, const RowKeys& k) {
+template <typename M, int FMT, bool TREE>
+__device__ __noinline__ bool hidden_unfinite(const AttnArgs& a, const KeysOf<TREE>& k) {
   bool found = false;
   for (int key = k.from; key <= k.to; ++key) {
     if (key >= k.first && key <= k.last) {
       key = k.last;
       continue;
+    }
+    if constexpr (TREE) {
+      if (key > k.last && key >= k.first && (tree_bits(a, k.tok, key - k.ctx) & 1u)) continue;
     }
     const int64_t r = cache_row(a, k, key);
     if constexpr (FMT == kInt8 || FMT == kE4M3) found = found || !(fabsf(a.vs[r]) < INFINITY);
@@ -229,17 +247,26 @@ __device__ __noinline__ bool hidden_unfinite(const AttnArgs& a, const RowKeys& k
   return __any_sync(0xffffffffu, found);
 }
 // to `part` ([d], maximum, sum), or where that is null to the output
-template <typename T, typename M, int FMT>
-__device__ __noinline__ void row_anew(const AttnArgs& a, const RowKeys& k, int tok, int head, float* part) {
+template <typename T, typename M, int FMT, bool TREE>
+__device__ __noinline__ void row_anew(const AttnArgs& a, const KeysOf<TREE>& k, int tok, int head, float* part) {
   float o[8], m, l;
-  row_softmax<T, M, FMT>(a, tok, head, k.first, 1, k.last + 1, [&](int key) { return cache_row(a, k, key); }, o, m, l);
+  bool sees = k.last >= k.first;
+  row_softmax<T, M, FMT, TREE>(a, tok, head, k.first, 1, (TREE ? k.to : k.last) + 1, [&](int key) {
+    if constexpr (TREE) {
+      if (key > k.last) {
+        if ((tree_bits(a, tok, key - k.ctx) & 1u) == 0) return (int64_t)-1;
+        sees = true;
+      }
+    }
+    return cache_row(a, k, key);
+  }, o, m, l);
   const int lane = threadIdx.x & 31;
   T* out = reinterpret_cast<T*>(a.out) + (int64_t)tok * a.ldo + (int64_t)head * a.d;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     if (lane + 32 * i >= a.d) continue;
     if (part != nullptr) part[lane + 32 * i] = o[i];
-    else out[lane + 32 * i] = from_f32<T>(k.last < k.first ? 0.f : o[i] / l);
+    else out[lane + 32 * i] = from_f32<T>(!sees ? 0.f : o[i] / l);
   }
   if (part != nullptr && lane == 0) *reinterpret_cast<float2*>(part + a.d) = make_float2(m, l);
 }

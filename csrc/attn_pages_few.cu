@@ -92,20 +92,24 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {   // 8 x 8 of 16-bi
 __device__ __forceinline__ int key_of(int i) { return (i & 1) ? ((i - 1) ^ 5) : i; }   // 0 5 2 7 4 1 6 3
 
 // Rows (bits of `rows`) of a list, or of its part (slot >= 0): formed anew over the keys from .. to that they see.
-template <typename T, int FMT, int D>
+template <typename T, int FMT, int D, bool TREE>
 __device__ __noinline__ void rows_anew(const AttnArgs& a, const PartArgs& pa, int own, int seg, int kvh, int from, int to, int slot, unsigned rows) {
   const Seg s = seg < own ? own_segment(a, seg) : group_segment(a, seg - own);
   const int group = a.hq / a.hkv;
   for (; rows != 0; rows &= rows - 1) {
     const int i = __ffs(rows) - 1, tok = s.row0 + i / group, head = kvh * group + i % group;
-    const int sq = seg < own ? seg : seq_of_row(a.cu, 0, a.num_seqs, tok), last = sq < 0 ? -1 : min(row_pos(a, sq, tok), min(to, s.hi - 1));
-    const RowKeys k = {s.table, kvh, from, max(from, s.lo), last, to};
+    const int sq = seg < own ? seg : seq_of_row(a.cu, 0, a.num_seqs, tok), ctx = TREE && sq >= 0 ? tree_context(a, sq) : 0;
+    const int last = sq < 0 ? -1 : min(TREE ? ctx - 1 : row_pos(a, sq, tok), min(to, s.hi - 1));
+    KeysOf<TREE> k;
+    k.table = s.table, k.kvh = kvh, k.from = from, k.first = max(from, s.lo), k.last = last, k.to = to;
+    // a prefix's keys are all cached ones: of those behind a row's context, which it does not see, no mask is asked
+    if constexpr (TREE) k.to = min(to, seg < own ? s.hi - 1 : last), k.tok = tok, k.ctx = ctx;
     float* whole = (seg < own ? pa.whole_own : pa.whole_group) + ((int64_t)tok * a.hq + head) * (D + kPad);
-    row_anew<T, T, FMT>(a, k, tok, head, slot >= 0 ? pa.slots + ((int64_t)slot * pa.rows + i) * (D + kPad) : a.groups == 0 ? nullptr : whole);
+    row_anew<T, T, FMT, TREE>(a, k, tok, head, slot >= 0 ? pa.slots + ((int64_t)slot * pa.rows + i) * (D + kPad) : a.groups == 0 ? nullptr : whole);
   }
 }
 
-template <typename T, int FMT, int D, int NT>
+template <typename T, int FMT, int D, int NT, bool TREE>
 __global__ void __launch_bounds__(32 * kWarps, Few<FMT, D, NT>::MIN_CTAS)
 attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnArgs a,
                       const __grid_constant__ PartArgs pa, const FewArgs f) {
@@ -269,6 +273,9 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     // ---- queries: row r (and r + 8) lies in the four lanes that hold its fragments, a lane's 16 bytes of a key facing its own columns of the row
     float qs[NT][2], qb[NT][2];            // of rows 2t, 2t + 1: score factor, what 128 added to a score
     int pos[NT][2], all_pos = 0x7fffffff, max_pos = -1;   // and their last visible keys; the least and the largest of all rows
+    // trees: the last of the cached tokens instead, and a bit for each of the new ones (16 rows are 16 of them at most) that the list has and the row sees
+    uint32_t bits[NT][2];
+    const int ctx = TREE && seg < f.own ? tree_context(a, seg) : 0;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int i = nt * 8 + r, tok = s.row0 + i / group;
@@ -331,18 +338,21 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
       }
       int p = -1;
+      uint32_t own_bits = 0;
       if (live) {
         const int sq = seg < f.own ? seg : seq_of_row(a.cu, 0, a.num_seqs, tok);
-        p = sq < 0 ? -1 : min(row_pos(a, sq, tok), s.hi - 1);
+        p = sq < 0 ? -1 : min(TREE ? tree_context(a, sq) - 1 : row_pos(a, sq, tok), s.hi - 1);
+        if (TREE && seg < f.own) own_bits = tree_bits(a, tok, 0) & bit_range(max(s.lo, 0) - ctx, s.hi - 1 - ctx);
       }
       all_pos = min(all_pos, __reduce_min_sync(0xffffffffu, live ? p : 0x7fffffff));
-      max_pos = max(max_pos, __reduce_max_sync(0xffffffffu, p));
+      max_pos = max(max_pos, __reduce_max_sync(0xffffffffu, TREE && own_bits != 0 ? ctx + 31 - __clz(own_bits) : p));
       const float f_s = FMT == kInt8 ? f_q * 16777216.f : f_q, f_b = f_q * 128.f * sum;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         qs[nt][c] = __shfl_sync(0xffffffffu, f_s, (2 * t + c) * 4);
         qb[nt][c] = __shfl_sync(0xffffffffu, f_b, (2 * t + c) * 4);
         pos[nt][c] = __shfl_sync(0xffffffffu, p, (2 * t + c) * 4);
+        if constexpr (TREE) bits[nt][c] = __shfl_sync(0xffffffffu, own_bits, (2 * t + c) * 4);
       }
     }
 
@@ -434,7 +444,11 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             else z *= (FMT != kF16Pages ? kf[i][c >> 1] : 1.f) * qs[nt][c & 1];
             if (edge) {
               const int key = tok0 + i * 16 + kk + 8 * (c >> 1);
-              if (key < s.lo || key > pos[nt][c & 1]) z = -INFINITY;
+              if constexpr (TREE) {
+                if (key < s.lo || (key > pos[nt][c & 1] && ((unsigned)(key - ctx) > 31u || (bits[nt][c & 1] >> (key - ctx) & 1u) == 0))) z = -INFINITY;
+              } else {
+                if (key < s.lo || key > pos[nt][c & 1]) z = -INFINITY;
+              }
             }
             grow = grow || z > m[nt][c & 1] + 8.f;
             if constexpr (FMT != kF16Pages) grow = grow || z + lv[i][c >> 1] > m2[nt][c & 1] + 8.f;
@@ -611,7 +625,7 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         const int tok = s.row0 + i / group, head = kvh * group + i % group;
         if (last) {
           // sum is NaN where a score was; a row without a visible key is zero
-          const bool sees = pos[nt][c] >= s.lo;
+          const bool sees = pos[nt][c] >= s.lo || (TREE && bits[nt][c] != 0);
           const float inv = 1.0f / sum;
           back *= inv, off *= inv;
           T* dst = reinterpret_cast<T*>(a.out) + (int64_t)tok * a.ldo + (int64_t)head * D;
@@ -637,7 +651,7 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
           if (r == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(ref, sum);
         }
       }
-    if (FMT != kInt8 && anew != 0) rows_anew<T, FMT, D>(a, pa, f.own, seg, kvh, base + u0 * UNIT, base + u1 * UNIT - 1, whole ? -1 : slot, anew);
+    if (FMT != kInt8 && anew != 0) rows_anew<T, FMT, D, TREE>(a, pa, f.own, seg, kvh, base + u0 * UNIT, base + u1 * UNIT - 1, whole ? -1 : slot, anew);
     cur += u1 - u0;
     if (cur < end) {
       z.cur = cur;
@@ -647,11 +661,11 @@ attn_pages_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   pdl_wait();
 }
 
-template <typename T, int FMT, int D, int NT>
-int launch(const AttnArgs& a, const PartArgs& p, int blocks, bool beside, cudaStream_t stream) {
+template <typename T, int FMT, int D, int NT, bool TREE>
+int launch_as(const AttnArgs& a, const PartArgs& p, int blocks, bool beside, cudaStream_t stream) {
   using C = Few<FMT, D, NT>;
   static PerDeviceSmem configured;
-  auto kern = attn_pages_few_kernel<T, FMT, D, NT>;
+  auto kern = attn_pages_few_kernel<T, FMT, D, NT, TREE>;
   FewArgs f;
   f.own = p.few_own ? a.num_seqs : 0;
   f.segs = f.own + (p.few_groups ? a.groups : 0);
@@ -677,6 +691,10 @@ int launch(const AttnArgs& a, const PartArgs& p, int blocks, bool beside, cudaSt
   cfg.numAttrs = beside || llmss_pdl_enabled() ? 1 : 0;
   LLMSS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, map_k, map_v, a, p, f));
   return 0;
+}
+template <typename T, int FMT, int D, int NT>
+int launch(const AttnArgs& a, const PartArgs& p, int blocks, bool beside, cudaStream_t stream) {
+  return a.masks != nullptr ? launch_as<T, FMT, D, NT, true>(a, p, blocks, beside, stream) : launch_as<T, FMT, D, NT, false>(a, p, blocks, beside, stream);
 }
 
 }  // namespace
