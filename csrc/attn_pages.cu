@@ -133,8 +133,13 @@ __global__ void __launch_bounds__(256, D < 256 && WARPS == 1 ? 5 : 4) attn_pages
     if (x == 0 ? has_own : has_group) {
       const Seg& sg = x == 0 ? own : gs;
       if (x == 0 ? p.few_own : p.few_groups) {
-        const FewInfo in = p.info[(int64_t)(x == 0 ? s : (p.few_own ? a.num_seqs : 0) + g) * a.hkv + kvh];
-        const int n = (t - sg.row0) * group + head % group;
+        int n = (t - sg.row0) * group + head % group;
+        int64_t list = (int64_t)(x == 0 ? s : (p.few_own ? a.num_seqs : 0) + g) * a.hkv + kvh;
+        if constexpr (TREE) {
+          const int tile = n / p.rows;
+          list = list * p.row_tiles + min(tile, p.row_tiles - 1), n -= min(tile, p.row_tiles - 1) * p.rows;   // (n >= rows: beyond the rows that the call gave)
+        }
+        const FewInfo in = p.info[list];
         if (in.first_slot < 0) {
           if (a.groups == 0) return;                      // the result is written already
           run[2 * x] = place(x == 0 ? p.whole_own : p.whole_group) + at;
@@ -302,7 +307,9 @@ __global__ void __launch_bounds__(256) attn_pages_expand_kernel(const __grid_con
 struct Plan {
   bool any;             // the simple kernel for the whole call
   bool few_own, few_groups;
+  bool tree;            // the kernel for trees, whose parts lie as those of the one for few rows
   int blocks, rows;     // of the kernel for few rows
+  int row_tiles;        // of the one for trees
   TilePlan tile;
   int own_splits, own_chunk, group_splits, group_chunk;
   bool direct;          // the tiled kernel writes the result itself
@@ -365,6 +372,20 @@ Plan plan_call(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv
   // up to 16 rows of a key head fit the narrow side of the warp-level product; a tile of 128 costs the tiled kernel the same whatever is in it
   p.few_own = own <= 16;
   p.few_groups = groups > 0 && grouped <= 16;
+  p.row_tiles = 1;
+  if (tree && (own > 16 || grouped > 16)) {
+    // all lists by the kernel for trees: blocks of two times 128 rows where there are more than 128 (and tensor memory holds two)
+    const int64_t most = own > grouped ? own : grouped;
+    p.tree = p.few_own = true;
+    p.few_groups = groups > 0;
+    p.rows = tile_rows(d, most);
+    p.row_tiles = (int)((most + p.rows - 1) / p.rows);
+    p.slots = (int64_t)2 * kTreeBlocks * p.rows * (d + kPad);
+    p.info = ((int64_t)num_seqs + groups) * hkv * p.row_tiles * 4;
+    p.whole = groups > 0 ? (int64_t)total_q * hq * (d + kPad) : 0;
+    p.floats = p.slots + p.info + 2 * p.whole;
+    return p;
+  }
   const bool tile_own = !p.few_own, tile_groups = groups > 0 && !p.few_groups;
   p.tile.rows = tile_rows(d, own > 16 && own > grouped ? own : grouped);
   if (tile_own) {
@@ -373,8 +394,7 @@ Plan plan_call(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv
     // of a list takes whatever is left of it, and a block without keys is not free (a microsecond on its SM)
     const int keys = groups > 0 ? (max_kv - g_max_len > max_q ? max_kv - g_max_len : max_q) : max_kv;
     stretches((int64_t)p.tile.own_tiles * hkv * num_seqs, keys, groups > 0, p.own_splits, p.own_chunk);
-    // (causal rows over 16-bit pages come here without groups where a prefix has no tokens, if at all)
-    p.direct = groups == 0 && p.own_splits == 1 && (tree || fmt != kF16Pages);
+    p.direct = groups == 0 && p.own_splits == 1 && fmt != kF16Pages;      // (16-bit pages come here without groups where a prefix has no tokens, if at all)
     // Every row tile converts all codes for itself, which takes the tiled kernel from 1100 to 2000 clocks per 64 keys; once for all costs a pass over the
     // cache (about 1200 clocks of an SM per 64 keys, and a launch).  4 portions of 1000 tokens over 1800, 16 tiles each: 251 -> 183 us; three tiles 89 -> 87
     // (16 sequences 198 -> 170), two tiles 69 -> 68, one 47 -> 47: from three tiles on.  Up to 1 GB of scratch
@@ -490,6 +510,7 @@ int attend(const void* q, int64_t ldq, const void* k_pages, const float* k_scale
     p.tile_own = take(plan.tile_own);
     p.tile_group = take(plan.tile_group);
     p.rows = plan.rows;
+    p.row_tiles = plan.row_tiles;
     p.few_own = plan.few_own;
     p.few_groups = plan.few_groups;
     p.own_splits = plan.own_splits;
@@ -523,14 +544,19 @@ int attend(const void* q, int64_t ldq, const void* k_pages, const float* k_scale
       ++*launches;
     }
     if (plan.direct) return 0;
-    if (plan.few_own || plan.few_groups) {
+    if (plan.tree) {
+      LLMSS_REQUIRE((int64_t)(num_seqs + a.groups) * hkv * plan.row_tiles * ((int64_t)(max_blocks > a.g_max_blocks ? max_blocks : a.g_max_blocks) * block_size / 64 + 2) < (1ll << 31),
+                    "attn_tree: 2^31 tiles of 64 keys and more");
+      if (int e = tree_launch(a, p, fmt, dtype, stream)) return e;
+      ++*launches;
+    } else if (plan.few_own || plan.few_groups) {
       if (int e = few_launch(a, p, fmt, dtype, plan.blocks, tiles, stream)) return e;
       ++*launches;
     }
     ++*launches;
     // parts of a row, about: runs of a list, or stretches
     const int64_t lists = ((int64_t)(plan.few_own ? num_seqs : 0) + (plan.few_groups ? a.groups : 0)) * hkv;
-    const int64_t runs = lists > 0 ? (int64_t)plan.blocks * kFewWarps / lists : 0;
+    const int64_t runs = lists > 0 ? (plan.tree ? kTreeBlocks : (int64_t)plan.blocks * kFewWarps) / (lists * plan.row_tiles) : 0;
     const int parts = (int)(runs > plan.own_splits + plan.group_splits ? runs : plan.own_splits + plan.group_splits);
 #define LLMSS_MERGE(T_) return d == 64 ? launch_merge<T_, 64>(a, p, parts, stream) : d == 128 ? launch_merge<T_, 128>(a, p, parts, stream) : launch_merge<T_, 256>(a, p, parts, stream)
     if (dtype == LLMSS_F16) LLMSS_MERGE(__half);

@@ -111,6 +111,7 @@ struct PartArgs {
   int own_splits, group_splits;   // or into this many stretches of keys each (0: not)
   int own_chunk, group_chunk;     // keys of a stretch
   int direct;                     // the tiled kernel writes results, not parts
+  int row_tiles;                  // trees: of `rows` rows each, that a segment has at most; info [segments][hkv][row_tiles]
 };
 
 struct Seg {
@@ -339,5 +340,7 @@ struct TilePlan {
   int own_tiles, group_tiles, rows;
 };
 int tile_launch(const AttnArgs& a, const PartArgs& p, const TilePlan& t, int fmt, int dtype, cudaStream_t stream);
+constexpr int kTreeBlocks = 148;   // attn_tree.cu: blocks, and so runs of a call
+int tree_launch(const AttnArgs& a, const PartArgs& p, int fmt, int dtype, cudaStream_t stream);
 
 }  // namespace pages

@@ -105,7 +105,7 @@ struct Block {
   int k_lo, k_hi;           // keys
 };
 // groups' lists first, since they are long, and of a list's rows the last first, since they see most
-template <int NQ, bool TREE>
+template <int NQ>
 __device__ __forceinline__ Block block_of(const AttnArgs& a, const TileArgs& ta) {
   Block b;
   const int in_groups = ta.group_tiles * ta.group_splits * a.hkv * a.groups;      // (group_tiles 0: groups are not this launch's)
@@ -121,7 +121,7 @@ __device__ __forceinline__ Block block_of(const AttnArgs& a, const TileArgs& ta)
   const int group = a.hq / a.hkv;
   b.nrows = b.s.rows * group, b.n0 = tile * (NQ * BM);
   int k_end = b.s.hi;
-  if (!TREE && b.is_own && b.n0 < b.nrows) k_end = min(k_end, row_pos(a, b.seg, b.s.row0 + (min(b.nrows, b.n0 + NQ * BM) - 1) / group) + 1);
+  if (b.is_own && b.n0 < b.nrows) k_end = min(k_end, row_pos(a, b.seg, b.s.row0 + (min(b.nrows, b.n0 + NQ * BM) - 1) / group) + 1);
   // stretch `split` of the list; the last one takes what lies behind it (lengths beyond the bounds the call gave)
   b.k_lo = max(b.s.lo, b.s.lo + b.split * chunk);
   b.k_hi = b.split == splits - 1 ? k_end : min(k_end, b.s.lo + (b.split + 1) * chunk);
@@ -129,20 +129,15 @@ __device__ __forceinline__ Block block_of(const AttnArgs& a, const TileArgs& ta)
 }
 
 // keys of row n of a block's list
-template <bool TREE>
-__device__ __forceinline__ KeysOf<TREE> keys_of(const AttnArgs& a, const Block& b, int n, int& tok, int& head) {
+template <int NQ>
+__device__ __forceinline__ RowKeys keys_of(const AttnArgs& a, const Block& b, int n, int& tok, int& head) {
   const int group = a.hq / a.hkv;
   tok = b.s.row0 + n / group, head = b.kvh * group + n % group;
-  const int sq = b.is_own ? b.seg : seq_of_row(a.cu, 0, a.num_seqs, tok), ctx = TREE && sq >= 0 ? tree_context(a, sq) : 0;
-  const int last = sq < 0 ? -1 : min(TREE ? ctx - 1 : row_pos(a, sq, tok), b.k_hi - 1);
-  KeysOf<TREE> k;
-  k.table = b.s.table, k.kvh = b.kvh, k.from = max(b.k_lo & ~(BN - 1), b.s.lo), k.first = b.k_lo, k.last = last, k.to = b.k_hi - 1;
-  // a prefix's keys are all cached ones: of those behind a row's context, which it does not see, no mask is asked (its bits lie in front of them)
-  if constexpr (TREE) k.tok = tok, k.ctx = b.is_own ? ctx : -(1 << 30);
-  return k;
+  const int sq = b.is_own ? b.seg : seq_of_row(a.cu, 0, a.num_seqs, tok);
+  return {b.s.table, b.kvh, max(b.k_lo & ~(BN - 1), b.s.lo), b.k_lo, sq < 0 ? -1 : min(row_pos(a, sq, tok), b.k_hi - 1), b.k_hi - 1};
 }
 // By a softmax warp: of its rows (sums in tensor memory, a lane each) those whose result is not finite because of a hidden key.
-template <typename T, int FMT, int D, int NQ, bool TREE>
+template <typename T, int FMT, int D, int NQ>
 __device__ __noinline__ unsigned spoiled_rows(const AttnArgs& a, const TileArgs& ta, uint32_t sums, bool mine) {
   using M = typename std::conditional<Tile<FMT, D, NQ>::SCALED, __half, T>::type;
   float x[4] = {0.f, 0.f, 0.f, 0.f};                     // NaN where a sum is not finite
@@ -159,27 +154,27 @@ __device__ __noinline__ unsigned spoiled_rows(const AttnArgs& a, const TileArgs&
   }
   unsigned spoiled = 0, rows = __ballot_sync(0xffffffffu, mine && (x[0] + x[1]) + (x[2] + x[3]) != 0.f);
   if (rows == 0) return 0;
-  const Block b = block_of<NQ, TREE>(a, ta);
+  const Block b = block_of<NQ>(a, ta);
   for (; rows != 0; rows &= rows - 1) {
     int tok, head;
-    if (hidden_unfinite<M, FMT, TREE>(a, keys_of<TREE>(a, b, b.n0 + (threadIdx.x & ~31) + __ffs(rows) - 1, tok, head))) spoiled |= rows & (0u - rows);
+    if (hidden_unfinite<M, FMT, false>(a, keys_of<NQ>(a, b, b.n0 + (threadIdx.x & ~31) + __ffs(rows) - 1, tok, head))) spoiled |= rows & (0u - rows);
   }
   return spoiled;
 }
-template <typename T, int FMT, int D, int NQ, bool TREE>
+template <typename T, int FMT, int D, int NQ>
 __device__ __noinline__ void rows_anew(const AttnArgs& a, const PartArgs& pa, const TileArgs& ta, unsigned rows) {
   using M = typename std::conditional<Tile<FMT, D, NQ>::SCALED, __half, T>::type;
-  const Block b = block_of<NQ, TREE>(a, ta);
+  const Block b = block_of<NQ>(a, ta);
   __syncwarp();                                          // behind the rows as they were
   for (; rows != 0; rows &= rows - 1) {
     int tok, head;
-    const KeysOf<TREE> k = keys_of<TREE>(a, b, b.n0 + (threadIdx.x & ~31) + __ffs(rows) - 1, tok, head);
+    const RowKeys k = keys_of<NQ>(a, b, b.n0 + (threadIdx.x & ~31) + __ffs(rows) - 1, tok, head);
     float* part = (b.is_own ? pa.tile_own : pa.tile_group) + (((int64_t)b.split * a.total_q + tok) * a.hq + head) * (D + kPad);
-    row_anew<T, M, FMT, TREE>(a, k, tok, head, ta.direct ? nullptr : part);
+    row_anew<T, M, FMT, false>(a, k, tok, head, ta.direct ? nullptr : part);
   }
 }
 
-template <typename T, int FMT, int D, int NQ, bool TREE>
+template <typename T, int FMT, int D, int NQ>
 __global__ void __maxnreg__((Tile<FMT, D, NQ>::REGS))
 attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnArgs a, const __grid_constant__ PartArgs pa, const __grid_constant__ TileArgs ta) {
   using C = Tile<FMT, D, NQ>;
@@ -214,7 +209,7 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   // behind the wait: the kernel for few rows starts beside this one without a wait of its own, and reads what the kernels before this one wrote
   pdl_launch_dependents();
 
-  const Block blk = block_of<NQ, TREE>(a, ta);
+  const Block blk = block_of<NQ>(a, ta);
   const Seg s = blk.s;
   const bool is_own = blk.is_own;
   const int seg = blk.seg, kvh = blk.kvh, split = blk.split, n0 = blk.n0, nrows = blk.nrows, k_lo = blk.k_lo, k_hi = blk.k_hi;
@@ -497,10 +492,8 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     int pos = 0x7fffffff;                                 // rows beyond the last look at everything and are dropped
     if (live) {
       const int sq = is_own ? seg : seq_of_row(a.cu, 0, a.num_seqs, tok);
-      pos = sq < 0 ? -1 : TREE ? tree_context(a, sq) - 1 : row_pos(a, sq, tok);
+      pos = sq < 0 ? -1 : row_pos(a, sq, tok);
     }
-    const int ctx = live ? pos + 1 : 0;                   // trees: cached tokens, which the row sees all; its mask says which others
-    bool sees_any = false;
     pos = min(pos, k_hi - 1);
     if (n_tiles > 0) {
       copies_wait<0>();
@@ -540,23 +533,9 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       const int hi = pos - kb, lo = k_lo - kb;
       if (__any_sync(0xffffffffu, hi < BN - 1 || lo > 0)) {
         partly = true;
-        if constexpr (TREE) {
-          const bool masked = live && is_own;
 #pragma unroll
-          for (int c = 0; c < BN / 32; ++c) {
-            const uint32_t see = (masked ? tree_bits(a, tok, kb + c * 32 - ctx) : ~0u) & bit_range(lo - c * 32, (masked ? k_hi - 1 - kb : hi) - c * 32);
-            sees_any = sees_any || see != 0;
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if ((see >> i & 1u) == 0) sc[c * 32 + i] = -INFINITY;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < BN; ++i)
-            if (i > hi || i < lo) sc[i] = -INFINITY;
-        }
-      } else if (TREE) {
-        sees_any = true;
+        for (int i = 0; i < BN; ++i)
+          if (i > hi || i < lo) sc[i] = -INFINITY;
       }
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -624,7 +603,7 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     // the other tile's products read keys and values too; its barriers' phases may lie behind by more than one, so that its own warps have to say it
     if constexpr (NQ > 1) asm volatile("bar.sync 1, %0;" ::"n"(32 * C::SOFT) : "memory");
     if (bad) l_run = __int_as_float(0x7fc00000);
-    const bool sees = TREE ? sees_any : pos >= k_lo;      // no visible key: zero
+    const bool sees = pos >= k_lo;                        // no visible key: zero
     const float down = C::SCALED ? exp2f(-up) : 1.0f;     // of outputs, to the sum's reference
     const float inv = down / l_run;
     const int stride = ta.direct ? D * 2 + 16 : D * 4 + 16;
@@ -656,8 +635,8 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     uint8_t* to = nullptr;
     // (out of line: what a block runs once comes cold from memory.  A direct result may go over the queries: those rows are left out here)
     unsigned anew = 0;
-    if constexpr (C::SCALED || TREE)
-      if (partly) anew = spoiled_rows<T, FMT, D, NQ, TREE>(a, ta, t_o(q) + off, live && !bad);
+    if constexpr (C::SCALED)
+      if (partly) anew = spoiled_rows<T, FMT, D, NQ>(a, ta, t_o(q) + off, live && !bad);
     if (live && (anew >> lane & 1) == 0) {
       if (ta.direct) {
         to = reinterpret_cast<uint8_t*>(reinterpret_cast<T*>(a.out) + (int64_t)tok * a.ldo + (int64_t)head * D);
@@ -685,9 +664,9 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     };
     if (ta.direct) rows_out(std::integral_constant<int, D * 2>{});
     else rows_out(std::integral_constant<int, D * 4>{});
-    if constexpr (!C::SCALED && !TREE)
-      if (partly) anew = spoiled_rows<T, FMT, D, NQ, TREE>(a, ta, t_o(q) + off, live && !bad);
-    if (anew != 0) rows_anew<T, FMT, D, NQ, TREE>(a, pa, ta, anew);
+    if constexpr (!C::SCALED)
+      if (partly) anew = spoiled_rows<T, FMT, D, NQ>(a, ta, t_o(q) + off, live && !bad);
+    if (anew != 0) rows_anew<T, FMT, D, NQ>(a, pa, ta, anew);
   }
 
   tcgen05_fence_before();
@@ -698,12 +677,12 @@ attn_pages_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   }
 }
 
-template <typename T, int FMT, int D, int NQ, bool TREE>
-int launch_as(const AttnArgs& a, const PartArgs& p, const TilePlan& t, cudaStream_t stream) {
+template <typename T, int FMT, int D, int NQ>
+int launch(const AttnArgs& a, const PartArgs& p, const TilePlan& t, cudaStream_t stream) {
   using C = Tile<FMT, D, NQ>;
   static_assert(C::SMEM <= 232448, "shared memory of a block");
   static PerDeviceSmem configured;
-  auto kern = attn_pages_tile_kernel<T, FMT, D, NQ, TREE>;
+  auto kern = attn_pages_tile_kernel<T, FMT, D, NQ>;
   LLMSS_CHECK_CUDA(configured.ensure(kern, C::SMEM));
   TileArgs ta;
   ta.own_tiles = t.own_tiles;
@@ -729,10 +708,6 @@ int launch_as(const AttnArgs& a, const PartArgs& p, const TilePlan& t, cudaStrea
   const dim3 grid((unsigned)blocks);
   LLMSS_CHECK_CUDA(launch_pdl(kern, grid, dim3(C::THREADS), (size_t)C::SMEM, stream, map_k, map_v, a, p, ta));
   return 0;
-}
-template <typename T, int FMT, int D, int NQ>
-int launch(const AttnArgs& a, const PartArgs& p, const TilePlan& t, cudaStream_t stream) {
-  return a.masks != nullptr ? launch_as<T, FMT, D, NQ, true>(a, p, t, stream) : launch_as<T, FMT, D, NQ, false>(a, p, t, stream);
 }
 
 template <typename T, int FMT>

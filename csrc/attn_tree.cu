@@ -1,0 +1,852 @@
+// Attention of trees of drafted tokens over cache pages on the 5th-generation tensor cores, for more than 16 query rows of a key head.
+//
+// A list is a (sequence, key head, up to 256 of its rows); a row is a (token, query head), so that grouped heads and a tree's tokens fill a tile's 128 rows and
+// a key is read once for all of them.  Rows see all cached keys, so that masks are looked at in a list's last tiles alone.  What bounds a call is reading
+// the cache: 64 keys of 128 columns in 16 bits are 32 KB, which an SM's share of the memory brings in 0.75 us, while the products of 128 rows take 0.3.
+//
+// So the work of a call, the sum of all lists in tiles of 64 keys, is cut into equal runs, one per SM, by the lengths that lie on the device; a block goes
+// from list to list, and its copies run ahead of it through a ring as deep as shared memory allows, over the ends of lists:
+//
+//   copying warps   one keys, one values, page by page (TMA, 128-byte swizzle), in the order K0, K1 V0, K2 V1 .. of a list; 8-bit codes and scales into a
+//                   ring of their own (bulk copies), from which
+//   converting warps (8-bit) write the tiles as f16: a code is an f16 number, so nothing is rounded
+//   issuing warps   one per 128 rows: S_j = Q K_j^T (two S buffers), O += P_j V_j with P_j in tensor memory over S_j
+//   softmax warps   a thread per row: S from tensor memory times the keys' scales, mask, running maximum (moved when exceeded by 2^8) and sum in 32 bits,
+//                   P times the values' scales back.  Those without a row of the list only keep the barriers going
+//
+// The values' scales join the probabilities before their one rounding to f16, relative to a power of two per tile (TileScales) that keeps them in range;
+// scaled and rounded codes (2^-11 of each key, value and probability) would make f16 results three times as far off.
+// A list within a block's run is finished there, one that crosses runs leaves its parts in scratch, at most two per block, and the merge kernel joins them.
+#include "attn_pages.cuh"
+
+namespace {
+
+using namespace pages;
+using namespace umma_lo;
+
+constexpr int BM = 128, BN = 64;
+constexpr int kScaleTiles = 16;    // of the 8-bit scales' ring
+constexpr int kKept = 64;          // lists' segments that a block keeps in shared memory
+constexpr int kLeastTiles = 2;     // of a run
+
+struct SegInfo {
+  int lo, hi, row0, rows;
+  int units, tiles;       // tiles of 64 keys, and of rows
+  int ctx;                // cached tokens in front of the new ones (own lists)
+};
+
+template <int FMT, int D, int NQ>
+struct Tree {
+  static constexpr bool BYTES = FMT != kF16Pages;
+  static constexpr int ROWS = NQ * BM;
+  static constexpr int SOFT = 4 * NQ;                                   // softmax warps
+  static constexpr int CONVERT = !BYTES ? 0 : NQ == 2 ? 4 : 8;
+  static constexpr int COPY = SOFT + NQ;                                // first copying warp
+  static constexpr int THREADS = 32 * (COPY + 2 + CONVERT);
+  static constexpr int Q_BYTES = ROWS * D * 2;
+  static constexpr int SLOT = BN * D * 2;                               // a tile of keys or values
+  static constexpr int RAW = BYTES ? BN * D : 0;                        // a tile of codes
+  static constexpr int SCALES = BYTES ? kScaleTiles * (2 * BN * 4 + 16) : 0;
+  static constexpr int FIXED = 1024 + Q_BYTES + SCALES + 1024 + kKept * (int)sizeof(SegInfo) + 64;
+  static constexpr int ROOM = 232448 - FIXED;
+  // 16 bits: all there is, up to 24.  8 bits: three to eight tiles in f16, codes in the rest; a tile's scales are looked at until its values' slot is free,
+  // which is RAWS + SLOTS copies behind: fewer than two per tile of scales
+  static constexpr int SLOTS = !BYTES ? (ROOM / SLOT < 24 ? ROOM / SLOT : 24) : D == 256 ? 3 : D == 128 ? 6 : 8;
+  static constexpr int RAWS = !BYTES ? 0 : (ROOM - SLOTS * SLOT) / RAW < 16 ? (ROOM - SLOTS * SLOT) / RAW : 16;
+  static constexpr int SMEM = FIXED + SLOTS * SLOT + RAWS * RAW;
+  static constexpr int TMEM = NQ * (2 * BN + D) <= 256 ? 256 : 512;
+  static_assert(SLOTS >= 3 && (!BYTES || (RAWS >= 3 && RAWS + SLOTS <= 2 * kScaleTiles - 4)), "rings");
+  static_assert((2 * SLOTS + 2 * RAWS + 7 * NQ + 2) * 8 <= 1024, "barriers");
+};
+
+struct TreeArgs {
+  int segs, own;          // lists' segments: sequences (own) and groups
+  int row_tiles;          // of a segment at most
+  int run;                // keys of a tile that lie in one page: 16, 32 or 64
+  uint32_t page_magic;    // (key / 16) 2 this >> 32: the key's page
+};
+
+__host__ __device__ constexpr uint32_t idesc(int fmt, int n, int b_mn) {   // kind::f16 with 32-bit sums; b_mn: B lies with its columns one after another
+  return (1u << 4) | ((uint32_t)fmt << 7) | ((uint32_t)fmt << 10) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {   // bytes 0: zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_wait_all() { asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+      "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// four codes as f16, two words
+template <int FMT>
+__device__ __forceinline__ void codes4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (FMT == kInt8) {
+    // 0x64uu is 1024 + u, u = code + 128
+    w ^= 0x80808080u;
+    const __half2 off = __floats2half2_rn(1152.f, 1152.f);
+    const uint32_t a = prmt(w, 0x64646464u, 0x4140), b = prmt(w, 0x64646464u, 0x4342);
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), off), y = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
+    lo = *reinterpret_cast<const uint32_t*>(&x), hi = *reinterpret_cast<const uint32_t*>(&y);
+  } else {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+  }
+}
+
+// 2^x without the MUFU pipe; 0 for what is below -127 (hidden keys weigh nothing, however large their values), and for NaN
+__device__ __forceinline__ float exp2_fma(float x) { return exp2_cubic(fmaxf(x, -127.0f)); }
+
+template <int ROWS>
+__device__ __forceinline__ SegInfo seg_info(const AttnArgs& a, const TreeArgs& ta, int i) {
+  const Seg s = i < ta.own ? own_segment(a, i) : group_segment(a, i - ta.own);
+  SegInfo x;
+  x.lo = s.lo, x.hi = s.hi, x.row0 = s.row0, x.rows = s.rows;
+  x.units = s.hi > s.lo && s.rows > 0 ? (s.hi - (s.lo & ~(BN - 1)) + BN - 1) / BN : 0;
+  x.tiles = s.rows > 0 ? min((s.rows * (a.hq / a.hkv) + ROWS - 1) / ROWS, ta.row_tiles) : 0;
+  x.ctx = i < ta.own ? tree_context(a, i) : 0;
+  return x;
+}
+
+// the part of a list that lies in a block's run
+struct Part {
+  SegInfo s;
+  const int* table;
+  bool own;
+  int seg, kvh, rt, n;    // segment, key head, tile of rows; tiles of keys of the list
+  int u0, u1;             // the part's
+  int base, lo, hi;       // first key of its first tile; its keys
+  int n0, nrows;          // first row; rows of the segment
+};
+// a place in a run
+struct Walk {
+  unsigned cur, end, before;
+  int seg;
+};
+
+// rows n0 + lane of a part, for what looks at them once more
+struct PartRows {
+  const int* table;
+  float* parts;           // of row n0 on; null: the result itself
+  int kvh, row0, n0, from, lo, hi, seg;      // seg: of own lists, else -1
+};
+__device__ __forceinline__ TreeKeys keys_of(const AttnArgs& a, const PartRows& p, int n, int& tok, int& head) {
+  const int group = a.hq / a.hkv;
+  tok = p.row0 + n / group, head = p.kvh * group + n % group;
+  const int sq = p.seg >= 0 ? p.seg : seq_of_row(a.cu, 0, a.num_seqs, tok), ctx = sq >= 0 ? tree_context(a, sq) : 0;
+  TreeKeys k;
+  k.table = p.table, k.kvh = p.kvh, k.from = p.from, k.first = p.lo, k.last = sq < 0 ? -1 : min(ctx - 1, p.hi - 1), k.to = p.hi - 1;
+  // a prefix's keys are all cached ones: of those behind a row's context, which it does not see, no mask is asked (its bits lie in front of them)
+  k.tok = tok, k.ctx = p.seg >= 0 ? ctx : -(1 << 30);
+  return k;
+}
+// By a softmax warp: of its rows (sums in tensor memory, a lane each) those whose result is not finite because of a hidden key.
+template <typename M, int FMT, int D>
+__device__ __noinline__ unsigned spoiled_rows(const AttnArgs& a, const PartRows& p, uint32_t sums, bool mine) {
+  float x[4] = {0.f, 0.f, 0.f, 0.f};                     // NaN where a sum is not finite
+#pragma unroll 1
+  for (int c = 0; c < D; c += 32) {
+    uint32_t r[32];
+    tmem_ld_32x32b_x32(sums + c, r);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+      ffma2(x[0], x[1], __uint_as_float(r[i]), __uint_as_float(r[i + 1]), 0.f, 0.f, x[0], x[1]);
+      ffma2(x[2], x[3], __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]), 0.f, 0.f, x[2], x[3]);
+    }
+  }
+  unsigned spoiled = 0, rows = __ballot_sync(0xffffffffu, mine && (x[0] + x[1]) + (x[2] + x[3]) != 0.f);
+  for (; rows != 0; rows &= rows - 1) {
+    int tok, head;
+    if (hidden_unfinite<M, FMT, true>(a, keys_of(a, p, p.n0 + __ffs(rows) - 1, tok, head))) spoiled |= rows & (0u - rows);
+  }
+  return spoiled;
+}
+template <typename T, typename M, int FMT, int D>
+__device__ __noinline__ void rows_anew(const AttnArgs& a, const PartRows& p, unsigned rows) {
+  __syncwarp();                                          // behind the rows as they were
+  for (; rows != 0; rows &= rows - 1) {
+    int tok, head;
+    const TreeKeys k = keys_of(a, p, p.n0 + __ffs(rows) - 1, tok, head);
+    row_anew<T, M, FMT, true>(a, k, tok, head, p.parts == nullptr ? nullptr : p.parts + (__ffs(rows) - 1) * (D + kPad));
+  }
+}
+
+template <typename T, int FMT, int D, int NQ>
+__global__ void __launch_bounds__(Tree<FMT, D, NQ>::THREADS, 1)
+attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnArgs a,
+                 const __grid_constant__ PartArgs pa, const __grid_constant__ TreeArgs ta) {
+  using C = Tree<FMT, D, NQ>;
+  using M = typename std::conditional<C::BYTES, __half, T>::type;   // type of the products
+  constexpr int DSUB = D / 64, ROWS = C::ROWS;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* s_q = smem;                                   // [NQ][DSUB][128 rows][128 bytes]
+  uint8_t* s_kv = s_q + C::Q_BYTES;                      // [SLOTS][DSUB][64 keys][128 bytes]
+  uint8_t* s_raw = s_kv + C::SLOTS * C::SLOT;            // [RAWS][64 keys of codes]
+  float* s_scale = reinterpret_cast<float*>(s_raw + C::RAWS * C::RAW);   // [tiles][keys', values'][64] (8-bit)
+  TileScales* s_tile = reinterpret_cast<TileScales*>(s_scale + (C::BYTES ? kScaleTiles * 2 * BN : 0));   // [tiles]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_raw + C::RAWS * C::RAW + C::SCALES);
+  uint64_t* bar_full = bars;                             // [SLOTS]
+  uint64_t* bar_empty = bars + C::SLOTS;
+  uint64_t* bar_s = bars + 2 * C::SLOTS;                 // [NQ][2] S ready
+  uint64_t* bar_p = bar_s + 2 * NQ;                      // [NQ][2] P written
+  uint64_t* bar_o = bar_p + 2 * NQ;                      // [NQ][2] P V done
+  uint64_t* bar_q = bar_o + 2 * NQ;                      // [NQ] a list's queries are in place
+  uint64_t* bar_part = bar_q + NQ;                       // a tile at a list's end, before its zeros
+  uint64_t* bar_raw = bar_part + 1;                      // [RAWS] codes have come
+  uint64_t* bar_used = bar_raw + C::RAWS;                // [RAWS] codes have been converted
+  SegInfo* s_info = reinterpret_cast<SegInfo*>(bars + 128);
+  unsigned* s_sum = reinterpret_cast<unsigned*>(s_info + kKept);         // [16] places of this block's run, and sums before them
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_used + C::RAWS);
+
+  // by a shuffle: numbers that the compiler knows to be the same in all lanes need no copies into uniform registers at every product
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  if (!C::BYTES && threadIdx.x == 32 * C::COPY) {
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::SLOTS; ++i) {
+      mbar_init(&bar_full[i], C::BYTES ? C::CONVERT : 1);
+      mbar_init(&bar_empty[i], NQ);
+    }
+    for (int i = 0; i < 2 * NQ; ++i) {
+      mbar_init(&bar_s[i], 1);
+      mbar_init(&bar_p[i], 4);
+      mbar_init(&bar_o[i], 1);
+    }
+    for (int i = 0; i < NQ; ++i) mbar_init(&bar_q[i], 4);
+    mbar_init(bar_part, 1);
+    for (int i = 0; i < C::RAWS; ++i) {
+      mbar_init(&bar_raw[i], 1);
+      mbar_init(&bar_used[i], C::CONVERT);
+    }
+    fence_mbar_init();
+  }
+  pdl_wait();
+  pdl_launch_dependents();                 // the merge reads lengths in front of its wait
+
+  // ---- this block's run (the host has checked that all lists together are below 2^31 tiles)
+  auto weight = [&](int i) {
+    const SegInfo x = seg_info<ROWS>(a, ta, i);
+    return (unsigned)x.units * x.tiles * a.hkv;
+  };
+  unsigned sum = 0;
+  for (int i = threadIdx.x; i < ta.segs; i += C::THREADS) sum += weight(i);
+  sum = __reduce_add_sync(0xffffffffu, sum);
+  if (lane == 0) s_sum[warp] = sum;
+  __syncthreads();
+  unsigned total = 0;
+  for (int i = 0; i < C::THREADS / 32; ++i) total += s_sum[i];
+  const unsigned per = max((total + gridDim.x - 1) / gridDim.x, (unsigned)kLeastTiles);
+  const unsigned begin = min(per * blockIdx.x, total), end = min(begin + per, total);
+  if (begin >= end) return;
+  __syncthreads();
+  if (warp == 0) {
+    unsigned before = 0;
+    for (int b = 0; b < ta.segs; b += 32) {
+      const unsigned n = b + lane < ta.segs ? weight(b + lane) : 0u;
+      unsigned inc = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned x = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += x;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, before + inc > begin);
+      if (hit) {
+        if (lane == __ffs(hit) - 1) s_sum[0] = b + lane, s_sum[1] = before + inc - n;
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, inc, 31);
+    }
+  }
+  if (warp == C::SOFT) {
+    tmem_alloc(tmem_slot, C::TMEM);
+    tmem_relinquish();
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  const int seg0 = s_sum[0];
+  Walk w = {begin, end, s_sum[1], seg0};
+  for (int i = threadIdx.x; i < kKept; i += C::THREADS)
+    if (seg0 + i < ta.segs) s_info[i] = seg_info<ROWS>(a, ta, seg0 + i);
+  __syncthreads();
+
+  const int group = a.hq / a.hkv;
+  auto next = [&](Part& p) {               // the part at w.cur, and on to the one behind it; false: the run is over
+    if (w.cur >= w.end) return false;
+    for (;; ++w.seg) {
+      p.s = w.seg - seg0 < kKept ? s_info[w.seg - seg0] : seg_info<ROWS>(a, ta, w.seg);
+      const unsigned all = (unsigned)p.s.units * p.s.tiles * a.hkv;
+      if (w.cur < w.before + all) break;
+      w.before += all;
+    }
+    p.seg = w.seg, p.own = w.seg < ta.own, p.n = p.s.units;
+    p.table = p.own ? a.tables + (int64_t)w.seg * a.max_blocks : a.g_tables + (int64_t)(w.seg - ta.own) * a.g_max_blocks;
+    const unsigned at = w.cur - w.before, list = at / p.n;
+    p.kvh = list / p.s.tiles, p.rt = list % p.s.tiles;
+    p.u0 = at - list * p.n;
+    p.u1 = min((unsigned)p.n, p.u0 + (w.end - w.cur));
+    w.cur += p.u1 - p.u0;
+    p.base = (p.s.lo & ~(BN - 1)) + p.u0 * BN;
+    p.lo = max(p.s.lo, p.base);
+    p.hi = min(p.s.hi, p.base + (p.u1 - p.u0) * BN);
+    p.n0 = p.rt * ROWS, p.nrows = p.s.rows * group;
+    return true;
+  };
+  // places of a list's tiles in the ring: K0, then K_{j+1}, V_j, and V of the last tile
+  auto key_at = [](int j) { return j == 0 ? 0 : 2 * j - 1; };
+  auto value_at = [](int j, int n) { return j + 1 < n ? 2 * j + 2 : 2 * n - 1; };
+  auto t_s = [&](int q, int b) { return tmem + q * (2 * BN + D) + b * BN; };
+  auto t_o = [&](int q) { return tmem + q * (2 * BN + D) + 2 * BN; };
+  Part p;
+
+  if (warp == C::COPY || warp == C::COPY + 1) {
+    // ===================== copying warps: all of one runs its loop, one lane issues
+    const bool value = warp == C::COPY + 1;
+    const uint64_t policy = l2_policy_evict_first();
+    const int run = ta.run, runs = BN / run;
+    uint32_t part_phase = 0;
+    unsigned tile0 = 0;                    // tiles of the parts before
+    while (next(p)) {
+      const int n = p.u1 - p.u0;
+      // cache rows of the runs of eight tiles from j on, one per lane (four lanes a tile)
+      auto look_up = [&](int j) {
+        const int key = p.base + (j + (lane >> 2)) * BN + min(lane & 3, runs - 1) * run;
+        if (key >= p.hi) return 0u;
+        const int pg = (int)__umulhi((unsigned)key >> 4 << 1, ta.page_magic);
+        return ((uint32_t)checked_block(__ldg(p.table + pg), a.num_blocks) * a.hkv + p.kvh) * a.page + (key - pg * a.page);
+      };
+      uint32_t rows = 0;
+      for (int j = 0; j < n; ++j) {
+        if ((j & 7) == 0) rows = look_up(j);
+        const int from = (j & 7) * 4, first = p.base + j * BN;
+        const int here = min(runs, (p.hi - first + run - 1) / run);     // runs that lie in the list
+        const unsigned place = 2 * tile0 + (value ? value_at(j, n) : key_at(j));
+        if constexpr (!C::BYTES) {
+          const unsigned slot = place % C::SLOTS;
+          mbar_wait(&bar_empty[slot], ((place / C::SLOTS) & 1) ^ 1, 80);   // a slot's first use waits for nobody
+          const bool part = value && (first < p.lo || first + BN > p.hi);
+          uint64_t* bar = part ? bar_part : &bar_full[slot];
+          uint8_t* dst = s_kv + slot * C::SLOT;
+          if (elect_one()) mbar_arrive_expect_tx(bar, here * run * D * 2);
+          for (int x = 0; x < here; ++x) {
+            const int row = (int)__shfl_sync(0xffffffffu, rows, from + x);
+            if (elect_one()) {
+#pragma unroll
+              for (int c = 0; c < DSUB; ++c) tma_load_2d(dst + c * (BN * 128) + x * run * 128, value ? &map_v : &map_k, bar, c * 128, row, policy);
+            }
+          }
+          __syncwarp();
+          if (part) {
+            // zeros where the list does not reach: 0 x NaN would be NaN
+            mbar_wait(bar_part, part_phase, 78);
+            part_phase ^= 1;
+            for (int x = lane; x < BN * DSUB * 8; x += 32) {
+              const int key = first + (x >> 3) % BN;
+              if (key < p.lo || key >= p.hi) *reinterpret_cast<uint4*>(dst + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar_full[slot]);
+          }
+        } else {
+          const unsigned slot = place % C::RAWS;
+          mbar_wait(&bar_used[slot], ((place / C::RAWS) & 1) ^ 1, 80);
+          uint8_t* dst = s_raw + slot * C::RAW;
+          const uint8_t* src = reinterpret_cast<const uint8_t*>(value ? a.v : a.k);
+          // scales of both sides come with the keys: the softmax looks at them before the values are there
+          float* scales = s_scale + ((tile0 + j) % kScaleTiles) * (2 * BN);
+          if (elect_one()) mbar_arrive_expect_tx(&bar_raw[slot], here * run * (D + (value ? 0 : 8)));
+          for (int x = 0; x < here; ++x) {
+            const uint32_t row = __shfl_sync(0xffffffffu, rows, from + x);
+            if (elect_one()) {
+              bulk_copy(dst + x * run * D, src + (uint64_t)row * D, run * D, &bar_raw[slot]);
+              if (!value) {
+                bulk_copy(scales + x * run, a.ks + row, run * 4, &bar_raw[slot]);
+                bulk_copy(scales + BN + x * run, a.vs + row, run * 4, &bar_raw[slot]);
+              }
+            }
+          }
+          __syncwarp();
+        }
+      }
+      tile0 += n;
+    }
+  } else if (warp > C::COPY + 1) {
+    // ===================== converting warps
+    if constexpr (C::BYTES) {
+      const int tid = threadIdx.x - 32 * (C::COPY + 2);
+      constexpr int PER = D / 16, KEYS = 32 * C::CONVERT / PER;      // 16-byte chunks of a key, keys between a thread's chunks
+      constexpr int CH = BN / KEYS;                                // a thread's chunks of a tile
+      const int key0 = tid / PER, ch = tid % PER;                  // this thread's first key, its place in every key
+      // eight lanes write one key: lanes of odd 64-column halves begin with their second chunk, so that no two meet in a bank
+      const int flip = (ch >> 2) & 1;
+      const uint32_t to = (ch >> 2) * (BN * 128) + key0 * 128, c0 = ((2 * (ch & 3) + flip) ^ (key0 & 7)) << 4;
+      static_assert(KEYS % 8 == 0, "every eighth key has the same place in the swizzle");
+      unsigned slot = 0, raw_slot = 0, tile0 = 0;
+      uint32_t phase = 1, raw_phase = 0;
+      while (next(p)) {
+        const int n = p.u1 - p.u0;
+        auto convert = [&](int j, bool value) {
+          const int first = p.base + j * BN;
+          const bool all = first >= p.lo && first + BN <= p.hi;
+          const uint8_t* raw = s_raw + raw_slot * C::RAW;
+          mbar_wait(&bar_raw[raw_slot], raw_phase, 77);
+          auto inside = [&](int key) { return all || (first + key >= p.lo && first + key < p.hi); };
+          uint4 x[CH];
+#pragma unroll
+          for (int c = 0; c < CH; ++c) {
+            const int key = key0 + c * KEYS;
+            x[c] = *reinterpret_cast<const uint4*>(raw + key * D + ch * 16);
+            if (!inside(key)) x[c] = make_uint4(0u, 0u, 0u, 0u);     // zeros where the list does not reach
+          }
+          if (!value && tid < 32) {
+            // the values' scales relative to the power of two above the largest
+            float* vs = s_scale + ((tile0 + j) % kScaleTiles) * (2 * BN) + BN;
+            const float v0 = inside(lane) ? vs[lane] : 0.f, v1 = inside(lane + 32) ? vs[lane + 32] : 0.f;
+            const int e = tile_exponent(v0, v1);
+            vs[lane] = v0 * two_to(-e), vs[lane + 32] = v1 * two_to(-e);
+            if (lane == 0) s_tile[(tile0 + j) % kScaleTiles].v_exp = (float)e;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar_used[raw_slot]);
+          if (++raw_slot == C::RAWS) raw_slot = 0, raw_phase ^= 1;
+          mbar_wait(&bar_empty[slot], phase, 81);
+          uint8_t* dst = s_kv + slot * C::SLOT + to;
+#pragma unroll
+          for (int c = 0; c < CH; ++c) {
+            uint4 y[2];
+            codes4<FMT>(x[c].x, y[0].x, y[0].y);
+            codes4<FMT>(x[c].y, y[0].z, y[0].w);
+            codes4<FMT>(x[c].z, y[1].x, y[1].y);
+            codes4<FMT>(x[c].w, y[1].z, y[1].w);
+            uint8_t* at = dst + c * (KEYS * 128);
+            *reinterpret_cast<uint4*>(at + c0) = flip ? y[1] : y[0];
+            *reinterpret_cast<uint4*>(at + (c0 ^ 16)) = flip ? y[0] : y[1];
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar_full[slot]);
+          if (++slot == C::SLOTS) slot = 0, phase ^= 1;
+        };
+        for (int j = 0; j <= n; ++j) {
+          if (j < n) convert(j, false);
+          if (j > 0) convert(j - 1, true);
+        }
+        tile0 += n;
+      }
+    }
+  } else if (warp >= C::SOFT) {
+    // ===================== issuing warps: all of one runs its loop, one lane issues
+    const int q = warp - C::SOFT;
+    const int fmt = std::is_same<M, __half>::value ? 0 : 1;
+    const uint32_t id_s = idesc(fmt, BN, 0), id_o = idesc(fmt, D, 1);
+    const uint32_t ql = desc_lo(smem_u32(s_q)) + q * (BM * D * 2 / 16), k_lo = desc_lo(smem_u32(s_kv)), v_lo = desc_lo(smem_u32(s_kv), BN * 128);
+    const uint32_t ts = t_s(q, 0), to = t_o(q);
+    unsigned tile0 = 0, mine = 0;          // tiles of the parts before; of them this warp's
+    uint32_t q_phase = 0;
+    while (next(p)) {
+      const int n = p.u1 - p.u0;
+      const unsigned at = 2 * tile0;
+      tile0 += n;
+      if (p.n0 + q * BM >= p.nrows) {
+        // no rows: slots are given back in the order they come
+        for (int x = 0; x < 2 * n; ++x) {
+          const unsigned place = at + x, slot = place % C::SLOTS;
+          mbar_wait(&bar_full[slot], (place / C::SLOTS) & 1, 82);
+          if (lane == 0) mbar_arrive(&bar_empty[slot]);
+          __syncwarp();
+        }
+        continue;
+      }
+      auto scores = [&](int j) {
+        const unsigned place = at + key_at(j), slot = place % C::SLOTS;
+        mbar_wait(&bar_full[slot], (place / C::SLOTS) & 1, 82);
+        tcgen05_fence_after();
+        const uint32_t kl = k_lo + slot * (C::SLOT / 16), b = (mine + j) & 1, d = ts + b * BN;
+        if (elect_one()) {
+#pragma unroll
+          for (int c = 0; c < DSUB; ++c)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) umma_ss(d, ql + (c * (BM * 128) + k * 32) / 16, kl + (c * (BN * 128) + k * 32) / 16, id_s, (c | k) ? 1u : 0u);
+          umma_commit(&bar_s[q * 2 + b]);
+          umma_commit(&bar_empty[slot]);
+        }
+        __syncwarp();
+      };
+      // the queries are in place, and what the list before left in tensor memory has been read
+      mbar_wait(&bar_q[q], q_phase, 79);
+      q_phase ^= 1;
+      for (int j = 0; j < min(n, 2); ++j) scores(j);
+      for (int j = 0; j < n; ++j) {
+        const unsigned place = at + value_at(j, n), slot = place % C::SLOTS, b = (mine + j) & 1, parity = ((mine + j) >> 1) & 1;
+        mbar_wait(&bar_full[slot], (place / C::SLOTS) & 1, 82);
+        mbar_wait(&bar_p[q * 2 + b], parity, 83);
+        tcgen05_fence_after();
+        const uint32_t vl = v_lo + slot * (C::SLOT / 16), pt = ts + b * BN;
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < BN / 16; ++k) umma_ts(to, pt + k * 8, vl + k * 128, id_o, (j > 0 || k > 0) ? 1u : 0u);
+          umma_commit(&bar_o[q * 2 + b]);
+          umma_commit(&bar_empty[slot]);
+        }
+        __syncwarp();
+        if (j + 2 < n) {
+          mbar_wait(&bar_o[q * 2 + b], parity, 84);              // P_j has been read: S_{j+2} goes over it
+          scores(j + 2);
+        }
+      }
+      mine += n;
+    }
+  } else {
+    // ===================== softmax: a thread per row
+    const int q = warp >> 2, quarter = warp & 3;
+    const uint32_t off = (uint32_t)(quarter * 32) << 16;
+    // this warp's 32 rows of queries, and where its outputs are staged: D / 64 pieces of 32 x 128 bytes, swizzled
+    uint8_t* s_mine = s_q + q * (BM * D * 2) + quarter * (32 * 128);
+    auto place = [&](int row, int ch) { return s_mine + (ch >> 3) * (BM * 128) + row * 128 + (((ch & 7) ^ (row & 7)) << 4); };
+    constexpr float kUp = std::is_same<M, __half>::value ? 7.0f : 0.0f;   // f16 ends at 2^16: probabilities are formed times 2^7, at most 2^15
+    unsigned tile0 = 0, mine = 0;          // tiles of the parts before; of them this warp's
+    while (next(p)) {
+      const int n = p.u1 - p.u0, n0 = p.n0 + q * BM + quarter * 32;
+      const unsigned at = tile0;
+      tile0 += n;
+      if (p.n0 + q * BM >= p.nrows) continue;
+      if (n0 >= p.nrows) {
+        // no rows of this warp's: its barriers go on, whatever the products make of them
+        if (lane == 0) mbar_arrive(&bar_q[q]);
+        for (int j = 0; j < n; ++j, ++mine) {
+          mbar_wait(&bar_s[q * 2 + (mine & 1)], (mine >> 1) & 1, 85);
+          if (lane == 0) mbar_arrive(&bar_p[q * 2 + (mine & 1)]);
+          __syncwarp();
+        }
+        continue;
+      }
+      const int row = n0 + lane;
+      const bool live = row < p.nrows;
+      const int tok = p.s.row0 + row / group, head = p.kvh * group + row % group;
+      float scale = a.scale_log2;
+      {
+        const int64_t from = live ? (int64_t)tok * a.ldq + (int64_t)head * D : -1;
+        constexpr int LANES = D / 8 < 32 ? D / 8 : 32, STEP = 32 / LANES;    // lanes of a row, rows of one copy of the warp
+        const int ch = lane % LANES;
+        // loops, not lines: what runs seldom comes from memory, eight instructions at a time
+#pragma unroll 2
+        for (int i = 0; i < 32; i += STEP) {
+          const int r = i + lane / LANES;
+          const int64_t x = __shfl_sync(0xffffffffu, from, r);
+          copy16(smem_u32(place(r, ch)), reinterpret_cast<const T*>(a.q) + (x < 0 ? 0 : x + ch * 8), x < 0 ? 0 : 16);
+        }
+        copies_wait_all();
+        __syncwarp();
+        if constexpr (!std::is_same<M, T>::value) {
+          // bf16 to f16 where they lie, each row by its own thread, after division by the power of two below its largest value
+          uint32_t top = 0;                               // largest absolute value, as bits: NaN lies above infinity
+#pragma unroll 4
+          for (int c = 0; c < D / 8; ++c) {
+            const uint4 x = *reinterpret_cast<const uint4*>(place(lane, c));
+            top = __vmaxu2(top, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
+          }
+          top = max(top & 0xffffu, top >> 16) >> 7;       // bf16: eight bits of exponent above seven of fraction
+          const int e = top == 255 ? 0 : max(-126, min(126, (int)top - 127));
+          const float down = two_to(-e);
+#pragma unroll 4
+          for (int c = 0; c < D / 8; ++c) {
+            uint4* x = reinterpret_cast<uint4*>(place(lane, c));
+            float y[8];
+            unpack8<T>(*x, y);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[k] *= down;
+            *x = pack8<__half>(y);
+          }
+          scale *= two_to(e);
+        }
+        fence_proxy_async_smem();
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar_q[q]);
+      }
+      // cached tokens, which the row sees all; its mask says which of the new ones (rows beyond the last see everything and are dropped)
+      int ctx = p.hi;
+      if (live) {
+        const int sq = p.own ? p.seg : seq_of_row(a.cu, 0, a.num_seqs, tok);
+        ctx = p.own ? p.s.ctx : sq < 0 ? 0 : tree_context(a, sq);
+      }
+      const bool masked = live && p.own;
+      const int pos = min(ctx, p.hi) - 1;
+      float m_run = -INFINITY, l_run = 0.f;
+      // outputs are sums of probabilities times 2^up: with scales, less the exponent of the values' largest so far.  The sum of probabilities stands relative
+      // to the maximum alone then: keys count whose values are far smaller than others
+      float up = C::BYTES ? INFINITY : kUp;
+      bool partly = false;                                // some row of the warp does not see some key of its tiles
+      bool bad = false;                                   // a score of the row is NaN: so is the result, whatever the exponentials made of it
+      bool sees = false;
+      for (int j = 0; j < n; ++j, ++mine) {
+        const int b = mine & 1, kb = p.base + j * BN;
+        mbar_wait(&bar_s[q * 2 + b], (mine >> 1) & 1, 85);
+        tcgen05_fence_after();
+        float sc[BN];
+        {
+          uint32_t r[BN / 32][32];
+#pragma unroll
+          for (int c = 0; c < BN / 32; ++c) tmem_ld_32x32b_x32(t_s(q, b) + off + c * 32, r[c]);
+          tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < BN / 32; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) sc[c * 32 + i] = __uint_as_float(r[c][i]);
+        }
+        const float* scales = s_scale + ((at + j) % kScaleTiles) * (2 * BN);
+        float v_exp = 0.f;
+        if constexpr (C::BYTES) {
+          v_exp = s_tile[(at + j) % kScaleTiles].v_exp;
+#pragma unroll
+          for (int i = 0; i < BN; i += 4) {
+            const float4 k4 = *reinterpret_cast<const float4*>(scales + i);
+            fmul2(sc[i], sc[i + 1], sc[i], sc[i + 1], k4.x, k4.y);
+            fmul2(sc[i + 2], sc[i + 3], sc[i + 2], sc[i + 3], k4.z, k4.w);
+          }
+        }
+        const int hi = pos - kb, lo = p.lo - kb;
+        uint32_t see[2] = {~0u, ~0u};
+        const bool edge = __any_sync(0xffffffffu, hi < BN - 1 || lo > 0);
+        if (edge) {
+          partly = true;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            see[c] = (masked ? tree_bits(a, tok, kb + c * 32 - ctx) : ~0u) & bit_range(lo - c * 32, (masked ? p.hi - 1 - kb : hi) - c * 32);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if ((see[c] >> i & 1u) == 0) sc[c * 32 + i] = -INFINITY;
+          }
+          sees = sees || (see[0] | see[1]) != 0;
+        } else {
+          sees = true;
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < BN; i += 8) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) mx[u] = max_nan(mx[u], max_nan(sc[i + 2 * u], sc[i + 2 * u + 1]));
+        }
+        const float m_tile = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * scale;
+        bad = bad || m_tile != m_tile;
+        const bool grow = m_tile > m_run + 8.0f;
+        const float m_new = grow ? m_tile : m_run;
+        float up_new = up;
+        if constexpr (C::BYTES) up_new = fminf(up, kUp - v_exp);
+        const float alpha = j > 0 && m_new > -INFINITY && (grow || up_new != up) ? exp2_fast((m_run - m_new) + (up_new - up)) : 1.0f;
+        const float fade = C::BYTES ? (j > 0 && grow ? exp2_fast(m_run - m_new) : 1.0f) : alpha;
+        m_run = m_new;
+        up = up_new;
+        // of this tile's probabilities; below 2^-32 they are zeros in f16, and by a factor of 2^-60 their sum still is what it is
+        const float lift = C::BYTES ? fmaxf(up + v_exp, -60.0f) : up;
+        const float neg = m_new == -INFINITY ? 0.f : lift - m_new;
+        float la[4] = {0.f, 0.f, 0.f, 0.f}, lb[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < BN / 32; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            float e[4], x[4];
+            const float* s4 = sc + c * 32 + i;
+            ffma2(e[0], e[1], s4[0], s4[1], scale, scale, neg, neg);
+            ffma2(e[2], e[3], s4[2], s4[3], scale, scale, neg, neg);
+            // every fourth exponential on the FMA pipe: the MUFU pipe alone would need as many clocks as a tile's products
+            x[0] = exp2_fast(e[0]), x[1] = exp2_fast(e[1]), x[2] = exp2_fast(e[2]), x[3] = exp2_fma(e[3]);
+            fadd2(la[(i >> 1) & 3], lb[(i >> 1) & 3], la[(i >> 1) & 3], lb[(i >> 1) & 3], x[0], x[1]);
+            fadd2(la[(i >> 1 & 3) + 1], lb[(i >> 1 & 3) + 1], la[(i >> 1 & 3) + 1], lb[(i >> 1 & 3) + 1], x[2], x[3]);
+            if constexpr (C::BYTES) {
+              const float4 v4 = *reinterpret_cast<const float4*>(scales + BN + c * 32 + i);
+              fmul2(x[0], x[1], x[0], x[1], v4.x, v4.y);
+              fmul2(x[2], x[3], x[2], x[3], v4.z, v4.w);
+            }
+            pk[i >> 1] = pack16<M>(x[0], x[1]);
+            pk[(i >> 1) + 1] = pack16<M>(x[2], x[3]);
+          }
+          if (C::BYTES && edge) {
+            // a hidden key weighs nothing whatever its value's scale is
+#pragma unroll
+            for (int i = 0; i < 16; ++i) pk[i] &= ((see[c] >> (2 * i) & 1u) ? 0xffffu : 0u) | ((see[c] >> (2 * i + 1) & 1u) ? 0xffff0000u : 0u);
+          }
+          tmem_st_x16(t_s(q, b) + off + c * 16, pk);
+        }
+        tmem_st_done();
+        const float l_tile = ((la[0] + lb[0]) + (la[1] + lb[1])) + ((la[2] + lb[2]) + (la[3] + lb[3]));
+        if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+          mbar_wait(&bar_o[q * 2 + (b ^ 1)], ((mine - 1) >> 1) & 1, 86);
+          tcgen05_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(t_o(q) + off + c * 32, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+            tmem_st_x32(t_o(q) + off + c * 32, r);
+          }
+          tmem_st_done();
+        }
+        l_run = l_run * fade + (C::BYTES ? l_tile * exp2_fast(-lift) : l_tile);
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar_p[q * 2 + b]);
+      }
+      mbar_wait(&bar_o[q * 2 + ((mine - 1) & 1)], ((mine - 1) >> 1) & 1, 87);
+      tcgen05_fence_after();
+
+      // ---- the list's result, or its part.  Rows go through shared memory, where this warp's queries were, and from there by the whole warp
+      if (bad) l_run = __int_as_float(0x7fc00000);
+      const bool whole = p.u0 == 0 && p.u1 == p.n, direct = whole && a.groups == 0;
+      const int slot = 2 * blockIdx.x + (p.u0 == 0 && at > 0 ? 1 : 0);
+      if (p.u0 == 0 && q == 0 && quarter == 0 && lane == 0) {
+        FewInfo in;
+        in.first_slot = whole ? -1 : slot;
+        in.first_warp = blockIdx.x;
+        in.last_warp = (w.cur - (p.u1 - p.u0) + p.n - 1) / per;
+        in.pad = 0;
+        pa.info[((int64_t)p.seg * a.hkv + p.kvh) * pa.row_tiles + p.rt] = in;
+      }
+      PartRows rows;
+      rows.table = p.table, rows.kvh = p.kvh, rows.row0 = p.s.row0, rows.n0 = n0, rows.from = max(p.base, p.s.lo), rows.lo = p.lo, rows.hi = p.hi;
+      rows.seg = p.own ? p.seg : -1;
+      rows.parts = direct ? nullptr : pa.slots + ((int64_t)slot * ROWS + q * BM + quarter * 32) * (D + kPad);
+      unsigned anew = 0;
+      if constexpr (FMT != kInt8)                         // (int8: a hidden value is 0 x a number)
+        if (partly) anew = spoiled_rows<M, FMT, D>(a, rows, t_o(q) + off, live && !bad);
+      uint8_t* out = nullptr;
+      // a part of a row that is finished here goes beside the groups' or own ones of the same row
+      float* part = whole ? (p.own ? pa.whole_own : pa.whole_group) + ((int64_t)tok * a.hq + head) * (D + kPad) : rows.parts + lane * (D + kPad);
+      if (live && (anew >> lane & 1) == 0) {
+        if (direct) {
+          out = reinterpret_cast<uint8_t*>(reinterpret_cast<T*>(a.out) + (int64_t)tok * a.ldo + (int64_t)head * D);
+        } else {
+          *reinterpret_cast<float2*>(part + D) = make_float2(C::BYTES ? m_run : m_run - up, l_run);
+          out = reinterpret_cast<uint8_t*>(part);
+        }
+      }
+      const float down = C::BYTES ? exp2f(-up) : 1.0f;    // of outputs, to the sum's reference
+      const float inv = direct ? down / l_run : down;
+      // 128 bytes of each of 32 rows: staged by the rows' threads, stored by eight lanes a row
+      auto store = [&](int piece, int to) {
+        __syncwarp();
+#pragma unroll 4
+        for (int i = 0; i < 32; i += 4) {
+          const int r = i + (lane >> 3);
+          const uint64_t x = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(out), r);
+          if (x != 0) *reinterpret_cast<uint4*>(x + to + (lane & 7) * 16) = *reinterpret_cast<const uint4*>(place(r, piece * 8 + (lane & 7)));
+        }
+      };
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(t_o(q) + off + c * 32, r);
+        tmem_ld_wait();
+        if (direct) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            float f8[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f8[e] = sees ? __uint_as_float(r[i + e]) * inv : 0.f;
+            *reinterpret_cast<uint4*>(place(lane, c * 4 + i / 8)) = pack8<T>(f8);
+          }
+          if (c & 1) store(c >> 1, (c >> 1) * 128);
+        } else {
+          const int piece = c % DSUB;
+          __syncwarp();                                   // what was staged there has been stored
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<float4*>(place(lane, piece * 8 + i / 4)) =
+                make_float4(__uint_as_float(r[i]) * inv, __uint_as_float(r[i + 1]) * inv, __uint_as_float(r[i + 2]) * inv, __uint_as_float(r[i + 3]) * inv);
+          store(piece, c * 128);
+        }
+      }
+      if (anew != 0) {
+        if (whole && !direct) {
+          // rows of a finished part lie apart
+          for (unsigned rest = anew; rest != 0; rest &= rest - 1) {
+            const int i = __ffs(rest) - 1;
+            PartRows one = rows;
+            one.n0 = n0 + i;
+            one.parts = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(part), i));
+            rows_anew<T, T, FMT, D>(a, one, 1u);
+          }
+        } else {
+          rows_anew<T, T, FMT, D>(a, rows, anew);
+        }
+      }
+      __syncwarp();                                       // what was staged has been stored: the next list's queries go over it
+    }
+  }
+
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == C::SOFT) {
+    tcgen05_fence_after();
+    tmem_dealloc(tmem, C::TMEM);
+  }
+}
+
+template <typename T, int FMT, int D, int NQ>
+int launch(const AttnArgs& a, const PartArgs& p, cudaStream_t stream) {
+  using C = Tree<FMT, D, NQ>;
+  static_assert(C::SMEM <= 232448, "shared memory of a block");
+  static PerDeviceSmem configured;
+  auto kern = attn_tree_kernel<T, FMT, D, NQ>;
+  LLMSS_CHECK_CUDA(configured.ensure(kern, C::SMEM));
+  TreeArgs ta;
+  ta.own = a.num_seqs;
+  ta.segs = a.num_seqs + a.groups;
+  ta.row_tiles = p.row_tiles;
+  ta.page_magic = (uint32_t)(((1ull << 31) + a.page / 16 - 1) / (a.page / 16));
+  ta.run = a.page % 64 == 0 ? 64 : a.page % 32 == 0 ? 32 : 16;
+  CUtensorMap map_k, map_v;
+  memset(&map_k, 0, sizeof(map_k));
+  memset(&map_v, 0, sizeof(map_v));
+  if (!C::BYTES) {
+    const int64_t rows = (int64_t)a.num_blocks * a.hkv * a.page;
+    if (int e = encode_pages(&map_k, a.k, rows, D * 2, ta.run)) return e;
+    if (int e = encode_pages(&map_v, a.v, rows, D * 2, ta.run)) return e;
+  }
+  LLMSS_CHECK_CUDA(launch_pdl(kern, dim3(kTreeBlocks), dim3(C::THREADS), (size_t)C::SMEM, stream, map_k, map_v, a, p, ta));
+  return 0;
+}
+
+template <typename T, int FMT>
+int by_size(const AttnArgs& a, const PartArgs& p, cudaStream_t stream) {
+  if (a.d == 256) return launch<T, FMT, 256, 1>(a, p, stream);
+  if (a.d == 128) return p.rows == 256 ? launch<T, FMT, 128, 2>(a, p, stream) : launch<T, FMT, 128, 1>(a, p, stream);
+  return p.rows == 256 ? launch<T, FMT, 64, 2>(a, p, stream) : launch<T, FMT, 64, 1>(a, p, stream);
+}
+
+}  // namespace
+
+namespace pages {
+
+int tree_launch(const AttnArgs& a, const PartArgs& p, int fmt, int dtype, cudaStream_t stream) {
+  if (dtype == LLMSS_F16)
+    return fmt == kInt8 ? by_size<__half, kInt8>(a, p, stream) : fmt == kE4M3 ? by_size<__half, kE4M3>(a, p, stream) : by_size<__half, kF16Pages>(a, p, stream);
+  return fmt == kInt8   ? by_size<__nv_bfloat16, kInt8>(a, p, stream)
+         : fmt == kE4M3 ? by_size<__nv_bfloat16, kE4M3>(a, p, stream)
+                        : by_size<__nv_bfloat16, kF16Pages>(a, p, stream);
+}
+
+}  // namespace pages
