@@ -381,7 +381,7 @@ Plan plan_call(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv
     p.rows = tile_rows(d, most);
     p.row_tiles = (int)((most + p.rows - 1) / p.rows);
     p.slots = (int64_t)2 * kTreeBlocks * p.rows * (d + kPad);
-    p.info = ((int64_t)num_seqs + groups) * hkv * p.row_tiles * 4;
+    p.info = groups > 0 ? ((int64_t)num_seqs + groups) * hkv * p.row_tiles * 4 : kTreeBlocks * 4;
     p.whole = groups > 0 ? (int64_t)total_q * hq * (d + kPad) : 0;
     p.floats = p.slots + p.info + 2 * p.whole;
     return p;
@@ -549,6 +549,10 @@ int attend(const void* q, int64_t ldq, const void* k_pages, const float* k_scale
                     "attn_tree: 2^31 tiles of 64 keys and more");
       if (int e = tree_launch(a, p, fmt, dtype, stream)) return e;
       ++*launches;
+      if (a.groups == 0) {
+        ++*launches;
+        return 0;
+      }
     } else if (plan.few_own || plan.few_groups) {
       if (int e = few_launch(a, p, fmt, dtype, plan.blocks, tiles, stream)) return e;
       ++*launches;

@@ -14,6 +14,10 @@
 //   softmax warps   a thread per row: S from tensor memory times the keys' scales, mask, running maximum (moved when exceeded by 2^8) and sum in 32 bits,
 //                   P times the values' scales back.  Those without a row of the list only keep the barriers going
 //
+// One warp per scheduler waits for its own loads and exponentials most of the time.  So there are two streams (tensor memory of 256 columns holds one):
+// two tiles of 128 rows over the same keys, or, where a segment has up to 128 rows, even and odd tiles of keys of the same rows (DUAL), each with scores,
+// outputs, maximum and sum of its own, which are joined at a list's end.
+//
 // The values' scales join the probabilities before their one rounding to f16, relative to a power of two per tile (TileScales) that keeps them in range;
 // scaled and rounded codes (2^-11 of each key, value and probability) would make f16 results three times as far off.
 // A list within a block's run is finished there, one that crosses runs leaves its parts in scratch, at most two per block, and the merge kernel joins them.
@@ -35,19 +39,22 @@ struct SegInfo {
   int ctx;                // cached tokens in front of the new ones (own lists)
 };
 
-template <int FMT, int D, int NQ>
+template <int FMT, int D, int NQ, bool DUAL>
 struct Tree {
   static constexpr bool BYTES = FMT != kF16Pages;
-  static constexpr int ROWS = NQ * BM;
+  static constexpr int QT = DUAL ? 1 : NQ;                              // tiles of 128 rows; NQ streams
+  static constexpr int ROWS = QT * BM;
   static constexpr int SOFT = 4 * NQ;                                   // softmax warps
   static constexpr int CONVERT = !BYTES ? 0 : NQ == 2 ? 4 : 8;
   static constexpr int COPY = SOFT + NQ;                                // first copying warp
-  static constexpr int THREADS = 32 * (COPY + 2 + CONVERT);
+  static constexpr int CONV = COPY + 2;                                 // first converting warp
+  static constexpr int THREADS = 32 * (CONV + CONVERT);
   static constexpr int Q_BYTES = ROWS * D * 2;
   static constexpr int SLOT = BN * D * 2;                               // a tile of keys or values
   static constexpr int RAW = BYTES ? BN * D : 0;                        // a tile of codes
   static constexpr int SCALES = BYTES ? kScaleTiles * (2 * BN * 4 + 16) : 0;
-  static constexpr int FIXED = 1024 + Q_BYTES + SCALES + 1024 + kKept * (int)sizeof(SegInfo) + 64;
+  static constexpr int JOIN = DUAL ? BM * (128 + 16) : 0;               // what a stream hands to the other: 32 columns of its rows, and their state
+  static constexpr int FIXED = 1024 + Q_BYTES + SCALES + JOIN + 1024 + kKept * (int)sizeof(SegInfo) + 64;
   static constexpr int ROOM = 232448 - FIXED;
   // 16 bits: all there is, up to 24.  8 bits: three to eight tiles in f16, codes in the rest; a tile's scales are looked at until its values' slot is free,
   // which is RAWS + SLOTS copies behind: fewer than two per tile of scales
@@ -55,7 +62,8 @@ struct Tree {
   static constexpr int RAWS = !BYTES ? 0 : (ROOM - SLOTS * SLOT) / RAW < 16 ? (ROOM - SLOTS * SLOT) / RAW : 16;
   static constexpr int SMEM = FIXED + SLOTS * SLOT + RAWS * RAW;
   static constexpr int TMEM = NQ * (2 * BN + D) <= 256 ? 256 : 512;
-  static_assert(SLOTS >= 3 && (!BYTES || (RAWS >= 3 && RAWS + SLOTS <= 2 * kScaleTiles - 4)), "rings");
+  static constexpr int RING = DUAL ? SLOTS / 2 : SLOTS;                 // slots of a ring: each stream's own (DUAL)
+  static_assert(RING >= (BYTES ? 3 : DUAL ? 5 : 4) && (!BYTES || (RAWS >= 3 && RAWS + SLOTS <= 2 * kScaleTiles - 4)), "rings");
   static_assert((2 * SLOTS + 2 * RAWS + 7 * NQ + 2) * 8 <= 1024, "barriers");
 };
 
@@ -108,8 +116,26 @@ __device__ __forceinline__ void codes4(uint32_t w, uint32_t& lo, uint32_t& hi) {
   }
 }
 
-// 2^x without the MUFU pipe; 0 for what is below -127 (hidden keys weigh nothing, however large their values), and for NaN
-__device__ __forceinline__ float exp2_fma(float x) { return exp2_cubic(fmaxf(x, -127.0f)); }
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^x of two numbers without the MUFU pipe (exp2_cubic, in pairs); 0 for what is below -127 (hidden keys weigh nothing, however large their values), and for NaN
+__device__ __forceinline__ void exp2_pair(float& y0, float& y1, float x0, float x1) {
+  using namespace packed;
+  const pair_t x = pack(fmaxf(x0, -127.0f), fmaxf(x1, -127.0f)), magic = both(12582912.0f);
+  const pair_t t = padd(x, magic), r = psub(x, psub(t, magic));
+  pair_t p = pfma(r, both(0.05459282f), both(0.24221784f));
+  p = pfma(r, p, both(0.6933686f));
+  p = pfma(r, p, both(1.0f));
+  const float2 tf = unpack(t), pf = unpack(p);
+  y0 = __int_as_float(__float_as_int(pf.x) + (__float_as_int(tf.x) << 23));     // (what the 1.5 2^23 of t holds besides x leaves the word)
+  y1 = __int_as_float(__float_as_int(pf.y) + (__float_as_int(tf.y) << 23));
+}
+// warps `quarter` of both streams
+__device__ __forceinline__ void pair_sync(int quarter) { asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory"); }
 
 template <int ROWS>
 __device__ __forceinline__ SegInfo seg_info(const AttnArgs& a, const TreeArgs& ta, int i) {
@@ -132,6 +158,11 @@ struct Part {
   int base, lo, hi;       // first key of its first tile; its keys
   int n0, nrows;          // first row; rows of the segment
 };
+// the list that a block begins and others go on with (where no groups share its rows): its first slot, < 0: none; the others' last block
+struct Cut {
+  int slot, last, seg, list;         // list: kvh row_tiles + tile of rows
+};
+static_assert(sizeof(Cut) == sizeof(FewInfo), "they share their place");
 // a place in a run
 struct Walk {
   unsigned cur, end, before;
@@ -186,21 +217,22 @@ __device__ __noinline__ void rows_anew(const AttnArgs& a, const PartRows& p, uns
   }
 }
 
-template <typename T, int FMT, int D, int NQ>
-__global__ void __launch_bounds__(Tree<FMT, D, NQ>::THREADS, 1)
+template <typename T, int FMT, int D, int NQ, bool DUAL>
+__global__ void __launch_bounds__(Tree<FMT, D, NQ, DUAL>::THREADS, 1)
 attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnArgs a,
                  const __grid_constant__ PartArgs pa, const __grid_constant__ TreeArgs ta) {
-  using C = Tree<FMT, D, NQ>;
+  using C = Tree<FMT, D, NQ, DUAL>;
   using M = typename std::conditional<C::BYTES, __half, T>::type;   // type of the products
   constexpr int DSUB = D / 64, ROWS = C::ROWS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint8_t* s_q = smem;                                   // [NQ][DSUB][128 rows][128 bytes]
+  uint8_t* s_q = smem;                                   // [QT][DSUB][128 rows][128 bytes]
   uint8_t* s_kv = s_q + C::Q_BYTES;                      // [SLOTS][DSUB][64 keys][128 bytes]
   uint8_t* s_raw = s_kv + C::SLOTS * C::SLOT;            // [RAWS][64 keys of codes]
   float* s_scale = reinterpret_cast<float*>(s_raw + C::RAWS * C::RAW);   // [tiles][keys', values'][64] (8-bit)
   TileScales* s_tile = reinterpret_cast<TileScales*>(s_scale + (C::BYTES ? kScaleTiles * 2 * BN : 0));   // [tiles]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(s_raw + C::RAWS * C::RAW + C::SCALES);
+  float4* s_join = reinterpret_cast<float4*>(s_raw + C::RAWS * C::RAW + C::SCALES);   // [4 warps][8][32 rows], then [128 rows] (DUAL)
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_raw + C::RAWS * C::RAW + C::SCALES + C::JOIN);
   uint64_t* bar_full = bars;                             // [SLOTS]
   uint64_t* bar_empty = bars + C::SLOTS;
   uint64_t* bar_s = bars + 2 * C::SLOTS;                 // [NQ][2] S ready
@@ -223,7 +255,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::SLOTS; ++i) {
       mbar_init(&bar_full[i], C::BYTES ? C::CONVERT : 1);
-      mbar_init(&bar_empty[i], NQ);
+      mbar_init(&bar_empty[i], C::QT);
     }
     for (int i = 0; i < 2 * NQ; ++i) {
       mbar_init(&bar_s[i], 1);
@@ -242,39 +274,15 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   pdl_launch_dependents();                 // the merge reads lengths in front of its wait
 
   // ---- this block's run (the host has checked that all lists together are below 2^31 tiles)
-  auto weight = [&](int i) {
-    const SegInfo x = seg_info<ROWS>(a, ta, i);
-    return (unsigned)x.units * x.tiles * a.hkv;
-  };
+  auto weigh = [&](const SegInfo& x) { return (unsigned)x.units * x.tiles * a.hkv; };
   unsigned sum = 0;
-  for (int i = threadIdx.x; i < ta.segs; i += C::THREADS) sum += weight(i);
+  for (int i = threadIdx.x; i < ta.segs; i += C::THREADS) {
+    const SegInfo x = seg_info<ROWS>(a, ta, i);
+    if (i < kKept) s_info[i] = x;
+    sum += weigh(x);
+  }
   sum = __reduce_add_sync(0xffffffffu, sum);
   if (lane == 0) s_sum[warp] = sum;
-  __syncthreads();
-  unsigned total = 0;
-  for (int i = 0; i < C::THREADS / 32; ++i) total += s_sum[i];
-  const unsigned per = max((total + gridDim.x - 1) / gridDim.x, (unsigned)kLeastTiles);
-  const unsigned begin = min(per * blockIdx.x, total), end = min(begin + per, total);
-  if (begin >= end) return;
-  __syncthreads();
-  if (warp == 0) {
-    unsigned before = 0;
-    for (int b = 0; b < ta.segs; b += 32) {
-      const unsigned n = b + lane < ta.segs ? weight(b + lane) : 0u;
-      unsigned inc = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned x = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += x;
-      }
-      const unsigned hit = __ballot_sync(0xffffffffu, before + inc > begin);
-      if (hit) {
-        if (lane == __ffs(hit) - 1) s_sum[0] = b + lane, s_sum[1] = before + inc - n;
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, inc, 31);
-    }
-  }
   if (warp == C::SOFT) {
     tmem_alloc(tmem_slot, C::TMEM);
     tmem_relinquish();
@@ -283,11 +291,37 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-  const int seg0 = s_sum[0];
-  Walk w = {begin, end, s_sum[1], seg0};
-  for (int i = threadIdx.x; i < kKept; i += C::THREADS)
-    if (seg0 + i < ta.segs) s_info[i] = seg_info<ROWS>(a, ta, seg0 + i);
-  __syncthreads();
+  unsigned total = 0;
+  for (int i = 0; i < C::THREADS / 32; ++i) total += s_sum[i];
+  const unsigned per = max((total + gridDim.x - 1) / gridDim.x, (unsigned)kLeastTiles);
+  const unsigned begin = min(per * blockIdx.x, total), end = min(begin + per, total);
+  // every warp finds the run's first segment for itself
+  Walk w = {begin, end, 0, 0};
+  int seg0 = 0;                            // of the segments that are kept
+  for (int b = 0; b < ta.segs && begin < end; b += 32) {
+    const unsigned n = b + lane < ta.segs ? weigh(b + lane < kKept ? s_info[b + lane] : seg_info<ROWS>(a, ta, b + lane)) : 0u;
+    unsigned inc = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned x = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += x;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, w.before + inc > begin);
+    if (hit) {
+      const int x = __ffs(hit) - 1;
+      w.seg = b + x;
+      w.before += __shfl_sync(0xffffffffu, inc - n, x);
+      break;
+    }
+    w.before += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  if (ta.segs > kKept) {
+    __syncthreads();
+    seg0 = w.seg;
+    for (int i = threadIdx.x; i < kKept; i += C::THREADS)
+      if (seg0 + i < ta.segs) s_info[i] = seg_info<ROWS>(a, ta, seg0 + i);
+    __syncthreads();
+  }
 
   const int group = a.hq / a.hkv;
   auto next = [&](Part& p) {               // the part at w.cur, and on to the one behind it; false: the run is over
@@ -311,10 +345,23 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     p.n0 = p.rt * ROWS, p.nrows = p.s.rows * group;
     return true;
   };
-  // places of a list's tiles in the ring: K0, then K_{j+1}, V_j, and V of the last tile
+  // places of a list's tiles in the order they come: K0, then K_{j+1}, V_j, and V of the last tile
   auto key_at = [](int j) { return j == 0 ? 0 : 2 * j - 1; };
   auto value_at = [](int j, int n) { return j + 1 < n ? 2 * j + 2 : 2 * n - 1; };
+  // Slot of tile j, with the parity of its use.  Two streams have a ring each, K and V in turn: a barrier tells a phase from the one before alone, so that
+  // who waits on a slot has to take part in each of its uses, and a stream takes no part in the other's tiles
+  struct Slot {
+    unsigned at;
+    uint32_t phase;
+  };
+  auto slot_of = [&](unsigned tile0, unsigned even0, int j, int n, bool value) {     // even0: of the tiles before, the first stream's
+    unsigned place;
+    if constexpr (DUAL) place = 2 * (((j & 1) ? tile0 - even0 : even0) + (j >> 1)) + value;
+    else place = 2 * tile0 + (value ? value_at(j, n) : key_at(j));
+    return Slot{place % C::RING + (DUAL && (j & 1) ? C::RING : 0), (place / C::RING) & 1};
+  };
   auto t_s = [&](int q, int b) { return tmem + q * (2 * BN + D) + b * BN; };
+  constexpr int STREAMS = DUAL ? 2 : 1;    // that share a list's tiles of keys
   auto t_o = [&](int q) { return tmem + q * (2 * BN + D) + 2 * BN; };
   Part p;
 
@@ -324,7 +371,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     const uint64_t policy = l2_policy_evict_first();
     const int run = ta.run, runs = BN / run;
     uint32_t part_phase = 0;
-    unsigned tile0 = 0;                    // tiles of the parts before
+    unsigned tile0 = 0, even0 = 0;         // tiles of the parts before
     while (next(p)) {
       const int n = p.u1 - p.u0;
       // cache rows of the runs of eight tiles from j on, one per lane (four lanes a tile)
@@ -339,10 +386,10 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         if ((j & 7) == 0) rows = look_up(j);
         const int from = (j & 7) * 4, first = p.base + j * BN;
         const int here = min(runs, (p.hi - first + run - 1) / run);     // runs that lie in the list
-        const unsigned place = 2 * tile0 + (value ? value_at(j, n) : key_at(j));
         if constexpr (!C::BYTES) {
-          const unsigned slot = place % C::SLOTS;
-          mbar_wait(&bar_empty[slot], ((place / C::SLOTS) & 1) ^ 1, 80);   // a slot's first use waits for nobody
+          const Slot to = slot_of(tile0, even0, j, n, value);
+          const unsigned slot = to.at;
+          mbar_wait(&bar_empty[slot], to.phase ^ 1, 80);                  // a slot's first use waits for nobody
           const bool part = value && (first < p.lo || first + BN > p.hi);
           uint64_t* bar = part ? bar_part : &bar_full[slot];
           uint8_t* dst = s_kv + slot * C::SLOT;
@@ -368,7 +415,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             if (lane == 0) mbar_arrive(&bar_full[slot]);
           }
         } else {
-          const unsigned slot = place % C::RAWS;
+          const unsigned place = 2 * tile0 + (value ? value_at(j, n) : key_at(j)), slot = place % C::RAWS;
           mbar_wait(&bar_used[slot], ((place / C::RAWS) & 1) ^ 1, 80);
           uint8_t* dst = s_raw + slot * C::RAW;
           const uint8_t* src = reinterpret_cast<const uint8_t*>(value ? a.v : a.k);
@@ -388,21 +435,21 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
           __syncwarp();
         }
       }
-      tile0 += n;
+      tile0 += n, even0 += (n + 1) / 2;
     }
-  } else if (warp > C::COPY + 1) {
+  } else if (warp >= C::CONV) {
     // ===================== converting warps
     if constexpr (C::BYTES) {
-      const int tid = threadIdx.x - 32 * (C::COPY + 2);
+      const int tid = threadIdx.x - 32 * C::CONV;
       constexpr int PER = D / 16, KEYS = 32 * C::CONVERT / PER;      // 16-byte chunks of a key, keys between a thread's chunks
       constexpr int CH = BN / KEYS;                                // a thread's chunks of a tile
-      const int key0 = tid / PER, ch = tid % PER;                  // this thread's first key, its place in every key
-      // eight lanes write one key: lanes of odd 64-column halves begin with their second chunk, so that no two meet in a bank
-      const int flip = (ch >> 2) & 1;
-      const uint32_t to = (ch >> 2) * (BN * 128) + key0 * 128, c0 = ((2 * (ch & 3) + flip) ^ (key0 & 7)) << 4;
+      // this thread's place in every key, and its first key: lanes of odd 64-column halves take the neighbouring one, so that of eight lanes that write
+      // the even chunks (or the odd ones) no two meet in a bank
+      const int ch = tid % PER, key0 = (tid / PER) ^ ((ch >> 2) & 1);
+      const uint32_t to = (ch >> 2) * (BN * 128) + key0 * 128, c0 = ((2 * (ch & 3)) ^ (key0 & 7)) << 4;
       static_assert(KEYS % 8 == 0, "every eighth key has the same place in the swizzle");
-      unsigned slot = 0, raw_slot = 0, tile0 = 0;
-      uint32_t phase = 1, raw_phase = 0;
+      unsigned raw_slot = 0, tile0 = 0, even0 = 0;
+      uint32_t raw_phase = 0;
       while (next(p)) {
         const int n = p.u1 - p.u0;
         auto convert = [&](int j, bool value) {
@@ -416,7 +463,11 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
           for (int c = 0; c < CH; ++c) {
             const int key = key0 + c * KEYS;
             x[c] = *reinterpret_cast<const uint4*>(raw + key * D + ch * 16);
-            if (!inside(key)) x[c] = make_uint4(0u, 0u, 0u, 0u);     // zeros where the list does not reach
+          }
+          if (!all) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+              if (!inside(key0 + c * KEYS)) x[c] = make_uint4(0u, 0u, 0u, 0u);     // zeros where the list does not reach
           }
           if (!value && tid < 32) {
             // the values' scales relative to the power of two above the largest
@@ -429,8 +480,9 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
           __syncwarp();
           if (lane == 0) mbar_arrive(&bar_used[raw_slot]);
           if (++raw_slot == C::RAWS) raw_slot = 0, raw_phase ^= 1;
-          mbar_wait(&bar_empty[slot], phase, 81);
-          uint8_t* dst = s_kv + slot * C::SLOT + to;
+          const Slot here = slot_of(tile0, even0, j, n, value);
+          mbar_wait(&bar_empty[here.at], here.phase ^ 1, 81);
+          uint8_t* dst = s_kv + here.at * C::SLOT + to;
 #pragma unroll
           for (int c = 0; c < CH; ++c) {
             uint4 y[2];
@@ -439,49 +491,47 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             codes4<FMT>(x[c].z, y[1].x, y[1].y);
             codes4<FMT>(x[c].w, y[1].z, y[1].w);
             uint8_t* at = dst + c * (KEYS * 128);
-            *reinterpret_cast<uint4*>(at + c0) = flip ? y[1] : y[0];
-            *reinterpret_cast<uint4*>(at + (c0 ^ 16)) = flip ? y[0] : y[1];
+            *reinterpret_cast<uint4*>(at + c0) = y[0];
+            *reinterpret_cast<uint4*>(at + (c0 ^ 16)) = y[1];
           }
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bar_full[slot]);
-          if (++slot == C::SLOTS) slot = 0, phase ^= 1;
+          if (lane == 0) mbar_arrive(&bar_full[here.at]);
         };
         for (int j = 0; j <= n; ++j) {
           if (j < n) convert(j, false);
           if (j > 0) convert(j - 1, true);
         }
-        tile0 += n;
+        tile0 += n, even0 += (n + 1) / 2;
       }
     }
-  } else if (warp >= C::SOFT) {
+  } else if (warp >= C::SOFT && warp < C::SOFT + NQ) {
     // ===================== issuing warps: all of one runs its loop, one lane issues
     const int q = warp - C::SOFT;
     const int fmt = std::is_same<M, __half>::value ? 0 : 1;
     const uint32_t id_s = idesc(fmt, BN, 0), id_o = idesc(fmt, D, 1);
-    const uint32_t ql = desc_lo(smem_u32(s_q)) + q * (BM * D * 2 / 16), k_lo = desc_lo(smem_u32(s_kv)), v_lo = desc_lo(smem_u32(s_kv), BN * 128);
+    const uint32_t ql = desc_lo(smem_u32(s_q)) + (DUAL ? 0 : q * (BM * D * 2 / 16)), k_lo = desc_lo(smem_u32(s_kv)), v_lo = desc_lo(smem_u32(s_kv), BN * 128);
     const uint32_t ts = t_s(q, 0), to = t_o(q);
-    unsigned tile0 = 0, mine = 0;          // tiles of the parts before; of them this warp's
+    unsigned tile0 = 0, even0 = 0, mine = 0;   // tiles of the parts before; of them this warp's
     uint32_t q_phase = 0;
-    while (next(p)) {
+    for (; next(p); tile0 += p.u1 - p.u0, even0 += (p.u1 - p.u0 + 1) / 2) {
       const int n = p.u1 - p.u0;
-      const unsigned at = 2 * tile0;
-      tile0 += n;
-      if (p.n0 + q * BM >= p.nrows) {
+      if (!DUAL && p.n0 + q * BM >= p.nrows) {
         // no rows: slots are given back in the order they come
         for (int x = 0; x < 2 * n; ++x) {
-          const unsigned place = at + x, slot = place % C::SLOTS;
-          mbar_wait(&bar_full[slot], (place / C::SLOTS) & 1, 82);
+          const unsigned place = 2 * tile0 + x, slot = place % C::RING;
+          mbar_wait(&bar_full[slot], (place / C::RING) & 1, 82);
           if (lane == 0) mbar_arrive(&bar_empty[slot]);
           __syncwarp();
         }
         continue;
       }
       auto scores = [&](int j) {
-        const unsigned place = at + key_at(j), slot = place % C::SLOTS;
-        mbar_wait(&bar_full[slot], (place / C::SLOTS) & 1, 82);
+        const Slot from = slot_of(tile0, even0, j, n, false);
+        const unsigned slot = from.at;
+        mbar_wait(&bar_full[slot], from.phase, 82);
         tcgen05_fence_after();
-        const uint32_t kl = k_lo + slot * (C::SLOT / 16), b = (mine + j) & 1, d = ts + b * BN;
+        const uint32_t kl = k_lo + slot * (C::SLOT / 16), b = (mine + j / STREAMS) & 1, d = ts + b * BN;
         if (elect_one()) {
 #pragma unroll
           for (int c = 0; c < DSUB; ++c)
@@ -493,47 +543,56 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         __syncwarp();
       };
       // the queries are in place, and what the list before left in tensor memory has been read
+      const int first = DUAL ? q : 0;      // this stream's tiles: first, first + STREAMS ..
+      if (n <= first) continue;
       mbar_wait(&bar_q[q], q_phase, 79);
       q_phase ^= 1;
-      for (int j = 0; j < min(n, 2); ++j) scores(j);
-      for (int j = 0; j < n; ++j) {
-        const unsigned place = at + value_at(j, n), slot = place % C::SLOTS, b = (mine + j) & 1, parity = ((mine + j) >> 1) & 1;
-        mbar_wait(&bar_full[slot], (place / C::SLOTS) & 1, 82);
+      for (int j = first; j < min(n, 2 * STREAMS); j += STREAMS) scores(j);
+      for (int j = first; j < n; j += STREAMS) {
+        const Slot from = slot_of(tile0, even0, j, n, true);
+        const unsigned i = mine + j / STREAMS, slot = from.at, b = i & 1, parity = (i >> 1) & 1;
+        mbar_wait(&bar_full[slot], from.phase, 82);
         mbar_wait(&bar_p[q * 2 + b], parity, 83);
         tcgen05_fence_after();
         const uint32_t vl = v_lo + slot * (C::SLOT / 16), pt = ts + b * BN;
         if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < BN / 16; ++k) umma_ts(to, pt + k * 8, vl + k * 128, id_o, (j > 0 || k > 0) ? 1u : 0u);
+          for (int k = 0; k < BN / 16; ++k) umma_ts(to, pt + k * 8, vl + k * 128, id_o, (j > first || k > 0) ? 1u : 0u);
           umma_commit(&bar_o[q * 2 + b]);
           umma_commit(&bar_empty[slot]);
         }
         __syncwarp();
-        if (j + 2 < n) {
-          mbar_wait(&bar_o[q * 2 + b], parity, 84);              // P_j has been read: S_{j+2} goes over it
-          scores(j + 2);
+        if (j + 2 * STREAMS < n) {
+          mbar_wait(&bar_o[q * 2 + b], parity, 84);              // P_j has been read: the scores two tiles on go over it
+          scores(j + 2 * STREAMS);
         }
       }
-      mine += n;
+      mine += (n - first + STREAMS - 1) / STREAMS;
     }
-  } else {
+  } else if (warp < C::SOFT) {
     // ===================== softmax: a thread per row
     const int q = warp >> 2, quarter = warp & 3;
     const uint32_t off = (uint32_t)(quarter * 32) << 16;
     // this warp's 32 rows of queries, and where its outputs are staged: D / 64 pieces of 32 x 128 bytes, swizzled
-    uint8_t* s_mine = s_q + q * (BM * D * 2) + quarter * (32 * 128);
+    uint8_t* s_mine = s_q + (DUAL ? 0 : q * (BM * D * 2)) + quarter * (32 * 128);
     auto place = [&](int row, int ch) { return s_mine + (ch >> 3) * (BM * 128) + row * 128 + (((ch & 7) ^ (row & 7)) << 4); };
     constexpr float kUp = std::is_same<M, __half>::value ? 7.0f : 0.0f;   // f16 ends at 2^16: probabilities are formed times 2^7, at most 2^15
+    auto queries_are_in = [&](int n) {     // for the streams that have a tile
+      mbar_arrive(&bar_q[q]);
+      if (DUAL && n > 1) mbar_arrive(&bar_q[1]);
+    };
     unsigned tile0 = 0, mine = 0;          // tiles of the parts before; of them this warp's
+    Cut cut = {-1, 0, 0, 0};
     while (next(p)) {
-      const int n = p.u1 - p.u0, n0 = p.n0 + q * BM + quarter * 32;
+      const int n = p.u1 - p.u0, q0 = DUAL ? 0 : q * BM, n0 = p.n0 + q0 + quarter * 32;
+      const int first = DUAL ? q : 0;      // this stream's tiles: first, first + STREAMS ..
       const unsigned at = tile0;
       tile0 += n;
-      if (p.n0 + q * BM >= p.nrows) continue;
+      if (p.n0 + q0 >= p.nrows) continue;
       if (n0 >= p.nrows) {
         // no rows of this warp's: its barriers go on, whatever the products make of them
-        if (lane == 0) mbar_arrive(&bar_q[q]);
-        for (int j = 0; j < n; ++j, ++mine) {
+        if (lane == 0 && first == 0) queries_are_in(n);
+        for (int j = first; j < n; j += STREAMS, ++mine) {
           mbar_wait(&bar_s[q * 2 + (mine & 1)], (mine >> 1) & 1, 85);
           if (lane == 0) mbar_arrive(&bar_p[q * 2 + (mine & 1)]);
           __syncwarp();
@@ -544,45 +603,57 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       const bool live = row < p.nrows;
       const int tok = p.s.row0 + row / group, head = p.kvh * group + row % group;
       float scale = a.scale_log2;
-      {
+      if (first == 0) {
         const int64_t from = live ? (int64_t)tok * a.ldq + (int64_t)head * D : -1;
-        constexpr int LANES = D / 8 < 32 ? D / 8 : 32, STEP = 32 / LANES;    // lanes of a row, rows of one copy of the warp
+        constexpr int LANES = D / 8, STEP = 32 / LANES;    // lanes of a row, rows of one step of the warp
         const int ch = lane % LANES;
         // loops, not lines: what runs seldom comes from memory, eight instructions at a time
+        if constexpr (std::is_same<M, T>::value) {
 #pragma unroll 2
-        for (int i = 0; i < 32; i += STEP) {
-          const int r = i + lane / LANES;
-          const int64_t x = __shfl_sync(0xffffffffu, from, r);
-          copy16(smem_u32(place(r, ch)), reinterpret_cast<const T*>(a.q) + (x < 0 ? 0 : x + ch * 8), x < 0 ? 0 : 16);
-        }
-        copies_wait_all();
-        __syncwarp();
-        if constexpr (!std::is_same<M, T>::value) {
-          // bf16 to f16 where they lie, each row by its own thread, after division by the power of two below its largest value
-          uint32_t top = 0;                               // largest absolute value, as bits: NaN lies above infinity
-#pragma unroll 4
-          for (int c = 0; c < D / 8; ++c) {
-            const uint4 x = *reinterpret_cast<const uint4*>(place(lane, c));
-            top = __vmaxu2(top, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
+          for (int i = 0; i < 32; i += STEP) {
+            const int r = i + lane / LANES;
+            const int64_t x = __shfl_sync(0xffffffffu, from, r);
+            copy16(smem_u32(place(r, ch)), reinterpret_cast<const T*>(a.q) + (x < 0 ? 0 : x + ch * 8), x < 0 ? 0 : 16);
           }
-          top = max(top & 0xffffu, top >> 16) >> 7;       // bf16: eight bits of exponent above seven of fraction
-          const int e = top == 255 ? 0 : max(-126, min(126, (int)top - 127));
-          const float down = two_to(-e);
-#pragma unroll 4
-          for (int c = 0; c < D / 8; ++c) {
-            uint4* x = reinterpret_cast<uint4*>(place(lane, c));
-            float y[8];
-            unpack8<T>(*x, y);
+          copies_wait_all();
+        } else {
+          // bf16 to f16 on the way, after division by the power of two below a row's largest value
+          constexpr int AHEAD = 32 / STEP < 8 ? 32 / STEP : 8;
+          for (int i0 = 0; i0 < 32; i0 += AHEAD * STEP) {
+            uint4 y[AHEAD];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) y[k] *= down;
-            *x = pack8<__half>(y);
+            for (int u = 0; u < AHEAD; ++u) {
+              const int64_t x = __shfl_sync(0xffffffffu, from, i0 + u * STEP + lane / LANES);
+              y[u] = x < 0 ? make_uint4(0u, 0u, 0u, 0u) : *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + x + ch * 8);
+            }
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+              // largest absolute value, as bits: NaN lies above infinity
+              uint32_t top = __vmaxu2(__vmaxu2(y[u].x & 0x7fff7fffu, y[u].y & 0x7fff7fffu), __vmaxu2(y[u].z & 0x7fff7fffu, y[u].w & 0x7fff7fffu));
+#pragma unroll
+              for (int o = 1; o < LANES; o <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
+              top = max(top & 0xffffu, top >> 16) >> 7;   // bf16: eight bits of exponent above seven of fraction
+              const int e = top == 255 ? 0 : max(-126, min(126, (int)top - 127)), r = i0 + u * STEP;
+              const float down = two_to(-e);
+              float z[8];
+              unpack8<T>(y[u], z);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) z[k] *= down;
+              *reinterpret_cast<uint4*>(place(r + lane / LANES, ch)) = pack8<__half>(z);
+              const int mine_e = __shfl_sync(0xffffffffu, e, (lane - r) % STEP * LANES);     // (of rows r .. r + STEP - 1)
+              if (lane >= r && lane < r + STEP) scale *= two_to(mine_e);
+            }
           }
-          scale *= two_to(e);
         }
         fence_proxy_async_smem();
         tcgen05_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bar_q[q]);
+        if (lane == 0) queries_are_in(n);
+        if (DUAL && !std::is_same<M, T>::value) s_join[4 * 8 * 32 + quarter * 32 + lane].x = scale;
+      }
+      if constexpr (DUAL && !std::is_same<M, T>::value) {
+        pair_sync(quarter);
+        if (q == 1) scale = s_join[4 * 8 * 32 + quarter * 32 + lane].x;
       }
       // cached tokens, which the row sees all; its mask says which of the new ones (rows beyond the last see everything and are dropped)
       int ctx = p.hi;
@@ -599,7 +670,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       bool partly = false;                                // some row of the warp does not see some key of its tiles
       bool bad = false;                                   // a score of the row is NaN: so is the result, whatever the exponentials made of it
       bool sees = false;
-      for (int j = 0; j < n; ++j, ++mine) {
+      for (int j = first; j < n; j += STREAMS, ++mine) {
         const int b = mine & 1, kb = p.base + j * BN;
         mbar_wait(&bar_s[q * 2 + b], (mine >> 1) & 1, 85);
         tcgen05_fence_after();
@@ -645,7 +716,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 #pragma unroll
         for (int i = 0; i < BN; i += 8) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) mx[u] = max_nan(mx[u], max_nan(sc[i + 2 * u], sc[i + 2 * u + 1]));
+          for (int u = 0; u < 4; ++u) mx[u] = max3_nan(mx[u], sc[i + 2 * u], sc[i + 2 * u + 1]);
         }
         const float m_tile = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * scale;
         bad = bad || m_tile != m_tile;
@@ -653,8 +724,8 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         const float m_new = grow ? m_tile : m_run;
         float up_new = up;
         if constexpr (C::BYTES) up_new = fminf(up, kUp - v_exp);
-        const float alpha = j > 0 && m_new > -INFINITY && (grow || up_new != up) ? exp2_fast((m_run - m_new) + (up_new - up)) : 1.0f;
-        const float fade = C::BYTES ? (j > 0 && grow ? exp2_fast(m_run - m_new) : 1.0f) : alpha;
+        const float alpha = j > first && m_new > -INFINITY && (grow || up_new != up) ? exp2_fast((m_run - m_new) + (up_new - up)) : 1.0f;
+        const float fade = C::BYTES ? (j > first && grow ? exp2_fast(m_run - m_new) : 1.0f) : alpha;
         m_run = m_new;
         up = up_new;
         // of this tile's probabilities; below 2^-32 they are zeros in f16, and by a factor of 2^-60 their sum still is what it is
@@ -670,8 +741,11 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             const float* s4 = sc + c * 32 + i;
             ffma2(e[0], e[1], s4[0], s4[1], scale, scale, neg, neg);
             ffma2(e[2], e[3], s4[2], s4[3], scale, scale, neg, neg);
-            // every fourth exponential on the FMA pipe: the MUFU pipe alone would need as many clocks as a tile's products
-            x[0] = exp2_fast(e[0]), x[1] = exp2_fast(e[1]), x[2] = exp2_fast(e[2]), x[3] = exp2_fma(e[3]);
+            // half of the exponentials on the FMA pipe: the MUFU pipe alone needs 1024 clocks for 256 rows of a tile.  A quarter where scales are applied
+            // and warps convert: there instructions are short as well
+            x[0] = exp2_fast(e[0]), x[1] = exp2_fast(e[1]);
+            if (C::BYTES && (i & 4)) x[2] = exp2_fast(e[2]), x[3] = exp2_fast(e[3]);
+            else exp2_pair(x[2], x[3], e[2], e[3]);
             fadd2(la[(i >> 1) & 3], lb[(i >> 1) & 3], la[(i >> 1) & 3], lb[(i >> 1) & 3], x[0], x[1]);
             fadd2(la[(i >> 1 & 3) + 1], lb[(i >> 1 & 3) + 1], la[(i >> 1 & 3) + 1], lb[(i >> 1 & 3) + 1], x[2], x[3]);
             if constexpr (C::BYTES) {
@@ -691,7 +765,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         }
         tmem_st_done();
         const float l_tile = ((la[0] + lb[0]) + (la[1] + lb[1])) + ((la[2] + lb[2]) + (la[3] + lb[3]));
-        if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+        if (j > first && __any_sync(0xffffffffu, alpha != 1.0f)) {
           mbar_wait(&bar_o[q * 2 + (b ^ 1)], ((mine - 1) >> 1) & 1, 86);
           tcgen05_fence_after();
 #pragma unroll 1
@@ -710,14 +784,17 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar_p[q * 2 + b]);
       }
-      mbar_wait(&bar_o[q * 2 + ((mine - 1) & 1)], ((mine - 1) >> 1) & 1, 87);
-      tcgen05_fence_after();
+      if (n > first) {
+        mbar_wait(&bar_o[q * 2 + ((mine - 1) & 1)], ((mine - 1) >> 1) & 1, 87);
+        tcgen05_fence_after();
+      }
 
       // ---- the list's result, or its part.  Rows go through shared memory, where this warp's queries were, and from there by the whole warp
       if (bad) l_run = __int_as_float(0x7fc00000);
       const bool whole = p.u0 == 0 && p.u1 == p.n, direct = whole && a.groups == 0;
       const int slot = 2 * blockIdx.x + (p.u0 == 0 && at > 0 ? 1 : 0);
-      if (p.u0 == 0 && q == 0 && quarter == 0 && lane == 0) {
+      if (p.u0 == 0 && !whole) cut = {slot, (int)((w.cur - (p.u1 - p.u0) + p.n - 1) / per), p.seg, p.kvh * pa.row_tiles + p.rt};
+      if (a.groups > 0 && p.u0 == 0 && q == 0 && quarter == 0 && lane == 0) {
         FewInfo in;
         in.first_slot = whole ? -1 : slot;
         in.first_warp = blockIdx.x;
@@ -728,10 +805,50 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       PartRows rows;
       rows.table = p.table, rows.kvh = p.kvh, rows.row0 = p.s.row0, rows.n0 = n0, rows.from = max(p.base, p.s.lo), rows.lo = p.lo, rows.hi = p.hi;
       rows.seg = p.own ? p.seg : -1;
-      rows.parts = direct ? nullptr : pa.slots + ((int64_t)slot * ROWS + q * BM + quarter * 32) * (D + kPad);
+      rows.parts = direct ? nullptr : pa.slots + ((int64_t)slot * ROWS + q0 + quarter * 32) * (D + kPad);
       unsigned anew = 0;
       if constexpr (FMT != kInt8)                         // (int8: a hidden value is 0 x a number)
-        if (partly) anew = spoiled_rows<M, FMT, D>(a, rows, t_o(q) + off, live && !bad);
+        if (partly && n > first) anew = spoiled_rows<M, FMT, D>(a, rows, t_o(q) + off, live && !bad);
+      // of outputs, to the sum's reference
+      float ref = C::BYTES ? m_run : m_run - up, down = C::BYTES ? exp2f(-up) : 1.0f, other = 0.f;
+      if constexpr (DUAL) {
+        float4* s_state = s_join + 4 * 8 * 32 + quarter * 32 + lane;
+        float4* s_cols = s_join + quarter * (8 * 32) + lane;
+        if (q == 1) {
+          // the odd tiles' rows, to the other stream
+          if (n > first) {
+            *s_state = make_float4(ref, l_run, __uint_as_float((sees ? 1u : 0u) | (anew >> lane & 1u) << 1), 0.f);
+            pair_sync(quarter);
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t r[32];
+              tmem_ld_32x32b_x32(t_o(q) + off + c * 32, r);
+              tmem_ld_wait();
+              if (c > 0) pair_sync(quarter);
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                s_cols[i * 32] = make_float4(__uint_as_float(r[4 * i]) * down, __uint_as_float(r[4 * i + 1]) * down, __uint_as_float(r[4 * i + 2]) * down,
+                                             __uint_as_float(r[4 * i + 3]) * down);
+              pair_sync(quarter);
+            }
+            pair_sync(quarter);            // before the next list's scales
+          }
+          continue;
+        }
+        if (n > 1) {
+          pair_sync(quarter);
+          const float4 st = *s_state;
+          const uint32_t flags = __float_as_uint(st.z);
+          const float top = fmaxf(ref, st.x), base = top == -INFINITY ? 0.f : top;
+          const float f0 = exp2f(ref - base);
+          other = exp2f(st.x - base);
+          l_run = l_run * f0 + st.y * other;
+          down *= f0;
+          ref = top;
+          sees = sees || (flags & 1u) != 0;
+          anew |= __ballot_sync(0xffffffffu, (flags & 2u) != 0);
+        }
+      }
       uint8_t* out = nullptr;
       // a part of a row that is finished here goes beside the groups' or own ones of the same row
       float* part = whole ? (p.own ? pa.whole_own : pa.whole_group) + ((int64_t)tok * a.hq + head) * (D + kPad) : rows.parts + lane * (D + kPad);
@@ -739,12 +856,13 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         if (direct) {
           out = reinterpret_cast<uint8_t*>(reinterpret_cast<T*>(a.out) + (int64_t)tok * a.ldo + (int64_t)head * D);
         } else {
-          *reinterpret_cast<float2*>(part + D) = make_float2(C::BYTES ? m_run : m_run - up, l_run);
+          *reinterpret_cast<float4*>(part + D) = make_float4(ref, l_run, sees ? 1.f : 0.f, 0.f);
           out = reinterpret_cast<uint8_t*>(part);
         }
       }
-      const float down = C::BYTES ? exp2f(-up) : 1.0f;    // of outputs, to the sum's reference
-      const float inv = direct ? down / l_run : down;
+      const float whole_l = direct ? 1.0f / l_run : 1.0f;
+      const float inv = down * whole_l;
+      other *= whole_l;
       // 128 bytes of each of 32 rows: staged by the rows' threads, stored by eight lanes a row
       auto store = [&](int piece, int to) {
         __syncwarp();
@@ -760,12 +878,26 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         uint32_t r[32];
         tmem_ld_32x32b_x32(t_o(q) + off + c * 32, r);
         tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * inv);
+        if (DUAL && n > 1) {
+          pair_sync(quarter);
+          const float4* s_cols = s_join + quarter * (8 * 32) + lane;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 x = s_cols[i * 32];
+            const float y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r[4 * i + e] = __float_as_uint(fmaf(y[e], other, __uint_as_float(r[4 * i + e])));
+          }
+          pair_sync(quarter);
+        }
         if (direct) {
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
             float f8[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f8[e] = sees ? __uint_as_float(r[i + e]) * inv : 0.f;
+            for (int e = 0; e < 8; ++e) f8[e] = sees ? __uint_as_float(r[i + e]) : 0.f;
             *reinterpret_cast<uint4*>(place(lane, c * 4 + i / 8)) = pack8<T>(f8);
           }
           if (c & 1) store(c >> 1, (c >> 1) * 128);
@@ -774,8 +906,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
           __syncwarp();                                   // what was staged there has been stored
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<float4*>(place(lane, piece * 8 + i / 4)) =
-                make_float4(__uint_as_float(r[i]) * inv, __uint_as_float(r[i + 1]) * inv, __uint_as_float(r[i + 2]) * inv, __uint_as_float(r[i + 3]) * inv);
+            *reinterpret_cast<uint4*>(place(lane, piece * 8 + i / 4)) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
           store(piece, c * 128);
         }
       }
@@ -795,6 +926,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       }
       __syncwarp();                                       // what was staged has been stored: the next list's queries go over it
     }
+    if (a.groups == 0 && warp == 0 && lane == 0) reinterpret_cast<Cut*>(pa.info)[blockIdx.x] = cut;
   }
 
   tcgen05_fence_before();
@@ -805,12 +937,90 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   }
 }
 
-template <typename T, int FMT, int D, int NQ>
+// Lists that blocks share, where no groups share their rows: a warp per row joins its parts as attn_pages_merge_kernel does.  A block's y-th part of the
+// grid takes every y-th eight rows of the one list that the tree kernel's block x began and did not finish, so that rows which are finished cost nothing
+// (a warp for each of them to find that out took 12 to 18 us for 8000 to 22000 rows).  Rows of sequences without a key become zero.
+constexpr int kMergeY = 16;
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(256) attn_tree_merge_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ PartArgs pa, const __grid_constant__ TreeArgs ta) {
+  constexpr int N = D / 32, VEC = N < 4 ? N : 4;          // columns of a lane, VEC neighbouring ones
+  using Vec = typename std::conditional<VEC == 4, float4, float2>::type;
+  using Out = typename std::conditional<VEC == 4, uint2, uint32_t>::type;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.hq / a.hkv, first = blockIdx.y * 8 + warp;
+  for (int s = blockIdx.x; s < a.num_seqs; s += gridDim.x) {              // lengths are not written by the kernel before
+    const SegInfo x = seg_info<ROWS>(a, ta, s);
+    if (x.units > 0 || x.rows == 0) continue;
+    for (int n = first; n < x.rows * a.hq; n += 8 * kMergeY) {
+      T* out = reinterpret_cast<T*>(a.out) + (int64_t)(x.row0 + n / a.hq) * a.ldo + (int64_t)(n % a.hq) * D;
+      for (int c = lane * 2; c < D; c += 64) *reinterpret_cast<uint32_t*>(out + c) = 0u;
+    }
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Cut cut = reinterpret_cast<const Cut*>(pa.info)[blockIdx.x];
+  if (cut.slot < 0) return;
+  const SegInfo x = seg_info<ROWS>(a, ta, cut.seg);
+  const int kvh = cut.list / ta.row_tiles, n0 = cut.list % ta.row_tiles * ROWS, rows = min(ROWS, x.rows * group - n0);
+  const int parts = cut.last - (int)blockIdx.x + 1;                       // slots: cut.slot, then the first one of each block behind this
+  const float* own = pa.slots + (int64_t)cut.slot * ROWS * (D + kPad);
+  const float* others = pa.slots + (int64_t)2 * blockIdx.x * ROWS * (D + kPad);
+  for (int n = first; n < rows; n += 8 * kMergeY) {
+    auto part = [&](int i) { return (i == 0 ? own : others + (int64_t)2 * i * ROWS * (D + kPad)) + n * (D + kPad); };
+    float o[N], m = -INFINITY, l = 0.f;
+    bool sees = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = 0.f;
+    for (int b = 0; b < parts; b += 32) {
+      const int k = min(32, parts - b);
+      float4 ml = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+      if (lane < k) ml = *reinterpret_cast<const float4*>(part(b + lane) + D);
+      sees = sees || __any_sync(0xffffffffu, ml.z != 0.f);
+      const float mn = fmaxf(m, warp_max(ml.x)), base = mn == -INFINITY ? 0.f : mn;
+      const float f = m == mn ? 1.f : exp2f(m - base), e = exp2f(ml.x - base);
+      l = l * f + warp_sum(ml.y * e);
+      m = mn;
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[i] *= f;
+      constexpr int AT_ONCE = 4;                                          // parts on their way
+      for (int j = 0; j < k; j += AT_ONCE) {
+        float w[AT_ONCE];
+        Vec v[AT_ONCE][N / VEC];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+          w[u] = j + u < k ? __shfl_sync(0xffffffffu, e, j + u) : 0.f;
+          const float* from = part(min(b + j + u, parts - 1));
+#pragma unroll
+          for (int i = 0; i < N / VEC; ++i) {
+            v[u][i] = Vec{};
+            if (w[u] != 0.f) v[u][i] = *reinterpret_cast<const Vec*>(from + i * 32 * VEC + lane * VEC);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u)
+#pragma unroll
+          for (int i = 0; i < N; ++i) o[i] = fmaf(w[u], reinterpret_cast<const float*>(&v[u][i / VEC])[i % VEC], o[i]);
+      }
+    }
+    // a row that sees nothing is zero; NaN where a score was; where all visible scores are minus infinity l is 0, and the row NaN
+    const float inv = sees ? 1.f / l : 0.f;
+    T* out = reinterpret_cast<T*>(a.out) + (int64_t)(x.row0 + (n0 + n) / group) * a.ldo + (int64_t)(kvh * group + (n0 + n) % group) * D;
+#pragma unroll
+    for (int i = 0; i < N; i += VEC) {
+      T v[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[e] = from_f32<T>(sees ? o[i + e] * inv : 0.f);
+      Out y;
+      memcpy(&y, v, sizeof(y));
+      *reinterpret_cast<Out*>(out + i * 32 + lane * VEC) = y;
+    }
+  }
+}
+
+template <typename T, int FMT, int D, int NQ, bool DUAL>
 int launch(const AttnArgs& a, const PartArgs& p, cudaStream_t stream) {
-  using C = Tree<FMT, D, NQ>;
+  using C = Tree<FMT, D, NQ, DUAL>;
   static_assert(C::SMEM <= 232448, "shared memory of a block");
   static PerDeviceSmem configured;
-  auto kern = attn_tree_kernel<T, FMT, D, NQ>;
+  auto kern = attn_tree_kernel<T, FMT, D, NQ, DUAL>;
   LLMSS_CHECK_CUDA(configured.ensure(kern, C::SMEM));
   TreeArgs ta;
   ta.own = a.num_seqs;
@@ -827,14 +1037,26 @@ int launch(const AttnArgs& a, const PartArgs& p, cudaStream_t stream) {
     if (int e = encode_pages(&map_v, a.v, rows, D * 2, ta.run)) return e;
   }
   LLMSS_CHECK_CUDA(launch_pdl(kern, dim3(kTreeBlocks), dim3(C::THREADS), (size_t)C::SMEM, stream, map_k, map_v, a, p, ta));
+  if (a.groups > 0) return 0;              // attn_pages_merge_kernel joins own and shared parts
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(kTreeBlocks, kMergeY);
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  LLMSS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attn_tree_merge_kernel<T, D, C::ROWS>, a, p, ta));
   return 0;
 }
 
 template <typename T, int FMT>
 int by_size(const AttnArgs& a, const PartArgs& p, cudaStream_t stream) {
-  if (a.d == 256) return launch<T, FMT, 256, 1>(a, p, stream);
-  if (a.d == 128) return p.rows == 256 ? launch<T, FMT, 128, 2>(a, p, stream) : launch<T, FMT, 128, 1>(a, p, stream);
-  return p.rows == 256 ? launch<T, FMT, 64, 2>(a, p, stream) : launch<T, FMT, 64, 1>(a, p, stream);
+  if (a.d == 256) return launch<T, FMT, 256, 1, false>(a, p, stream);
+  if (a.d == 128) return p.rows == 256 ? launch<T, FMT, 128, 2, false>(a, p, stream) : launch<T, FMT, 128, 2, true>(a, p, stream);
+  return p.rows == 256 ? launch<T, FMT, 64, 2, false>(a, p, stream) : launch<T, FMT, 64, 2, true>(a, p, stream);
 }
 
 }  // namespace

@@ -119,6 +119,30 @@ def test_rows_of_a_tree_see_their_ancestors(case, hq, hkv, d, kind, dtype, shape
     assert not ((less - want).abs() <= tol).all()
 
 
+# the card full of lists: many tiles of keys one after another for every block, of lists that end and begin in its run
+FULL = {
+    "up_to_128_rows": ([30, 12, 7, 25] * 6, [2100, 3900, 64, 1000] * 6),
+    "up_to_256_rows": ([60, 33, 7, 40] * 6, [2100, 3900, 64, 1000] * 6),
+    "short_lists": ([9, 30, 5] * 20, [0, 40, 130] * 20),
+}
+
+
+@pytest.mark.parametrize("kind,dtype", [(None, BF), (I8, BF), (E4, HF)])
+@pytest.mark.parametrize("hq,hkv,d", [(16, 4, 64), (32, 8, 128), (16, 4, 256), (12, 1, 128)])
+@pytest.mark.parametrize("case", sorted(FULL))
+def test_runs_of_many_tiles(case, hq, hkv, d, kind, dtype):
+    new, ctx = FULL[case]
+    batch, seen = make_batch(new, ctx, 64, [], "cuda", seed=4)
+    rng = random.Random(len(case))
+    set_masks(batch, seen, [s for n in new for s in ancestors(random_parents(n, rng))])
+    q = queries(sum(new), hq * d, dtype)
+    k, v = (make_pages(seen.blocks, hkv, 64, d, kind, dtype, "cuda", seed=i) for i in range(2))
+    want, tol, _ = expected(q, k, v, batch, seen, hq, hkv, d, d ** -0.5)
+    for _ in range(3):
+        out = ops.attention(q, torch.full_like(q, NAN), batch, k, v, hq, hkv, d, d ** -0.5, 0, 0, 0)
+        assert ((out.double() - want).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("kind", [None, I8])
 @pytest.mark.parametrize("hq,hkv,d", [(4, 4, 64), (8, 2, 128), (4, 4, 256), (6, 3, 96)])
 @pytest.mark.parametrize("case", sorted(TREES))
