@@ -17,6 +17,7 @@ from time import time
 
 import torch
 
+from llmss_b200.engine.drafts import PromptLookup
 from llmss_b200.engine.engine import Engine
 from llmss_b200.engine.runner import SamplingParams
 from llmss_b200.parallel.comm import comm_for
@@ -42,6 +43,9 @@ def get_args(argv=None):
                         help="keep generating past the model's context over the most recent tokens (rotary-position models)")
     parser.add_argument("--kv_cache_dtype", type=str, default=None, choices=["int8", "fp8"],
                         help="keep the KV cache in 8 bits (models with multi-head keys and values)")
+    parser.add_argument("--draft_tokens", type=int, default=0,
+                        help="check up to this many guesses per sequence and step, taken from where the last tokens stood before (with --use_cache; "
+                             "models with multi-head keys and values)")
     return parser.parse_args(argv)
 
 
@@ -68,7 +72,8 @@ def main(argv=None):
 
     engine = Engine.from_pretrained(args.pretrained_model_path, dtype=getattr(torch, args.dtype), device=device,
                                     process_group=process_group, max_batch=max(1, len(args.prompts or args.prompt_ids)),
-                                    eos_token_id=None, sliding_window=args.sliding_window, kv_cache_dtype=args.kv_cache_dtype)
+                                    eos_token_id=None, sliding_window=args.sliding_window, kv_cache_dtype=args.kv_cache_dtype,
+                                    drafter=PromptLookup(size=args.draft_tokens) if args.draft_tokens else None)
     max_len = engine.runner.max_seq_len
 
     # rank 0 tokenises; ids are shared with one broadcast (reference N5, generate.py:73-85)

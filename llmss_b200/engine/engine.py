@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import time
 from dataclasses import dataclass, field
-from typing import Dict, List, Optional, Sequence
+from typing import Callable, Dict, List, Optional, Sequence
 
 import torch
 
@@ -57,7 +57,11 @@ class Engine:
                  num_blocks: Optional[int] = None, use_cuda_graph: Optional[bool] = None,
                  max_prefill_tokens: int = 16384, eos_token_id: Optional[int] = None,
                  prefill_chunk: Optional[int] = None, sliding_window: bool = False, prefix_cache: bool = False,
-                 pool_tokens: Optional[int] = None, kv_cache_dtype: Optional[str] = None, shared_prefix: bool = False):
+                 pool_tokens: Optional[int] = None, kv_cache_dtype: Optional[str] = None, shared_prefix: bool = False,
+                 drafter: Optional[Callable] = None):
+        """``drafter``: called with a running sequence's tokens before each decode step, returns guesses for what follows as (tokens, parents), e.g.
+        ``engine.drafts.PromptLookup()``.  A step checks them all at once and a sequence gains as many tokens as were guessed right and one; the
+        tokens are those that one step per token gives, to the rounding of its products."""
         self.model = model
         self.core = model.core if hasattr(model, "core") else model
         self.comm = self.core.comm
@@ -65,6 +69,9 @@ class Engine:
                                   num_blocks=num_blocks, use_cuda_graph=use_cuda_graph, prefill_chunk=prefill_chunk,
                                   sliding_window=sliding_window, prefix_cache=prefix_cache, pool_tokens=pool_tokens,
                                   kv_cache_dtype=kv_cache_dtype, shared_prefix=shared_prefix)
+        if drafter is not None and (self.runner.sliding or not hasattr(self.runner.kv, "row_tensors")):
+            raise ValueError("drafter: needs a model with multi-head K / V pages and no sliding window")
+        self.drafter = drafter
         self.max_batch = max_batch
         self.max_prefill_tokens = max_prefill_tokens
         self.eos_token_id = eos_token_id
@@ -227,6 +234,11 @@ class Engine:
             return outs
         if not self.running:
             return outs
+        if self.drafter is not None:
+            self.running = [s for s in self.running if not s.finished]
+            drafts = [self.drafter(s.prompt + s.output) for s in self.running]
+            if any(len(tokens) for tokens, _ in drafts):
+                return outs + self._draft_step(drafts)
         if self._dirty:
             self.running = self.runner.by_prefix([s for s in self.running if not s.finished])
             self.runner.set_batch(self.running)
@@ -255,6 +267,25 @@ class Engine:
                 METRICS.observe("tpot_seconds", st.tpot or 0.0)
                 self._finish(s)
         METRICS.inc("decode_tokens", n_active)
+        return outs
+
+    def _draft_step(self, drafts) -> List[StepOutput]:
+        t0 = time.perf_counter()
+        got = self.runner.check_drafts(self.running, drafts)
+        t1 = time.perf_counter()
+        METRICS.observe("decode_step_seconds", t1 - t0)
+        METRICS.set("batch_occupancy", len(self.running))
+        outs: List[StepOutput] = []
+        for s, tokens in zip(self.running, got):
+            st = self.stats[s.seq_id]
+            st.last_token, st.n_out = t1, st.n_out + len(tokens)
+            done = self._is_done(s, tokens[-1])
+            outs += [StepOutput(s.seq_id, t, done and i + 1 == len(tokens)) for i, t in enumerate(tokens)]
+            if done:
+                METRICS.observe("tpot_seconds", st.tpot or 0.0)
+                self._finish(s)
+        self._dirty = True                      # a step of single tokens behind this one binds its rows anew
+        METRICS.inc("decode_tokens", sum(len(t) for t in got))
         return outs
 
     # ------------------------------------------------------------------ convenience

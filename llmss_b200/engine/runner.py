@@ -327,6 +327,64 @@ class ModelRunner:
             s.length += len(toks)
         return logits[:, :self.spec.vocab]
 
+    @torch.no_grad()
+    def check_drafts(self, seqs: Sequence[SeqState], drafts: Sequence[tuple]) -> List[List[int]]:
+        """One step over trees of guesses.  ``drafts[i]`` = (tokens, parents) are guesses for what ``seqs[i]`` goes on with: a guess's parent is its place
+        among them, -1 for those right behind the last token; parents come first.  Returns the tokens that each sequence gains, one at least: what is drawn
+        at its last token, at the guess which that is, and so on until no guess is what was drawn.  Draws are numbered by the place they are for, so these
+        are the tokens that one step per token would have given.  Guesses that the cache has no room for are left out, the last ones first.
+
+        Tokens behind an end-of-sequence token, ``max_new_tokens`` or ``max_seq_len`` are dropped."""
+        if not isinstance(self.core, DecoderLM) or self.sliding:
+            raise ValueError("check_drafts: needs a model with multi-head K / V pages and no sliding window")
+        if len(drafts) != len(seqs):
+            raise ValueError(f"check_drafts: {len(drafts)} trees for {len(seqs)} sequences")
+        bs, spare = self.block_size, self.alloc.num_free - self._outstanding
+        token_lists, trees, depths = [], [], []
+        for s, (tokens, up) in zip(seqs, drafts):
+            if len(tokens) != len(up) or any(not -1 <= p < j for j, p in enumerate(up)):
+                raise ValueError(f"check_drafts: a parent for each guess, in front of it, got {len(tokens)} guesses and parents {list(up)}")
+            if any(not 0 <= t < self.spec.vocab for t in tokens):
+                raise ValueError(f"check_drafts: guesses are tokens below {self.spec.vocab}")
+            if not s.output or s.length + 1 > self.max_seq_len:
+                raise ValueError(f"check_drafts: sequence {s.seq_id} has no token to go on from, or no place for it")
+            # what was promised at admission, and what nobody was promised
+            room = min((len(s.blocks) + s.reserved + max(spare, 0)) * bs, self.max_seq_len) - s.length
+            n = max(1, min(1 + len(tokens), room, ops.MAX_TREE))
+            spare -= max(0, self.blocks_needed(s.length + n) - len(s.blocks) - s.reserved)
+            self._grow(s, s.length + n)
+            token_lists.append([s.output[-1]] + list(tokens[:n - 1]))
+            trees.append([-1] + [p + 1 for p in up[:n - 1]])
+            depth = [0]
+            for p in up[:n - 1]:
+                depth.append(depth[p + 1] + 1)
+            depths.append(depth)
+        batch = BatchInput.build(token_lists, [s.length for s in seqs], [s.blocks for s in seqs], bs, self.device, max_blocks=self.max_blocks_per_seq,
+                                 pad_to=self.core.tp * 16 if self.core.tp > 1 else 1, parents=trees)
+        logits = self.core.forward(batch, self.kv, last_only=False)
+        rows, dev = batch.tokens.numel(), self.device
+        pad = rows - sum(len(d) for d in depths)
+        ints = [[int(s.params.is_greedy), s.params.top_k, request_seed(s.params, s.seq_id), len(s.output) + x] for s, d in zip(seqs, depths) for x in d]
+        floats = [[s.params.temperature, s.params.top_p] for s, d in zip(seqs, depths) for _ in d]
+        ints = torch.tensor(ints + [[1, 0, 0, 0]] * pad, dtype=torch.int32).t().contiguous().to(dev)
+        floats = torch.tensor(floats + [[1.0, 1.0]] * pad, dtype=torch.float32).t().contiguous().to(dev)
+        rng = ints[2:].t().contiguous()
+        sampled = ops.sample(logits, ints[0], floats[0], ints[1], floats[1], rng, vocab=self.spec.vocab)
+        got = ops.accept_drafts(sampled, batch, self.kv.row_tensors())
+        counts, tokens = got.counts.tolist(), got.tokens.tolist()
+        out = []
+        for s, c, row in zip(seqs, counts, tokens):
+            new = row[:max(1, min(c, s.params.max_new_tokens - len(s.output), self.max_seq_len - s.length - 1))]
+            if s.eos is not None and s.eos in new:
+                new = new[:new.index(s.eos) + 1]
+            s.output += new
+            s.length += len(new)
+            out.append(new)
+        self.stats["draft_steps"] = self.stats.get("draft_steps", 0) + 1
+        METRICS.inc("drafted_tokens", sum(len(d) - 1 for d in depths))
+        METRICS.inc("accepted_drafts", sum(len(x) - 1 for x in out))
+        return out
+
     # ------------------------------------------------------------------ prefill
     @torch.no_grad()
     def prefill(self, seqs: Sequence[SeqState], rng_steps: Optional[Sequence[int]] = None) -> List[int]:

@@ -15,7 +15,7 @@ import torch
 
 from . import cuda_impl as cu
 from . import reference as ref
-from .drafts import Accepted, StepLayout
+from .drafts import MAX_TREE, Accepted, StepLayout
 from .pages import QuantPages
 from .reference import (DECAY_HEAD, DECAY_TOKEN_CHANNEL, DECAY_TOKEN_HEAD, GATE_NONE, GATE_SIGMOID, GATE_SILU, UNARY_NEG_EXP,
                         UNARY_TANH, distance_bias_table, rotary_frequencies, window_bias_table)

@@ -1,0 +1,117 @@
+"""Engines that check drafted tokens, on the CPU: the same tokens as one step per token, whatever is guessed."""
+import random
+
+import pytest
+import torch
+
+from llmss_b200.engine.drafts import PromptLookup
+from llmss_b200.engine.engine import Engine
+from llmss_b200.engine.runner import SamplingParams
+from tiny import make_tiny
+
+GREEDY = dict(is_greedy=True)
+DRAWN = dict(is_greedy=False, temperature=0.8, top_p=0.9, top_k=20, seed=5)
+
+
+class Guesser:
+    """Trees around a known continuation: parts of it, mistakes, the same token twice, now and then nothing."""
+
+    def __init__(self, known, seed):
+        self.known, self.rng, self.steps = known, random.Random(seed), 0
+
+    def __call__(self, tokens):
+        self.steps += 1
+        rng, at = self.rng, None
+        for prompt, out in self.known:
+            n = len(tokens) - len(prompt)
+            if tokens[:len(prompt)] == prompt and n >= 0 and out[:n] == tokens[len(prompt):]:
+                at = out[n:]
+        if at is None or rng.random() < 0.2:
+            return [], []
+        guesses, parents, trunk = [], [], -1
+        for t in at[:rng.randrange(0, 6)]:
+            for _ in range(rng.randrange(0, 3)):
+                guesses.append(rng.choice([t, rng.randrange(100)]))
+                parents.append(rng.choice([trunk, rng.randrange(-1, len(guesses) - 1)]))
+            guesses.append(t if rng.random() < 0.9 else rng.randrange(100))
+            parents.append(trunk)
+            trunk = len(guesses) - 1
+        return guesses, parents
+
+
+def prompts_of(cfg, lengths=(9, 17, 3, 30, 12)):
+    return [torch.randint(0, 100, (n,), generator=torch.Generator().manual_seed(n)).tolist() for n in lengths]
+
+
+@pytest.mark.parametrize("family", ["gptj", "llama", "gpt_bigcode", "opt"])
+@pytest.mark.parametrize("how", [GREEDY, DRAWN], ids=["greedy", "drawn"])
+@pytest.mark.parametrize("kw", [{}, dict(kv_cache_dtype="int8"), dict(prefix_cache=True)], ids=["plain", "int8", "prefix"])
+def test_the_same_tokens_as_one_step_per_token(tmp_path, family, how, kw):
+    cfg, _ = make_tiny(family, tmp_path)
+    prompts = prompts_of(cfg)
+    params = [SamplingParams(max_new_tokens=m, **how) for m in (14, 20, 9, 25, 1)]
+    make = lambda **more: Engine.from_pretrained(str(tmp_path), dtype=torch.float32, device="cpu", max_batch=3, max_seq_len=64, block_size=8, **kw, **more)
+    want = make().generate(prompts, params)
+    drafter = Guesser(list(zip(prompts, want)), 3)
+    eng = make(drafter=drafter)
+    assert eng.generate(prompts, params) == want
+    assert drafter.steps < sum(len(w) - 1 for w in want)               # fewer steps than tokens
+    assert eng.runner.alloc.num_free == eng.runner.alloc.num_blocks - 1 and eng.runner._outstanding == 0
+    again = make(drafter=PromptLookup(size=5))
+    assert again.generate(prompts, params) == want
+
+
+def test_guesses_end_with_the_sequence(tmp_path):
+    """max_seq_len, an end-of-sequence token inside of a path, a cache without a block to spare."""
+    cfg, _ = make_tiny("llama", tmp_path)
+    prompt = prompts_of(cfg, (20,))[0]
+    plain = Engine.from_pretrained(str(tmp_path), dtype=torch.float32, device="cpu", max_batch=2, max_seq_len=40, block_size=4)
+    want = plain.generate([prompt], SamplingParams(max_new_tokens=60, **GREEDY))[0]
+    assert len(want) == 20
+    oracle = lambda out: lambda tokens: ((out + [1, 2, 3])[len(tokens) - 20:][:10], list(range(-1, len((out + [1, 2, 3])[len(tokens) - 20:][:10]) - 1)))
+    make = lambda **kw: Engine.from_pretrained(str(tmp_path), dtype=torch.float32, device="cpu", max_batch=2, max_seq_len=40, block_size=4, **kw)
+    assert make(drafter=oracle(want)).generate([prompt], SamplingParams(max_new_tokens=60, **GREEDY))[0] == want
+    tight = make(drafter=oracle(want), num_blocks=1 + 7)                # 20 + 8 tokens and nothing else
+    assert tight.generate([prompt], SamplingParams(max_new_tokens=8, **GREEDY))[0] == want[:8]
+    eos = next(t for i, t in enumerate(want[3:9]) if t not in want[:3 + i])
+    cut = want[:want.index(eos) + 1]
+    assert make(drafter=oracle(want), eos_token_id=eos).generate([prompt], SamplingParams(max_new_tokens=30, **GREEDY))[0] == cut
+
+
+def test_outputs_of_a_step_come_token_by_token(tmp_path):
+    cfg, _ = make_tiny("gptj", tmp_path)
+    prompt = prompts_of(cfg, (9,))[0]
+    make = lambda **kw: Engine.from_pretrained(str(tmp_path), dtype=torch.float32, device="cpu", max_batch=2, max_seq_len=64, **kw)
+    want = make().generate([prompt], SamplingParams(max_new_tokens=7, **GREEDY))[0]
+    eng = make(drafter=lambda tokens: (want[len(tokens) - 9:], list(range(-1, len(want) - (len(tokens) - 9) - 1))))
+    rid = eng.add_request(prompt, SamplingParams(max_new_tokens=7, **GREEDY))
+    first, second = eng.step(), eng.step()
+    assert [o.token for o in first] == want[:1] and [o.token for o in second] == want[1:]
+    assert [o.finished for o in second] == [False] * 5 + [True] and all(o.request_id == rid for o in second)
+    assert not eng.has_work() or not [s for s in eng.running if not s.finished]
+
+
+def test_prompt_lookup():
+    look = PromptLookup(size=5, length=3, branches=2, match=2)
+    assert look([7]) == ([], []) and look([1, 2, 3]) == ([], [])
+    # "5 6" stood at 0 (then 1 2 3) and at 5 (then 1 9 9); the later one comes first, the common beginning once
+    assert look([5, 6, 1, 2, 3, 5, 6, 1, 9, 9, 5, 6]) == ([1, 9, 9, 2, 3], [-1, 0, 1, 0, 3])
+    assert look([4, 8, 4]) == ([8, 4], [-1, 0])
+    assert PromptLookup(size=2, window=4)([9, 9, 9, 9, 1, 2, 1]) == ([2, 1], [-1, 0])
+    with pytest.raises(ValueError):
+        PromptLookup(size=0)
+
+
+def test_refusals(tmp_path):
+    make_tiny("gptj", tmp_path)
+    make = lambda **kw: Engine.from_pretrained(str(tmp_path), dtype=torch.float32, device="cpu", max_batch=2, max_seq_len=64, **kw)
+    with pytest.raises(ValueError, match="drafter"):
+        make(drafter=PromptLookup(), sliding_window=True)
+    eng = make()
+    eng.add_request([1, 2, 3], SamplingParams(max_new_tokens=9, **GREEDY))
+    eng.step()
+    s = eng.running[0]
+    for bad in ([([1, 2], [-1])], [([1, 2], [-1, 1])], [([1], [-2])], [([1000], [-1])], [([-1], [-1])], []):
+        with pytest.raises(ValueError, match="check_drafts"):
+            eng.runner.check_drafts([s], bad)
+    assert len(eng.runner.check_drafts([s], [([], [])])[0]) == 1

@@ -1,0 +1,138 @@
+"""Steps that check drafted tokens, as a program runs them on the GPU: an engine's, and a captured one whose lengths stay on the device."""
+import random
+
+import pytest
+import torch
+
+from drafts_oracle import random_parents
+from llmss_b200 import ops
+from llmss_b200.engine.batch import BatchInput, DraftTree
+from llmss_b200.engine.drafts import PromptLookup
+from llmss_b200.engine.engine import Engine
+from llmss_b200.engine.runner import SamplingParams, SeqState
+from test_draft_steps_cpu import GREEDY, Guesser, prompts_of
+from tiny import make_tiny
+
+pytestmark = pytest.mark.gpu
+
+
+def held_to_the_model(eng, prompts, outputs, step):
+    """Every token is the best one of a teacher-forced pass, or as good: roundings of ``step`` (half a step of the type) in some twenty places on the way
+    to a logit add up to less than 32 of them, in both passes."""
+    for p, out in zip(prompts, outputs):
+        s = SeqState(10 ** 6, [], SamplingParams(), eos=None)
+        logits = eng.runner.forward_tokens([s], [p + out[:-1]], [list(range(len(p) - 1, len(p) + len(out) - 1))]).float()
+        eng.runner.release(s)
+        got = logits.gather(1, torch.tensor(out, device=logits.device)[:, None])[:, 0]
+        assert (logits.amax(1) - got <= 64 * step * logits.abs().amax(1)).all()
+
+
+@pytest.mark.parametrize("family", ["gptj", "llama", "gpt_bigcode", "opt"])
+@pytest.mark.parametrize("kw", [{}, dict(kv_cache_dtype="fp8"), dict(prefix_cache=True)], ids=["plain", "fp8", "prefix"])
+def test_an_engine_that_checks_guesses(tmp_path, family, kw):
+    cfg, _ = make_tiny(family, tmp_path, hidden=256)
+    prompts = prompts_of(cfg)
+    params = [SamplingParams(max_new_tokens=m, **GREEDY) for m in (14, 20, 9, 25, 1)]
+    make = lambda **more: Engine.from_pretrained(str(tmp_path), dtype=torch.float16, device="cuda", max_batch=3, max_seq_len=64, block_size=16, **kw, **more)
+    plain = make()
+    known = plain.generate(prompts, params)
+    drafter = Guesser(list(zip(prompts, known)), 3)
+    eng = make(drafter=drafter)
+    got = eng.generate(prompts, params)
+    assert [len(x) for x in got] == [len(x) for x in known] and drafter.steps < sum(len(w) - 1 for w in known)
+    if "kv_cache_dtype" not in kw:
+        held_to_the_model(plain, prompts, got, 2.0 ** -11)
+    assert eng.runner.alloc.num_free == eng.runner.alloc.num_blocks - 1 and eng.runner._outstanding == 0
+    looked = make(drafter=PromptLookup()).generate(prompts, params)
+    assert [len(x) for x in looked] == [len(x) for x in known]
+
+
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("nodes", [[6, 1, 4], [40, 33, 5]])
+def test_a_captured_step_with_lengths_on_the_device(nodes, quantised):
+    """Layout, write, attention and acceptance in one graph; what a step accepted is where the next one begins."""
+    hq, hkv, d, page, B, steps = 4, 2, 64, 16, 3, 5
+    rng, gen = random.Random(1), torch.Generator().manual_seed(1)
+    blocks, T, width = 200, sum(nodes), 40
+    dt = torch.bfloat16
+    tables = torch.tensor(rng.sample(range(1, blocks), B * width), dtype=torch.int32).view(B, width).cuda()
+    parents = torch.tensor([p for n in nodes for p in random_parents(n, rng)], dtype=torch.int32).cuda()
+    new = torch.tensor(nodes, dtype=torch.int32).cuda()
+    qkv_of = [torch.randn(T, (hq + 2 * hkv) * d, generator=gen).to(dt).cuda() for _ in range(steps)]
+    tokens_of = [torch.randint(0, 2, (T,), generator=gen, dtype=torch.int32).cuda() for _ in range(steps)]
+    sampled_of = [torch.randint(0, 2, (T,), generator=gen, dtype=torch.int32).cuda() for _ in range(steps)]
+
+    def state():
+        data = torch.zeros(1, 2, blocks, hkv, page, d, dtype=torch.int8 if quantised else dt, device="cuda")
+        scale = torch.zeros(1, 2, blocks, hkv, page, device="cuda")
+        s = {"context": torch.tensor([20, 0, 33], dtype=torch.int32).cuda(), "data": data, "scale": scale, "qkv": torch.empty_like(qkv_of[0]),
+             "tokens": torch.empty_like(tokens_of[0]), "sampled": torch.empty_like(sampled_of[0])}
+        s["pages"] = [data, scale] if quantised else [data]
+        s["kv"] = [ops.QuantPages(data[0, i], scale[0, i]) if quantised else data[0, i] for i in range(2)]
+        return s
+
+    def step(s):
+        at = ops.step_layout(s["context"], new, tables, page, T, max(nodes), parents=parents)
+        ops.rope_kv_write(s["qkv"], at.positions, at.slot_mapping, *s["kv"], hq, hkv, d, d, ops.ROPE_NEOX, 10000.0, 0, hq * d, (hq + hkv) * d)
+        batch = BatchInput(tokens=s["tokens"], positions=at.positions, slot_mapping=at.slot_mapping, block_tables=at.block_tables, seq_lens=at.seq_lens,
+                           cu_q=at.cu_q, last_idx=at.last_idx, num_seqs=B, max_q=max(nodes), max_kv=width * page, is_decode=False, is_fresh_prefill=False,
+                           tree=DraftTree(parents=parents, masks=at.masks))
+        out = torch.zeros(T, hq * d, dtype=dt, device="cuda")
+        ops.attention(s["qkv"], out, batch, *s["kv"], hq, hkv, d, d ** -0.5, 0, 0, 0)
+        got = ops.accept_drafts(s["sampled"], batch, s["pages"])
+        s["context"].copy_(got.context_lens)
+        return out, got
+
+    def feed(s, i):
+        s["qkv"].copy_(qkv_of[i])
+        s["tokens"].copy_(tokens_of[i])
+        s["sampled"].copy_(sampled_of[i])
+
+    eager, captured = state(), state()
+    feed(captured, 0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(captured)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, got = step(captured)
+    for n, x in state().items():
+        if torch.is_tensor(x):
+            captured[n].copy_(x)
+    gained = 0
+    for i in range(steps):
+        feed(eager, i)
+        feed(captured, i)
+        want_out, want = step(eager)
+        graph.replay()
+        assert torch.equal(out, want_out) and all(torch.equal(a, b) for a, b in zip(got, want))
+        assert torch.equal(captured["data"], eager["data"]) and torch.equal(captured["scale"], eager["scale"])
+        gained += int(want.counts.sum())
+    assert eager["context"].tolist() != [20, 0, 33] and int(eager["context"].sum()) == 53 + gained
+
+
+def test_calls_on_two_streams_at_once():
+    """Each call has a scratch of its own."""
+    from drafts_oracle import ancestors, expected, set_masks
+    from pages_oracle import make_batch, make_pages
+
+    cases = []
+    for i, (new, hq, hkv, d, kind) in enumerate([([30] * 20, 16, 2, 128, None), ([9] * 30, 8, 2, 64, torch.int8)]):
+        batch, seen = make_batch(new, [900 + 37 * j for j in range(len(new))], 16, [], "cuda", seed=i)
+        rng = random.Random(i)
+        set_masks(batch, seen, [s for n in new for s in ancestors(random_parents(n, rng))])
+        k, v = (make_pages(seen.blocks, hkv, 16, d, kind, torch.bfloat16, "cuda", seed=j) for j in range(2))
+        q = torch.randn(sum(new), hq * d, generator=torch.Generator().manual_seed(i)).bfloat16().cuda()
+        want, tol, _ = expected(q, k, v, batch, seen, hq, hkv, d, d ** -0.5)
+        cases.append((q, k, v, batch, hq, hkv, d, want, tol, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(10):
+        for q, k, v, batch, hq, hkv, d, want, tol, stream in cases:
+            with torch.cuda.stream(stream):
+                outs.append((ops.attention(q, torch.empty_like(q), batch, k, v, hq, hkv, d, d ** -0.5, 0, 0, 0), want, tol))
+    torch.cuda.synchronize()
+    for out, want, tol in outs:
+        assert ((out.double() - want).abs() <= tol).all()
