@@ -122,18 +122,17 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   return d;
 }
 
-// 2^x of two numbers without the MUFU pipe (exp2_cubic, in pairs); 0 for what is below -127 (hidden keys weigh nothing, however large their values), and for NaN
-__device__ __forceinline__ void exp2_pair(float& y0, float& y1, float x0, float x1) {
-  using namespace packed;
-  const pair_t x = pack(fmaxf(x0, -127.0f), fmaxf(x1, -127.0f)), magic = both(12582912.0f);
-  const pair_t t = padd(x, magic), r = psub(x, psub(t, magic));
-  pair_t p = pfma(r, both(0.05459282f), both(0.24221784f));
-  p = pfma(r, p, both(0.6933686f));
-  p = pfma(r, p, both(1.0f));
-  const float2 tf = unpack(t), pf = unpack(p);
-  y0 = __int_as_float(__float_as_int(pf.x) + (__float_as_int(tf.x) << 23));     // (what the 1.5 2^23 of t holds besides x leaves the word)
-  y1 = __int_as_float(__float_as_int(pf.y) + (__float_as_int(tf.y) << 23));
+// 2^x without the MUFU pipe (exp2_cubic with the exponent added by a multiplication); 0 for what is below -127 (hidden keys weigh nothing, however large their
+// values), and for NaN
+__device__ __forceinline__ float exp2_fma(float x) {
+  x = fmaxf(x, -127.0f);
+  const float t = x + 12582912.0f, r = x - (t - 12582912.0f);
+  float p = fmaf(r, 0.05459282f, 0.24221784f);
+  p = fmaf(r, p, 0.6933686f);
+  p = fmaf(r, p, 1.0f);
+  return __int_as_float(__float_as_int(t) * (1 << 23) + __float_as_int(p));     // (what the 1.5 2^23 of t holds besides x leaves the word)
 }
+
 // warps `quarter` of both streams
 __device__ __forceinline__ void pair_sync(int quarter) { asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory"); }
 
@@ -172,7 +171,8 @@ struct Walk {
 // rows n0 + lane of a part, for what looks at them once more
 struct PartRows {
   const int* table;
-  float* parts;           // of row n0 on; null: the result itself
+  float* parts;           // of row n0: numbers 4 i .. 4 i + 3 of row r at parts + r rs + i cs; null: the result itself
+  int rs, cs;
   int kvh, row0, n0, from, lo, hi, seg;      // seg: of own lists, else -1
 };
 __device__ __forceinline__ TreeKeys keys_of(const AttnArgs& a, const PartRows& p, int n, int& tok, int& head) {
@@ -209,11 +209,27 @@ __device__ __noinline__ unsigned spoiled_rows(const AttnArgs& a, const PartRows&
 }
 template <typename T, typename M, int FMT, int D>
 __device__ __noinline__ void rows_anew(const AttnArgs& a, const PartRows& p, unsigned rows) {
+  const int lane = threadIdx.x & 31;
   __syncwarp();                                          // behind the rows as they were
   for (; rows != 0; rows &= rows - 1) {
     int tok, head;
-    const TreeKeys k = keys_of(a, p, p.n0 + __ffs(rows) - 1, tok, head);
-    row_anew<T, M, FMT, true>(a, k, tok, head, p.parts == nullptr ? nullptr : p.parts + (__ffs(rows) - 1) * (D + kPad));
+    const int row = __ffs(rows) - 1;
+    const TreeKeys k = keys_of(a, p, p.n0 + row, tok, head);
+    if (p.parts == nullptr) {
+      row_anew<T, M, FMT, true>(a, k, tok, head, nullptr);
+      continue;
+    }
+    float o[8], m, l;
+    bool sees = false;
+    row_softmax<T, M, FMT, true>(a, tok, head, k.first, 1, k.to + 1, [&](int key) {
+      if (key > k.last && (tree_bits(a, tok, key - k.ctx) & 1u) == 0) return (int64_t)-1;
+      sees = true;
+      return cache_row(a, k, key);
+    }, o, m, l);
+    float* part = p.parts + row * p.rs;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) part[(int64_t)((lane + 32 * i) >> 2) * p.cs + (lane & 3)] = o[i];
+    if (lane == 0) *reinterpret_cast<float4*>(part + (int64_t)(D / 4) * p.cs) = make_float4(m, l, sees ? 1.f : 0.f, 0.f);
   }
 }
 
@@ -741,11 +757,9 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             const float* s4 = sc + c * 32 + i;
             ffma2(e[0], e[1], s4[0], s4[1], scale, scale, neg, neg);
             ffma2(e[2], e[3], s4[2], s4[3], scale, scale, neg, neg);
-            // half of the exponentials on the FMA pipe: the MUFU pipe alone needs 1024 clocks for 256 rows of a tile.  A quarter where scales are applied
-            // and warps convert: there instructions are short as well
-            x[0] = exp2_fast(e[0]), x[1] = exp2_fast(e[1]);
-            if (C::BYTES && (i & 4)) x[2] = exp2_fast(e[2]), x[3] = exp2_fast(e[3]);
-            else exp2_pair(x[2], x[3], e[2], e[3]);
+            // An exponential of the MUFU pipe takes 8 clocks, one on the FMA pipe 12 of what everything else needs too: every fourth there (half of them:
+            // 6 trees of 40 tokens over 24000 4 % slower), and none where scales are applied and warps convert
+            x[0] = exp2_fast(e[0]), x[1] = exp2_fast(e[1]), x[2] = exp2_fast(e[2]), x[3] = C::BYTES ? exp2_fast(e[3]) : exp2_fma(e[3]);
             fadd2(la[(i >> 1) & 3], lb[(i >> 1) & 3], la[(i >> 1) & 3], lb[(i >> 1) & 3], x[0], x[1]);
             fadd2(la[(i >> 1 & 3) + 1], lb[(i >> 1 & 3) + 1], la[(i >> 1 & 3) + 1], lb[(i >> 1 & 3) + 1], x[2], x[3]);
             if constexpr (C::BYTES) {
@@ -789,7 +803,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         tcgen05_fence_after();
       }
 
-      // ---- the list's result, or its part.  Rows go through shared memory, where this warp's queries were, and from there by the whole warp
+      // ---- the list's result, through shared memory where this warp's queries were, or its part
       if (bad) l_run = __int_as_float(0x7fc00000);
       const bool whole = p.u0 == 0 && p.u1 == p.n, direct = whole && a.groups == 0;
       const int slot = 2 * blockIdx.x + (p.u0 == 0 && at > 0 ? 1 : 0);
@@ -805,7 +819,11 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       PartRows rows;
       rows.table = p.table, rows.kvh = p.kvh, rows.row0 = p.s.row0, rows.n0 = n0, rows.from = max(p.base, p.s.lo), rows.lo = p.lo, rows.hi = p.hi;
       rows.seg = p.own ? p.seg : -1;
-      rows.parts = direct ? nullptr : pa.slots + ((int64_t)slot * ROWS + q0 + quarter * 32) * (D + kPad);
+      // parts lie with the same numbers of all rows beside one another, so that a row's thread stores them as they are; by rows where the general merge
+      // joins them with a group's
+      const bool compact = a.groups == 0;
+      rows.rs = compact ? 4 : D + kPad, rows.cs = compact ? ROWS * 4 : 4;
+      rows.parts = direct ? nullptr : pa.slots + (int64_t)slot * ROWS * (D + kPad) + (q0 + quarter * 32) * rows.rs;
       unsigned anew = 0;
       if constexpr (FMT != kInt8)                         // (int8: a hidden value is 0 x a number)
         if (partly && n > first) anew = spoiled_rows<M, FMT, D>(a, rows, t_o(q) + off, live && !bad);
@@ -851,19 +869,18 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       }
       uint8_t* out = nullptr;
       // a part of a row that is finished here goes beside the groups' or own ones of the same row
-      float* part = whole ? (p.own ? pa.whole_own : pa.whole_group) + ((int64_t)tok * a.hq + head) * (D + kPad) : rows.parts + lane * (D + kPad);
+      float* part = whole ? (p.own ? pa.whole_own : pa.whole_group) + ((int64_t)tok * a.hq + head) * (D + kPad) : rows.parts + lane * rows.rs;
       if (live && (anew >> lane & 1) == 0) {
         if (direct) {
           out = reinterpret_cast<uint8_t*>(reinterpret_cast<T*>(a.out) + (int64_t)tok * a.ldo + (int64_t)head * D);
         } else {
-          *reinterpret_cast<float4*>(part + D) = make_float4(ref, l_run, sees ? 1.f : 0.f, 0.f);
-          out = reinterpret_cast<uint8_t*>(part);
+          *reinterpret_cast<float4*>(part + (D / 4) * rows.cs) = make_float4(ref, l_run, sees ? 1.f : 0.f, 0.f);
         }
       }
       const float whole_l = direct ? 1.0f / l_run : 1.0f;
       const float inv = down * whole_l;
       other *= whole_l;
-      // 128 bytes of each of 32 rows: staged by the rows' threads, stored by eight lanes a row
+      // results: 128 bytes of each of 32 rows, staged by the rows' threads, stored by eight lanes a row
       auto store = [&](int piece, int to) {
         __syncwarp();
 #pragma unroll 4
@@ -901,13 +918,9 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             *reinterpret_cast<uint4*>(place(lane, c * 4 + i / 8)) = pack8<T>(f8);
           }
           if (c & 1) store(c >> 1, (c >> 1) * 128);
-        } else {
-          const int piece = c % DSUB;
-          __syncwarp();                                   // what was staged there has been stored
+        } else if (live && (anew >> lane & 1) == 0) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<uint4*>(place(lane, piece * 8 + i / 4)) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
-          store(piece, c * 128);
+          for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(part + (c * 8 + i / 4) * rows.cs) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
         }
       }
       if (anew != 0) {
@@ -917,6 +930,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             const int i = __ffs(rest) - 1;
             PartRows one = rows;
             one.n0 = n0 + i;
+            one.rs = 0, one.cs = 4;
             one.parts = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(part), i));
             rows_anew<T, T, FMT, D>(a, one, 1u);
           }
@@ -937,15 +951,13 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   }
 }
 
-// Lists that blocks share, where no groups share their rows: a warp per row joins its parts as attn_pages_merge_kernel does.  A block's y-th part of the
-// grid takes every y-th eight rows of the one list that the tree kernel's block x began and did not finish, so that rows which are finished cost nothing
-// (a warp for each of them to find that out took 12 to 18 us for 8000 to 22000 rows).  Rows of sequences without a key become zero.
+// Lists that blocks share, where no groups share their rows: joined as attn_pages_merge_kernel does, a thread per row and four columns, eight rows by
+// sixteen columns a warp (128 bytes of a part at once, 32 of a result).  The grid's x-th blocks take the one list that the tree kernel's block x began and
+// did not finish, so that rows which are finished cost nothing (a warp for each of them to find that out took 12 to 18 us for 8000 to 22000 rows).  Rows of
+// sequences without a key become zero.
 constexpr int kMergeY = 16;
 template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(256) attn_tree_merge_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ PartArgs pa, const __grid_constant__ TreeArgs ta) {
-  constexpr int N = D / 32, VEC = N < 4 ? N : 4;          // columns of a lane, VEC neighbouring ones
-  using Vec = typename std::conditional<VEC == 4, float4, float2>::type;
-  using Out = typename std::conditional<VEC == 4, uint2, uint32_t>::type;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.hq / a.hkv, first = blockIdx.y * 8 + warp;
   for (int s = blockIdx.x; s < a.num_seqs; s += gridDim.x) {              // lengths are not written by the kernel before
     const SegInfo x = seg_info<ROWS>(a, ta, s);
@@ -961,57 +973,37 @@ __global__ void __launch_bounds__(256) attn_tree_merge_kernel(const __grid_const
   const SegInfo x = seg_info<ROWS>(a, ta, cut.seg);
   const int kvh = cut.list / ta.row_tiles, n0 = cut.list % ta.row_tiles * ROWS, rows = min(ROWS, x.rows * group - n0);
   const int parts = cut.last - (int)blockIdx.x + 1;                       // slots: cut.slot, then the first one of each block behind this
-  const float* own = pa.slots + (int64_t)cut.slot * ROWS * (D + kPad);
-  const float* others = pa.slots + (int64_t)2 * blockIdx.x * ROWS * (D + kPad);
-  for (int n = first; n < rows; n += 8 * kMergeY) {
-    auto part = [&](int i) { return (i == 0 ? own : others + (int64_t)2 * i * ROWS * (D + kPad)) + n * (D + kPad); };
-    float o[N], m = -INFINITY, l = 0.f;
+  for (int item = first; item < (rows + 7) / 8 * (D / 16); item += 8 * kMergeY) {
+    const int n = item / (D / 16) * 8 + (lane & 7), col4 = item % (D / 16) * 4 + (lane >> 3);
+    if (n >= rows) continue;
+    auto slot = [&](int i) { return pa.slots + (int64_t)(i == 0 ? cut.slot : 2 * ((int)blockIdx.x + i)) * ROWS * (D + kPad) + n * 4; };
+    float m = -INFINITY;
     bool sees = false;
-#pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = 0.f;
-    for (int b = 0; b < parts; b += 32) {
-      const int k = min(32, parts - b);
-      float4 ml = make_float4(-INFINITY, 0.f, 0.f, 0.f);
-      if (lane < k) ml = *reinterpret_cast<const float4*>(part(b + lane) + D);
-      sees = sees || __any_sync(0xffffffffu, ml.z != 0.f);
-      const float mn = fmaxf(m, warp_max(ml.x)), base = mn == -INFINITY ? 0.f : mn;
-      const float f = m == mn ? 1.f : exp2f(m - base), e = exp2f(ml.x - base);
-      l = l * f + warp_sum(ml.y * e);
-      m = mn;
-#pragma unroll
-      for (int i = 0; i < N; ++i) o[i] *= f;
-      constexpr int AT_ONCE = 4;                                          // parts on their way
-      for (int j = 0; j < k; j += AT_ONCE) {
-        float w[AT_ONCE];
-        Vec v[AT_ONCE][N / VEC];
-#pragma unroll
-        for (int u = 0; u < AT_ONCE; ++u) {
-          w[u] = j + u < k ? __shfl_sync(0xffffffffu, e, j + u) : 0.f;
-          const float* from = part(min(b + j + u, parts - 1));
-#pragma unroll
-          for (int i = 0; i < N / VEC; ++i) {
-            v[u][i] = Vec{};
-            if (w[u] != 0.f) v[u][i] = *reinterpret_cast<const Vec*>(from + i * 32 * VEC + lane * VEC);
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < AT_ONCE; ++u)
-#pragma unroll
-          for (int i = 0; i < N; ++i) o[i] = fmaf(w[u], reinterpret_cast<const float*>(&v[u][i / VEC])[i % VEC], o[i]);
-      }
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) {
+      const float4 st = *reinterpret_cast<const float4*>(slot(i) + D * ROWS);
+      m = fmaxf(m, st.x);
+      sees = sees || st.z != 0.f;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) {
+      const float* from = slot(i);
+      const float4 st = *reinterpret_cast<const float4*>(from + D * ROWS), v = *reinterpret_cast<const float4*>(from + col4 * (ROWS * 4));
+      const float w = exp2f(st.x - base);                                 // 0 of a part in which the row sees nothing
+      l = fmaf(st.y, w, l);
+      if (w != 0.f) o[0] = fmaf(v.x, w, o[0]), o[1] = fmaf(v.y, w, o[1]), o[2] = fmaf(v.z, w, o[2]), o[3] = fmaf(v.w, w, o[3]);
     }
     // a row that sees nothing is zero; NaN where a score was; where all visible scores are minus infinity l is 0, and the row NaN
-    const float inv = sees ? 1.f / l : 0.f;
-    T* out = reinterpret_cast<T*>(a.out) + (int64_t)(x.row0 + (n0 + n) / group) * a.ldo + (int64_t)(kvh * group + (n0 + n) % group) * D;
+    const float inv = 1.f / l;
+    T* out = reinterpret_cast<T*>(a.out) + (int64_t)(x.row0 + (n0 + n) / group) * a.ldo + (int64_t)(kvh * group + (n0 + n) % group) * D + col4 * 4;
+    T y[4];
 #pragma unroll
-    for (int i = 0; i < N; i += VEC) {
-      T v[VEC];
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] = from_f32<T>(sees ? o[i + e] * inv : 0.f);
-      Out y;
-      memcpy(&y, v, sizeof(y));
-      *reinterpret_cast<Out*>(out + i * 32 + lane * VEC) = y;
-    }
+    for (int e = 0; e < 4; ++e) y[e] = from_f32<T>(sees ? o[e] * inv : 0.f);
+    uint2 packed;
+    memcpy(&packed, y, sizeof(packed));
+    *reinterpret_cast<uint2*>(out) = packed;
   }
 }
 
