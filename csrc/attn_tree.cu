@@ -159,7 +159,7 @@ struct Part {
 };
 // the list that a block begins and others go on with (where no groups share its rows): its first slot, < 0: none; the others' last block
 struct Cut {
-  int slot, last, seg, list;         // list: kvh row_tiles + tile of rows
+  int slot, last_rows, row0, list;   // last block, rows << 16; first row of the segment; kvh row_tiles + tile of rows
 };
 static_assert(sizeof(Cut) == sizeof(FewInfo), "they share their place");
 // a place in a run
@@ -807,7 +807,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       if (bad) l_run = __int_as_float(0x7fc00000);
       const bool whole = p.u0 == 0 && p.u1 == p.n, direct = whole && a.groups == 0;
       const int slot = 2 * blockIdx.x + (p.u0 == 0 && at > 0 ? 1 : 0);
-      if (p.u0 == 0 && !whole) cut = {slot, (int)((w.cur - (p.u1 - p.u0) + p.n - 1) / per), p.seg, p.kvh * pa.row_tiles + p.rt};
+      if (p.u0 == 0 && !whole) cut = {slot, (int)((w.cur - (p.u1 - p.u0) + p.n - 1) / per) | min(ROWS, p.nrows - p.n0) << 16, p.s.row0, p.kvh * pa.row_tiles + p.rt};
       if (a.groups > 0 && p.u0 == 0 && q == 0 && quarter == 0 && lane == 0) {
         FewInfo in;
         in.first_slot = whole ? -1 : slot;
@@ -970,34 +970,44 @@ __global__ void __launch_bounds__(256) attn_tree_merge_kernel(const __grid_const
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Cut cut = reinterpret_cast<const Cut*>(pa.info)[blockIdx.x];
   if (cut.slot < 0) return;
-  const SegInfo x = seg_info<ROWS>(a, ta, cut.seg);
-  const int kvh = cut.list / ta.row_tiles, n0 = cut.list % ta.row_tiles * ROWS, rows = min(ROWS, x.rows * group - n0);
-  const int parts = cut.last - (int)blockIdx.x + 1;                       // slots: cut.slot, then the first one of each block behind this
+  const int kvh = cut.list / ta.row_tiles, n0 = cut.list % ta.row_tiles * ROWS, rows = cut.last_rows >> 16;
+  const int parts = (cut.last_rows & 0xffff) - (int)blockIdx.x + 1;       // slots: cut.slot, then the first one of each block behind this
   for (int item = first; item < (rows + 7) / 8 * (D / 16); item += 8 * kMergeY) {
     const int n = item / (D / 16) * 8 + (lane & 7), col4 = item % (D / 16) * 4 + (lane >> 3);
     if (n >= rows) continue;
-    auto slot = [&](int i) { return pa.slots + (int64_t)(i == 0 ? cut.slot : 2 * ((int)blockIdx.x + i)) * ROWS * (D + kPad) + n * 4; };
-    float m = -INFINITY;
+    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
     bool sees = false;
-#pragma unroll 4
-    for (int i = 0; i < parts; ++i) {
-      const float4 st = *reinterpret_cast<const float4*>(slot(i) + D * ROWS);
-      m = fmaxf(m, st.x);
-      sees = sees || st.z != 0.f;
-    }
-    const float base = m == -INFINITY ? 0.f : m;
-    float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int i = 0; i < parts; ++i) {
-      const float* from = slot(i);
-      const float4 st = *reinterpret_cast<const float4*>(from + D * ROWS), v = *reinterpret_cast<const float4*>(from + col4 * (ROWS * 4));
-      const float w = exp2f(st.x - base);                                 // 0 of a part in which the row sees nothing
-      l = fmaf(st.y, w, l);
-      if (w != 0.f) o[0] = fmaf(v.x, w, o[0]), o[1] = fmaf(v.y, w, o[1]), o[2] = fmaf(v.z, w, o[2]), o[3] = fmaf(v.w, w, o[3]);
+    constexpr int AT_ONCE = 4;                                            // parts on their way
+    for (int i = 0; i < parts; i += AT_ONCE) {
+      float4 st[AT_ONCE], v[AT_ONCE];
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        st[u] = make_float4(-INFINITY, 0.f, 0.f, 0.f), v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i + u < parts) {
+          const float* from = pa.slots + (int64_t)(i + u == 0 ? cut.slot : 2 * ((int)blockIdx.x + i + u)) * ROWS * (D + kPad) + n * 4;
+          st[u] = *reinterpret_cast<const float4*>(from + D * ROWS);
+          v[u] = *reinterpret_cast<const float4*>(from + col4 * (ROWS * 4));
+        }
+      }
+      float mn = m;
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) mn = fmaxf(mn, st[u].x);
+      const float base = mn == -INFINITY ? 0.f : mn, f = m == mn ? 1.f : exp2f(m - base);
+      m = mn;
+      l *= f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] *= f;
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        const float w = exp2f(st[u].x - base);                            // 0 of a part in which the row sees nothing
+        sees = sees || st[u].z != 0.f;
+        l = fmaf(st[u].y, w, l);
+        if (w != 0.f) o[0] = fmaf(v[u].x, w, o[0]), o[1] = fmaf(v[u].y, w, o[1]), o[2] = fmaf(v[u].z, w, o[2]), o[3] = fmaf(v[u].w, w, o[3]);
+      }
     }
     // a row that sees nothing is zero; NaN where a score was; where all visible scores are minus infinity l is 0, and the row NaN
     const float inv = 1.f / l;
-    T* out = reinterpret_cast<T*>(a.out) + (int64_t)(x.row0 + (n0 + n) / group) * a.ldo + (int64_t)(kvh * group + (n0 + n) % group) * D + col4 * 4;
+    T* out = reinterpret_cast<T*>(a.out) + (int64_t)(cut.row0 + (n0 + n) / group) * a.ldo + (int64_t)(kvh * group + (n0 + n) % group) * D + col4 * 4;
     T y[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] = from_f32<T>(sees ? o[e] * inv : 0.f);
