@@ -409,8 +409,8 @@ def step_layout(context_lens, new_lens, pages, page_size, rows, max_new, page_co
     B, mb, words = drafts.check_layout(context_lens, new_lens, pages, page_size, rows, max_new, page_counts, max_blocks, parents)
     # one allocation: views of it are cheaper than tensors
     lists = page_counts is not None
-    last, lens, cu, positions, slots, tables, masks = torch.empty(4 * B + 1 + rows * (2 + words) + (B * mb if lists else 0), dtype=torch.int32, device=context_lens.device) \
-        .split([2 * B, B, B + 1, rows, rows, B * mb if lists else 0, rows * words])
+    sizes = (2 * B, B, B + 1, rows, rows, B * mb if lists else 0, rows * words)
+    last, lens, cu, positions, slots, tables, masks = context_lens.new_empty(sum(sizes)).split_with_sizes(sizes)
     tables = tables.view(B, mb) if lists else pages if pages.shape[0] == B else pages[:B]
     rc = _lib.load().llmss_step_layout(context_lens.data_ptr(), new_lens.data_ptr(), pages.data_ptr(), pages.numel(), page_counts.data_ptr() if lists else None,
                                        parents.data_ptr() if words else None, last.data_ptr(), lens.data_ptr(), cu.data_ptr(), positions.data_ptr(),
@@ -431,7 +431,7 @@ def accept_drafts(sampled, batch, pages):
             return accept_drafts(sampled, batch, pages)
     planes, blocks, heads, size = drafts.check_accept(sampled, batch, pages)
     B, wide, parents = batch.num_seqs, batch.max_q, batch.tree.parents
-    tokens, path, counts, context = torch.empty(2 * B * (wide + 1), dtype=torch.int32, device=sampled.device).split([B * wide, B * wide, B, B])
+    tokens, path, counts, context = sampled.new_empty(2 * B * (wide + 1)).split_with_sizes((B * wide, B * wide, B, B))
     outs = (tokens.data_ptr(), counts.data_ptr(), path.data_ptr(), context.data_ptr())
     pages = [x for x in pages if x.numel()]
     lib = _lib.load()

@@ -77,10 +77,11 @@ def check_accept(sampled, batch, pages):
     if not pages:
         return 0, 0, 1, 1
     lead = pages[0].shape[:-1]
-    if len(lead) < 3:
+    n = len(lead)
+    if n < 3:
         raise ValueError(f"accept_drafts: cache tensors are [.., blocks, heads, block_size, d], got {tuple(pages[0].shape)}")
     for x in pages:
-        if x.shape[:len(lead)] != lead or not x.is_contiguous() or x.get_device() != dev or (x.numel() == 0 and lead.numel() > 0):
+        if x.shape[:n] != lead or not x.is_contiguous() or x.get_device() != dev or (x.numel() == 0 and lead.numel() > 0):
             raise ValueError(f"accept_drafts: cache tensors are contiguous, on {sampled.device}, and alike up to a row ({tuple(lead)}), got {tuple(x.shape)} "
                              f"on {x.device}")
     return lead[:-3].numel(), lead[-3], lead[-2], lead[-1]
