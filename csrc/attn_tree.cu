@@ -1,8 +1,9 @@
 // Attention of trees of drafted tokens over cache pages on the 5th-generation tensor cores, for more than 16 query rows of a key head.
 //
+//   s_jk = scale (q_j . K_k)     p = softmax over {k < ctx} and {ctx + a : bit a of mask_j}     out_j = sum_k p_jk V_k
+//
 // A list is a (sequence, key head, up to 256 of its rows); a row is a (token, query head), so that grouped heads and a tree's tokens fill a tile's 128 rows and
-// a key is read once for all of them.  Rows see all cached keys, so that masks are looked at in a list's last tiles alone.  What bounds a call is reading
-// the cache: 64 keys of 128 columns in 16 bits are 32 KB, which an SM's share of the memory brings in 0.75 us, while the products of 128 rows take 0.3.
+// a key is read once for all of them.  Rows see all cached keys, so that masks are looked at in a list's last tiles alone.
 //
 // So the work of a call, the sum of all lists in tiles of 64 keys, is cut into equal runs, one per SM, by the lengths that lie on the device; a block goes
 // from list to list, and its copies run ahead of it through a ring as deep as shared memory allows, over the ends of lists:
@@ -18,8 +19,14 @@
 // two tiles of 128 rows over the same keys, or, where a segment has up to 128 rows, even and odd tiles of keys of the same rows (DUAL), each with scores,
 // outputs, maximum and sum of its own, which are joined at a list's end.
 //
+// What bounds it: 64 keys of 128 columns in 16 bits are 32 KB, which an SM's share of the memory brings in 0.75 us; their products with 256 rows are 0.55 us of
+// the tensor pipe, and the softmax of 256 rows takes 0.95, two warps on a scheduler (1480 clocks: 750 are exponentials of the MUFU pipe, about 700 other
+// instructions, of which one takes 2 to 3 clocks with two warps).  6 trees of 40 tokens over 24000, 32 / 8 heads: 142 us, 0.65 of the copy rate.  In 8 bits memory
+// would need 0.39 us, but codes, scales of keys and scales of values are 480 more instructions a tile and scheduler: 48 trees of 24 tokens over 1500, 147 us,
+// 0.18 of the copy rate; a warp of its own for every fourth half of a tile instead of all for each: 157.
+//
 // The values' scales join the probabilities before their one rounding to f16, relative to a power of two per tile (TileScales) that keeps them in range;
-// scaled and rounded codes (2^-11 of each key, value and probability) would make f16 results three times as far off.
+// scaled and rounded codes (2^-11 of each key, value and probability) make f16 results off by 6.1e-4 instead of 2.9e-4.
 // A list within a block's run is finished there, one that crosses runs leaves its parts in scratch, at most two per block, and the merge kernel joins them.
 #include "attn_pages.cuh"
 
@@ -57,7 +64,7 @@ struct Tree {
   static constexpr int FIXED = 1024 + Q_BYTES + SCALES + JOIN + 1024 + kKept * (int)sizeof(SegInfo) + 64;
   static constexpr int ROOM = 232448 - FIXED;
   // 16 bits: all there is, up to 24.  8 bits: three to eight tiles in f16, codes in the rest; a tile's scales are looked at until its values' slot is free,
-  // which is RAWS + SLOTS copies behind: fewer than two per tile of scales
+  // and the keys sixteen tiles on are copied RAWS + SLOTS copies behind that at the earliest: fewer than two per tile of scales
   static constexpr int SLOTS = !BYTES ? (ROOM / SLOT < 24 ? ROOM / SLOT : 24) : D == 256 ? 3 : D == 128 ? 6 : 8;
   static constexpr int RAWS = !BYTES ? 0 : (ROOM - SLOTS * SLOT) / RAW < 16 ? (ROOM - SLOTS * SLOT) / RAW : 16;
   static constexpr int SMEM = FIXED + SLOTS * SLOT + RAWS * RAW;

@@ -73,6 +73,19 @@ def test_step_layout_of_lengths_that_do_not_fit():
     assert got.slot_mapping.tolist() == [18, 19, 8] + [-1] * 6 and got.block_tables.tolist() == [[9, 4], [0, 0], [0, 0]]
 
 
+def test_calls_without_sequences_or_rows():
+    none = ints([]).cuda()
+    got = ops.step_layout(none, none, none, 16, 3, 0, page_counts=none, max_blocks=2)
+    assert got.cu_q.tolist() == [0] and got.slot_mapping.tolist() == [-1] * 3 and got.block_tables.shape == (0, 2) and got.last_idx.numel() == 0
+    got = ops.step_layout(ints([4, 9]).cuda(), ints([0, 0]).cuda(), ints([[1], [2]]).cuda(), 16, 0, 0, parents=none)
+    assert got.cu_q.tolist() == [0, 0, 0] and got.seq_lens.tolist() == [4, 9] and got.last_idx.tolist() == [-1, -1] and got.masks.shape == (0, 0)
+    batch = BatchInput.build([[], []], [4, 9], [[1], [2]], 16, "cuda", parents=[[], []])
+    data = torch.randn(2, 4, 3, 16, 8).cuda()
+    old = data.clone()
+    got = ops.accept_drafts(none, batch, [data])
+    assert got.counts.tolist() == [0, 0] and got.context_lens.tolist() == [4, 9] and got.tokens.shape == (2, 0) and torch.equal(data, old)
+
+
 def test_build_is_the_same_on_both_devices():
     rng = random.Random(3)
     new, ctx = [[rng.randrange(99) for _ in range(n)] for n in (1, 40, 0, 7)], [5, 0, 3, 64]
@@ -124,7 +137,40 @@ FULL = {
     "up_to_128_rows": ([30, 12, 7, 25] * 6, [2100, 3900, 64, 1000] * 6),
     "up_to_256_rows": ([60, 33, 7, 40] * 6, [2100, 3900, 64, 1000] * 6),
     "short_lists": ([9, 30, 5] * 20, [0, 40, 130] * 20),
+    "more_sequences_than_a_block_keeps": ([9, 30, 0, 5, 18] * 40, [0, 140, 7, 33, 65] * 40),
 }
+
+
+@pytest.mark.parametrize("page", [48, 128, 16 * 7])
+@pytest.mark.parametrize("kind", [None, I8])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 64), (16, 4, 128)])
+def test_pages_of_any_multiple_of_sixteen(hq, hkv, d, kind, page):
+    new, ctx, rng = [20, 3, 70], [500, 47, 131], random.Random(page)
+    batch, seen = make_batch(new, ctx, page, [], "cuda", seed=4)
+    set_masks(batch, seen, [s for n in new for s in ancestors(random_parents(n, rng))])
+    q = queries(sum(new), hq * d, BF)
+    k, v = (make_pages(seen.blocks, hkv, page, d, kind, BF, "cuda", seed=i) for i in range(2))
+    out = ops.attention(q, torch.full_like(q, NAN), batch, k, v, hq, hkv, d, d ** -0.5, 0, 0, 0)
+    want, tol, _ = expected(q, k, v, batch, seen, hq, hkv, d, d ** -0.5)
+    assert ((out.double() - want).abs() <= tol).all()
+
+
+def test_bounds_of_a_captured_step():
+    """Generous bounds, as a captured step gives them: every kernel goes by the lengths themselves."""
+    hq, hkv, d = 16, 4, 128
+    for new in ([2, 1, 3], [20, 3, 31], [1, 1, 1]):
+        batch, seen = make_batch(new, [500, 47, 131], 64, [], "cuda", seed=4)
+        rng = random.Random(0)
+        for max_q in (max(new), 30, 64, 200):
+            if max_q < max(new):
+                continue
+            batch.max_q, batch.max_kv = max_q, 100000
+            set_masks(batch, seen, [s for n in new for s in ancestors(random_parents(n, rng))])
+            q = queries(sum(new), hq * d, BF)
+            k, v = (make_pages(seen.blocks, hkv, 64, d, None, BF, "cuda", seed=i) for i in range(2))
+            out = ops.attention(q, torch.full_like(q, NAN), batch, k, v, hq, hkv, d, d ** -0.5, 0, 0, 0)
+            want, tol, _ = expected(q, k, v, batch, seen, hq, hkv, d, d ** -0.5)
+            assert ((out.double() - want).abs() <= tol).all()
 
 
 @pytest.mark.parametrize("kind,dtype", [(None, BF), (I8, BF), (E4, HF)])
