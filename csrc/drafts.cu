@@ -281,7 +281,7 @@ LLMSS_API int llmss_accept_drafts(const int* tokens, const int* parents, const i
   LLMSS_REQUIRE(page > 0 && heads > 0, "accept_drafts: pages of %d tokens and %d heads", page, heads);
   LLMSS_REQUIRE((int64_t)num_blocks * heads * page < (1ll << 31), "accept_drafts: 2^31 cache rows and more");
   LLMSS_REQUIRE((int64_t)planes * heads < (1ll << 31) && (int64_t)max_blocks * page < (1ll << 31), "accept_drafts: sizes of 2^31 and more");
-  LLMSS_REQUIRE((out_tokens != nullptr) == (counts != nullptr) && (counts != nullptr) == (path != nullptr) && (path != nullptr) == (context != nullptr),
+  LLMSS_REQUIRE((counts != nullptr) == (context != nullptr) && (max_q == 0 || ((out_tokens != nullptr) == (counts != nullptr) && (path != nullptr) == (counts != nullptr))),
                 "accept_drafts: all outputs or none");
   AcceptArgs a;
   memset(&a, 0, sizeof(a));
@@ -304,7 +304,7 @@ LLMSS_API int llmss_accept_drafts(const int* tokens, const int* parents, const i
   a.max_blocks = max_blocks;
   a.page = page;
   a.num_blocks = num_blocks;
-  a.write = out_tokens != nullptr;
+  a.write = counts != nullptr;
   int64_t widest = 1;
   for (int s = 0; s < num_sets; ++s) {
     LLMSS_REQUIRE(bases[s] != nullptr && row_bytes[s] > 0, "accept_drafts: tensor %d is null or has rows of %d bytes", s, row_bytes[s]);
