@@ -374,13 +374,14 @@ Plan plan_call(int num_seqs, int max_q, int max_kv, int total_q, int hq, int hkv
   p.few_groups = groups > 0 && grouped <= 16;
   p.row_tiles = 1;
   if (tree && (own > 16 || grouped > 16)) {
-    // All lists by the kernel for trees: two times 128 rows where there are more than 128 (and tensor memory holds two).  Lists of 128 rows each instead: 6 trees
-    // of 40 tokens over 24000, 32 / 8 heads, 171 -> 211 us, 8 of 170 over 3000 in 8 bits 97 -> 106.  From 17 rows on, where the one for few rows would have to
-    // read every key again
+    // All lists by the kernel for trees, from 17 rows on, where the one for few rows would have to read every key again.  Two times 128 rows where the bound is
+    // more than 128 (and tensor memory holds two): 6 trees of up to 60 tokens over 24000, 32 / 8 heads, 165 us, with lists of 128 rows each 226.  8 bits, where
+    // two threads share a row: more than 192, since lists below the bound are many: 48 of up to 36 tokens (144 rows) over 1500 144 us, with 128 rows 122; 8 of
+    // up to 255 rows over 3000 91 and 101
     const int64_t most = own > grouped ? own : grouped;
     p.tree = p.few_own = true;
     p.few_groups = groups > 0;
-    p.rows = tile_rows(d, most);
+    p.rows = fmt != kF16Pages && most <= 192 ? 128 : tile_rows(d, most);
     p.row_tiles = (int)((most + p.rows - 1) / p.rows);
     p.slots = (int64_t)2 * kTreeBlocks * p.rows * (d + kPad);
     p.info = groups > 0 ? ((int64_t)num_seqs + groups) * hkv * p.row_tiles * 4 : kTreeBlocks * 4;

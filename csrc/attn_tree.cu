@@ -10,20 +10,19 @@
 //
 //   copying warps   one keys, one values, page by page (TMA, 128-byte swizzle), in the order K0, K1 V0, K2 V1 .. of a list; 8-bit codes and scales into a
 //                   ring of their own (bulk copies), from which
-//   converting warps (8-bit) write the tiles as f16: a code is an f16 number, so nothing is rounded
+//   converting warps (8-bit) write the tiles as f16: a code is an f16 number, so nothing is rounded.  One each for keys and values of even tiles and of odd ones
+//                   (all for every tile where heads have 256 columns): waits and fences cost a warp as much as its codes do
 //   issuing warps   one per 128 rows: S_j = Q K_j^T (two S buffers), O += P_j V_j with P_j in tensor memory over S_j
-//   softmax warps   a thread per row: S from tensor memory times the keys' scales, mask, running maximum (moved when exceeded by 2^8) and sum in 32 bits,
-//                   P times the values' scales back.  Those without a row of the list only keep the barriers going
+//   softmax warps   one or two threads per row, with 64 or 32 keys of a tile: S from tensor memory times the keys' scales, mask, maximum of the row (the running one
+//                   moves when it is exceeded by 2^8), sum in 32 bits, P times the values' scales back.  Those without a row of the list only keep the
+//                   barriers going
 //
-// One warp per scheduler waits for its own loads and exponentials most of the time.  So there are two streams (tensor memory of 256 columns holds one):
-// two tiles of 128 rows over the same keys, or, where a segment has up to 128 rows, even and odd tiles of keys of the same rows (DUAL), each with scores,
-// outputs, maximum and sum of its own, which are joined at a list's end.
-//
-// What bounds it: 64 keys of 128 columns in 16 bits are 32 KB, which an SM's share of the memory brings in 0.75 us; their products with 256 rows are 0.55 us of
-// the tensor pipe, and the softmax of 256 rows takes 0.95, two warps on a scheduler (1480 clocks: 750 are exponentials of the MUFU pipe, about 700 other
-// instructions, of which one takes 2 to 3 clocks with two warps).  6 trees of 40 tokens over 24000, 32 / 8 heads: 142 us, 0.65 of the copy rate.  In 8 bits memory
-// would need 0.39 us, but codes, scales of keys and scales of values are 480 more instructions a tile and scheduler: 48 trees of 24 tokens over 1500, 147 us,
-// 0.18 of the copy rate; a warp of its own for every fourth half of a tile instead of all for each: 157.
+// What bounds it: 64 keys of 128 columns in 16 bits are 32 KB, which an SM's share of the memory brings in 0.75 us; their products with 256 rows take the tensor
+// pipe and the shared memory that it reads 0.6 to 0.7 (queries are read again for every tile), and the softmax of 256 rows 0.6 (750 clocks of exponentials in
+// the MUFU pipe, 700 of other instructions beside them), each waiting for the other at a tile's ends: 6 trees of 40 tokens over 24000, 32 / 8 heads, whose rows
+// fill 160 of the 256, 142 us, 0.65 of the copy rate.  In 8 bits memory would need 0.39 us, but codes, scales of keys and scales of values are 480 more
+// instructions a tile and scheduler: 48 trees of 24 tokens over 1500, 119 us, 0.23 of the copy rate (one thread a row 150, and that with one converting warp
+// for every fourth half of a tile 157; two threads a row without that 142).
 //
 // The values' scales join the probabilities before their one rounding to f16, relative to a power of two per tile (TileScales) that keeps them in range;
 // scaled and rounded codes (2^-11 of each key, value and probability) make f16 results off by 6.1e-4 instead of 2.9e-4.
@@ -46,13 +45,16 @@ struct SegInfo {
   int ctx;                // cached tokens in front of the new ones (own lists)
 };
 
-template <int FMT, int D, int NQ, bool DUAL>
+template <int FMT, int D, int NQ>
 struct Tree {
   static constexpr bool BYTES = FMT != kF16Pages;
-  static constexpr int QT = DUAL ? 1 : NQ;                              // tiles of 128 rows; NQ streams
-  static constexpr int ROWS = QT * BM;
-  static constexpr int SOFT = 4 * NQ;                                   // softmax warps
-  static constexpr int CONVERT = !BYTES ? 0 : NQ == 2 ? 4 : 8;
+  static constexpr int ROWS = NQ * BM;                                  // NQ tiles of 128 rows
+  // Threads of a row.  With two a scheduler has twice as many warps for the same instructions (an instruction is done in 2 to 4 clocks with one, in 1.2 to 2.3
+  // with four); where there are eight softmax warps already and nothing is converted, one is faster (6 trees of 40 tokens over 24000 165 us, with two 191)
+  static constexpr int SHARE = BYTES || NQ == 1 ? 2 : 1, COLS = BN / SHARE;
+  static constexpr int SOFT = 4 * NQ * SHARE;                           // softmax warps
+  // converting warps, in groups that take every so many halves of tiles
+  static constexpr int CONVERT = BYTES ? 4 : 0, GROUPS = !BYTES ? 0 : D == 256 ? 1 : 4;
   static constexpr int COPY = SOFT + NQ;                                // first copying warp
   static constexpr int CONV = COPY + 2;                                 // first converting warp
   static constexpr int THREADS = 32 * (CONV + CONVERT);
@@ -60,17 +62,21 @@ struct Tree {
   static constexpr int SLOT = BN * D * 2;                               // a tile of keys or values
   static constexpr int RAW = BYTES ? BN * D : 0;                        // a tile of codes
   static constexpr int SCALES = BYTES ? kScaleTiles * (2 * BN * 4 + 16) : 0;
-  static constexpr int JOIN = DUAL ? BM * (128 + 16) : 0;               // what a stream hands to the other: 32 columns of its rows, and their state
-  static constexpr int FIXED = 1024 + Q_BYTES + SCALES + JOIN + 1024 + kKept * (int)sizeof(SegInfo) + 64;
+  static constexpr int PAIR = NQ * BM * (2 * 2 * 4 + 2 * 8 + 4);        // what the two threads of a row tell each other
+  static constexpr int FIXED = 1024 + Q_BYTES + SCALES + PAIR + 1024 + kKept * (int)sizeof(SegInfo) + 128;
   static constexpr int ROOM = 232448 - FIXED;
   // 16 bits: all there is, up to 24.  8 bits: three to eight tiles in f16, codes in the rest; a tile's scales are looked at until its values' slot is free,
   // and the keys sixteen tiles on are copied RAWS + SLOTS copies behind that at the earliest: fewer than two per tile of scales
-  static constexpr int SLOTS = !BYTES ? (ROOM / SLOT < 24 ? ROOM / SLOT : 24) : D == 256 ? 3 : D == 128 ? 6 : 8;
-  static constexpr int RAWS = !BYTES ? 0 : (ROOM - SLOTS * SLOT) / RAW < 16 ? (ROOM - SLOTS * SLOT) / RAW : 16;
+  static constexpr int SLOTS = !BYTES ? (ROOM / SLOT < 24 ? ROOM / SLOT : 24) : D == 256 ? 3 : D == 128 ? 4 : 8;
+  static constexpr int MOST = !BYTES ? 0 : (ROOM - SLOTS * SLOT) / RAW, RAWS = GROUPS == 4 ? (MOST < 12 ? MOST / 4 * 4 : 12) : MOST;
   static constexpr int SMEM = FIXED + SLOTS * SLOT + RAWS * RAW;
   static constexpr int TMEM = NQ * (2 * BN + D) <= 256 ? 256 : 512;
-  static constexpr int RING = DUAL ? SLOTS / 2 : SLOTS;                 // slots of a ring: each stream's own (DUAL)
-  static_assert(RING >= (BYTES ? 3 : DUAL ? 5 : 4) && (!BYTES || (RAWS >= 3 && RAWS + SLOTS <= 2 * kScaleTiles - 4)), "rings");
+  // Even and odd tiles have a ring each, K and V in turn, where converting warps take halves of tiles alone: a barrier tells a phase from the one before
+  // only, so that who waits on a slot has to take part in each of its uses
+  static constexpr bool TWO = GROUPS == 4;
+  static constexpr int RING = TWO ? SLOTS / 2 : SLOTS;
+  static_assert(RING >= (TWO ? 2 : BYTES ? 3 : 4) && (GROUPS != 4 || (RING % 2 == 0 && RAWS % 4 == 0)), "rings");
+  static_assert(!BYTES || (RAWS >= 3 && (GROUPS == 4 ? RAWS / 2 + RING + 5 < kScaleTiles : RAWS + SLOTS <= 2 * kScaleTiles - 4)), "scales");
   static_assert((2 * SLOTS + 2 * RAWS + 7 * NQ + 2) * 8 <= 1024, "barriers");
 };
 
@@ -140,8 +146,8 @@ __device__ __forceinline__ float exp2_fma(float x) {
   return __int_as_float(__float_as_int(t) * (1 << 23) + __float_as_int(p));     // (what the 1.5 2^23 of t holds besides x leaves the word)
 }
 
-// warps `quarter` of both streams
-__device__ __forceinline__ void pair_sync(int quarter) { asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory"); }
+// the two warps of 32 rows
+__device__ __forceinline__ void pair_sync(int pair) { asm volatile("bar.sync %0, 64;" ::"r"(pair + 1) : "memory"); }
 
 template <int ROWS>
 __device__ __forceinline__ SegInfo seg_info(const AttnArgs& a, const TreeArgs& ta, int i) {
@@ -240,22 +246,24 @@ __device__ __noinline__ void rows_anew(const AttnArgs& a, const PartRows& p, uns
   }
 }
 
-template <typename T, int FMT, int D, int NQ, bool DUAL>
-__global__ void __launch_bounds__(Tree<FMT, D, NQ, DUAL>::THREADS, 1)
+template <typename T, int FMT, int D, int NQ>
+__global__ void __launch_bounds__(Tree<FMT, D, NQ>::THREADS, 1)
 attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnArgs a,
                  const __grid_constant__ PartArgs pa, const __grid_constant__ TreeArgs ta) {
-  using C = Tree<FMT, D, NQ, DUAL>;
+  using C = Tree<FMT, D, NQ>;
   using M = typename std::conditional<C::BYTES, __half, T>::type;   // type of the products
   constexpr int DSUB = D / 64, ROWS = C::ROWS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint8_t* s_q = smem;                                   // [QT][DSUB][128 rows][128 bytes]
+  uint8_t* s_q = smem;                                   // [NQ][DSUB][128 rows][128 bytes]
   uint8_t* s_kv = s_q + C::Q_BYTES;                      // [SLOTS][DSUB][64 keys][128 bytes]
   uint8_t* s_raw = s_kv + C::SLOTS * C::SLOT;            // [RAWS][64 keys of codes]
   float* s_scale = reinterpret_cast<float*>(s_raw + C::RAWS * C::RAW);   // [tiles][keys', values'][64] (8-bit)
   TileScales* s_tile = reinterpret_cast<TileScales*>(s_scale + (C::BYTES ? kScaleTiles * 2 * BN : 0));   // [tiles]
-  float4* s_join = reinterpret_cast<float4*>(s_raw + C::RAWS * C::RAW + C::SCALES);   // [4 warps][8][32 rows], then [128 rows] (DUAL)
-  uint64_t* bars = reinterpret_cast<uint64_t*>(s_raw + C::RAWS * C::RAW + C::SCALES + C::JOIN);
+  float* s_max = reinterpret_cast<float*>(s_raw + C::RAWS * C::RAW + C::SCALES);          // [two tiles][NQ][two threads][128 rows]
+  float2* s_sum = reinterpret_cast<float2*>(s_max + 2 * 2 * ROWS);                        // [NQ][two threads][128 rows]: sum, flags
+  float* s_unit = reinterpret_cast<float*>(s_sum + 2 * ROWS);                             // [rows]: what the queries were divided by
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_raw + C::RAWS * C::RAW + C::SCALES + C::PAIR);
   uint64_t* bar_full = bars;                             // [SLOTS]
   uint64_t* bar_empty = bars + C::SLOTS;
   uint64_t* bar_s = bars + 2 * C::SLOTS;                 // [NQ][2] S ready
@@ -266,7 +274,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   uint64_t* bar_raw = bar_part + 1;                      // [RAWS] codes have come
   uint64_t* bar_used = bar_raw + C::RAWS;                // [RAWS] codes have been converted
   SegInfo* s_info = reinterpret_cast<SegInfo*>(bars + 128);
-  unsigned* s_sum = reinterpret_cast<unsigned*>(s_info + kKept);         // [16] places of this block's run, and sums before them
+  unsigned* s_total = reinterpret_cast<unsigned*>(s_info + kKept);       // [warps] tiles of the lists that a warp looked at
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_used + C::RAWS);
 
   // by a shuffle: numbers that the compiler knows to be the same in all lanes need no copies into uniform registers at every product
@@ -277,19 +285,19 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   }
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::SLOTS; ++i) {
-      mbar_init(&bar_full[i], C::BYTES ? C::CONVERT : 1);
-      mbar_init(&bar_empty[i], C::QT);
+      mbar_init(&bar_full[i], C::BYTES ? C::CONVERT / C::GROUPS : 1);
+      mbar_init(&bar_empty[i], NQ);
     }
     for (int i = 0; i < 2 * NQ; ++i) {
       mbar_init(&bar_s[i], 1);
-      mbar_init(&bar_p[i], 4);
+      mbar_init(&bar_p[i], 4 * C::SHARE);
       mbar_init(&bar_o[i], 1);
     }
-    for (int i = 0; i < NQ; ++i) mbar_init(&bar_q[i], 4);
+    for (int i = 0; i < NQ; ++i) mbar_init(&bar_q[i], 4 * C::SHARE);
     mbar_init(bar_part, 1);
     for (int i = 0; i < C::RAWS; ++i) {
       mbar_init(&bar_raw[i], 1);
-      mbar_init(&bar_used[i], C::CONVERT);
+      mbar_init(&bar_used[i], C::CONVERT / (C::BYTES ? C::GROUPS : 1));
     }
     fence_mbar_init();
   }
@@ -305,7 +313,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     sum += weigh(x);
   }
   sum = __reduce_add_sync(0xffffffffu, sum);
-  if (lane == 0) s_sum[warp] = sum;
+  if (lane == 0) s_total[warp] = sum;
   if (warp == C::SOFT) {
     tmem_alloc(tmem_slot, C::TMEM);
     tmem_relinquish();
@@ -315,7 +323,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   tcgen05_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   unsigned total = 0;
-  for (int i = 0; i < C::THREADS / 32; ++i) total += s_sum[i];
+  for (int i = 0; i < C::THREADS / 32; ++i) total += s_total[i];
   const unsigned per = max((total + gridDim.x - 1) / gridDim.x, (unsigned)kLeastTiles);
   const unsigned begin = min(per * blockIdx.x, total), end = min(begin + per, total);
   // every warp finds the run's first segment for itself
@@ -371,20 +379,23 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   // places of a list's tiles in the order they come: K0, then K_{j+1}, V_j, and V of the last tile
   auto key_at = [](int j) { return j == 0 ? 0 : 2 * j - 1; };
   auto value_at = [](int j, int n) { return j + 1 < n ? 2 * j + 2 : 2 * n - 1; };
-  // Slot of tile j, with the parity of its use.  Two streams have a ring each, K and V in turn: a barrier tells a phase from the one before alone, so that
-  // who waits on a slot has to take part in each of its uses, and a stream takes no part in the other's tiles
+  // slot of tile j, with the parity of its use
   struct Slot {
     unsigned at;
     uint32_t phase;
   };
-  auto slot_of = [&](unsigned tile0, unsigned even0, int j, int n, bool value) {     // even0: of the tiles before, the first stream's
-    unsigned place;
-    if constexpr (DUAL) place = 2 * (((j & 1) ? tile0 - even0 : even0) + (j >> 1)) + value;
-    else place = 2 * tile0 + (value ? value_at(j, n) : key_at(j));
-    return Slot{place % C::RING + (DUAL && (j & 1) ? C::RING : 0), (place / C::RING) & 1};
+  auto of_parity = [](unsigned tile0, unsigned even0, int j) { return ((j & 1) ? tile0 - even0 : even0) + (j >> 1); };   // even0: even tiles of those before
+  auto slot_of = [&](unsigned tile0, unsigned even0, int j, int n, bool value) {
+    const unsigned place = C::TWO ? 2 * of_parity(tile0, even0, j) + value : 2 * tile0 + (value ? value_at(j, n) : key_at(j));
+    return Slot{place % C::RING + (C::TWO && (j & 1) ? C::RING : 0), (place / C::RING) & 1};
+  };
+  // of a tile's codes: a ring for each group of converting warps
+  auto raw_of = [&](unsigned tile0, unsigned even0, int j, int n, bool value) {
+    constexpr int RAW_RING = C::GROUPS == 4 ? C::RAWS / 4 : C::RAWS < 1 ? 1 : C::RAWS;
+    const unsigned place = C::GROUPS == 4 ? of_parity(tile0, even0, j) : 2 * tile0 + (value ? value_at(j, n) : key_at(j));
+    return Slot{place % RAW_RING + (C::GROUPS == 4 ? (2 * (j & 1) + value) * RAW_RING : 0), (place / RAW_RING) & 1};
   };
   auto t_s = [&](int q, int b) { return tmem + q * (2 * BN + D) + b * BN; };
-  constexpr int STREAMS = DUAL ? 2 : 1;    // that share a list's tiles of keys
   auto t_o = [&](int q) { return tmem + q * (2 * BN + D) + 2 * BN; };
   Part p;
 
@@ -438,8 +449,9 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             if (lane == 0) mbar_arrive(&bar_full[slot]);
           }
         } else {
-          const unsigned place = 2 * tile0 + (value ? value_at(j, n) : key_at(j)), slot = place % C::RAWS;
-          mbar_wait(&bar_used[slot], ((place / C::RAWS) & 1) ^ 1, 80);
+          const Slot to = raw_of(tile0, even0, j, n, value);
+          const unsigned slot = to.at;
+          mbar_wait(&bar_used[slot], to.phase ^ 1, 80);
           uint8_t* dst = s_raw + slot * C::RAW;
           const uint8_t* src = reinterpret_cast<const uint8_t*>(value ? a.v : a.k);
           // scales of both sides come with the keys: the softmax looks at them before the values are there
@@ -463,35 +475,25 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   } else if (warp >= C::CONV) {
     // ===================== converting warps
     if constexpr (C::BYTES) {
-      const int tid = threadIdx.x - 32 * C::CONV;
-      constexpr int PER = D / 16, KEYS = 32 * C::CONVERT / PER;      // 16-byte chunks of a key, keys between a thread's chunks
+      constexpr int WARPS = C::CONVERT / C::GROUPS;                // of a group
+      const int tid = (warp - C::CONV) % WARPS * 32 + lane, mine = (warp - C::CONV) / WARPS;     // this group takes 2 (j & 1) + value == mine, or all
+      constexpr int PER = D / 16, KEYS = 32 * WARPS / PER;         // 16-byte chunks of a key, keys between a thread's chunks
       constexpr int CH = BN / KEYS;                                // a thread's chunks of a tile
       // this thread's place in every key, and its first key: lanes of odd 64-column halves take the neighbouring one, so that of eight lanes that write
       // the even chunks (or the odd ones) no two meet in a bank
       const int ch = tid % PER, key0 = (tid / PER) ^ ((ch >> 2) & 1);
       const uint32_t to = (ch >> 2) * (BN * 128) + key0 * 128, c0 = ((2 * (ch & 3)) ^ (key0 & 7)) << 4;
-      static_assert(KEYS % 8 == 0, "every eighth key has the same place in the swizzle");
-      unsigned raw_slot = 0, tile0 = 0, even0 = 0;
-      uint32_t raw_phase = 0;
+      static_assert(KEYS % 4 == 0, "every fourth key has the same place in the swizzle but for one bit");
+      unsigned tile0 = 0, even0 = 0;
       while (next(p)) {
         const int n = p.u1 - p.u0;
         auto convert = [&](int j, bool value) {
           const int first = p.base + j * BN;
           const bool all = first >= p.lo && first + BN <= p.hi;
-          const uint8_t* raw = s_raw + raw_slot * C::RAW;
-          mbar_wait(&bar_raw[raw_slot], raw_phase, 77);
+          const Slot from = raw_of(tile0, even0, j, n, value), here = slot_of(tile0, even0, j, n, value);
+          const uint8_t* raw = s_raw + from.at * C::RAW + key0 * D + ch * 16;
+          mbar_wait(&bar_raw[from.at], from.phase, 77);
           auto inside = [&](int key) { return all || (first + key >= p.lo && first + key < p.hi); };
-          uint4 x[CH];
-#pragma unroll
-          for (int c = 0; c < CH; ++c) {
-            const int key = key0 + c * KEYS;
-            x[c] = *reinterpret_cast<const uint4*>(raw + key * D + ch * 16);
-          }
-          if (!all) {
-#pragma unroll
-            for (int c = 0; c < CH; ++c)
-              if (!inside(key0 + c * KEYS)) x[c] = make_uint4(0u, 0u, 0u, 0u);     // zeros where the list does not reach
-          }
           if (!value && tid < 32) {
             // the values' scales relative to the power of two above the largest
             float* vs = s_scale + ((tile0 + j) % kScaleTiles) * (2 * BN) + BN;
@@ -500,30 +502,46 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             vs[lane] = v0 * two_to(-e), vs[lane + 32] = v1 * two_to(-e);
             if (lane == 0) s_tile[(tile0 + j) % kScaleTiles].v_exp = (float)e;
           }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bar_used[raw_slot]);
-          if (++raw_slot == C::RAWS) raw_slot = 0, raw_phase ^= 1;
-          const Slot here = slot_of(tile0, even0, j, n, value);
           mbar_wait(&bar_empty[here.at], here.phase ^ 1, 81);
           uint8_t* dst = s_kv + here.at * C::SLOT + to;
+          constexpr int BATCH = CH < 4 ? CH : 4;
+#pragma unroll 2
+          for (int c1 = 0; c1 < CH; c1 += BATCH) {
+            uint4 x[BATCH];
 #pragma unroll
-          for (int c = 0; c < CH; ++c) {
-            uint4 y[2];
-            codes4<FMT>(x[c].x, y[0].x, y[0].y);
-            codes4<FMT>(x[c].y, y[0].z, y[0].w);
-            codes4<FMT>(x[c].z, y[1].x, y[1].y);
-            codes4<FMT>(x[c].w, y[1].z, y[1].w);
-            uint8_t* at = dst + c * (KEYS * 128);
-            *reinterpret_cast<uint4*>(at + c0) = y[0];
-            *reinterpret_cast<uint4*>(at + (c0 ^ 16)) = y[1];
+            for (int c = 0; c < BATCH; ++c) x[c] = *reinterpret_cast<const uint4*>(raw + (c1 + c) * (KEYS * D));
+            if (!all) {
+#pragma unroll
+              for (int c = 0; c < BATCH; ++c)
+                if (!inside(key0 + (c1 + c) * KEYS)) x[c] = make_uint4(0u, 0u, 0u, 0u);     // zeros where the list does not reach
+            }
+#pragma unroll
+            for (int c = 0; c < BATCH; ++c) {
+              uint4 y[2];
+              codes4<FMT>(x[c].x, y[0].x, y[0].y);
+              codes4<FMT>(x[c].y, y[0].z, y[0].w);
+              codes4<FMT>(x[c].z, y[1].x, y[1].y);
+              codes4<FMT>(x[c].w, y[1].z, y[1].w);
+              uint8_t* at = dst + (c1 + c) * (KEYS * 128);
+              const uint32_t chunk = c0 ^ (KEYS % 8 != 0 && (c & 1) ? 64u : 0u);
+              *reinterpret_cast<uint4*>(at + chunk) = y[0];
+              *reinterpret_cast<uint4*>(at + (chunk ^ 16)) = y[1];
+            }
           }
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bar_full[here.at]);
+          if (lane == 0) {
+            mbar_arrive(&bar_used[from.at]);
+            mbar_arrive(&bar_full[here.at]);
+          }
         };
-        for (int j = 0; j <= n; ++j) {
-          if (j < n) convert(j, false);
-          if (j > 0) convert(j - 1, true);
+        if constexpr (C::GROUPS == 4) {
+          for (int j = mine >> 1; j < n; j += 2) convert(j, mine & 1);
+        } else {
+          for (int j = 0; j <= n; ++j) {
+            if (j < n) convert(j, false);
+            if (j > 0) convert(j - 1, true);
+          }
         }
         tile0 += n, even0 += (n + 1) / 2;
       }
@@ -533,19 +551,23 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     const int q = warp - C::SOFT;
     const int fmt = std::is_same<M, __half>::value ? 0 : 1;
     const uint32_t id_s = idesc(fmt, BN, 0), id_o = idesc(fmt, D, 1);
-    const uint32_t ql = desc_lo(smem_u32(s_q)) + (DUAL ? 0 : q * (BM * D * 2 / 16)), k_lo = desc_lo(smem_u32(s_kv)), v_lo = desc_lo(smem_u32(s_kv), BN * 128);
+    const uint32_t ql = desc_lo(smem_u32(s_q)) + q * (BM * D * 2 / 16), k_lo = desc_lo(smem_u32(s_kv)), v_lo = desc_lo(smem_u32(s_kv), BN * 128);
     const uint32_t ts = t_s(q, 0), to = t_o(q);
     unsigned tile0 = 0, even0 = 0, mine = 0;   // tiles of the parts before; of them this warp's
     uint32_t q_phase = 0;
     for (; next(p); tile0 += p.u1 - p.u0, even0 += (p.u1 - p.u0 + 1) / 2) {
       const int n = p.u1 - p.u0;
-      if (!DUAL && p.n0 + q * BM >= p.nrows) {
-        // no rows: slots are given back in the order they come
-        for (int x = 0; x < 2 * n; ++x) {
-          const unsigned place = 2 * tile0 + x, slot = place % C::RING;
-          mbar_wait(&bar_full[slot], (place / C::RING) & 1, 82);
-          if (lane == 0) mbar_arrive(&bar_empty[slot]);
+      if (p.n0 + q * BM >= p.nrows) {
+        // no rows: slots are given back in the order in which their tiles come
+        auto give_back = [&](int j, bool value) {
+          const Slot from = slot_of(tile0, even0, j, n, value);
+          mbar_wait(&bar_full[from.at], from.phase, 82);
+          if (lane == 0) mbar_arrive(&bar_empty[from.at]);
           __syncwarp();
+        };
+        for (int j = 0; j <= n; ++j) {
+          if (j < n) give_back(j, false);
+          if (j > 0) give_back(j - 1, true);
         }
         continue;
       }
@@ -554,7 +576,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         const unsigned slot = from.at;
         mbar_wait(&bar_full[slot], from.phase, 82);
         tcgen05_fence_after();
-        const uint32_t kl = k_lo + slot * (C::SLOT / 16), b = (mine + j / STREAMS) & 1, d = ts + b * BN;
+        const uint32_t kl = k_lo + slot * (C::SLOT / 16), b = (mine + j) & 1, d = ts + b * BN;
         if (elect_one()) {
 #pragma unroll
           for (int c = 0; c < DSUB; ++c)
@@ -566,56 +588,53 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         __syncwarp();
       };
       // the queries are in place, and what the list before left in tensor memory has been read
-      const int first = DUAL ? q : 0;      // this stream's tiles: first, first + STREAMS ..
-      if (n <= first) continue;
       mbar_wait(&bar_q[q], q_phase, 79);
       q_phase ^= 1;
-      for (int j = first; j < min(n, 2 * STREAMS); j += STREAMS) scores(j);
-      for (int j = first; j < n; j += STREAMS) {
+      for (int j = 0; j < min(n, 2); ++j) scores(j);
+      for (int j = 0; j < n; ++j) {
         const Slot from = slot_of(tile0, even0, j, n, true);
-        const unsigned i = mine + j / STREAMS, slot = from.at, b = i & 1, parity = (i >> 1) & 1;
+        const unsigned slot = from.at, b = (mine + j) & 1, parity = ((mine + j) >> 1) & 1;
         mbar_wait(&bar_full[slot], from.phase, 82);
         mbar_wait(&bar_p[q * 2 + b], parity, 83);
         tcgen05_fence_after();
         const uint32_t vl = v_lo + slot * (C::SLOT / 16), pt = ts + b * BN;
         if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < BN / 16; ++k) umma_ts(to, pt + k * 8, vl + k * 128, id_o, (j > first || k > 0) ? 1u : 0u);
+          for (int k = 0; k < BN / 16; ++k) umma_ts(to, pt + k * 8, vl + k * 128, id_o, (j > 0 || k > 0) ? 1u : 0u);
           umma_commit(&bar_o[q * 2 + b]);
           umma_commit(&bar_empty[slot]);
         }
         __syncwarp();
-        if (j + 2 * STREAMS < n) {
+        if (j + 2 < n) {
           mbar_wait(&bar_o[q * 2 + b], parity, 84);              // P_j has been read: the scores two tiles on go over it
-          scores(j + 2 * STREAMS);
+          scores(j + 2);
         }
       }
-      mine += (n - first + STREAMS - 1) / STREAMS;
+      mine += n;
     }
   } else if (warp < C::SOFT) {
-    // ===================== softmax: a thread per row
-    const int q = warp >> 2, quarter = warp & 3;
+    // ===================== softmax: a row's one or two threads, in warps `half` 0 and 1
+    constexpr int SHARE = C::SHARE, COLS = C::COLS;
+    const int q = warp / (4 * SHARE), quarter = warp & 3, half = SHARE == 2 ? (warp >> 2) & 1 : 0, pair = q * 4 + quarter;
     const uint32_t off = (uint32_t)(quarter * 32) << 16;
-    // this warp's 32 rows of queries, and where its outputs are staged: D / 64 pieces of 32 x 128 bytes, swizzled
-    uint8_t* s_mine = s_q + (DUAL ? 0 : q * (BM * D * 2)) + quarter * (32 * 128);
+    // these rows' queries, and where their outputs are staged: D / 64 pieces of 32 x 128 bytes, swizzled
+    uint8_t* s_mine = s_q + q * (BM * D * 2) + quarter * (32 * 128);
     auto place = [&](int row, int ch) { return s_mine + (ch >> 3) * (BM * 128) + row * 128 + (((ch & 7) ^ (row & 7)) << 4); };
+    float* s_tops = s_max + (q * 2 + half) * BM + quarter * 32 + lane;   // this thread's; the other one's 128 numbers on or back, the other tile's 2 * ROWS on
+    const int other = half ? -BM : BM;
+    float2* s_sums = s_sum + (q * 2 + half) * BM + quarter * 32 + lane;
     constexpr float kUp = std::is_same<M, __half>::value ? 7.0f : 0.0f;   // f16 ends at 2^16: probabilities are formed times 2^7, at most 2^15
-    auto queries_are_in = [&](int n) {     // for the streams that have a tile
-      mbar_arrive(&bar_q[q]);
-      if (DUAL && n > 1) mbar_arrive(&bar_q[1]);
-    };
     unsigned tile0 = 0, mine = 0;          // tiles of the parts before; of them this warp's
     Cut cut = {-1, 0, 0, 0};
     while (next(p)) {
-      const int n = p.u1 - p.u0, q0 = DUAL ? 0 : q * BM, n0 = p.n0 + q0 + quarter * 32;
-      const int first = DUAL ? q : 0;      // this stream's tiles: first, first + STREAMS ..
+      const int n = p.u1 - p.u0, n0 = p.n0 + q * BM + quarter * 32;
       const unsigned at = tile0;
       tile0 += n;
-      if (p.n0 + q0 >= p.nrows) continue;
+      if (p.n0 + q * BM >= p.nrows) continue;
       if (n0 >= p.nrows) {
         // no rows of this warp's: its barriers go on, whatever the products make of them
-        if (lane == 0 && first == 0) queries_are_in(n);
-        for (int j = first; j < n; j += STREAMS, ++mine) {
+        if (lane == 0) mbar_arrive(&bar_q[q]);
+        for (int j = 0; j < n; ++j, ++mine) {
           mbar_wait(&bar_s[q * 2 + (mine & 1)], (mine >> 1) & 1, 85);
           if (lane == 0) mbar_arrive(&bar_p[q * 2 + (mine & 1)]);
           __syncwarp();
@@ -626,23 +645,26 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       const bool live = row < p.nrows;
       const int tok = p.s.row0 + row / group, head = p.kvh * group + row % group;
       float scale = a.scale_log2;
-      if (first == 0) {
+      {
+        if (SHARE == 2) pair_sync(pair);   // what the other warp staged there has been stored
+        // 32 / SHARE rows of queries each
         const int64_t from = live ? (int64_t)tok * a.ldq + (int64_t)head * D : -1;
         constexpr int LANES = D / 8, STEP = 32 / LANES;    // lanes of a row, rows of one step of the warp
-        const int ch = lane % LANES;
+        constexpr int MINE = 32 / SHARE;
+        const int ch = lane % LANES, r0 = half * MINE;
         // loops, not lines: what runs seldom comes from memory, eight instructions at a time
         if constexpr (std::is_same<M, T>::value) {
 #pragma unroll 2
-          for (int i = 0; i < 32; i += STEP) {
-            const int r = i + lane / LANES;
+          for (int i = 0; i < MINE; i += STEP) {
+            const int r = r0 + i + lane / LANES;
             const int64_t x = __shfl_sync(0xffffffffu, from, r);
             copy16(smem_u32(place(r, ch)), reinterpret_cast<const T*>(a.q) + (x < 0 ? 0 : x + ch * 8), x < 0 ? 0 : 16);
           }
           copies_wait_all();
         } else {
           // bf16 to f16 on the way, after division by the power of two below a row's largest value
-          constexpr int AHEAD = 32 / STEP < 8 ? 32 / STEP : 8;
-          for (int i0 = 0; i0 < 32; i0 += AHEAD * STEP) {
+          constexpr int AHEAD = MINE / STEP < 8 ? MINE / STEP : 8;
+          for (int i0 = r0; i0 < r0 + MINE; i0 += AHEAD * STEP) {
             uint4 y[AHEAD];
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
@@ -656,27 +678,25 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 #pragma unroll
               for (int o = 1; o < LANES; o <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
               top = max(top & 0xffffu, top >> 16) >> 7;   // bf16: eight bits of exponent above seven of fraction
-              const int e = top == 255 ? 0 : max(-126, min(126, (int)top - 127)), r = i0 + u * STEP;
+              const int e = top == 255 ? 0 : max(-126, min(126, (int)top - 127)), r = i0 + u * STEP + lane / LANES;
               const float down = two_to(-e);
               float z[8];
               unpack8<T>(y[u], z);
 #pragma unroll
               for (int k = 0; k < 8; ++k) z[k] *= down;
-              *reinterpret_cast<uint4*>(place(r + lane / LANES, ch)) = pack8<__half>(z);
-              const int mine_e = __shfl_sync(0xffffffffu, e, (lane - r) % STEP * LANES);     // (of rows r .. r + STEP - 1)
-              if (lane >= r && lane < r + STEP) scale *= two_to(mine_e);
+              *reinterpret_cast<uint4*>(place(r, ch)) = pack8<__half>(z);
+              if (ch == 0) s_unit[q * BM + quarter * 32 + r] = two_to(e);
             }
           }
         }
         fence_proxy_async_smem();
         tcgen05_fence_before();
         __syncwarp();
-        if (lane == 0) queries_are_in(n);
-        if (DUAL && !std::is_same<M, T>::value) s_join[4 * 8 * 32 + quarter * 32 + lane].x = scale;
-      }
-      if constexpr (DUAL && !std::is_same<M, T>::value) {
-        pair_sync(quarter);
-        if (q == 1) scale = s_join[4 * 8 * 32 + quarter * 32 + lane].x;
+        if (lane == 0) mbar_arrive(&bar_q[q]);
+        if constexpr (!std::is_same<M, T>::value) {
+          if (SHARE == 2) pair_sync(pair);
+          scale *= s_unit[q * BM + quarter * 32 + lane];
+        }
       }
       // cached tokens, which the row sees all; its mask says which of the new ones (rows beyond the last see everything and are dropped)
       int ctx = p.hi;
@@ -690,65 +710,67 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       // outputs are sums of probabilities times 2^up: with scales, less the exponent of the values' largest so far.  The sum of probabilities stands relative
       // to the maximum alone then: keys count whose values are far smaller than others
       float up = C::BYTES ? INFINITY : kUp;
-      bool partly = false;                                // some row of the warp does not see some key of its tiles
       bool bad = false;                                   // a score of the row is NaN: so is the result, whatever the exponentials made of it
       bool sees = false;
-      for (int j = first; j < n; j += STREAMS, ++mine) {
-        const int b = mine & 1, kb = p.base + j * BN;
+      for (int j = 0; j < n; ++j, ++mine) {
+        const int b = mine & 1, kb = p.base + j * BN + half * COLS;       // this thread's first key
         mbar_wait(&bar_s[q * 2 + b], (mine >> 1) & 1, 85);
         tcgen05_fence_after();
-        float sc[BN];
+        float sc[COLS];
         {
-          uint32_t r[BN / 32][32];
+          uint32_t r[COLS / 32][32];
 #pragma unroll
-          for (int c = 0; c < BN / 32; ++c) tmem_ld_32x32b_x32(t_s(q, b) + off + c * 32, r[c]);
+          for (int c = 0; c < COLS / 32; ++c) tmem_ld_32x32b_x32(t_s(q, b) + off + half * COLS + c * 32, r[c]);
           tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < BN / 32; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) sc[c * 32 + i] = __uint_as_float(r[c][i]);
+          for (int i = 0; i < COLS; ++i) sc[i] = __uint_as_float(r[i / 32][i % 32]);
         }
-        const float* scales = s_scale + ((at + j) % kScaleTiles) * (2 * BN);
+        const float* scales = s_scale + ((at + j) % kScaleTiles) * (2 * BN) + half * COLS;
         float v_exp = 0.f;
         if constexpr (C::BYTES) {
           v_exp = s_tile[(at + j) % kScaleTiles].v_exp;
 #pragma unroll
-          for (int i = 0; i < BN; i += 4) {
+          for (int i = 0; i < COLS; i += 4) {
             const float4 k4 = *reinterpret_cast<const float4*>(scales + i);
             fmul2(sc[i], sc[i + 1], sc[i], sc[i + 1], k4.x, k4.y);
             fmul2(sc[i + 2], sc[i + 3], sc[i + 2], sc[i + 3], k4.z, k4.w);
           }
         }
         const int hi = pos - kb, lo = p.lo - kb;
-        uint32_t see[2] = {~0u, ~0u};
-        const bool edge = __any_sync(0xffffffffu, hi < BN - 1 || lo > 0);
+        uint32_t see[COLS / 32];
+        const bool edge = __any_sync(0xffffffffu, hi < COLS - 1 || lo > 0);
         if (edge) {
-          partly = true;
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
+          for (int c = 0; c < COLS / 32; ++c) {
             see[c] = (masked ? tree_bits(a, tok, kb + c * 32 - ctx) : ~0u) & bit_range(lo - c * 32, (masked ? p.hi - 1 - kb : hi) - c * 32);
+            sees = sees || see[c] != 0;
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if ((see[c] >> i & 1u) == 0) sc[c * 32 + i] = -INFINITY;
           }
-          sees = sees || (see[0] | see[1]) != 0;
         } else {
           sees = true;
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < BN; i += 8) {
+        for (int i = 0; i < COLS; i += 8) {
 #pragma unroll
           for (int u = 0; u < 4; ++u) mx[u] = max3_nan(mx[u], sc[i + 2 * u], sc[i + 2 * u + 1]);
         }
-        const float m_tile = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * scale;
+        float m_tile = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * scale;
+        if constexpr (SHARE == 2) {
+          // both threads go by the maximum of the row's 64 scores; behind their meeting S has been read by both, and P may go over it
+          s_tops[b * (2 * ROWS)] = m_tile;
+          pair_sync(pair);
+          m_tile = max_nan(m_tile, s_tops[b * (2 * ROWS) + other]);
+        }
         bad = bad || m_tile != m_tile;
         const bool grow = m_tile > m_run + 8.0f;
         const float m_new = grow ? m_tile : m_run;
         float up_new = up;
         if constexpr (C::BYTES) up_new = fminf(up, kUp - v_exp);
-        const float alpha = j > first && m_new > -INFINITY && (grow || up_new != up) ? exp2_fast((m_run - m_new) + (up_new - up)) : 1.0f;
-        const float fade = C::BYTES ? (j > first && grow ? exp2_fast(m_run - m_new) : 1.0f) : alpha;
+        const float alpha = j > 0 && m_new > -INFINITY && (grow || up_new != up) ? exp2_fast((m_run - m_new) + (up_new - up)) : 1.0f;
+        const float fade = C::BYTES ? (j > 0 && grow ? exp2_fast(m_run - m_new) : 1.0f) : alpha;
         m_run = m_new;
         up = up_new;
         // of this tile's probabilities; below 2^-32 they are zeros in f16, and by a factor of 2^-60 their sum still is what it is
@@ -756,7 +778,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         const float neg = m_new == -INFINITY ? 0.f : lift - m_new;
         float la[4] = {0.f, 0.f, 0.f, 0.f}, lb[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < BN / 32; ++c) {
+        for (int c = 0; c < COLS / 32; ++c) {
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
@@ -782,15 +804,15 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 #pragma unroll
             for (int i = 0; i < 16; ++i) pk[i] &= ((see[c] >> (2 * i) & 1u) ? 0xffffu : 0u) | ((see[c] >> (2 * i + 1) & 1u) ? 0xffff0000u : 0u);
           }
-          tmem_st_x16(t_s(q, b) + off + c * 16, pk);
+          tmem_st_x16(t_s(q, b) + off + half * (COLS / 2) + c * 16, pk);
         }
         tmem_st_done();
         const float l_tile = ((la[0] + lb[0]) + (la[1] + lb[1])) + ((la[2] + lb[2]) + (la[3] + lb[3]));
-        if (j > first && __any_sync(0xffffffffu, alpha != 1.0f)) {
+        if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
           mbar_wait(&bar_o[q * 2 + (b ^ 1)], ((mine - 1) >> 1) & 1, 86);
           tcgen05_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
+          for (int c = half * (D / 32 / SHARE); c < (half + 1) * (D / 32 / SHARE); ++c) {
             uint32_t r[32];
             tmem_ld_32x32b_x32(t_o(q) + off + c * 32, r);
             tmem_ld_wait();
@@ -805,17 +827,14 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar_p[q * 2 + b]);
       }
-      if (n > first) {
-        mbar_wait(&bar_o[q * 2 + ((mine - 1) & 1)], ((mine - 1) >> 1) & 1, 87);
-        tcgen05_fence_after();
-      }
+      mbar_wait(&bar_o[q * 2 + ((mine - 1) & 1)], ((mine - 1) >> 1) & 1, 87);
+      tcgen05_fence_after();
 
-      // ---- the list's result, through shared memory where this warp's queries were, or its part
-      if (bad) l_run = __int_as_float(0x7fc00000);
+      // ---- the list's result, through shared memory where these rows' queries were, or its part; each thread its share of the columns
       const bool whole = p.u0 == 0 && p.u1 == p.n, direct = whole && a.groups == 0;
       const int slot = 2 * blockIdx.x + (p.u0 == 0 && at > 0 ? 1 : 0);
       if (p.u0 == 0 && !whole) cut = {slot, (int)((w.cur - (p.u1 - p.u0) + p.n - 1) / per) | min(ROWS, p.nrows - p.n0) << 16, p.s.row0, p.kvh * pa.row_tiles + p.rt};
-      if (a.groups > 0 && p.u0 == 0 && q == 0 && quarter == 0 && lane == 0) {
+      if (a.groups > 0 && p.u0 == 0 && warp == 0 && lane == 0) {
         FewInfo in;
         in.first_slot = whole ? -1 : slot;
         in.first_warp = blockIdx.x;
@@ -830,107 +849,61 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       // joins them with a group's
       const bool compact = a.groups == 0;
       rows.rs = compact ? 4 : D + kPad, rows.cs = compact ? ROWS * 4 : 4;
-      rows.parts = direct ? nullptr : pa.slots + (int64_t)slot * ROWS * (D + kPad) + (q0 + quarter * 32) * rows.rs;
+      rows.parts = direct ? nullptr : pa.slots + (int64_t)slot * ROWS * (D + kPad) + (q * BM + quarter * 32) * rows.rs;
       unsigned anew = 0;
-      if constexpr (FMT != kInt8)                         // (int8: a hidden value is 0 x a number)
-        if (partly && n > first) anew = spoiled_rows<M, FMT, D>(a, rows, t_o(q) + off, live && !bad);
-      // of outputs, to the sum's reference
-      float ref = C::BYTES ? m_run : m_run - up, down = C::BYTES ? exp2f(-up) : 1.0f, other = 0.f;
-      if constexpr (DUAL) {
-        float4* s_state = s_join + 4 * 8 * 32 + quarter * 32 + lane;
-        float4* s_cols = s_join + quarter * (8 * 32) + lane;
-        if (q == 1) {
-          // the odd tiles' rows, to the other stream
-          if (n > first) {
-            *s_state = make_float4(ref, l_run, __uint_as_float((sees ? 1u : 0u) | (anew >> lane & 1u) << 1), 0.f);
-            pair_sync(quarter);
-#pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t r[32];
-              tmem_ld_32x32b_x32(t_o(q) + off + c * 32, r);
-              tmem_ld_wait();
-              if (c > 0) pair_sync(quarter);
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                s_cols[i * 32] = make_float4(__uint_as_float(r[4 * i]) * down, __uint_as_float(r[4 * i + 1]) * down, __uint_as_float(r[4 * i + 2]) * down,
-                                             __uint_as_float(r[4 * i + 3]) * down);
-              pair_sync(quarter);
-            }
-            pair_sync(quarter);            // before the next list's scales
-          }
-          continue;
-        }
-        if (n > 1) {
-          pair_sync(quarter);
-          const float4 st = *s_state;
-          const uint32_t flags = __float_as_uint(st.z);
-          const float top = fmaxf(ref, st.x), base = top == -INFINITY ? 0.f : top;
-          const float f0 = exp2f(ref - base);
-          other = exp2f(st.x - base);
-          l_run = l_run * f0 + st.y * other;
-          down *= f0;
-          ref = top;
-          sees = sees || (flags & 1u) != 0;
-          anew |= __ballot_sync(0xffffffffu, (flags & 2u) != 0);
-        }
+      if constexpr (FMT != kInt8) {                       // (int8: a hidden value is 0 x a number)
+        // one of the rows does not see all keys (what lies beyond the list's are zeros)
+        if (half == 0 && __any_sync(0xffffffffu, pos < p.hi - 1)) anew = spoiled_rows<M, FMT, D>(a, rows, t_o(q) + off, live && !bad);
       }
+      if constexpr (SHARE == 2) {
+        *s_sums = make_float2(l_run, __uint_as_float((sees ? 1u : 0u) | (anew >> lane & 1u) << 1));
+        pair_sync(pair);
+        const float2 theirs = s_sums[other];
+        const uint32_t flags = __float_as_uint(theirs.y);
+        l_run += theirs.x;
+        sees = sees || (flags & 1u) != 0;
+        anew |= __ballot_sync(0xffffffffu, (flags & 2u) != 0);
+      }
+      if (bad) l_run = __int_as_float(0x7fc00000);
+      const float ref = C::BYTES ? m_run : m_run - up, down = C::BYTES ? exp2f(-up) : 1.0f;      // of outputs, to the sum's reference
+      const bool stored = live && (anew >> lane & 1) == 0;
       uint8_t* out = nullptr;
       // a part of a row that is finished here goes beside the groups' or own ones of the same row
       float* part = whole ? (p.own ? pa.whole_own : pa.whole_group) + ((int64_t)tok * a.hq + head) * (D + kPad) : rows.parts + lane * rows.rs;
-      if (live && (anew >> lane & 1) == 0) {
-        if (direct) {
-          out = reinterpret_cast<uint8_t*>(reinterpret_cast<T*>(a.out) + (int64_t)tok * a.ldo + (int64_t)head * D);
-        } else {
-          *reinterpret_cast<float4*>(part + (D / 4) * rows.cs) = make_float4(ref, l_run, sees ? 1.f : 0.f, 0.f);
-        }
+      if (stored) {
+        if (direct) out = reinterpret_cast<uint8_t*>(reinterpret_cast<T*>(a.out) + (int64_t)tok * a.ldo + (int64_t)head * D);
+        else if (half == 0) *reinterpret_cast<float4*>(part + (D / 4) * rows.cs) = make_float4(ref, l_run, sees ? 1.f : 0.f, 0.f);
       }
-      const float whole_l = direct ? 1.0f / l_run : 1.0f;
-      const float inv = down * whole_l;
-      other *= whole_l;
-      // results: 128 bytes of each of 32 rows, staged by the rows' threads, stored by eight lanes a row
-      auto store = [&](int piece, int to) {
-        __syncwarp();
-#pragma unroll 4
-        for (int i = 0; i < 32; i += 4) {
-          const int r = i + (lane >> 3);
-          const uint64_t x = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(out), r);
-          if (x != 0) *reinterpret_cast<uint4*>(x + to + (lane & 7) * 16) = *reinterpret_cast<const uint4*>(place(r, piece * 8 + (lane & 7)));
-        }
-      };
+      const float inv = direct ? down / l_run : down;
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
+      for (int c = half * (D / 32 / SHARE); c < (half + 1) * (D / 32 / SHARE); ++c) {
         uint32_t r[32];
         tmem_ld_32x32b_x32(t_o(q) + off + c * 32, r);
         tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * inv);
-        if (DUAL && n > 1) {
-          pair_sync(quarter);
-          const float4* s_cols = s_join + quarter * (8 * 32) + lane;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float4 x = s_cols[i * 32];
-            const float y[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) r[4 * i + e] = __float_as_uint(fmaf(y[e], other, __uint_as_float(r[4 * i + e])));
-          }
-          pair_sync(quarter);
-        }
         if (direct) {
+          // 64 bytes of each of 32 rows, staged by the rows' threads, stored by four lanes a row
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
             float f8[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f8[e] = sees ? __uint_as_float(r[i + e]) : 0.f;
+            for (int e = 0; e < 8; ++e) f8[e] = sees ? __uint_as_float(r[i + e]) * inv : 0.f;
             *reinterpret_cast<uint4*>(place(lane, c * 4 + i / 8)) = pack8<T>(f8);
           }
-          if (c & 1) store(c >> 1, (c >> 1) * 128);
-        } else if (live && (anew >> lane & 1) == 0) {
+          __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(part + (c * 8 + i / 4) * rows.cs) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+          for (int i = 0; i < 32; i += 8) {
+            const int x = i + (lane >> 2);
+            const uint64_t to = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(out), x);
+            if (to != 0) *reinterpret_cast<uint4*>(to + c * 64 + (lane & 3) * 16) = *reinterpret_cast<const uint4*>(place(x, c * 4 + (lane & 3)));
+          }
+        } else if (stored) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<float4*>(part + (c * 8 + i / 4) * rows.cs) =
+                make_float4(__uint_as_float(r[i]) * inv, __uint_as_float(r[i + 1]) * inv, __uint_as_float(r[i + 2]) * inv, __uint_as_float(r[i + 3]) * inv);
         }
       }
-      if (anew != 0) {
+      if (half == 0 && anew != 0) {
         if (whole && !direct) {
           // rows of a finished part lie apart
           for (unsigned rest = anew; rest != 0; rest &= rest - 1) {
@@ -945,7 +918,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
           rows_anew<T, T, FMT, D>(a, rows, anew);
         }
       }
-      __syncwarp();                                       // what was staged has been stored: the next list's queries go over it
+      __syncwarp();                                       // what was staged has been stored
     }
     if (a.groups == 0 && warp == 0 && lane == 0) reinterpret_cast<Cut*>(pa.info)[blockIdx.x] = cut;
   }
@@ -1024,12 +997,12 @@ __global__ void __launch_bounds__(256) attn_tree_merge_kernel(const __grid_const
   }
 }
 
-template <typename T, int FMT, int D, int NQ, bool DUAL>
+template <typename T, int FMT, int D, int NQ>
 int launch(const AttnArgs& a, const PartArgs& p, cudaStream_t stream) {
-  using C = Tree<FMT, D, NQ, DUAL>;
+  using C = Tree<FMT, D, NQ>;
   static_assert(C::SMEM <= 232448, "shared memory of a block");
   static PerDeviceSmem configured;
-  auto kern = attn_tree_kernel<T, FMT, D, NQ, DUAL>;
+  auto kern = attn_tree_kernel<T, FMT, D, NQ>;
   LLMSS_CHECK_CUDA(configured.ensure(kern, C::SMEM));
   TreeArgs ta;
   ta.own = a.num_seqs;
@@ -1063,9 +1036,9 @@ int launch(const AttnArgs& a, const PartArgs& p, cudaStream_t stream) {
 
 template <typename T, int FMT>
 int by_size(const AttnArgs& a, const PartArgs& p, cudaStream_t stream) {
-  if (a.d == 256) return launch<T, FMT, 256, 1, false>(a, p, stream);
-  if (a.d == 128) return p.rows == 256 ? launch<T, FMT, 128, 2, false>(a, p, stream) : launch<T, FMT, 128, 2, true>(a, p, stream);
-  return p.rows == 256 ? launch<T, FMT, 64, 2, false>(a, p, stream) : launch<T, FMT, 64, 2, true>(a, p, stream);
+  if (a.d == 256) return launch<T, FMT, 256, 1>(a, p, stream);
+  if (a.d == 128) return p.rows == 256 ? launch<T, FMT, 128, 2>(a, p, stream) : launch<T, FMT, 128, 1>(a, p, stream);
+  return p.rows == 256 ? launch<T, FMT, 64, 2>(a, p, stream) : launch<T, FMT, 64, 1>(a, p, stream);
 }
 
 }  // namespace
