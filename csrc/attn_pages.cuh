@@ -1,11 +1,12 @@
-// Shared by the kernels of attention over cache pages (attn_pages.cu, attn_pages_few.cu, attn_pages_tile.cu).
+// Shared by the kernels of attention over cache pages (attn_pages.cu, attn_pages_few.cu, attn_pages_tile.cu, attn_tree.cu).
 //
 // Causal attention over a paged cache in 16 or 8 bits, with cached tokens that groups of sequences share.
 //
 //   s_jk = scale (q_j . K_k)      K_k = ks_k code_k      p = softmax over the keys k <= pos_j      out_j = sum_k p_jk vs_k code_k
 //
 // A sequence of a group (SharedPrefix) finds its first len keys in the group's pages and the others in its own; a softmax over both is the merge
-// of the two parts by their maxima and sums.
+// of the two parts by their maxima and sums.  Rows of a tree of drafted tokens (masks) see all keys in front of their sequence's new ones, and of those the
+// ones that their mask names.
 #pragma once
 #include "common.cuh"
 

@@ -14,6 +14,9 @@
 // The scale of a value row joins its probability in the exponent, with a maximum of its own.  Maxima move when a score exceeds them by 8 only, and what is
 // rounded to f16 is formed times 2^7, so that it is at most 2^15 whatever the scales are.
 //
+// Rows of a tree (TREE) see all cached keys and those of the new ones whose bit their mask has: 16 rows are at most 16 new tokens, so that a row's bits are one
+// register, looked at in the units behind the cached keys alone.  64 trees of 10 tokens over 1040, 16 heads of 256: 187 us, 0.93 of the copy rate.
+//
 // The work of a call is the sum of all (sequence, key head) lists in units of 16 keys (32 where a key is 64 bytes); each warp takes an equal run of it,
 // wherever sequences begin and end, and waits for no other.  A list within a warp's run is finished there; one that crosses runs leaves its parts in
 // scratch, at most two per warp, and the merge kernel joins them.

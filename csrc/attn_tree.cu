@@ -27,6 +27,9 @@
 // The values' scales join the probabilities before their one rounding to f16, relative to a power of two per tile (TileScales) that keeps them in range;
 // scaled and rounded codes (2^-11 of each key, value and probability) make f16 results off by 6.1e-4 instead of 2.9e-4.
 // A list within a block's run is finished there, one that crosses runs leaves its parts in scratch, at most two per block, and the merge kernel joins them.
+
+// A row that is formed anew takes a warp 0.7 us per key, 32 of them over 10^6 keys 22 s, and the block's other warps wait meanwhile: waits end after 60 s here.
+#define LLMSS_SPIN_TIMEOUT_NS 60000000000ull
 #include "attn_pages.cuh"
 
 namespace {
@@ -143,7 +146,7 @@ __device__ __forceinline__ float exp2_fma(float x) {
   float p = fmaf(r, 0.05459282f, 0.24221784f);
   p = fmaf(r, p, 0.6933686f);
   p = fmaf(r, p, 1.0f);
-  return __int_as_float(__float_as_int(t) * (1 << 23) + __float_as_int(p));     // (what the 1.5 2^23 of t holds besides x leaves the word)
+  return __uint_as_float(__float_as_uint(t) * (1u << 23) + __float_as_uint(p));     // (what the 1.5 2^23 of t holds besides x leaves the word)
 }
 
 // the two warps of 32 rows

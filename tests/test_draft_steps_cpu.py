@@ -115,3 +115,19 @@ def test_refusals(tmp_path):
         with pytest.raises(ValueError, match="check_drafts"):
             eng.runner.check_drafts([s], bad)
     assert len(eng.runner.check_drafts([s], [([], [])])[0]) == 1
+
+
+def test_generate_with_draft_tokens(tmp_path, monkeypatch, capsys):
+    import sys
+    from pathlib import Path
+
+    monkeypatch.syspath_prepend(str(Path(__file__).resolve().parents[1]))
+    monkeypatch.setenv("WORLD_SIZE", "1")
+    monkeypatch.setenv("RANK", "0")
+    import generate
+
+    make_tiny("llama", tmp_path)
+    args = ["--pretrained_model_path", str(tmp_path), "--prompt_ids", "5 17 3 5 17", "8 9 8", "--max_new_tokens", "12", "--is_greedy", "--use_cache", "--dtype", "float32"]
+    want = generate.main(args)
+    assert generate.main(args + ["--draft_tokens", "6"]) == want
+    assert len(want) == 2 and all(len(x) == 12 for x in want)
